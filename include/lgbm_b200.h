@@ -529,6 +529,108 @@ int lgbm_b200_predictor_destroy(lgbm_b200_predictor* p);
 int lgbm_b200_predict(lgbm_b200_predictor* p, const double* rows, int64_t num_rows,
                       int32_t raw_score, double* out);
 
+/* ---- Expert layers: rows routed to experts, products grouped by expert ----
+ *
+ * The rows of a batch ("tokens") are routed to k of E experts each, the tokens * k slots
+ * are grouped by expert, every expert multiplies its ragged range of rows, and a token's
+ * k results are joined: what a leaf-wise model does with its leaves, with a learned matrix
+ * in each. No counterpart in the reference.
+ *
+ * Conventions of these entry points
+ *  - All array pointers are DEVICE pointers on the current device. The work is enqueued on
+ *    `stream` (a cudaStream_t; NULL is the legacy default stream) and not waited for. They
+ *    allocate nothing: where scratch is needed the caller passes it, at least as large as
+ *    the _workspace function says, 16-byte aligned; it is free again once the stream has
+ *    passed the call.
+ *  - Pitches are in elements; the innermost axis is contiguous. Outputs are contiguous.
+ *  - offsets[E + 1], index, chosen and position are device data that the host does not
+ *    check. Kernels clamp offsets to the rows given and skip indices outside them.
+ *  - At most 512 experts, 16 chosen a token, 2^31 - 65537 rows.
+ *  - Sums and softmax statistics are in f32, results rounded once to their type. No result
+ *    depends on the order of atomics: the same inputs give the same bits. */
+#define LGBM_B200_DTYPE_F32 0
+#define LGBM_B200_DTYPE_BF16 1
+#define LGBM_B200_DTYPE_F16 2
+
+/* logits [tokens][experts] (pitch >= experts). Per token the k largest logits, ties to the
+ * lower expert: chosen (descending logit) and weights, their softmax over the chosen
+ * (normalize != 0) or over all experts. -inf is never chosen: a token with fewer than k
+ * other logits has chosen -1 and weight 0 in its last slots. NaN ranks first, and its
+ * token's weights are NaN. Grouping, stable in slot order: offsets[e] is expert e's first
+ * row, offsets[experts] the number of assigned slots; position[slot] is the slot's row (a
+ * permutation of tokens * k: slots without an expert come last) and rows[position] its
+ * token. */
+int64_t lgbm_b200_experts_route_workspace(int64_t tokens, int32_t experts, int32_t k);
+int lgbm_b200_experts_route(const void* logits, int32_t dtype, int64_t tokens, int32_t experts,
+                            int64_t pitch, int32_t k, int32_t normalize, float* weights,
+                            int32_t* chosen, int32_t* position, int32_t* rows, int32_t* offsets,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+/* dlogits [tokens][experts] of the logits' type from dweights [tokens][k] and the results
+ * of lgbm_b200_experts_route on the same logits, k and normalize. */
+int lgbm_b200_experts_route_backward(const float* dweights, const float* weights,
+                                     const int32_t* chosen, const void* logits, int32_t dtype,
+                                     int64_t tokens, int32_t experts, int64_t pitch, int32_t k,
+                                     int32_t normalize, void* dlogits, void* stream);
+
+/* Products grouped by expert, bf16 or f16, accumulated in f32; row r belongs to the expert
+ * e with offsets[e] <= r < offsets[e + 1]:
+ *   y[r]  = w[e] x[index ? index[r] : r]    [rows][outer]; w [experts][outer][inner]
+ *   dx[r] = dy[r] w[e]                      [rows][inner]
+ *   dw[e] = sum of dy[r]^T x[...]           [experts][outer][inner], of `out_dtype`: the
+ *                                           inputs' type or f32
+ * Rows of y and dx that belong to no expert are 0, and so is the dw of an expert without
+ * rows. An index outside [0, x_rows) stands for a row of zeros. x, dy and w are read in
+ * place when their base and pitch are multiples of 16 bytes, else copied to the workspace
+ * first; mode: 0 y, 1 dx, 2 dw. */
+int64_t lgbm_b200_experts_matmul_workspace(int32_t mode, const void* x, int64_t x_pitch,
+                                           const int32_t* index, const void* dy,
+                                           int64_t dy_pitch, const void* w, int64_t rows,
+                                           int32_t experts, int32_t inner, int32_t outer);
+int lgbm_b200_experts_matmul(const void* x, int64_t x_rows, int64_t x_pitch,
+                             const int32_t* index, const void* w, const int32_t* offsets,
+                             int32_t dtype, int64_t rows, int32_t experts, int32_t inner,
+                             int32_t outer, void* y, void* workspace, int64_t workspace_bytes,
+                             void* stream);
+int lgbm_b200_experts_matmul_input_grad(const void* dy, int64_t dy_pitch, const void* w,
+                                        const int32_t* offsets, int32_t dtype, int64_t rows,
+                                        int32_t experts, int32_t inner, int32_t outer, void* dx,
+                                        void* workspace, int64_t workspace_bytes, void* stream);
+int lgbm_b200_experts_matmul_weight_grad(const void* dy, int64_t dy_pitch, const void* x,
+                                         int64_t x_rows, int64_t x_pitch, const int32_t* index,
+                                         const int32_t* offsets, int32_t dtype,
+                                         int32_t out_dtype, int64_t rows, int32_t experts,
+                                         int32_t inner, int32_t outer, void* dw, void* workspace,
+                                         int64_t workspace_bytes, void* stream);
+/* Every wait inside the product kernels is bounded. One that ran out leaves its outputs
+ * incomplete and sets a bit here: this call waits for the device, reads the bits of the
+ * current device and clears them. */
+int lgbm_b200_experts_errors(uint32_t* bits_out);
+
+/* out[t] = sum over j of weights[t][j] * y[position[t][j]] (weights NULL: 1); a position
+ * outside [0, rows) adds nothing. */
+int lgbm_b200_experts_combine(const void* y, int32_t dtype, int64_t rows, int32_t width,
+                              int64_t pitch, const int32_t* position, const float* weights,
+                              int64_t tokens, int32_t k, void* out, void* stream);
+/* dy[position[t][j]] = weights[t][j] * dout[t]; dweights[t][j] (NULL: not wanted, y is not
+ * read) = <dout[t], y[position[t][j]]>. rows must be tokens * k and position a permutation
+ * of them, as lgbm_b200_experts_route makes it. */
+int lgbm_b200_experts_combine_backward(const void* dout, const void* y, int32_t dtype,
+                                       int64_t rows, int32_t width, int64_t dout_pitch,
+                                       int64_t pitch, const int32_t* position,
+                                       const float* weights, int64_t tokens, int32_t k, void* dy,
+                                       float* dweights, void* stream);
+
+/* out = (residual +) x * keep / (1 - p) over rows x width elements numbered row by row.
+ * Element i is kept when its 16 random bits are at least D = round(p * 65536); the scale
+ * is 65536 / (65536 - D), exact for that D. Bits: Philox4x32-10 of counter (i / 8, offset)
+ * and key seed; element i takes the low (i even) or high half of word (i % 8) / 2. The
+ * mask is never stored: the gradient of x is the same call on the gradient of out,
+ * without a residual. A dropped element is 0 whatever it held. `out` may be x or
+ * residual when they are contiguous. */
+int lgbm_b200_experts_dropout(const void* x, const void* residual, int32_t dtype, int64_t rows,
+                              int64_t width, int64_t pitch, int64_t residual_pitch, double p,
+                              uint64_t seed, uint64_t offset, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

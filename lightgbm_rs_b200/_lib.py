@@ -27,6 +27,7 @@ _P = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _u32 = ctypes.c_uint32
+_u64 = ctypes.c_uint64
 _f64 = ctypes.c_double
 
 
@@ -155,6 +156,26 @@ _SIGS = {
     "lgbm_b200_predictor_create": ([_i32, _P, _P], ctypes.c_int),
     "lgbm_b200_predictor_destroy": ([_P], ctypes.c_int),
     "lgbm_b200_predict": ([_P, _P, _i64, _i32, _P], ctypes.c_int),
+    "lgbm_b200_experts_route_workspace": ([_i64, _i32, _i32], _i64),
+    "lgbm_b200_experts_route": ([_P, _i32, _i64, _i32, _i64, _i32, _i32, _P, _P, _P, _P, _P, _P,
+                                 _i64, _P], ctypes.c_int),
+    "lgbm_b200_experts_route_backward": ([_P, _P, _P, _P, _i32, _i64, _i32, _i64, _i32, _i32, _P,
+                                          _P], ctypes.c_int),
+    "lgbm_b200_experts_matmul_workspace": ([_i32, _P, _i64, _P, _P, _i64, _P, _i64, _i32, _i32,
+                                            _i32], _i64),
+    "lgbm_b200_experts_matmul": ([_P, _i64, _i64, _P, _P, _P, _i32, _i64, _i32, _i32, _i32, _P,
+                                  _P, _i64, _P], ctypes.c_int),
+    "lgbm_b200_experts_matmul_input_grad": ([_P, _i64, _P, _P, _i32, _i64, _i32, _i32, _i32, _P,
+                                             _P, _i64, _P], ctypes.c_int),
+    "lgbm_b200_experts_matmul_weight_grad": ([_P, _i64, _P, _i64, _i64, _P, _P, _i32, _i32, _i64,
+                                              _i32, _i32, _i32, _P, _P, _i64, _P], ctypes.c_int),
+    "lgbm_b200_experts_errors": ([_P], ctypes.c_int),
+    "lgbm_b200_experts_combine": ([_P, _i32, _i64, _i32, _i64, _P, _P, _i64, _i32, _P, _P],
+                                  ctypes.c_int),
+    "lgbm_b200_experts_combine_backward": ([_P, _P, _i32, _i64, _i32, _i64, _i64, _P, _P, _i64,
+                                            _i32, _P, _P, _P], ctypes.c_int),
+    "lgbm_b200_experts_dropout": ([_P, _P, _i32, _i64, _i64, _i64, _i64, _f64, _u64, _u64, _P,
+                                   _P], ctypes.c_int),
 }
 
 _lib = None

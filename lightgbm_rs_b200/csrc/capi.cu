@@ -258,6 +258,10 @@ bool have_device() {
 
 }  // namespace
 
+namespace lgbm_b200 {
+int set_last_error(int code, const char* msg) { return fail(code, "%s", msg); }
+}  // namespace lgbm_b200
+
 // ----------------------------------------------------------------------------------
 // Dataset
 // ----------------------------------------------------------------------------------

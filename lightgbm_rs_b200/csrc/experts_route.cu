@@ -1,0 +1,454 @@
+// Routing rows to experts: the k largest logits of every row with their softmax weights, and
+// the rows' places when grouped by expert; the gradient of the weights.
+#include "experts.cuh"
+
+namespace lgbm_b200 {
+namespace experts {
+namespace {
+
+constexpr int kRouteThreads = 128;   // k_route_select, k_route_place
+constexpr int kRouteChunk = 64;      // logit columns staged at a time
+constexpr uint32_t kKeyEmpty = 0x007FFFFFu;  // key of -inf: never chosen
+
+// Order-preserving key of a logit: larger logit, larger key; -0 and +0 are one value, NaN
+// ranks above everything (it is then chosen, and its row's weights are NaN).
+__device__ __forceinline__ uint32_t logit_key(float v) {
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  const uint32_t key = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  return v != v ? 0xFFFFFFFFu : key;
+}
+__device__ __forceinline__ float key_logit(uint32_t key) {
+  return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+
+// Stable places of a block's slots, in slot order. chosen(i) gives slot i's expert (-1:
+// none); base[e] is the first place of the block's rows of expert e (e = experts: the slots
+// without an expert). Each warp ranks a contiguous run of slots: among 32 slots by matching
+// lanes, across its runs by a counter per expert that only it writes.
+template <int THREADS, typename Chosen>
+__device__ void place_slots(int slots, int64_t first_slot, int experts, int k,
+                            const Chosen& chosen, int32_t* base, int32_t* hist,
+                            int32_t* position, int32_t* rows) {
+  constexpr int kWarps = THREADS / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = experts + 1;
+  for (int i = threadIdx.x; i < kWarps * groups; i += THREADS) hist[i] = 0;
+  __syncthreads();
+  const int per_warp = ((slots + THREADS - 1) / THREADS) * 32;
+  const int begin = warp * per_warp;
+  int32_t* mine = hist + warp * groups;
+  for (int i0 = begin; i0 < begin + per_warp && i0 < slots; i0 += 32) {
+    const int i = i0 + lane;
+    int e = -2;
+    if (i < slots) {
+      e = chosen(i);
+      if (e < 0) e = experts;
+    }
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, e);
+    if (e >= 0 && (same & ((1u << lane) - 1u)) == 0) mine[e] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < groups; e += THREADS) {
+    int32_t at = base[e];
+    for (int w = 0; w < kWarps; ++w) {
+      const int32_t n = hist[w * groups + e];
+      hist[w * groups + e] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  for (int i0 = begin; i0 < begin + per_warp && i0 < slots; i0 += 32) {
+    const int i = i0 + lane;
+    int e = -2;
+    if (i < slots) {
+      e = chosen(i);
+      if (e < 0) e = experts;
+    }
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, e);
+    const uint32_t before = same & ((1u << lane) - 1u);
+    int32_t at = 0;
+    if (e >= 0) at = mine[e];
+    __syncwarp();
+    if (e >= 0) {
+      if (before == 0) mine[e] = at + __popc(same);
+      at += __popc(before);
+      position[first_slot + i] = at;
+      rows[at] = (int32_t)((first_slot + i) / k);
+    }
+    __syncwarp();
+  }
+}
+
+// Exclusive prefix of n <= kMaxExperts + 1 counts in shared memory by the first warp.
+__device__ void prefix_counts(int32_t* counts, int n) {
+  if (threadIdx.x < 32) {
+    int32_t carry = 0;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int i = i0 + threadIdx.x;
+      const int32_t v = i < n ? counts[i] : 0;
+      int32_t s = v;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int32_t o = __shfl_up_sync(0xFFFFFFFFu, s, d);
+        if ((int)threadIdx.x >= d) s += o;
+      }
+      if (i < n) counts[i] = carry + s - v;
+      carry += __shfl_sync(0xFFFFFFFFu, s, 31);
+    }
+  }
+}
+
+// The k largest logits of tokens [first, first + THREADS / L), L lanes a token: each lane
+// keeps the KP largest of its columns in registers, sorted, and the lanes' lists are merged
+// by k rounds of a maximum over (key, lowest column). Logits come through shared memory in
+// chunks of columns, so that global reads stay coalesced whatever L is.
+template <typename T, int L, int KP, int THREADS>
+__device__ void select_tokens(const T* logits, int64_t tokens, int experts, int64_t pitch,
+                              int k, bool normalize, int64_t first, uint32_t* tile,
+                              float* weights, int32_t* chosen, int (&ids)[KP]) {
+  constexpr int kTokens = THREADS / L;
+  constexpr int kStride = kRouteChunk + L;  // lanes of different tokens hit different banks
+  const int sub = threadIdx.x % L, tok = threadIdx.x / L;
+  uint32_t key[KP];
+  int idx[KP];
+#pragma unroll
+  for (int j = 0; j < KP; ++j) {
+    key[j] = kKeyEmpty;
+    idx[j] = -1;
+  }
+  float z = 0.0f;  // sum of exp(logit - largest so far) over this lane's columns
+  for (int e0 = 0; e0 < experts; e0 += kRouteChunk) {
+    const int n = min(kRouteChunk, experts - e0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kTokens * kRouteChunk; i += THREADS) {
+      const int r = i / kRouteChunk, c = i % kRouteChunk;
+      if (c < n && first + r < tokens)
+        tile[r * kStride + c] = logit_key(to_f32<T>(logits[(first + r) * pitch + e0 + c]));
+    }
+    __syncthreads();
+    if (first + tok < tokens) {
+      const uint32_t* row = tile + tok * kStride;
+      const uint32_t top = key[0];
+      for (int c = sub; c < n; c += L) {
+        const uint32_t v = row[c];
+        if (v > key[KP - 1]) {
+          // v > key[j] fails for the entries that stay before it: equal keys keep the
+          // lower column first
+#pragma unroll
+          for (int j = KP - 1; j > 0; --j) {
+            const bool up = v > key[j - 1];
+            const bool here = v > key[j];
+            idx[j] = up ? idx[j - 1] : (here ? e0 + c : idx[j]);
+            key[j] = up ? key[j - 1] : (here ? v : key[j]);
+          }
+          if (v > key[0]) {
+            key[0] = v;
+            idx[0] = e0 + c;
+          }
+        }
+      }
+      if (!normalize && key[0] != kKeyEmpty) {
+        const float m = key_logit(key[0]);
+        if (top != key[0]) z *= top == kKeyEmpty ? 0.0f : expf(key_logit(top) - m);
+        for (int c = sub; c < n; c += L) z += expf(key_logit(row[c]) - m);
+      }
+    }
+  }
+  const uint32_t lane_top = key[0];
+  uint32_t win_key[KP];
+#pragma unroll
+  for (int j = 0; j < KP; ++j) {
+    // (key, lowest column first): the largest of the lanes' first entries
+    uint64_t best = ((uint64_t)key[0] << 32) | (uint32_t)~idx[0];
+    const uint64_t own = best;
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) {
+      const uint64_t o = __shfl_xor_sync(0xFFFFFFFFu, best, d);
+      best = o > best ? o : best;
+    }
+    win_key[j] = (uint32_t)(best >> 32);
+    ids[j] = win_key[j] == kKeyEmpty ? -1 : ~(int)(uint32_t)best;
+    if (own == best && win_key[j] != kKeyEmpty) {
+#pragma unroll
+      for (int i = 0; i + 1 < KP; ++i) {
+        key[i] = key[i + 1];
+        idx[i] = idx[i + 1];
+      }
+      key[KP - 1] = kKeyEmpty;
+      idx[KP - 1] = -1;
+    }
+  }
+  const float m = win_key[0] == kKeyEmpty ? 0.0f : key_logit(win_key[0]);
+  float e[KP];
+  float total = 0.0f;
+#pragma unroll
+  for (int j = 0; j < KP; ++j) {
+    e[j] = ids[j] >= 0 ? expf(key_logit(win_key[j]) - m) : 0.0f;
+    if (j < k) total += e[j];
+  }
+  if (!normalize) {
+    total = lane_top == kKeyEmpty ? 0.0f : z * expf(key_logit(lane_top) - m);
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+  }
+  if (first + tok < tokens && sub == 0) {
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+      if (j < k) {
+        weights[(first + tok) * k + j] = ids[j] >= 0 ? e[j] / total : 0.0f;
+        chosen[(first + tok) * k + j] = ids[j];
+      }
+  }
+}
+
+// First of three launches: choice and weights, and each block's rows per expert.
+template <typename T, int L, int KP>
+__global__ void __launch_bounds__(kRouteThreads)
+    k_route_select(const T* logits, int64_t tokens, int experts, int64_t pitch, int k,
+                   bool normalize, float* weights, int32_t* chosen, int32_t* counts) {
+  __shared__ uint32_t tile[(kRouteThreads / L) * (kRouteChunk + L)];
+  __shared__ int32_t hist[kMaxExperts + 1];
+  constexpr int kTokens = kRouteThreads / L;
+  for (int i = threadIdx.x; i <= experts; i += kRouteThreads) hist[i] = 0;
+  int ids[KP];
+  const int64_t first = (int64_t)blockIdx.x * kTokens;
+  select_tokens<T, L, KP, kRouteThreads>(logits, tokens, experts, pitch, k, normalize, first,
+                                         tile, weights, chosen, ids);
+  if (threadIdx.x % L == 0 && first + threadIdx.x / L < tokens) {
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+      if (j < k) atomicAdd(&hist[ids[j] < 0 ? experts : ids[j]], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e <= experts; e += kRouteThreads)
+    counts[(int64_t)e * gridDim.x + blockIdx.x] = hist[e];
+}
+
+// Second: per expert, the exclusive prefix of the blocks' counts; one warp an expert.
+__global__ void __launch_bounds__(256) k_route_scan(int32_t* counts, int32_t* totals, int groups,
+                                                    int blocks) {
+  const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (e >= groups) return;
+  int32_t* row = counts + (int64_t)e * blocks;
+  int32_t carry = 0;
+  for (int i0 = 0; i0 < blocks; i0 += 32) {
+    const int i = i0 + lane;
+    const int32_t v = i < blocks ? row[i] : 0;
+    int32_t s = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int32_t o = __shfl_up_sync(0xFFFFFFFFu, s, d);
+      if (lane >= d) s += o;
+    }
+    if (i < blocks) row[i] = carry + s - v;
+    carry += __shfl_sync(0xFFFFFFFFu, s, 31);
+  }
+  if (lane == 0) totals[e] = carry;
+}
+
+// Third: offsets, and every slot's place.
+__global__ void __launch_bounds__(kRouteThreads)
+    k_route_place(const int32_t* chosen, const int32_t* counts, const int32_t* totals,
+                  int64_t tokens, int experts, int k, int block_tokens, int32_t* position,
+                  int32_t* rows, int32_t* offsets) {
+  extern __shared__ int32_t smem[];
+  int32_t* base = smem;
+  int32_t* hist = smem + experts + 1;
+  for (int e = threadIdx.x; e <= experts; e += kRouteThreads) base[e] = totals[e];
+  __syncthreads();
+  prefix_counts(base, experts + 1);
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= experts; e += kRouteThreads) offsets[e] = base[e];
+  __syncthreads();
+  for (int e = threadIdx.x; e <= experts; e += kRouteThreads)
+    base[e] += counts[(int64_t)e * gridDim.x + blockIdx.x];
+  const int64_t first = (int64_t)blockIdx.x * block_tokens;
+  const int n = (int)min((int64_t)block_tokens, tokens - first) * k;
+  const int32_t* mine = chosen + first * k;
+  place_slots<kRouteThreads>(
+      n, first * k, experts, k, [&](int i) { return mine[i]; }, base, hist, position, rows);
+}
+
+// A few tokens: all of it in one block, 32 lanes a token.
+constexpr int kSmallThreads = 512;
+constexpr int kSmallTokens = 64;  // most tokens this path takes: four rounds of 16
+
+template <typename T, int KP>
+__global__ void __launch_bounds__(kSmallThreads)
+    k_route_small(const T* logits, int tokens, int experts, int64_t pitch, int k,
+                  bool normalize, float* weights, int32_t* chosen, int32_t* position,
+                  int32_t* rows, int32_t* offsets) {
+  extern __shared__ int32_t smem[];
+  constexpr int kTokens = kSmallThreads / 32;
+  uint32_t* tile = reinterpret_cast<uint32_t*>(smem);       // kTokens * (chunk + 32)
+  int32_t* ids = smem + kTokens * (kRouteChunk + 32);       // kSmallTokens * k
+  int32_t* base = ids + kSmallTokens * kMaxChosen;          // experts + 1
+  int32_t* hist = base + experts + 1;                       // warps * (experts + 1)
+  for (int e = threadIdx.x; e <= experts; e += kSmallThreads) base[e] = 0;
+  for (int first = 0; first < tokens; first += kTokens) {
+    int mine[KP];
+    select_tokens<T, 32, KP, kSmallThreads>(logits, tokens, experts, pitch, k, normalize, first,
+                                            tile, weights, chosen, mine);
+    const int t = first + threadIdx.x / 32;
+    if (threadIdx.x % 32 == 0 && t < tokens) {
+#pragma unroll
+      for (int j = 0; j < KP; ++j)
+        if (j < k) {
+          ids[t * k + j] = mine[j];
+          atomicAdd(&base[mine[j] < 0 ? experts : mine[j]], 1);
+        }
+    }
+  }
+  __syncthreads();
+  prefix_counts(base, experts + 1);
+  __syncthreads();
+  for (int e = threadIdx.x; e <= experts; e += kSmallThreads) offsets[e] = base[e];
+  place_slots<kSmallThreads>(
+      tokens * k, 0, experts, k, [&](int i) { return ids[i]; }, base, hist, position, rows);
+}
+
+// Gradient of the logits, `lanes` lanes a token: with p the softmax (over the chosen experts
+// or over all) and g the gradient of the weights, dl_e = p_e ([e chosen] g_e - sum w g).
+// Over all experts the softmax is recomputed from one chosen logit: the first chosen one is
+// the largest, m, and its weight is 1 / sum exp(l - m).
+template <typename T, int KP>
+__global__ void __launch_bounds__(256)
+    k_route_backward(const float* dweights, const float* weights, const int32_t* chosen,
+                     const T* logits, int64_t tokens, int experts, int64_t pitch, int k,
+                     bool normalize, int lanes, T* dlogits) {
+  const int64_t t = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+  if (t >= tokens) return;
+  int id[KP];
+  float val[KP];
+  float s = 0.0f, w0 = 0.0f;
+#pragma unroll
+  for (int j = 0; j < KP; ++j) {
+    id[j] = -1;
+    val[j] = 0.0f;
+    if (j < k) {
+      id[j] = chosen[t * k + j];
+      const float w = weights[t * k + j];
+      if (j == 0) w0 = w;
+      if (id[j] >= 0) {
+        const float g = dweights[t * k + j];
+        s = fmaf(w, g, s);
+        val[j] = normalize ? g : w * g;
+      }
+    }
+  }
+  const bool any = id[0] >= 0 && id[0] < experts;
+  float m = 0.0f;
+  if (normalize) {
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+      if (j < k && id[j] >= 0) val[j] = weights[t * k + j] * (val[j] - s);
+  } else if (any) {
+    m = to_f32<T>(logits[t * pitch + id[0]]);
+  }
+  for (int e = threadIdx.x % lanes; e < experts; e += lanes) {
+    float d = 0.0f;
+    if (!normalize && any) d = -(expf(to_f32<T>(logits[t * pitch + e]) - m) * w0) * s;
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+      if (id[j] == e) d += val[j];
+    dlogits[t * experts + e] = from_f32<T>(d);
+  }
+}
+
+int route_lanes(int64_t tokens) { return tokens >= 16384 ? 1 : 8; }
+
+template <typename T, int KP>
+cudaError_t route_typed(const T* logits, int64_t tokens, int experts, int64_t pitch, int k,
+                        bool normalize, float* weights, int32_t* chosen, int32_t* position,
+                        int32_t* rows, int32_t* offsets, int32_t* ws, cudaStream_t st) {
+  if (tokens <= kSmallTokens) {
+    const size_t smem = sizeof(int32_t) * ((kSmallThreads / 32) * (kRouteChunk + 32) +
+                                           kSmallTokens * kMaxChosen +
+                                           (experts + 1) * (1 + kSmallThreads / 32));
+    k_route_small<T, KP><<<1, kSmallThreads, smem, st>>>(logits, (int)tokens, experts, pitch, k,
+                                                         normalize, weights, chosen, position,
+                                                         rows, offsets);
+    return cudaGetLastError();
+  }
+  const int lanes = route_lanes(tokens);
+  const int block_tokens = kRouteThreads / lanes;
+  const int blocks = (int)((tokens + block_tokens - 1) / block_tokens);
+  int32_t* totals = ws;
+  int32_t* counts = ws + experts + 1;
+  if (lanes == 1)
+    k_route_select<T, 1, KP><<<blocks, kRouteThreads, 0, st>>>(
+        logits, tokens, experts, pitch, k, normalize, weights, chosen, counts);
+  else
+    k_route_select<T, 8, KP><<<blocks, kRouteThreads, 0, st>>>(
+        logits, tokens, experts, pitch, k, normalize, weights, chosen, counts);
+  k_route_scan<<<(experts + 8) / 8, 256, 0, st>>>(counts, totals, experts + 1, blocks);
+  const size_t smem = sizeof(int32_t) * (experts + 1) * (1 + kRouteThreads / 32);
+  k_route_place<<<blocks, kRouteThreads, smem, st>>>(chosen, counts, totals, tokens, experts, k,
+                                                     block_tokens, position, rows, offsets);
+  return cudaGetLastError();
+}
+
+// KP: k rounded up, so that the sorted list stays in registers.
+template <typename F>
+cudaError_t with_chosen(int k, F&& f) {
+  if (k == 1) return f(std::integral_constant<int, 1>());
+  if (k == 2) return f(std::integral_constant<int, 2>());
+  if (k <= 4) return f(std::integral_constant<int, 4>());
+  if (k <= 8) return f(std::integral_constant<int, 8>());
+  return f(std::integral_constant<int, kMaxChosen>());
+}
+
+template <typename F>
+cudaError_t with_type(int32_t dtype, F&& f) {
+  if (dtype == LGBM_B200_DTYPE_F32) return f(float());
+  if (dtype == LGBM_B200_DTYPE_BF16) return f(__nv_bfloat16());
+  return f(__half());
+}
+
+}  // namespace
+
+int64_t route_workspace(int64_t tokens, int32_t experts, int32_t k) {
+  (void)k;
+  if (tokens <= kSmallTokens) return 0;
+  const int64_t block_tokens = kRouteThreads / route_lanes(tokens);
+  const int64_t blocks = (tokens + block_tokens - 1) / block_tokens;
+  return (int64_t)sizeof(int32_t) * (experts + 1) * (blocks + 1);
+}
+
+cudaError_t launch_route(const void* logits, int32_t dtype, int64_t tokens, int32_t experts,
+                         int64_t pitch, int32_t k, bool normalize, float* weights,
+                         int32_t* chosen, int32_t* position, int32_t* rows, int32_t* offsets,
+                         void* workspace, cudaStream_t st) {
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    return with_chosen(k, [&](auto kp) {
+      return route_typed<T, decltype(kp)::value>(
+          static_cast<const T*>(logits), tokens, experts, pitch, k, normalize, weights, chosen,
+          position, rows, offsets, static_cast<int32_t*>(workspace), st);
+    });
+  });
+}
+
+cudaError_t launch_route_backward(const float* dweights, const float* weights,
+                                  const int32_t* chosen, const void* logits, int32_t dtype,
+                                  int64_t tokens, int32_t experts, int64_t pitch, int32_t k,
+                                  bool normalize, void* dlogits, cudaStream_t st) {
+  int lanes = 32;  // the smallest power of two that covers the experts, at most a warp
+  while (lanes > 1 && lanes / 2 >= experts) lanes /= 2;
+  const int64_t per_block = 256 / lanes;
+  const int64_t blocks = (tokens + per_block - 1) / per_block;
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    return with_chosen(k, [&](auto kp) {
+      k_route_backward<T, decltype(kp)::value><<<(unsigned)blocks, 256, 0, st>>>(
+          dweights, weights, chosen, static_cast<const T*>(logits), tokens, experts, pitch, k,
+          normalize, lanes, static_cast<T*>(dlogits));
+      return cudaGetLastError();
+    });
+  });
+}
+
+}  // namespace experts
+}  // namespace lgbm_b200

@@ -1,0 +1,306 @@
+// Row operators of the expert layer: the weighted combination of each token's rows with its
+// gradient, and dropout from a counter-based generator.
+#include <algorithm>
+
+#include "experts.cuh"
+
+namespace lgbm_b200 {
+namespace experts {
+namespace {
+
+constexpr int kRowThreads = 256;
+
+// out[t] = sum_j w[t, j] y[position[t, j]] in f32, rounded once. A row of `lanes` threads a
+// token; the k rows are read independently of each other, four in flight a thread.
+template <typename T, int V>
+__global__ void __launch_bounds__(kRowThreads)
+    k_combine(const T* y, int64_t rows, int width, int64_t pitch, const int32_t* position,
+              const float* weights, int64_t tokens, int k, int lanes, T* out) {
+  const int64_t t = (int64_t)blockIdx.x * (kRowThreads / lanes) + threadIdx.x / lanes;
+  if (t >= tokens) return;
+  for (int c = (threadIdx.x % lanes) * V; c < width; c += lanes * V) {
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+#pragma unroll 4
+    for (int j = 0; j < k; ++j) {
+      const int32_t at = position[t * k + j];
+      const float w = weights ? weights[t * k + j] : 1.0f;
+      if (at >= 0 && at < rows) {
+        float v[V];
+        load_f32<T, V>(y + at * pitch + c, v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+      }
+    }
+    store_f32<T, V>(out + t * width + c, acc);
+  }
+}
+
+// dy[position[t, j]] = w[t, j] dout[t] and dw[t, j] = <dout[t], y[position[t, j]]>, JC chosen
+// rows at a time: dout is read once for them. The dot products are summed over the token's
+// lanes in a fixed order, so they do not change from run to run.
+template <typename T, int V, int LANES, int JC>
+__global__ void __launch_bounds__(kRowThreads)
+    k_combine_backward(const T* dout, const T* y, int64_t rows, int width, int64_t dout_pitch,
+                       int64_t pitch, const int32_t* position, const float* weights,
+                       int64_t tokens, int k, T* dy, float* dweights) {
+  __shared__ float part[kRowThreads / 32][JC];
+  const int64_t t = (int64_t)blockIdx.x * (kRowThreads / LANES) + threadIdx.x / LANES;
+  const int lane = threadIdx.x % LANES;
+  if (t >= tokens) return;  // whole warps: LANES is 32 or the block
+  for (int j0 = 0; j0 < k; j0 += JC) {
+    int64_t at[JC];
+    float w[JC], dot[JC];
+#pragma unroll
+    for (int j = 0; j < JC; ++j) {
+      at[j] = -1;
+      w[j] = dot[j] = 0.0f;
+      if (j0 + j < k) {
+        const int32_t p = position[t * k + j0 + j];
+        if (p >= 0 && p < rows) at[j] = p;
+        w[j] = weights ? weights[t * k + j0 + j] : 1.0f;
+      }
+    }
+    for (int c = lane * V; c < width; c += LANES * V) {
+      float g[V], v[JC][V];
+      load_f32<T, V>(dout + t * dout_pitch + c, g);
+#pragma unroll
+      for (int j = 0; j < JC; ++j)
+        if (at[j] >= 0 && dweights) load_f32<T, V>(y + at[j] * pitch + c, v[j]);
+#pragma unroll
+      for (int j = 0; j < JC; ++j) {
+        if (at[j] < 0) continue;
+        float d[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          d[i] = w[j] * g[i];
+          if (dweights) dot[j] = fmaf(g[i], v[j][i], dot[j]);
+        }
+        store_f32<T, V>(dy + at[j] * width + c, d);
+      }
+    }
+    if (!dweights) continue;
+#pragma unroll
+    for (int j = 0; j < JC; ++j)
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) dot[j] += __shfl_xor_sync(0xFFFFFFFFu, dot[j], d);
+    if constexpr (LANES > 32) {
+      if (threadIdx.x % 32 == 0)
+#pragma unroll
+        for (int j = 0; j < JC; ++j) part[threadIdx.x / 32][j] = dot[j];
+      __syncthreads();
+      if (threadIdx.x == 0)
+#pragma unroll
+        for (int j = 0; j < JC; ++j) {
+          float s = 0.0f;
+          for (int i = 0; i < LANES / 32; ++i) s += part[i][j];
+          if (j0 + j < k) dweights[t * k + j0 + j] = s;
+        }
+      __syncthreads();
+    } else if (lane == 0) {
+#pragma unroll
+      for (int j = 0; j < JC; ++j)
+        if (j0 + j < k) dweights[t * k + j0 + j] = dot[j];
+    }
+  }
+}
+
+// Philox4x32-10 (J. Salmon, M. Moraes, R. Dror, D. Shaw, "Parallel random numbers: as easy
+// as 1, 2, 3", 2011): ten rounds of two 32 x 32 -> 64 bit products and xors on a counter of
+// 128 bits, keyed by 64 bits.
+__device__ __forceinline__ uint4 philox(uint64_t block, uint64_t offset, uint32_t k0,
+                                        uint32_t k1) {
+  uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32);
+  uint32_t c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t p = (uint64_t)0xD2511F53u * c0, q = (uint64_t)0xCD9E8D57u * c2;
+    const uint32_t n0 = (uint32_t)(q >> 32) ^ c1 ^ k0, n2 = (uint32_t)(p >> 32) ^ c3 ^ k1;
+    c1 = (uint32_t)q;
+    c3 = (uint32_t)p;
+    c0 = n0;
+    c2 = n2;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+__device__ __forceinline__ uint32_t half_word(const uint4& r, int i) {
+  const uint32_t w = i < 2 ? r.x : i < 4 ? r.y : i < 6 ? r.z : r.w;
+  return (i & 1) ? w >> 16 : w & 0xFFFFu;
+}
+
+// Element i takes 16 bits of block i / 8 and is kept when they are at least `drop`: the mask
+// is recomputed wherever it is needed and never stored. One thread makes one block and
+// handles its eight elements. VEC: rows of one pitch that 16-byte accesses can walk (a
+// contiguous array counts as one row). A dropped element is 0 whatever it held.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kRowThreads)
+    k_dropout(const T* x, const T* residual, int64_t n, int64_t width, int64_t pitch,
+              int64_t residual_pitch, uint32_t drop, float scale, uint64_t seed,
+              uint64_t offset, T* out) {
+  const int64_t blocks = (n + 7) / 8;
+  for (int64_t b = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; b < blocks;
+       b += (int64_t)gridDim.x * kRowThreads) {
+    const int64_t i0 = b * 8;
+    if (VEC && i0 + 8 <= n) {
+      int64_t at = i0, rat = i0;
+      if (width != n) {
+        const int64_t r = i0 / width, c = i0 - r * width;
+        at = r * pitch + c;
+        rat = r * residual_pitch + c;
+      }
+      constexpr int V = 16 / (int)sizeof(T);
+      float v[8], a[8];
+#pragma unroll
+      for (int i = 0; i < 8; i += V)
+        load_f32<T, V>(x + at + i, reinterpret_cast<float(&)[V]>(v[i]));
+      if (residual)
+#pragma unroll
+        for (int i = 0; i < 8; i += V)
+          load_f32<T, V>(residual + rat + i, reinterpret_cast<float(&)[V]>(a[i]));
+      const uint4 rnd = philox((uint64_t)b, offset, (uint32_t)seed, (uint32_t)(seed >> 32));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = half_word(rnd, i) >= drop ? v[i] * scale : 0.0f;
+        if (residual) v[i] += a[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i += V)
+        store_f32<T, V>(out + i0 + i, reinterpret_cast<float(&)[V]>(v[i]));
+    } else {
+      const uint4 rnd = philox((uint64_t)b, offset, (uint32_t)seed, (uint32_t)(seed >> 32));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i0 + i >= n) break;
+        const int64_t r = (i0 + i) / width, c = (i0 + i) - r * width;
+        float v = to_f32<T>(x[r * pitch + c]);
+        v = half_word(rnd, i) >= drop ? v * scale : 0.0f;
+        if (residual) v += to_f32<T>(residual[r * residual_pitch + c]);
+        out[i0 + i] = from_f32<T>(v);
+      }
+    }
+  }
+}
+
+// Threads that share a token's row: the smallest power of two that covers it, 32 to 256.
+int row_lanes(int64_t vectors) {
+  int lanes = 1;
+  while (lanes < kRowThreads && lanes < vectors) lanes *= 2;
+  return lanes;
+}
+
+template <typename F>
+cudaError_t with_type(int32_t dtype, F&& f) {
+  if (dtype == LGBM_B200_DTYPE_F32) return f(float());
+  if (dtype == LGBM_B200_DTYPE_BF16) return f(__nv_bfloat16());
+  return f(__half());
+}
+
+template <typename T, int V>
+cudaError_t combine_typed(const T* y, int64_t rows, int width, int64_t pitch,
+                          const int32_t* position, const float* weights, int64_t tokens, int k,
+                          T* out, cudaStream_t st) {
+  const int lanes = row_lanes((width + V - 1) / V);
+  const int64_t per_block = kRowThreads / lanes;
+  k_combine<T, V><<<(unsigned)((tokens + per_block - 1) / per_block), kRowThreads, 0, st>>>(
+      y, rows, width, pitch, position, weights, tokens, k, lanes, out);
+  return cudaGetLastError();
+}
+
+template <typename T, int V, int LANES>
+cudaError_t combine_backward_typed(const T* dout, const T* y, int64_t rows, int width,
+                                   int64_t dout_pitch, int64_t pitch, const int32_t* position,
+                                   const float* weights, int64_t tokens, int k, T* dy,
+                                   float* dweights, cudaStream_t st) {
+  const int64_t per_block = kRowThreads / LANES;
+  const unsigned blocks = (unsigned)((tokens + per_block - 1) / per_block);
+  if (k <= 2)
+    k_combine_backward<T, V, LANES, 2><<<blocks, kRowThreads, 0, st>>>(
+        dout, y, rows, width, dout_pitch, pitch, position, weights, tokens, k, dy, dweights);
+  else
+    k_combine_backward<T, V, LANES, 4><<<blocks, kRowThreads, 0, st>>>(
+        dout, y, rows, width, dout_pitch, pitch, position, weights, tokens, k, dy, dweights);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_combine(const void* y, int32_t dtype, int64_t rows, int32_t width,
+                           int64_t pitch, const int32_t* position, const float* weights,
+                           int64_t tokens, int32_t k, void* out, cudaStream_t st) {
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    constexpr int V = 16 / sizeof(T);
+    const T* p = static_cast<const T*>(y);
+    T* o = static_cast<T*>(out);
+    if (width % V == 0 && pitch % V == 0 && aligned16(y) && aligned16(out))
+      return combine_typed<T, V>(p, rows, width, pitch, position, weights, tokens, k, o, st);
+    return combine_typed<T, 1>(p, rows, width, pitch, position, weights, tokens, k, o, st);
+  });
+}
+
+cudaError_t launch_combine_backward(const void* dout, const void* y, int32_t dtype,
+                                    int64_t rows, int32_t width, int64_t dout_pitch,
+                                    int64_t pitch, const int32_t* position,
+                                    const float* weights, int64_t tokens, int32_t k, void* dy,
+                                    float* dweights, cudaStream_t st) {
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    constexpr int V = 16 / sizeof(T);
+    const T* g = static_cast<const T*>(dout);
+    const T* p = static_cast<const T*>(y);
+    T* o = static_cast<T*>(dy);
+    const bool vec = width % V == 0 && dout_pitch % V == 0 && pitch % V == 0 &&
+                     aligned16(dout) && aligned16(y) && aligned16(dy);
+    auto go = [&](auto v, auto lanes) {
+      return combine_backward_typed<T, decltype(v)::value, decltype(lanes)::value>(
+          g, p, rows, width, dout_pitch, pitch, position, weights, tokens, k, o, dweights, st);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Vec = std::integral_constant<int, V>;
+    using Warp = std::integral_constant<int, 32>;
+    using Block = std::integral_constant<int, kRowThreads>;
+    // A block a token while a warp a token would leave SMs without work or a lane with a
+    // long row.
+    const bool wide = (width + (vec ? V : 1) - 1) / (vec ? V : 1) >= kRowThreads / 2;
+    if (vec) return wide ? go(Vec(), Block()) : go(Vec(), Warp());
+    return wide ? go(One(), Block()) : go(One(), Warp());
+  });
+}
+
+cudaError_t launch_dropout(const void* x, const void* residual, int32_t dtype, int64_t rows,
+                           int64_t width, int64_t pitch, int64_t residual_pitch, uint32_t drop,
+                           uint64_t seed, uint64_t offset, void* out, cudaStream_t st) {
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    constexpr int V = 16 / sizeof(T);
+    const int64_t n = rows * width;
+    if (n == 0) return cudaSuccess;
+    if (pitch == width && (!residual || residual_pitch == width)) {
+      width = n;  // contiguous: one row
+      pitch = residual_pitch = n;
+    }
+    const bool vec = aligned16(x) && aligned16(out) && (!residual || aligned16(residual)) &&
+                     (width == n || (width % 8 == 0 && pitch % V == 0 &&
+                                     (!residual || residual_pitch % V == 0)));
+    const float scale = drop < 65536u ? (float)(65536.0 / (65536.0 - (double)drop)) : 0.0f;
+    const int64_t want = ((n + 7) / 8 + kRowThreads - 1) / kRowThreads;
+    const unsigned blocks = (unsigned)std::min<int64_t>(want, 0x7FFFFFFF);
+    const T* p = static_cast<const T*>(x);
+    const T* r = static_cast<const T*>(residual);
+    T* o = static_cast<T*>(out);
+    if (vec)
+      k_dropout<T, true><<<blocks, kRowThreads, 0, st>>>(p, r, n, width, pitch, residual_pitch,
+                                                         drop, scale, seed, offset, o);
+    else
+      k_dropout<T, false><<<blocks, kRowThreads, 0, st>>>(p, r, n, width, pitch, residual_pitch,
+                                                          drop, scale, seed, offset, o);
+    return cudaGetLastError();
+  });
+}
+
+}  // namespace experts
+}  // namespace lgbm_b200
