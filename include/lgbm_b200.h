@@ -601,6 +601,20 @@ int lgbm_b200_experts_matmul_weight_grad(const void* dy, int64_t dy_pitch, const
                                          int32_t out_dtype, int64_t rows, int32_t experts,
                                          int32_t inner, int32_t outer, void* dw, void* workspace,
                                          int64_t workspace_bytes, void* stream);
+/* y as lgbm_b200_experts_matmul, for a few rows an expert, with weights of 4 bits in groups
+ * of group_size (32, 64 or 128) along the inner axis:
+ *   w[e][n][k] = scales[e][n][k / group_size] * (q - z)
+ * q: the weight's 4 bits, packed like a 4-bit bin row: [experts][outer][stride] bytes, weight
+ * 2i in the low half of byte i, stride = ceil(inner / 2) rounded up to 16, 16-byte aligned
+ * base. scales: x's type, [experts][outer][ceil(inner / group_size)]. z: zeros[e][n][group]
+ * (0..15), or 8 where zeros is NULL. Products of q - z are summed in f32 within a group,
+ * then scaled in f32: no weight is rounded to 16 bits. */
+int lgbm_b200_experts_matmul_w4(const void* x, int64_t x_rows, int64_t x_pitch,
+                                const int32_t* index, const uint8_t* q, const void* scales,
+                                const uint8_t* zeros, int32_t group_size,
+                                const int32_t* offsets, int32_t dtype, int64_t rows,
+                                int32_t experts, int32_t inner, int32_t outer, void* y,
+                                void* stream);
 /* Every wait inside the product kernels is bounded. One that ran out leaves its outputs
  * incomplete and sets a bit here: this call waits for the device, reads the bits of the
  * current device and clears them. */

@@ -169,6 +169,8 @@ _SIGS = {
                                              _P, _i64, _P], ctypes.c_int),
     "lgbm_b200_experts_matmul_weight_grad": ([_P, _i64, _P, _i64, _i64, _P, _P, _i32, _i32, _i64,
                                               _i32, _i32, _i32, _P, _P, _i64, _P], ctypes.c_int),
+    "lgbm_b200_experts_matmul_w4": ([_P, _i64, _i64, _P, _P, _P, _P, _i32, _P, _i32, _i64, _i32,
+                                     _i32, _i32, _P, _P], ctypes.c_int),
     "lgbm_b200_experts_errors": ([_P], ctypes.c_int),
     "lgbm_b200_experts_combine": ([_P, _i32, _i64, _i32, _i64, _P, _P, _i64, _i32, _P, _P],
                                   ctypes.c_int),

@@ -120,5 +120,22 @@ int64_t matmul_workspace(const MatmulCall& c);
 cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st);
 cudaError_t read_matmul_errors(uint32_t* bits);
 
+// experts_few.cu
+struct FewCall {
+  int32_t dtype;
+  const void* x;           // [x_rows, inner]
+  int64_t x_rows, x_pitch;
+  const int32_t* index;    // row of x of every grouped row, or null
+  const void* w;           // [experts, outer, inner], or 4 bits
+  int32_t group_size;      // 0: weights of 16 bits, else 32, 64 or 128
+  const void* scales;
+  const uint8_t* zeros;
+  const int32_t* offsets;
+  int64_t rows;
+  int32_t experts, inner, outer;
+  void* y;
+};
+cudaError_t launch_few(const FewCall& c, cudaStream_t st);
+
 }  // namespace experts
 }  // namespace lgbm_b200

@@ -288,6 +288,39 @@ int lgbm_b200_experts_matmul_weight_grad(const void* dy, int64_t dy_pitch, const
   return run_product("experts_matmul_weight_grad", c, workspace, workspace_bytes, stream);
 }
 
+int lgbm_b200_experts_matmul_w4(const void* x, int64_t x_rows, int64_t x_pitch,
+                                const int32_t* index, const uint8_t* q, const void* scales,
+                                const uint8_t* zeros, int32_t group_size,
+                                const int32_t* offsets, int32_t dtype, int64_t rows,
+                                int32_t experts, int32_t inner, int32_t outer, void* y,
+                                void* stream) {
+  const char* what = "experts_matmul_w4";
+  MatmulCall c{};
+  c.dtype = c.out_dtype = dtype;
+  c.x = x;
+  c.x_rows = x_rows;
+  c.x_pitch = x_pitch;
+  c.index = index;
+  c.w = q;
+  c.offsets = offsets;
+  c.rows = rows;
+  c.experts = experts;
+  c.inner = inner;
+  c.outer = outer;
+  c.out = y;
+  if (int rc = check_product(what, c)) return rc;
+  if (group_size != 32 && group_size != 64 && group_size != 128)
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: group size %d is not 32, 64 or 128", what,
+                  group_size);
+  if (!scales) return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
+  if (!aligned16(q))
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: weights are not 16-byte aligned", what);
+  if (rows == 0) return LGBM_B200_OK;
+  FewCall f{dtype, x,      x_rows, x_pitch, index, q,     group_size, scales,
+            zeros, offsets, rows,   experts, inner, outer, y};
+  return launched(launch_few(f, reinterpret_cast<cudaStream_t>(stream)), what);
+}
+
 int lgbm_b200_experts_errors(uint32_t* bits_out) {
   if (!bits_out) return refuse(LGBM_B200_INVALID_ARGUMENT, "experts_errors: null argument");
   return launched(read_matmul_errors(bits_out), "experts_errors");

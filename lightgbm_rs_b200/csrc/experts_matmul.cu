@@ -662,8 +662,12 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, int64_t rows, const Ope
 
 }  // namespace
 
+// Few rows an expert: the forward product streams the weights instead (experts_few.cu).
+bool few_rows(const MatmulCall& c) { return c.mode == 0 && c.rows <= 16 * (int64_t)c.experts; }
+
 int64_t matmul_workspace(const MatmulCall& c) {
   int64_t n = 0;
+  if (few_rows(c)) return 0;
   if (c.mode != 1 && (c.index || !walkable(c.x, c.x_pitch))) n += copy_bytes(c.rows, c.inner);
   if (c.mode != 0 && !walkable(c.dy, c.dy_pitch)) n += copy_bytes(c.rows, c.outer);
   if (c.mode != 2 && !(aligned16(c.w) && c.inner % 8 == 0))
@@ -672,6 +676,22 @@ int64_t matmul_workspace(const MatmulCall& c) {
 }
 
 cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st) {
+  if (few_rows(c)) {
+    FewCall f{};
+    f.dtype = c.dtype;
+    f.x = c.x;
+    f.x_rows = c.x_rows;
+    f.x_pitch = c.x_pitch;
+    f.index = c.index;
+    f.w = c.w;
+    f.offsets = c.offsets;
+    f.rows = c.rows;
+    f.experts = c.experts;
+    f.inner = c.inner;
+    f.outer = c.outer;
+    f.y = c.out;
+    return launch_few(f, st);
+  }
   char* ws = static_cast<char*>(workspace);
   MatArgs g{};
   g.offsets = c.offsets;

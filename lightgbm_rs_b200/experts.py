@@ -5,6 +5,7 @@ for every token from a gate's logits (experts masked with -inf are never picked:
 all but those of the leaf a tree sends the token to) and groups the T * k slots by expert;
 `grouped_matmul` multiplies each expert's ragged range of rows by its matrix; `combine` joins
 a token's k results; `dropout` regularises while training. Each has its gradient beside it.
+`grouped_matmul_w4` serves a few rows from weights of 4 bits.
 
     r = experts.route(logits, k)                                # [T, E]
     h = experts.grouped_matmul(x, w1, r.offsets, rows=r.rows)   # x [T, K], w1 [E, H, K]
@@ -26,7 +27,7 @@ import torch
 from . import _lib as C
 
 __all__ = ["Routing", "route", "route_backward", "grouped_matmul", "grouped_matmul_backward",
-           "combine", "combine_backward", "dropout", "dropout_backward", "check_errors"]
+           "grouped_matmul_w4", "quantize_w4", "combine", "combine_backward", "dropout", "dropout_backward", "check_errors"]
 
 Routing = namedtuple("Routing", ["weights", "experts", "position", "rows", "offsets"])
 Routing.__doc__ = """What `route` returns, M = T * k slots:
@@ -211,6 +212,61 @@ def grouped_matmul_backward(dy, x, w, offsets, rows=None, grad_dtype=None, need_
               x_pitch, ip, op, dtype, _DTYPES[grad_dtype], m, experts, inner, outer,
               dw.data_ptr(), wsp, need)
     return dx, dw
+
+
+def grouped_matmul_w4(x, q, scales, offsets, zeros=None, rows=None, group_size=128):
+    """`grouped_matmul` with 4-bit weights, for a few rows an expert: w = scales (q - zeros)
+    in groups of `group_size` (32, 64 or 128) along the inner axis. q [E, outer, stride]
+    uint8 packed like a 4-bit bin row (weight 2i in the low half of byte i, stride
+    ceil(inner / 2) rounded up to 16); scales [E, outer, groups] of x's type; zeros
+    [E, outer, groups] uint8 (None: 8). `quantize_w4` makes them."""
+    x, pitch = _rows2d("grouped_matmul_w4", x, _HALVES)
+    inner, dev, size = x.shape[1], x.device, int(group_size)
+    if q.dim() != 3 or scales.dim() != 3 or size not in (32, 64, 128):
+        _refuse(f"grouped_matmul_w4: q {tuple(q.shape)}, scales {tuple(scales.shape)}, groups "
+                f"of {group_size}")
+    experts, outer, _ = q.shape
+    q = _same("grouped_matmul_w4: q", q, dev, torch.uint8,
+              torch.Size((experts, outer, (inner + 31) // 32 * 16)))
+    shape = torch.Size((experts, outer, -(-inner // size)))
+    scales = _same("grouped_matmul_w4: scales", scales, dev, x.dtype, shape)
+    if zeros is not None:
+        zeros = _same("grouped_matmul_w4: zeros", zeros, dev, torch.uint8, shape)
+    offsets = _same("grouped_matmul_w4: offsets", offsets, dev, torch.int32,
+                    torch.Size((experts + 1,)))
+    m, index = _index("grouped_matmul_w4", rows, x)
+    y = _empty((m, outer), dtype=x.dtype, device=dev)
+    _call(dev, C.lib().lgbm_b200_experts_matmul_w4, x.data_ptr(), x.shape[0], pitch,
+          None if index is None else index.data_ptr(), q.data_ptr(), scales.data_ptr(),
+          None if zeros is None else zeros.data_ptr(), size, offsets.data_ptr(),
+          _HALVES[x.dtype], m, experts, inner, outer, y.data_ptr())
+    return y
+
+
+def quantize_w4(w, group_size=128, symmetric=False):
+    """(q, scales, zeros) of weights [E, outer, inner] (bf16 or f16) for `grouped_matmul_w4`,
+    once, when a trained layer is laid out for serving. Each group's range, stretched to hold
+    0, is divided into 15 steps; symmetric: 7 steps to its largest magnitude, zeros None."""
+    if w.dim() != 3 or w.dtype not in _HALVES or group_size not in (32, 64, 128):
+        _refuse(f"quantize_w4: {tuple(w.shape)} {w.dtype}, groups of {group_size}")
+    experts, outer, inner = w.shape
+    groups = -(-inner // group_size)
+    v = torch.nn.functional.pad(w.float(), (0, groups * group_size - inner))
+    v = v.view(experts, outer, groups, group_size)
+    if symmetric:
+        scales = v.abs().amax(3) / 7
+        zero = torch.full_like(scales, 8)
+    else:
+        low, high = v.amin(3).clamp(max=0), v.amax(3).clamp(min=0)
+        scales = (high - low) / 15
+        zero = torch.where(scales > 0, -low / scales, 8.0).round().clamp(0, 15)
+    scales = scales.to(w.dtype)
+    s = scales.float()[..., None]
+    q = (torch.where(s > 0, v / s, 0.0).round() + zero[..., None]).clamp(0, 15).to(torch.uint8)
+    q = q.view(experts, outer, -1)[:, :, :inner]
+    q = torch.nn.functional.pad(q, (0, (inner + 31) // 32 * 32 - inner))
+    q = (q[:, :, 0::2] | q[:, :, 1::2] << 4).contiguous()
+    return q, scales.contiguous(), None if symmetric else zero.to(torch.uint8).contiguous()
 
 
 def combine(y, position, weights=None):

@@ -40,7 +40,7 @@ def test_arguments_are_refused_with_a_status(capi):
     assert mm(p, 4, 8, None, p, p, 1, 4, 513, 8, 8, p, None, 0, None) == cap
     assert mm(p, 4, 7, None, p, p, 1, 4, 2, 8, 8, p, None, 0, None) == length
     assert mm(p, 5, 8, None, p, p, 1, 4, 2, 8, 8, p, None, 0, None) == length
-    assert mm(p, 4, 9, None, p, p, 1, 4, 2, 9, 8, p, None, 0, None) == length  # workspace
+    assert mm(p, 400, 9, None, p, p, 1, 400, 2, 9, 8, p, None, 0, None) == length  # workspace
     assert mm(p, 4, 8, None, None, p, 1, 4, 2, 8, 8, p, None, 0, None) == bad
     assert mm(p, 0, 8, None, p, p, 1, 0, 2, 8, 8, p, None, 0, None) == capi.OK
     dw = L.lgbm_b200_experts_matmul_weight_grad
@@ -48,6 +48,11 @@ def test_arguments_are_refused_with_a_status(capi):
     assert dw(p, 7, p, 4, 8, None, p, 1, 1, 4, 2, 8, 8, p, None, 0, None) == length
     dx = L.lgbm_b200_experts_matmul_input_grad
     assert dx(None, 8, p, p, 1, 4, 2, 8, 8, p, None, 0, None) == bad
+    w4 = L.lgbm_b200_experts_matmul_w4
+    assert w4(p, 4, 8, None, p, p, None, 48, p, 1, 4, 2, 8, 8, p, None) == bad
+    assert w4(p, 4, 8, None, p + 8, p, None, 32, p, 1, 4, 2, 8, 8, p, None) == bad
+    assert w4(p, 4, 8, None, p, None, None, 32, p, 1, 4, 2, 8, 8, p, None) == bad
+    assert w4(p, 4, 8, None, p, p, None, 32, p, 0, 4, 2, 8, 8, p, None) == bad
 
     comb = L.lgbm_b200_experts_combine
     assert comb(p, 3, 4, 8, 8, p, None, 2, 2, p, None) == bad
@@ -68,8 +73,8 @@ def test_arguments_are_refused_with_a_status(capi):
 def test_workspace_only_where_an_operand_must_be_copied(capi):
     ws = capi.lib().lgbm_b200_experts_matmul_workspace
     p = 1 << 20
-    assert ws(0, p, 64, None, None, 0, p, 100, 4, 64, 33) == 0
-    assert ws(0, p, 64, None, None, 0, p + 2, 100, 4, 64, 33) > 0
-    assert ws(0, p, 65, None, None, 0, p, 100, 4, 64, 33) > 0
-    assert ws(1, None, 0, None, p, 33, p, 100, 4, 64, 33) > 0
-    assert ws(2, p, 64, None, p, 40, None, 100, 4, 64, 33) == 0
+    assert ws(0, p, 64, None, None, 0, p, 1000, 4, 64, 33) == 0
+    assert ws(0, p, 64, None, None, 0, p + 2, 1000, 4, 64, 33) > 0
+    assert ws(0, p, 65, None, None, 0, p, 1000, 4, 64, 33) > 0
+    assert ws(1, None, 0, None, p, 33, p, 1000, 4, 64, 33) > 0
+    assert ws(2, p, 64, None, p, 40, None, 1000, 4, 64, 33) == 0

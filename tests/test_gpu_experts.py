@@ -335,6 +335,92 @@ def test_products_without_rows(ops):
     assert dx.shape == (0, 32) and not dw.any()
 
 
+# ------------------------------------------------------------------------- few rows, 4 bits
+
+
+FEW = [  # counts, tail rows, inner, outer
+    ([1], 0, 1, 1), ([0, 1, 0, 1], 0, 4096, 300), ([3, 0, 9], 2, 700, 129), ([8, 8, 8, 8], 0, 512, 128),
+    ([33, 0, 0, 1], 3, 513, 1000), ([65], 0, 2000, 72), ([2] * 40, 1, 75, 50), ([1] * 300, 0, 64, 40),
+    ([0, 0, 0], 4, 100, 20), ([7, 1, 30, 2, 0, 5], 0, 1028, 260),
+]
+
+
+@pytest.mark.parametrize("through_rows", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("counts,tail,inner,outer", FEW)
+def test_product_of_few_rows(ops, counts, tail, inner, outer, dtype, through_rows):
+    dt, g = DTYPES[dtype], gen(inner + outer)
+    m, E = sum(counts) + tail, len(counts)
+    tokens = m // 2 + 3 if through_rows else m
+    x = torch.randn(tokens, inner, generator=g, device="cuda").to(dt)
+    w = (torch.randn(E, outer, inner, generator=g, device="cuda") * inner ** -0.5).to(dt)
+    rows = None
+    if through_rows:
+        rows = torch.randint(-1, tokens + 1, (m,), generator=g, device="cuda").int()
+    off = offsets_of(counts)
+    _, y64, mag = product64(x, w, off, rows)
+    close(ops.grouped_matmul(x, w, off, rows=rows), y64, inner * 2.0 ** -23 * mag)
+
+
+def unpacked(q, scales, zeros, inner, group):
+    v = torch.stack([q & 15, q >> 4], 3).flatten(2)[:, :, :inner].double()
+    at = torch.arange(inner, device="cuda") // group
+    z = 8.0 if zeros is None else zeros.double()[:, :, at]
+    return (v - z) * scales.double()[:, :, at]
+
+
+@pytest.mark.parametrize("with_zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("counts,tail,inner,outer", FEW)
+def test_product_w4(ops, counts, tail, inner, outer, dtype, group, with_zeros):
+    """Every weight is scale * (q - z) exactly; n products and n / group scalings in f32."""
+    dt, g = DTYPES[dtype], gen(inner * 3 + group)
+    m, E = sum(counts) + tail, len(counts)
+    x = torch.randn(m, inner, generator=g, device="cuda").to(dt)
+    q = torch.randint(0, 256, (E, outer, (inner + 31) // 32 * 16), generator=g, device="cuda",
+                      dtype=torch.uint8)  # what the padding holds does not matter
+    groups = -(-inner // group)
+    scales = torch.randn(E, outer, groups, generator=g, device="cuda").to(dt)
+    zeros = None
+    if with_zeros:
+        zeros = torch.randint(0, 16, (E, outer, groups), generator=g, device="cuda",
+                              dtype=torch.uint8)
+    off = offsets_of(counts)
+    w = unpacked(q, scales, zeros, inner, group)
+    _, y64, _ = product64(x, w, off, None)
+    # inside a group the sum runs over |x| |q - z|, whatever cancels there
+    _, _, mag = product64(x, w.abs(), off, None)
+    got = ops.grouped_matmul_w4(x, q, scales, off, zeros=zeros, group_size=group)
+    close(got, y64, (inner + groups) * 2.0 ** -23 * mag)
+
+
+def test_w4_through_rows_and_strides(ops):
+    g = gen(21)
+    big = torch.randn(9, 400, generator=g, device="cuda").to(torch.float16)
+    q = torch.randint(0, 256, (3, 60, 112), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.rand(3, 60, 4, generator=g, device="cuda").half()
+    rows = torch.tensor([8, 0, -1, 5, 5, 9, 2], device="cuda", dtype=torch.int32)
+    off = offsets_of([2, 4, 1])
+    for x in (big[:, 5:205], big[:, 8:208], big[:, ::2]):
+        w = unpacked(q, scales, None, 200, 64)
+        _, y64, mag = product64(x, w, off, rows)
+        got = ops.grouped_matmul_w4(x, q, scales, off, rows=rows, group_size=64)
+        close(got, y64, 204 * 2.0 ** -23 * mag)
+
+
+@pytest.mark.parametrize("inner,group", [(256, 128), (75, 32), (700, 64)])
+def test_quantize_w4_error(ops, inner, group):
+    """Rounding to the nearest of the group's steps: half a step, where the step (the scale) is
+    first rounded to bf16 (2^-8 of up to 15 steps, and the zero point moves by half a step)."""
+    w = torch.randn(3, 40, inner, generator=gen(2), device="cuda").to(torch.bfloat16)
+    for symmetric in (False, True):
+        q, s, z = ops.quantize_w4(w, group, symmetric=symmetric)
+        step = s.double()[:, :, torch.arange(inner, device="cuda") // group]
+        off = (unpacked(q, s, z, inner, group) - w.double()).abs()
+        assert (off <= step * (1.0 + 15 * 2.0 ** -8)).all()
+
+
 # ---------------------------------------------------------------------------- combine
 
 
@@ -530,6 +616,7 @@ def refusals():
     bf, i32 = torch.bfloat16, torch.int32
     c = lambda *s, dtype=torch.float32: torch.zeros(*s, device="cuda", dtype=dtype)  # noqa
     off = lambda n: c(n, dtype=i32)  # noqa
+    u8 = lambda *s: c(*s, dtype=torch.uint8)  # noqa
     return [
         lambda o: o.route(c(4, 5), 0),
         lambda o: o.route(c(4, 5), 6),
@@ -551,6 +638,15 @@ def refusals():
                                             c(2, 8, 8, dtype=bf), off(3)),
         lambda o: o.grouped_matmul_backward(c(4, 8, dtype=bf), c(4, 8, dtype=bf),
                                             c(2, 8, 8, dtype=bf), off(3), grad_dtype=torch.float16),
+        lambda o: o.grouped_matmul_w4(c(4, 64, dtype=bf), u8(2, 8, 32), c(2, 8, 2, dtype=bf), off(3),
+                                      group_size=48),
+        lambda o: o.grouped_matmul_w4(c(4, 64, dtype=bf), u8(2, 8, 31), c(2, 8, 2, dtype=bf), off(3),
+                                      group_size=32),
+        lambda o: o.grouped_matmul_w4(c(4, 64, dtype=bf), u8(2, 8, 32), c(2, 8, 1, dtype=bf), off(3),
+                                      group_size=32),
+        lambda o: o.grouped_matmul_w4(c(4, 64, dtype=bf), u8(2, 8, 32), c(2, 8, 2), off(3),
+                                      group_size=32),
+        lambda o: o.grouped_matmul_w4(c(4, 64), u8(2, 8, 32), c(2, 8, 2), off(3), group_size=32),
         lambda o: o.combine(c(4, 8), c(2, 2).long()),
         lambda o: o.combine(c(4, 8), off(4)),
         lambda o: o.combine(c(4, 8), c(2, 2, dtype=i32), c(2, 3)),
@@ -565,11 +661,11 @@ def refusals():
     ]
 
 
-@pytest.mark.parametrize("i", range(28))
+@pytest.mark.parametrize("i", range(33))
 def test_refusals(ops, i):
     from lightgbm_rs_b200 import LightGBMError
 
     calls = refusals()
-    assert len(calls) == 28
+    assert len(calls) == 33
     with pytest.raises(LightGBMError):
         calls[i](ops)
