@@ -639,8 +639,8 @@ int lgbm_b200_experts_combine_backward(const void* dout, const void* y, int32_t 
  * is 65536 / (65536 - D), exact for that D. Bits: Philox4x32-10 of counter (i / 8, offset)
  * and key seed; element i takes the low (i even) or high half of word (i % 8) / 2. The
  * mask is never stored: the gradient of x is the same call on the gradient of out,
- * without a residual. A dropped element is 0 whatever it held. `out` may be x or
- * residual when they are contiguous. */
+ * without a residual. A dropped element is 0 whatever it held. `out` overlaps
+ * neither x nor residual. */
 int lgbm_b200_experts_dropout(const void* x, const void* residual, int32_t dtype, int64_t rows,
                               int64_t width, int64_t pitch, int64_t residual_pitch, double p,
                               uint64_t seed, uint64_t offset, void* out, void* stream);

@@ -7,6 +7,8 @@
 #pragma once
 
 #include <cstdint>
+#include <type_traits>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -45,34 +47,69 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// V consecutive elements as floats; V * sizeof(T) is 16 (one 16-byte access, `p` aligned to
-// it) or V is 1.
-template <typename T, int V>
-__device__ __forceinline__ void load_f32(const T* p, float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = to_f32<T>(*p);
-  } else {
-    static_assert(V * sizeof(T) == 16, "one 16-byte access");
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p));
-    const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = to_f32<T>(e[i]);
-  }
+// 2^x and e^x with ex2.approx (2 units in the last place); results below 2^-126 are 0.
+__device__ __forceinline__ float fast_exp(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
 }
 
+// V elements as they lie in memory (V * sizeof(T) is 16, or V is 1), to be loaded first and
+// converted later: a conversion right behind its load would wait for it.
 template <typename T, int V>
-__device__ __forceinline__ void store_f32(T* p, const float (&v)[V]) {
-  if constexpr (V == 1) {
-    *p = from_f32<T>(v[0]);
-  } else {
-    static_assert(V * sizeof(T) == 16, "one 16-byte access");
-    uint4 raw;
-    T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = from_f32<T>(v[i]);
-    *reinterpret_cast<uint4*>(p) = raw;
+struct Raw {
+  uint4 bits;
+  __device__ __forceinline__ void load(const T* p) {
+    bits = __ldg(reinterpret_cast<const uint4*>(p));
   }
-}
+  __device__ __forceinline__ void get(float (&v)[V]) const {
+    const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          v[2 * i] = __uint_as_float(w[i] << 16);
+          v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          v[2 * i] = f.x;
+          v[2 * i + 1] = f.y;
+        }
+      }
+    }
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&v)[V]) {
+    uint32_t w[4];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          const __nv_bfloat162 q = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&q);
+        } else {
+          const __half2 q = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&q);
+        }
+      }
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <typename T>
+struct Raw<T, 1> {
+  T value;
+  __device__ __forceinline__ void load(const T* p) { value = __ldg(p); }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = to_f32<T>(value); }
+  static __device__ __forceinline__ void store(T* p, const float (&v)[1]) {
+    *p = from_f32<T>(v[0]);
+  }
+};
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 inline int elem_size(int32_t dtype) { return dtype == LGBM_B200_DTYPE_F32 ? 4 : 2; }

@@ -35,13 +35,10 @@ namespace cg = cooperative_groups;
 constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
 constexpr int kOutBlock = 16 * kFewWarps;  // outputs of a block
-constexpr int kFewRows = 32;               // rows of an item: four column tiles of 8
-constexpr int kPanel = 512;                // inner length of x and scales staged at a time
-constexpr int kRing = 3;                   // stages a warp
 constexpr int kRowBytes = 128;             // of a weight row in a stage
 constexpr int kRowPitch = kRowBytes + 16;  // 36 words: 8 rows x 16 bytes hit all banks once
 constexpr int kStageBytes = 16 * kRowPitch;
-constexpr int kScalePitch = kPanel / 32 + 1;  // odd: 8 rows hit 8 banks
+constexpr int kMaxSplit = 8;               // blocks of a cluster
 
 struct FewArgs {
   const void* x;
@@ -59,7 +56,8 @@ struct FewArgs {
   void* y;
   int32_t blocks;          // blocks along the outputs
   int32_t split;           // blocks of a cluster along the inner axis
-  int32_t slice;           // inner length of each, a multiple of kPanel
+  int32_t slice;           // inner length of each, a multiple of 256
+  int32_t panel;           // inner length of x and scales staged at a time, same
   int32_t x_vec;           // x may be read 16 bytes at a time
   int32_t w_align;         // 16, 8, 4 or 2: alignment of every weight row
 };
@@ -145,28 +143,45 @@ __device__ __forceinline__ uint32_t sub2<__nv_bfloat16>(uint32_t a, uint32_t b) 
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-template <bool W4>
+// Layout of a block's shared memory. TILES column tiles of 8 rows make an item.
+template <bool W4, int TILES>
 struct FewShape {
+  static constexpr int kRows = 8 * TILES;
+  // sized so that two blocks share an SM
+  static constexpr int kMaxPanel = TILES == 1 ? 1024 : 512;
+  static constexpr int kRing = TILES == 1 ? 4 : 3;  // stages a warp
   static constexpr int kStageInner = W4 ? 2 * kRowBytes : kRowBytes / 2;
   // bytes of a staged token: the fragment loads of 8 tokens hit different banks
-  static constexpr int kTokenPitch = kPanel * 2 + (W4 ? 64 : 16);
-  static constexpr int kTokens = kFewRows * kTokenPitch;
-  static constexpr int kScales = W4 ? kOutBlock * kScalePitch * 4 : 0;
-  static constexpr int kSmem = kTokens + 2 * kScales + kFewWarps * kRing * kStageBytes;
-  static_assert(kFewRows * kOutBlock * 4 <= kTokens, "partial sums fit over the tokens");
+  static __host__ __device__ int token_pitch(int panel) { return panel * 2 + (W4 ? 64 : 16); }
+  // 16-bit scales (and zero points) of an output: an odd number of words, 8 rows hit 8 banks
+  static __host__ __device__ int scale_pitch(int panel, int shift) { return (panel >> shift) + 2; }
+  static __host__ __device__ int tokens(int panel) {
+    const int need = kRows * token_pitch(panel), sums = kRows * kOutBlock * 4;
+    return need > sums ? need : sums;  // the partial sums lie over the tokens
+  }
+  static __host__ __device__ int scales(int panel, int shift) {
+    return W4 ? (kOutBlock * scale_pitch(panel, shift) * 2 + 15) / 16 * 16 : 0;
+  }
+  static __host__ int total(int panel, int shift) {
+    return tokens(panel) + 2 * scales(panel, shift) + kFewWarps * kRing * kStageBytes;
+  }
 };
 
-template <typename T, bool W4>
+template <typename T, bool W4, int TILES>
 __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g) {
-  using S = FewShape<W4>;
+  using S = FewShape<W4, TILES>;
+  constexpr int kFewRows = S::kRows, kRing = S::kRing;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int32_t item[3];
-  uint8_t* tokens = smem;
-  float* scales = reinterpret_cast<float*>(smem + S::kTokens);
-  uint32_t* zeros = reinterpret_cast<uint32_t*>(smem + S::kTokens + S::kScales);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t ring =
-      shared_addr(smem + S::kTokens + 2 * S::kScales) + warp * kRing * kStageBytes;
+  const int tpitch = S::token_pitch(g.panel), spitch = S::scale_pitch(g.panel, g.group_shift);
+  uint8_t* tokens = smem;
+  T* scales = reinterpret_cast<T*>(smem + S::tokens(g.panel));
+  uint16_t* zeros = reinterpret_cast<uint16_t*>(smem + S::tokens(g.panel) +
+                                                S::scales(g.panel, g.group_shift));
+  const uint32_t ring = shared_addr(smem + S::tokens(g.panel) +
+                                    2 * S::scales(g.panel, g.group_shift)) +
+                        warp * kRing * kStageBytes;
   const int gq = lane >> 2, tq = lane & 3;  // row and column quad of the matrix fragments
 
   // The item of this block: rows [begin, begin + n) of one expert. Items are numbered expert
@@ -242,61 +257,67 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  float acc[4][4];
+  float acc[TILES][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < TILES; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
 
 #pragma unroll
   for (int i = 0; i < kRing - 1; ++i) load_stage(i);
 
-  const T* x = static_cast<const T*>(g.x);
-  for (int i = 0; i < stages; ++i) {
-    const int k0 = i * S::kStageInner;  // within the slice
-    if (k0 % kPanel == 0) {
+  const uint16_t* x = static_cast<const uint16_t*>(g.x);
+  int kp = g.panel;  // inner position in the panel
+  for (int i = 0; i < stages; ++i, kp += S::kStageInner) {
+    if (kp == g.panel) {
+      kp = 0;
+      const int k0 = k_begin + i * S::kStageInner;
       if (i > 0) __syncthreads();
       // tokens of this panel, 8 inner elements a thread; zeros past the rows and the slice
-      for (int p = threadIdx.x; p < tiles * 8 * (kPanel / 8); p += kFewThreads) {
-        const int r = p / (kPanel / 8), c = p % (kPanel / 8) * 8, k = k_begin + k0 + c;
-        uint32_t v[4] = {0, 0, 0, 0};
+      const int vecs = g.panel / 8;
+      for (int r = warp; r < 8 * tiles; r += kFewWarps) {
         int64_t at = -1;
         if (r < nrows) at = g.index ? g.index[begin + r] : begin + r;
-        if (at >= 0 && at < g.x_rows && k < k_end) {
-          const uint16_t* src =
-              reinterpret_cast<const uint16_t*>(x) + at * g.x_pitch + k;
-          if (g.x_vec && k + 8 <= k_end) {
-            const uint4 q = __ldg(reinterpret_cast<const uint4*>(src));
-            v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
-          } else {
+        const bool inside = at >= 0 && at < g.x_rows;
+        const uint16_t* src = x + (inside ? at : 0) * g.x_pitch;
+        for (int c = lane; c < vecs; c += 32) {
+          const int k = k0 + c * 8;
+          uint32_t v[4] = {0, 0, 0, 0};
+          if (inside && k < k_end) {
+            if (g.x_vec && k + 8 <= k_end) {
+              const uint4 q = __ldg(reinterpret_cast<const uint4*>(src + k));
+              v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+            } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (k + j < k_end) v[j / 2] |= (uint32_t)src[j] << (16 * (j & 1));
+              for (int j = 0; j < 8; ++j)
+                if (k + j < k_end) v[j / 2] |= (uint32_t)src[k + j] << (16 * (j & 1));
+            }
           }
+          if (W4) {  // pairs (0, 4), (1, 5), (2, 6), (3, 7)
+            const uint32_t p0 = __byte_perm(v[0], v[2], 0x5410),
+                           p1 = __byte_perm(v[0], v[2], 0x7632),
+                           p2 = __byte_perm(v[1], v[3], 0x5410),
+                           p3 = __byte_perm(v[1], v[3], 0x7632);
+            v[0] = p0, v[1] = p1, v[2] = p2, v[3] = p3;
+          }
+          *reinterpret_cast<uint4*>(tokens + r * tpitch + c * 16) =
+              make_uint4(v[0], v[1], v[2], v[3]);
         }
-        if (W4) {  // pairs (0, 4), (1, 5), (2, 6), (3, 7)
-          const uint32_t a = __byte_perm(v[0], v[2], 0x5410), b = __byte_perm(v[0], v[2], 0x7632),
-                         c2 = __byte_perm(v[1], v[3], 0x5410),
-                         d = __byte_perm(v[1], v[3], 0x7632);
-          v[0] = a, v[1] = b, v[2] = c2, v[3] = d;
-        }
-        *reinterpret_cast<uint4*>(tokens + r * S::kTokenPitch + c * 2) =
-            make_uint4(v[0], v[1], v[2], v[3]);
       }
       if (W4) {
-        const int per = kPanel >> g.group_shift;
-        const int first = (k_begin + k0) >> g.group_shift;
-        for (int p = threadIdx.x; p < kOutBlock * per; p += kFewThreads) {
-          const int r = p / per, c = p % per;
-          float s = 0.0f;
+        const int bits = 31 - __clz(g.panel >> g.group_shift);
+        const int first = k0 >> g.group_shift;
+        for (int p = threadIdx.x; p < kOutBlock << bits; p += kFewThreads) {
+          const int r = p >> bits, c = p & ((1 << bits) - 1);
+          T s = from_f32<T>(0.0f);
           uint32_t z = 8;
           if (out0 + r < g.outer && first + c < g.groups) {
             const int64_t at = ((int64_t)expert * g.outer + out0 + r) * g.groups + first + c;
-            s = to_f32<T>(static_cast<const T*>(g.scales)[at]);
+            s = static_cast<const T*>(g.scales)[at];
             if (g.zeros) z = g.zeros[at] & 15;
           }
-          scales[r * kScalePitch + c] = s;
-          zeros[r * kScalePitch + c] = (Magic<T>::kBits + z) * 0x10001u;
+          scales[r * spitch + c] = s;
+          zeros[r * spitch + c] = (uint16_t)(Magic<T>::kBits + z);
         }
       }
       __syncthreads();
@@ -305,24 +326,25 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
     asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
     __syncwarp();
     const uint32_t st = ring + (i % kRing) * kStageBytes;
-    const int kp = k0 % kPanel;
     if constexpr (W4) {
       const uint32_t a_at = st + gq * kRowPitch + tq * 4;
-      float part[4][4];
+      const uint8_t* b_at = tokens + gq * tpitch + (kp + tq * 8) * 2;
+      const int s_at = (warp * 16 + gq) * spitch;
+      float part[TILES][4];
 #pragma unroll
       for (int j = 0; j < S::kStageInner / 32; ++j) {
-        const int sg = (kp + j * 32) >> g.group_shift;
-        const int lo = (warp * 16 + gq) * kScalePitch + sg, hi = lo + 8 * kScalePitch;
+        const int lo = s_at + ((kp + j * 32) >> g.group_shift), hi = lo + 8 * spitch;
         if (((j * 32) & ((1 << g.group_shift) - 1)) == 0) {
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
+          for (int n = 0; n < TILES; ++n)
 #pragma unroll
             for (int q = 0; q < 4; ++q) part[n][q] = 0.0f;
         }
         uint32_t wl, wh;
         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wl) : "r"(a_at + j * 16));
         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wh) : "r"(a_at + j * 16 + 8 * kRowPitch));
-        const uint32_t zl = zeros[lo], zh = zeros[hi];
+        const uint32_t zl = g.zeros ? zeros[lo] * 0x10001u : (Magic<T>::kBits + 8) * 0x10001u;
+        const uint32_t zh = g.zeros ? zeros[hi] * 0x10001u : (Magic<T>::kBits + 8) * 0x10001u;
         uint32_t pl[4], ph[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -331,28 +353,27 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
         }
         const uint32_t a0[4] = {pl[0], ph[0], pl[1], ph[1]}, a1[4] = {pl[2], ph[2], pl[3], ph[3]};
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          if (n < tiles) {
-            const uint4 b = *reinterpret_cast<const uint4*>(
-                tokens + (n * 8 + gq) * S::kTokenPitch + (kp + j * 32 + tq * 8) * 2);
+        for (int n = 0; n < TILES; ++n) {
+          if (TILES == 1 || n < tiles) {
+            const uint4 b = *reinterpret_cast<const uint4*>(b_at + n * 8 * tpitch + j * 64);
             mma_16816<T>(part[n], a0, b.x, b.y);
             mma_16816<T>(part[n], a1, b.z, b.w);
           }
         }
         if (((j * 32 + 32) & ((1 << g.group_shift) - 1)) == 0) {
-          const float sl = scales[lo], sh = scales[hi];
+          const float sl = to_f32<T>(scales[lo]), sh = to_f32<T>(scales[hi]);
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
-            if (n < tiles) {
-              acc[n][0] = fmaf(sl, part[n][0], acc[n][0]);
-              acc[n][1] = fmaf(sl, part[n][1], acc[n][1]);
-              acc[n][2] = fmaf(sh, part[n][2], acc[n][2]);
-              acc[n][3] = fmaf(sh, part[n][3], acc[n][3]);
-            }
+          for (int n = 0; n < TILES; ++n) {
+            acc[n][0] = fmaf(sl, part[n][0], acc[n][0]);
+            acc[n][1] = fmaf(sl, part[n][1], acc[n][1]);
+            acc[n][2] = fmaf(sh, part[n][2], acc[n][2]);
+            acc[n][3] = fmaf(sh, part[n][3], acc[n][3]);
+          }
         }
       }
     } else {
       const uint32_t a_at = st + (lane & 15) * kRowPitch + (lane >> 4) * 16;
+      const uint8_t* b_at = tokens + gq * tpitch + kp * 2 + tq * 4;
 #pragma unroll
       for (int j = 0; j < S::kStageInner / 16; ++j) {
         uint32_t a[4];
@@ -361,9 +382,9 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
                      : "r"(a_at + j * 32)
                      : "memory");
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          if (n < tiles) {
-            const uint8_t* b = tokens + (n * 8 + gq) * S::kTokenPitch + (kp + j * 16) * 2 + tq * 4;
+        for (int n = 0; n < TILES; ++n) {
+          if (TILES == 1 || n < tiles) {
+            const uint8_t* b = b_at + n * 8 * tpitch + j * 32;
             mma_16816<T>(acc[n], a, *reinterpret_cast<const uint32_t*>(b),
                          *reinterpret_cast<const uint32_t*>(b + 16));
           }
@@ -379,7 +400,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
   __syncthreads();
   float* sums = reinterpret_cast<float*>(tokens);
 #pragma unroll
-  for (int n = 0; n < 4; ++n)
+  for (int n = 0; n < TILES; ++n)
     if (n < tiles) {
       float* at = sums + (n * 8 + 2 * tq) * kOutBlock + warp * 16 + gq;
       at[0] = acc[n][0];
@@ -415,8 +436,9 @@ struct FewDevice {
 };
 FewDevice g_few_devices[kMaxDevices];
 
-template <typename T, bool W4>
-cudaError_t launch_few_typed(FewArgs g, cudaStream_t st) {
+template <typename T, bool W4, int TILES>
+cudaError_t launch_few_tiles(FewArgs g, cudaStream_t st) {
+  using S = FewShape<W4, TILES>;
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
@@ -424,30 +446,32 @@ cudaError_t launch_few_typed(FewArgs g, cudaStream_t st) {
   {
     FewDevice& d = g_few_devices[dev];
     std::lock_guard<std::mutex> lock(d.mu);
-    const uint32_t bit = 1u << (2 * (int)W4 + (int)(sizeof(T) == 2 && std::is_same<T, __half>()));
+    const uint32_t bit = 1u << (4 * (TILES > 1) + 2 * W4 + std::is_same<T, __half>::value);
     if (!(d.ready & bit)) {
-      err = cudaFuncSetAttribute(k_grouped_few<T, W4>,
+      err = cudaFuncSetAttribute(k_grouped_few<T, W4, TILES>,
                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 FewShape<W4>::kSmem);
+                                 S::total(S::kMaxPanel, 5));
       if (err != cudaSuccess) return err;
       d.ready |= bit;
     }
   }
   const int64_t blocks = (g.outer + kOutBlock - 1) / kOutBlock;
-  const int64_t items = std::min<int64_t>(g.experts + 1, g.rows) + g.rows / kFewRows;
-  // Split the inner axis, in whole panels, while the blocks would not fill the SMs twice.
-  const int64_t panels = (g.inner + kPanel - 1) / kPanel;
+  const int64_t items = std::min<int64_t>(g.experts + 1, g.rows) + g.rows / S::kRows;
+  // Split the inner axis, in steps of at least 512, while the blocks would not fill the SMs.
   const int64_t busy = blocks * std::min<int64_t>(g.experts, g.rows);
   int split = 1;
-  while (split < 8 && split * 2 <= panels && busy * split < 2 * 148) split *= 2;
+  while (split < kMaxSplit && split * 1024 <= g.inner && busy * split < 148) split *= 2;
+  const int64_t steps = (g.inner + 255) / 256;
   g.blocks = (int32_t)blocks;
   g.split = split;
-  g.slice = (int32_t)((panels + split - 1) / split * kPanel);
-  cudaLaunchConfig_t cfg{};
+  g.slice = (int32_t)((steps + split - 1) / split * 256);
+  g.panel = 256;
+  while (g.panel < S::kMaxPanel && g.panel < g.slice) g.panel *= 2;
   if (blocks * split * items > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(blocks * split * items), 1, 1);
   cfg.blockDim = dim3(kFewThreads, 1, 1);
-  cfg.dynamicSmemBytes = FewShape<W4>::kSmem;
+  cfg.dynamicSmemBytes = (size_t)S::total(g.panel, g.group_shift);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -455,7 +479,15 @@ cudaError_t launch_few_typed(FewArgs g, cudaStream_t st) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = split > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, k_grouped_few<T, W4>, g);
+  return cudaLaunchKernelEx(&cfg, k_grouped_few<T, W4, TILES>, g);
+}
+
+template <typename T, bool W4>
+cudaError_t launch_few_typed(const FewArgs& g, cudaStream_t st) {
+  // Items of 8 rows while few experts can have more: no test for absent column tiles in the
+  // inner loop, and the tokens of twice the inner length in shared memory.
+  return g.rows <= 4 * (int64_t)g.experts || g.rows <= 8 ? launch_few_tiles<T, W4, 1>(g, st)
+                                                         : launch_few_tiles<T, W4, 4>(g, st);
 }
 
 }  // namespace

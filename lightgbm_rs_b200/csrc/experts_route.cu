@@ -6,7 +6,7 @@ namespace lgbm_b200 {
 namespace experts {
 namespace {
 
-constexpr int kRouteThreads = 128;   // k_route_select, k_route_place
+constexpr int kRouteThreads = 128;   // k_route_place
 constexpr int kRouteChunk = 64;      // logit columns staged at a time
 constexpr uint32_t kKeyEmpty = 0x007FFFFFu;  // key of -inf: never chosen
 
@@ -202,26 +202,95 @@ __device__ void select_tokens(const T* logits, int64_t tokens, int experts, int6
   }
 }
 
-// First of three launches: choice and weights, and each block's rows per expert.
-template <typename T, int L, int KP>
-__global__ void __launch_bounds__(kRouteThreads)
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xFFFFFFFF;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+constexpr int kSelectThreads = 256;
+constexpr int kSelectTokens = 128;  // of a block: 16 a warp, one after the other
+
+// First of three launches for many tokens: choice and weights, and each block's rows per
+// expert. A warp a token: its logits lie in registers, expert e in lane e % 32, and each of
+// the k choices is one maximum over the warp (NaN wins), the first place that holds it, and
+// its removal. The next token's logits are on their way meanwhile.
+template <typename T, int NV>
+__global__ void __launch_bounds__(kSelectThreads)
     k_route_select(const T* logits, int64_t tokens, int experts, int64_t pitch, int k,
                    bool normalize, float* weights, int32_t* chosen, int32_t* counts) {
-  __shared__ uint32_t tile[(kRouteThreads / L) * (kRouteChunk + L)];
   __shared__ int32_t hist[kMaxExperts + 1];
-  constexpr int kTokens = kRouteThreads / L;
-  for (int i = threadIdx.x; i <= experts; i += kRouteThreads) hist[i] = 0;
-  int ids[KP];
-  const int64_t first = (int64_t)blockIdx.x * kTokens;
-  select_tokens<T, L, KP, kRouteThreads>(logits, tokens, experts, pitch, k, normalize, first,
-                                         tile, weights, chosen, ids);
-  if (threadIdx.x % L == 0 && first + threadIdx.x / L < tokens) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i <= experts; i += kSelectThreads) hist[i] = 0;
+  __syncthreads();
+  constexpr int kPerWarp = kSelectTokens / (kSelectThreads / 32);
+  const int64_t first = (int64_t)blockIdx.x * kSelectTokens + warp * kPerWarp;
+  const int64_t last = min(first + kPerWarp, tokens);
+  const float kNone = -__int_as_float(0x7F800000);
+  float next[NV];
+  auto fetch = [&](int64_t t) {
 #pragma unroll
-    for (int j = 0; j < KP; ++j)
-      if (j < k) atomicAdd(&hist[ids[j] < 0 ? experts : ids[j]], 1);
+    for (int i = 0; i < NV; ++i) {
+      const int e = i * 32 + lane;
+      next[i] = t < last && e < experts ? to_f32<T>(logits[t * pitch + e]) : kNone;
+    }
+  };
+  fetch(first);
+  for (int64_t t = first; t < last; ++t) {
+    float v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = next[i];
+    fetch(t + 1);
+    float top = v[0];
+#pragma unroll
+    for (int i = 1; i < NV; ++i) top = max_nan(top, v[i]);
+    const float m = warp_max_nan(top);
+    float total = 0.0f, my_logit = kNone;
+    int my_id = -1;
+    if (!normalize) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) total += fast_exp(v[i] - m);
+    }
+    for (int j = 0; j < k; ++j) {
+      const float best = j == 0 ? m : warp_max_nan(top);
+      if (best == kNone) break;  // the same in every lane
+      // the lowest expert among those that hold it: the first register of each lane, then
+      // the lowest of the lanes
+      int at = NV * 32;
+      const bool nan = best != best;
+#pragma unroll
+      for (int i = NV - 1; i >= 0; --i)
+        if (v[i] == best || (nan && v[i] != v[i])) at = i * 32;
+      const int id = (int)__reduce_min_sync(0xFFFFFFFFu, (uint32_t)(at + lane));
+      const int out = lane == (id & 31) ? id >> 5 : -1;
+      top = kNone;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (i == out) v[i] = kNone;
+        top = max_nan(top, v[i]);
+      }
+      if (lane == j) {
+        my_logit = best;
+        my_id = id;
+      }
+    }
+    const float mine = my_id >= 0 ? expf(my_logit - m) : 0.0f;
+    if (normalize) total = mine;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+    if (lane < k) {
+      weights[t * k + lane] = my_id >= 0 ? mine / total : 0.0f;
+      chosen[t * k + lane] = my_id;
+      atomicAdd(&hist[my_id < 0 ? experts : my_id], 1);
+    }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e <= experts; e += kRouteThreads)
+  for (int e = threadIdx.x; e <= experts; e += kSelectThreads)
     counts[(int64_t)e * gridDim.x + blockIdx.x] = hist[e];
 }
 
@@ -310,54 +379,57 @@ __global__ void __launch_bounds__(kSmallThreads)
 }
 
 // Gradient of the logits, `lanes` lanes a token: with p the softmax (over the chosen experts
-// or over all) and g the gradient of the weights, dl_e = p_e ([e chosen] g_e - sum w g).
-// Over all experts the softmax is recomputed from one chosen logit: the first chosen one is
-// the largest, m, and its weight is 1 / sum exp(l - m).
-template <typename T, int KP>
+// or over all) and g the gradient of the weights, dl_e = p_e ([e chosen] g_e - sum w g). For
+// a chosen expert p_e is its weight. Over all experts the others' p is recomputed from one
+// chosen logit: the first chosen one is the largest, m, and its weight is 1 / sum exp(l - m).
+// The row is written as if nothing were chosen, then the chosen places again.
+template <typename T, int NV>
 __global__ void __launch_bounds__(256)
     k_route_backward(const float* dweights, const float* weights, const int32_t* chosen,
                      const T* logits, int64_t tokens, int experts, int64_t pitch, int k,
-                     bool normalize, int lanes, T* dlogits) {
-  const int64_t t = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
-  if (t >= tokens) return;
-  int id[KP];
-  float val[KP];
-  float s = 0.0f, w0 = 0.0f;
+                     bool normalize, int shift, T* dlogits) {
+  const int lanes = 1 << shift;  // at least k, and enough for NV experts a lane
+  const int64_t t = (int64_t)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
+  const int sub = threadIdx.x & (lanes - 1);
+  const bool live = t < tokens;
+  const T* row = logits + t * pitch;
+  T v[NV];
+  if (live && !normalize) {
 #pragma unroll
-  for (int j = 0; j < KP; ++j) {
-    id[j] = -1;
-    val[j] = 0.0f;
-    if (j < k) {
-      id[j] = chosen[t * k + j];
-      const float w = weights[t * k + j];
-      if (j == 0) w0 = w;
-      if (id[j] >= 0) {
-        const float g = dweights[t * k + j];
-        s = fmaf(w, g, s);
-        val[j] = normalize ? g : w * g;
-      }
+    for (int i = 0; i < NV; ++i)
+      if (i * lanes + sub < experts) v[i] = __ldg(row + i * lanes + sub);
+  }
+  int id = -1;
+  float w = 0.0f, g = 0.0f, m = 0.0f;
+  if (live && sub < k) {
+    id = chosen[t * k + sub];
+    if (id >= 0 && id < experts) {
+      w = weights[t * k + sub];
+      g = dweights[t * k + sub];
+      if (sub == 0 && !normalize) m = to_f32<T>(row[id]);
+    } else {
+      id = -1;
     }
   }
-  const bool any = id[0] >= 0 && id[0] < experts;
-  float m = 0.0f;
-  if (normalize) {
+  float s = w * g;
+  for (int d = lanes >> 1; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+  m = __shfl_sync(0xFFFFFFFFu, m, 0, lanes);
+  // every other weight is 0 where the first is missing, and so is s
+  const float scale = -s * __shfl_sync(0xFFFFFFFFu, w, 0, lanes);
+  const bool any = __shfl_sync(0xFFFFFFFFu, id, 0, lanes) >= 0;
+  if (live) {
+    T* out = dlogits + t * experts;
 #pragma unroll
-    for (int j = 0; j < KP; ++j)
-      if (j < k && id[j] >= 0) val[j] = weights[t * k + j] * (val[j] - s);
-  } else if (any) {
-    m = to_f32<T>(logits[t * pitch + id[0]]);
+    for (int i = 0; i < NV; ++i) {
+      const int e = i * lanes + sub;
+      if (e < experts)
+        out[e] = from_f32<T>(normalize || !any ? 0.0f
+                                               : fast_exp(to_f32<T>(v[i]) - m) * scale);
+    }
   }
-  for (int e = threadIdx.x % lanes; e < experts; e += lanes) {
-    float d = 0.0f;
-    if (!normalize && any) d = -(expf(to_f32<T>(logits[t * pitch + e]) - m) * w0) * s;
-#pragma unroll
-    for (int j = 0; j < KP; ++j)
-      if (id[j] == e) d += val[j];
-    dlogits[t * experts + e] = from_f32<T>(d);
-  }
+  __syncwarp();
+  if (id >= 0) dlogits[t * experts + id] = from_f32<T>(w * (g - s));
 }
-
-int route_lanes(int64_t tokens) { return tokens >= 16384 ? 1 : 8; }
 
 template <typename T, int KP>
 cudaError_t route_typed(const T* logits, int64_t tokens, int experts, int64_t pitch, int k,
@@ -372,21 +444,22 @@ cudaError_t route_typed(const T* logits, int64_t tokens, int experts, int64_t pi
                                                          rows, offsets);
     return cudaGetLastError();
   }
-  const int lanes = route_lanes(tokens);
-  const int block_tokens = kRouteThreads / lanes;
-  const int blocks = (int)((tokens + block_tokens - 1) / block_tokens);
+  const int blocks = (int)((tokens + kSelectTokens - 1) / kSelectTokens);
   int32_t* totals = ws;
   int32_t* counts = ws + experts + 1;
-  if (lanes == 1)
-    k_route_select<T, 1, KP><<<blocks, kRouteThreads, 0, st>>>(
+  auto select = [&](auto nv) {
+    k_route_select<T, decltype(nv)::value><<<blocks, kSelectThreads, 0, st>>>(
         logits, tokens, experts, pitch, k, normalize, weights, chosen, counts);
-  else
-    k_route_select<T, 8, KP><<<blocks, kRouteThreads, 0, st>>>(
-        logits, tokens, experts, pitch, k, normalize, weights, chosen, counts);
+  };
+  if (experts <= 32) select(std::integral_constant<int, 1>());
+  else if (experts <= 64) select(std::integral_constant<int, 2>());
+  else if (experts <= 128) select(std::integral_constant<int, 4>());
+  else if (experts <= 256) select(std::integral_constant<int, 8>());
+  else select(std::integral_constant<int, 16>());
   k_route_scan<<<(experts + 8) / 8, 256, 0, st>>>(counts, totals, experts + 1, blocks);
   const size_t smem = sizeof(int32_t) * (experts + 1) * (1 + kRouteThreads / 32);
   k_route_place<<<blocks, kRouteThreads, smem, st>>>(chosen, counts, totals, tokens, experts, k,
-                                                     block_tokens, position, rows, offsets);
+                                                     kSelectTokens, position, rows, offsets);
   return cudaGetLastError();
 }
 
@@ -412,8 +485,7 @@ cudaError_t with_type(int32_t dtype, F&& f) {
 int64_t route_workspace(int64_t tokens, int32_t experts, int32_t k) {
   (void)k;
   if (tokens <= kSmallTokens) return 0;
-  const int64_t block_tokens = kRouteThreads / route_lanes(tokens);
-  const int64_t blocks = (tokens + block_tokens - 1) / block_tokens;
+  const int64_t blocks = (tokens + kSelectTokens - 1) / kSelectTokens;
   return (int64_t)sizeof(int32_t) * (experts + 1) * (blocks + 1);
 }
 
@@ -435,18 +507,23 @@ cudaError_t launch_route_backward(const float* dweights, const float* weights,
                                   const int32_t* chosen, const void* logits, int32_t dtype,
                                   int64_t tokens, int32_t experts, int64_t pitch, int32_t k,
                                   bool normalize, void* dlogits, cudaStream_t st) {
-  int lanes = 32;  // the smallest power of two that covers the experts, at most a warp
-  while (lanes > 1 && lanes / 2 >= experts) lanes /= 2;
-  const int64_t per_block = 256 / lanes;
-  const int64_t blocks = (tokens + per_block - 1) / per_block;
+  int shift = 0;  // lanes of a token: the smallest power of two that covers the experts, or 32
+  while (shift < 5 && (1 << shift) < experts) ++shift;
+  const int64_t per_block = 256 >> shift;
+  const unsigned blocks = (unsigned)((tokens + per_block - 1) / per_block);
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    return with_chosen(k, [&](auto kp) {
-      k_route_backward<T, decltype(kp)::value><<<(unsigned)blocks, 256, 0, st>>>(
+    auto go = [&](auto nv) {
+      k_route_backward<T, decltype(nv)::value><<<blocks, 256, 0, st>>>(
           dweights, weights, chosen, static_cast<const T*>(logits), tokens, experts, pitch, k,
-          normalize, lanes, static_cast<T*>(dlogits));
+          normalize, shift, static_cast<T*>(dlogits));
       return cudaGetLastError();
-    });
+    };
+    if (experts <= 32) return go(std::integral_constant<int, 1>());
+    if (experts <= 64) return go(std::integral_constant<int, 2>());
+    if (experts <= 128) return go(std::integral_constant<int, 4>());
+    if (experts <= 256) return go(std::integral_constant<int, 8>());
+    return go(std::integral_constant<int, 16>());
   });
 }
 

@@ -1,7 +1,5 @@
 // Row operators of the expert layer: the weighted combination of each token's rows with its
 // gradient, and dropout from a counter-based generator.
-#include <algorithm>
-
 #include "experts.cuh"
 
 namespace lgbm_b200 {
@@ -11,8 +9,8 @@ namespace {
 constexpr int kRowThreads = 256;
 
 // out[t] = sum_j w[t, j] y[position[t, j]] in f32, rounded once. A row of `lanes` threads a
-// token; the k rows are read independently of each other, four in flight a thread.
-template <typename T, int V>
+// token; JC rows are read at a time, all loads before the first use.
+template <typename T, int V, int JC>
 __global__ void __launch_bounds__(kRowThreads)
     k_combine(const T* y, int64_t rows, int width, int64_t pitch, const int32_t* position,
               const float* weights, int64_t tokens, int k, int lanes, T* out) {
@@ -22,18 +20,27 @@ __global__ void __launch_bounds__(kRowThreads)
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-    for (int j = 0; j < k; ++j) {
-      const int32_t at = position[t * k + j];
-      const float w = weights ? weights[t * k + j] : 1.0f;
-      if (at >= 0 && at < rows) {
-        float v[V];
-        load_f32<T, V>(y + at * pitch + c, v);
+    for (int j0 = 0; j0 < k; j0 += JC) {
+      float w[JC];
+      Raw<T, V> v[JC];
+      bool in[JC];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+      for (int j = 0; j < JC; ++j) {
+        const int32_t at = j0 + j < k ? position[t * k + j0 + j] : -1;
+        in[j] = at >= 0 && at < rows;
+        w[j] = weights && j0 + j < k ? weights[t * k + j0 + j] : 1.0f;
+        if (in[j]) v[j].load(y + at * pitch + c);
       }
+#pragma unroll
+      for (int j = 0; j < JC; ++j)
+        if (in[j]) {
+          float e[V];
+          v[j].get(e);
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[i] = fmaf(w[j], e[i], acc[i]);
+        }
     }
-    store_f32<T, V>(out + t * width + c, acc);
+    Raw<T, V>::store(out + t * width + c, acc);
   }
 }
 
@@ -63,21 +70,25 @@ __global__ void __launch_bounds__(kRowThreads)
       }
     }
     for (int c = lane * V; c < width; c += LANES * V) {
-      float g[V], v[JC][V];
-      load_f32<T, V>(dout + t * dout_pitch + c, g);
+      Raw<T, V> rg, rv[JC];
+      rg.load(dout + t * dout_pitch + c);
 #pragma unroll
       for (int j = 0; j < JC; ++j)
-        if (at[j] >= 0 && dweights) load_f32<T, V>(y + at[j] * pitch + c, v[j]);
+        if (at[j] >= 0 && dweights) rv[j].load(y + at[j] * pitch + c);
+      float g[V];
+      rg.get(g);
 #pragma unroll
       for (int j = 0; j < JC; ++j) {
         if (at[j] < 0) continue;
         float d[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          d[i] = w[j] * g[i];
-          if (dweights) dot[j] = fmaf(g[i], v[j][i], dot[j]);
+        for (int i = 0; i < V; ++i) d[i] = w[j] * g[i];
+        Raw<T, V>::store(dy + at[j] * width + c, d);
+        if (dweights) {
+          rv[j].get(d);
+#pragma unroll
+          for (int i = 0; i < V; ++i) dot[j] = fmaf(g[i], d[i], dot[j]);
         }
-        store_f32<T, V>(dy + at[j] * width + c, d);
       }
     }
     if (!dweights) continue;
@@ -127,60 +138,63 @@ __device__ __forceinline__ uint4 philox(uint64_t block, uint64_t offset, uint32_
   return make_uint4(c0, c1, c2, c3);
 }
 
-__device__ __forceinline__ uint32_t half_word(const uint4& r, int i) {
-  const uint32_t w = i < 2 ? r.x : i < 4 ? r.y : i < 6 ? r.z : r.w;
-  return (i & 1) ? w >> 16 : w & 0xFFFFu;
-}
+constexpr int kDropUnroll = 2;  // blocks of eight elements a thread
 
 // Element i takes 16 bits of block i / 8 and is kept when they are at least `drop`: the mask
-// is recomputed wherever it is needed and never stored. One thread makes one block and
-// handles its eight elements. VEC: rows of one pitch that 16-byte accesses can walk (a
-// contiguous array counts as one row). A dropped element is 0 whatever it held.
-template <typename T, bool VEC>
+// is recomputed wherever it is needed and never stored. With cut = drop * 2^16 - 1 a high
+// half is kept when its whole word is above cut, and a low half when it is after a shift by
+// 16: no half is taken out of its word. (drop 2^16 gives the cut 2^32 - 1, which nothing
+// passes; drop 0 would need -1 and is a flag.) A dropped element is 0 whatever it held. A
+// thread makes kDropUnroll blocks and handles their eight elements each, all loads first.
+// VEC: rows of one pitch that 16-byte accesses can walk; a contiguous array is one row.
+template <typename T, bool VEC, bool RES>
 __global__ void __launch_bounds__(kRowThreads)
-    k_dropout(const T* x, const T* residual, int64_t n, int64_t width, int64_t pitch,
-              int64_t residual_pitch, uint32_t drop, float scale, uint64_t seed,
-              uint64_t offset, T* out) {
-  const int64_t blocks = (n + 7) / 8;
-  for (int64_t b = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; b < blocks;
-       b += (int64_t)gridDim.x * kRowThreads) {
-    const int64_t i0 = b * 8;
-    if (VEC && i0 + 8 <= n) {
-      int64_t at = i0, rat = i0;
-      if (width != n) {
-        const int64_t r = i0 / width, c = i0 - r * width;
-        at = r * pitch + c;
-        rat = r * residual_pitch + c;
+    k_dropout(const T* __restrict__ x, const T* residual, int64_t n, int64_t width,
+              int64_t pitch, int64_t residual_pitch, uint32_t cut, bool all, float scale,
+              uint32_t k0, uint32_t k1, uint64_t offset, T* out) {
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+  constexpr int kParts = 8 / V;
+  const int64_t b0 = (int64_t)blockIdx.x * (kRowThreads * kDropUnroll) + threadIdx.x;
+  Raw<T, V> v[kDropUnroll][kParts], a[kDropUnroll][RES ? kParts : 1];
+#pragma unroll
+  for (int u = 0; u < kDropUnroll; ++u) {
+    const int64_t i0 = (b0 + u * kRowThreads) * 8;
+#pragma unroll
+    for (int h = 0; h < kParts; ++h) {
+      const int64_t i = i0 + h * V;  // VEC: n is a multiple of V wherever i0 + 8 > n
+      if (i < n) {
+        int64_t at = i, rat = i;
+        if (width != n) {
+          const int64_t r = i / width, c = i - r * width;
+          at = r * pitch + c;
+          rat = r * residual_pitch + c;
+        }
+        v[u][h].load(x + at);
+        if constexpr (RES) a[u][h].load(residual + rat);
       }
-      constexpr int V = 16 / (int)sizeof(T);
-      float v[8], a[8];
+    }
+  }
 #pragma unroll
-      for (int i = 0; i < 8; i += V)
-        load_f32<T, V>(x + at + i, reinterpret_cast<float(&)[V]>(v[i]));
-      if (residual)
+  for (int u = 0; u < kDropUnroll; ++u) {
+    const int64_t b = b0 + u * kRowThreads;
+    if (b * 8 >= n) break;
+    const uint4 rnd = philox((uint64_t)b, offset, k0, k1);
+    const uint32_t words[4] = {rnd.x, rnd.y, rnd.z, rnd.w};
 #pragma unroll
-        for (int i = 0; i < 8; i += V)
-          load_f32<T, V>(residual + rat + i, reinterpret_cast<float(&)[V]>(a[i]));
-      const uint4 rnd = philox((uint64_t)b, offset, (uint32_t)seed, (uint32_t)(seed >> 32));
+    for (int h = 0; h < kParts; ++h) {
+      if (b * 8 + h * V >= n) break;
+      float e[V], r[V];
+      v[u][h].get(e);
+      if constexpr (RES) a[u][h].get(r);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = half_word(rnd, i) >= drop ? v[i] * scale : 0.0f;
-        if (residual) v[i] += a[i];
+      for (int i = 0; i < V; ++i) {
+        const int at = h * V + i;
+        const uint32_t w = (at & 1) ? words[at / 2] : words[at / 2] << 16;
+        // a low half has zeros below it after the shift: above cut means at least drop * 2^16
+        e[i] = all || w > cut ? e[i] * scale : 0.0f;
+        if constexpr (RES) e[i] += r[i];
       }
-#pragma unroll
-      for (int i = 0; i < 8; i += V)
-        store_f32<T, V>(out + i0 + i, reinterpret_cast<float(&)[V]>(v[i]));
-    } else {
-      const uint4 rnd = philox((uint64_t)b, offset, (uint32_t)seed, (uint32_t)(seed >> 32));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i0 + i >= n) break;
-        const int64_t r = (i0 + i) / width, c = (i0 + i) - r * width;
-        float v = to_f32<T>(x[r * pitch + c]);
-        v = half_word(rnd, i) >= drop ? v * scale : 0.0f;
-        if (residual) v += to_f32<T>(residual[r * residual_pitch + c]);
-        out[i0 + i] = from_f32<T>(v);
-      }
+      Raw<T, V>::store(out + b * 8 + h * V, e);
     }
   }
 }
@@ -205,8 +219,13 @@ cudaError_t combine_typed(const T* y, int64_t rows, int width, int64_t pitch,
                           T* out, cudaStream_t st) {
   const int lanes = row_lanes((width + V - 1) / V);
   const int64_t per_block = kRowThreads / lanes;
-  k_combine<T, V><<<(unsigned)((tokens + per_block - 1) / per_block), kRowThreads, 0, st>>>(
-      y, rows, width, pitch, position, weights, tokens, k, lanes, out);
+  const unsigned blocks = (unsigned)((tokens + per_block - 1) / per_block);
+  if (k <= 2)
+    k_combine<T, V, 2><<<blocks, kRowThreads, 0, st>>>(y, rows, width, pitch, position, weights,
+                                                       tokens, k, lanes, out);
+  else
+    k_combine<T, V, 4><<<blocks, kRowThreads, 0, st>>>(y, rows, width, pitch, position, weights,
+                                                       tokens, k, lanes, out);
   return cudaGetLastError();
 }
 
@@ -263,9 +282,8 @@ cudaError_t launch_combine_backward(const void* dout, const void* y, int32_t dty
     using Vec = std::integral_constant<int, V>;
     using Warp = std::integral_constant<int, 32>;
     using Block = std::integral_constant<int, kRowThreads>;
-    // A block a token while a warp a token would leave SMs without work or a lane with a
-    // long row.
-    const bool wide = (width + (vec ? V : 1) - 1) / (vec ? V : 1) >= kRowThreads / 2;
+    // A block a token while a warp a token would leave SMs without work.
+    const bool wide = tokens < 148 * 16 && (width + (vec ? V : 1) - 1) / (vec ? V : 1) > 64;
     if (vec) return wide ? go(Vec(), Block()) : go(Vec(), Warp());
     return wide ? go(One(), Block()) : go(One(), Warp());
   });
@@ -283,21 +301,28 @@ cudaError_t launch_dropout(const void* x, const void* residual, int32_t dtype, i
       width = n;  // contiguous: one row
       pitch = residual_pitch = n;
     }
+    // 16 bytes at a time: whole groups of V in every row (of the array, when contiguous)
     const bool vec = aligned16(x) && aligned16(out) && (!residual || aligned16(residual)) &&
-                     (width == n || (width % 8 == 0 && pitch % V == 0 &&
-                                     (!residual || residual_pitch % V == 0)));
+                     (width == n ? n % V == 0
+                                 : width % 8 == 0 && pitch % V == 0 &&
+                                       (!residual || residual_pitch % V == 0));
     const float scale = drop < 65536u ? (float)(65536.0 / (65536.0 - (double)drop)) : 0.0f;
-    const int64_t want = ((n + 7) / 8 + kRowThreads - 1) / kRowThreads;
-    const unsigned blocks = (unsigned)std::min<int64_t>(want, 0x7FFFFFFF);
-    const T* p = static_cast<const T*>(x);
-    const T* r = static_cast<const T*>(residual);
-    T* o = static_cast<T*>(out);
+    const uint32_t cut = drop == 0 ? 0u : (uint32_t)(((uint64_t)drop << 16) - 1);
+    const int64_t per_block = (int64_t)kRowThreads * kDropUnroll * 8;
+    const int64_t want = (n + per_block - 1) / per_block;
+    if (want > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    auto go = [&](auto v, auto r) {
+      k_dropout<T, decltype(v)::value, decltype(r)::value>
+          <<<(unsigned)want, kRowThreads, 0, st>>>(
+              static_cast<const T*>(x), static_cast<const T*>(residual), n, width, pitch,
+              residual_pitch, cut, drop == 0, scale, (uint32_t)seed, (uint32_t)(seed >> 32),
+              offset, static_cast<T*>(out));
+    };
     if (vec)
-      k_dropout<T, true><<<blocks, kRowThreads, 0, st>>>(p, r, n, width, pitch, residual_pitch,
-                                                         drop, scale, seed, offset, o);
+      residual ? go(std::true_type(), std::true_type()) : go(std::true_type(), std::false_type());
     else
-      k_dropout<T, false><<<blocks, kRowThreads, 0, st>>>(p, r, n, width, pitch, residual_pitch,
-                                                          drop, scale, seed, offset, o);
+      residual ? go(std::false_type(), std::true_type())
+               : go(std::false_type(), std::false_type());
     return cudaGetLastError();
   });
 }
