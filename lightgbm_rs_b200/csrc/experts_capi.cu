@@ -66,7 +66,8 @@ int check_product(const char* what, const MatmulCall& c) {
   if (!c.offsets || (!c.out && (c.rows > 0 || c.mode == 2)) || (c.rows > 0 && ((c.mode != 1 && !c.x) || (c.mode != 0 && !c.dy))) ||
       (c.mode != 2 && !c.w))
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
-  if (c.mode != 1 && (c.x_pitch < c.inner || c.x_rows < 0 || (!c.index && c.x_rows != c.rows)))
+  if (c.mode != 1 && (c.x_pitch < c.inner || c.x_rows < (c.rows > 0) || c.x_rows > kMaxRows ||
+                      (!c.index && c.x_rows != c.rows)))
     return refuse(LGBM_B200_LENGTH_MISMATCH,
                   "%s: x has %lld rows of pitch %lld, want %lld of at least %d", what,
                   (long long)c.x_rows, (long long)c.x_pitch, (long long)c.rows, c.inner);

@@ -20,7 +20,7 @@
 // q - z are summed in f32 inside a scale group and the group's sum is multiplied by its
 // scale in f32: no weight is ever rounded.
 #include <algorithm>
-#include <mutex>
+#include <atomic>
 
 #include <cooperative_groups.h>
 
@@ -48,7 +48,6 @@ struct FewArgs {
   int64_t w_pitch;         // bytes of a weight row
   const void* scales;      // [E][outer][groups], type of x
   const uint8_t* zeros;    // [E][outer][groups] or null: 8
-  int32_t group_shift;     // log2 of the group size
   int32_t groups;
   const int32_t* offsets;
   int32_t experts, inner, outer;
@@ -59,7 +58,6 @@ struct FewArgs {
   int32_t slice;           // inner length of each, a multiple of 256
   int32_t panel;           // inner length of x and scales staged at a time, same
   int32_t x_vec;           // x may be read 16 bytes at a time
-  int32_t w_align;         // 16, 8, 4 or 2: alignment of every weight row
 };
 
 __device__ __forceinline__ uint32_t shared_addr(const void* p) {
@@ -67,19 +65,14 @@ __device__ __forceinline__ uint32_t shared_addr(const void* p) {
 }
 
 // 16 bytes of global memory to shared, of which the first `valid` (0..16) are read and the
-// rest are zeros; `align` is the alignment of `src`.
-__device__ __forceinline__ void copy16(uint32_t dst, const char* src, int valid, int align) {
-  if (align == 16) {
+// rest are zeros. ALIGN: of `src`, 16, 4 or 2 bytes.
+template <int ALIGN>
+__device__ __forceinline__ void copy16(uint32_t dst, const char* src, int valid) {
+  if constexpr (ALIGN == 16) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                  "r"(valid)
                  : "memory");
-  } else if (align == 8) {
-#pragma unroll
-    for (int i = 0; i < 16; i += 8)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + i),
-                   "l"(valid > i ? src + i : src), "r"(min(max(valid - i, 0), 8))
-                   : "memory");
-  } else if (align == 4) {
+  } else if constexpr (ALIGN == 4) {
 #pragma unroll
     for (int i = 0; i < 16; i += 4)
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + i),
@@ -102,7 +95,7 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
 template <>
 __device__ __forceinline__ void mma_16816<__half>(float (&c)[4], const uint32_t (&a)[4],
                                                   uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -111,7 +104,7 @@ __device__ __forceinline__ void mma_16816<__half>(float (&c)[4], const uint32_t 
 template <>
 __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4],
                                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -143,9 +136,13 @@ __device__ __forceinline__ uint32_t sub2<__nv_bfloat16>(uint32_t a, uint32_t b) 
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Layout of a block's shared memory. TILES column tiles of 8 rows make an item.
-template <bool W4, int TILES>
+// A kernel's variant: TILES column tiles of 8 rows make an item; SHIFT is log2 of the scale
+// group's size, 0 with weights of 16 bits, whose rows are aligned to ALIGN bytes.
+template <typename T_, int TILES_, int SHIFT_, bool ZEROS_, int ALIGN_>
 struct FewShape {
+  using T = T_;
+  static constexpr int TILES = TILES_, SHIFT = SHIFT_, ALIGN = ALIGN_;
+  static constexpr bool W4 = SHIFT > 0, ZEROS = ZEROS_;
   static constexpr int kRows = 8 * TILES;
   // sized so that two blocks share an SM
   static constexpr int kMaxPanel = TILES == 1 ? 1024 : 512;
@@ -154,34 +151,34 @@ struct FewShape {
   // bytes of a staged token: the fragment loads of 8 tokens hit different banks
   static __host__ __device__ int token_pitch(int panel) { return panel * 2 + (W4 ? 64 : 16); }
   // 16-bit scales (and zero points) of an output: an odd number of words, 8 rows hit 8 banks
-  static __host__ __device__ int scale_pitch(int panel, int shift) { return (panel >> shift) + 2; }
+  static __host__ __device__ int scale_pitch(int panel) { return (panel >> SHIFT) + 2; }
   static __host__ __device__ int tokens(int panel) {
     const int need = kRows * token_pitch(panel), sums = kRows * kOutBlock * 4;
     return need > sums ? need : sums;  // the partial sums lie over the tokens
   }
-  static __host__ __device__ int scales(int panel, int shift) {
-    return W4 ? (kOutBlock * scale_pitch(panel, shift) * 2 + 15) / 16 * 16 : 0;
+  static __host__ __device__ int scales(int panel) {
+    return W4 ? (kOutBlock * scale_pitch(panel) * 2 + 15) / 16 * 16 : 0;
   }
-  static __host__ int total(int panel, int shift) {
-    return tokens(panel) + 2 * scales(panel, shift) + kFewWarps * kRing * kStageBytes;
+  static __host__ __device__ int ring(int panel) {
+    return tokens(panel) + (ZEROS ? 2 : 1) * scales(panel);
   }
+  static __host__ int total(int panel) { return ring(panel) + kFewWarps * kRing * kStageBytes; }
 };
 
-template <typename T, bool W4, int TILES>
+template <typename S>
 __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g) {
-  using S = FewShape<W4, TILES>;
+  using T = typename S::T;
+  constexpr int TILES = S::TILES, SHIFT = S::SHIFT;
+  constexpr bool W4 = S::W4;
   constexpr int kFewRows = S::kRows, kRing = S::kRing;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int32_t item[3];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tpitch = S::token_pitch(g.panel), spitch = S::scale_pitch(g.panel, g.group_shift);
+  const int tpitch = S::token_pitch(g.panel), spitch = S::scale_pitch(g.panel);
   uint8_t* tokens = smem;
   T* scales = reinterpret_cast<T*>(smem + S::tokens(g.panel));
-  uint16_t* zeros = reinterpret_cast<uint16_t*>(smem + S::tokens(g.panel) +
-                                                S::scales(g.panel, g.group_shift));
-  const uint32_t ring = shared_addr(smem + S::tokens(g.panel) +
-                                    2 * S::scales(g.panel, g.group_shift)) +
-                        warp * kRing * kStageBytes;
+  uint16_t* zeros = reinterpret_cast<uint16_t*>(smem + S::tokens(g.panel) + S::scales(g.panel));
+  uint8_t* ring = smem + S::ring(g.panel) + warp * kRing * kStageBytes;
   const int gq = lane >> 2, tq = lane & 3;  // row and column quad of the matrix fragments
 
   // The item of this block: rows [begin, begin + n) of one expert. Items are numbered expert
@@ -240,20 +237,26 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
   const int row_bytes = W4 ? (int)g.w_pitch : g.inner * 2;
   const int stages = k_end > k_begin ? (k_end - k_begin + S::kStageInner - 1) / S::kStageInner : 0;
   const int byte0 = W4 ? k_begin / 2 : k_begin * 2;
+  // this lane's piece of rows lane / 8 + 4 j of a stage
+  const char* src0 = wbase + (int64_t)(lane >> 3) * g.w_pitch + byte0 + (lane & 7) * 16;
+  const uint32_t dst0 = shared_addr(ring) + (lane >> 3) * kRowPitch + (lane & 7) * 16;
+  const int rest0 = row_bytes - byte0 - (lane & 7) * 16, rows_in = g.outer - my_row0 - (lane >> 3);
+  int load_slot = 0;
   auto load_stage = [&](int i) {
     if (i < stages) {
-      const int at = byte0 + i * kRowBytes + (lane & 7) * 16;
-      const uint32_t dst = ring + (i % kRing) * kStageBytes + (lane & 7) * 16;
+      const int rest = min(max(rest0 - i * kRowBytes, 0), 16);
+      const char* src = src0 + i * kRowBytes;
+      const uint32_t dst = dst0 + load_slot * kStageBytes;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int row = (lane >> 3) + 4 * j;
-        int valid = min(max(row_bytes - at, 0), 16);
-        if (my_row0 + row >= g.outer) valid = 0;
-        const char* src = valid ? wbase + (int64_t)row * g.w_pitch + at
-                                : static_cast<const char*>(g.w);
-        copy16(dst + row * kRowPitch, src, valid, g.w_align);
+        const int valid = 4 * j < rows_in ? rest : 0;
+        copy16<S::ALIGN>(dst + 4 * j * kRowPitch,
+                         valid ? src + (int64_t)(4 * j) * g.w_pitch
+                               : static_cast<const char*>(g.w),
+                         valid);
       }
     }
+    load_slot = load_slot + 1 == kRing ? 0 : load_slot + 1;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
@@ -268,6 +271,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
 
   const uint16_t* x = static_cast<const uint16_t*>(g.x);
   int kp = g.panel;  // inner position in the panel
+  int slot = 0;      // stage of the ring to multiply next
   for (int i = 0; i < stages; ++i, kp += S::kStageInner) {
     if (kp == g.panel) {
       kp = 0;
@@ -304,20 +308,17 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
               make_uint4(v[0], v[1], v[2], v[3]);
         }
       }
-      if (W4) {
-        const int bits = 31 - __clz(g.panel >> g.group_shift);
-        const int first = k0 >> g.group_shift;
+      if constexpr (W4) {
+        const int bits = 31 - __clz(g.panel >> SHIFT);
+        const int first = k0 >> SHIFT;
         for (int p = threadIdx.x; p < kOutBlock << bits; p += kFewThreads) {
           const int r = p >> bits, c = p & ((1 << bits) - 1);
-          T s = from_f32<T>(0.0f);
-          uint32_t z = 8;
-          if (out0 + r < g.outer && first + c < g.groups) {
-            const int64_t at = ((int64_t)expert * g.outer + out0 + r) * g.groups + first + c;
-            s = static_cast<const T*>(g.scales)[at];
-            if (g.zeros) z = g.zeros[at] & 15;
-          }
-          scales[r * spitch + c] = s;
-          zeros[r * spitch + c] = (uint16_t)(Magic<T>::kBits + z);
+          const bool in = out0 + r < g.outer && first + c < g.groups;
+          const int64_t at = ((int64_t)expert * g.outer + out0 + r) * g.groups + first + c;
+          scales[r * spitch + c] =
+              in ? static_cast<const T*>(g.scales)[at] : from_f32<T>(0.0f);
+          if constexpr (S::ZEROS)
+            zeros[r * spitch + c] = (uint16_t)(Magic<T>::kBits + (in ? g.zeros[at] & 15 : 8));
         }
       }
       __syncthreads();
@@ -325,54 +326,57 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
     load_stage(i + kRing - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
     __syncwarp();
-    const uint32_t st = ring + (i % kRing) * kStageBytes;
+    const uint8_t* st = ring + slot * kStageBytes;
+    slot = slot + 1 == kRing ? 0 : slot + 1;
     if constexpr (W4) {
-      const uint32_t a_at = st + gq * kRowPitch + tq * 4;
+      const uint8_t* a_at = st + gq * kRowPitch + tq * 4;
       const uint8_t* b_at = tokens + gq * tpitch + (kp + tq * 8) * 2;
-      const int s_at = (warp * 16 + gq) * spitch;
-      float part[TILES][4];
-#pragma unroll
-      for (int j = 0; j < S::kStageInner / 32; ++j) {
-        const int lo = s_at + ((kp + j * 32) >> g.group_shift), hi = lo + 8 * spitch;
-        if (((j * 32) & ((1 << g.group_shift) - 1)) == 0) {
-#pragma unroll
-          for (int n = 0; n < TILES; ++n)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) part[n][q] = 0.0f;
+      const int lo0 = (warp * 16 + gq) * spitch + (kp >> SHIFT);
+      constexpr int kSteps = (1 << SHIFT) / 32;  // of 32 in a scale group
+#pragma unroll(TILES == 1 ? 8 : 1)
+      for (int j0 = 0; j0 < S::kStageInner / 32; j0 += kSteps) {
+        const int lo = lo0 + j0 / kSteps, hi = lo + 8 * spitch;
+        uint32_t zl = (Magic<T>::kBits + 8) * 0x10001u, zh = zl;
+        if constexpr (S::ZEROS) {
+          zl = zeros[lo] * 0x10001u;
+          zh = zeros[hi] * 0x10001u;
         }
-        uint32_t wl, wh;
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wl) : "r"(a_at + j * 16));
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wh) : "r"(a_at + j * 16 + 8 * kRowPitch));
-        const uint32_t zl = g.zeros ? zeros[lo] * 0x10001u : (Magic<T>::kBits + 8) * 0x10001u;
-        const uint32_t zh = g.zeros ? zeros[hi] * 0x10001u : (Magic<T>::kBits + 8) * 0x10001u;
-        uint32_t pl[4], ph[4];
+        float part[TILES][4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          pl[q] = sub2<T>(((wl >> (4 * q)) & 0x000F000Fu) | Magic<T>::kBits * 0x10001u, zl);
-          ph[q] = sub2<T>(((wh >> (4 * q)) & 0x000F000Fu) | Magic<T>::kBits * 0x10001u, zh);
-        }
-        const uint32_t a0[4] = {pl[0], ph[0], pl[1], ph[1]}, a1[4] = {pl[2], ph[2], pl[3], ph[3]};
+        for (int n = 0; n < TILES; ++n)
 #pragma unroll
-        for (int n = 0; n < TILES; ++n) {
-          if (TILES == 1 || n < tiles) {
-            const uint4 b = *reinterpret_cast<const uint4*>(b_at + n * 8 * tpitch + j * 64);
-            mma_16816<T>(part[n], a0, b.x, b.y);
-            mma_16816<T>(part[n], a1, b.z, b.w);
+          for (int q = 0; q < 4; ++q) part[n][q] = 0.0f;
+#pragma unroll
+        for (int j = j0; j < j0 + kSteps; ++j) {
+          const uint32_t wl = *reinterpret_cast<const uint32_t*>(a_at + j * 16);
+          const uint32_t wh = *reinterpret_cast<const uint32_t*>(a_at + j * 16 + 8 * kRowPitch);
+          uint32_t pl[4], ph[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            pl[q] = sub2<T>(((wl >> (4 * q)) & 0x000F000Fu) | Magic<T>::kBits * 0x10001u, zl);
+            ph[q] = sub2<T>(((wh >> (4 * q)) & 0x000F000Fu) | Magic<T>::kBits * 0x10001u, zh);
           }
-        }
-        if (((j * 32 + 32) & ((1 << g.group_shift) - 1)) == 0) {
-          const float sl = to_f32<T>(scales[lo]), sh = to_f32<T>(scales[hi]);
+          const uint32_t a0[4] = {pl[0], ph[0], pl[1], ph[1]}, a1[4] = {pl[2], ph[2], pl[3], ph[3]};
 #pragma unroll
           for (int n = 0; n < TILES; ++n) {
-            acc[n][0] = fmaf(sl, part[n][0], acc[n][0]);
-            acc[n][1] = fmaf(sl, part[n][1], acc[n][1]);
-            acc[n][2] = fmaf(sh, part[n][2], acc[n][2]);
-            acc[n][3] = fmaf(sh, part[n][3], acc[n][3]);
+            if (TILES == 1 || n < tiles) {
+              const uint4 b = *reinterpret_cast<const uint4*>(b_at + n * 8 * tpitch + j * 64);
+              mma_16816<T>(part[n], a0, b.x, b.y);
+              mma_16816<T>(part[n], a1, b.z, b.w);
+            }
           }
+        }
+        const float sl = to_f32<T>(scales[lo]), sh = to_f32<T>(scales[hi]);
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) {
+          acc[n][0] = fmaf(sl, part[n][0], acc[n][0]);
+          acc[n][1] = fmaf(sl, part[n][1], acc[n][1]);
+          acc[n][2] = fmaf(sh, part[n][2], acc[n][2]);
+          acc[n][3] = fmaf(sh, part[n][3], acc[n][3]);
         }
       }
     } else {
-      const uint32_t a_at = st + (lane & 15) * kRowPitch + (lane >> 4) * 16;
+      const uint32_t a_at = shared_addr(st) + (lane & 15) * kRowPitch + (lane >> 4) * 16;
       const uint8_t* b_at = tokens + gq * tpitch + kp * 2 + tq * 4;
 #pragma unroll
       for (int j = 0; j < S::kStageInner / 16; ++j) {
@@ -430,30 +434,19 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
 }
 
 constexpr int kMaxDevices = 64;
-struct FewDevice {
-  std::mutex mu;
-  uint32_t ready = 0;  // instantiations whose shared memory limit is raised, one bit each
-};
-FewDevice g_few_devices[kMaxDevices];
 
-template <typename T, bool W4, int TILES>
-cudaError_t launch_few_tiles(FewArgs g, cudaStream_t st) {
-  using S = FewShape<W4, TILES>;
+template <typename S>
+cudaError_t launch_few_shape(FewArgs g, cudaStream_t st) {
+  static std::atomic<bool> ready[kMaxDevices];  // the kernel's shared memory limit is raised
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
-  {
-    FewDevice& d = g_few_devices[dev];
-    std::lock_guard<std::mutex> lock(d.mu);
-    const uint32_t bit = 1u << (4 * (TILES > 1) + 2 * W4 + std::is_same<T, __half>::value);
-    if (!(d.ready & bit)) {
-      err = cudaFuncSetAttribute(k_grouped_few<T, W4, TILES>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 S::total(S::kMaxPanel, 5));
-      if (err != cudaSuccess) return err;
-      d.ready |= bit;
-    }
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    err = cudaFuncSetAttribute(k_grouped_few<S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               S::total(S::kMaxPanel));
+    if (err != cudaSuccess) return err;
+    ready[dev].store(true, std::memory_order_release);
   }
   const int64_t blocks = (g.outer + kOutBlock - 1) / kOutBlock;
   const int64_t items = std::min<int64_t>(g.experts + 1, g.rows) + g.rows / S::kRows;
@@ -471,7 +464,7 @@ cudaError_t launch_few_tiles(FewArgs g, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(blocks * split * items), 1, 1);
   cfg.blockDim = dim3(kFewThreads, 1, 1);
-  cfg.dynamicSmemBytes = (size_t)S::total(g.panel, g.group_shift);
+  cfg.dynamicSmemBytes = (size_t)S::total(g.panel);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -479,15 +472,33 @@ cudaError_t launch_few_tiles(FewArgs g, cudaStream_t st) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = split > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, k_grouped_few<T, W4, TILES>, g);
+  return cudaLaunchKernelEx(&cfg, k_grouped_few<S>, g);
 }
 
-template <typename T, bool W4>
-cudaError_t launch_few_typed(const FewArgs& g, cudaStream_t st) {
+template <typename T, int SHIFT, bool ZEROS, int ALIGN>
+cudaError_t launch_few_rows(const FewArgs& g, cudaStream_t st) {
   // Items of 8 rows while few experts can have more: no test for absent column tiles in the
   // inner loop, and the tokens of twice the inner length in shared memory.
-  return g.rows <= 4 * (int64_t)g.experts || g.rows <= 8 ? launch_few_tiles<T, W4, 1>(g, st)
-                                                         : launch_few_tiles<T, W4, 4>(g, st);
+  return g.rows <= 4 * (int64_t)g.experts || g.rows <= 8
+             ? launch_few_shape<FewShape<T, 1, SHIFT, ZEROS, ALIGN>>(g, st)
+             : launch_few_shape<FewShape<T, 4, SHIFT, ZEROS, ALIGN>>(g, st);
+}
+
+template <typename T>
+cudaError_t launch_few_typed(const FewArgs& g, int group_size, int align, cudaStream_t st) {
+  if (group_size == 0) {
+    if (align == 16) return launch_few_rows<T, 0, false, 16>(g, st);
+    if (align == 4) return launch_few_rows<T, 0, false, 4>(g, st);
+    return launch_few_rows<T, 0, false, 2>(g, st);
+  }
+  if (group_size == 32)
+    return g.zeros ? launch_few_rows<T, 5, true, 16>(g, st)
+                   : launch_few_rows<T, 5, false, 16>(g, st);
+  if (group_size == 64)
+    return g.zeros ? launch_few_rows<T, 6, true, 16>(g, st)
+                   : launch_few_rows<T, 6, false, 16>(g, st);
+  return g.zeros ? launch_few_rows<T, 7, true, 16>(g, st)
+                 : launch_few_rows<T, 7, false, 16>(g, st);
 }
 
 }  // namespace
@@ -506,22 +517,20 @@ cudaError_t launch_few(const FewCall& c, cudaStream_t st) {
   g.rows = c.rows;
   g.y = c.y;
   g.x_vec = aligned16(c.x) && c.x_pitch % 8 == 0;
-  const bool half = c.dtype == LGBM_B200_DTYPE_F16;
+  int align = 16;
   if (c.group_size == 0) {
     g.w_pitch = (int64_t)c.inner * 2;
     const uintptr_t bits = reinterpret_cast<uintptr_t>(c.w) | (uintptr_t)g.w_pitch;
-    g.w_align = bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
-    return half ? launch_few_typed<__half, false>(g, st)
-                : launch_few_typed<__nv_bfloat16, false>(g, st);
+    align = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
+  } else {
+    g.w_pitch = (c.inner + 31) / 32 * 16;
+    g.scales = c.scales;
+    g.zeros = c.zeros;
+    g.groups = (c.inner + c.group_size - 1) / c.group_size;
   }
-  g.w_pitch = (c.inner + 31) / 32 * 16;
-  g.w_align = 16;
-  g.scales = c.scales;
-  g.zeros = c.zeros;
-  g.group_shift = c.group_size == 32 ? 5 : c.group_size == 64 ? 6 : 7;
-  g.groups = (c.inner + c.group_size - 1) / c.group_size;
-  return half ? launch_few_typed<__half, true>(g, st)
-              : launch_few_typed<__nv_bfloat16, true>(g, st);
+  return c.dtype == LGBM_B200_DTYPE_F16
+             ? launch_few_typed<__half>(g, c.group_size, align, st)
+             : launch_few_typed<__nv_bfloat16>(g, c.group_size, align, st);
 }
 
 }  // namespace experts

@@ -6,19 +6,33 @@
 //   WEIGHT    dw[e, n, k] = sum_{r in group e} dy[r, n] x[r, k]
 //
 // Rows are grouped: group e is rows offsets[e] .. offsets[e + 1]. All three are one kernel:
-// D (128 x BN, f32 in tensor memory) += A (128 x 64) B (64 x BN) over blocks of 64 of the
-// reduction; only the operands' layouts differ. An operand whose reduction axis is contiguous
-// in memory is staged K-major, else MN-major (panels of 64 columns), both with 128-byte
-// swizzle, so nothing is transposed on the way. A persistent grid walks the tiles of all
-// groups; one warp issues TMA loads, one issues the matrix instructions, four write results
-// out of one half of tensor memory while the next tile accumulates in the other.
+// D (f32 in tensor memory) += A B over blocks of 64 of the reduction; only the operands'
+// layouts differ. An operand whose reduction axis is contiguous in memory is staged K-major,
+// else MN-major (panels of 64 columns), both with 128-byte swizzle, so nothing is transposed
+// on the way. A persistent grid walks the tiles of all groups; in every CTA one warp issues
+// TMA loads, one the matrix instructions, and four write results out of one half of tensor
+// memory while the next tile accumulates in the other.
+//
+// Pairs. A 128 x 256 tile of one CTA takes in 48 KB for each 512 cycles of matrix work: the
+// SMs together ask more of L2 than it gives. Two CTAs of a cluster therefore share a
+// 256 x 256 tile (cta_group::2): each loads half of A and half of B, 32 KB, and the even one
+// multiplies for both. Single CTAs remain for groups of few rows and for few columns.
+//
+// Operands that TMA cannot walk (x read through an index; rows that do not start at 16 bytes:
+// 700 features are 1400 bytes) are first copied to rows that it can (k_stage_rows), which
+// costs their bytes twice more. Two ways without that copy were built and measured on 65536
+// gathered rows of 2048 against 4096 outputs, where the product takes 0.77 ms and the copy
+// 0.13: TMA gathers of four rows took about 20 cycles a row of 128 bytes (2.5 ms in all), and
+// six warps of asynchronous 16-byte copies, each waiting out its own block's latency, 1.5.
 //
 // Ragged ends. FORWARD / INPUT: a tile's rows past its group's end are computed from the next
 // group's rows and not stored (a row of A only reaches its own row of D). Rows past the last
 // group form one more group without a reduction: zeros. WEIGHT: the reduction itself ends
-// inside a block; the rows past the end are zeroed in both operands in shared memory (in
-// both, so that an infinity or NaN of the next group cannot make 0 * inf).
+// inside a block. That block's rows are gathered, and those past the end are asked for
+// outside the tensor, which TMA fills with zeros, in both operands: an infinity or NaN of the
+// next group cannot make 0 * inf.
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 
 #include <cuda.h>  // types of the tensor map; the encoder is looked up at run time
@@ -30,10 +44,10 @@ namespace experts {
 namespace {
 
 constexpr int kMatThreads = 192;   // warp 0 loads, warp 1 multiplies, warps 2..5 store
-constexpr int kTileM = 128;
+constexpr int kTileM = 128;       // rows of D of a CTA
 constexpr int kTileK = 64;         // 128 bytes of a 16-bit type: one swizzle row
 constexpr int kStoreBytes = 4 * 32 * 128;  // one 32 x 128 B staging block a storing warp
-constexpr int kBand = 16;          // row tiles of a band, see tile_of
+constexpr int kBandRows = 2048;    // rows of D of a band, see tile_of
 constexpr uint64_t kWaitNs = 2000000000;
 
 enum Mode { FORWARD = 0, INPUT = 1, WEIGHT = 2 };
@@ -45,7 +59,7 @@ struct MatArgs {
   int32_t drows;       // WEIGHT: rows of D in a group
   int32_t reduction;   // FORWARD, INPUT: length of the reduction
   int32_t out_kind;    // LGBM_B200_DTYPE_*
-  int32_t vec;         // 16-byte stores
+  int32_t unit;        // bytes of a store: what the alignment of every row of D allows
   uint32_t idesc;
   int64_t rows;
   int64_t out_pitch;
@@ -62,8 +76,19 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) {
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-__device__ __forceinline__ void bar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+// Arrives at the barrier at this address of the cluster's first CTA.
+__device__ __forceinline__ uint32_t leader_addr(uint32_t addr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
 }
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
@@ -73,7 +98,7 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(bar), "r"(parity)
@@ -104,34 +129,86 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(p));
   return p != 0;
 }
+// TMA loads into this CTA's shared memory. In a pair the barrier is the first CTA's.
+template <int CTAS>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y,
                                             uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(bar)
-      : "memory");
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
 }
+template <int CTAS>
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y,
                                             int z, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-      : "memory");
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
 }
+// Four rows of 64 elements to 512 consecutive bytes (swizzled by address, as a tile is); a
+// row outside the tensor reads as zeros.
+template <int CTAS>
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x,
+                                            const int (&row)[4], uint32_t bar) {
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4"
+        ".mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4"
+        ".mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
+        : "memory");
+}
+template <int CTAS>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                         bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
 }
+// Arrives, when the matrix work issued so far is done, at this barrier of every CTA at it.
+template <int CTAS>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   bar)
-               : "memory");
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
 }
 // 32 lanes x 32 columns of f32 of this warp's quarter of tensor memory.
 __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
@@ -145,7 +222,28 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
         "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]),
         "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Two f32 as one word of 16-bit values.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(uint32_t lo, uint32_t hi) {
+  const float x = __uint_as_float(lo), y = __uint_as_float(hi);
+  if constexpr (BF16) {
+    const __nv_bfloat162 q = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&q);
+  } else {
+    const __half2 q = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&q);
+  }
+}
+__device__ __forceinline__ void store_piece(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                            uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle (layout 2), version 1. `lead` and
@@ -165,29 +263,81 @@ struct Tile {
   int32_t red;     // length of the reduction
 };
 
-// Tile `t` of a group of mt x nt tiles: bands of kBand row tiles, column by column inside a
+// Tile `t` of a group of mt x nt tiles: bands of `band` row tiles, column by column inside a
 // band, so that the CTAs at work at one time share a few row tiles and a few column tiles.
-__device__ __forceinline__ void tile_of(int t, int mt, int nt, int& m, int& n) {
-  const int band = t / (kBand * nt), r = t - band * kBand * nt;
-  const int h = min(kBand, mt - band * kBand);
+__device__ __forceinline__ void tile_of(int t, int mt, int nt, int band, int& m, int& n) {
+  const int b = t / (band * nt), r = t - b * band * nt;
+  const int h = min(band, mt - b * band);
   n = r / h;
-  m = band * kBand + (r - n * h);
+  m = b * band + (r - n * h);
 }
 
-template <int MODE, int BN>
+// CTAS CTAs share a tile of 128 CTAS rows and BN columns of D.
+template <int BN, int CTAS>
 struct Shape {
-  static constexpr int kStageBytes = (kTileM + BN) * 128;
-  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-  static constexpr int kTmemCols = 2 * BN;  // two accumulators
+  static constexpr int kRows = kTileM * CTAS;
+  static constexpr int kCols = BN / CTAS;  // columns of B that a CTA loads
+  static constexpr int kStageBytes = (kTileM + kCols) * 128;
+  static constexpr int kStages = 196608 / kStageBytes;  // 4, 6 or 8: 192 KB
+  static constexpr int kTmemCols = 2 * BN;              // two accumulators
+  static constexpr int kBand = kBandRows / kRows;
   static constexpr int kSmem =
-      1024 + kStages * kStageBytes + kStoreBytes + 4 * (kMaxExperts + 2) + 256;
+      1024 + kStages * kStageBytes + kStoreBytes + 8 * (kMaxExperts + 2) + 256;
 };
 
-template <int MODE, int BN>
+// One 32-row block of a storing warp, from its staging block to `dst` (row pitch in bytes),
+// `bytes` of each row, UNIT bytes at a time.
+template <int UNIT>
+__device__ __forceinline__ void store_rows(uint32_t stage, char* dst, int64_t pitch, int nrows,
+                                           int bytes, int lane) {
+  constexpr int kLanes = 128 / UNIT < 32 ? 128 / UNIT : 32;  // of a row
+  constexpr int kPerStep = 32 / kLanes;                      // rows
+#pragma unroll 4
+  for (int i0 = 0; i0 < 32; i0 += kPerStep) {
+    const int i = i0 + lane / kLanes;
+#pragma unroll
+    for (int at = lane % kLanes * UNIT; at < 128; at += kLanes * UNIT) {
+      const uint32_t from = stage + i * 128 + (((at >> 4) ^ (i & 7)) << 4) + (at & 15);
+      char* to = dst + i * pitch + at;
+      if (i < nrows && at + UNIT <= bytes) {
+        if constexpr (UNIT == 16) {
+          uint32_t w[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(from)
+                       : "memory");
+          *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else if constexpr (UNIT == 8) {
+          uint32_t w[2];
+          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                       : "=r"(w[0]), "=r"(w[1])
+                       : "r"(from)
+                       : "memory");
+          *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+        } else if constexpr (UNIT == 4) {
+          uint32_t w;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
+          *reinterpret_cast<uint32_t*>(to) = w;
+        } else {
+          uint16_t w;
+          asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(from) : "memory");
+          *reinterpret_cast<uint16_t*>(to) = w;
+        }
+      }
+    }
+  }
+}
+
+struct Maps {
+  CUtensorMap a, b;              // tiles of 64 columns
+  CUtensorMap a_rows, b_rows;    // single rows of 64 columns, for gathers
+  CUtensorMap out;               // 32 rows of 128 bytes
+};
+
+template <int MODE, int BN, int CTAS>
 __global__ void __launch_bounds__(kMatThreads, 1)
-    k_grouped_matmul(const __grid_constant__ CUtensorMap map_a,
-                     const __grid_constant__ CUtensorMap map_b, const MatArgs g) {
-  using S = Shape<MODE, BN>;
+    k_grouped_matmul(const __grid_constant__ Maps maps, const MatArgs g) {
+  using S = Shape<BN, CTAS>;
   constexpr int kStages = S::kStages;
   constexpr uint32_t kABytes = kTileM * 128;
   extern __shared__ uint8_t smem_raw[];
@@ -196,12 +346,14 @@ __global__ void __launch_bounds__(kMatThreads, 1)
   const uint32_t base = smem_addr(smem);
   const uint32_t store_base = base + kStages * S::kStageBytes;
   int32_t* cum = reinterpret_cast<int32_t*>(smem + kStages * S::kStageBytes + kStoreBytes);
+  int32_t* off = cum + kMaxExperts + 2;  // the groups' first rows, then the end
   uint64_t* bars = reinterpret_cast<uint64_t*>(
-      (reinterpret_cast<uintptr_t>(cum + kMaxExperts + 2) + 15) & ~(uintptr_t)15);
+      (reinterpret_cast<uintptr_t>(off + kMaxExperts + 2) + 15) & ~(uintptr_t)15);
   const uint32_t full = smem_addr(bars), empty = full + 8 * kStages,
                  acc_full = empty + 8 * kStages, acc_empty = acc_full + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CTAS == 2 ? blockIdx.x & 1 : 0;  // in the pair; the even CTA multiplies
 
   if (warp == 0) {
     if (lane == 0) {
@@ -211,77 +363,94 @@ __global__ void __launch_bounds__(kMatThreads, 1)
       }
       for (int i = 0; i < 2; ++i) {
         bar_init(acc_full + 8 * i, 1);
-        bar_init(acc_empty + 8 * i, 4);
+        bar_init(acc_empty + 8 * i, 4 * CTAS);
       }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
-      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.b) : "memory");
     }
   } else if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_addr(tmem_slot)),
-                 "r"((uint32_t)S::kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (CTAS == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_addr(tmem_slot)),
+                   "r"((uint32_t)S::kTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_addr(tmem_slot)),
+                   "r"((uint32_t)S::kTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
   } else if (warp == 2) {
-    // first tile of every group; FORWARD and INPUT have one group more, the rows past the
-    // last offset
-    const int groups = MODE == WEIGHT ? g.experts : g.experts + 1;
+    // The groups' rows, clamped (off[i] to off[i + 1]; overlaps of offsets that decrease are
+    // cut off), and the first tile of every group. The rows past the last offset are one
+    // group more; WEIGHT has no tiles for them.
     const int nt = (g.cols + BN - 1) / BN;
-    int32_t carry = 0;
-    for (int i0 = 0; i0 < groups; i0 += 32) {
+    int32_t carry = 0, reach = 0;
+    for (int i0 = 0; i0 <= g.experts; i0 += 32) {
+      const int i = i0 + lane;
+      int32_t b = i <= g.experts ? (int32_t)min(max((int64_t)g.offsets[i], (int64_t)0), g.rows) : 0;
+      b = max(b, reach);
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int32_t o = __shfl_up_sync(0xFFFFFFFFu, b, d);
+        if (lane >= d) b = max(b, o);
+      }
+      reach = __shfl_sync(0xFFFFFFFFu, b, 31);
+      if (i <= g.experts) off[i] = b;
+    }
+    if (lane == 0) off[g.experts + 1] = (int32_t)g.rows;
+    __syncwarp();
+    for (int i0 = 0; i0 <= g.experts; i0 += 32) {
       const int i = i0 + lane;
       int32_t v = 0;
-      if (i < groups) {
-        if (MODE == WEIGHT) {
-          v = (g.drows + kTileM - 1) / kTileM * nt;
-        } else {
-          int64_t b = min(max((int64_t)g.offsets[i], (int64_t)0), g.rows);
-          int64_t e = i < g.experts ? min(max((int64_t)g.offsets[i + 1], b), g.rows) : g.rows;
-          v = (int32_t)((e - b + kTileM - 1) / kTileM) * nt;
-        }
-      }
+      if (MODE == WEIGHT)
+        v = i < g.experts ? (g.drows + S::kRows - 1) / S::kRows * nt : 0;
+      else if (i <= g.experts)
+        v = (off[i + 1] - off[i] + S::kRows - 1) / S::kRows * nt;
       int32_t s = v;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int32_t o = __shfl_up_sync(0xFFFFFFFFu, s, d);
         if (lane >= d) s += o;
       }
-      if (i < groups) cum[i] = carry + s - v;
+      if (i <= g.experts) cum[i] = carry + s - v;
       carry += __shfl_sync(0xFFFFFFFFu, s, 31);
     }
-    if (lane == 0) cum[groups] = carry;
+    if (lane == 0) cum[g.experts + 1] = carry;
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();  // the other CTA's barriers are set up too
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  const int groups = MODE == WEIGHT ? g.experts : g.experts + 1;
-  const int tiles = cum[groups];
+  const int tiles = cum[g.experts + 1];
   const int nt = (g.cols + BN - 1) / BN;
+  const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   auto decode = [&](int t) {
-    int lo = 0, hi = groups;  // the last group that starts at or before t
+    int lo = 0, hi = g.experts + 1;  // the last group that starts at or before t
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (cum[mid] <= t) lo = mid; else hi = mid;
     }
-    int64_t b = min(max((int64_t)g.offsets[lo], (int64_t)0), g.rows);
-    int64_t e = lo < g.experts ? min(max((int64_t)g.offsets[lo + 1], b), g.rows) : g.rows;
+    const int b = off[lo], e = off[lo + 1];
     Tile r;
     r.group = lo;
     int m, n;
-    const int drows = MODE == WEIGHT ? g.drows : (int)(e - b);
-    tile_of(t - cum[lo], (drows + kTileM - 1) / kTileM, nt, m, n);
+    const int drows = MODE == WEIGHT ? g.drows : e - b;
+    tile_of(t - cum[lo], (drows + S::kRows - 1) / S::kRows, nt, S::kBand, m, n);
     r.n0 = n * BN;
+    r.m0 = m * S::kRows + rank * kTileM;
     if (MODE == WEIGHT) {
-      r.m0 = m * kTileM;
       r.m_end = g.drows;
-      r.red0 = (int)b;
-      r.red = (int)(e - b);
+      r.red0 = b;
+      r.red = e - b;
     } else {
-      r.m0 = (int)b + m * kTileM;
-      r.m_end = (int)e;
+      r.m0 += b;
+      r.m_end = e;
       r.red0 = 0;
       r.red = lo < g.experts ? g.reduction : 0;
     }
@@ -291,29 +460,48 @@ __global__ void __launch_bounds__(kMatThreads, 1)
   bool ok = true;
   if (warp == 0) {
     uint32_t it = 0;
-    for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+    for (int t = first; ok && t < tiles; t += step) {
       const Tile r = decode(t);
+      const int nb = r.n0 + rank * S::kCols;  // first column of this CTA's share of B
       for (int k0 = 0; k0 < r.red; k0 += kTileK, ++it) {
         const uint32_t s = it % kStages;
         if (it >= kStages && !(ok = bar_wait(empty + 8 * s, (it / kStages - 1) & 1))) break;
-        if (elect_one()) {
-          const uint32_t a = base + s * S::kStageBytes, b = a + kABytes, bar = full + 8 * s;
-          bar_expect(bar, S::kStageBytes);
+        const uint32_t a = base + s * S::kStageBytes, b = a + kABytes;
+        const uint32_t bar = CTAS == 2 ? leader_addr(full + 8 * s) : full + 8 * s;
+        if (rank == 0 && elect_one()) bar_expect(full + 8 * s, CTAS * S::kStageBytes);
+        __syncwarp();
+        if (MODE == WEIGHT && r.red - k0 < kTileK) {
+          // the group's end: rows one by one, lanes 0..15 and 16..31 a panel each, and the
+          // first row outside the tensor for those past the end
+          int row[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int at = 4 * (lane & 15) + j;
+            row[j] = at < r.red - k0 ? r.red0 + k0 + at : (int)g.rows;
+          }
+          tma_gather4<CTAS>(a + (lane >> 4) * 8192 + (lane & 15) * 512, &maps.a_rows,
+                            r.m0 + 64 * (lane >> 4), row, bar);
+#pragma unroll
+          for (int j = 0; j < S::kCols / 64; j += 2)
+            if (j + (lane >> 4) < S::kCols / 64)
+              tma_gather4<CTAS>(b + (j + (lane >> 4)) * 8192 + (lane & 15) * 512, &maps.b_rows,
+                                nb + 64 * (j + (lane >> 4)), row, bar);
+        } else if (elect_one()) {
           if (MODE == WEIGHT) {
 #pragma unroll
             for (int j = 0; j < kTileM / 64; ++j)
-              tma_load_2d(a + j * 8192, &map_a, r.m0 + 64 * j, r.red0 + k0, bar);
+              tma_load_2d<CTAS>(a + j * 8192, &maps.a, r.m0 + 64 * j, r.red0 + k0, bar);
 #pragma unroll
-            for (int j = 0; j < BN / 64; ++j)
-              tma_load_2d(b + j * 8192, &map_b, r.n0 + 64 * j, r.red0 + k0, bar);
+            for (int j = 0; j < S::kCols / 64; ++j)
+              tma_load_2d<CTAS>(b + j * 8192, &maps.b, nb + 64 * j, r.red0 + k0, bar);
           } else {
-            tma_load_2d(a, &map_a, k0, r.m0, bar);
+            tma_load_2d<CTAS>(a, &maps.a, k0, r.m0, bar);
             if (MODE == FORWARD) {
-              tma_load_3d(b, &map_b, k0, r.n0, r.group, bar);
+              tma_load_3d<CTAS>(b, &maps.b, k0, nb, r.group, bar);
             } else {
 #pragma unroll
-              for (int j = 0; j < BN / 64; ++j)
-                tma_load_3d(b + j * 8192, &map_b, r.n0 + 64 * j, k0, r.group, bar);
+              for (int j = 0; j < S::kCols / 64; ++j)
+                tma_load_3d<CTAS>(b + j * 8192, &maps.b, nb + 64 * j, k0, r.group, bar);
             }
           }
         }
@@ -321,13 +509,14 @@ __global__ void __launch_bounds__(kMatThreads, 1)
       }
     }
     // no copy may be in flight when the CTA ends: a load whose block nobody multiplied
-    // (another warp gave up) has still landed before the CTA leaves
-    if (!ok)
+    // (another warp gave up) has landed, two seconds later, before the CTAs leave; the
+    // first CTA, whose barrier counts the loads of both, looks
+    if (!ok && rank == 0)
       for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
         bar_wait(full + 8 * (i % kStages), (i / kStages) & 1);
   } else if (warp == 1) {
     uint32_t it = 0, tile = 0;
-    for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+    for (int t = first; rank == 0 && ok && t < tiles; t += step) {
       const Tile r = decode(t);
       if (r.red == 0) continue;
       const uint32_t acc = tile & 1, d = tmem + acc * BN;
@@ -336,25 +525,10 @@ __global__ void __launch_bounds__(kMatThreads, 1)
       for (int k0 = 0; k0 < r.red; k0 += kTileK, ++it) {
         const uint32_t s = it % kStages;
         if (!(ok = bar_wait(full + 8 * s, (it / kStages) & 1))) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t a = base + s * S::kStageBytes, b = a + kABytes;
-        int steps = kTileK / 16;
-        if (MODE == WEIGHT && r.red - k0 < kTileK) {
-          // the group ends inside this block: whole steps past it are left out, and the rows
-          // between its end and the last step's are zeroed in every panel
-          const int valid = r.red - k0;
-          steps = (valid + 15) / 16;
-          const int rest = steps * 16 - valid;
-          constexpr int kPanels = (kTileM + BN) / 64;
-          for (int i = lane; i < rest * kPanels * 8; i += 32) {
-            const int panel = i / (rest * 8), row = i / 8 % rest;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                             a + panel * 8192 + (valid + row) * 128 + (i & 7) * 16),
-                         "r"(0)
-                         : "memory");
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
+        // the last block in whole steps of 16: what lies past the end in them is zeros
+        const int steps = (min(r.red - k0, kTileK) + 15) / 16;
         if (elect_one()) {
           for (int k = 0; k < steps; ++k) {
             // 16 of the reduction: 32 bytes along a K-major row, 16 rows of an MN-major panel
@@ -362,24 +536,27 @@ __global__ void __launch_bounds__(kMatThreads, 1)
                                                : smem_desc(a + k * 32, 16, 1024);
             const uint64_t db = MODE == FORWARD ? smem_desc(b + k * 32, 16, 1024)
                                                 : smem_desc(b + k * 2048, 8192, 1024);
-            mma_f16(d, da, db, g.idesc, k0 > 0 || k > 0);
+            mma_f16<CTAS>(d, da, db, g.idesc, k0 > 0 || k > 0);
           }
-          mma_commit(empty + 8 * s);
+          mma_commit<CTAS>(empty + 8 * s);
         }
         __syncwarp();
       }
       if (!ok) break;
-      if (elect_one()) mma_commit(acc_full + 8 * acc);
+      if (elect_one()) mma_commit<CTAS>(acc_full + 8 * acc);
       __syncwarp();
       ++tile;
     }
   } else {
     const int quarter = warp & 3;
     const uint32_t stage = store_base + (warp - 2) * 4096;
-    const int bytes = g.out_kind == LGBM_B200_DTYPE_F32 ? 4 : 2;
+    const bool wide = g.out_kind == LGBM_B200_DTYPE_F32;
+    const int bytes = wide ? 4 : 2;
     const int per_chunk = 128 / bytes;  // columns of a 128-byte staging row
+    const int64_t pitch = g.out_pitch * bytes;
+    const uint32_t row_at = stage + lane * 128, swizzle = lane & 7;
     uint32_t tile = 0;
-    for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+    for (int t = first; ok && t < tiles; t += step) {
       const Tile r = decode(t);
       const uint32_t acc = tile & 1;
       if (r.red > 0) {
@@ -387,132 +564,141 @@ __global__ void __launch_bounds__(kMatThreads, 1)
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
       const int row0 = r.m0 + quarter * 32;
+      const uint32_t from = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
       char* out = static_cast<char*>(g.out);
-      if (MODE == WEIGHT) out += (int64_t)r.group * g.drows * g.out_pitch * bytes;
-      const int ncols = min(BN, g.cols - r.n0);
-      for (int c0 = 0; c0 < ncols; c0 += per_chunk) {
-        // this lane's row into the staging block, 16-byte pieces swizzled by row
-        for (int h = 0; h < per_chunk; h += 32) {
-          uint32_t v[32];
-          if (r.red > 0) {
-            tmem_load32(tmem + acc * BN + ((uint32_t)(quarter * 32) << 16) + c0 + h, v);
-          } else {
+      int out_row = row0;  // of D as one matrix
+      if (MODE == WEIGHT) {
+        out += (int64_t)r.group * g.drows * pitch;
+        out_row += r.group * g.drows;
+      }
+      const int ncols = min(BN, g.cols - r.n0), nrows = min(32, r.m_end - row0);
+      // whole 32-row blocks leave by TMA, which also cuts off the last columns
+      const bool by_tma = g.unit == 16 && nrows == 32;
+      for (int c0 = 0; c0 < ncols && nrows > 0; c0 += per_chunk) {
+        // this lane's row of the chunk
+        uint32_t v[64];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0;
-          }
-          if (g.out_kind == LGBM_B200_DTYPE_F32) {
-#pragma unroll
-            for (int p = 0; p < 8; ++p)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                               stage + lane * 128 + ((p ^ (lane & 7)) << 4)),
-                           "r"(v[4 * p]), "r"(v[4 * p + 1]), "r"(v[4 * p + 2]), "r"(v[4 * p + 3])
-                           : "memory");
-          } else {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float x = __uint_as_float(v[2 * i]), y = __uint_as_float(v[2 * i + 1]);
-              if (g.out_kind == LGBM_B200_DTYPE_BF16) {
-                const __nv_bfloat162 q = __floats2bfloat162_rn(x, y);
-                w[i] = *reinterpret_cast<const uint32_t*>(&q);
-              } else {
-                const __half2 q = __floats2half2_rn(x, y);
-                w[i] = *reinterpret_cast<const uint32_t*>(&q);
-              }
-            }
-#pragma unroll
-            for (int p = 0; p < 4; ++p)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                               stage + lane * 128 + (((h / 8 + p) ^ (lane & 7)) << 4)),
-                           "r"(w[4 * p]), "r"(w[4 * p + 1]), "r"(w[4 * p + 2]), "r"(w[4 * p + 3])
-                           : "memory");
-          }
+        for (int i = 0; i < 64; ++i) v[i] = 0;
+        if (r.red > 0) {
+          tmem_load32(from + c0, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+          if (!wide) tmem_load32(from + c0 + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
+          tmem_wait();
         }
+        // the staging block is free when the last store has read it
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
-        const int n = min(per_chunk, ncols - c0);
-        char* dst = out + ((int64_t)row0 * g.out_pitch + r.n0 + c0) * bytes;
-        const int nrows = min(32, r.m_end - row0);
-        if (g.vec && n * bytes % 16 == 0) {
-          // 8 lanes a row, 4 rows a store
-          for (int i = lane >> 3; i < nrows; i += 4) {
-            const int p = lane & 7;
-            if (p * 16 < n * bytes) {
-              uint32_t w[4];
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                           : "r"(stage + i * 128 + ((p ^ (i & 7)) << 4))
-                           : "memory");
-              *reinterpret_cast<uint4*>(dst + (int64_t)i * g.out_pitch * bytes + p * 16) =
-                  make_uint4(w[0], w[1], w[2], w[3]);
-            }
+        // 16-byte pieces, swizzled by row
+        if (wide) {
+#pragma unroll
+          for (int p = 0; p < 8; ++p)
+            store_piece(row_at + ((p ^ swizzle) << 4), v[4 * p], v[4 * p + 1], v[4 * p + 2],
+                        v[4 * p + 3]);
+        } else if (g.out_kind == LGBM_B200_DTYPE_BF16) {
+#pragma unroll
+          for (int p = 0; p < 8; ++p)
+            store_piece(row_at + ((p ^ swizzle) << 4), pack2<true>(v[8 * p], v[8 * p + 1]),
+                        pack2<true>(v[8 * p + 2], v[8 * p + 3]),
+                        pack2<true>(v[8 * p + 4], v[8 * p + 5]),
+                        pack2<true>(v[8 * p + 6], v[8 * p + 7]));
+        } else {
+#pragma unroll
+          for (int p = 0; p < 8; ++p)
+            store_piece(row_at + ((p ^ swizzle) << 4), pack2<false>(v[8 * p], v[8 * p + 1]),
+                        pack2<false>(v[8 * p + 2], v[8 * p + 3]),
+                        pack2<false>(v[8 * p + 4], v[8 * p + 5]),
+                        pack2<false>(v[8 * p + 6], v[8 * p + 7]));
+        }
+        if (by_tma) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            asm volatile(
+                "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                    &maps.out),
+                "r"(r.n0 + c0), "r"(out_row), "r"(stage)
+                : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         } else {
-          for (int i = 0; i < nrows; ++i)
-            for (int c = lane; c < n; c += 32) {
-              const uint32_t at = stage + i * 128 + (((c * bytes >> 4) ^ (i & 7)) << 4) +
-                                  (c * bytes & 15);
-              if (bytes == 4) {
-                uint32_t w;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
-                *reinterpret_cast<uint32_t*>(dst + ((int64_t)i * g.out_pitch + c) * 4) = w;
-              } else {
-                uint16_t w;
-                asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(at) : "memory");
-                *reinterpret_cast<uint16_t*>(dst + ((int64_t)i * g.out_pitch + c) * 2) = w;
-              }
-            }
+          __syncwarp();
+          const int n = min(per_chunk, ncols - c0) * bytes;
+          char* dst = out + (int64_t)row0 * pitch + (int64_t)(r.n0 + c0) * bytes;
+          if (g.unit == 16) store_rows<16>(stage, dst, pitch, nrows, n, lane);
+          else if (g.unit == 8) store_rows<8>(stage, dst, pitch, nrows, n, lane);
+          else if (g.unit == 4) store_rows<4>(stage, dst, pitch, nrows, n, lane);
+          else store_rows<2>(stage, dst, pitch, nrows, n, lane);
         }
         __syncwarp();
       }
       if (r.red > 0) {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) bar_arrive(acc_empty + 8 * acc);
+        if (lane == 0)
+          bar_arrive_cluster(CTAS == 2 ? leader_addr(acc_empty + 8 * acc) : acc_empty + 8 * acc);
         ++tile;
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   if (!ok && lane == 0) atomicOr(g.error, 1u);
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();  // neither leaves while the other may still reach it
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                 "r"((uint32_t)S::kTmemCols));
+  if (warp == 1) {
+    if constexpr (CTAS == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                   "r"((uint32_t)S::kTmemCols));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                   "r"((uint32_t)S::kTmemCols));
+  }
 }
 
 // Rows copied to a pitch that TMA can walk: dst[r] = src[index ? index[r] : r], the columns
 // between `width` and `dst_pitch` zero; a row whose index is outside is zero.
+// UNIT bytes of a row are read at a time (its alignment), 16 written; a thread takes kStageRun
+// pieces, all loads first.
+constexpr int kStageRun = 4;
+
+template <int UNIT>
 __global__ void __launch_bounds__(256)
-    k_stage_rows(const uint16_t* src, int64_t src_rows, int64_t rows, int width, int64_t pitch,
-                 const int32_t* index, uint16_t* dst, int64_t dst_pitch, int words) {
-  const int per_row = (int)(dst_pitch / 8);
-  const int64_t total = rows * per_row;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per_row;
-    const int c = (int)(i - r * per_row) * 8;
-    const int64_t at = index ? index[r] : r;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (at >= 0 && at < src_rows) {
-      const uint16_t* p = src + at * pitch + c;
-      if (words == 8 && c + 8 <= width) {
-        v = *reinterpret_cast<const uint4*>(p);
-      } else if (words >= 4 && c + 8 <= width) {
-        const uint2 lo = *reinterpret_cast<const uint2*>(p);
-        const uint2 hi = *reinterpret_cast<const uint2*>(p + 4);
-        v = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      } else {
-        uint16_t e[8];
+    k_stage_rows(const char* __restrict__ src, int32_t src_rows, int64_t pieces, int bytes,
+                 int64_t pitch, const int32_t* __restrict__ index, uint4* dst, uint32_t per_row) {
+  const int64_t first = (int64_t)blockIdx.x * (256 * kStageRun) + threadIdx.x;
+  uint4 v[kStageRun];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = c + j < width ? p[j] : (uint16_t)0;
-        v = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
-                       e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
-      }
+  for (int u = 0; u < kStageRun; ++u) {
+    const int64_t i = first + u * 256;
+    v[u] = make_uint4(0, 0, 0, 0);
+    if (i >= pieces) continue;
+    const int64_t r = (uint64_t)i < 0xFFFFFFFFu ? (uint32_t)i / per_row : i / per_row;
+    const int c = (int)(i - r * per_row) * 16;
+    const int64_t at = index ? index[r] : r;
+    if (at < 0 || (index && at >= src_rows)) continue;
+    const char* p = src + at * pitch + c;
+    if (UNIT == 16 && c + 16 <= bytes) {
+      v[u] = __ldg(reinterpret_cast<const uint4*>(p));
+    } else if (UNIT >= 8 && c + 16 <= bytes) {
+      const uint2 lo = __ldg(reinterpret_cast<const uint2*>(p));
+      const uint2 hi = __ldg(reinterpret_cast<const uint2*>(p + 8));
+      v[u] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    } else if (UNIT >= 4 && c + 16 <= bytes) {
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
+      v[u] = make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
+    } else {
+      uint32_t e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        e[j] = c + 2 * j < bytes ? __ldg(reinterpret_cast<const uint16_t*>(p) + j) : 0;
+      v[u] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16,
+                        e[6] | e[7] << 16);
     }
-    *reinterpret_cast<uint4*>(dst + r * dst_pitch + c) = v;
   }
+#pragma unroll
+  for (int u = 0; u < kStageRun; ++u)
+    if (first + u * 256 < pieces) dst[first + u * 256] = v[u];
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -533,18 +719,20 @@ EncodeTiled encoder() {
   return fn;
 }
 
-// A tensor of 16-bit elements, innermost axis first; boxes of 64 x `box1` elements, 128-byte
-// swizzle, zeros outside the tensor.
+// A tensor, innermost axis first; boxes of 128 bytes x `box1` rows (one row for gathers),
+// 128-byte swizzle, zeros outside the tensor.
 bool encode(CUtensorMap* map, int32_t dtype, const void* base, int rank, const int64_t* dims,
             const int64_t* pitches, int box1) {
+  const int bytes = elem_size(dtype);
   cuuint64_t d[3], s[2];
-  cuuint32_t box[3] = {64, (cuuint32_t)box1, 1}, step[3] = {1, 1, 1};
+  cuuint32_t box[3] = {(cuuint32_t)(128 / bytes), (cuuint32_t)box1, 1}, step[3] = {1, 1, 1};
   for (int i = 0; i < rank; ++i) d[i] = (cuuint64_t)dims[i];
-  for (int i = 0; i + 1 < rank; ++i) s[i] = (cuuint64_t)pitches[i] * 2;
+  for (int i = 0; i + 1 < rank; ++i) s[i] = (cuuint64_t)pitches[i] * bytes;
   const EncodeTiled fn = encoder();
   return fn && fn(map,
-                  dtype == LGBM_B200_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                  dtype == LGBM_B200_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                  : dtype == LGBM_B200_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                   (cuuint32_t)rank, const_cast<void*>(base), d, s, box, step,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -555,17 +743,15 @@ bool encode(CUtensorMap* map, int32_t dtype, const void* base, int rank, const i
 constexpr int kMaxDevices = 64;
 struct DeviceInfo {
   std::mutex mu;
-  int sms = 0;
   uint32_t* error = nullptr;
-  uint32_t smem_set = 0;  // instantiations whose shared memory limit is raised, one bit each
 };
 DeviceInfo g_devices[kMaxDevices];
 
-template <int MODE, int BN>
-cudaError_t launch_tiles(const CUtensorMap& a, const CUtensorMap& b, MatArgs g,
-                         int64_t most_tiles, cudaStream_t st) {
-  using S = Shape<MODE, BN>;
-  int dev = 0, sms = 0;
+template <int MODE, int BN, int CTAS>
+cudaError_t launch_tiles(const Maps& maps, MatArgs g, int64_t most_tiles, cudaStream_t st) {
+  using S = Shape<BN, CTAS>;
+  static std::atomic<int> most_ready[kMaxDevices];  // tiles at work at a time; 0: not set up
+  int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
@@ -574,24 +760,38 @@ cudaError_t launch_tiles(const CUtensorMap& a, const CUtensorMap& b, MatArgs g,
     std::lock_guard<std::mutex> lock(d.mu);
     if (!d.error) {
       void* p = nullptr;
-      err = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
-      if (err == cudaSuccess) err = cudaGetSymbolAddress(&p, g_matmul_error);
+      err = cudaGetSymbolAddress(&p, g_matmul_error);
       if (err != cudaSuccess) return err;
       d.error = static_cast<uint32_t*>(p);
     }
-    constexpr uint32_t bit = 1u << (MODE * 3 + (BN == 64 ? 0 : BN == 128 ? 1 : 2));
-    if (!(d.smem_set & bit)) {
-      err = cudaFuncSetAttribute(k_grouped_matmul<MODE, BN>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-      if (err != cudaSuccess) return err;
-      d.smem_set |= bit;
-    }
     g.error = d.error;
-    sms = d.sms;
   }
-  const int grid = (int)std::min<int64_t>(sms, most_tiles);
-  k_grouped_matmul<MODE, BN><<<grid, kMatThreads, S::kSmem, st>>>(a, b, g);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(CTAS, 1, 1);
+  cfg.blockDim = dim3(kMatThreads, 1, 1);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CTAS;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = CTAS == 2 ? 1 : 0;
+  int most = most_ready[dev].load(std::memory_order_acquire);
+  if (most == 0) {
+    err = cudaFuncSetAttribute(k_grouped_matmul<MODE, BN, CTAS>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    // a pair that finds no room would start when the others have finished: ask how many fit
+    if (err == cudaSuccess && CTAS == 2)
+      err = cudaOccupancyMaxActiveClusters(&most, k_grouped_matmul<MODE, BN, CTAS>, &cfg);
+    else if (err == cudaSuccess)
+      err = cudaDeviceGetAttribute(&most, cudaDevAttrMultiProcessorCount, dev);
+    if (err != cudaSuccess) return err;
+    if (most < 1) return cudaErrorInvalidConfiguration;
+    most_ready[dev].store(most, std::memory_order_release);
+  }
+  cfg.gridDim.x = (unsigned)(std::min<int64_t>(most, most_tiles) * CTAS);
+  return cudaLaunchKernelEx(&cfg, k_grouped_matmul<MODE, BN, CTAS>, maps, g);
 }
 
 // An operand as TMA can read it: 16-byte base and pitches, or a copy in the workspace.
@@ -609,61 +809,86 @@ int64_t copy_bytes(int64_t rows, int64_t width) {
 cudaError_t stage(Operand& o, int64_t src_rows, int64_t rows, int width, const int32_t* index,
                   char*& workspace, cudaStream_t st) {
   const int64_t dst_pitch = padded(width);
-  uint16_t* dst = reinterpret_cast<uint16_t*>(workspace);
+  uint4* dst = reinterpret_cast<uint4*>(workspace);
   workspace += copy_bytes(rows, width);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(o.p) | (uintptr_t)(o.pitch * 2);
-  const int words = bits % 16 == 0 ? 8 : bits % 8 == 0 ? 4 : 1;
-  const int64_t want = (rows * (dst_pitch / 8) + 255) / 256;
-  k_stage_rows<<<(unsigned)std::min<int64_t>(want, 1 << 20), 256, 0, st>>>(
-      static_cast<const uint16_t*>(o.p), src_rows, rows, width, o.pitch, index, dst, dst_pitch,
-      words);
+  const int64_t pieces = rows * (dst_pitch / 8);
+  const int64_t blocks = (pieces + 256 * kStageRun - 1) / (256 * kStageRun);
+  if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+  auto go = [&](auto unit) {
+    k_stage_rows<decltype(unit)::value><<<(unsigned)blocks, 256, 0, st>>>(
+        static_cast<const char*>(o.p), (int32_t)src_rows, pieces, width * 2, o.pitch * 2, index,
+        dst, (uint32_t)(dst_pitch / 8));
+  };
+  if (bits % 16 == 0) go(std::integral_constant<int, 16>());
+  else if (bits % 8 == 0) go(std::integral_constant<int, 8>());
+  else if (bits % 4 == 0) go(std::integral_constant<int, 4>());
+  else go(std::integral_constant<int, 2>());
   o.p = dst;
   o.pitch = dst_pitch;
   return cudaGetLastError();
 }
 
-uint32_t instruction(int32_t dtype, bool a_mn, bool b_mn, int bn) {
+uint32_t instruction(int32_t dtype, bool a_mn, bool b_mn, int m, int n) {
   const uint32_t type = dtype == LGBM_B200_DTYPE_BF16 ? 1 : 0;
   return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)a_mn << 15) |
-         ((uint32_t)b_mn << 16) | ((uint32_t)(bn / 8) << 17) | ((uint32_t)(kTileM / 16) << 24);
+         ((uint32_t)b_mn << 16) | ((uint32_t)(n / 8) << 17) | ((uint32_t)(m / 16) << 24);
 }
 
+// a: x (FORWARD) or dy; b: w, or x (WEIGHT).
 template <int MODE>
-cudaError_t run_tiles(const Operand& a, int64_t a_width, int64_t rows, const Operand& b,
-                      int64_t b_width, int32_t dtype, MatArgs g, cudaStream_t st) {
+cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64_t b_width,
+                      int32_t dtype, MatArgs g, cudaStream_t st) {
   const int bytes = elem_size(g.out_kind);
-  g.vec = aligned16(g.out) && g.out_pitch * bytes % 16 == 0 &&
-          (int64_t)g.drows * g.out_pitch * bytes % 16 == 0;
-  auto go = [&](auto bn_c) -> cudaError_t {
-    constexpr int BN = decltype(bn_c)::value;
-    CUtensorMap ma, mb;
-    const int64_t da[3] = {a_width, rows, 1}, pa[2] = {a.pitch, 0};
-    bool fine = encode(&ma, dtype, a.p, 2, da, pa, MODE == WEIGHT ? 64 : kTileM);
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(g.out) | (uintptr_t)(g.out_pitch * bytes) |
+                         (uintptr_t)(g.cols * bytes);
+  g.unit = bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
+  auto go = [&](auto bn_c, auto ctas_c) -> cudaError_t {
+    constexpr int BN = decltype(bn_c)::value, CTAS = decltype(ctas_c)::value;
+    using S = Shape<BN, CTAS>;
+    Maps maps;
+    const int64_t da[3] = {a_width, g.rows, 1}, pa[2] = {a.pitch, 0};
+    bool fine = encode(&maps.a, dtype, a.p, 2, da, pa, MODE == WEIGHT ? 64 : kTileM);
+    if (MODE == WEIGHT) fine = fine && encode(&maps.a_rows, dtype, a.p, 2, da, pa, 1);
+    else maps.a_rows = maps.a;
+    maps.b_rows = maps.a;  // not used unless set below
     if (MODE == WEIGHT) {
-      const int64_t db[3] = {b_width, rows, 1}, pb[2] = {b.pitch, 0};
-      fine = fine && encode(&mb, dtype, b.p, 2, db, pb, 64);
+      const int64_t db[3] = {b_width, g.rows, 1}, pb[2] = {b.pitch, 0};
+      fine = fine && encode(&maps.b, dtype, b.p, 2, db, pb, 64) &&
+             encode(&maps.b_rows, dtype, b.p, 2, db, pb, 1);
     } else {
       const int64_t n = MODE == FORWARD ? g.cols : g.reduction;
       const int64_t db[3] = {b_width, n, g.experts}, pb[2] = {b.pitch, b.pitch * n};
-      fine = fine && encode(&mb, dtype, b.p, 3, db, pb, MODE == FORWARD ? BN : 64);
+      fine = fine && encode(&maps.b, dtype, b.p, 3, db, pb, MODE == FORWARD ? S::kCols : 64);
+    }
+    maps.out = maps.a;  // not used unless set
+    const int64_t rows_d = MODE == WEIGHT ? (int64_t)g.experts * g.drows : g.rows;
+    if (g.unit == 16 && rows_d > INT32_MAX) g.unit = 8;  // no coordinate for its last rows
+    if (g.unit == 16) {
+      const int64_t dd[3] = {g.cols, rows_d, 1}, pd[2] = {g.out_pitch, 0};
+      fine = fine && encode(&maps.out, g.out_kind, g.out, 2, dd, pd, 32);
     }
     if (!fine) return cudaErrorInvalidValue;
-    g.idesc = instruction(dtype, MODE == WEIGHT, MODE != FORWARD, BN);
+    g.idesc = instruction(dtype, MODE == WEIGHT, MODE != FORWARD, S::kRows, BN);
     const int64_t nt = (g.cols + BN - 1) / BN;
     const int64_t most = MODE == WEIGHT
-                             ? (int64_t)g.experts * ((g.drows + kTileM - 1) / kTileM) * nt
-                             : (rows / kTileM + g.experts + 1) * nt;
-    return launch_tiles<MODE, BN>(ma, mb, g, most, st);
+                             ? (int64_t)g.experts * ((g.drows + S::kRows - 1) / S::kRows) * nt
+                             : (g.rows / S::kRows + g.experts + 1) * nt;
+    return launch_tiles<MODE, BN, CTAS>(maps, g, most, st);
   };
-  if (g.cols <= 64) return go(std::integral_constant<int, 64>());
-  if (g.cols <= 128) return go(std::integral_constant<int, 128>());
-  return go(std::integral_constant<int, 256>());
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (g.cols <= 64) return go(std::integral_constant<int, 64>(), One());
+  if (g.cols <= 128) return go(std::integral_constant<int, 128>(), One());
+  const bool tall = MODE == WEIGHT ? g.drows > kTileM : g.rows >= (int64_t)kTileM * g.experts;
+  return tall ? go(std::integral_constant<int, 256>(), Two())
+              : go(std::integral_constant<int, 256>(), One());
 }
 
 }  // namespace
 
 // Few rows an expert: the forward product streams the weights instead (experts_few.cu).
-bool few_rows(const MatmulCall& c) { return c.mode == 0 && c.rows <= 16 * (int64_t)c.experts; }
+static bool few_rows(const MatmulCall& c) { return c.mode == 0 && c.rows <= 16 * (int64_t)c.experts; }
 
 int64_t matmul_workspace(const MatmulCall& c) {
   int64_t n = 0;
@@ -713,18 +938,18 @@ cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st)
     g.cols = c.outer;
     g.reduction = c.inner;
     g.out_pitch = c.outer;
-    return run_tiles<FORWARD>(x, c.inner, c.rows, w, c.inner, c.dtype, g, st);
+    return run_tiles<FORWARD>(x, c.inner, w, c.inner, c.dtype, g, st);
   }
   if (c.mode == 1) {
     g.cols = c.inner;
     g.reduction = c.outer;
     g.out_pitch = c.inner;
-    return run_tiles<INPUT>(dy, c.outer, c.rows, w, c.inner, c.dtype, g, st);
+    return run_tiles<INPUT>(dy, c.outer, w, c.inner, c.dtype, g, st);
   }
   g.cols = c.inner;
   g.drows = c.outer;
   g.out_pitch = c.inner;
-  return run_tiles<WEIGHT>(dy, c.outer, c.rows, x, c.inner, c.dtype, g, st);
+  return run_tiles<WEIGHT>(dy, c.outer, x, c.inner, c.dtype, g, st);
 }
 
 cudaError_t read_matmul_errors(uint32_t* bits) {

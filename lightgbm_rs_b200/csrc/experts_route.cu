@@ -202,11 +202,6 @@ __device__ void select_tokens(const T* logits, int64_t tokens, int experts, int6
   }
 }
 
-__device__ __forceinline__ float warp_max_nan(float v) {
-  float r;
-  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xFFFFFFFF;" : "=f"(r) : "f"(v));
-  return r;
-}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -217,72 +212,123 @@ constexpr int kSelectThreads = 256;
 constexpr int kSelectTokens = 128;  // of a block: 16 a warp, one after the other
 
 // First of three launches for many tokens: choice and weights, and each block's rows per
-// expert. A warp a token: its logits lie in registers, expert e in lane e % 32, and each of
-// the k choices is one maximum over the warp (NaN wins), the first place that holds it, and
-// its removal. The next token's logits are on their way meanwhile.
-template <typename T, int NV>
+// expert. A warp a token, its logits in registers, expert e in lane e % 32; the next token's
+// are on their way meanwhile. Searching all registers once a choice is what would cost most,
+// so the choice has two stages: the k lanes with the largest maxima (ties to the lower
+// expert) hold the k largest logits among them, since each lane left out has k elements
+// before all of its own; their k * NV logits are dealt out to the 32 lanes, CN each, and the
+// k choices are made there, each one a maximum over the warp, the first expert that holds
+// it, and its removal. Keys order as the logits do, with NaN above everything.
+template <typename T, int NV, int CN>
 __global__ void __launch_bounds__(kSelectThreads)
     k_route_select(const T* logits, int64_t tokens, int experts, int64_t pitch, int k,
                    bool normalize, float* weights, int32_t* chosen, int32_t* counts) {
+  constexpr uint32_t kAll = 0xFFFFFFFFu;
+  constexpr int kWarps = kSelectThreads / 32;
+  constexpr bool kTwoStages = CN < NV;
   __shared__ int32_t hist[kMaxExperts + 1];
+  __shared__ float dealt[kTwoStages ? kWarps : 1][kTwoStages ? CN * 32 : 1];
+  __shared__ int32_t dealt_lane[kTwoStages ? kWarps : 1][kMaxChosen];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i <= experts; i += kSelectThreads) hist[i] = 0;
   __syncthreads();
-  constexpr int kPerWarp = kSelectTokens / (kSelectThreads / 32);
+  constexpr int kPerWarp = kSelectTokens / kWarps;
   const int64_t first = (int64_t)blockIdx.x * kSelectTokens + warp * kPerWarp;
   const int64_t last = min(first + kPerWarp, tokens);
   const float kNone = -__int_as_float(0x7F800000);
   float next[NV];
-  auto fetch = [&](int64_t t) {
+  auto fetch = [&](const T* row) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = i * 32 + lane;
-      next[i] = t < last && e < experts ? to_f32<T>(logits[t * pitch + e]) : kNone;
-    }
+    for (int i = 0; i < NV; ++i)
+      next[i] = i * 32 + lane < experts ? to_f32<T>(row[i * 32 + lane]) : kNone;
   };
-  fetch(first);
+  if (first < last) fetch(logits + first * pitch);
   for (int64_t t = first; t < last; ++t) {
     float v[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] = next[i];
-    fetch(t + 1);
+    if (t + 1 < last) fetch(logits + (t + 1) * pitch);
     float top = v[0];
 #pragma unroll
     for (int i = 1; i < NV; ++i) top = max_nan(top, v[i]);
-    const float m = warp_max_nan(top);
-    float total = 0.0f, my_logit = kNone;
+
+    uint32_t key[CN];
+    int id[CN];  // expert of a candidate
+    if constexpr (kTwoStages) {
+      // this lane's first register that holds its maximum (NaN: the first NaN)
+      int at = 0;
+#pragma unroll
+      for (int i = NV - 1; i >= 0; --i)
+        if (v[i] == top) at = i;
+      if (top != top) {
+#pragma unroll
+        for (int i = NV - 1; i >= 0; --i)
+          if (v[i] != v[i]) at = i;
+      }
+      uint32_t lane_key = logit_key(top);
+      for (int c = lane; c < CN * 32; c += 32) dealt[warp][c] = kNone;
+      __syncwarp();
+      for (int j = 0; j < k; ++j) {
+        const uint32_t best = __reduce_max_sync(kAll, lane_key);
+        if (best == kKeyEmpty) break;
+        const int e = (int)__reduce_min_sync(
+            kAll, lane_key == best ? (uint32_t)(at * 32 + lane) : kAll);
+        if (lane == (e & 31)) {
+          lane_key = kKeyEmpty;
+          dealt_lane[warp][j] = lane;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) dealt[warp][j * NV + i] = v[i];
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < CN; ++c) {
+        const int from = c * 32 + lane;
+        const float x = from < k * NV ? dealt[warp][from] : kNone;
+        key[c] = logit_key(x);
+        id[c] = x == kNone ? 0 : (from % NV) * 32 + dealt_lane[warp][from / NV];
+      }
+      __syncwarp();
+    } else {
+#pragma unroll
+      for (int c = 0; c < CN; ++c) {
+        key[c] = logit_key(v[c]);
+        id[c] = c * 32 + lane;
+      }
+    }
+
+    uint32_t my_key = kKeyEmpty;
     int my_id = -1;
+    float m = 0.0f;
+    for (int j = 0; j < k; ++j) {
+      uint32_t mine = key[0];
+#pragma unroll
+      for (int c = 1; c < CN; ++c) mine = max(mine, key[c]);
+      const uint32_t best = __reduce_max_sync(kAll, mine);
+      if (best == kKeyEmpty) break;  // the same in every lane
+      if (j == 0) m = key_logit(best);
+      uint32_t e = kAll;
+#pragma unroll
+      for (int c = 0; c < CN; ++c)
+        if (key[c] == best) e = min(e, (uint32_t)id[c]);
+      e = __reduce_min_sync(kAll, e);
+#pragma unroll
+      for (int c = 0; c < CN; ++c)
+        if ((uint32_t)id[c] == e) key[c] = kKeyEmpty;
+      if (lane == j) {
+        my_key = best;
+        my_id = (int)e;
+      }
+    }
+    const float mine = my_id >= 0 ? expf(key_logit(my_key) - m) : 0.0f;
+    float total = mine;
     if (!normalize) {
+      total = 0.0f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) total += fast_exp(v[i] - m);
     }
-    for (int j = 0; j < k; ++j) {
-      const float best = j == 0 ? m : warp_max_nan(top);
-      if (best == kNone) break;  // the same in every lane
-      // the lowest expert among those that hold it: the first register of each lane, then
-      // the lowest of the lanes
-      int at = NV * 32;
-      const bool nan = best != best;
 #pragma unroll
-      for (int i = NV - 1; i >= 0; --i)
-        if (v[i] == best || (nan && v[i] != v[i])) at = i * 32;
-      const int id = (int)__reduce_min_sync(0xFFFFFFFFu, (uint32_t)(at + lane));
-      const int out = lane == (id & 31) ? id >> 5 : -1;
-      top = kNone;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (i == out) v[i] = kNone;
-        top = max_nan(top, v[i]);
-      }
-      if (lane == j) {
-        my_logit = best;
-        my_id = id;
-      }
-    }
-    const float mine = my_id >= 0 ? expf(my_logit - m) : 0.0f;
-    if (normalize) total = mine;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(kAll, total, d);
     if (lane < k) {
       weights[t * k + lane] = my_id >= 0 ? mine / total : 0.0f;
       chosen[t * k + lane] = my_id;
@@ -448,8 +494,17 @@ cudaError_t route_typed(const T* logits, int64_t tokens, int experts, int64_t pi
   int32_t* totals = ws;
   int32_t* counts = ws + experts + 1;
   auto select = [&](auto nv) {
-    k_route_select<T, decltype(nv)::value><<<blocks, kSelectThreads, 0, st>>>(
-        logits, tokens, experts, pitch, k, normalize, weights, chosen, counts);
+    constexpr int NV = decltype(nv)::value;
+    auto deal = [&](auto cn) {
+      constexpr int CN = decltype(cn)::value < NV ? decltype(cn)::value : NV;
+      k_route_select<T, NV, CN><<<blocks, kSelectThreads, 0, st>>>(
+          logits, tokens, experts, pitch, k, normalize, weights, chosen, counts);
+    };
+    const int most = k * NV;  // candidates of the second stage
+    if (most <= 32) deal(std::integral_constant<int, 1>());
+    else if (most <= 64) deal(std::integral_constant<int, 2>());
+    else if (most <= 128) deal(std::integral_constant<int, 4>());
+    else deal(std::integral_constant<int, 8>());
   };
   if (experts <= 32) select(std::integral_constant<int, 1>());
   else if (experts <= 64) select(std::integral_constant<int, 2>());

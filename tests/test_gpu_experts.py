@@ -230,11 +230,12 @@ def test_products(ops, counts, tail, inner, outer, dtype):
         close(dwf[e], want, counts[e] * 2.0 ** -23 * mag)
 
 
-@pytest.mark.parametrize("inner,outer", [(96, 80), (75, 50)])
-def test_products_through_rows(ops, inner, outer):
+@pytest.mark.parametrize("counts", [[70, 0, 9, 130], [700, 0, 70, 333]])
+@pytest.mark.parametrize("inner,outer", [(96, 80), (75, 50), (264, 392), (130, 300)])
+def test_products_through_rows(ops, inner, outer, counts):
     """Tokens gathered through `rows`: repeated, unused and out of range (a row of zeros)."""
     g = gen(3)
-    counts, tokens = [70, 0, 9, 130], 60
+    tokens = 60
     m = sum(counts)
     x = torch.randn(tokens, inner, generator=g, device="cuda").to(torch.bfloat16)
     w = torch.randn(4, outer, inner, generator=g, device="cuda").to(torch.bfloat16)
@@ -253,22 +254,22 @@ def test_products_through_rows(ops, inner, outer):
               counts[e] * 2.0 ** -23 * (dy[s].double().abs().T @ x64[s].abs()))
 
 
-def test_products_neighbours_do_not_leak(ops):
+@pytest.mark.parametrize("counts,inner,outer", [([37, 50, 41], 96, 72), ([200, 77, 300], 264, 272)])
+def test_products_neighbours_do_not_leak(ops, counts, inner, outer):
     """Infinities and NaN in one expert's rows and weights stay in its results."""
     g = gen(8)
-    counts = [37, 50, 41]
-    m = sum(counts)
-    x = torch.randn(m, 96, generator=g, device="cuda").to(torch.bfloat16)
-    w = torch.randn(3, 72, 96, generator=g, device="cuda").to(torch.bfloat16)
-    dy = torch.randn(m, 72, generator=g, device="cuda").to(torch.bfloat16)
+    m, lo, hi = sum(counts), counts[0], counts[0] + counts[1]
+    x = torch.randn(m, inner, generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.randn(3, outer, inner, generator=g, device="cuda").to(torch.bfloat16)
+    dy = torch.randn(m, outer, generator=g, device="cuda").to(torch.bfloat16)
     off = offsets_of(counts)
     clean = [ops.grouped_matmul(x, w, off), *ops.grouped_matmul_backward(dy, x, w, off)]
-    x[37:87], dy[37:87], w[1] = math.nan, math.inf, math.nan
+    x[lo:hi], dy[lo:hi], w[1] = math.nan, math.inf, math.nan
     dirty = [ops.grouped_matmul(x, w, off), *ops.grouped_matmul_backward(dy, x, w, off)]
     for a, b, groups in zip(clean, dirty, (False, False, True)):
-        for s in ((0, 2) if groups else (slice(0, 37), slice(87, m))):
+        for s in ((0, 2) if groups else (slice(0, lo), slice(hi, m))):
             assert torch.equal(a[s], b[s])
-        assert torch.isnan(b[1] if groups else b[37:87]).all()
+        assert torch.isnan(b[1] if groups else b[lo:hi]).all()
 
 
 def test_products_read_strides_in_place(ops):
