@@ -10,7 +10,7 @@
 // layouts differ. An operand whose reduction axis is contiguous in memory is staged K-major,
 // else MN-major (panels of 64 columns), both with 128-byte swizzle, so nothing is transposed
 // on the way. A persistent grid walks the tiles of all groups; in every CTA one warp issues
-// TMA loads, one the matrix instructions, and four write results out of one half of tensor
+// TMA loads, one the matrix instructions, and eight write results out of one half of tensor
 // memory while the next tile accumulates in the other.
 //
 // Pairs. A 128 x 256 tile of one CTA takes in 48 KB for each 512 cycles of matrix work: the
@@ -28,9 +28,11 @@
 // Ragged ends. FORWARD / INPUT: a tile's rows past its group's end are computed from the next
 // group's rows and not stored (a row of A only reaches its own row of D). Rows past the last
 // group form one more group without a reduction: zeros. WEIGHT: the reduction itself ends
-// inside a block. That block's rows are gathered, and those past the end are asked for
-// outside the tensor, which TMA fills with zeros, in both operands: an infinity or NaN of the
-// next group cannot make 0 * inf.
+// inside a block. Steps of 16 past the end are left out, and in the last step the rows past
+// it are overwritten with zeros in shared memory, in both operands: an infinity or NaN of the
+// next group cannot make 0 * inf. In a pair each CTA's second warp does that to its own half
+// and the odd one tells the even one. (Gathering that block's rows one by one, with zeros
+// from TMA for those outside, took five times a block's time, once a tile.)
 #include <algorithm>
 #include <atomic>
 #include <mutex>
@@ -43,10 +45,12 @@ namespace lgbm_b200 {
 namespace experts {
 namespace {
 
-constexpr int kMatThreads = 192;   // warp 0 loads, warp 1 multiplies, warps 2..5 store
+constexpr int kStoreWarps = 8;     // warps 2..9 write results out
+constexpr int kMatThreads = 64 + 32 * kStoreWarps;  // warp 0 loads, warp 1 multiplies
 constexpr int kTileM = 128;       // rows of D of a CTA
 constexpr int kTileK = 64;         // 128 bytes of a 16-bit type: one swizzle row
-constexpr int kStoreBytes = 4 * 32 * 128;  // one 32 x 128 B staging block a storing warp
+constexpr int kStoreRow = 64;      // bytes of a row in a storing warp's staging block
+constexpr int kStoreBytes = kStoreWarps * 32 * kStoreRow;
 constexpr int kBandRows = 2048;    // rows of D of a band, see tile_of
 constexpr uint64_t kWaitNs = 2000000000;
 
@@ -162,24 +166,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
-// Four rows of 64 elements to 512 consecutive bytes (swizzled by address, as a tile is); a
-// row outside the tensor reads as zeros.
-template <int CTAS>
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x,
-                                            const int (&row)[4], uint32_t bar) {
-  if constexpr (CTAS == 2)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4"
-        ".mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
-        : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4"
-        ".mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
-        : "memory");
-}
 template <int CTAS>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                         bool accumulate) {
@@ -210,7 +196,16 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
         "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
         : "memory");
 }
-// 32 lanes x 32 columns of f32 of this warp's quarter of tensor memory.
+// 32 lanes x 16 columns of f32 of this warp's quarter of tensor memory, and 32 columns.
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15])
+      : "r"(addr));
+}
 __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -282,56 +277,60 @@ struct Shape {
   static constexpr int kTmemCols = 2 * BN;              // two accumulators
   static constexpr int kBand = kBandRows / kRows;
   static constexpr int kSmem =
-      1024 + kStages * kStageBytes + kStoreBytes + 8 * (kMaxExperts + 2) + 256;
+      1024 + kStages * kStageBytes + kStoreBytes + 8 * (kMaxExperts + 2) + 512;
 };
+
+// Where piece `p` (16 bytes) of row `row` lies in a staging block: the 64-byte swizzle of TMA.
+__device__ __forceinline__ uint32_t staged(int row, int p) {
+  return row * kStoreRow + ((p ^ ((row >> 1) & 3)) << 4);
+}
 
 // One 32-row block of a storing warp, from its staging block to `dst` (row pitch in bytes),
 // `bytes` of each row, UNIT bytes at a time.
 template <int UNIT>
 __device__ __forceinline__ void store_rows(uint32_t stage, char* dst, int64_t pitch, int nrows,
                                            int bytes, int lane) {
-  constexpr int kLanes = 128 / UNIT < 32 ? 128 / UNIT : 32;  // of a row
-  constexpr int kPerStep = 32 / kLanes;                      // rows
-#pragma unroll 4
+  constexpr int kLanes = kStoreRow / UNIT;  // of a row
+  constexpr int kPerStep = 32 / kLanes;     // rows
+  const int at = lane % kLanes * UNIT;
+  if (at + UNIT > bytes) return;
+  char* to = dst + (lane / kLanes) * pitch + at;
+#pragma unroll 8
   for (int i0 = 0; i0 < 32; i0 += kPerStep) {
     const int i = i0 + lane / kLanes;
-#pragma unroll
-    for (int at = lane % kLanes * UNIT; at < 128; at += kLanes * UNIT) {
-      const uint32_t from = stage + i * 128 + (((at >> 4) ^ (i & 7)) << 4) + (at & 15);
-      char* to = dst + i * pitch + at;
-      if (i < nrows && at + UNIT <= bytes) {
-        if constexpr (UNIT == 16) {
-          uint32_t w[4];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(from)
-                       : "memory");
-          *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else if constexpr (UNIT == 8) {
-          uint32_t w[2];
-          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
-                       : "=r"(w[0]), "=r"(w[1])
-                       : "r"(from)
-                       : "memory");
-          *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-        } else if constexpr (UNIT == 4) {
-          uint32_t w;
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
-          *reinterpret_cast<uint32_t*>(to) = w;
-        } else {
-          uint16_t w;
-          asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(from) : "memory");
-          *reinterpret_cast<uint16_t*>(to) = w;
-        }
+    if (i < nrows) {
+      const uint32_t from = stage + staged(i, at >> 4) + (at & 15);
+      if constexpr (UNIT == 16) {
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(from)
+                     : "memory");
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else if constexpr (UNIT == 8) {
+        uint32_t w[2];
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                     : "=r"(w[0]), "=r"(w[1])
+                     : "r"(from)
+                     : "memory");
+        *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+      } else if constexpr (UNIT == 4) {
+        uint32_t w;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
+        *reinterpret_cast<uint32_t*>(to) = w;
+      } else {
+        uint16_t w;
+        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(from) : "memory");
+        *reinterpret_cast<uint16_t*>(to) = w;
       }
     }
+    to += kPerStep * pitch;
   }
 }
 
 struct Maps {
-  CUtensorMap a, b;              // tiles of 64 columns
-  CUtensorMap a_rows, b_rows;    // single rows of 64 columns, for gathers
-  CUtensorMap out;               // 32 rows of 128 bytes
+  CUtensorMap a, b;  // tiles of 64 columns
+  CUtensorMap out;   // 32 rows of 64 bytes
 };
 
 template <int MODE, int BN, int CTAS>
@@ -349,9 +348,12 @@ __global__ void __launch_bounds__(kMatThreads, 1)
   int32_t* off = cum + kMaxExperts + 2;  // the groups' first rows, then the end
   uint64_t* bars = reinterpret_cast<uint64_t*>(
       (reinterpret_cast<uintptr_t>(off + kMaxExperts + 2) + 15) & ~(uintptr_t)15);
+  // end_full, end_peer (WEIGHT): a group's last block has landed in this CTA; the odd CTA has
+  // zeroed its rows past the end. Used in turn, one a last block.
   const uint32_t full = smem_addr(bars), empty = full + 8 * kStages,
-                 acc_full = empty + 8 * kStages, acc_empty = acc_full + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
+                 acc_full = empty + 8 * kStages, acc_empty = acc_full + 16,
+                 end_full = acc_empty + 16, end_peer = end_full + 8 * kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * kStages + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CTAS == 2 ? blockIdx.x & 1 : 0;  // in the pair; the even CTA multiplies
 
@@ -360,10 +362,12 @@ __global__ void __launch_bounds__(kMatThreads, 1)
       for (int i = 0; i < kStages; ++i) {
         bar_init(full + 8 * i, 1);
         bar_init(empty + 8 * i, 1);
+        bar_init(end_full + 8 * i, 1);
+        bar_init(end_peer + 8 * i, 1);
       }
       for (int i = 0; i < 2; ++i) {
         bar_init(acc_full + 8 * i, 1);
-        bar_init(acc_empty + 8 * i, 4 * CTAS);
+        bar_init(acc_empty + 8 * i, kStoreWarps * CTAS);
       }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
@@ -459,7 +463,7 @@ __global__ void __launch_bounds__(kMatThreads, 1)
 
   bool ok = true;
   if (warp == 0) {
-    uint32_t it = 0;
+    uint32_t it = 0, ends = 0;
     for (int t = first; ok && t < tiles; t += step) {
       const Tile r = decode(t);
       const int nb = r.n0 + rank * S::kCols;  // first column of this CTA's share of B
@@ -467,26 +471,17 @@ __global__ void __launch_bounds__(kMatThreads, 1)
         const uint32_t s = it % kStages;
         if (it >= kStages && !(ok = bar_wait(empty + 8 * s, (it / kStages - 1) & 1))) break;
         const uint32_t a = base + s * S::kStageBytes, b = a + kABytes;
-        const uint32_t bar = CTAS == 2 ? leader_addr(full + 8 * s) : full + 8 * s;
-        if (rank == 0 && elect_one()) bar_expect(full + 8 * s, CTAS * S::kStageBytes);
-        __syncwarp();
-        if (MODE == WEIGHT && r.red - k0 < kTileK) {
-          // the group's end: rows one by one, lanes 0..15 and 16..31 a panel each, and the
-          // first row outside the tensor for those past the end
-          int row[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int at = 4 * (lane & 15) + j;
-            row[j] = at < r.red - k0 ? r.red0 + k0 + at : (int)g.rows;
+        uint32_t bar = CTAS == 2 ? leader_addr(full + 8 * s) : full + 8 * s;
+        const bool end = MODE == WEIGHT && r.red - k0 < kTileK;
+        if (elect_one()) {
+          if (end) {
+            // lands at this CTA's own barrier; the stage's turns over without bytes
+            bar = end_full + 8 * (ends % kStages);
+            bar_expect(bar, S::kStageBytes);
+            if (rank == 0) bar_expect(full + 8 * s, 0);
+          } else if (rank == 0) {
+            bar_expect(full + 8 * s, CTAS * S::kStageBytes);
           }
-          tma_gather4<CTAS>(a + (lane >> 4) * 8192 + (lane & 15) * 512, &maps.a_rows,
-                            r.m0 + 64 * (lane >> 4), row, bar);
-#pragma unroll
-          for (int j = 0; j < S::kCols / 64; j += 2)
-            if (j + (lane >> 4) < S::kCols / 64)
-              tma_gather4<CTAS>(b + (j + (lane >> 4)) * 8192 + (lane & 15) * 512, &maps.b_rows,
-                                nb + 64 * (j + (lane >> 4)), row, bar);
-        } else if (elect_one()) {
           if (MODE == WEIGHT) {
 #pragma unroll
             for (int j = 0; j < kTileM / 64; ++j)
@@ -506,29 +501,53 @@ __global__ void __launch_bounds__(kMatThreads, 1)
           }
         }
         __syncwarp();
+        if (end) ++ends;
       }
     }
-    // no copy may be in flight when the CTA ends: a load whose block nobody multiplied
-    // (another warp gave up) has landed, two seconds later, before the CTAs leave; the
-    // first CTA, whose barrier counts the loads of both, looks
-    if (!ok && rank == 0)
-      for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
+    // no copy may be in flight when the CTA ends: one whose block nobody multiplied (another
+    // warp gave up, two seconds ago) has landed when these waits return or run out
+    if (!ok) {
+      for (uint32_t i = it > kStages ? it - kStages : 0; rank == 0 && i < it; ++i)
         bar_wait(full + 8 * (i % kStages), (i / kStages) & 1);
+      if (ends > 0) bar_wait(end_full + 8 * ((ends - 1) % kStages), ((ends - 1) / kStages) & 1);
+    }
   } else if (warp == 1) {
-    uint32_t it = 0, tile = 0;
-    for (int t = first; rank == 0 && ok && t < tiles; t += step) {
+    uint32_t it = 0, tile = 0, ends = 0;
+    for (int t = first; ok && t < tiles; t += step) {
       const Tile r = decode(t);
       if (r.red == 0) continue;
       const uint32_t acc = tile & 1, d = tmem + acc * BN;
-      if (tile >= 2 && !(ok = bar_wait(acc_empty + 8 * acc, (tile / 2 - 1) & 1))) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (rank == 0) {
+        if (tile >= 2 && !(ok = bar_wait(acc_empty + 8 * acc, (tile / 2 - 1) & 1))) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
       for (int k0 = 0; k0 < r.red; k0 += kTileK, ++it) {
         const uint32_t s = it % kStages;
+        const uint32_t a = base + s * S::kStageBytes, b = a + kABytes;
+        // the last block in whole steps of 16
+        const int valid = min(r.red - k0, kTileK), steps = (valid + 15) / 16;
+        const bool end = MODE == WEIGHT && valid < kTileK;
+        if (end) {
+          const uint32_t slot = 8 * (ends % kStages), parity = (ends / kStages) & 1;
+          ++ends;
+          if (!(ok = bar_wait(end_full + slot, parity))) break;
+          const int rest = steps * 16 - valid;
+          constexpr int kPanels = (kTileM + S::kCols) / 64;
+          for (int i = lane; i < rest * kPanels * 8; i += 32) {
+            const int panel = i / (rest * 8), row = i / 8 % rest;
+            store_piece(a + panel * 8192 + (valid + row) * 128 + (i & 7) * 16, 0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (rank == 1) {
+            if (lane == 0) bar_arrive_cluster(leader_addr(end_peer + slot));
+          } else if (CTAS == 2 && !(ok = bar_wait(end_peer + slot, parity))) {
+            break;
+          }
+        }
+        if (rank == 1) continue;  // the even CTA multiplies for both
         if (!(ok = bar_wait(full + 8 * s, (it / kStages) & 1))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t a = base + s * S::kStageBytes, b = a + kABytes;
-        // the last block in whole steps of 16: what lies past the end in them is zeros
-        const int steps = (min(r.red - k0, kTileK) + 15) / 16;
         if (elect_one()) {
           for (int k = 0; k < steps; ++k) {
             // 16 of the reduction: 32 bytes along a K-major row, 16 rows of an MN-major panel
@@ -543,18 +562,17 @@ __global__ void __launch_bounds__(kMatThreads, 1)
         __syncwarp();
       }
       if (!ok) break;
-      if (elect_one()) mma_commit<CTAS>(acc_full + 8 * acc);
+      if (rank == 0 && elect_one()) mma_commit<CTAS>(acc_full + 8 * acc);
       __syncwarp();
       ++tile;
     }
   } else {
-    const int quarter = warp & 3;
-    const uint32_t stage = store_base + (warp - 2) * 4096;
+    const int quarter = warp & 3, half = (warp - 2) >> 2;  // of the lanes; of the chunks
+    const uint32_t stage = store_base + (warp - 2) * 32 * kStoreRow;
     const bool wide = g.out_kind == LGBM_B200_DTYPE_F32;
     const int bytes = wide ? 4 : 2;
-    const int per_chunk = 128 / bytes;  // columns of a 128-byte staging row
+    const int per_chunk = kStoreRow / bytes;  // columns of a staging row
     const int64_t pitch = g.out_pitch * bytes;
-    const uint32_t row_at = stage + lane * 128, swizzle = lane & 7;
     uint32_t tile = 0;
     for (int t = first; ok && t < tiles; t += step) {
       const Tile r = decode(t);
@@ -574,40 +592,33 @@ __global__ void __launch_bounds__(kMatThreads, 1)
       const int ncols = min(BN, g.cols - r.n0), nrows = min(32, r.m_end - row0);
       // whole 32-row blocks leave by TMA, which also cuts off the last columns
       const bool by_tma = g.unit == 16 && nrows == 32;
-      for (int c0 = 0; c0 < ncols && nrows > 0; c0 += per_chunk) {
+      for (int c0 = half * per_chunk; c0 < ncols && nrows > 0; c0 += 2 * per_chunk) {
         // this lane's row of the chunk
-        uint32_t v[64];
+        uint32_t v[32], w[16];
+        if (r.red == 0) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) v[i] = 0;
-        if (r.red > 0) {
-          tmem_load32(from + c0, reinterpret_cast<uint32_t(&)[32]>(v[0]));
-          if (!wide) tmem_load32(from + c0 + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
+          for (int i = 0; i < 16; ++i) w[i] = 0;
+        } else if (wide) {
+          tmem_load16(from + c0, w);
           tmem_wait();
+        } else {
+          tmem_load32(from + c0, v);
+          tmem_wait();
+          if (g.out_kind == LGBM_B200_DTYPE_BF16) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = pack2<true>(v[2 * i], v[2 * i + 1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = pack2<false>(v[2 * i], v[2 * i + 1]);
+          }
         }
         // the staging block is free when the last store has read it
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
-        // 16-byte pieces, swizzled by row
-        if (wide) {
 #pragma unroll
-          for (int p = 0; p < 8; ++p)
-            store_piece(row_at + ((p ^ swizzle) << 4), v[4 * p], v[4 * p + 1], v[4 * p + 2],
-                        v[4 * p + 3]);
-        } else if (g.out_kind == LGBM_B200_DTYPE_BF16) {
-#pragma unroll
-          for (int p = 0; p < 8; ++p)
-            store_piece(row_at + ((p ^ swizzle) << 4), pack2<true>(v[8 * p], v[8 * p + 1]),
-                        pack2<true>(v[8 * p + 2], v[8 * p + 3]),
-                        pack2<true>(v[8 * p + 4], v[8 * p + 5]),
-                        pack2<true>(v[8 * p + 6], v[8 * p + 7]));
-        } else {
-#pragma unroll
-          for (int p = 0; p < 8; ++p)
-            store_piece(row_at + ((p ^ swizzle) << 4), pack2<false>(v[8 * p], v[8 * p + 1]),
-                        pack2<false>(v[8 * p + 2], v[8 * p + 3]),
-                        pack2<false>(v[8 * p + 4], v[8 * p + 5]),
-                        pack2<false>(v[8 * p + 6], v[8 * p + 7]));
-        }
+        for (int p = 0; p < 4; ++p)
+          store_piece(stage + staged(lane, p), w[4 * p], w[4 * p + 1], w[4 * p + 2],
+                      w[4 * p + 3]);
         if (by_tma) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
@@ -719,13 +730,13 @@ EncodeTiled encoder() {
   return fn;
 }
 
-// A tensor, innermost axis first; boxes of 128 bytes x `box1` rows (one row for gathers),
-// 128-byte swizzle, zeros outside the tensor.
+// A tensor, innermost axis first; boxes of `row` bytes (64 or 128, swizzled alike) x `box1`
+// rows, zeros outside the tensor.
 bool encode(CUtensorMap* map, int32_t dtype, const void* base, int rank, const int64_t* dims,
-            const int64_t* pitches, int box1) {
+            const int64_t* pitches, int box1, int row = 128) {
   const int bytes = elem_size(dtype);
   cuuint64_t d[3], s[2];
-  cuuint32_t box[3] = {(cuuint32_t)(128 / bytes), (cuuint32_t)box1, 1}, step[3] = {1, 1, 1};
+  cuuint32_t box[3] = {(cuuint32_t)(row / bytes), (cuuint32_t)box1, 1}, step[3] = {1, 1, 1};
   for (int i = 0; i < rank; ++i) d[i] = (cuuint64_t)dims[i];
   for (int i = 0; i + 1 < rank; ++i) s[i] = (cuuint64_t)pitches[i] * bytes;
   const EncodeTiled fn = encoder();
@@ -734,7 +745,8 @@ bool encode(CUtensorMap* map, int32_t dtype, const void* base, int rank, const i
                   : dtype == LGBM_B200_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                   (cuuint32_t)rank, const_cast<void*>(base), d, s, box, step,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -849,13 +861,9 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
     Maps maps;
     const int64_t da[3] = {a_width, g.rows, 1}, pa[2] = {a.pitch, 0};
     bool fine = encode(&maps.a, dtype, a.p, 2, da, pa, MODE == WEIGHT ? 64 : kTileM);
-    if (MODE == WEIGHT) fine = fine && encode(&maps.a_rows, dtype, a.p, 2, da, pa, 1);
-    else maps.a_rows = maps.a;
-    maps.b_rows = maps.a;  // not used unless set below
     if (MODE == WEIGHT) {
       const int64_t db[3] = {b_width, g.rows, 1}, pb[2] = {b.pitch, 0};
-      fine = fine && encode(&maps.b, dtype, b.p, 2, db, pb, 64) &&
-             encode(&maps.b_rows, dtype, b.p, 2, db, pb, 1);
+      fine = fine && encode(&maps.b, dtype, b.p, 2, db, pb, 64);
     } else {
       const int64_t n = MODE == FORWARD ? g.cols : g.reduction;
       const int64_t db[3] = {b_width, n, g.experts}, pb[2] = {b.pitch, b.pitch * n};
@@ -866,7 +874,7 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
     if (g.unit == 16 && rows_d > INT32_MAX) g.unit = 8;  // no coordinate for its last rows
     if (g.unit == 16) {
       const int64_t dd[3] = {g.cols, rows_d, 1}, pd[2] = {g.out_pitch, 0};
-      fine = fine && encode(&maps.out, g.out_kind, g.out, 2, dd, pd, 32);
+      fine = fine && encode(&maps.out, g.out_kind, g.out, 2, dd, pd, 32, kStoreRow);
     }
     if (!fine) return cudaErrorInvalidValue;
     g.idesc = instruction(dtype, MODE == WEIGHT, MODE != FORWARD, S::kRows, BN);
