@@ -143,30 +143,33 @@ struct FewShape {
   using T = T_;
   static constexpr int TILES = TILES_, SHIFT = SHIFT_, ALIGN = ALIGN_;
   static constexpr bool W4 = SHIFT > 0, ZEROS = ZEROS_;
+  // Blocks that share an SM, and stages of a warp's ring: with 4 bits the arithmetic wants
+  // warps, with 16 bits the memory wants bytes in flight (4 x 16 KB a block).
+  static constexpr int kBlocks = W4 && TILES == 1 ? 3 : 2;
+  static constexpr int kRing = !W4 && TILES == 1 ? 5 : 3;
+  static constexpr int kMaxPanel = 512;
   static constexpr int kRows = 8 * TILES;
-  // sized so that two blocks share an SM
-  static constexpr int kMaxPanel = TILES == 1 ? 1024 : 512;
-  static constexpr int kRing = TILES == 1 ? 4 : 3;  // stages a warp
   static constexpr int kStageInner = W4 ? 2 * kRowBytes : kRowBytes / 2;
+  // Scales (and zero points) of a warp's 16 outputs in a stage: two sets, one in use. An
+  // output's are an odd number of words apart, so 8 outputs hit 8 banks.
+  static constexpr int kGroups = W4 ? kStageInner >> SHIFT : 0;
+  static constexpr int kScalePitch = kGroups + 2;
+  static constexpr int kScaleBytes = W4 ? 16 * kScalePitch * 2 : 0;
+  static constexpr int kScaleLane = W4 ? (16 * kGroups + 31) / 32 : 1;  // a lane's share
   // bytes of a staged token: the fragment loads of 8 tokens hit different banks
   static __host__ __device__ int token_pitch(int panel) { return panel * 2 + (W4 ? 64 : 16); }
-  // 16-bit scales (and zero points) of an output: an odd number of words, 8 rows hit 8 banks
-  static __host__ __device__ int scale_pitch(int panel) { return (panel >> SHIFT) + 2; }
   static __host__ __device__ int tokens(int panel) {
     const int need = kRows * token_pitch(panel), sums = kRows * kOutBlock * 4;
     return need > sums ? need : sums;  // the partial sums lie over the tokens
   }
-  static __host__ __device__ int scales(int panel) {
-    return W4 ? (kOutBlock * scale_pitch(panel) * 2 + 15) / 16 * 16 : 0;
-  }
   static __host__ __device__ int ring(int panel) {
-    return tokens(panel) + (ZEROS ? 2 : 1) * scales(panel);
+    return tokens(panel) + kFewWarps * 2 * (ZEROS ? 2 : 1) * kScaleBytes;
   }
   static __host__ int total(int panel) { return ring(panel) + kFewWarps * kRing * kStageBytes; }
 };
 
 template <typename S>
-__global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g) {
+__global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const FewArgs g) {
   using T = typename S::T;
   constexpr int TILES = S::TILES, SHIFT = S::SHIFT;
   constexpr bool W4 = S::W4;
@@ -174,10 +177,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int32_t item[3];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tpitch = S::token_pitch(g.panel), spitch = S::scale_pitch(g.panel);
+  const int tpitch = S::token_pitch(g.panel);
   uint8_t* tokens = smem;
-  T* scales = reinterpret_cast<T*>(smem + S::tokens(g.panel));
-  uint16_t* zeros = reinterpret_cast<uint16_t*>(smem + S::tokens(g.panel) + S::scales(g.panel));
+  uint8_t* scale_sets =
+      smem + S::tokens(g.panel) + warp * 2 * (S::ZEROS ? 2 : 1) * S::kScaleBytes;
   uint8_t* ring = smem + S::ring(g.panel) + warp * kRing * kStageBytes;
   const int gq = lane >> 2, tq = lane & 3;  // row and column quad of the matrix fragments
 
@@ -241,23 +244,123 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
   const char* src0 = wbase + (int64_t)(lane >> 3) * g.w_pitch + byte0 + (lane & 7) * 16;
   const uint32_t dst0 = shared_addr(ring) + (lane >> 3) * kRowPitch + (lane & 7) * 16;
   const int rest0 = row_bytes - byte0 - (lane & 7) * 16, rows_in = g.outer - my_row0 - (lane >> 3);
+  const int64_t step4 = 4 * g.w_pitch;
   int load_slot = 0;
   auto load_stage = [&](int i) {
     if (i < stages) {
-      const int rest = min(max(rest0 - i * kRowBytes, 0), 16);
       const char* src = src0 + i * kRowBytes;
       const uint32_t dst = dst0 + load_slot * kStageBytes;
+      const int rest = rest0 - i * kRowBytes;
+      if (S::ALIGN == 16 && my_row0 + 16 <= g.outer &&
+          byte0 + (i + 1) * kRowBytes <= row_bytes) {  // all of it exists
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int valid = 4 * j < rows_in ? rest : 0;
-        copy16<S::ALIGN>(dst + 4 * j * kRowPitch,
-                         valid ? src + (int64_t)(4 * j) * g.w_pitch
-                               : static_cast<const char*>(g.w),
-                         valid);
+        for (int j = 0; j < 4; ++j)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 4 * j * kRowPitch),
+                       "l"(src + j * step4)
+                       : "memory");
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int valid = 4 * j < rows_in ? min(max(rest, 0), 16) : 0;
+          copy16<S::ALIGN>(dst + 4 * j * kRowPitch,
+                           valid ? src + j * step4 : static_cast<const char*>(g.w), valid);
+        }
       }
     }
     load_slot = load_slot + 1 == kRing ? 0 : load_slot + 1;
     asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  // Scales of stage i into registers, and from there into set i % 2: the loads of a stage are
+  // in flight while the stage before it is multiplied.
+  // (As words, loaded under a branch: a half-register result, or a select behind the load,
+  // would wait for it.)
+  uint32_t next_scale[S::kScaleLane], next_zero[S::kScaleLane];
+  const uint16_t* scale0 = static_cast<const uint16_t*>(g.scales) +
+                           ((int64_t)expert * g.outer + my_row0) * g.groups + (k_begin >> SHIFT);
+  const uint8_t* zero0 = g.zeros + ((int64_t)expert * g.outer + my_row0) * g.groups +
+                         (k_begin >> SHIFT);
+  auto fetch_scales = [&](int i) {
+    if constexpr (W4) {
+#pragma unroll
+      for (int j = 0; j < S::kScaleLane; ++j) {
+        const int p = lane + 32 * j, r = p / S::kGroups, c = i * S::kGroups + p % S::kGroups;
+        next_scale[j] = 0;
+        next_zero[j] = 8;
+        if (r < 16 && my_row0 + r < g.outer && (k_begin >> SHIFT) + c < g.groups && i < stages) {
+          asm volatile("ld.global.nc.u16 %0, [%1];"
+                       : "=r"(next_scale[j])
+                       : "l"(scale0 + r * g.groups + c));
+          if constexpr (S::ZEROS)
+            asm volatile("ld.global.nc.u8 %0, [%1];"
+                         : "=r"(next_zero[j])
+                         : "l"(zero0 + r * g.groups + c));
+        }
+      }
+    }
+  };
+  auto keep_scales = [&](int i) {
+    if constexpr (W4) {
+      uint16_t* set = reinterpret_cast<uint16_t*>(scale_sets + (i & 1) * S::kScaleBytes);
+      uint16_t* zset = reinterpret_cast<uint16_t*>(scale_sets + (2 + (i & 1)) * S::kScaleBytes);
+#pragma unroll
+      for (int j = 0; j < S::kScaleLane; ++j) {
+        const int p = lane + 32 * j, at = p / S::kGroups * S::kScalePitch + p % S::kGroups;
+        if (p < 16 * S::kGroups) {
+          set[at] = (uint16_t)next_scale[j];
+          if constexpr (S::ZEROS) zset[at] = (uint16_t)(Magic<T>::kBits + (next_zero[j] & 15));
+        }
+      }
+    }
+  };
+
+  // Tokens of a panel: warp w brings rows w, w + 8, ..; 16-byte pieces lane, lane + 32. Held
+  // in registers until the panel before is done with.
+  constexpr int kPieces = S::kMaxPanel / 8 / 32;
+  uint4 next_tokens[TILES][kPieces];
+  const uint16_t* token_row[TILES];
+#pragma unroll
+  for (int q = 0; q < TILES; ++q) {
+    const int r = warp + 8 * q;
+    int64_t at = -1;
+    if (r < nrows) at = g.index ? g.index[begin + r] : begin + r;
+    token_row[q] = at >= 0 && at < g.x_rows
+                       ? static_cast<const uint16_t*>(g.x) + at * g.x_pitch
+                       : nullptr;
+  }
+  auto fetch_tokens = [&](int k0) {
+#pragma unroll
+    for (int q = 0; q < TILES; ++q)
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        const int k = k0 + (lane + 32 * p) * 8;
+        next_tokens[q][p] = make_uint4(0, 0, 0, 0);
+        if (token_row[q] && k < k_end && (lane + 32 * p) * 8 < g.panel) {
+          if (g.x_vec && k + 8 <= k_end) {
+            next_tokens[q][p] = __ldg(reinterpret_cast<const uint4*>(token_row[q] + k));
+          } else {
+            uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (k + j < k_end) v[j / 2] |= (uint32_t)token_row[q][k + j] << (16 * (j & 1));
+            next_tokens[q][p] = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+  };
+  auto keep_tokens = [&] {
+#pragma unroll
+    for (int q = 0; q < TILES; ++q)
+      if (q < tiles)
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+          uint4 v = next_tokens[q][p];
+          if (W4)  // pairs (0, 4), (1, 5), (2, 6), (3, 7)
+            v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                           __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+          if ((lane + 32 * p) * 8 < g.panel)
+            *reinterpret_cast<uint4*>(tokens + (warp + 8 * q) * tpitch + (lane + 32 * p) * 16) = v;
+        }
   };
 
   float acc[TILES][4];
@@ -268,62 +371,22 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
 
 #pragma unroll
   for (int i = 0; i < kRing - 1; ++i) load_stage(i);
+  fetch_scales(0);
+  fetch_tokens(k_begin);
+  keep_scales(0);
 
-  const uint16_t* x = static_cast<const uint16_t*>(g.x);
   int kp = g.panel;  // inner position in the panel
   int slot = 0;      // stage of the ring to multiply next
   for (int i = 0; i < stages; ++i, kp += S::kStageInner) {
     if (kp == g.panel) {
       kp = 0;
-      const int k0 = k_begin + i * S::kStageInner;
       if (i > 0) __syncthreads();
-      // tokens of this panel, 8 inner elements a thread; zeros past the rows and the slice
-      const int vecs = g.panel / 8;
-      for (int r = warp; r < 8 * tiles; r += kFewWarps) {
-        int64_t at = -1;
-        if (r < nrows) at = g.index ? g.index[begin + r] : begin + r;
-        const bool inside = at >= 0 && at < g.x_rows;
-        const uint16_t* src = x + (inside ? at : 0) * g.x_pitch;
-        for (int c = lane; c < vecs; c += 32) {
-          const int k = k0 + c * 8;
-          uint32_t v[4] = {0, 0, 0, 0};
-          if (inside && k < k_end) {
-            if (g.x_vec && k + 8 <= k_end) {
-              const uint4 q = __ldg(reinterpret_cast<const uint4*>(src + k));
-              v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
-            } else {
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (k + j < k_end) v[j / 2] |= (uint32_t)src[k + j] << (16 * (j & 1));
-            }
-          }
-          if (W4) {  // pairs (0, 4), (1, 5), (2, 6), (3, 7)
-            const uint32_t p0 = __byte_perm(v[0], v[2], 0x5410),
-                           p1 = __byte_perm(v[0], v[2], 0x7632),
-                           p2 = __byte_perm(v[1], v[3], 0x5410),
-                           p3 = __byte_perm(v[1], v[3], 0x7632);
-            v[0] = p0, v[1] = p1, v[2] = p2, v[3] = p3;
-          }
-          *reinterpret_cast<uint4*>(tokens + r * tpitch + c * 16) =
-              make_uint4(v[0], v[1], v[2], v[3]);
-        }
-      }
-      if constexpr (W4) {
-        const int bits = 31 - __clz(g.panel >> SHIFT);
-        const int first = k0 >> SHIFT;
-        for (int p = threadIdx.x; p < kOutBlock << bits; p += kFewThreads) {
-          const int r = p >> bits, c = p & ((1 << bits) - 1);
-          const bool in = out0 + r < g.outer && first + c < g.groups;
-          const int64_t at = ((int64_t)expert * g.outer + out0 + r) * g.groups + first + c;
-          scales[r * spitch + c] =
-              in ? static_cast<const T*>(g.scales)[at] : from_f32<T>(0.0f);
-          if constexpr (S::ZEROS)
-            zeros[r * spitch + c] = (uint16_t)(Magic<T>::kBits + (in ? g.zeros[at] & 15 : 8));
-        }
-      }
+      keep_tokens();
       __syncthreads();
+      fetch_tokens(k_begin + i * S::kStageInner + g.panel);
     }
     load_stage(i + kRing - 1);
+    fetch_scales(i + 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
     __syncwarp();
     const uint8_t* st = ring + slot * kStageBytes;
@@ -331,11 +394,14 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
     if constexpr (W4) {
       const uint8_t* a_at = st + gq * kRowPitch + tq * 4;
       const uint8_t* b_at = tokens + gq * tpitch + (kp + tq * 8) * 2;
-      const int lo0 = (warp * 16 + gq) * spitch + (kp >> SHIFT);
+      const T* scales =
+          reinterpret_cast<const T*>(scale_sets + (i & 1) * S::kScaleBytes);
+      const uint16_t* zeros =
+          reinterpret_cast<const uint16_t*>(scale_sets + (2 + (i & 1)) * S::kScaleBytes);
       constexpr int kSteps = (1 << SHIFT) / 32;  // of 32 in a scale group
-#pragma unroll(TILES == 1 ? 8 : 1)
+#pragma unroll(TILES == 1 ? 2 : 1)
       for (int j0 = 0; j0 < S::kStageInner / 32; j0 += kSteps) {
-        const int lo = lo0 + j0 / kSteps, hi = lo + 8 * spitch;
+        const int lo = gq * S::kScalePitch + j0 / kSteps, hi = lo + 8 * S::kScalePitch;
         uint32_t zl = (Magic<T>::kBits + 8) * 0x10001u, zh = zl;
         if constexpr (S::ZEROS) {
           zl = zeros[lo] * 0x10001u;
@@ -395,6 +461,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_grouped_few(const FewArgs g)
         }
       }
     }
+    keep_scales(i + 1);
     __syncwarp();
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
