@@ -1,4 +1,5 @@
-"""Build the in-tree shared library lightgbm_rs_b200/liblgbm_b200.so for sm_100a.
+"""Build the in-tree shared library lightgbm_rs_b200/liblgbm_b200.so for sm_100a, and the
+Python module lightgbm_rs_b200/_experts.so that hands torch tensors to it.
 
 Incremental: objects under lightgbm_rs_b200/_build/ are rebuilt when a source or
 header is newer. Usage: python -m lightgbm_rs_b200.build [--force]
@@ -17,6 +18,8 @@ CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "liblgbm_b200.so")
+BINDING_SRC = os.path.join(CSRC, "experts_torch.cpp")
+BINDING = os.path.join(PKG, "_experts.so")
 NVCC = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
 HOST_CXX = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else (shutil.which("g++") or "g++")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -53,6 +56,7 @@ def _compile(src, obj, extra=()):
 def build(force=False, verbose=False, ptxas_info=False):
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cpp")))
+    srcs.remove(BINDING_SRC)
     deps = _headers()
     jobs = []
     objs = []
@@ -79,6 +83,36 @@ def build(force=False, verbose=False, ptxas_info=False):
     return LIB
 
 
+def build_binding(force=False):
+    """The torch binding, against the installed torch's headers; it finds the library beside
+    itself and torch's own libraries already loaded."""
+    build()
+    obj = os.path.join(BUILD, "experts_torch.cpp.o")
+    header = os.path.join(INCLUDE, "lgbm_b200.h")
+    if not force and not _stale(obj, BINDING_SRC, [header]) and os.path.exists(BINDING) and \
+            os.path.getmtime(BINDING) >= os.path.getmtime(obj):
+        return BINDING
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ext
+
+    includes = ext.include_paths("cuda") + [sysconfig.get_paths()["include"]]
+    _compile(BINDING_SRC, obj, [f"-isystem{p}" for p in includes] + [
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"])
+    tmp = BINDING + ".tmp"
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [HOST_CXX, "-shared", "-o", tmp, obj, f"-L{PKG}", "-l:liblgbm_b200.so",
+           "-Wl,-rpath,$ORIGIN", f"-L{libs}"] + [
+        f"-l{n}" for n in ("c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch", "torch_python")]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 if __name__ == "__main__":
     lib = build(force="--force" in sys.argv, verbose=True, ptxas_info="--ptxas" in sys.argv)
     print(lib)
+    print(build_binding(force="--force" in sys.argv))
