@@ -62,6 +62,17 @@ struct Raw {
   __device__ __forceinline__ void load(const T* p) {
     bits = __ldg(reinterpret_cast<const uint4*>(p));
   }
+  // The first n of V elements; the others are whatever.
+  __device__ __forceinline__ void load_some(const T* p, int n) {
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) {
+        if constexpr (sizeof(T) == 4) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+        else w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p) + i) << (16 * (i & 1));
+      }
+    bits = make_uint4(w[0], w[1], w[2], w[3]);
+  }
   __device__ __forceinline__ void get(float (&v)[V]) const {
     const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
     if constexpr (sizeof(T) == 4) {
@@ -105,6 +116,7 @@ template <typename T>
 struct Raw<T, 1> {
   T value;
   __device__ __forceinline__ void load(const T* p) { value = __ldg(p); }
+  __device__ __forceinline__ void load_some(const T* p, int) { value = __ldg(p); }
   __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = to_f32<T>(value); }
   static __device__ __forceinline__ void store(T* p, const float (&v)[1]) {
     *p = from_f32<T>(v[0]);

@@ -150,12 +150,13 @@ struct FewShape {
   static constexpr int kMaxPanel = 512;
   static constexpr int kRows = 8 * TILES;
   static constexpr int kStageInner = W4 ? 2 * kRowBytes : kRowBytes / 2;
-  // Scales (and zero points) of a warp's 16 outputs in a stage: two sets, one in use. An
-  // output's are an odd number of words apart, so 8 outputs hit 8 banks.
-  static constexpr int kGroups = W4 ? kStageInner >> SHIFT : 0;
+  // Scales (and zero points) of a warp's 16 outputs in a stage: two sets, one in use; two
+  // lanes bring an output's, kScaleLane each. An output's are kScalePitch apart, so that 8
+  // outputs hit different banks.
+  static constexpr int kGroups = W4 ? kStageInner >> SHIFT : 2;
   static constexpr int kScalePitch = kGroups + 2;
   static constexpr int kScaleBytes = W4 ? 16 * kScalePitch * 2 : 0;
-  static constexpr int kScaleLane = W4 ? (16 * kGroups + 31) / 32 : 1;  // a lane's share
+  static constexpr int kScaleLane = kGroups / 2;
   // bytes of a staged token: the fragment loads of 8 tokens hit different banks
   static __host__ __device__ int token_pitch(int panel) { return panel * 2 + (W4 ? 64 : 16); }
   static __host__ __device__ int tokens(int panel) {
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   int load_slot = 0;
   auto load_stage = [&](int i) {
     if (i < stages) {
-      const char* src = src0 + i * kRowBytes;
+      const char* src = src0 + i * kRowBytes;  // of the slice's stage i
       const uint32_t dst = dst0 + load_slot * kStageBytes;
       const int rest = rest0 - i * kRowBytes;
       if (S::ALIGN == 16 && my_row0 + 16 <= g.outer &&
@@ -276,39 +277,48 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   // (As words, loaded under a branch: a half-register result, or a select behind the load,
   // would wait for it.)
   uint32_t next_scale[S::kScaleLane], next_zero[S::kScaleLane];
-  const uint16_t* scale0 = static_cast<const uint16_t*>(g.scales) +
-                           ((int64_t)expert * g.outer + my_row0) * g.groups + (k_begin >> SHIFT);
-  const uint8_t* zero0 = g.zeros + ((int64_t)expert * g.outer + my_row0) * g.groups +
-                         (k_begin >> SHIFT);
-  auto fetch_scales = [&](int i) {
+  const int scale_row = lane >> 1, scale_col = (lane & 1) * S::kScaleLane;
+  const int64_t scale_at = ((int64_t)expert * g.outer + my_row0 + scale_row) * g.groups +
+                           (k_begin >> SHIFT) + scale_col;
+  const uint16_t* scale_src = static_cast<const uint16_t*>(g.scales) + scale_at;
+  const uint8_t* zero_src = S::ZEROS ? g.zeros + scale_at : nullptr;
+  // groups left from this lane's first one; none for an output that does not exist
+  int scale_left = my_row0 + scale_row < g.outer
+                       ? g.groups - (k_begin >> SHIFT) - scale_col : 0;
+  auto fetch_scales = [&] {  // of the next stage
     if constexpr (W4) {
 #pragma unroll
       for (int j = 0; j < S::kScaleLane; ++j) {
-        const int p = lane + 32 * j, r = p / S::kGroups, c = i * S::kGroups + p % S::kGroups;
         next_scale[j] = 0;
         next_zero[j] = 8;
-        if (r < 16 && my_row0 + r < g.outer && (k_begin >> SHIFT) + c < g.groups && i < stages) {
-          asm volatile("ld.global.nc.u16 %0, [%1];"
-                       : "=r"(next_scale[j])
-                       : "l"(scale0 + r * g.groups + c));
+        if (j < scale_left) {
+          asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(next_scale[j]) : "l"(scale_src + j));
           if constexpr (S::ZEROS)
-            asm volatile("ld.global.nc.u8 %0, [%1];"
-                         : "=r"(next_zero[j])
-                         : "l"(zero0 + r * g.groups + c));
+            asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(next_zero[j]) : "l"(zero_src + j));
         }
       }
+      scale_src += S::kGroups;
+      if constexpr (S::ZEROS) zero_src += S::kGroups;
+      scale_left -= S::kGroups;
     }
   };
   auto keep_scales = [&](int i) {
     if constexpr (W4) {
-      uint16_t* set = reinterpret_cast<uint16_t*>(scale_sets + (i & 1) * S::kScaleBytes);
-      uint16_t* zset = reinterpret_cast<uint16_t*>(scale_sets + (2 + (i & 1)) * S::kScaleBytes);
+      const int at = scale_row * S::kScalePitch + scale_col;
+      uint16_t* set = reinterpret_cast<uint16_t*>(scale_sets + (i & 1) * S::kScaleBytes) + at;
+      uint16_t* zset =
+          reinterpret_cast<uint16_t*>(scale_sets + (2 + (i & 1)) * S::kScaleBytes) + at;
+      if constexpr (S::kScaleLane == 1) {
+        set[0] = (uint16_t)next_scale[0];
+        if constexpr (S::ZEROS) zset[0] = (uint16_t)(Magic<T>::kBits + (next_zero[0] & 15));
+      } else {
 #pragma unroll
-      for (int j = 0; j < S::kScaleLane; ++j) {
-        const int p = lane + 32 * j, at = p / S::kGroups * S::kScalePitch + p % S::kGroups;
-        if (p < 16 * S::kGroups) {
-          set[at] = (uint16_t)next_scale[j];
-          if constexpr (S::ZEROS) zset[at] = (uint16_t)(Magic<T>::kBits + (next_zero[j] & 15));
+        for (int j = 0; j < S::kScaleLane; j += 2) {
+          *reinterpret_cast<uint32_t*>(set + j) = next_scale[j] | next_scale[j + 1] << 16;
+          if constexpr (S::ZEROS)
+            *reinterpret_cast<uint32_t*>(zset + j) =
+                Magic<T>::kBits * 0x10001u +
+                ((next_zero[j] & 15) | (next_zero[j + 1] & 15) << 16);
         }
       }
     }
@@ -371,7 +381,7 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
 
 #pragma unroll
   for (int i = 0; i < kRing - 1; ++i) load_stage(i);
-  fetch_scales(0);
+  fetch_scales();
   fetch_tokens(k_begin);
   keep_scales(0);
 
@@ -386,7 +396,7 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
       fetch_tokens(k_begin + i * S::kStageInner + g.panel);
     }
     load_stage(i + kRing - 1);
-    fetch_scales(i + 1);
+    if (i + 1 < stages) fetch_scales();
     asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
     __syncwarp();
     const uint8_t* st = ring + slot * kStageBytes;
@@ -399,7 +409,7 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
       const uint16_t* zeros =
           reinterpret_cast<const uint16_t*>(scale_sets + (2 + (i & 1)) * S::kScaleBytes);
       constexpr int kSteps = (1 << SHIFT) / 32;  // of 32 in a scale group
-#pragma unroll(TILES == 1 ? 2 : 1)
+#pragma unroll(TILES == 1 ? 8 : 1)
       for (int j0 = 0; j0 < S::kStageInner / 32; j0 += kSteps) {
         const int lo = gq * S::kScalePitch + j0 / kSteps, hi = lo + 8 * S::kScalePitch;
         uint32_t zl = (Magic<T>::kBits + 8) * 0x10001u, zh = zl;

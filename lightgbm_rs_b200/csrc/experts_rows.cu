@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kRowThreads)
     const int64_t i0 = (b0 + u * kRowThreads) * 8;
 #pragma unroll
     for (int h = 0; h < kParts; ++h) {
-      const int64_t i = i0 + h * V;  // VEC: n is a multiple of V wherever i0 + 8 > n
+      const int64_t i = i0 + h * V;
       if (i < n) {
         int64_t at = i, rat = i;
         if (width != n) {
@@ -169,8 +169,13 @@ __global__ void __launch_bounds__(kRowThreads)
           at = r * pitch + c;
           rat = r * residual_pitch + c;
         }
-        v[u][h].load(x + at);
-        if constexpr (RES) a[u][h].load(residual + rat);
+        if (i + V <= n) {
+          v[u][h].load(x + at);
+          if constexpr (RES) a[u][h].load(residual + rat);
+        } else {
+          v[u][h].load_some(x + at, (int)(n - i));
+          if constexpr (RES) a[u][h].load_some(residual + rat, (int)(n - i));
+        }
       }
     }
   }
@@ -194,7 +199,14 @@ __global__ void __launch_bounds__(kRowThreads)
         e[i] = all || w > cut ? e[i] * scale : 0.0f;
         if constexpr (RES) e[i] += r[i];
       }
-      Raw<T, V>::store(out + b * 8 + h * V, e);
+      const int64_t at = b * 8 + h * V;
+      if (at + V <= n) {
+        Raw<T, V>::store(out + at, e);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (at + i < n) out[at + i] = from_f32<T>(e[i]);
+      }
     }
   }
 }
@@ -301,11 +313,11 @@ cudaError_t launch_dropout(const void* x, const void* residual, int32_t dtype, i
       width = n;  // contiguous: one row
       pitch = residual_pitch = n;
     }
-    // 16 bytes at a time: whole groups of V in every row (of the array, when contiguous)
+    // 16 bytes at a time: whole groups of 8 in every row; an array that is one row may end
+    // anywhere
     const bool vec = aligned16(x) && aligned16(out) && (!residual || aligned16(residual)) &&
-                     (width == n ? n % V == 0
-                                 : width % 8 == 0 && pitch % V == 0 &&
-                                       (!residual || residual_pitch % V == 0));
+                     (width == n || (width % 8 == 0 && pitch % V == 0 &&
+                                     (!residual || residual_pitch % V == 0)));
     const float scale = drop < 65536u ? (float)(65536.0 / (65536.0 - (double)drop)) : 0.0f;
     const uint32_t cut = drop == 0 ? 0u : (uint32_t)(((uint64_t)drop << 16) - 1);
     const int64_t per_block = (int64_t)kRowThreads * kDropUnroll * 8;
