@@ -576,31 +576,34 @@ int lgbm_b200_experts_route_backward(const float* dweights, const float* weights
  * e with offsets[e] <= r < offsets[e + 1]:
  *   y[r]  = w[e] x[index ? index[r] : r]    [rows][outer]; w [experts][outer][inner]
  *   dx[r] = dy[r] w[e]                      [rows][inner]
- *   dw[e] = sum of dy[r]^T x[...]           [experts][outer][inner], of `out_dtype`: the
+ *   dw[e] = sum of dy[r]^T x[...]           [experts][outer][inner], of `grad_dtype`: the
  *                                           inputs' type or f32
  * Rows of y and dx that belong to no expert are 0, and so is the dw of an expert without
  * rows. An index outside [0, x_rows) stands for a row of zeros. x, dy and w are read in
  * place when their base and pitch are multiples of 16 bytes, else copied to the workspace
- * first; mode: 0 y, 1 dx, 2 dw. */
-int64_t lgbm_b200_experts_matmul_workspace(int32_t mode, const void* x, int64_t x_pitch,
-                                           const int32_t* index, const void* dy,
-                                           int64_t dy_pitch, const void* w, int64_t rows,
-                                           int32_t experts, int32_t inner, int32_t outer);
+ * first. */
+int64_t lgbm_b200_experts_matmul_workspace(const void* x, int64_t x_pitch, const int32_t* index,
+                                           const void* w, int64_t rows, int32_t experts,
+                                           int32_t inner, int32_t outer);
 int lgbm_b200_experts_matmul(const void* x, int64_t x_rows, int64_t x_pitch,
                              const int32_t* index, const void* w, const int32_t* offsets,
                              int32_t dtype, int64_t rows, int32_t experts, int32_t inner,
                              int32_t outer, void* y, void* workspace, int64_t workspace_bytes,
                              void* stream);
-int lgbm_b200_experts_matmul_input_grad(const void* dy, int64_t dy_pitch, const void* w,
-                                        const int32_t* offsets, int32_t dtype, int64_t rows,
-                                        int32_t experts, int32_t inner, int32_t outer, void* dx,
-                                        void* workspace, int64_t workspace_bytes, void* stream);
-int lgbm_b200_experts_matmul_weight_grad(const void* dy, int64_t dy_pitch, const void* x,
-                                         int64_t x_rows, int64_t x_pitch, const int32_t* index,
-                                         const int32_t* offsets, int32_t dtype,
-                                         int32_t out_dtype, int64_t rows, int32_t experts,
-                                         int32_t inner, int32_t outer, void* dw, void* workspace,
-                                         int64_t workspace_bytes, void* stream);
+/* Both gradients, or one of them: dx or dw NULL is not wanted (w is read for dx only, x for
+ * dw only). */
+int64_t lgbm_b200_experts_matmul_backward_workspace(const void* dy, int64_t dy_pitch,
+                                                    const void* x, int64_t x_pitch,
+                                                    const int32_t* index, const void* w,
+                                                    int64_t rows, int32_t experts, int32_t inner,
+                                                    int32_t outer, int32_t want_dx,
+                                                    int32_t want_dw);
+int lgbm_b200_experts_matmul_backward(const void* dy, int64_t dy_pitch, const void* x,
+                                      int64_t x_rows, int64_t x_pitch, const int32_t* index,
+                                      const void* w, const int32_t* offsets, int32_t dtype,
+                                      int32_t grad_dtype, int64_t rows, int32_t experts,
+                                      int32_t inner, int32_t outer, void* dx, void* dw,
+                                      void* workspace, int64_t workspace_bytes, void* stream);
 /* y as lgbm_b200_experts_matmul, for a few rows an expert, with weights of 4 bits in groups
  * of group_size (32, 64 or 128) along the inner axis:
  *   w[e][n][k] = scales[e][n][k / group_size] * (q - z)

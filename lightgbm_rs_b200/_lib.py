@@ -161,14 +161,13 @@ _SIGS = {
                                  _i64, _P], ctypes.c_int),
     "lgbm_b200_experts_route_backward": ([_P, _P, _P, _P, _i32, _i64, _i32, _i64, _i32, _i32, _P,
                                           _P], ctypes.c_int),
-    "lgbm_b200_experts_matmul_workspace": ([_i32, _P, _i64, _P, _P, _i64, _P, _i64, _i32, _i32,
-                                            _i32], _i64),
+    "lgbm_b200_experts_matmul_workspace": ([_P, _i64, _P, _P, _i64, _i32, _i32, _i32], _i64),
     "lgbm_b200_experts_matmul": ([_P, _i64, _i64, _P, _P, _P, _i32, _i64, _i32, _i32, _i32, _P,
                                   _P, _i64, _P], ctypes.c_int),
-    "lgbm_b200_experts_matmul_input_grad": ([_P, _i64, _P, _P, _i32, _i64, _i32, _i32, _i32, _P,
-                                             _P, _i64, _P], ctypes.c_int),
-    "lgbm_b200_experts_matmul_weight_grad": ([_P, _i64, _P, _i64, _i64, _P, _P, _i32, _i32, _i64,
-                                              _i32, _i32, _i32, _P, _P, _i64, _P], ctypes.c_int),
+    "lgbm_b200_experts_matmul_backward_workspace": ([_P, _i64, _P, _i64, _P, _P, _i64, _i32, _i32,
+                                                     _i32, _i32, _i32], _i64),
+    "lgbm_b200_experts_matmul_backward": ([_P, _i64, _P, _i64, _i64, _P, _P, _P, _i32, _i32, _i64,
+                                           _i32, _i32, _i32, _P, _P, _P, _i64, _P], ctypes.c_int),
     "lgbm_b200_experts_matmul_w4": ([_P, _i64, _i64, _P, _P, _P, _P, _i32, _P, _i32, _i64, _i32,
                                      _i32, _i32, _P, _P], ctypes.c_int),
     "lgbm_b200_experts_errors": ([_P], ctypes.c_int),

@@ -152,18 +152,17 @@ cudaError_t launch_dropout(const void* x, const void* residual, int32_t dtype, i
 
 // experts_matmul.cu
 struct MatmulCall {
-  int32_t mode;             // 0 forward, 1 input gradient, 2 weight gradient
-  int32_t dtype, out_dtype;
-  const void* x;            // [x_rows, inner], or null (mode 1)
+  int32_t dtype, grad_dtype;
+  const void* x;            // [x_rows, inner]; null where no result needs it
   int64_t x_rows, x_pitch;
   const int32_t* index;     // row of x of every grouped row, or null
-  const void* dy;           // [rows, outer], or null (mode 0)
+  const void* dy;           // [rows, outer], gradients only
   int64_t dy_pitch;
-  const void* w;            // [experts, outer, inner], or null (mode 2)
+  const void* w;            // [experts, outer, inner]; null where no result needs it
   const int32_t* offsets;
   int64_t rows;
   int32_t experts, inner, outer;
-  void* out;
+  void *y, *dx, *dw;        // results, null: not wanted
 };
 int64_t matmul_workspace(const MatmulCall& c);
 cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st);

@@ -54,24 +54,26 @@ int check_gate(const char* what, int32_t dtype, int64_t tokens, int32_t experts,
 int check_product(const char* what, const MatmulCall& c) {
   if (c.dtype != LGBM_B200_DTYPE_BF16 && c.dtype != LGBM_B200_DTYPE_F16)
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: dtype %d is not bf16 or f16", what, c.dtype);
-  if (c.out_dtype != c.dtype && !(c.mode == 2 && c.out_dtype == LGBM_B200_DTYPE_F32))
-    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: output dtype %d", what, c.out_dtype);
+  if (c.dw && c.grad_dtype != c.dtype && c.grad_dtype != LGBM_B200_DTYPE_F32)
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: dw's dtype %d", what, c.grad_dtype);
   if (c.rows < 0 || c.experts < 1 || c.inner < 1 || c.outer < 1)
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: rows %lld, experts %d, inner %d, outer %d",
                   what, (long long)c.rows, c.experts, c.inner, c.outer);
-  if (c.experts > kMaxExperts || c.rows > kMaxRows)
+  if (c.experts > kMaxExperts || c.rows > kMaxRows || c.x_rows > kMaxRows)
     return refuse(LGBM_B200_CAPABILITY_UNAVAILABLE,
-                  "%s: %d experts (at most %d), %lld rows (at most %lld)", what, c.experts,
-                  kMaxExperts, (long long)c.rows, (long long)kMaxRows);
-  if (!c.offsets || (!c.out && (c.rows > 0 || c.mode == 2)) || (c.rows > 0 && ((c.mode != 1 && !c.x) || (c.mode != 0 && !c.dy))) ||
-      (c.mode != 2 && !c.w))
+                  "%s: %d experts (at most %d), %lld rows of %lld (at most %lld)", what,
+                  c.experts, kMaxExperts, (long long)c.rows, (long long)c.x_rows,
+                  (long long)kMaxRows);
+  const bool reads_x = c.y || c.dw, reads_dy = c.dx || c.dw, reads_w = c.y || c.dx;
+  if (!c.offsets || (c.rows > 0 && ((reads_x && !c.x) || (reads_dy && !c.dy))) ||
+      (reads_w && !c.w))
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
-  if (c.mode != 1 && (c.x_pitch < c.inner || c.x_rows < (c.rows > 0) || c.x_rows > kMaxRows ||
-                      (!c.index && c.x_rows != c.rows)))
+  if (reads_x && (c.x_pitch < c.inner || c.x_rows < (c.rows > 0) ||
+                  (!c.index && c.x_rows != c.rows)))
     return refuse(LGBM_B200_LENGTH_MISMATCH,
                   "%s: x has %lld rows of pitch %lld, want %lld of at least %d", what,
                   (long long)c.x_rows, (long long)c.x_pitch, (long long)c.rows, c.inner);
-  if (c.mode != 0 && c.dy_pitch < c.outer)
+  if (reads_dy && c.dy_pitch < c.outer)
     return refuse(LGBM_B200_LENGTH_MISMATCH, "%s: dy pitch %lld < outer %d", what,
                   (long long)c.dy_pitch, c.outer);
   return LGBM_B200_OK;
@@ -82,11 +84,11 @@ int run_product(const char* what, const MatmulCall& c, void* workspace, int64_t 
   if (int rc = check_product(what, c)) return rc;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (c.rows == 0) {
-    if (c.mode != 2) return LGBM_B200_OK;
-    return launched(cudaMemsetAsync(c.out, 0,
-                                    (size_t)c.experts * c.outer * c.inner * elem_size(c.out_dtype),
-                                    st),
-                    what);
+    if (!c.dw) return LGBM_B200_OK;
+    return launched(
+        cudaMemsetAsync(c.dw, 0, (size_t)c.experts * c.outer * c.inner * elem_size(c.grad_dtype),
+                        st),
+        what);
   }
   const int64_t need = matmul_workspace(c);
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace))))
@@ -204,23 +206,21 @@ int lgbm_b200_experts_dropout(const void* x, const void* residual, int32_t dtype
                   what);
 }
 
-int64_t lgbm_b200_experts_matmul_workspace(int32_t mode, const void* x, int64_t x_pitch,
-                                           const int32_t* index, const void* dy,
-                                           int64_t dy_pitch, const void* w, int64_t rows,
-                                           int32_t experts, int32_t inner, int32_t outer) {
+int64_t lgbm_b200_experts_matmul_workspace(const void* x, int64_t x_pitch, const int32_t* index,
+                                           const void* w, int64_t rows, int32_t experts,
+                                           int32_t inner, int32_t outer) {
+  if (rows < 1 || experts < 1 || inner < 1 || outer < 1) return 0;
   MatmulCall c{};
-  c.mode = mode;
   c.x = x;
   c.x_pitch = x_pitch;
   c.index = index;
-  c.dy = dy;
-  c.dy_pitch = dy_pitch;
   c.w = w;
   c.rows = rows;
   c.experts = experts;
   c.inner = inner;
   c.outer = outer;
-  return rows < 1 || experts < 1 || inner < 1 || outer < 1 ? 0 : matmul_workspace(c);
+  c.y = &c;  // wanted; not written here
+  return matmul_workspace(c);
 }
 
 int lgbm_b200_experts_matmul(const void* x, int64_t x_rows, int64_t x_pitch,
@@ -228,65 +228,74 @@ int lgbm_b200_experts_matmul(const void* x, int64_t x_rows, int64_t x_pitch,
                              int32_t dtype, int64_t rows, int32_t experts, int32_t inner,
                              int32_t outer, void* y, void* workspace, int64_t workspace_bytes,
                              void* stream) {
+  const char* what = "experts_matmul";
+  if (!y && rows > 0) return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
   MatmulCall c{};
-  c.mode = 0;
-  c.dtype = c.out_dtype = dtype;
-  c.x = x;
-  c.x_rows = x_rows;
-  c.x_pitch = x_pitch;
-  c.index = index;
-  c.w = w;
-  c.offsets = offsets;
-  c.rows = rows;
-  c.experts = experts;
-  c.inner = inner;
-  c.outer = outer;
-  c.out = y;
-  return run_product("experts_matmul", c, workspace, workspace_bytes, stream);
-}
-
-int lgbm_b200_experts_matmul_input_grad(const void* dy, int64_t dy_pitch, const void* w,
-                                        const int32_t* offsets, int32_t dtype, int64_t rows,
-                                        int32_t experts, int32_t inner, int32_t outer, void* dx,
-                                        void* workspace, int64_t workspace_bytes, void* stream) {
-  MatmulCall c{};
-  c.mode = 1;
-  c.dtype = c.out_dtype = dtype;
-  c.dy = dy;
-  c.dy_pitch = dy_pitch;
-  c.w = w;
-  c.offsets = offsets;
-  c.rows = rows;
-  c.experts = experts;
-  c.inner = inner;
-  c.outer = outer;
-  c.out = dx;
-  return run_product("experts_matmul_input_grad", c, workspace, workspace_bytes, stream);
-}
-
-int lgbm_b200_experts_matmul_weight_grad(const void* dy, int64_t dy_pitch, const void* x,
-                                         int64_t x_rows, int64_t x_pitch, const int32_t* index,
-                                         const int32_t* offsets, int32_t dtype,
-                                         int32_t out_dtype, int64_t rows, int32_t experts,
-                                         int32_t inner, int32_t outer, void* dw, void* workspace,
-                                         int64_t workspace_bytes, void* stream) {
-  MatmulCall c{};
-  c.mode = 2;
   c.dtype = dtype;
-  c.out_dtype = out_dtype;
+  c.x = x;
+  c.x_rows = x_rows;
+  c.x_pitch = x_pitch;
+  c.index = index;
+  c.w = w;
+  c.offsets = offsets;
+  c.rows = rows;
+  c.experts = experts;
+  c.inner = inner;
+  c.outer = outer;
+  c.y = y ? y : &c;  // no rows: nothing is written
+  return run_product(what, c, workspace, workspace_bytes, stream);
+}
+
+int64_t lgbm_b200_experts_matmul_backward_workspace(const void* dy, int64_t dy_pitch,
+                                                    const void* x, int64_t x_pitch,
+                                                    const int32_t* index, const void* w,
+                                                    int64_t rows, int32_t experts, int32_t inner,
+                                                    int32_t outer, int32_t want_dx,
+                                                    int32_t want_dw) {
+  if (rows < 1 || experts < 1 || inner < 1 || outer < 1) return 0;
+  MatmulCall c{};
+  c.x = x;
+  c.x_pitch = x_pitch;
+  c.index = index;
+  c.dy = dy;
+  c.dy_pitch = dy_pitch;
+  c.w = w;
+  c.rows = rows;
+  c.experts = experts;
+  c.inner = inner;
+  c.outer = outer;
+  c.dx = want_dx ? &c : nullptr;  // wanted; not written here
+  c.dw = want_dw ? &c : nullptr;
+  return matmul_workspace(c);
+}
+
+int lgbm_b200_experts_matmul_backward(const void* dy, int64_t dy_pitch, const void* x,
+                                      int64_t x_rows, int64_t x_pitch, const int32_t* index,
+                                      const void* w, const int32_t* offsets, int32_t dtype,
+                                      int32_t grad_dtype, int64_t rows, int32_t experts,
+                                      int32_t inner, int32_t outer, void* dx, void* dw,
+                                      void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "experts_matmul_backward";
+  if (!dx && !dw && rows > 0)
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: neither dx nor dw is wanted", what);
+  MatmulCall c{};
+  c.dtype = dtype;
+  c.grad_dtype = grad_dtype;
   c.x = x;
   c.x_rows = x_rows;
   c.x_pitch = x_pitch;
   c.index = index;
   c.dy = dy;
   c.dy_pitch = dy_pitch;
+  c.w = w;
   c.offsets = offsets;
   c.rows = rows;
   c.experts = experts;
   c.inner = inner;
   c.outer = outer;
-  c.out = dw;
-  return run_product("experts_matmul_weight_grad", c, workspace, workspace_bytes, stream);
+  c.dx = dx;
+  c.dw = dw;
+  return run_product(what, c, workspace, workspace_bytes, stream);
 }
 
 int lgbm_b200_experts_matmul_w4(const void* x, int64_t x_rows, int64_t x_pitch,
@@ -296,8 +305,9 @@ int lgbm_b200_experts_matmul_w4(const void* x, int64_t x_rows, int64_t x_pitch,
                                 int32_t experts, int32_t inner, int32_t outer, void* y,
                                 void* stream) {
   const char* what = "experts_matmul_w4";
+  if (!y && rows > 0) return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
   MatmulCall c{};
-  c.dtype = c.out_dtype = dtype;
+  c.dtype = dtype;
   c.x = x;
   c.x_rows = x_rows;
   c.x_pitch = x_pitch;
@@ -308,7 +318,7 @@ int lgbm_b200_experts_matmul_w4(const void* x, int64_t x_rows, int64_t x_pitch,
   c.experts = experts;
   c.inner = inner;
   c.outer = outer;
-  c.out = y;
+  c.y = y ? y : &c;  // no rows: nothing is written
   if (int rc = check_product(what, c)) return rc;
   if (group_size != 32 && group_size != 64 && group_size != 128)
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: group size %d is not 32, 64 or 128", what,

@@ -896,16 +896,23 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
 }  // namespace
 
 // Few rows an expert: the forward product streams the weights instead (experts_few.cu).
-static bool few_rows(const MatmulCall& c) { return c.mode == 0 && c.rows <= 16 * (int64_t)c.experts; }
+static bool few_rows(const MatmulCall& c) {
+  return c.y && c.rows <= 16 * (int64_t)c.experts;
+}
+static bool copies_x(const MatmulCall& c) {
+  return ((c.y && !few_rows(c)) || c.dw) && (c.index || !walkable(c.x, c.x_pitch));
+}
+static bool copies_dy(const MatmulCall& c) {
+  return (c.dx || c.dw) && !walkable(c.dy, c.dy_pitch);
+}
+static bool copies_w(const MatmulCall& c) {
+  return ((c.y && !few_rows(c)) || c.dx) && !(aligned16(c.w) && c.inner % 8 == 0);
+}
 
 int64_t matmul_workspace(const MatmulCall& c) {
-  int64_t n = 0;
-  if (few_rows(c)) return 0;
-  if (c.mode != 1 && (c.index || !walkable(c.x, c.x_pitch))) n += copy_bytes(c.rows, c.inner);
-  if (c.mode != 0 && !walkable(c.dy, c.dy_pitch)) n += copy_bytes(c.rows, c.outer);
-  if (c.mode != 2 && !(aligned16(c.w) && c.inner % 8 == 0))
-    n += copy_bytes((int64_t)c.experts * c.outer, c.inner);
-  return n;
+  return (copies_x(c) ? copy_bytes(c.rows, c.inner) : 0) +
+         (copies_dy(c) ? copy_bytes(c.rows, c.outer) : 0) +
+         (copies_w(c) ? copy_bytes((int64_t)c.experts * c.outer, c.inner) : 0);
 }
 
 cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st) {
@@ -922,42 +929,47 @@ cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st)
     f.experts = c.experts;
     f.inner = c.inner;
     f.outer = c.outer;
-    f.y = c.out;
+    f.y = c.y;
     return launch_few(f, st);
   }
   char* ws = static_cast<char*>(workspace);
+  Operand x{c.x, c.x_pitch}, dy{c.dy, c.dy_pitch}, w{c.w, c.inner};
+  cudaError_t err = cudaSuccess;
+  if (copies_x(c)) err = stage(x, c.x_rows, c.rows, c.inner, c.index, ws, st);
+  if (err == cudaSuccess && copies_dy(c))
+    err = stage(dy, c.rows, c.rows, c.outer, nullptr, ws, st);
+  const int64_t w_rows = (int64_t)c.experts * c.outer;
+  if (err == cudaSuccess && copies_w(c))
+    err = stage(w, w_rows, w_rows, c.inner, nullptr, ws, st);
   MatArgs g{};
   g.offsets = c.offsets;
   g.experts = c.experts;
   g.rows = c.rows;
-  g.out = c.out;
-  g.out_kind = c.out_dtype;
-  Operand x{c.x, c.x_pitch}, dy{c.dy, c.dy_pitch}, w{c.w, c.inner};
-  cudaError_t err = cudaSuccess;
-  if (c.mode != 1 && (c.index || !walkable(c.x, c.x_pitch)))
-    err = stage(x, c.x_rows, c.rows, c.inner, c.index, ws, st);
-  if (err == cudaSuccess && c.mode != 0 && !walkable(c.dy, c.dy_pitch))
-    err = stage(dy, c.rows, c.rows, c.outer, nullptr, ws, st);
-  if (err == cudaSuccess && c.mode != 2 && !(aligned16(c.w) && c.inner % 8 == 0))
-    err = stage(w, (int64_t)c.experts * c.outer, (int64_t)c.experts * c.outer, c.inner, nullptr,
-                ws, st);
-  if (err != cudaSuccess) return err;
-  if (c.mode == 0) {
+  if (err == cudaSuccess && c.y) {
+    g.out = c.y;
+    g.out_kind = c.dtype;
     g.cols = c.outer;
     g.reduction = c.inner;
     g.out_pitch = c.outer;
-    return run_tiles<FORWARD>(x, c.inner, w, c.inner, c.dtype, g, st);
+    err = run_tiles<FORWARD>(x, c.inner, w, c.inner, c.dtype, g, st);
   }
-  if (c.mode == 1) {
+  if (err == cudaSuccess && c.dx) {
+    g.out = c.dx;
+    g.out_kind = c.dtype;
     g.cols = c.inner;
     g.reduction = c.outer;
     g.out_pitch = c.inner;
-    return run_tiles<INPUT>(dy, c.outer, w, c.inner, c.dtype, g, st);
+    err = run_tiles<INPUT>(dy, c.outer, w, c.inner, c.dtype, g, st);
   }
-  g.cols = c.inner;
-  g.drows = c.outer;
-  g.out_pitch = c.inner;
-  return run_tiles<WEIGHT>(dy, c.outer, x, c.inner, c.dtype, g, st);
+  if (err == cudaSuccess && c.dw) {
+    g.out = c.dw;
+    g.out_kind = c.grad_dtype;
+    g.cols = c.inner;
+    g.drows = c.outer;
+    g.out_pitch = c.inner;
+    err = run_tiles<WEIGHT>(dy, c.outer, x, c.inner, c.dtype, g, st);
+  }
+  return err;
 }
 
 cudaError_t read_matmul_errors(uint32_t* bits) {

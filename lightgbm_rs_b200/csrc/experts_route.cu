@@ -227,8 +227,6 @@ __global__ void __launch_bounds__(kSelectThreads)
   constexpr int kWarps = kSelectThreads / 32;
   constexpr bool kTwoStages = CN < NV;
   __shared__ int32_t hist[kMaxExperts + 1];
-  __shared__ float dealt[kTwoStages ? kWarps : 1][kTwoStages ? CN * 32 : 1];
-  __shared__ int32_t dealt_lane[kTwoStages ? kWarps : 1][kMaxChosen];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i <= experts; i += kSelectThreads) hist[i] = 0;
   __syncthreads();
@@ -266,29 +264,32 @@ __global__ void __launch_bounds__(kSelectThreads)
           if (v[i] != v[i]) at = i;
       }
       uint32_t lane_key = logit_key(top);
-      for (int c = lane; c < CN * 32; c += 32) dealt[warp][c] = kNone;
-      __syncwarp();
+      int from[CN];  // lane that this lane's candidates come from: number (32 c + lane) / NV
+#pragma unroll
+      for (int c = 0; c < CN; ++c) from[c] = -1;
       for (int j = 0; j < k; ++j) {
         const uint32_t best = __reduce_max_sync(kAll, lane_key);
         if (best == kKeyEmpty) break;
-        const int e = (int)__reduce_min_sync(
-            kAll, lane_key == best ? (uint32_t)(at * 32 + lane) : kAll);
-        if (lane == (e & 31)) {
-          lane_key = kKeyEmpty;
-          dealt_lane[warp][j] = lane;
+        const int owner = (int)(__reduce_min_sync(kAll, lane_key == best
+                                                            ? (uint32_t)(at * 32 + lane)
+                                                            : kAll) & 31);
+        if (lane == owner) lane_key = kKeyEmpty;
 #pragma unroll
-          for (int i = 0; i < NV; ++i) dealt[warp][j * NV + i] = v[i];
-        }
+        for (int c = 0; c < CN; ++c)
+          if ((c * 32 + lane) / NV == j) from[c] = owner;
       }
-      __syncwarp();
+      // candidate lane % NV of each lane's source
 #pragma unroll
       for (int c = 0; c < CN; ++c) {
-        const int from = c * 32 + lane;
-        const float x = from < k * NV ? dealt[warp][from] : kNone;
-        key[c] = logit_key(x);
-        id[c] = x == kNone ? 0 : (from % NV) * 32 + dealt_lane[warp][from / NV];
+        float x = kNone;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const float y = __shfl_sync(kAll, v[i], from[c] & 31);
+          if (lane % NV == i) x = y;
+        }
+        key[c] = from[c] < 0 ? kKeyEmpty : logit_key(x);
+        id[c] = key[c] == kKeyEmpty ? 0 : (lane % NV) * 32 + from[c];
       }
-      __syncwarp();
     } else {
 #pragma unroll
       for (int c = 0; c < CN; ++c) {
@@ -429,21 +430,23 @@ __global__ void __launch_bounds__(kSmallThreads)
 // a chosen expert p_e is its weight. Over all experts the others' p is recomputed from one
 // chosen logit: the first chosen one is the largest, m, and its weight is 1 / sum exp(l - m).
 // The row is written as if nothing were chosen, then the chosen places again.
-template <typename T, int NV>
+// LANES is at least k; NV experts a lane.
+template <typename T, int LANES, int NV>
 __global__ void __launch_bounds__(256)
-    k_route_backward(const float* dweights, const float* weights, const int32_t* chosen,
-                     const T* logits, int64_t tokens, int experts, int64_t pitch, int k,
-                     bool normalize, int shift, T* dlogits) {
-  const int lanes = 1 << shift;  // at least k, and enough for NV experts a lane
-  const int64_t t = (int64_t)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
-  const int sub = threadIdx.x & (lanes - 1);
+    k_route_backward(const float* __restrict__ dweights, const float* __restrict__ weights,
+                     const int32_t* __restrict__ chosen, const T* __restrict__ logits,
+                     int64_t tokens, int experts, int64_t pitch, int k, bool normalize,
+                     T* __restrict__ dlogits) {
+  const int64_t t = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int sub = threadIdx.x % LANES;
   const bool live = t < tokens;
   const T* row = logits + t * pitch;
+  T* out = dlogits + t * experts;
   T v[NV];
   if (live && !normalize) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (i * lanes + sub < experts) v[i] = __ldg(row + i * lanes + sub);
+      if (i * LANES + sub < experts) v[i] = __ldg(row + i * LANES + sub);
   }
   int id = -1;
   float w = 0.0f, g = 0.0f, m = 0.0f;
@@ -458,23 +461,26 @@ __global__ void __launch_bounds__(256)
     }
   }
   float s = w * g;
-  for (int d = lanes >> 1; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-  m = __shfl_sync(0xFFFFFFFFu, m, 0, lanes);
-  // every other weight is 0 where the first is missing, and so is s
-  const float scale = -s * __shfl_sync(0xFFFFFFFFu, w, 0, lanes);
-  const bool any = __shfl_sync(0xFFFFFFFFu, id, 0, lanes) >= 0;
-  if (live) {
-    T* out = dlogits + t * experts;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = i * lanes + sub;
-      if (e < experts)
-        out[e] = from_f32<T>(normalize || !any ? 0.0f
-                                               : fast_exp(to_f32<T>(v[i]) - m) * scale);
+  for (int d = LANES >> 1; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+  m = __shfl_sync(0xFFFFFFFFu, m, 0, LANES);
+  // every other weight is 0 where the first is missing, and so is s
+  const float scale = -s * __shfl_sync(0xFFFFFFFFu, w, 0, LANES);
+  const bool any = __shfl_sync(0xFFFFFFFFu, id, 0, LANES) >= 0;
+  if (live) {
+    if (normalize || !any) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (i * LANES + sub < experts) out[i * LANES + sub] = from_f32<T>(0.0f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (i * LANES + sub < experts)
+          out[i * LANES + sub] = from_f32<T>(fast_exp(to_f32<T>(v[i]) - m) * scale);
     }
   }
   __syncwarp();
-  if (id >= 0) dlogits[t * experts + id] = from_f32<T>(w * (g - s));
+  if (id >= 0) out[id] = from_f32<T>(w * (g - s));
 }
 
 template <typename T, int KP>
@@ -562,23 +568,27 @@ cudaError_t launch_route_backward(const float* dweights, const float* weights,
                                   const int32_t* chosen, const void* logits, int32_t dtype,
                                   int64_t tokens, int32_t experts, int64_t pitch, int32_t k,
                                   bool normalize, void* dlogits, cudaStream_t st) {
-  int shift = 0;  // lanes of a token: the smallest power of two that covers the experts, or 32
-  while (shift < 5 && (1 << shift) < experts) ++shift;
-  const int64_t per_block = 256 >> shift;
-  const unsigned blocks = (unsigned)((tokens + per_block - 1) / per_block);
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    auto go = [&](auto nv) {
-      k_route_backward<T, decltype(nv)::value><<<blocks, 256, 0, st>>>(
+    auto go = [&](auto lanes, auto nv) {
+      constexpr int LANES = decltype(lanes)::value;
+      const int64_t per_block = 256 / LANES;
+      const unsigned blocks = (unsigned)((tokens + per_block - 1) / per_block);
+      k_route_backward<T, LANES, decltype(nv)::value><<<blocks, 256, 0, st>>>(
           dweights, weights, chosen, static_cast<const T*>(logits), tokens, experts, pitch, k,
-          normalize, shift, static_cast<T*>(dlogits));
+          normalize, static_cast<T*>(dlogits));
       return cudaGetLastError();
     };
-    if (experts <= 32) return go(std::integral_constant<int, 1>());
-    if (experts <= 64) return go(std::integral_constant<int, 2>());
-    if (experts <= 128) return go(std::integral_constant<int, 4>());
-    if (experts <= 256) return go(std::integral_constant<int, 8>());
-    return go(std::integral_constant<int, 16>());
+    using One = std::integral_constant<int, 1>;
+    using Warp = std::integral_constant<int, 32>;
+    if (experts <= 4) return go(std::integral_constant<int, 4>(), One());
+    if (experts <= 8) return go(std::integral_constant<int, 8>(), One());
+    if (experts <= 16) return go(std::integral_constant<int, 16>(), One());
+    if (experts <= 32) return go(Warp(), One());
+    if (experts <= 64) return go(Warp(), std::integral_constant<int, 2>());
+    if (experts <= 128) return go(Warp(), std::integral_constant<int, 4>());
+    if (experts <= 256) return go(Warp(), std::integral_constant<int, 8>());
+    return go(Warp(), std::integral_constant<int, 16>());
   });
 }
 

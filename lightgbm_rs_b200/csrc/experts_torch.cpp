@@ -246,8 +246,8 @@ PyObject* grouped_matmul(PyObject* const* a) {
   On on(dev);
   Tensor y = make(dev, p.x.t.scalar_type(), {p.rows, p.outer});
   Scratch ws(dev, lgbm_b200_experts_matmul_workspace(
-                      0, p.x.p(), p.x.pitch, p.ip(), nullptr, 0, p.w.data_ptr(), p.rows,
-                      (int32_t)p.experts, (int32_t)p.inner, (int32_t)p.outer));
+                      p.x.p(), p.x.pitch, p.ip(), p.w.data_ptr(), p.rows, (int32_t)p.experts,
+                      (int32_t)p.inner, (int32_t)p.outer));
   check(lgbm_b200_experts_matmul(p.x.p(), p.x.rows, p.x.pitch, p.ip(), p.w.data_ptr(),
                                  p.offsets.data_ptr<int32_t>(), p.x.dtype, p.rows,
                                  (int32_t)p.experts, (int32_t)p.inner, (int32_t)p.outer,
@@ -271,24 +271,17 @@ PyObject* grouped_matmul_backward(PyObject* const* a) {
   const int32_t experts = (int32_t)p.experts, inner = (int32_t)p.inner, outer = (int32_t)p.outer;
   On on(dev);
   Tensor dx, dw;
-  if (flag(a[6])) {
-    dx = make(dev, type, {p.rows, p.inner});
-    Scratch ws(dev, lgbm_b200_experts_matmul_workspace(1, nullptr, 0, nullptr, dy.p(), dy.pitch,
-                                                       p.w.data_ptr(), p.rows, experts, inner,
-                                                       outer));
-    check(lgbm_b200_experts_matmul_input_grad(
-        dy.p(), dy.pitch, p.w.data_ptr(), p.offsets.data_ptr<int32_t>(), p.x.dtype, p.rows,
-        experts, inner, outer, dx.data_ptr(), ws.p(), ws.bytes, on.stream));
-  }
-  if (flag(a[7])) {
-    dw = make(dev, wide ? at::kFloat : type, {p.experts, p.outer, p.inner});
-    Scratch ws(dev, lgbm_b200_experts_matmul_workspace(2, p.x.p(), p.x.pitch, p.ip(), dy.p(),
-                                                       dy.pitch, nullptr, p.rows, experts, inner,
-                                                       outer));
-    check(lgbm_b200_experts_matmul_weight_grad(
-        dy.p(), dy.pitch, p.x.p(), p.x.rows, p.x.pitch, p.ip(), p.offsets.data_ptr<int32_t>(),
-        p.x.dtype, wide ? LGBM_B200_DTYPE_F32 : p.x.dtype, p.rows, experts, inner, outer,
-        dw.data_ptr(), ws.p(), ws.bytes, on.stream));
+  if (flag(a[6])) dx = make(dev, type, {p.rows, p.inner});
+  if (flag(a[7])) dw = make(dev, wide ? at::kFloat : type, {p.experts, p.outer, p.inner});
+  if (dx.defined() || dw.defined()) {
+    Scratch ws(dev, lgbm_b200_experts_matmul_backward_workspace(
+                        dy.p(), dy.pitch, p.x.p(), p.x.pitch, p.ip(), p.w.data_ptr(), p.rows,
+                        experts, inner, outer, dx.defined(), dw.defined()));
+    check(lgbm_b200_experts_matmul_backward(
+        dy.p(), dy.pitch, p.x.p(), p.x.rows, p.x.pitch, p.ip(), p.w.data_ptr(),
+        p.offsets.data_ptr<int32_t>(), p.x.dtype, wide ? LGBM_B200_DTYPE_F32 : p.x.dtype, p.rows,
+        experts, inner, outer, dx.defined() ? dx.data_ptr() : nullptr,
+        dw.defined() ? dw.data_ptr() : nullptr, ws.p(), ws.bytes, on.stream));
   }
   return wrap_all(dx, dw);
 }

@@ -43,11 +43,15 @@ def test_arguments_are_refused_with_a_status(capi):
     assert mm(p, 400, 9, None, p, p, 1, 400, 2, 9, 8, p, None, 0, None) == length  # workspace
     assert mm(p, 4, 8, None, None, p, 1, 4, 2, 8, 8, p, None, 0, None) == bad
     assert mm(p, 0, 8, None, p, p, 1, 0, 2, 8, 8, p, None, 0, None) == capi.OK
-    dw = L.lgbm_b200_experts_matmul_weight_grad
-    assert dw(p, 8, p, 4, 8, None, p, 1, 2, 4, 2, 8, 8, p, None, 0, None) == bad
-    assert dw(p, 7, p, 4, 8, None, p, 1, 1, 4, 2, 8, 8, p, None, 0, None) == length
-    dx = L.lgbm_b200_experts_matmul_input_grad
-    assert dx(None, 8, p, p, 1, 4, 2, 8, 8, p, None, 0, None) == bad
+    assert mm(p, 4, 8, None, p, p, 1, 4, 2, 8, 8, None, None, 0, None) == bad  # no result
+    back = L.lgbm_b200_experts_matmul_backward
+    assert back(p, 8, p, 4, 8, None, p, p, 1, 2, 4, 2, 8, 8, p, p, None, 0, None) == bad  # dw f16
+    assert back(p, 7, p, 4, 8, None, p, p, 1, 1, 4, 2, 8, 8, p, p, None, 0, None) == length
+    assert back(None, 8, p, 4, 8, None, p, p, 1, 1, 4, 2, 8, 8, p, p, None, 0, None) == bad
+    assert back(p, 8, p, 4, 8, None, p, p, 1, 1, 4, 2, 8, 8, None, None, None, 0, None) == bad
+    assert back(p, 8, p, 4, 8, None, None, p, 1, 1, 4, 2, 8, 8, p, None, None, 0, None) == bad
+    assert back(p, 9, p, 4, 8, None, p, p, 1, 1, 4, 2, 8, 9, p, p, None, 0, None) == length
+
     w4 = L.lgbm_b200_experts_matmul_w4
     assert w4(p, 4, 8, None, p, p, None, 48, p, 1, 4, 2, 8, 8, p, None) == bad
     assert w4(p, 4, 8, None, p + 8, p, None, 32, p, 1, 4, 2, 8, 8, p, None) == bad
@@ -73,8 +77,12 @@ def test_arguments_are_refused_with_a_status(capi):
 def test_workspace_only_where_an_operand_must_be_copied(capi):
     ws = capi.lib().lgbm_b200_experts_matmul_workspace
     p = 1 << 20
-    assert ws(0, p, 64, None, None, 0, p, 1000, 4, 64, 33) == 0
-    assert ws(0, p, 64, None, None, 0, p + 2, 1000, 4, 64, 33) > 0
-    assert ws(0, p, 65, None, None, 0, p, 1000, 4, 64, 33) > 0
-    assert ws(1, None, 0, None, p, 33, p, 1000, 4, 64, 33) > 0
-    assert ws(2, p, 64, None, p, 40, None, 1000, 4, 64, 33) == 0
+    assert ws(p, 64, None, p, 1000, 4, 64, 33) == 0
+    assert ws(p, 64, None, p + 2, 1000, 4, 64, 33) > 0
+    assert ws(p, 65, None, p, 1000, 4, 65, 33) > 0
+    assert ws(p, 64, p, p, 1000, 4, 64, 33) > 0     # gathered rows
+    assert ws(p, 65, p, p, 60, 4, 65, 33) == 0      # few rows are read where they are
+    back = capi.lib().lgbm_b200_experts_matmul_backward_workspace
+    one = back(p, 33, p, 64, None, p, 1000, 4, 64, 33, 1, 0)
+    assert one > 0 and back(p, 33, p, 64, None, p, 1000, 4, 64, 33, 1, 1) == one  # dy once
+    assert back(p, 40, p, 64, None, p, 1000, 4, 64, 33, 1, 1) == 0
