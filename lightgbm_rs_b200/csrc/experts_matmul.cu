@@ -33,6 +33,12 @@
 // next group cannot make 0 * inf. In a pair each CTA's second warp does that to its own half
 // and the odd one tells the even one. (Gathering that block's rows one by one, with zeros
 // from TMA for those outside, took five times a block's time, once a tile.)
+// Precision. The tensor cores cut a sum off when they add to it: on sums of random signs the
+// error grew with the length, 1.5e-5 of the result at 4096 rows (f32 sums in another order: 9e-7).
+// A result rounded to 16 bits does not show it. A weight gradient kept in f32 would, so there
+// the reduction is accumulated in runs of 768 rows, alternating between the two halves of
+// tensor memory, and the storing warps, twice as many there so that the sums fit their
+// registers, add the runs up in f32: 7e-7 whatever the length.
 #include <algorithm>
 #include <atomic>
 #include <mutex>
@@ -45,16 +51,14 @@ namespace lgbm_b200 {
 namespace experts {
 namespace {
 
-constexpr int kStoreWarps = 8;     // warps 2..9 write results out
-constexpr int kMatThreads = 64 + 32 * kStoreWarps;  // warp 0 loads, warp 1 multiplies
 constexpr int kTileM = 128;       // rows of D of a CTA
 constexpr int kTileK = 64;         // 128 bytes of a 16-bit type: one swizzle row
 constexpr int kStoreRow = 64;      // bytes of a row in a storing warp's staging block
-constexpr int kStoreBytes = kStoreWarps * 32 * kStoreRow;
 constexpr int kBandRows = 2048;    // rows of D of a band, see tile_of
 constexpr uint64_t kWaitNs = 2000000000;
 
-enum Mode { FORWARD = 0, INPUT = 1, WEIGHT = 2 };
+enum Mode { FORWARD = 0, INPUT = 1, WEIGHT = 2, WEIGHT_F32 = 3 };
+constexpr int kRun = 768;  // rows of a run of WEIGHT_F32
 
 struct MatArgs {
   const int32_t* offsets;
@@ -267,14 +271,18 @@ __device__ __forceinline__ void tile_of(int t, int mt, int nt, int band, int& m,
   m = b * band + (r - n * h);
 }
 
-// CTAS CTAs share a tile of 128 CTAS rows and BN columns of D.
-template <int BN, int CTAS>
+// CTAS CTAs share a tile of 128 CTAS rows and BN columns of D. Warp 0 loads, warp 1
+// multiplies, the others write results out.
+template <int KIND, int BN, int CTAS>
 struct Shape {
+  static constexpr int kStoreWarps = KIND == WEIGHT_F32 ? 16 : 8;
+  static constexpr int kThreads = 64 + 32 * kStoreWarps;
+  static constexpr int kStoreBytes = kStoreWarps * 32 * kStoreRow;
   static constexpr int kRows = kTileM * CTAS;
   static constexpr int kCols = BN / CTAS;  // columns of B that a CTA loads
   static constexpr int kStageBytes = (kTileM + kCols) * 128;
-  static constexpr int kStages = 196608 / kStageBytes;  // 4, 6 or 8: 192 KB
-  static constexpr int kTmemCols = 2 * BN;              // two accumulators
+  static constexpr int kStages = (212992 - kStoreBytes) / kStageBytes;  // 3 to 8
+  static constexpr int kTmemCols = 2 * BN;                              // two accumulators
   static constexpr int kBand = kBandRows / kRows;
   static constexpr int kSmem =
       1024 + kStages * kStageBytes + kStoreBytes + 8 * (kMaxExperts + 2) + 512;
@@ -333,10 +341,12 @@ struct Maps {
   CUtensorMap out;   // 32 rows of 64 bytes
 };
 
-template <int MODE, int BN, int CTAS>
-__global__ void __launch_bounds__(kMatThreads, 1)
+template <int KIND, int BN, int CTAS>
+__global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     k_grouped_matmul(const __grid_constant__ Maps maps, const MatArgs g) {
-  using S = Shape<BN, CTAS>;
+  using S = Shape<KIND, BN, CTAS>;
+  constexpr int MODE = KIND == WEIGHT_F32 ? (int)WEIGHT : KIND;
+  constexpr bool kRuns = KIND == WEIGHT_F32;
   constexpr int kStages = S::kStages;
   constexpr uint32_t kABytes = kTileM * 128;
   extern __shared__ uint8_t smem_raw[];
@@ -344,7 +354,7 @@ __global__ void __launch_bounds__(kMatThreads, 1)
   uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const uint32_t base = smem_addr(smem);
   const uint32_t store_base = base + kStages * S::kStageBytes;
-  int32_t* cum = reinterpret_cast<int32_t*>(smem + kStages * S::kStageBytes + kStoreBytes);
+  int32_t* cum = reinterpret_cast<int32_t*>(smem + kStages * S::kStageBytes + S::kStoreBytes);
   int32_t* off = cum + kMaxExperts + 2;  // the groups' first rows, then the end
   uint64_t* bars = reinterpret_cast<uint64_t*>(
       (reinterpret_cast<uintptr_t>(off + kMaxExperts + 2) + 15) & ~(uintptr_t)15);
@@ -367,7 +377,7 @@ __global__ void __launch_bounds__(kMatThreads, 1)
       }
       for (int i = 0; i < 2; ++i) {
         bar_init(acc_full + 8 * i, 1);
-        bar_init(acc_empty + 8 * i, kStoreWarps * CTAS);
+        bar_init(acc_empty + 8 * i, S::kStoreWarps * CTAS);
       }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
@@ -512,16 +522,20 @@ __global__ void __launch_bounds__(kMatThreads, 1)
       if (ends > 0) bar_wait(end_full + 8 * ((ends - 1) % kStages), ((ends - 1) / kStages) & 1);
     }
   } else if (warp == 1) {
-    uint32_t it = 0, tile = 0, ends = 0;
+    uint32_t it = 0, tile = 0, ends = 0;  // tile: accumulations so far, one or more a tile
     for (int t = first; ok && t < tiles; t += step) {
       const Tile r = decode(t);
-      if (r.red == 0) continue;
-      const uint32_t acc = tile & 1, d = tmem + acc * BN;
-      if (rank == 0) {
-        if (tile >= 2 && !(ok = bar_wait(acc_empty + 8 * acc, (tile / 2 - 1) & 1))) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      }
+      uint32_t acc = 0, d = 0;
       for (int k0 = 0; k0 < r.red; k0 += kTileK, ++it) {
+        const bool begin = kRuns ? k0 % kRun == 0 : k0 == 0;
+        if (begin) {
+          acc = tile & 1;
+          d = tmem + acc * BN;
+          if (rank == 0) {
+            if (tile >= 2 && !(ok = bar_wait(acc_empty + 8 * acc, (tile / 2 - 1) & 1))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          }
+        }
         const uint32_t s = it % kStages;
         const uint32_t a = base + s * S::kStageBytes, b = a + kABytes;
         // the last block in whole steps of 16
@@ -545,6 +559,8 @@ __global__ void __launch_bounds__(kMatThreads, 1)
             break;
           }
         }
+        const bool done = k0 + kTileK >= r.red || (kRuns && (k0 + kTileK) % kRun == 0);
+        if (done) ++tile;
         if (rank == 1) continue;  // the even CTA multiplies for both
         if (!(ok = bar_wait(full + 8 * s, (it / kStages) & 1))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -555,34 +571,37 @@ __global__ void __launch_bounds__(kMatThreads, 1)
                                                : smem_desc(a + k * 32, 16, 1024);
             const uint64_t db = MODE == FORWARD ? smem_desc(b + k * 32, 16, 1024)
                                                 : smem_desc(b + k * 2048, 8192, 1024);
-            mma_f16<CTAS>(d, da, db, g.idesc, k0 > 0 || k > 0);
+            mma_f16<CTAS>(d, da, db, g.idesc, !begin || k > 0);
           }
           mma_commit<CTAS>(empty + 8 * s);
+          if (done) mma_commit<CTAS>(acc_full + 8 * acc);
         }
         __syncwarp();
       }
-      if (!ok) break;
-      if (rank == 0 && elect_one()) mma_commit<CTAS>(acc_full + 8 * acc);
-      __syncwarp();
-      ++tile;
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;  // of the lanes; of the chunks
+    const int quarter = warp & 3, part = (warp - 2) >> 2;  // of the lanes; of the chunks
+    constexpr int kParts = S::kStoreWarps / 4;
     const uint32_t stage = store_base + (warp - 2) * 32 * kStoreRow;
-    const bool wide = g.out_kind == LGBM_B200_DTYPE_F32;
-    const int bytes = wide ? 4 : 2;
-    const int per_chunk = kStoreRow / bytes;  // columns of a staging row
+    constexpr int bytes = kRuns ? 4 : 2;
+    constexpr int per_chunk = kStoreRow / bytes;  // columns of a staging row
     const int64_t pitch = g.out_pitch * bytes;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    auto accumulated = [&](uint32_t tile) {  // accumulation `tile` is complete
+      if (!bar_wait(acc_full + 8 * (tile & 1), (tile / 2) & 1)) return false;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      return true;
+    };
+    auto release = [&](uint32_t tile) {  // and has been read
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      const uint32_t bar = acc_empty + 8 * (tile & 1);
+      if (lane == 0) bar_arrive_cluster(CTAS == 2 ? leader_addr(bar) : bar);
+    };
     uint32_t tile = 0;
     for (int t = first; ok && t < tiles; t += step) {
       const Tile r = decode(t);
-      const uint32_t acc = tile & 1;
-      if (r.red > 0) {
-        if (!(ok = bar_wait(acc_full + 8 * acc, (tile / 2) & 1))) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      }
       const int row0 = r.m0 + quarter * 32;
-      const uint32_t from = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
       char* out = static_cast<char*>(g.out);
       int out_row = row0;  // of D as one matrix
       if (MODE == WEIGHT) {
@@ -592,26 +611,8 @@ __global__ void __launch_bounds__(kMatThreads, 1)
       const int ncols = min(BN, g.cols - r.n0), nrows = min(32, r.m_end - row0);
       // whole 32-row blocks leave by TMA, which also cuts off the last columns
       const bool by_tma = g.unit == 16 && nrows == 32;
-      for (int c0 = half * per_chunk; c0 < ncols && nrows > 0; c0 += 2 * per_chunk) {
-        // this lane's row of the chunk
-        uint32_t v[32], w[16];
-        if (r.red == 0) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = 0;
-        } else if (wide) {
-          tmem_load16(from + c0, w);
-          tmem_wait();
-        } else {
-          tmem_load32(from + c0, v);
-          tmem_wait();
-          if (g.out_kind == LGBM_B200_DTYPE_BF16) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = pack2<true>(v[2 * i], v[2 * i + 1]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = pack2<false>(v[2 * i], v[2 * i + 1]);
-          }
-        }
+      // this lane's row of a chunk, 64 bytes, through the staging block to D
+      auto put = [&](const uint32_t* w, int c0) {
         // the staging block is free when the last store has read it
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
@@ -640,13 +641,58 @@ __global__ void __launch_bounds__(kMatThreads, 1)
           else store_rows<2>(stage, dst, pitch, nrows, n, lane);
         }
         __syncwarp();
-      }
-      if (r.red > 0) {
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0)
-          bar_arrive_cluster(CTAS == 2 ? leader_addr(acc_empty + 8 * acc) : acc_empty + 8 * acc);
-        ++tile;
+      };
+      if (kRuns && r.red > kRun) {
+        constexpr int kMine = BN / per_chunk / kParts;  // chunks of this warp
+        uint32_t sum[kMine][16];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sum[i][j] = 0;
+        for (int k0 = 0; k0 < r.red; k0 += kRun, ++tile) {
+          if (!(ok = accumulated(tile))) break;
+          const uint32_t from = tmem + (tile & 1) * BN + lanes + part * per_chunk;
+#pragma unroll
+          for (int i = 0; i < kMine; ++i) {
+            uint32_t v[16];
+            tmem_load16(from + i * kParts * per_chunk, v);
+            tmem_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              sum[i][j] = __float_as_uint(__uint_as_float(sum[i][j]) + __uint_as_float(v[j]));
+          }
+          release(tile);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+          if ((i * kParts + part) * per_chunk < ncols && nrows > 0)
+            put(sum[i], (i * kParts + part) * per_chunk);
+      } else {
+        if (r.red > 0 && !(ok = accumulated(tile))) break;
+        const uint32_t from = tmem + (tile & 1) * BN + lanes;
+        for (int c0 = part * per_chunk; c0 < ncols && nrows > 0; c0 += kParts * per_chunk) {
+          uint32_t v[32], w[16];
+          if (r.red == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = 0;
+          } else if constexpr (kRuns) {
+            tmem_load16(from + c0, w);
+            tmem_wait();
+          } else {
+            tmem_load32(from + c0, v);
+            tmem_wait();
+            if (g.out_kind == LGBM_B200_DTYPE_BF16) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = pack2<true>(v[2 * i], v[2 * i + 1]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = pack2<false>(v[2 * i], v[2 * i + 1]);
+            }
+          }
+          put(w, c0);
+        }
+        if (r.red > 0) release(tile++);
       }
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -759,9 +805,9 @@ struct DeviceInfo {
 };
 DeviceInfo g_devices[kMaxDevices];
 
-template <int MODE, int BN, int CTAS>
+template <int KIND, int BN, int CTAS>
 cudaError_t launch_tiles(const Maps& maps, MatArgs g, int64_t most_tiles, cudaStream_t st) {
-  using S = Shape<BN, CTAS>;
+  using S = Shape<KIND, BN, CTAS>;
   static std::atomic<int> most_ready[kMaxDevices];  // tiles at work at a time; 0: not set up
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
@@ -780,7 +826,7 @@ cudaError_t launch_tiles(const Maps& maps, MatArgs g, int64_t most_tiles, cudaSt
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(CTAS, 1, 1);
-  cfg.blockDim = dim3(kMatThreads, 1, 1);
+  cfg.blockDim = dim3(S::kThreads, 1, 1);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -791,11 +837,11 @@ cudaError_t launch_tiles(const Maps& maps, MatArgs g, int64_t most_tiles, cudaSt
   cfg.numAttrs = CTAS == 2 ? 1 : 0;
   int most = most_ready[dev].load(std::memory_order_acquire);
   if (most == 0) {
-    err = cudaFuncSetAttribute(k_grouped_matmul<MODE, BN, CTAS>,
+    err = cudaFuncSetAttribute(k_grouped_matmul<KIND, BN, CTAS>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     // a pair that finds no room would start when the others have finished: ask how many fit
     if (err == cudaSuccess && CTAS == 2)
-      err = cudaOccupancyMaxActiveClusters(&most, k_grouped_matmul<MODE, BN, CTAS>, &cfg);
+      err = cudaOccupancyMaxActiveClusters(&most, k_grouped_matmul<KIND, BN, CTAS>, &cfg);
     else if (err == cudaSuccess)
       err = cudaDeviceGetAttribute(&most, cudaDevAttrMultiProcessorCount, dev);
     if (err != cudaSuccess) return err;
@@ -803,7 +849,7 @@ cudaError_t launch_tiles(const Maps& maps, MatArgs g, int64_t most_tiles, cudaSt
     most_ready[dev].store(most, std::memory_order_release);
   }
   cfg.gridDim.x = (unsigned)(std::min<int64_t>(most, most_tiles) * CTAS);
-  return cudaLaunchKernelEx(&cfg, k_grouped_matmul<MODE, BN, CTAS>, maps, g);
+  return cudaLaunchKernelEx(&cfg, k_grouped_matmul<KIND, BN, CTAS>, maps, g);
 }
 
 // An operand as TMA can read it: 16-byte base and pitches, or a copy in the workspace.
@@ -857,7 +903,7 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
   g.unit = bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
   auto go = [&](auto bn_c, auto ctas_c) -> cudaError_t {
     constexpr int BN = decltype(bn_c)::value, CTAS = decltype(ctas_c)::value;
-    using S = Shape<BN, CTAS>;
+    using S = Shape<MODE, BN, CTAS>;
     Maps maps;
     const int64_t da[3] = {a_width, g.rows, 1}, pa[2] = {a.pitch, 0};
     bool fine = encode(&maps.a, dtype, a.p, 2, da, pa, MODE == WEIGHT ? 64 : kTileM);
@@ -882,6 +928,8 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
     const int64_t most = MODE == WEIGHT
                              ? (int64_t)g.experts * ((g.drows + S::kRows - 1) / S::kRows) * nt
                              : (g.rows / S::kRows + g.experts + 1) * nt;
+    if (MODE == WEIGHT && g.out_kind == LGBM_B200_DTYPE_F32)
+      return launch_tiles<WEIGHT_F32, BN, CTAS>(maps, g, most, st);
     return launch_tiles<MODE, BN, CTAS>(maps, g, most, st);
   };
   using One = std::integral_constant<int, 1>;

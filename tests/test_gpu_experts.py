@@ -230,6 +230,23 @@ def test_products(ops, counts, tail, inner, outer, dtype):
         close(dwf[e], want, counts[e] * 2.0 ** -23 * mag)
 
 
+@pytest.mark.parametrize("inner,outer", [(264, 200), (64, 64), (130, 129)])
+def test_weight_gradient_in_32_bits_stays_precise(ops, inner, outer):
+    """n rows summed in runs of 768, each in 48 steps that cut off at most 2^-23 of the sum,
+    the runs added with a rounding of 2^-24 each: for random signs, in the 2-norm, at most
+    (48 + n / 1536) 2^-23 of the result. One sum of n / 16 steps would be off by more."""
+    g = gen(31)
+    n = 9000
+    x = torch.randn(n, inner, generator=g, device="cuda").to(torch.bfloat16)
+    dy = torch.randn(n, outer, generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.zeros(2, outer, inner, device="cuda", dtype=torch.bfloat16)
+    off = offsets_of([0, n])
+    dw = ops.grouped_matmul_backward(dy, x, w, off, need_dx=False, grad_dtype=torch.float32)[1]
+    want = dy.double().T @ x.double()
+    assert float((dw[1].double() - want).norm() / want.norm()) < (48 + n / 1536) * 2.0 ** -23
+    assert not dw[0].any()
+
+
 @pytest.mark.parametrize("counts", [[70, 0, 9, 130], [700, 0, 70, 333]])
 @pytest.mark.parametrize("inner,outer", [(96, 80), (75, 50), (264, 392), (130, 300)])
 def test_products_through_rows(ops, inner, outer, counts):
