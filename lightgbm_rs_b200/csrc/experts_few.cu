@@ -111,6 +111,15 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const ui
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// (w & mask) | magic in one instruction: with both constants in registers. As immediates they
+// took two, and the kernel is bound by the integer pipe (16 rows of 32 x 4096 x 2000: 55 us
+// against 51).
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
+  return r;
+}
+
 template <typename T>
 struct Magic;
 template <>
@@ -121,6 +130,19 @@ template <>
 struct Magic<__nv_bfloat16> {
   static constexpr uint32_t kBits = 0x4300;  // 128: the low 7 bits count ones
 };
+
+// The low (h = 0) or high half of a word as f32.
+template <typename T>
+__device__ __forceinline__ float half_of(uint32_t w, int h);
+template <>
+__device__ __forceinline__ float half_of<__nv_bfloat16>(uint32_t w, int h) {
+  return __uint_as_float(h ? w & 0xFFFF0000u : w << 16);
+}
+template <>
+__device__ __forceinline__ float half_of<__half>(uint32_t w, int h) {
+  const __half2 v = *reinterpret_cast<__half2*>(&w);
+  return h ? __high2float(v) : __low2float(v);
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b);
@@ -287,14 +309,23 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
                        ? g.groups - (k_begin >> SHIFT) - scale_col : 0;
   auto fetch_scales = [&] {  // of the next stage
     if constexpr (W4) {
+      if (scale_left >= S::kScaleLane) {
 #pragma unroll
-      for (int j = 0; j < S::kScaleLane; ++j) {
-        next_scale[j] = 0;
-        next_zero[j] = 8;
-        if (j < scale_left) {
+        for (int j = 0; j < S::kScaleLane; ++j) {
           asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(next_scale[j]) : "l"(scale_src + j));
           if constexpr (S::ZEROS)
             asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(next_zero[j]) : "l"(zero_src + j));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < S::kScaleLane; ++j) {
+          next_scale[j] = 0;
+          next_zero[j] = 8;
+          if (j < scale_left) {
+            asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(next_scale[j]) : "l"(scale_src + j));
+            if constexpr (S::ZEROS)
+              asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(next_zero[j]) : "l"(zero_src + j));
+          }
         }
       }
       scale_src += S::kGroups;
@@ -328,6 +359,10 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   // in registers until the panel before is done with.
   constexpr int kPieces = S::kMaxPanel / 8 / 32;
   uint4 next_tokens[TILES][kPieces];
+#pragma unroll
+  for (int q = 0; q < TILES; ++q)
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) next_tokens[q][p] = make_uint4(0, 0, 0, 0);
   const uint16_t* token_row[TILES];
 #pragma unroll
   for (int q = 0; q < TILES; ++q) {
@@ -340,12 +375,13 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   }
   auto fetch_tokens = [&](int k0) {
 #pragma unroll
-    for (int q = 0; q < TILES; ++q)
+    for (int q = 0; q < TILES; ++q) {
+      if (!token_row[q]) continue;
 #pragma unroll
       for (int p = 0; p < kPieces; ++p) {
         const int k = k0 + (lane + 32 * p) * 8;
         next_tokens[q][p] = make_uint4(0, 0, 0, 0);
-        if (token_row[q] && k < k_end && (lane + 32 * p) * 8 < g.panel) {
+        if (k < k_end && (lane + 32 * p) * 8 < g.panel) {
           if (g.x_vec && k + 8 <= k_end) {
             next_tokens[q][p] = __ldg(reinterpret_cast<const uint4*>(token_row[q] + k));
           } else {
@@ -357,11 +393,12 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
           }
         }
       }
+    }
   };
-  auto keep_tokens = [&] {
+  auto keep_tokens = [&](bool first) {
 #pragma unroll
     for (int q = 0; q < TILES; ++q)
-      if (q < tiles)
+      if (token_row[q] || (first && q < tiles))  // rows of zeros stay
 #pragma unroll
         for (int p = 0; p < kPieces; ++p) {
           uint4 v = next_tokens[q][p];
@@ -385,13 +422,16 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   fetch_tokens(k_begin);
   keep_scales(0);
 
+  uint32_t mask, magic;
+  asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(mask));
+  asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(Magic<T>::kBits * 0x10001u));
   int kp = g.panel;  // inner position in the panel
   int slot = 0;      // stage of the ring to multiply next
   for (int i = 0; i < stages; ++i, kp += S::kStageInner) {
     if (kp == g.panel) {
       kp = 0;
       if (i > 0) __syncthreads();
-      keep_tokens();
+      keep_tokens(i == 0);
       __syncthreads();
       fetch_tokens(k_begin + i * S::kStageInner + g.panel);
     }
@@ -409,46 +449,58 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
       const uint16_t* zeros =
           reinterpret_cast<const uint16_t*>(scale_sets + (2 + (i & 1)) * S::kScaleBytes);
       constexpr int kSteps = (1 << SHIFT) / 32;  // of 32 in a scale group
-#pragma unroll(TILES == 1 ? 8 : 1)
-      for (int j0 = 0; j0 < S::kStageInner / 32; j0 += kSteps) {
-        const int lo = gq * S::kScalePitch + j0 / kSteps, hi = lo + 8 * S::kScalePitch;
-        uint32_t zl = (Magic<T>::kBits + 8) * 0x10001u, zh = zl;
+#pragma unroll(TILES == 1 ? 4 : 1)
+      for (int g2 = 0; g2 < S::kGroups; g2 += 2) {  // two scale groups: a word of each kind
+        const int lo = gq * S::kScalePitch + g2, hi = lo + 8 * S::kScalePitch;
+        const uint32_t sl2 = *reinterpret_cast<const uint32_t*>(scales + lo);
+        const uint32_t sh2 = *reinterpret_cast<const uint32_t*>(scales + hi);
+        uint32_t zl2 = 0, zh2 = 0;
         if constexpr (S::ZEROS) {
-          zl = zeros[lo] * 0x10001u;
-          zh = zeros[hi] * 0x10001u;
+          zl2 = *reinterpret_cast<const uint32_t*>(zeros + lo);
+          zh2 = *reinterpret_cast<const uint32_t*>(zeros + hi);
         }
-        float part[TILES][4];
 #pragma unroll
-        for (int n = 0; n < TILES; ++n)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) part[n][q] = 0.0f;
-#pragma unroll
-        for (int j = j0; j < j0 + kSteps; ++j) {
-          const uint32_t wl = *reinterpret_cast<const uint32_t*>(a_at + j * 16);
-          const uint32_t wh = *reinterpret_cast<const uint32_t*>(a_at + j * 16 + 8 * kRowPitch);
-          uint32_t pl[4], ph[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            pl[q] = sub2<T>(((wl >> (4 * q)) & 0x000F000Fu) | Magic<T>::kBits * 0x10001u, zl);
-            ph[q] = sub2<T>(((wh >> (4 * q)) & 0x000F000Fu) | Magic<T>::kBits * 0x10001u, zh);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t zl = (Magic<T>::kBits + 8) * 0x10001u, zh = zl;
+          if constexpr (S::ZEROS) {
+            zl = __byte_perm(zl2, 0, h ? 0x3232 : 0x1010);
+            zh = __byte_perm(zh2, 0, h ? 0x3232 : 0x1010);
           }
-          const uint32_t a0[4] = {pl[0], ph[0], pl[1], ph[1]}, a1[4] = {pl[2], ph[2], pl[3], ph[3]};
+          float part[TILES][4];
 #pragma unroll
-          for (int n = 0; n < TILES; ++n) {
-            if (TILES == 1 || n < tiles) {
-              const uint4 b = *reinterpret_cast<const uint4*>(b_at + n * 8 * tpitch + j * 64);
-              mma_16816<T>(part[n], a0, b.x, b.y);
-              mma_16816<T>(part[n], a1, b.z, b.w);
+          for (int n = 0; n < TILES; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) part[n][q] = 0.0f;
+#pragma unroll
+          for (int i2 = 0; i2 < kSteps; ++i2) {
+            const int j = (g2 + h) * kSteps + i2;
+            const uint32_t wl = *reinterpret_cast<const uint32_t*>(a_at + j * 16);
+            const uint32_t wh = *reinterpret_cast<const uint32_t*>(a_at + j * 16 + 8 * kRowPitch);
+            uint32_t pl[4], ph[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              pl[q] = sub2<T>(and_or(wl >> (4 * q), mask, magic), zl);
+              ph[q] = sub2<T>(and_or(wh >> (4 * q), mask, magic), zh);
+            }
+            const uint32_t a0[4] = {pl[0], ph[0], pl[1], ph[1]},
+                           a1[4] = {pl[2], ph[2], pl[3], ph[3]};
+#pragma unroll
+            for (int n = 0; n < TILES; ++n) {
+              if (TILES == 1 || n < tiles) {
+                const uint4 b = *reinterpret_cast<const uint4*>(b_at + n * 8 * tpitch + j * 64);
+                mma_16816<T>(part[n], a0, b.x, b.y);
+                mma_16816<T>(part[n], a1, b.z, b.w);
+              }
             }
           }
-        }
-        const float sl = to_f32<T>(scales[lo]), sh = to_f32<T>(scales[hi]);
+          const float sl = half_of<T>(sl2, h), sh = half_of<T>(sh2, h);
 #pragma unroll
-        for (int n = 0; n < TILES; ++n) {
-          acc[n][0] = fmaf(sl, part[n][0], acc[n][0]);
-          acc[n][1] = fmaf(sl, part[n][1], acc[n][1]);
-          acc[n][2] = fmaf(sh, part[n][2], acc[n][2]);
-          acc[n][3] = fmaf(sh, part[n][3], acc[n][3]);
+          for (int n = 0; n < TILES; ++n) {
+            acc[n][0] = fmaf(sl, part[n][0], acc[n][0]);
+            acc[n][1] = fmaf(sl, part[n][1], acc[n][1]);
+            acc[n][2] = fmaf(sh, part[n][2], acc[n][2]);
+            acc[n][3] = fmaf(sh, part[n][3], acc[n][3]);
+          }
         }
       }
     } else {
