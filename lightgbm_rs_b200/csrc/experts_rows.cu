@@ -147,11 +147,13 @@ constexpr int kDropUnroll = 2;  // blocks of eight elements a thread
 // passes; drop 0 would need -1 and is a flag.) A dropped element is 0 whatever it held. A
 // thread makes kDropUnroll blocks and handles their eight elements each, all loads first.
 // VEC: rows of one pitch that 16-byte accesses can walk; a contiguous array is one row.
-template <typename T, bool VEC, bool RES>
-__global__ void __launch_bounds__(kRowThreads)
-    k_dropout(const T* __restrict__ x, const T* residual, int64_t n, int64_t width,
-              int64_t pitch, int64_t residual_pitch, uint32_t cut, bool all, float scale,
-              uint32_t k0, uint32_t k1, uint64_t offset, T* out) {
+// FULL: no end of the array inside the block of threads.
+template <typename T, bool VEC, bool RES, bool FULL>
+__device__ __forceinline__ void drop_block(const T* __restrict__ x, const T* __restrict__ residual,
+                                           int64_t n, int64_t width, int64_t pitch,
+                                           int64_t residual_pitch, uint32_t cut, bool all,
+                                           float scale, uint32_t k0, uint32_t k1,
+                                           uint64_t offset, T* __restrict__ out) {
   constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
   constexpr int kParts = 8 / V;
   const int64_t b0 = (int64_t)blockIdx.x * (kRowThreads * kDropUnroll) + threadIdx.x;
@@ -162,14 +164,14 @@ __global__ void __launch_bounds__(kRowThreads)
 #pragma unroll
     for (int h = 0; h < kParts; ++h) {
       const int64_t i = i0 + h * V;
-      if (i < n) {
+      if (FULL || i < n) {
         int64_t at = i, rat = i;
-        if (width != n) {
+        if (!FULL && width != n) {
           const int64_t r = i / width, c = i - r * width;
           at = r * pitch + c;
           rat = r * residual_pitch + c;
         }
-        if (i + V <= n) {
+        if (FULL || i + V <= n) {
           v[u][h].load(x + at);
           if constexpr (RES) a[u][h].load(residual + rat);
         } else {
@@ -182,25 +184,25 @@ __global__ void __launch_bounds__(kRowThreads)
 #pragma unroll
   for (int u = 0; u < kDropUnroll; ++u) {
     const int64_t b = b0 + u * kRowThreads;
-    if (b * 8 >= n) break;
+    if (!FULL && b * 8 >= n) break;
     const uint4 rnd = philox((uint64_t)b, offset, k0, k1);
     const uint32_t words[4] = {rnd.x, rnd.y, rnd.z, rnd.w};
 #pragma unroll
     for (int h = 0; h < kParts; ++h) {
-      if (b * 8 + h * V >= n) break;
+      const int64_t at = b * 8 + h * V;
+      if (!FULL && at >= n) break;
       float e[V], r[V];
       v[u][h].get(e);
       if constexpr (RES) a[u][h].get(r);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int at = h * V + i;
-        const uint32_t w = (at & 1) ? words[at / 2] : words[at / 2] << 16;
+        const int j = h * V + i;
         // a low half has zeros below it after the shift: above cut means at least drop * 2^16
+        const uint32_t w = (j & 1) ? words[j / 2] : words[j / 2] << 16;
         e[i] = all || w > cut ? e[i] * scale : 0.0f;
         if constexpr (RES) e[i] += r[i];
       }
-      const int64_t at = b * 8 + h * V;
-      if (at + V <= n) {
+      if (FULL || at + V <= n) {
         Raw<T, V>::store(out + at, e);
       } else {
 #pragma unroll
@@ -209,6 +211,20 @@ __global__ void __launch_bounds__(kRowThreads)
       }
     }
   }
+}
+
+template <typename T, bool VEC, bool RES>
+__global__ void __launch_bounds__(kRowThreads)
+    k_dropout(const T* __restrict__ x, const T* __restrict__ residual, int64_t n, int64_t width,
+              int64_t pitch, int64_t residual_pitch, uint32_t cut, bool all, float scale,
+              uint32_t k0, uint32_t k1, uint64_t offset, T* __restrict__ out) {
+  const int64_t end = ((int64_t)blockIdx.x + 1) * (kRowThreads * kDropUnroll * 8);
+  if (VEC && width == n && end <= n)
+    drop_block<T, VEC, RES, VEC>(x, residual, n, width, pitch, residual_pitch, cut, all, scale,
+                                 k0, k1, offset, out);
+  else
+    drop_block<T, VEC, RES, false>(x, residual, n, width, pitch, residual_pitch, cut, all, scale,
+                                   k0, k1, offset, out);
 }
 
 // Threads that share a token's row: the smallest power of two that covers it, 32 to 256.
