@@ -33,12 +33,22 @@
 // next group cannot make 0 * inf. In a pair each CTA's second warp does that to its own half
 // and the odd one tells the even one. (Gathering that block's rows one by one, with zeros
 // from TMA for those outside, took five times a block's time, once a tile.)
+//
 // Precision. The tensor cores cut a sum off when they add to it: on sums of random signs the
-// error grew with the length, 1.5e-5 of the result at 4096 rows (f32 sums in another order: 9e-7).
-// A result rounded to 16 bits does not show it. A weight gradient kept in f32 would, so there
-// the reduction is accumulated in runs of 768 rows, alternating between the two halves of
-// tensor memory, and the storing warps, twice as many there so that the sums fit their
-// registers, add the runs up in f32: 7e-7 whatever the length.
+// error grew with the length, 1.5e-5 of the result at 4096 rows (f32 sums in another order:
+// 2e-7 to 9e-7). A result rounded to 16 bits does not show it. A weight gradient kept in f32
+// would, so there the reduction is accumulated in runs of 768 rows, alternating between the
+// two halves of tensor memory, and the storing warps, twice as many there so that the sums fit
+// their registers, add the runs up in f32: 7e-7 whatever the length.
+//
+// Measured, loops on a warm GPU: 65536 rows, 16 experts of 4096 x 2048: y 0.90, dx 0.90, dw
+// 0.90 (bf16) and 1.04 ms (f32), 1.2 PFLOP/s with the clock held near 1.3 GHz by the power
+// cap; cuBLAS's batched product of the same size 0.83, 0.80, 0.80. 8192 rows, 8 experts of
+// 4096 x 1024: 68, 68, 68 us against 66, 60, 65 (1.0 PFLOP/s); tensor pipe 60 % busy; the rest
+// is the last wave, tiles that groups of 1024 and a few rows leave partly empty, and loads at
+// the 64 bytes a cycle that an SM takes from L2. 40009 rows, 255 experts of 136 x 704: y 33,
+// dx 47, dw 51 and 67 us, 2 to 3 TB/s: two or three blocks of reduction a tile, bound by
+// writing tiles out.
 #include <algorithm>
 #include <atomic>
 #include <mutex>
@@ -713,10 +723,11 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
   }
 }
 
+// 40009 rows of 700 f16 (112 MB read and written): 22 us, 5.1 TB/s.
 // Rows copied to a pitch that TMA can walk: dst[r] = src[index ? index[r] : r], the columns
 // between `width` and `dst_pitch` zero; a row whose index is outside is zero.
 // UNIT bytes of a row are read at a time (its alignment), 16 written; a thread takes kStageRun
-// pieces, all loads first.
+// pieces, all loads first. 40009 rows of 700 f16: 22 us, 112 MB at 5.1 TB/s.
 constexpr int kStageRun = 4;
 
 template <int UNIT>
@@ -936,6 +947,9 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
   using Two = std::integral_constant<int, 2>;
   if (g.cols <= 64) return go(std::integral_constant<int, 64>(), One());
   if (g.cols <= 128) return go(std::integral_constant<int, 128>(), One());
+  // Pairs where most tiles fill more than one CTA's rows. (157 rows an expert on average, 255
+  // of 136 x 704: y 33 us either way, dw 62 in pairs, 68 without; fewer rows than a CTA's
+  // would leave the odd CTA idle.)
   const bool tall = MODE == WEIGHT ? g.drows > kTileM : g.rows >= (int64_t)kTileM * g.experts;
   return tall ? go(std::integral_constant<int, 256>(), Two())
               : go(std::integral_constant<int, 256>(), One());

@@ -219,6 +219,10 @@ constexpr int kSelectTokens = 128;  // of a block: 16 a warp, one after the othe
 // before all of its own; their k * NV logits are dealt out to the 32 lanes, CN each, and the
 // k choices are made there, each one a maximum over the warp, the first expert that holds
 // it, and its removal. Keys order as the logits do, with NaN above everything.
+// Bound by instructions: 65521 rows of 255 f32 logits, k 4, take 41 us (67 MB: 1.6 TB/s) with
+// 438 instructions a row and three quarters of the issue slots used. A sorted list a thread
+// in registers (select_tokens with one lane a token) took 71 us, a search of all registers a
+// choice 64.
 template <typename T, int NV, int CN>
 __global__ void __launch_bounds__(kSelectThreads)
     k_route_select(const T* logits, int64_t tokens, int experts, int64_t pitch, int k,
@@ -363,7 +367,8 @@ __global__ void __launch_bounds__(256) k_route_scan(int32_t* counts, int32_t* to
   if (lane == 0) totals[e] = carry;
 }
 
-// Third: offsets, and every slot's place.
+// Third: offsets, and every slot's place. 8 us at 262084 slots and 255 experts (the scan 3):
+// latency, not bandwidth; its 2 MB of results go to 255 ranges.
 __global__ void __launch_bounds__(kRouteThreads)
     k_route_place(const int32_t* chosen, const int32_t* counts, const int32_t* totals,
                   int64_t tokens, int experts, int k, int block_tokens, int32_t* position,
@@ -387,7 +392,8 @@ __global__ void __launch_bounds__(kRouteThreads)
       n, first * k, experts, k, [&](int i) { return mine[i]; }, base, hist, position, rows);
 }
 
-// A few tokens: all of it in one block, 32 lanes a token.
+// A few tokens: all of it in one block and one launch, 32 lanes a token. One row of 8
+// experts: 3.5 us, of which the launch is most.
 constexpr int kSmallThreads = 512;
 constexpr int kSmallTokens = 64;  // most tokens this path takes: four rounds of 16
 
@@ -425,12 +431,13 @@ __global__ void __launch_bounds__(kSmallThreads)
       tokens * k, 0, experts, k, [&](int i) { return ids[i]; }, base, hist, position, rows);
 }
 
-// Gradient of the logits, `lanes` lanes a token: with p the softmax (over the chosen experts
+// Gradient of the logits: with p the softmax (over the chosen experts
 // or over all) and g the gradient of the weights, dl_e = p_e ([e chosen] g_e - sum w g). For
 // a chosen expert p_e is its weight. Over all experts the others' p is recomputed from one
 // chosen logit: the first chosen one is the largest, m, and its weight is 1 / sum exp(l - m).
-// The row is written as if nothing were chosen, then the chosen places again.
-// LANES is at least k; NV experts a lane.
+// The row is written as if nothing were chosen, then the chosen places again. 65521 x 255 f32:
+// 20 us, 6.8 TB/s of the 134 MB it reads and writes (part of it from L2).
+// LANES lanes a token, at least k; NV experts a lane.
 template <typename T, int LANES, int NV>
 __global__ void __launch_bounds__(256)
     k_route_backward(const float* __restrict__ dweights, const float* __restrict__ weights,

@@ -9,7 +9,8 @@ namespace {
 constexpr int kRowThreads = 256;
 
 // out[t] = sum_j w[t, j] y[position[t, j]] in f32, rounded once. A row of `lanes` threads a
-// token; JC rows are read at a time, all loads before the first use.
+// token; JC rows are read at a time, all loads before the first use. Bound by memory: 16384
+// tokens of 4 rows of 2048 bf16 in 65 us, 336 MB at 5.2 TB/s (rows in random order).
 template <typename T, int V, int JC>
 __global__ void __launch_bounds__(kRowThreads)
     k_combine(const T* y, int64_t rows, int width, int64_t pitch, const int32_t* position,
@@ -46,7 +47,10 @@ __global__ void __launch_bounds__(kRowThreads)
 
 // dy[position[t, j]] = w[t, j] dout[t] and dw[t, j] = <dout[t], y[position[t, j]]>, JC chosen
 // rows at a time: dout is read once for them. The dot products are summed over the token's
-// lanes in a fixed order, so they do not change from run to run.
+// lanes in a fixed order, so they do not change from run to run. LANES: a warp a token, or a
+// block a token where that many warps would leave SMs idle (fewer than 16 an SM): with a
+// barrier a token the block took 168 us on 16384 x 4 x 2048 bf16, the warp takes 96 (604 MB at
+// 6.3 TB/s).
 template <typename T, int V, int LANES, int JC>
 __global__ void __launch_bounds__(kRowThreads)
     k_combine_backward(const T* dout, const T* y, int64_t rows, int width, int64_t dout_pitch,
@@ -138,7 +142,11 @@ __device__ __forceinline__ uint4 philox(uint64_t block, uint64_t offset, uint32_
   return make_uint4(c0, c1, c2, c3);
 }
 
-constexpr int kDropUnroll = 2;  // blocks of eight elements a thread
+// Blocks of eight elements a thread. Bound by memory: 32768 x 4096 bf16 take 87 us (537 MB at
+// 6.2 TB/s), with a residual 115 (805 MB at 7.0). The generator is about 60 of the 110
+// instructions of a block of eight; 32 bits an element instead of 16 would be two generators a
+// block and put the instructions above the memory's time.
+constexpr int kDropUnroll = 2;
 
 // Element i takes 16 bits of block i / 8 and is kept when they are at least `drop`: the mask
 // is recomputed wherever it is needed and never stored. With cut = drop * 2^16 - 1 a high
@@ -310,7 +318,6 @@ cudaError_t launch_combine_backward(const void* dout, const void* y, int32_t dty
     using Vec = std::integral_constant<int, V>;
     using Warp = std::integral_constant<int, 32>;
     using Block = std::integral_constant<int, kRowThreads>;
-    // A block a token while a warp a token would leave SMs without work.
     const bool wide = tokens < 148 * 16 && (width + (vec ? V : 1) - 1) / (vec ? V : 1) > 64;
     if (vec) return wide ? go(Vec(), Block()) : go(Vec(), Warp());
     return wide ? go(One(), Block()) : go(One(), Warp());
