@@ -948,7 +948,7 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
   if (g.cols <= 64) return go(std::integral_constant<int, 64>(), One());
   if (g.cols <= 128) return go(std::integral_constant<int, 128>(), One());
   // Pairs where most tiles fill more than one CTA's rows. (157 rows an expert on average, 255
-  // of 136 x 704: y 33 us either way, dw 62 in pairs, 68 without; fewer rows than a CTA's
+  // of 136 x 704: y 33 us either way, dw 54 in pairs, 68 without; fewer rows than a CTA's
   // would leave the odd CTA idle.)
   const bool tall = MODE == WEIGHT ? g.drows > kTileM : g.rows >= (int64_t)kTileM * g.experts;
   return tall ? go(std::integral_constant<int, 256>(), Two())

@@ -630,6 +630,89 @@ def test_same_bits_every_time_and_on_another_stream(ops):
     assert all(torch.equal(a, b) for a, b in zip(first, second))
 
 
+def test_layer_against_autograd(ops):
+    """A whole layer, tokens shared by two experts each, against torch's autograd in f64 on the
+    same bf16 weights. On the way to a gradient at most five results are rounded to bf16 (h, y,
+    dy, dh, dx), each by 2^-8 of itself at most: 5 * 2^-8 in the 2-norm."""
+    g = gen(44)
+    T, E, k, K, H, N = 150, 6, 2, 24, 40, 16
+    bf = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.bfloat16)  # noqa
+    x, w1, w2, dout = bf(T, K), bf(E, H, K) * 0.2, bf(E, N, H) * 0.2, bf(T, N)
+    logits = torch.randn(T, E, generator=g, device="cuda")
+    for normalize in (True, False):
+        r = ops.route(logits, k, normalize=normalize)
+        h = ops.grouped_matmul(x, w1, r.offsets, rows=r.rows)
+        y = ops.grouped_matmul(h, w2, r.offsets)
+        out = ops.combine(y, r.position, r.weights)
+        dy, dwt = ops.combine_backward(dout, y, r.position, r.weights)
+        dh, dw2 = ops.grouped_matmul_backward(dy, h, w2, r.offsets, grad_dtype=torch.float32)
+        dxs, dw1 = ops.grouped_matmul_backward(dh, x, w1, r.offsets, rows=r.rows,
+                                               grad_dtype=torch.float32)
+        got = [out, ops.combine(dxs, r.position), dw1, dw2,
+               ops.route_backward(dwt, logits, r, normalize=normalize)]
+        p = [t.double().requires_grad_() for t in (x, w1, w2, logits)]
+        e = r.experts.long()
+        soft = (p[3].gather(1, e) if normalize else p[3]).softmax(1)
+        wt = soft if normalize else soft.gather(1, e)
+        each = torch.einsum("tknh,tkh->tkn", p[2][e], torch.einsum("tkhc,tc->tkh", p[1][e], p[0]))
+        ref = (wt[:, :, None] * each).sum(1)
+        want = [ref.detach(), *torch.autograd.grad(ref, p, dout.double())]
+        for a, b in zip(got, want):
+            assert float((a.double() - b).norm() / b.norm()) < 5 * 2.0 ** -8
+
+
+def test_graph_capture(ops):
+    """Routing and products read their offsets on the device: a step replays on new inputs."""
+    g = gen(45)
+    x = torch.randn(300, 64, generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.randn(5, 72, 64, generator=g, device="cuda").to(torch.bfloat16)
+    logits = torch.randn(300, 5, generator=g, device="cuda")
+
+    def step():
+        r = ops.route(logits, 2)
+        y = ops.dropout(ops.grouped_matmul(x, w, r.offsets, rows=r.rows), 0.25, 3)
+        return ops.combine(y, r.position, r.weights)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    logits.copy_(torch.randn(300, 5, generator=g, device="cuda"))
+    x.copy_(torch.randn(300, 64, generator=g, device="cuda"))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, step())
+
+
+def test_offsets_pass_32_bits(ops):
+    """Tensors of more than 2^32 elements: the last rows, weights and elements."""
+    g = gen(46)
+    n = (1 << 32) + 4099
+    x = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    x[-4099:] = 1
+    got = ops.dropout(x, 0.5, 17, 2)[-4099:]
+    keep, scale = kept(4099, 0.5, 17, 2, first=1 << 32)
+    assert torch.equal(got.double(), keep.double() * scale)
+    del x, got
+
+    y = torch.empty(70_000, 64_000, device="cuda", dtype=torch.bfloat16)  # 4.48e9
+    y[-2:] = torch.randn(2, 64_000, generator=g, device="cuda").to(torch.bfloat16)
+    pos = torch.tensor([[69_999, 69_998]], dtype=torch.int32, device="cuda")
+    wt = torch.tensor([[0.5, -2.0]], device="cuda")
+    want = 0.5 * y[-1:].double() - 2.0 * y[-2:-1].double()
+    close(ops.combine(y, pos, wt), want, 2.0 ** -22 * (y[-1:].double().abs() + 2 * y[-2:-1].abs()))
+    del y
+
+    w = torch.zeros(70, 8192, 8192, device="cuda", dtype=torch.bfloat16)  # 4.7e9
+    w[-1] = torch.randn(8192, 8192, generator=g, device="cuda").to(torch.bfloat16)
+    for m in (3, 70 * 40):  # streamed, and in tiles
+        xs = torch.randn(m, 8192, generator=g, device="cuda").to(torch.bfloat16)
+        off = offsets_of([0] * 69 + [m])
+        want = xs.double() @ w[-1].double().T
+        mag = xs.double().abs() @ w[-1].double().abs().T
+        close(ops.grouped_matmul(xs, w, off), want, 8192 * 2.0 ** -23 * mag)
+
+
 def refusals():
     bf, i32 = torch.bfloat16, torch.int32
     c = lambda *s, dtype=torch.float32: torch.zeros(*s, device="cuda", dtype=dtype)  # noqa
