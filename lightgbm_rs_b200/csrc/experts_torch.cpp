@@ -99,6 +99,27 @@ Tensor make(c10::Device dev, at::ScalarType type, at::IntArrayRef shape) {
   return at::detail::empty_cuda(shape, type, dev, std::nullopt);
 }
 
+// Contiguous tensors cut out of one block of memory, which lives as long as any of them: small
+// results of one call cost one allocation. Offsets and sizes in bytes are multiples of 16.
+class Block {
+ public:
+  Block(c10::Device dev, int64_t bytes) : base_(make(dev, at::kByte, {bytes})) {}
+  static int64_t bytes(int64_t elements) { return (elements * 4 + 15) / 16 * 16; }
+  Tensor cut(at::ScalarType type, at::IntArrayRef shape) {  // 4-byte elements
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+        c10::Storage(base_.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+        c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(at_ / 4);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+    at_ += bytes(t.numel());
+    return t;
+  }
+
+ private:
+  Tensor base_;
+  int64_t at_ = 0;
+};
+
 // The device made current, and its current stream.
 struct On {
   c10::cuda::CUDAGuard guard;
@@ -165,9 +186,11 @@ PyObject* route(PyObject* const* a) {
   if (l.width > INT32_MAX) refuse(LGBM_B200_CAPABILITY_UNAVAILABLE, what, ": too many experts");
   const auto dev = l.t.device();
   On on(dev);
-  Tensor weights = make(dev, at::kFloat, {l.rows, k}), chosen = make(dev, at::kInt, {l.rows, k}),
-         position = make(dev, at::kInt, {l.rows, k}), rows = make(dev, at::kInt, {l.rows * k}),
-         offsets = make(dev, at::kInt, {l.width + 1});
+  const int64_t slots = l.rows * k;
+  Block block(dev, 4 * Block::bytes(slots) + Block::bytes(l.width + 1));
+  Tensor weights = block.cut(at::kFloat, {l.rows, k}), chosen = block.cut(at::kInt, {l.rows, k}),
+         position = block.cut(at::kInt, {l.rows, k}), rows = block.cut(at::kInt, {slots}),
+         offsets = block.cut(at::kInt, {l.width + 1});
   Scratch ws(dev, lgbm_b200_experts_route_workspace(l.rows, (int32_t)l.width, (int32_t)k));
   check(lgbm_b200_experts_route(l.p(), l.dtype, l.rows, (int32_t)l.width, l.pitch, (int32_t)k,
                                 normalize, weights.data_ptr<float>(), chosen.data_ptr<int32_t>(),
