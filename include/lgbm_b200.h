@@ -545,7 +545,7 @@ int lgbm_b200_predict(lgbm_b200_predictor* p, const double* rows, int64_t num_ro
  *  - Pitches are in elements; the innermost axis is contiguous. Outputs are contiguous.
  *  - offsets[E + 1], index, chosen and position are device data that the host does not
  *    check. Kernels clamp offsets to the rows given and skip indices outside them.
- *  - At most 512 experts, 16 chosen a token, 2^31 - 65537 rows.
+ *  - At most 512 experts, 16 chosen a token, 2^31 - 65537 rows, products 2^28 wide.
  *  - Sums and softmax statistics are in f32, results rounded once to their type. No result
  *    depends on the order of atomics: the same inputs give the same bits. */
 #define LGBM_B200_DTYPE_F32 0

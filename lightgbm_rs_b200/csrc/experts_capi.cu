@@ -34,6 +34,8 @@ bool is_float(int32_t dtype) {
 
 // Grouped rows are counted in 32 bits, with room for a tile past the last one.
 constexpr int64_t kMaxRows = 0x7FFFFFFFll - 65536;
+// Bytes of a row of a product's operand are counted in 32 bits.
+constexpr int32_t kMaxWidth = 1 << 28;
 
 int check_gate(const char* what, int32_t dtype, int64_t tokens, int32_t experts, int64_t pitch,
                int32_t k) {
@@ -59,11 +61,13 @@ int check_product(const char* what, const MatmulCall& c) {
   if (c.rows < 0 || c.experts < 1 || c.inner < 1 || c.outer < 1)
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: rows %lld, experts %d, inner %d, outer %d",
                   what, (long long)c.rows, c.experts, c.inner, c.outer);
-  if (c.experts > kMaxExperts || c.rows > kMaxRows || c.x_rows > kMaxRows)
+  if (c.experts > kMaxExperts || c.rows > kMaxRows || c.x_rows > kMaxRows ||
+      c.inner > kMaxWidth || c.outer > kMaxWidth)
     return refuse(LGBM_B200_CAPABILITY_UNAVAILABLE,
-                  "%s: %d experts (at most %d), %lld rows of %lld (at most %lld)", what,
-                  c.experts, kMaxExperts, (long long)c.rows, (long long)c.x_rows,
-                  (long long)kMaxRows);
+                  "%s: %d experts (at most %d), %lld rows of %lld (at most %lld), inner %d and "
+                  "outer %d (at most %d)",
+                  what, c.experts, kMaxExperts, (long long)c.rows, (long long)c.x_rows,
+                  (long long)kMaxRows, c.inner, c.outer, kMaxWidth);
   const bool reads_x = c.y || c.dw, reads_dy = c.dx || c.dw, reads_w = c.y || c.dx;
   if (!c.offsets || (c.rows > 0 && ((reads_x && !c.x) || (reads_dy && !c.dy))) ||
       (reads_w && !c.w))

@@ -469,6 +469,12 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     r.n0 = n * BN;
     r.m0 = m * S::kRows + rank * kTileM;
     if (MODE == WEIGHT) {
+      // Every group has the same tiles, the last row tile perhaps nearly empty: rotated by
+      // group, so that a CTA does not meet the same one in each (their step through the tiles
+      // is even).
+      const int mt = (g.drows + S::kRows - 1) / S::kRows;
+      m = (m + lo) % mt;
+      r.m0 = m * S::kRows + rank * kTileM;
       r.m_end = g.drows;
       r.red0 = b;
       r.red = e - b;
@@ -726,47 +732,53 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
 // 40009 rows of 700 f16 (112 MB read and written): 22 us, 5.1 TB/s.
 // Rows copied to a pitch that TMA can walk: dst[r] = src[index ? index[r] : r], the columns
 // between `width` and `dst_pitch` zero; a row whose index is outside is zero.
-// UNIT bytes of a row are read at a time (its alignment), 16 written; a thread takes kStageRun
-// pieces, all loads first. 40009 rows of 700 f16: 22 us, 112 MB at 5.1 TB/s.
+// A warp a row, 16 bytes a lane and kStageRun of them at a time, all loads first. UNIT bytes
+// are read at a time: the rows' alignment.
 constexpr int kStageRun = 4;
 
 template <int UNIT>
-__global__ void __launch_bounds__(256)
-    k_stage_rows(const char* __restrict__ src, int32_t src_rows, int64_t pieces, int bytes,
-                 int64_t pitch, const int32_t* __restrict__ index, uint4* dst, uint32_t per_row) {
-  const int64_t first = (int64_t)blockIdx.x * (256 * kStageRun) + threadIdx.x;
-  uint4 v[kStageRun];
-#pragma unroll
-  for (int u = 0; u < kStageRun; ++u) {
-    const int64_t i = first + u * 256;
-    v[u] = make_uint4(0, 0, 0, 0);
-    if (i >= pieces) continue;
-    const int64_t r = (uint64_t)i < 0xFFFFFFFFu ? (uint32_t)i / per_row : i / per_row;
-    const int c = (int)(i - r * per_row) * 16;
-    const int64_t at = index ? index[r] : r;
-    if (at < 0 || (index && at >= src_rows)) continue;
-    const char* p = src + at * pitch + c;
-    if (UNIT == 16 && c + 16 <= bytes) {
-      v[u] = __ldg(reinterpret_cast<const uint4*>(p));
-    } else if (UNIT >= 8 && c + 16 <= bytes) {
-      const uint2 lo = __ldg(reinterpret_cast<const uint2*>(p));
-      const uint2 hi = __ldg(reinterpret_cast<const uint2*>(p + 8));
-      v[u] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-    } else if (UNIT >= 4 && c + 16 <= bytes) {
-      const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
-      v[u] = make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
-    } else {
-      uint32_t e[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        e[j] = c + 2 * j < bytes ? __ldg(reinterpret_cast<const uint16_t*>(p) + j) : 0;
-      v[u] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16,
-                        e[6] | e[7] << 16);
-    }
+__device__ __forceinline__ uint4 stage_piece(const char* p, int left) {  // left: bytes of the row
+  if (UNIT == 16 && left >= 16) return __ldg(reinterpret_cast<const uint4*>(p));
+  if (UNIT >= 8 && left >= 16) {
+    const uint2 lo = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 hi = __ldg(reinterpret_cast<const uint2*>(p + 8));
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
   }
+  if (UNIT >= 4 && left >= 16) {
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
+    return make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
+  }
+  uint32_t e[8];
 #pragma unroll
-  for (int u = 0; u < kStageRun; ++u)
-    if (first + u * 256 < pieces) dst[first + u * 256] = v[u];
+  for (int j = 0; j < 8; ++j)
+    e[j] = 2 * j < left ? __ldg(reinterpret_cast<const uint16_t*>(p) + j) : 0;
+  return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+}
+
+template <int UNIT>
+__global__ void __launch_bounds__(256)
+    k_stage_rows(const char* __restrict__ src, int64_t src_rows, int64_t rows, int bytes,
+                 int64_t pitch, const int32_t* __restrict__ index, char* __restrict__ dst,
+                 int dst_bytes) {
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const int64_t at = index ? index[r] : r;
+  const bool inside = at >= 0 && at < src_rows;
+  const char* from = src + (inside ? at : 0) * pitch;
+  char* to = dst + r * dst_bytes;
+  for (int c0 = lane * 16; c0 < dst_bytes; c0 += 512 * kStageRun) {
+    uint4 v[kStageRun];
+#pragma unroll
+    for (int u = 0; u < kStageRun; ++u) {
+      const int c = c0 + 512 * u;
+      v[u] = make_uint4(0, 0, 0, 0);
+      if (inside && c < bytes) v[u] = stage_piece<UNIT>(from + c, bytes - c);
+    }
+#pragma unroll
+    for (int u = 0; u < kStageRun; ++u)
+      if (c0 + 512 * u < dst_bytes) *reinterpret_cast<uint4*>(to + c0 + 512 * u) = v[u];
+  }
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -878,16 +890,15 @@ int64_t copy_bytes(int64_t rows, int64_t width) {
 cudaError_t stage(Operand& o, int64_t src_rows, int64_t rows, int width, const int32_t* index,
                   char*& workspace, cudaStream_t st) {
   const int64_t dst_pitch = padded(width);
-  uint4* dst = reinterpret_cast<uint4*>(workspace);
+  char* dst = workspace;
   workspace += copy_bytes(rows, width);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(o.p) | (uintptr_t)(o.pitch * 2);
-  const int64_t pieces = rows * (dst_pitch / 8);
-  const int64_t blocks = (pieces + 256 * kStageRun - 1) / (256 * kStageRun);
+  const int64_t blocks = (rows + 7) / 8;
   if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
   auto go = [&](auto unit) {
     k_stage_rows<decltype(unit)::value><<<(unsigned)blocks, 256, 0, st>>>(
-        static_cast<const char*>(o.p), (int32_t)src_rows, pieces, width * 2, o.pitch * 2, index,
-        dst, (uint32_t)(dst_pitch / 8));
+        static_cast<const char*>(o.p), src_rows, rows, width * 2, o.pitch * 2, index, dst,
+        (int)(dst_pitch * 2));
   };
   if (bits % 16 == 0) go(std::integral_constant<int, 16>());
   else if (bits % 8 == 0) go(std::integral_constant<int, 8>());
@@ -950,7 +961,7 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
   // Pairs where most tiles fill more than one CTA's rows. (157 rows an expert on average, 255
   // of 136 x 704: y 33 us either way, dw 54 in pairs, 68 without; fewer rows than a CTA's
   // would leave the odd CTA idle.)
-  const bool tall = MODE == WEIGHT ? g.drows > kTileM : g.rows >= (int64_t)kTileM * g.experts;
+  const bool tall = MODE == WEIGHT ? g.drows >= kTileM * 3 / 2 : g.rows >= (int64_t)kTileM * g.experts;
   return tall ? go(std::integral_constant<int, 256>(), Two())
               : go(std::integral_constant<int, 256>(), One());
 }

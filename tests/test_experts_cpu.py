@@ -38,6 +38,8 @@ def test_arguments_are_refused_with_a_status(capi):
     assert mm(p, 4, 8, None, p, p, 0, 4, 2, 8, 8, p, None, 0, None) == bad   # f32
     assert mm(p, 4, 8, None, p, p, 1, 4, 0, 8, 8, p, None, 0, None) == bad   # no experts
     assert mm(p, 4, 8, None, p, p, 1, 4, 513, 8, 8, p, None, 0, None) == cap
+    wide = (1 << 28) + 8
+    assert mm(p, 4, wide, None, p, p, 1, 4, 2, wide, 8, p, None, 0, None) == cap
     assert mm(p, 4, 7, None, p, p, 1, 4, 2, 8, 8, p, None, 0, None) == length
     assert mm(p, 5, 8, None, p, p, 1, 4, 2, 8, 8, p, None, 0, None) == length
     assert mm(p, 400, 9, None, p, p, 1, 400, 2, 9, 8, p, None, 0, None) == length  # workspace
