@@ -22,7 +22,7 @@
 // 700 features are 1400 bytes) are first copied to rows that it can (k_stage_rows), which
 // costs their bytes twice more. Two ways without that copy were built and measured on 65536
 // gathered rows of 2048 against 4096 outputs, where the product takes 0.77 ms and the copy
-// 0.13: TMA gathers of four rows took about 20 cycles a row of 128 bytes (2.5 ms in all), and
+// 0.08: TMA gathers of four rows took about 20 cycles a row of 128 bytes (2.5 ms in all), and
 // six warps of asynchronous 16-byte copies, each waiting out its own block's latency, 1.5.
 //
 // Ragged ends. FORWARD / INPUT: a tile's rows past its group's end are computed from the next
@@ -47,8 +47,8 @@
 // 4096 x 1024: 68, 68, 68 us against 66, 60, 65 (1.0 PFLOP/s); tensor pipe 60 % busy; the rest
 // is the last wave, tiles that groups of 1024 and a few rows leave partly empty, and loads at
 // the 64 bytes a cycle that an SM takes from L2. 40009 rows, 255 experts of 136 x 704: y 33,
-// dx 47, dw 51 and 67 us, 2 to 3 TB/s: two or three blocks of reduction a tile, bound by
-// writing tiles out.
+// dx 47, dw 47 and 59 us, 2 to 3 TB/s: two or three blocks of reduction a tile, bound by
+// writing tiles out. (Dealing dw's tiles out longest group first gained nothing.)
 #include <algorithm>
 #include <atomic>
 #include <mutex>
@@ -733,7 +733,8 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
 // Rows copied to a pitch that TMA can walk: dst[r] = src[index ? index[r] : r], the columns
 // between `width` and `dst_pitch` zero; a row whose index is outside is zero.
 // A warp a row, 16 bytes a lane and kStageRun of them at a time, all loads first. UNIT bytes
-// are read at a time: the rows' alignment.
+// are read at a time: the rows' alignment. 40009 rows of 700 f16: 18 us, 112 MB at 6.2 TB/s (a
+// thread a piece, with a division each, took 22).
 constexpr int kStageRun = 4;
 
 template <int UNIT>
@@ -958,9 +959,9 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
   using Two = std::integral_constant<int, 2>;
   if (g.cols <= 64) return go(std::integral_constant<int, 64>(), One());
   if (g.cols <= 128) return go(std::integral_constant<int, 128>(), One());
-  // Pairs where most tiles fill more than one CTA's rows. (157 rows an expert on average, 255
-  // of 136 x 704: y 33 us either way, dw 54 in pairs, 68 without; fewer rows than a CTA's
-  // would leave the odd CTA idle.)
+  // Pairs where most tiles fill more than one and a half CTAs' rows, or an expert's rows more
+  // than one's: else the odd CTA of a pair has little to do. (255 experts of 136 x 704 with 157
+  // rows on average: y 33 us either way; dw in f32 67 in pairs, 59 without.)
   const bool tall = MODE == WEIGHT ? g.drows >= kTileM * 3 / 2 : g.rows >= (int64_t)kTileM * g.experts;
   return tall ? go(std::integral_constant<int, 256>(), Two())
               : go(std::integral_constant<int, 256>(), One());
