@@ -209,7 +209,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 constexpr int kSelectThreads = 256;
-constexpr int kSelectTokens = 128;  // of a block: 16 a warp, one after the other
+// Tokens of a block: a warp takes 1 to 16 of them, one after the other. One costs about 1.5 us,
+// most of it the waits of its own choices, so few tokens are spread over up to 256 blocks
+// before a warp takes more (109 rows of 199, k 6: 3.4 us, in blocks of 128 25; 1167 of 330: 3.8
+// and 30); 16 a warp keep the counts, a number a block and expert, below the logits' bytes.
+int select_tokens_of(int64_t tokens) {
+  int n = kSelectThreads / 32;
+  while (n < kSelectThreads / 2 && (tokens + n - 1) / n > 256) n *= 2;
+  return n;
+}
 
 // First of three launches for many tokens: choice and weights, and each block's rows per
 // expert. A warp a token, its logits in registers, expert e in lane e % 32; the next token's
@@ -226,7 +234,8 @@ constexpr int kSelectTokens = 128;  // of a block: 16 a warp, one after the othe
 template <typename T, int NV, int CN>
 __global__ void __launch_bounds__(kSelectThreads)
     k_route_select(const T* logits, int64_t tokens, int experts, int64_t pitch, int k,
-                   bool normalize, float* weights, int32_t* chosen, int32_t* counts) {
+                   bool normalize, int block_tokens, float* weights, int32_t* chosen,
+                   int32_t* counts) {
   constexpr uint32_t kAll = 0xFFFFFFFFu;
   constexpr int kWarps = kSelectThreads / 32;
   constexpr bool kTwoStages = CN < NV;
@@ -234,9 +243,9 @@ __global__ void __launch_bounds__(kSelectThreads)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i <= experts; i += kSelectThreads) hist[i] = 0;
   __syncthreads();
-  constexpr int kPerWarp = kSelectTokens / kWarps;
-  const int64_t first = (int64_t)blockIdx.x * kSelectTokens + warp * kPerWarp;
-  const int64_t last = min(first + kPerWarp, tokens);
+  const int per_warp = block_tokens / kWarps;
+  const int64_t first = (int64_t)blockIdx.x * block_tokens + warp * per_warp;
+  const int64_t last = min(first + per_warp, tokens);
   const float kNone = -__int_as_float(0x7F800000);
   float next[NV];
   auto fetch = [&](const T* row) {
@@ -503,7 +512,8 @@ cudaError_t route_typed(const T* logits, int64_t tokens, int experts, int64_t pi
                                                          rows, offsets);
     return cudaGetLastError();
   }
-  const int blocks = (int)((tokens + kSelectTokens - 1) / kSelectTokens);
+  const int block_tokens = select_tokens_of(tokens);
+  const int blocks = (int)((tokens + block_tokens - 1) / block_tokens);
   int32_t* totals = ws;
   int32_t* counts = ws + experts + 1;
   auto select = [&](auto nv) {
@@ -511,7 +521,7 @@ cudaError_t route_typed(const T* logits, int64_t tokens, int experts, int64_t pi
     auto deal = [&](auto cn) {
       constexpr int CN = decltype(cn)::value < NV ? decltype(cn)::value : NV;
       k_route_select<T, NV, CN><<<blocks, kSelectThreads, 0, st>>>(
-          logits, tokens, experts, pitch, k, normalize, weights, chosen, counts);
+          logits, tokens, experts, pitch, k, normalize, block_tokens, weights, chosen, counts);
     };
     const int most = k * NV;  // candidates of the second stage
     if (most <= 32) deal(std::integral_constant<int, 1>());
@@ -527,7 +537,7 @@ cudaError_t route_typed(const T* logits, int64_t tokens, int experts, int64_t pi
   k_route_scan<<<(experts + 8) / 8, 256, 0, st>>>(counts, totals, experts + 1, blocks);
   const size_t smem = sizeof(int32_t) * (experts + 1) * (1 + kRouteThreads / 32);
   k_route_place<<<blocks, kRouteThreads, smem, st>>>(chosen, counts, totals, tokens, experts, k,
-                                                     kSelectTokens, position, rows, offsets);
+                                                     block_tokens, position, rows, offsets);
   return cudaGetLastError();
 }
 
@@ -553,7 +563,8 @@ cudaError_t with_type(int32_t dtype, F&& f) {
 int64_t route_workspace(int64_t tokens, int32_t experts, int32_t k) {
   (void)k;
   if (tokens <= kSmallTokens) return 0;
-  const int64_t blocks = (tokens + kSelectTokens - 1) / kSelectTokens;
+  const int block_tokens = select_tokens_of(tokens);
+  const int64_t blocks = (tokens + block_tokens - 1) / block_tokens;
   return (int64_t)sizeof(int32_t) * (experts + 1) * (blocks + 1);
 }
 

@@ -118,6 +118,12 @@ def test_route(ops, tokens, experts, k, normalize, dtype):
     close(d, torch.from_numpy(want).cuda(), torch.from_numpy(scale).cuda() * 1024 * 2 ** -24)
 
 
+@pytest.mark.parametrize("tokens", [66, 109, 2047, 2049, 4096, 9001, 33000])
+def test_route_blocks(ops, tokens):
+    """Numbers of tokens at which a block takes another share of them."""
+    test_route(ops, tokens, 37, 3, False, "f32")
+
+
 def test_route_nan_and_infinity(ops):
     x = torch.zeros(4, 6, device="cuda")
     x[0, 3] = math.nan
@@ -245,6 +251,30 @@ def test_weight_gradient_in_32_bits_stays_precise(ops, inner, outer):
     want = dy.double().T @ x.double()
     assert float((dw[1].double() - want).norm() / want.norm()) < (48 + n / 1536) * 2.0 ** -23
     assert not dw[0].any()
+
+
+@pytest.mark.parametrize("counts,tail", [([3000, 0], 5), ([1, 0, 1500, 700], 0),
+                                         ([64, 63, 2049], 1), ([600], 0), ([0, 0, 4000, 1], 3)])
+@pytest.mark.parametrize("inner,outer", [(80, 56), (129, 300), (264, 200), (1, 1), (130, 3)])
+def test_weight_gradient_in_parts(ops, counts, tail, inner, outer):
+    """Few outputs and many rows: an expert's rows are summed in parts and the parts joined."""
+    g = gen(inner + len(counts))
+    m, E = sum(counts) + tail, len(counts)
+    x = torch.randn(m, inner, generator=g, device="cuda").to(torch.bfloat16)
+    dy = torch.randn(m, outer, generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.zeros(E, outer, inner, device="cuda", dtype=torch.bfloat16)
+    if tail:
+        x[-1], dy[-1] = math.nan, math.inf
+    off = offsets_of(counts)
+    o = off.tolist()
+    for grad in (torch.float32, torch.bfloat16):
+        dw = ops.grouped_matmul_backward(dy, x, w, off, need_dx=False, grad_dtype=grad)[1]
+        again = ops.grouped_matmul_backward(dy, x, w, off, need_dx=False, grad_dtype=grad)[1]
+        assert torch.equal(dw, again)
+        for e in range(E):
+            s = slice(o[e], o[e + 1])
+            want = dy[s].double().T @ x[s].double()
+            close(dw[e], want, counts[e] * 2.0 ** -23 * (dy[s].double().abs().T @ x[s].double().abs()))
 
 
 @pytest.mark.parametrize("counts", [[70, 0, 9, 130], [700, 0, 70, 333]])
