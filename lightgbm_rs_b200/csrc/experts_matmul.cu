@@ -72,7 +72,8 @@ constexpr int kRun = 768;  // rows of a run of WEIGHT_F32
 
 struct MatArgs {
   const int32_t* offsets;
-  int32_t experts;
+  int32_t experts;     // groups: WEIGHT has `parts` of each expert's
+  int32_t parts;
   int32_t cols;        // columns of D in a group
   int32_t drows;       // WEIGHT: rows of D in a group
   int32_t reduction;   // FORWARD, INPUT: length of the reduction
@@ -413,9 +414,10 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     // group more; WEIGHT has no tiles for them.
     const int nt = (g.cols + BN - 1) / BN;
     int32_t carry = 0, reach = 0;
-    for (int i0 = 0; i0 <= g.experts; i0 += 32) {
+    const int experts = MODE == WEIGHT ? g.experts / g.parts : g.experts;
+    for (int i0 = 0; i0 <= experts; i0 += 32) {
       const int i = i0 + lane;
-      int32_t b = i <= g.experts ? (int32_t)min(max((int64_t)g.offsets[i], (int64_t)0), g.rows) : 0;
+      int32_t b = i <= experts ? (int32_t)min(max((int64_t)g.offsets[i], (int64_t)0), g.rows) : 0;
       b = max(b, reach);
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -423,7 +425,19 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
         if (lane >= d) b = max(b, o);
       }
       reach = __shfl_sync(0xFFFFFFFFu, b, 31);
-      if (i <= g.experts) off[i] = b;
+      if (i <= experts) off[i] = b;
+    }
+    if (MODE == WEIGHT && g.parts > 1) {  // each expert's rows in equal parts of whole blocks
+      __syncwarp();
+      for (int i = lane; i <= g.experts; i += 32) {
+        const int e = i / g.parts, part = i % g.parts;
+        const int32_t n = e < experts ? off[e + 1] - off[e] : 0;
+        const int32_t each = (n / kTileK + g.parts) / g.parts * kTileK;
+        cum[i] = off[e] + (int32_t)min((int64_t)each * part, (int64_t)n);
+      }
+      __syncwarp();
+      for (int i = lane; i <= g.experts; i += 32) off[i] = cum[i];
+      __syncwarp();
     }
     if (lane == 0) off[g.experts + 1] = (int32_t)g.rows;
     __syncwarp();
@@ -729,7 +743,6 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
   }
 }
 
-// 40009 rows of 700 f16 (112 MB read and written): 22 us, 5.1 TB/s.
 // Rows copied to a pitch that TMA can walk: dst[r] = src[index ? index[r] : r], the columns
 // between `width` and `dst_pitch` zero; a row whose index is outside is zero.
 // A warp a row, 16 bytes a lane and kStageRun of them at a time, all loads first. UNIT bytes
@@ -916,6 +929,9 @@ uint32_t instruction(int32_t dtype, bool a_mn, bool b_mn, int m, int n) {
          ((uint32_t)b_mn << 16) | ((uint32_t)(n / 8) << 17) | ((uint32_t)(m / 16) << 24);
 }
 
+// Whether an expert's weight gradient of more than 128 columns is multiplied by pairs.
+bool weight_pairs(int64_t drows) { return drows >= kTileM * 3 / 2; }
+
 // a: x (FORWARD) or dy; b: w, or x (WEIGHT).
 template <int MODE>
 cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64_t b_width,
@@ -962,9 +978,44 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
   // Pairs where most tiles fill more than one and a half CTAs' rows, or an expert's rows more
   // than one's: else the odd CTA of a pair has little to do. (255 experts of 136 x 704 with 157
   // rows on average: y 33 us either way; dw in f32 67 in pairs, 59 without.)
-  const bool tall = MODE == WEIGHT ? g.drows >= kTileM * 3 / 2 : g.rows >= (int64_t)kTileM * g.experts;
+  const bool tall = MODE == WEIGHT ? weight_pairs(g.drows) : g.rows >= (int64_t)kTileM * g.experts;
   return tall ? go(std::integral_constant<int, 256>(), Two())
               : go(std::integral_constant<int, 256>(), One());
+}
+
+// Sums of the parts of a weight gradient, always in the same order: part[e][p][n] to out[e][n],
+// n in [0, count). V elements a thread.
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+    k_join_parts(const float* part, int parts, int64_t count, int64_t total, T* out) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
+  if (i >= total) return;
+  const int64_t e = i / count;
+  const float* p = part + e * count * (parts - 1) + i;  // (e * parts) * count + i - e * count
+  float sum[V] = {};
+#pragma unroll 4
+  for (int k = 0; k < parts; ++k, p += count) {
+    if constexpr (V == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p);
+      sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+    } else {
+      sum[0] += *p;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) out[i + j] = from_f32<T>(sum[j]);
+}
+
+template <typename T>
+cudaError_t join_parts(const float* part, int parts, int64_t count, int experts, T* out,
+                       cudaStream_t st) {
+  const int64_t total = count * experts;
+  const auto blocks = [&](int v) { return (unsigned)((total / v + 255) / 256); };
+  if (count % 4 == 0)
+    k_join_parts<T, 4><<<blocks(4), 256, 0, st>>>(part, parts, count, total, out);
+  else
+    k_join_parts<T, 1><<<blocks(1), 256, 0, st>>>(part, parts, count, total, out);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -991,8 +1042,28 @@ static bool copies_w(const MatmulCall& c) {
   return ((c.y && !few_rows(c)) || c.dx) && !(aligned16(c.w) && c.inner % 8 == 0);
 }
 
+// Parts of each expert's rows that a weight gradient is summed in, 1: not split. Its tiles are
+// its outputs', so few and small experts leave SMs idle while others walk all rows. Parts give
+// every SM a tile; each has 256 rows on average at least, since a tile's start and end cost
+// about that much and each part is written and read once in f32. Measured with the joining,
+// without parts: 60330 rows, 3 experts of 80 x 2864 in f32 82, 183 us; 35996 rows, 19 of 56 x 80
+// in bf16 18, 51; 1514 rows, 2 of 128 x 320 15.4, 17.4.
+static int weight_parts(const MatmulCall& c) {
+  const bool pairs = c.inner > 128 && weight_pairs(c.outer);
+  const int64_t bn = c.inner <= 64 ? 64 : c.inner <= 128 ? 128 : 256;
+  const int64_t tile_rows = pairs ? 2 * kTileM : kTileM;
+  const int64_t tiles = c.experts * ((c.outer + tile_rows - 1) / tile_rows) * ((c.inner + bn - 1) / bn);
+  const int64_t parts = std::min(std::min((pairs ? 74 : 148) / tiles, c.rows / (256 * (int64_t)c.experts)),
+                                 (int64_t)(kMaxExperts / c.experts));
+  return c.dw && parts > 1 ? (int)parts : 1;
+}
+static int64_t parts_bytes(const MatmulCall& c) {
+  const int parts = weight_parts(c);
+  return parts > 1 ? sizeof(float) * parts * c.experts * (int64_t)c.outer * c.inner : 0;
+}
+
 int64_t matmul_workspace(const MatmulCall& c) {
-  return (copies_x(c) ? copy_bytes(c.rows, c.inner) : 0) +
+  return parts_bytes(c) + (copies_x(c) ? copy_bytes(c.rows, c.inner) : 0) +
          (copies_dy(c) ? copy_bytes(c.rows, c.outer) : 0) +
          (copies_w(c) ? copy_bytes((int64_t)c.experts * c.outer, c.inner) : 0);
 }
@@ -1026,6 +1097,7 @@ cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st)
   MatArgs g{};
   g.offsets = c.offsets;
   g.experts = c.experts;
+  g.parts = 1;
   g.rows = c.rows;
   if (err == cudaSuccess && c.y) {
     g.out = c.y;
@@ -1044,12 +1116,24 @@ cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st)
     err = run_tiles<INPUT>(dy, c.outer, w, c.inner, c.dtype, g, st);
   }
   if (err == cudaSuccess && c.dw) {
-    g.out = c.dw;
-    g.out_kind = c.grad_dtype;
+    g.parts = weight_parts(c);
+    g.experts *= g.parts;
+    g.out = g.parts > 1 ? ws : c.dw;  // ws: the end of the copies
+    g.out_kind = g.parts > 1 ? (int32_t)LGBM_B200_DTYPE_F32 : c.grad_dtype;
     g.cols = c.inner;
     g.drows = c.outer;
     g.out_pitch = c.inner;
     err = run_tiles<WEIGHT>(dy, c.outer, x, c.inner, c.dtype, g, st);
+    if (err == cudaSuccess && g.parts > 1) {
+      const int64_t count = (int64_t)c.outer * c.inner;
+      const float* part = reinterpret_cast<const float*>(ws);
+      if (c.grad_dtype == LGBM_B200_DTYPE_F32)
+        err = join_parts(part, g.parts, count, c.experts, static_cast<float*>(c.dw), st);
+      else if (c.grad_dtype == LGBM_B200_DTYPE_BF16)
+        err = join_parts(part, g.parts, count, c.experts, static_cast<__nv_bfloat16*>(c.dw), st);
+      else
+        err = join_parts(part, g.parts, count, c.experts, static_cast<__half*>(c.dw), st);
+    }
   }
   return err;
 }
