@@ -745,22 +745,21 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
 
 // Rows copied to a pitch that TMA can walk: dst[r] = src[index ? index[r] : r], the columns
 // between `width` and `dst_pitch` zero; a row whose index is outside is zero.
-// A warp a row, 16 bytes a lane and kStageRun of them at a time, all loads first. UNIT bytes
-// are read at a time: the rows' alignment. 40009 rows of 700 f16: 18 us, 112 MB at 6.2 TB/s (a
-// thread a piece, with a division each, took 22).
+// 2^LOG lanes a row and kRunOf pieces of 16 bytes a lane at a time, all loads first: a warp a
+// row and four pieces from 512 bytes on, half as many lanes as pieces for short rows. UNIT is
+// the rows' alignment, 2 for all below 8. Measured, rows x columns: 40009 x 700 (8 bytes) 18 us,
+// 6.1 TB/s read and written; 65536 x 2755 110 us, 6.6; 7884 x 3977 25 us, 5.0; 40009 x 129 6.9
+// us (a warp a row and 2 bytes a load 10), 500000 x 21 10 us (44).
 constexpr int kStageRun = 4;
 
+// `left`: bytes of the row from p on.
 template <int UNIT>
-__device__ __forceinline__ uint4 stage_piece(const char* p, int left) {  // left: bytes of the row
+__device__ __forceinline__ uint4 stage_piece(const char* p, int left) {
   if (UNIT == 16 && left >= 16) return __ldg(reinterpret_cast<const uint4*>(p));
   if (UNIT >= 8 && left >= 16) {
     const uint2 lo = __ldg(reinterpret_cast<const uint2*>(p));
     const uint2 hi = __ldg(reinterpret_cast<const uint2*>(p + 8));
     return make_uint4(lo.x, lo.y, hi.x, hi.y);
-  }
-  if (UNIT >= 4 && left >= 16) {
-    const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
-    return make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
   }
   uint32_t e[8];
 #pragma unroll
@@ -769,29 +768,76 @@ __device__ __forceinline__ uint4 stage_piece(const char* p, int left) {  // left
   return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
 }
 
-template <int UNIT>
+// The same from any even address: the one or two aligned pieces that hold it, loaded by
+// stage_load, shifted here. (Eight loads of 2 bytes a piece pass through L1 one by one.)
+struct StagePair { uint4 a, b; };
+__device__ __forceinline__ StagePair stage_load(const char* p, int left) {
+  const int s = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+  const uint4* q = reinterpret_cast<const uint4*>(p - s);
+  return {__ldg(q), __ldg(q + (s + min(left, 16) > 16))};
+}
+__device__ __forceinline__ uint4 stage_shift(const StagePair& v, int s, int left) {
+  uint32_t w[8] = {v.a.x, v.a.y, v.a.z, v.a.w, v.b.x, v.b.y, v.b.z, v.b.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = s & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = s & 4 ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = s & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+  if (left < 16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = left >= 4 * i + 4 ? w[i] : left > 4 * i ? w[i] & 0xFFFFu : 0;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int UNIT, int LOG>
 __global__ void __launch_bounds__(256)
     k_stage_rows(const char* __restrict__ src, int64_t src_rows, int64_t rows, int bytes,
                  int64_t pitch, const int32_t* __restrict__ index, char* __restrict__ dst,
                  int dst_bytes) {
-  const int lane = threadIdx.x & 31;
-  const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  constexpr int kLanes = 1 << LOG, kRunOf = LOG == 5 ? kStageRun : 2, kStep = 16 * kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const int64_t r = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   if (r >= rows) return;
   const int64_t at = index ? index[r] : r;
   const bool inside = at >= 0 && at < src_rows;
   const char* from = src + (inside ? at : 0) * pitch;
   char* to = dst + r * dst_bytes;
-  for (int c0 = lane * 16; c0 < dst_bytes; c0 += 512 * kStageRun) {
-    uint4 v[kStageRun];
+  if constexpr (UNIT < 8) {
+    // aligned pieces may begin before a row and end behind it, but not outside the source
+    const int s = (int)(reinterpret_cast<uintptr_t>(from) & 15);
+    const int64_t behind = src + (src_rows - 1) * pitch - from;  // from this row's end to the last's
+    if (inside && from - s >= src && (-(s + bytes) & 15) <= behind) {
+      for (int c0 = lane * 16; c0 < dst_bytes; c0 += kStep * kRunOf) {
+        StagePair v[kRunOf];
 #pragma unroll
-    for (int u = 0; u < kStageRun; ++u) {
-      const int c = c0 + 512 * u;
+        for (int u = 0; u < kRunOf; ++u) {
+          const int c = c0 + kStep * u;
+          v[u] = c < bytes ? stage_load(from + c, bytes - c) : StagePair();
+        }
+#pragma unroll
+        for (int u = 0; u < kRunOf; ++u) {
+          const int c = c0 + kStep * u;
+          if (c < dst_bytes)
+            *reinterpret_cast<uint4*>(to + c) = stage_shift(v[u], s, bytes - c);
+        }
+      }
+      return;
+    }
+  }
+  for (int c0 = lane * 16; c0 < dst_bytes; c0 += kStep * kRunOf) {
+    uint4 v[kRunOf];
+#pragma unroll
+    for (int u = 0; u < kRunOf; ++u) {
+      const int c = c0 + kStep * u;
       v[u] = make_uint4(0, 0, 0, 0);
       if (inside && c < bytes) v[u] = stage_piece<UNIT>(from + c, bytes - c);
     }
 #pragma unroll
-    for (int u = 0; u < kStageRun; ++u)
-      if (c0 + 512 * u < dst_bytes) *reinterpret_cast<uint4*>(to + c0 + 512 * u) = v[u];
+    for (int u = 0; u < kRunOf; ++u)
+      if (c0 + kStep * u < dst_bytes) *reinterpret_cast<uint4*>(to + c0 + kStep * u) = v[u];
   }
 }
 
@@ -907,20 +953,27 @@ cudaError_t stage(Operand& o, int64_t src_rows, int64_t rows, int width, const i
   char* dst = workspace;
   workspace += copy_bytes(rows, width);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(o.p) | (uintptr_t)(o.pitch * 2);
-  const int64_t blocks = (rows + 7) / 8;
-  if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-  auto go = [&](auto unit) {
-    k_stage_rows<decltype(unit)::value><<<(unsigned)blocks, 256, 0, st>>>(
+  auto go = [&](auto unit, auto log) {
+    constexpr int kRows = 256 >> decltype(log)::value;
+    const int64_t blocks = (rows + kRows - 1) / kRows;
+    if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    k_stage_rows<decltype(unit)::value, decltype(log)::value><<<(unsigned)blocks, 256, 0, st>>>(
         static_cast<const char*>(o.p), src_rows, rows, width * 2, o.pitch * 2, index, dst,
         (int)(dst_pitch * 2));
+    return cudaGetLastError();
   };
-  if (bits % 16 == 0) go(std::integral_constant<int, 16>());
-  else if (bits % 8 == 0) go(std::integral_constant<int, 8>());
-  else if (bits % 4 == 0) go(std::integral_constant<int, 4>());
-  else go(std::integral_constant<int, 2>());
+  auto with_lanes = [&](auto unit) {
+    if (dst_pitch <= 32) return go(unit, std::integral_constant<int, 1>());
+    if (dst_pitch <= 128) return go(unit, std::integral_constant<int, 3>());
+    if (dst_pitch <= 256) return go(unit, std::integral_constant<int, 4>());
+    return go(unit, std::integral_constant<int, 5>());
+  };
+  const cudaError_t err = bits % 16 == 0  ? with_lanes(std::integral_constant<int, 16>())
+                          : bits % 8 == 0 ? with_lanes(std::integral_constant<int, 8>())
+                                          : with_lanes(std::integral_constant<int, 2>());
   o.p = dst;
   o.pitch = dst_pitch;
-  return cudaGetLastError();
+  return err;
 }
 
 uint32_t instruction(int32_t dtype, bool a_mn, bool b_mn, int m, int n) {

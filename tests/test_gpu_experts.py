@@ -253,6 +253,32 @@ def test_weight_gradient_in_32_bits_stays_precise(ops, inner, outer):
     assert not dw[0].any()
 
 
+@pytest.mark.parametrize("inner", [1, 7, 9, 24, 31, 37, 127, 129, 260, 517])
+@pytest.mark.parametrize("start", range(8))
+def test_operands_at_any_address(ops, inner, start):
+    """x and dy start `start` elements into rows of their own pitch, NaN around them; values are
+    small integers, so that every sum is exact."""
+    g = gen(inner)
+    m, E, outer = 150, 2, inner + start
+    off = offsets_of([90, 60])
+
+    def view(rows, width, pitch):
+        t = torch.full((rows * pitch + start + 8,), math.nan, device="cuda", dtype=torch.float16)
+        v = t[start:start + rows * pitch].view(rows, pitch)[:, :width]
+        return v.copy_(torch.randint(-2, 3, (rows, width), generator=g, device="cuda"))
+
+    x = view(m, inner, inner + start % 3)
+    dy = view(m, outer, outer + start % 5)
+    w = torch.randint(-1, 2, (E, outer, inner), generator=g, device="cuda").half()
+    _, y, _ = product64(x, w, off, None)
+    _, dx, _ = product64(dy, w.transpose(1, 2), off, None)
+    assert torch.equal(ops.grouped_matmul(x, w, off).double(), y)
+    got, dw = ops.grouped_matmul_backward(dy, x, w, off)
+    assert torch.equal(got.double(), dx)
+    for e, s in enumerate((slice(0, 90), slice(90, 150))):
+        assert torch.equal(dw[e].double(), dy[s].double().T @ x[s].double())
+
+
 @pytest.mark.parametrize("counts,tail", [([3000, 0], 5), ([1, 0, 1500, 700], 0),
                                          ([64, 63, 2049], 1), ([600], 0), ([0, 0, 4000, 1], 3)])
 @pytest.mark.parametrize("inner,outer", [(80, 56), (129, 300), (264, 200), (1, 1), (130, 3)])
