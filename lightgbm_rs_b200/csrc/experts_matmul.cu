@@ -749,7 +749,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
 // row and four pieces from 512 bytes on, half as many lanes as pieces for short rows. UNIT is
 // the rows' alignment, 2 for all below 8. Measured, rows x columns: 40009 x 700 (8 bytes) 18 us,
 // 6.1 TB/s read and written; 65536 x 2755 110 us, 6.6; 7884 x 3977 25 us, 5.0; 40009 x 129 6.9
-// us (a warp a row and 2 bytes a load 10), 500000 x 21 10 us (44).
+// us (a warp a row 10.7), 500000 x 21 10 us (a warp a row and 2 bytes a load: 44 for 556780).
 constexpr int kStageRun = 4;
 
 // `left`: bytes of the row from p on.
@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(256)
   if constexpr (UNIT < 8) {
     // aligned pieces may begin before a row and end behind it, but not outside the source
     const int s = (int)(reinterpret_cast<uintptr_t>(from) & 15);
-    const int64_t behind = src + (src_rows - 1) * pitch - from;  // from this row's end to the last's
+    const int64_t behind = src + (src_rows - 1) * pitch - from;  // this row's end to the last's
     if (inside && from - s >= src && (-(s + bytes) & 15) <= behind) {
       for (int c0 = lane * 16; c0 < dst_bytes; c0 += kStep * kRunOf) {
         StagePair v[kRunOf];
@@ -1105,9 +1105,10 @@ static int weight_parts(const MatmulCall& c) {
   const bool pairs = c.inner > 128 && weight_pairs(c.outer);
   const int64_t bn = c.inner <= 64 ? 64 : c.inner <= 128 ? 128 : 256;
   const int64_t tile_rows = pairs ? 2 * kTileM : kTileM;
-  const int64_t tiles = c.experts * ((c.outer + tile_rows - 1) / tile_rows) * ((c.inner + bn - 1) / bn);
-  const int64_t parts = std::min(std::min((pairs ? 74 : 148) / tiles, c.rows / (256 * (int64_t)c.experts)),
-                                 (int64_t)(kMaxExperts / c.experts));
+  const int64_t tiles =
+      c.experts * ((c.outer + tile_rows - 1) / tile_rows) * ((c.inner + bn - 1) / bn);
+  const int64_t parts = std::min({(pairs ? 74 : 148) / tiles, c.rows / (256 * (int64_t)c.experts),
+                                  (int64_t)(kMaxExperts / c.experts)});
   return c.dw && parts > 1 ? (int)parts : 1;
 }
 static int64_t parts_bytes(const MatmulCall& c) {
