@@ -214,18 +214,20 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   const int gq = lane >> 2, tq = lane & 3;  // row and column quad of the matrix fragments
 
   // The item of this block: rows [begin, begin + n) of one expert. Items are numbered expert
-  // by expert, then the rows past the last offset (expert = experts: zeros).
+  // by expert, then the rows past the last offset and those before the first (expert >= experts:
+  // zeros).
   if (warp == 0) {
     int want = blockIdx.x / (g.blocks * g.split);
     bool found = false;
-    for (int i0 = 0; i0 <= g.experts && !found; i0 += 32) {
+    for (int i0 = 0; i0 <= g.experts + 1 && !found; i0 += 32) {
       const int e = i0 + lane;
       int64_t b = 0, n = 0;
-      if (e <= g.experts) {
-        b = min(max((int64_t)g.offsets[e], (int64_t)0), g.rows);
+      if (e <= g.experts + 1) {
+        b = min(max((int64_t)g.offsets[e <= g.experts ? e : 0], (int64_t)0), g.rows);
         const int64_t end =
             e < g.experts ? min(max((int64_t)g.offsets[e + 1], b), g.rows) : g.rows;
         n = end - b;
+        if (e > g.experts) n = b, b = 0;
       }
       const int items = (int)((n + kFewRows - 1) / kFewRows);
       int s = items;
@@ -253,7 +255,7 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   const int out0 = blockIdx.x / g.split % g.blocks * kOutBlock;
   const int k_begin = rank * g.slice, k_end = min(g.inner, k_begin + g.slice);
   T* y = static_cast<T*>(g.y);
-  if (expert == g.experts) {
+  if (expert >= g.experts) {
     if (rank == 0)
       for (int i = threadIdx.x; i < nrows * kOutBlock; i += kFewThreads) {
         const int r = i / kOutBlock, n = out0 + i % kOutBlock;
@@ -584,7 +586,8 @@ cudaError_t launch_few_shape(FewArgs g, cudaStream_t st) {
     ready[dev].store(true, std::memory_order_release);
   }
   const int64_t blocks = (g.outer + kOutBlock - 1) / kOutBlock;
-  const int64_t items = std::min<int64_t>(g.experts + 1, g.rows) + g.rows / S::kRows;
+  // every group of rows, the two without an expert among them, has one ragged item at most
+  const int64_t items = std::min<int64_t>(g.experts + 2, g.rows) + g.rows / S::kRows;
   // Split the inner axis, in steps of at least 512, while the blocks would not fill the SMs.
   const int64_t busy = blocks * std::min<int64_t>(g.experts, g.rows);
   int split = 1;

@@ -27,7 +27,7 @@
 //
 // Ragged ends. FORWARD / INPUT: a tile's rows past its group's end are computed from the next
 // group's rows and not stored (a row of A only reaches its own row of D). Rows past the last
-// group form one more group without a reduction: zeros. WEIGHT: the reduction itself ends
+// group and rows before the first form two more groups without a reduction: zeros. WEIGHT: the reduction itself ends
 // inside a block. Steps of 16 past the end are left out, and in the last step the rows past
 // it are overwritten with zeros in shared memory, in both operands: an infinity or NaN of the
 // next group cannot make 0 * inf. In a pair each CTA's second warp does that to its own half
@@ -66,6 +66,9 @@ constexpr int kTileK = 64;         // 128 bytes of a 16-bit type: one swizzle ro
 constexpr int kStoreRow = 64;      // bytes of a row in a storing warp's staging block
 constexpr int kBandRows = 2048;    // rows of D of a band, see tile_of
 constexpr uint64_t kWaitNs = 2000000000;
+// Entries of the table of groups: the experts, the rows past the last and before the first, the
+// end.
+constexpr int kGroupSlots = kMaxExperts + 3;
 
 enum Mode { FORWARD = 0, INPUT = 1, WEIGHT = 2, WEIGHT_F32 = 3 };
 constexpr int kRun = 768;  // rows of a run of WEIGHT_F32
@@ -296,7 +299,7 @@ struct Shape {
   static constexpr int kTmemCols = 2 * BN;                              // two accumulators
   static constexpr int kBand = kBandRows / kRows;
   static constexpr int kSmem =
-      1024 + kStages * kStageBytes + kStoreBytes + 8 * (kMaxExperts + 2) + 512;
+      1024 + kStages * kStageBytes + kStoreBytes + 8 * kGroupSlots + 512;
 };
 
 // Where piece `p` (16 bytes) of row `row` lies in a staging block: the 64-byte swizzle of TMA.
@@ -366,9 +369,9 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
   const uint32_t base = smem_addr(smem);
   const uint32_t store_base = base + kStages * S::kStageBytes;
   int32_t* cum = reinterpret_cast<int32_t*>(smem + kStages * S::kStageBytes + S::kStoreBytes);
-  int32_t* off = cum + kMaxExperts + 2;  // the groups' first rows, then the end
+  int32_t* off = cum + kGroupSlots;  // the experts' first rows, the last one's end, all rows
   uint64_t* bars = reinterpret_cast<uint64_t*>(
-      (reinterpret_cast<uintptr_t>(off + kMaxExperts + 2) + 15) & ~(uintptr_t)15);
+      (reinterpret_cast<uintptr_t>(off + kGroupSlots) + 15) & ~(uintptr_t)15);
   // end_full, end_peer (WEIGHT): a group's last block has landed in this CTA; the odd CTA has
   // zeroed its rows past the end. Used in turn, one a last block.
   const uint32_t full = smem_addr(bars), empty = full + 8 * kStages,
@@ -410,8 +413,8 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     }
   } else if (warp == 2) {
     // The groups' rows, clamped (off[i] to off[i + 1]; overlaps of offsets that decrease are
-    // cut off), and the first tile of every group. The rows past the last offset are one
-    // group more; WEIGHT has no tiles for them.
+    // cut off), and the first tile of every group. The rows past the last offset are one group
+    // more, those before the first another; WEIGHT has no tiles for them.
     const int nt = (g.cols + BN - 1) / BN;
     int32_t carry = 0, reach = 0;
     const int experts = MODE == WEIGHT ? g.experts / g.parts : g.experts;
@@ -441,40 +444,41 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     }
     if (lane == 0) off[g.experts + 1] = (int32_t)g.rows;
     __syncwarp();
-    for (int i0 = 0; i0 <= g.experts; i0 += 32) {
+    for (int i0 = 0; i0 <= g.experts + 1; i0 += 32) {
       const int i = i0 + lane;
       int32_t v = 0;
       if (MODE == WEIGHT)
         v = i < g.experts ? (g.drows + S::kRows - 1) / S::kRows * nt : 0;
-      else if (i <= g.experts)
-        v = (off[i + 1] - off[i] + S::kRows - 1) / S::kRows * nt;
+      else if (i <= g.experts + 1)
+        v = ((i <= g.experts ? off[i + 1] - off[i] : off[0]) + S::kRows - 1) / S::kRows * nt;
       int32_t s = v;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int32_t o = __shfl_up_sync(0xFFFFFFFFu, s, d);
         if (lane >= d) s += o;
       }
-      if (i <= g.experts) cum[i] = carry + s - v;
+      if (i <= g.experts + 1) cum[i] = carry + s - v;
       carry += __shfl_sync(0xFFFFFFFFu, s, 31);
     }
-    if (lane == 0) cum[g.experts + 1] = carry;
+    if (lane == 0) cum[g.experts + 2] = carry;
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if constexpr (CTAS == 2) cluster_sync();  // the other CTA's barriers are set up too
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  const int tiles = cum[g.experts + 1];
+  const int tiles = cum[g.experts + 2];
   const int nt = (g.cols + BN - 1) / BN;
   const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   auto decode = [&](int t) {
-    int lo = 0, hi = g.experts + 1;  // the last group that starts at or before t
+    int lo = 0, hi = g.experts + 2;  // the last group that starts at or before t
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (cum[mid] <= t) lo = mid; else hi = mid;
     }
-    const int b = off[lo], e = off[lo + 1];
+    const bool lead = lo > g.experts;  // the rows before the first expert's
+    const int b = lead ? 0 : off[lo], e = lead ? off[0] : off[lo + 1];
     Tile r;
     r.group = lo;
     int m, n;
@@ -1019,7 +1023,7 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
     const int64_t nt = (g.cols + BN - 1) / BN;
     const int64_t most = MODE == WEIGHT
                              ? (int64_t)g.experts * ((g.drows + S::kRows - 1) / S::kRows) * nt
-                             : (g.rows / S::kRows + g.experts + 1) * nt;
+                             : (g.rows / S::kRows + g.experts + 2) * nt;
     if (MODE == WEIGHT && g.out_kind == LGBM_B200_DTYPE_F32)
       return launch_tiles<WEIGHT_F32, BN, CTAS>(maps, g, most, st);
     return launch_tiles<MODE, BN, CTAS>(maps, g, most, st);
