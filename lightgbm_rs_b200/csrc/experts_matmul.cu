@@ -66,8 +66,8 @@ constexpr int kTileK = 64;         // 128 bytes of a 16-bit type: one swizzle ro
 constexpr int kStoreRow = 64;      // bytes of a row in a storing warp's staging block
 constexpr int kBandRows = 2048;    // rows of D of a band, see tile_of
 constexpr uint64_t kWaitNs = 2000000000;
-// Entries of the table of groups: the experts, the rows past the last and before the first, the
-// end.
+// Entries of the table of groups: the rows before the first expert's, the experts, the rows past
+// the last one's, the end.
 constexpr int kGroupSlots = kMaxExperts + 3;
 
 enum Mode { FORWARD = 0, INPUT = 1, WEIGHT = 2, WEIGHT_F32 = 3 };
@@ -268,7 +268,7 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint
 }
 
 struct Tile {
-  int32_t group;
+  int32_t expert;
   int32_t m0;      // first row of D: of all rows (FORWARD, INPUT), of the group (WEIGHT)
   int32_t m_end;   // rows of D end here
   int32_t n0;
@@ -360,6 +360,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     k_grouped_matmul(const __grid_constant__ Maps maps, const MatArgs g) {
   using S = Shape<KIND, BN, CTAS>;
   constexpr int MODE = KIND == WEIGHT_F32 ? (int)WEIGHT : KIND;
+  constexpr int kLead = MODE == WEIGHT ? 0 : 1;  // groups before the first expert's
   constexpr bool kRuns = KIND == WEIGHT_F32;
   constexpr int kStages = S::kStages;
   constexpr uint32_t kABytes = kTileM * 128;
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
   const uint32_t base = smem_addr(smem);
   const uint32_t store_base = base + kStages * S::kStageBytes;
   int32_t* cum = reinterpret_cast<int32_t*>(smem + kStages * S::kStageBytes + S::kStoreBytes);
-  int32_t* off = cum + kGroupSlots;  // the experts' first rows, the last one's end, all rows
+  int32_t* off = cum + kGroupSlots;  // the groups' first rows, then the end
   uint64_t* bars = reinterpret_cast<uint64_t*>(
       (reinterpret_cast<uintptr_t>(off + kGroupSlots) + 15) & ~(uintptr_t)15);
   // end_full, end_peer (WEIGHT): a group's last block has landed in this CTA; the odd CTA has
@@ -378,6 +379,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
                  acc_full = empty + 8 * kStages, acc_empty = acc_full + 16,
                  end_full = acc_empty + 16, end_peer = end_full + 8 * kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * kStages + 4);
+  const int groups = g.experts + 2 * kLead;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CTAS == 2 ? blockIdx.x & 1 : 0;  // in the pair; the even CTA multiplies
 
@@ -413,8 +415,8 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     }
   } else if (warp == 2) {
     // The groups' rows, clamped (off[i] to off[i + 1]; overlaps of offsets that decrease are
-    // cut off), and the first tile of every group. The rows past the last offset are one group
-    // more, those before the first another; WEIGHT has no tiles for them.
+    // cut off), and the first tile of every group. The rows before the first offset are a group
+    // of their own and so are those past the last; WEIGHT needs neither.
     const int nt = (g.cols + BN - 1) / BN;
     int32_t carry = 0, reach = 0;
     const int experts = MODE == WEIGHT ? g.experts / g.parts : g.experts;
@@ -428,7 +430,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
         if (lane >= d) b = max(b, o);
       }
       reach = __shfl_sync(0xFFFFFFFFu, b, 31);
-      if (i <= experts) off[i] = b;
+      if (i <= experts) off[kLead + i] = b;
     }
     if (MODE == WEIGHT && g.parts > 1) {  // each expert's rows in equal parts of whole blocks
       __syncwarp();
@@ -442,45 +444,45 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
       for (int i = lane; i <= g.experts; i += 32) off[i] = cum[i];
       __syncwarp();
     }
-    if (lane == 0) off[g.experts + 1] = (int32_t)g.rows;
+    if (kLead > 0 && lane == 0) {
+      off[0] = 0;
+      off[kLead + g.experts + 1] = (int32_t)g.rows;
+    }
     __syncwarp();
-    for (int i0 = 0; i0 <= g.experts + 1; i0 += 32) {
+    for (int i0 = 0; i0 < groups; i0 += 32) {
       const int i = i0 + lane;
       int32_t v = 0;
-      if (MODE == WEIGHT)
-        v = i < g.experts ? (g.drows + S::kRows - 1) / S::kRows * nt : 0;
-      else if (i <= g.experts + 1)
-        v = ((i <= g.experts ? off[i + 1] - off[i] : off[0]) + S::kRows - 1) / S::kRows * nt;
+      if (i < groups)
+        v = ((MODE == WEIGHT ? g.drows : off[i + 1] - off[i]) + S::kRows - 1) / S::kRows * nt;
       int32_t s = v;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int32_t o = __shfl_up_sync(0xFFFFFFFFu, s, d);
         if (lane >= d) s += o;
       }
-      if (i <= g.experts + 1) cum[i] = carry + s - v;
+      if (i < groups) cum[i] = carry + s - v;
       carry += __shfl_sync(0xFFFFFFFFu, s, 31);
     }
-    if (lane == 0) cum[g.experts + 2] = carry;
+    if (lane == 0) cum[groups] = carry;
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if constexpr (CTAS == 2) cluster_sync();  // the other CTA's barriers are set up too
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  const int tiles = cum[g.experts + 2];
+  const int tiles = cum[groups];
   const int nt = (g.cols + BN - 1) / BN;
   const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   auto decode = [&](int t) {
-    int lo = 0, hi = g.experts + 2;  // the last group that starts at or before t
+    int lo = 0, hi = groups;  // the last group that starts at or before t
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (cum[mid] <= t) lo = mid; else hi = mid;
     }
-    const bool lead = lo > g.experts;  // the rows before the first expert's
-    const int b = lead ? 0 : off[lo], e = lead ? off[0] : off[lo + 1];
+    const int b = off[lo], e = off[lo + 1];
     Tile r;
-    r.group = lo;
+    r.expert = lo - kLead;
     int m, n;
     const int drows = MODE == WEIGHT ? g.drows : e - b;
     tile_of(t - cum[lo], (drows + S::kRows - 1) / S::kRows, nt, S::kBand, m, n);
@@ -500,7 +502,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
       r.m0 += b;
       r.m_end = e;
       r.red0 = 0;
-      r.red = lo < g.experts ? g.reduction : 0;
+      r.red = r.expert >= 0 && r.expert < g.experts ? g.reduction : 0;
     }
     return r;
   };
@@ -536,11 +538,11 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
           } else {
             tma_load_2d<CTAS>(a, &maps.a, k0, r.m0, bar);
             if (MODE == FORWARD) {
-              tma_load_3d<CTAS>(b, &maps.b, k0, nb, r.group, bar);
+              tma_load_3d<CTAS>(b, &maps.b, k0, nb, r.expert, bar);
             } else {
 #pragma unroll
               for (int j = 0; j < S::kCols / 64; ++j)
-                tma_load_3d<CTAS>(b + j * 8192, &maps.b, nb + 64 * j, k0, r.group, bar);
+                tma_load_3d<CTAS>(b + j * 8192, &maps.b, nb + 64 * j, k0, r.expert, bar);
             }
           }
         }
@@ -639,8 +641,8 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
       char* out = static_cast<char*>(g.out);
       int out_row = row0;  // of D as one matrix
       if (MODE == WEIGHT) {
-        out += (int64_t)r.group * g.drows * pitch;
-        out_row += r.group * g.drows;
+        out += (int64_t)r.expert * g.drows * pitch;
+        out_row += r.expert * g.drows;
       }
       const int ncols = min(BN, g.cols - r.n0), nrows = min(32, r.m_end - row0);
       // whole 32-row blocks leave by TMA, which also cuts off the last columns
