@@ -418,11 +418,25 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
         }
   };
 
-  float acc[TILES][4];
+  // acc is what the matrix instructions add to. They cut off at most 2^-23 of it each time, so
+  // with weights of 16 bits a panel's sums (at most 32 times) go to `total`, in f32; 4-bit
+  // weights' leave them at every scale group.
+  float acc[TILES][4], total[TILES][4];
 #pragma unroll
   for (int j = 0; j < TILES; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+    for (int i = 0; i < 4; ++i) acc[j][i] = total[j][i] = 0.0f;
+  auto keep_sums = [&] {
+    if constexpr (!W4) {
+#pragma unroll
+      for (int j = 0; j < TILES; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          total[j][i] += acc[j][i];
+          acc[j][i] = 0.0f;
+        }
+    }
+  };
 
 #pragma unroll
   for (int i = 0; i < kRing - 1; ++i) load_stage(i);
@@ -439,6 +453,7 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
     if (kp == g.panel) {
       kp = 0;
       if (i > 0) __syncthreads();
+      keep_sums();
       keep_tokens(i == 0);
       __syncthreads();
       fetch_tokens(k_begin + i * S::kStageInner + g.panel);
@@ -536,6 +551,7 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 
+  keep_sums();
   // partial sums as [row][output], over the tokens; with a split inner axis the blocks of
   // the cluster each add up and store a share of the rows
   __syncthreads();
@@ -544,10 +560,10 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   for (int n = 0; n < TILES; ++n)
     if (n < tiles) {
       float* at = sums + (n * 8 + 2 * tq) * kOutBlock + warp * 16 + gq;
-      at[0] = acc[n][0];
-      at[kOutBlock] = acc[n][1];
-      at[8] = acc[n][2];
-      at[kOutBlock + 8] = acc[n][3];
+      at[0] = W4 ? acc[n][0] : total[n][0];
+      at[kOutBlock] = W4 ? acc[n][1] : total[n][1];
+      at[8] = W4 ? acc[n][2] : total[n][2];
+      at[kOutBlock + 8] = W4 ? acc[n][3] : total[n][3];
     }
   if (g.split == 1) {
     __syncthreads();

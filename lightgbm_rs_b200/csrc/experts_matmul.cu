@@ -34,12 +34,19 @@
 // and the odd one tells the even one. (Gathering that block's rows one by one, with zeros
 // from TMA for those outside, took five times a block's time, once a tile.)
 //
-// Precision. The tensor cores cut a sum off when they add to it: on sums of random signs the
-// error grew with the length, 1.5e-5 of the result at 4096 rows (f32 sums in another order:
-// 2e-7 to 9e-7). A result rounded to 16 bits does not show it. A weight gradient kept in f32
-// would, so there the reduction is accumulated in runs of 768 rows, alternating between the
-// two halves of tensor memory, and the storing warps, twice as many there so that the sums fit
-// their registers, add the runs up in f32: 7e-7 whatever the length.
+// Precision. The tensor cores cut a sum off when they add to it: 16 terms at a time, at most
+// 2^-23 of the sum each time. With terms of one sign nearly all of that was measured at every
+// addition: 1.6e-3 of the result at 2^18 terms in one piece, three times f16's unit roundoff.
+// A reduction is therefore accumulated in runs, which the storing warps add up in f32
+// (a rounding of 2^-24 a run). Results of 16 bits: runs of 4096, which cut off at most 3.1e-5, a
+// sixteenth of f16's unit roundoff. The second run on goes to the other half of tensor memory
+// and is added to the first half there, while the tensor cores wait (16 groups of 4096 rows on
+// average, 4096 x 2048: 2 %). Holding the sums in registers instead cost the tiles of one run up
+// to 45 % (255 experts of 129 x 700: the code of their odd stores spilled). A weight
+// gradient kept in f32 would show runs of that length, so there they are of 768, alternate
+// between the halves without a wait, and the sums stay in the registers of twice as many storing
+// warps: 7e-7 of the result up to 2^16 rows of random sign (1.3e-6 of one sign), 1.0e-6 (1.4e-6)
+// at 2^20, against 1.7e-5 (1.2e-4) of f32 sums one by one.
 //
 // Measured, loops on a warm GPU: 65536 rows, 16 experts of 4096 x 2048: y 0.90, dx 0.90, dw
 // 0.90 (bf16) and 1.04 ms (f32), 1.2 PFLOP/s with the clock held near 1.3 GHz by the power
@@ -71,7 +78,6 @@ constexpr uint64_t kWaitNs = 2000000000;
 constexpr int kGroupSlots = kMaxExperts + 3;
 
 enum Mode { FORWARD = 0, INPUT = 1, WEIGHT = 2, WEIGHT_F32 = 3 };
-constexpr int kRun = 768;  // rows of a run of WEIGHT_F32
 
 struct MatArgs {
   const int32_t* offsets;
@@ -236,6 +242,14 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
         "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 "
+      "[%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -290,6 +304,7 @@ __device__ __forceinline__ void tile_of(int t, int mt, int nt, int band, int& m,
 template <int KIND, int BN, int CTAS>
 struct Shape {
   static constexpr int kStoreWarps = KIND == WEIGHT_F32 ? 16 : 8;
+  static constexpr int kRun = KIND == WEIGHT_F32 ? 768 : 4096;  // see "Precision" above
   static constexpr int kThreads = 64 + 32 * kStoreWarps;
   static constexpr int kStoreBytes = kStoreWarps * 32 * kStoreRow;
   static constexpr int kRows = kTileM * CTAS;
@@ -361,7 +376,8 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
   using S = Shape<KIND, BN, CTAS>;
   constexpr int MODE = KIND == WEIGHT_F32 ? (int)WEIGHT : KIND;
   constexpr int kLead = MODE == WEIGHT ? 0 : 1;  // groups before the first expert's
-  constexpr bool kRuns = KIND == WEIGHT_F32;
+  constexpr bool kWide = KIND == WEIGHT_F32;  // results of 32 bits
+  constexpr int kRun = S::kRun;
   constexpr int kStages = S::kStages;
   constexpr uint32_t kABytes = kTileM * 128;
   extern __shared__ uint8_t smem_raw[];
@@ -507,6 +523,16 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     return r;
   };
 
+  // The half of tensor memory that run `run` of a tile goes to, and how often it was used before:
+  // the multiplying and the storing warps count alike. WEIGHT_F32's runs alternate between the
+  // halves; the others' tiles do, and their later runs all take the half that the first has not.
+  uint32_t half = 1, used0 = 0, used1 = 0;
+  auto take = [&](int run, uint32_t& acc) {
+    if (kWide || run == 0) half ^= 1;
+    acc = kWide || run == 0 ? half : half ^ 1;
+    return acc ? used1++ : used0++;
+  };
+
   bool ok = true;
   if (warp == 0) {
     uint32_t it = 0, ends = 0;
@@ -558,17 +584,17 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
       if (ends > 0) bar_wait(end_full + 8 * ((ends - 1) % kStages), ((ends - 1) / kStages) & 1);
     }
   } else if (warp == 1) {
-    uint32_t it = 0, tile = 0, ends = 0;  // tile: accumulations so far, one or more a tile
+    uint32_t it = 0, ends = 0;
     for (int t = first; ok && t < tiles; t += step) {
       const Tile r = decode(t);
       uint32_t acc = 0, d = 0;
       for (int k0 = 0; k0 < r.red; k0 += kTileK, ++it) {
-        const bool begin = kRuns ? k0 % kRun == 0 : k0 == 0;
+        const bool begin = k0 % kRun == 0;
         if (begin) {
-          acc = tile & 1;
+          const uint32_t used = take(k0 / kRun, acc);
           d = tmem + acc * BN;
           if (rank == 0) {
-            if (tile >= 2 && !(ok = bar_wait(acc_empty + 8 * acc, (tile / 2 - 1) & 1))) break;
+            if (used > 0 && !(ok = bar_wait(acc_empty + 8 * acc, (used - 1) & 1))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           }
         }
@@ -595,8 +621,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
             break;
           }
         }
-        const bool done = k0 + kTileK >= r.red || (kRuns && (k0 + kTileK) % kRun == 0);
-        if (done) ++tile;
+        const bool done = k0 + kTileK >= r.red || (k0 + kTileK) % kRun == 0;
         if (rank == 1) continue;  // the even CTA multiplies for both
         if (!(ok = bar_wait(full + 8 * s, (it / kStages) & 1))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -619,22 +644,22 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     const int quarter = warp & 3, part = (warp - 2) >> 2;  // of the lanes; of the chunks
     constexpr int kParts = S::kStoreWarps / 4;
     const uint32_t stage = store_base + (warp - 2) * 32 * kStoreRow;
-    constexpr int bytes = kRuns ? 4 : 2;
+    constexpr int bytes = kWide ? 4 : 2;
     constexpr int per_chunk = kStoreRow / bytes;  // columns of a staging row
     const int64_t pitch = g.out_pitch * bytes;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    auto accumulated = [&](uint32_t tile) {  // accumulation `tile` is complete
-      if (!bar_wait(acc_full + 8 * (tile & 1), (tile / 2) & 1)) return false;
+    auto accumulated = [&](int run, uint32_t& acc) {  // waits for that run
+      const uint32_t used = take(run, acc);
+      if (!bar_wait(acc_full + 8 * acc, used & 1)) return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       return true;
     };
-    auto release = [&](uint32_t tile) {  // and has been read
+    auto release = [&](uint32_t acc) {  // this half has been read
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      const uint32_t bar = acc_empty + 8 * (tile & 1);
+      const uint32_t bar = acc_empty + 8 * acc;
       if (lane == 0) bar_arrive_cluster(CTAS == 2 ? leader_addr(bar) : bar);
     };
-    uint32_t tile = 0;
     for (int t = first; ok && t < tiles; t += step) {
       const Tile r = decode(t);
       const int row0 = r.m0 + quarter * 32;
@@ -678,16 +703,17 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
         }
         __syncwarp();
       };
-      if (kRuns && r.red > kRun) {
+      uint32_t acc = 0;
+      if (kWide && r.red > kRun) {
         constexpr int kMine = BN / per_chunk / kParts;  // chunks of this warp
         uint32_t sum[kMine][16];
 #pragma unroll
         for (int i = 0; i < kMine; ++i)
 #pragma unroll
           for (int j = 0; j < 16; ++j) sum[i][j] = 0;
-        for (int k0 = 0; k0 < r.red; k0 += kRun, ++tile) {
-          if (!(ok = accumulated(tile))) break;
-          const uint32_t from = tmem + (tile & 1) * BN + lanes + part * per_chunk;
+        for (int k0 = 0; k0 < r.red; k0 += kRun) {
+          if (!(ok = accumulated(k0 / kRun, acc))) break;
+          const uint32_t from = tmem + acc * BN + lanes + part * per_chunk;
 #pragma unroll
           for (int i = 0; i < kMine; ++i) {
             uint32_t v[16];
@@ -697,7 +723,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
             for (int j = 0; j < 16; ++j)
               sum[i][j] = __float_as_uint(__uint_as_float(sum[i][j]) + __uint_as_float(v[j]));
           }
-          release(tile);
+          release(acc);
         }
         if (!ok) break;
 #pragma unroll
@@ -705,14 +731,37 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
           if ((i * kParts + part) * per_chunk < ncols && nrows > 0)
             put(sum[i], (i * kParts + part) * per_chunk);
       } else {
-        if (r.red > 0 && !(ok = accumulated(tile))) break;
-        const uint32_t from = tmem + (tile & 1) * BN + lanes;
+        if (r.red > 0 && !(ok = accumulated(0, acc))) break;
+        const uint32_t from = tmem + acc * BN + lanes;
+        if constexpr (!kWide) {
+          // each later run is added to the first one's half, where the sum leaves from
+          for (int k0 = kRun; k0 < r.red; k0 += kRun) {
+            uint32_t other;
+            if (!(ok = accumulated(k0 / kRun, other))) break;
+#pragma unroll 1
+            for (int c0 = part * per_chunk; c0 < BN; c0 += kParts * per_chunk)
+#pragma unroll 1
+              for (int c = c0; c < c0 + per_chunk; c += 16) {
+                uint32_t sum[16], v[16];
+                tmem_load16(from + c, sum);
+                tmem_load16(tmem + other * BN + lanes + c, v);
+                tmem_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  sum[j] = __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(v[j]));
+                tmem_store16(from + c, sum);
+              }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            release(other);
+          }
+          if (!ok) break;
+        }
         for (int c0 = part * per_chunk; c0 < ncols && nrows > 0; c0 += kParts * per_chunk) {
           uint32_t v[32], w[16];
           if (r.red == 0) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = 0;
-          } else if constexpr (kRuns) {
+          } else if constexpr (kWide) {
             tmem_load16(from + c0, w);
             tmem_wait();
           } else {
@@ -728,7 +777,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
           }
           put(w, c0);
         }
-        if (r.red > 0) release(tile++);
+        if (r.red > 0) release(acc);
       }
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");

@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_experts import gen, offsets_of, product64, unpacked  # noqa: E402
+from test_gpu_experts import DTYPES, UNIT, gen, offsets_of, product64, unpacked  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -96,3 +96,71 @@ def test_a_shard_of_the_experts(ops):
     lo, hi = int(off[2]), int(off[5])
     assert torch.equal(part[lo:hi], whole[lo:hi])
     assert not part[:lo].any() and not part[hi:].any()
+
+
+# --------------------------------------------------------------------------- long sums
+
+
+RUN = 4096  # longest sum the tensor cores make in one piece for a result of 16 bits
+
+
+def spread(g, rows, cols, dtype, lo=0.0):
+    """Numbers of one sign whose columns have scales in [1/2, 1): sums over the rows fall evenly
+    over the result type's spacings, so that its roundings cancel in the mean."""
+    t = torch.rand(rows, cols, generator=g, device="cuda") / 16
+    return t.mul_(torch.rand(cols, generator=g, device="cuda") / 2 + 0.5).to(dtype)
+
+
+def bias(got, want):
+    return float(((got.double() - want) / want).mean())
+
+
+def bias_limit(n, dtype, independent):
+    """Adding to a sum cuts off at most 2^-23 of it, RUN / 16 times in a run; the n / RUN runs are
+    added in f32. The result's rounding (at most a unit, half of it in the root mean square)
+    cancels over `independent` results, to six standard deviations."""
+    return (RUN / 16 + n / (2 * RUN)) * 2.0 ** -23 + 6 * UNIT[dtype] / 2 / math.sqrt(independent)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n,inner,outer", [(1 << 18, 1536, 2048), (1 << 17, 64, 9600),
+                                           (1 << 17, 128, 9600), (1 << 17, 19200, 100)])
+def test_weight_gradient_of_long_groups(ops, n, inner, outer, dtype):
+    """One expert, outputs enough that its rows are not summed in parts, all terms of one sign:
+    what the additions cut off adds up. In one piece it is 1.6e-3 of the result at 2^18 rows."""
+    dt, g = DTYPES[dtype], gen(n + inner)
+    x, dy = spread(g, n, inner, dt), spread(g, n, outer, dt)
+    w = torch.empty(2, outer, inner, device="cuda", dtype=dt)
+    off = offsets_of([n, 0])
+    dw = ops.grouped_matmul_backward(dy, x, w, off, need_dx=False)[1]
+    want = torch.zeros(outer, inner, device="cuda", dtype=torch.float64)
+    for r in range(0, n, 1 << 14):
+        want += dy[r:r + (1 << 14)].double().T @ x[r:r + (1 << 14)].double()
+    assert abs(bias(dw[0], want)) <= bias_limit(n, dt, max(inner, outer))
+    # each element: as above, and one rounding
+    lim = (RUN / 16 + n / RUN) * 2.0 ** -23 + UNIT[dt]
+    assert (((dw[0].double() - want) / want).abs() <= lim).all()
+    assert not dw[1].any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,experts,cols", [(300, 1, 64), (300, 1, 128), (300, 3, 300),
+                                               (300, 1, 300), (3, 1, 19200), (30, 1, 19200)])
+def test_products_of_long_reductions(ops, rows, experts, cols, dtype):
+    """y over 2^17 inputs and dx over 2^17 outputs, streamed (3 rows) and in every tile shape."""
+    n = 1 << 17 if cols < 1000 else 1 << 16
+    dt, g = DTYPES[dtype], gen(rows + cols)
+    a = spread(g, n, rows, dt).t().contiguous()
+    b = spread(g, n, cols, dt).t().contiguous()
+    off = offsets_of([rows // experts] * experts)
+    w = b.expand(experts, cols, n).contiguous()
+    want = torch.cat([a.double() @ b[c:c + 512].double().T for c in range(0, cols, 512)], 1)
+    got = [ops.grouped_matmul(a, w, off)]
+    del w
+    if cols < 1000:
+        w = b.t().expand(experts, n, cols).contiguous()
+        got.append(ops.grouped_matmul_backward(a, a[:, :cols], w, off, need_dw=False)[0])
+    for y in got:
+        assert abs(bias(y, want)) <= bias_limit(n, dt, max(rows, cols))
+        lim = (RUN / 16 + n / RUN) * 2.0 ** -23 + UNIT[dt]
+        assert (((y.double() - want) / want).abs() <= lim).all()
