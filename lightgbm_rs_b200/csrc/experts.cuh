@@ -47,13 +47,6 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// 2^x and e^x with ex2.approx (2 units in the last place); results below 2^-126 are 0.
-__device__ __forceinline__ float fast_exp(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
-  return r;
-}
-
 // V elements as they lie in memory (V * sizeof(T) is 16, or V is 1), to be loaded first and
 // converted later: a conversion right behind its load would wait for it.
 template <typename T, int V>

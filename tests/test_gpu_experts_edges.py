@@ -164,3 +164,25 @@ def test_products_of_long_reductions(ops, rows, experts, cols, dtype):
         assert abs(bias(y, want)) <= bias_limit(n, dt, max(rows, cols))
         lim = (RUN / 16 + n / RUN) * 2.0 ** -23 + UNIT[dt]
         assert (((y.double() - want) / want).abs() <= lim).all()
+
+
+# -------------------------------------------------------------------------------- router
+
+
+@pytest.mark.parametrize("tokens", [3, 100])
+def test_route_gradient_of_far_logits(ops, tokens):
+    """Softmax over all: the unchosen experts' gradient is -p_e p_0 g with p_e down to e^-80. In
+    units of 2^-24: exp 4 (its argument is exact here), the weight's sum of up to 7 additions and
+    quotient 8, p_0 g and the two products 3, the weight twice: 23. Results below 2^-126 are spaced
+    by 2^-149."""
+    g = gen(tokens)
+    x = -(20 + torch.randint(0, 60 * 1024, (tokens, 40), generator=g, device="cuda") / 1024)
+    x[:, 7] = 0
+    dw = torch.randn(tokens, 1, generator=g, device="cuda")
+    r = ops.route(x, 1, normalize=False)
+    d = ops.route_backward(dw, x, r, normalize=False)
+    p = x.double().softmax(1)
+    want = -p * p[:, 7:8] * dw.double()
+    off = (d.double() - want).abs()
+    off[:, 7] = 0
+    assert (off <= 24 * 2.0 ** -24 * want.abs() + 2.0 ** -150).all()
