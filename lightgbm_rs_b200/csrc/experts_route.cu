@@ -7,7 +7,6 @@ namespace experts {
 namespace {
 
 constexpr int kRouteThreads = 256;   // k_route_place
-constexpr int kRouteChunk = 64;      // logit columns staged at a time
 constexpr uint32_t kKeyEmpty = 0x007FFFFFu;  // key of -inf: never chosen
 
 // Order-preserving key of a logit: larger logit, larger key; -0 and +0 are one value, NaN
@@ -99,109 +98,6 @@ __device__ void prefix_counts(int32_t* counts, int n) {
   }
 }
 
-// The k largest logits of tokens [first, first + THREADS / L), L lanes a token: each lane
-// keeps the KP largest of its columns in registers, sorted, and the lanes' lists are merged
-// by k rounds of a maximum over (key, lowest column). Logits come through shared memory in
-// chunks of columns, so that global reads stay coalesced whatever L is.
-template <typename T, int L, int KP, int THREADS>
-__device__ void select_tokens(const T* logits, int64_t tokens, int experts, int64_t pitch,
-                              int k, bool normalize, int64_t first, uint32_t* tile,
-                              float* weights, int32_t* chosen, int (&ids)[KP]) {
-  constexpr int kTokens = THREADS / L;
-  constexpr int kStride = kRouteChunk + L;  // lanes of different tokens hit different banks
-  const int sub = threadIdx.x % L, tok = threadIdx.x / L;
-  uint32_t key[KP];
-  int idx[KP];
-#pragma unroll
-  for (int j = 0; j < KP; ++j) {
-    key[j] = kKeyEmpty;
-    idx[j] = -1;
-  }
-  float z = 0.0f;  // sum of exp(logit - largest so far) over this lane's columns
-  for (int e0 = 0; e0 < experts; e0 += kRouteChunk) {
-    const int n = min(kRouteChunk, experts - e0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < kTokens * kRouteChunk; i += THREADS) {
-      const int r = i / kRouteChunk, c = i % kRouteChunk;
-      if (c < n && first + r < tokens)
-        tile[r * kStride + c] = logit_key(to_f32<T>(logits[(first + r) * pitch + e0 + c]));
-    }
-    __syncthreads();
-    if (first + tok < tokens) {
-      const uint32_t* row = tile + tok * kStride;
-      const uint32_t top = key[0];
-      for (int c = sub; c < n; c += L) {
-        const uint32_t v = row[c];
-        if (v > key[KP - 1]) {
-          // v > key[j] fails for the entries that stay before it: equal keys keep the
-          // lower column first
-#pragma unroll
-          for (int j = KP - 1; j > 0; --j) {
-            const bool up = v > key[j - 1];
-            const bool here = v > key[j];
-            idx[j] = up ? idx[j - 1] : (here ? e0 + c : idx[j]);
-            key[j] = up ? key[j - 1] : (here ? v : key[j]);
-          }
-          if (v > key[0]) {
-            key[0] = v;
-            idx[0] = e0 + c;
-          }
-        }
-      }
-      if (!normalize && key[0] != kKeyEmpty) {
-        const float m = key_logit(key[0]);
-        if (top != key[0]) z *= top == kKeyEmpty ? 0.0f : expf(key_logit(top) - m);
-        for (int c = sub; c < n; c += L) z += expf(key_logit(row[c]) - m);
-      }
-    }
-  }
-  const uint32_t lane_top = key[0];
-  uint32_t win_key[KP];
-#pragma unroll
-  for (int j = 0; j < KP; ++j) {
-    // (key, lowest column first): the largest of the lanes' first entries
-    uint64_t best = ((uint64_t)key[0] << 32) | (uint32_t)~idx[0];
-    const uint64_t own = best;
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) {
-      const uint64_t o = __shfl_xor_sync(0xFFFFFFFFu, best, d);
-      best = o > best ? o : best;
-    }
-    win_key[j] = (uint32_t)(best >> 32);
-    ids[j] = win_key[j] == kKeyEmpty ? -1 : ~(int)(uint32_t)best;
-    if (own == best && win_key[j] != kKeyEmpty) {
-#pragma unroll
-      for (int i = 0; i + 1 < KP; ++i) {
-        key[i] = key[i + 1];
-        idx[i] = idx[i + 1];
-      }
-      key[KP - 1] = kKeyEmpty;
-      idx[KP - 1] = -1;
-    }
-  }
-  const float m = win_key[0] == kKeyEmpty ? 0.0f : key_logit(win_key[0]);
-  float e[KP];
-  float total = 0.0f;
-#pragma unroll
-  for (int j = 0; j < KP; ++j) {
-    e[j] = ids[j] >= 0 ? expf(key_logit(win_key[j]) - m) : 0.0f;
-    if (j < k) total += e[j];
-  }
-  if (!normalize) {
-    total = lane_top == kKeyEmpty ? 0.0f : z * expf(key_logit(lane_top) - m);
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
-  }
-  if (first + tok < tokens && sub == 0) {
-#pragma unroll
-    for (int j = 0; j < KP; ++j)
-      if (j < k) {
-        weights[(first + tok) * k + j] = ids[j] >= 0 ? e[j] / total : 0.0f;
-        chosen[(first + tok) * k + j] = ids[j];
-      }
-  }
-}
-
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -209,13 +105,121 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // e^x for a term of a softmax's sum, x <= 0, in two instructions (with expf routing 65521 x 255
-// takes 55.4 us instead of 51.6). The product is rounded, so a term is off by (|x| + 4) 2^-24 of itself. In the sum
-// that is at most (ln E + 4) 2^-24 of the whole, 10 units for 512 experts, since the mean of |x|
-// under the softmax is its entropy less ln of the sum. A single term's result takes expf.
+// takes 55.4 us instead of 51.6). The product is rounded, so a term is off by (|x| + 4) 2^-24 of
+// itself. In the sum that is at most (ln E + 4) 2^-24 of the whole, 10 units for 512 experts,
+// since the mean of |x| under the softmax is its entropy less ln of the sum. A result that is a
+// single term takes expf.
 __device__ __forceinline__ float exp_term(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
   return r;
+}
+
+struct Choice {
+  int id;            // an expert, -1: none left
+  float own, total;  // weight: own / total
+  __device__ __forceinline__ float weight() const { return id >= 0 ? own / total : 0.0f; }
+};
+
+// One token's choice by a warp, the j-th in lane j: expert i * 32 + lane is v[i], -inf where there
+// is none. Searching all registers once a choice
+// is what would cost most, so with CN < NV the choice has two stages: the k lanes with the
+// largest maxima (ties to the lower expert) hold the k largest logits among them, since each lane
+// left out has k elements before all of its own; their k * NV logits are dealt out to the 32
+// lanes, CN each, and the k choices are made there, each one a maximum over the warp, the first
+// expert that holds it, and its removal. Keys order as the logits do, with NaN above everything.
+// The weights' bits depend on the token alone, not on NV, CN or the batch.
+template <int NV, int CN>
+__device__ __forceinline__ Choice choose(const float (&v)[NV], int k, bool normalize) {
+  constexpr uint32_t kAll = 0xFFFFFFFFu;
+  constexpr bool kTwoStages = CN < NV;
+  const int lane = threadIdx.x & 31;
+  const float kNone = -__int_as_float(0x7F800000);
+  float top = v[0];
+#pragma unroll
+  for (int i = 1; i < NV; ++i) top = max_nan(top, v[i]);
+
+  uint32_t key[CN];
+  int id[CN];  // expert of a candidate
+  if constexpr (kTwoStages) {
+    // this lane's first register that holds its maximum (NaN: the first NaN)
+    int at = 0;
+#pragma unroll
+    for (int i = NV - 1; i >= 0; --i)
+      if (v[i] == top) at = i;
+    if (top != top) {
+#pragma unroll
+      for (int i = NV - 1; i >= 0; --i)
+        if (v[i] != v[i]) at = i;
+    }
+    uint32_t lane_key = logit_key(top);
+    int from[CN];  // lane that this lane's candidates come from: number (32 c + lane) / NV
+#pragma unroll
+    for (int c = 0; c < CN; ++c) from[c] = -1;
+    for (int j = 0; j < k; ++j) {
+      const uint32_t best = __reduce_max_sync(kAll, lane_key);
+      if (best == kKeyEmpty) break;
+      const int owner = (int)(__reduce_min_sync(kAll, lane_key == best
+                                                          ? (uint32_t)(at * 32 + lane)
+                                                          : kAll) & 31);
+      if (lane == owner) lane_key = kKeyEmpty;
+#pragma unroll
+      for (int c = 0; c < CN; ++c)
+        if ((c * 32 + lane) / NV == j) from[c] = owner;
+    }
+    // candidate lane % NV of each lane's source
+#pragma unroll
+    for (int c = 0; c < CN; ++c) {
+      float x = kNone;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const float y = __shfl_sync(kAll, v[i], from[c] & 31);
+        if (lane % NV == i) x = y;
+      }
+      key[c] = from[c] < 0 ? kKeyEmpty : logit_key(x);
+      id[c] = key[c] == kKeyEmpty ? 0 : (lane % NV) * 32 + from[c];
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < CN; ++c) {
+      key[c] = logit_key(v[c]);
+      id[c] = c * 32 + lane;
+    }
+  }
+
+  uint32_t my_key = kKeyEmpty;
+  int my_id = -1;
+  float m = 0.0f;
+  for (int j = 0; j < k; ++j) {
+    uint32_t mine = key[0];
+#pragma unroll
+    for (int c = 1; c < CN; ++c) mine = max(mine, key[c]);
+    const uint32_t best = __reduce_max_sync(kAll, mine);
+    if (best == kKeyEmpty) break;  // the same in every lane
+    if (j == 0) m = key_logit(best);
+    uint32_t e = kAll;
+#pragma unroll
+    for (int c = 0; c < CN; ++c)
+      if (key[c] == best) e = min(e, (uint32_t)id[c]);
+    e = __reduce_min_sync(kAll, e);
+#pragma unroll
+    for (int c = 0; c < CN; ++c)
+      if ((uint32_t)id[c] == e) key[c] = kKeyEmpty;
+    if (lane == j) {
+      my_key = best;
+      my_id = (int)e;
+    }
+  }
+  const float mine = my_id >= 0 ? expf(key_logit(my_key) - m) : 0.0f;
+  float total = mine;
+  if (!normalize) {
+    total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) total += exp_term(v[i] - m);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(kAll, total, d);
+  return {my_id, mine, total};
 }
 
 constexpr int kSelectThreads = 256;
@@ -230,25 +234,16 @@ int select_tokens_of(int64_t tokens) {
 }
 
 // First of three launches for many tokens: choice and weights, and each block's rows per
-// expert. A warp a token, its logits in registers, expert e in lane e % 32; the next token's
-// are on their way meanwhile. Searching all registers once a choice is what would cost most,
-// so the choice has two stages: the k lanes with the largest maxima (ties to the lower
-// expert) hold the k largest logits among them, since each lane left out has k elements
-// before all of its own; their k * NV logits are dealt out to the 32 lanes, CN each, and the
-// k choices are made there, each one a maximum over the warp, the first expert that holds
-// it, and its removal. Keys order as the logits do, with NaN above everything.
+// expert. A warp a token, its logits in registers; the next token's are on their way meanwhile.
 // Bound by instructions: 65521 rows of 255 f32 logits, k 4, take 41 us (67 MB: 1.6 TB/s) with
 // 438 instructions a row and three quarters of the issue slots used. A sorted list a thread
-// in registers (select_tokens with one lane a token) took 71 us, a search of all registers a
-// choice 64.
+// in registers took 71 us, a search of all registers a choice 64.
 template <typename T, int NV, int CN>
 __global__ void __launch_bounds__(kSelectThreads)
     k_route_select(const T* logits, int64_t tokens, int experts, int64_t pitch, int k,
                    bool normalize, int block_tokens, float* weights, int32_t* chosen,
                    int32_t* counts) {
-  constexpr uint32_t kAll = 0xFFFFFFFFu;
   constexpr int kWarps = kSelectThreads / 32;
-  constexpr bool kTwoStages = CN < NV;
   __shared__ int32_t hist[kMaxExperts + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i <= experts; i += kSelectThreads) hist[i] = 0;
@@ -269,94 +264,11 @@ __global__ void __launch_bounds__(kSelectThreads)
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] = next[i];
     if (t + 1 < last) fetch(logits + (t + 1) * pitch);
-    float top = v[0];
-#pragma unroll
-    for (int i = 1; i < NV; ++i) top = max_nan(top, v[i]);
-
-    uint32_t key[CN];
-    int id[CN];  // expert of a candidate
-    if constexpr (kTwoStages) {
-      // this lane's first register that holds its maximum (NaN: the first NaN)
-      int at = 0;
-#pragma unroll
-      for (int i = NV - 1; i >= 0; --i)
-        if (v[i] == top) at = i;
-      if (top != top) {
-#pragma unroll
-        for (int i = NV - 1; i >= 0; --i)
-          if (v[i] != v[i]) at = i;
-      }
-      uint32_t lane_key = logit_key(top);
-      int from[CN];  // lane that this lane's candidates come from: number (32 c + lane) / NV
-#pragma unroll
-      for (int c = 0; c < CN; ++c) from[c] = -1;
-      for (int j = 0; j < k; ++j) {
-        const uint32_t best = __reduce_max_sync(kAll, lane_key);
-        if (best == kKeyEmpty) break;
-        const int owner = (int)(__reduce_min_sync(kAll, lane_key == best
-                                                            ? (uint32_t)(at * 32 + lane)
-                                                            : kAll) & 31);
-        if (lane == owner) lane_key = kKeyEmpty;
-#pragma unroll
-        for (int c = 0; c < CN; ++c)
-          if ((c * 32 + lane) / NV == j) from[c] = owner;
-      }
-      // candidate lane % NV of each lane's source
-#pragma unroll
-      for (int c = 0; c < CN; ++c) {
-        float x = kNone;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const float y = __shfl_sync(kAll, v[i], from[c] & 31);
-          if (lane % NV == i) x = y;
-        }
-        key[c] = from[c] < 0 ? kKeyEmpty : logit_key(x);
-        id[c] = key[c] == kKeyEmpty ? 0 : (lane % NV) * 32 + from[c];
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < CN; ++c) {
-        key[c] = logit_key(v[c]);
-        id[c] = c * 32 + lane;
-      }
-    }
-
-    uint32_t my_key = kKeyEmpty;
-    int my_id = -1;
-    float m = 0.0f;
-    for (int j = 0; j < k; ++j) {
-      uint32_t mine = key[0];
-#pragma unroll
-      for (int c = 1; c < CN; ++c) mine = max(mine, key[c]);
-      const uint32_t best = __reduce_max_sync(kAll, mine);
-      if (best == kKeyEmpty) break;  // the same in every lane
-      if (j == 0) m = key_logit(best);
-      uint32_t e = kAll;
-#pragma unroll
-      for (int c = 0; c < CN; ++c)
-        if (key[c] == best) e = min(e, (uint32_t)id[c]);
-      e = __reduce_min_sync(kAll, e);
-#pragma unroll
-      for (int c = 0; c < CN; ++c)
-        if ((uint32_t)id[c] == e) key[c] = kKeyEmpty;
-      if (lane == j) {
-        my_key = best;
-        my_id = (int)e;
-      }
-    }
-    const float mine = my_id >= 0 ? expf(key_logit(my_key) - m) : 0.0f;
-    float total = mine;
-    if (!normalize) {
-      total = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) total += exp_term(v[i] - m);
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(kAll, total, d);
+    const Choice c = choose<NV, CN>(v, k, normalize);
     if (lane < k) {
-      weights[t * k + lane] = my_id >= 0 ? mine / total : 0.0f;
-      chosen[t * k + lane] = my_id;
-      atomicAdd(&hist[my_id < 0 ? experts : my_id], 1);
+      weights[t * k + lane] = c.weight();
+      chosen[t * k + lane] = c.id;
+      atomicAdd(&hist[c.id < 0 ? experts : c.id], 1);
     }
   }
   __syncthreads();
@@ -411,35 +323,36 @@ __global__ void __launch_bounds__(kRouteThreads)
       n, first * k, experts, k, [&](int i) { return mine[i]; }, base, hist, position, rows);
 }
 
-// A few tokens: all of it in one block and one launch, 32 lanes a token. One row of 8
-// experts: 3.5 us, of which the launch is most.
+// A few tokens: all of it in one block and one launch, a warp a token. One row of 8 experts: 2.9
+// us, of which the launch is most; 64 rows of 64, k 2, 6.5; 64 of 255, k 4, 9.8. (Three launches
+// take 8.7 at 109 rows of 199, k 6.)
 constexpr int kSmallThreads = 512;
-constexpr int kSmallTokens = 64;  // most tokens this path takes: four rounds of 16
+constexpr int kSmallTokens = 64;  // most tokens this path takes: four a warp
 
-template <typename T, int KP>
+template <typename T, int NV>
 __global__ void __launch_bounds__(kSmallThreads)
     k_route_small(const T* logits, int tokens, int experts, int64_t pitch, int k,
                   bool normalize, float* weights, int32_t* chosen, int32_t* position,
                   int32_t* rows, int32_t* offsets) {
   extern __shared__ int32_t smem[];
-  constexpr int kTokens = kSmallThreads / 32;
-  uint32_t* tile = reinterpret_cast<uint32_t*>(smem);       // kTokens * (chunk + 32)
-  int32_t* ids = smem + kTokens * (kRouteChunk + 32);       // kSmallTokens * k
-  int32_t* base = ids + kSmallTokens * kMaxChosen;          // experts + 1
-  int32_t* hist = base + experts + 1;                       // warps * (experts + 1)
+  int32_t* ids = smem;                                 // kSmallTokens * k
+  int32_t* base = ids + kSmallTokens * kMaxChosen;     // experts + 1
+  int32_t* hist = base + experts + 1;                  // warps * (experts + 1)
+  const int lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e <= experts; e += kSmallThreads) base[e] = 0;
-  for (int first = 0; first < tokens; first += kTokens) {
-    int mine[KP];
-    select_tokens<T, 32, KP, kSmallThreads>(logits, tokens, experts, pitch, k, normalize, first,
-                                            tile, weights, chosen, mine);
-    const int t = first + threadIdx.x / 32;
-    if (threadIdx.x % 32 == 0 && t < tokens) {
+  __syncthreads();
+  for (int t = threadIdx.x >> 5; t < tokens; t += kSmallThreads / 32) {
+    float v[NV];
 #pragma unroll
-      for (int j = 0; j < KP; ++j)
-        if (j < k) {
-          ids[t * k + j] = mine[j];
-          atomicAdd(&base[mine[j] < 0 ? experts : mine[j]], 1);
-        }
+    for (int i = 0; i < NV; ++i)
+      v[i] = i * 32 + lane < experts ? to_f32<T>(logits[t * pitch + i * 32 + lane])
+                                     : -__int_as_float(0x7F800000);
+    const Choice c = choose<NV, NV>(v, k, normalize);
+    if (lane < k) {
+      weights[t * k + lane] = c.weight();
+      chosen[t * k + lane] = c.id;
+      ids[t * k + lane] = c.id;
+      atomicAdd(&base[c.id < 0 ? experts : c.id], 1);
     }
   }
   __syncthreads();
@@ -511,24 +424,35 @@ __global__ void __launch_bounds__(256)
   if (id >= 0) out[id] = from_f32<T>(w * (g - s));
 }
 
-template <typename T, int KP>
+// Registers of logits a lane.
+template <typename F>
+void with_width(int experts, F&& f) {
+  if (experts <= 32) f(std::integral_constant<int, 1>());
+  else if (experts <= 64) f(std::integral_constant<int, 2>());
+  else if (experts <= 128) f(std::integral_constant<int, 4>());
+  else if (experts <= 256) f(std::integral_constant<int, 8>());
+  else f(std::integral_constant<int, 16>());
+}
+
+template <typename T>
 cudaError_t route_typed(const T* logits, int64_t tokens, int experts, int64_t pitch, int k,
                         bool normalize, float* weights, int32_t* chosen, int32_t* position,
                         int32_t* rows, int32_t* offsets, int32_t* ws, cudaStream_t st) {
   if (tokens <= kSmallTokens) {
-    const size_t smem = sizeof(int32_t) * ((kSmallThreads / 32) * (kRouteChunk + 32) +
-                                           kSmallTokens * kMaxChosen +
+    const size_t smem = sizeof(int32_t) * (kSmallTokens * kMaxChosen +
                                            (experts + 1) * (1 + kSmallThreads / 32));
-    k_route_small<T, KP><<<1, kSmallThreads, smem, st>>>(logits, (int)tokens, experts, pitch, k,
-                                                         normalize, weights, chosen, position,
-                                                         rows, offsets);
+    with_width(experts, [&](auto nv) {
+      k_route_small<T, decltype(nv)::value><<<1, kSmallThreads, smem, st>>>(
+          logits, (int)tokens, experts, pitch, k, normalize, weights, chosen, position, rows,
+          offsets);
+    });
     return cudaGetLastError();
   }
   const int block_tokens = select_tokens_of(tokens);
   const int blocks = (int)((tokens + block_tokens - 1) / block_tokens);
   int32_t* totals = ws;
   int32_t* counts = ws + experts + 1;
-  auto select = [&](auto nv) {
+  with_width(experts, [&](auto nv) {
     constexpr int NV = decltype(nv)::value;
     auto deal = [&](auto cn) {
       constexpr int CN = decltype(cn)::value < NV ? decltype(cn)::value : NV;
@@ -540,27 +464,12 @@ cudaError_t route_typed(const T* logits, int64_t tokens, int experts, int64_t pi
     else if (most <= 64) deal(std::integral_constant<int, 2>());
     else if (most <= 128) deal(std::integral_constant<int, 4>());
     else deal(std::integral_constant<int, 8>());
-  };
-  if (experts <= 32) select(std::integral_constant<int, 1>());
-  else if (experts <= 64) select(std::integral_constant<int, 2>());
-  else if (experts <= 128) select(std::integral_constant<int, 4>());
-  else if (experts <= 256) select(std::integral_constant<int, 8>());
-  else select(std::integral_constant<int, 16>());
+  });
   k_route_scan<<<(experts + 8) / 8, 256, 0, st>>>(counts, totals, experts + 1, blocks);
   const size_t smem = sizeof(int32_t) * (experts + 1) * (1 + kRouteThreads / 32);
   k_route_place<<<blocks, kRouteThreads, smem, st>>>(chosen, counts, totals, tokens, experts, k,
                                                      block_tokens, position, rows, offsets);
   return cudaGetLastError();
-}
-
-// KP: k rounded up, so that the sorted list stays in registers.
-template <typename F>
-cudaError_t with_chosen(int k, F&& f) {
-  if (k == 1) return f(std::integral_constant<int, 1>());
-  if (k == 2) return f(std::integral_constant<int, 2>());
-  if (k <= 4) return f(std::integral_constant<int, 4>());
-  if (k <= 8) return f(std::integral_constant<int, 8>());
-  return f(std::integral_constant<int, kMaxChosen>());
 }
 
 template <typename F>
@@ -586,11 +495,9 @@ cudaError_t launch_route(const void* logits, int32_t dtype, int64_t tokens, int3
                          void* workspace, cudaStream_t st) {
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    return with_chosen(k, [&](auto kp) {
-      return route_typed<T, decltype(kp)::value>(
-          static_cast<const T*>(logits), tokens, experts, pitch, k, normalize, weights, chosen,
-          position, rows, offsets, static_cast<int32_t*>(workspace), st);
-    });
+    return route_typed<T>(static_cast<const T*>(logits), tokens, experts, pitch, k, normalize,
+                          weights, chosen, position, rows, offsets,
+                          static_cast<int32_t*>(workspace), st);
   });
 }
 

@@ -186,3 +186,17 @@ def test_route_gradient_of_far_logits(ops, tokens):
     off = (d.double() - want).abs()
     off[:, 7] = 0
     assert (off <= 24 * 2.0 ** -24 * want.abs() + 2.0 ** -150).all()
+
+
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("experts,k", [(1, 1), (8, 2), (31, 8), (64, 4), (130, 5), (255, 4), (512, 16)])
+def test_route_does_not_depend_on_the_batch(ops, experts, k, normalize):
+    """A token's choice and weights have the same bits served alone and in a batch."""
+    g = gen(experts)
+    x = torch.randn(130, experts, generator=g, device="cuda") * 4
+    x.masked_fill_(torch.rand(130, experts, generator=g, device="cuda") > 0.8, -math.inf)
+    whole = ops.route(x, k, normalize=normalize)
+    for size in (1, 7, 64, 65):
+        part = ops.route(x[:size], k, normalize=normalize)
+        assert torch.equal(part.experts, whole.experts[:size])
+        assert torch.equal(part.weights, whole.weights[:size])
