@@ -159,7 +159,7 @@ struct MatmulCall {
 };
 int64_t matmul_workspace(const MatmulCall& c);
 cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st);
-cudaError_t read_matmul_errors(uint32_t* bits);
+cudaError_t take_matmul_errors(uint32_t* bits);
 
 // experts_few.cu
 struct FewCall {

@@ -1,5 +1,5 @@
 // C entry points of the expert-layer operators: argument checks, then the launches. Nothing
-// here waits for the device, allocates or throws.
+// here allocates or throws, and nothing but lgbm_b200_experts_errors waits for the device.
 #include <cstdarg>
 #include <cstdio>
 
@@ -338,7 +338,7 @@ int lgbm_b200_experts_matmul_w4(const void* x, int64_t x_rows, int64_t x_pitch,
 
 int lgbm_b200_experts_errors(uint32_t* bits_out) {
   if (!bits_out) return refuse(LGBM_B200_INVALID_ARGUMENT, "experts_errors: null argument");
-  return launched(read_matmul_errors(bits_out), "experts_errors");
+  return launched(take_matmul_errors(bits_out), "experts_errors");
 }
 
 }  // extern "C"

@@ -1247,12 +1247,21 @@ cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st)
   return err;
 }
 
-cudaError_t read_matmul_errors(uint32_t* bits) {
-  cudaError_t err = cudaMemcpyFromSymbol(bits, g_matmul_error, sizeof(*bits));
-  const uint32_t zero = 0;
-  if (err == cudaSuccess && *bits)
-    err = cudaMemcpyToSymbol(g_matmul_error, &zero, sizeof(zero));
-  return err;
+// Moves the error bits to where no kernel sets any, in one step: a bit that another thread's
+// kernel sets meanwhile is in this answer or in the next.
+__device__ uint32_t g_taken_error;
+__global__ void k_take_errors() { g_taken_error = atomicExch(&g_matmul_error, 0u); }
+
+// Waits for the whole device: work on streams that do not order with the legacy default stream,
+// as those of torch's pool, would go unnoticed otherwise.
+cudaError_t take_matmul_errors(uint32_t* bits) {
+  static std::mutex mu;  // g_taken_error is one word a device
+  cudaError_t err = cudaDeviceSynchronize();
+  if (err != cudaSuccess) return err;
+  std::lock_guard<std::mutex> lock(mu);
+  k_take_errors<<<1, 1>>>();
+  err = cudaGetLastError();
+  return err != cudaSuccess ? err : cudaMemcpyFromSymbol(bits, g_taken_error, sizeof(*bits));
 }
 
 }  // namespace experts

@@ -449,12 +449,16 @@ PyObject* dropout(PyObject* const* a) {
 // errors() -> bits
 PyObject* errors(PyObject* const*) {
   uint32_t bits = 0;
-  check(lgbm_b200_experts_errors(&bits));
+  int rc;
+  Py_BEGIN_ALLOW_THREADS  // it waits for the device
+  rc = lgbm_b200_experts_errors(&bits);
+  Py_END_ALLOW_THREADS
+  check(rc);
   return PyLong_FromUnsignedLong(bits);
 }
 
-// One Python entry point: the argument count, the GIL (kept: nothing here waits but errors),
-// and C++ exceptions as Python ones.
+// One Python entry point: the argument count, the GIL (kept: nothing here waits but errors, which
+// releases it), and C++ exceptions as Python ones.
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS

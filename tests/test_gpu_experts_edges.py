@@ -200,3 +200,19 @@ def test_route_does_not_depend_on_the_batch(ops, experts, k, normalize):
         part = ops.route(x[:size], k, normalize=normalize)
         assert torch.equal(part.experts, whole.experts[:size])
         assert torch.equal(part.weights, whole.weights[:size])
+
+
+# ----------------------------------------------------------------------- check_errors
+
+
+def test_check_errors_waits_for_side_streams(ops):
+    """A stream of torch's pool does not order with the legacy default stream: the check has to
+    wait for the device, or it reads the error word of kernels that still run."""
+    ops.check_errors()  # the first call loads the module, which waits too
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)  # cycles: a fifth of a second
+        done = side.record_event()
+    ops.check_errors()
+    assert done.query()
