@@ -5,6 +5,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -60,7 +61,12 @@ int dtype_of(const char* what, const Tensor& t, bool halves) {
 
 Tensor tensor(const char* what, PyObject* o) {
   if (!THPVariable_Check(o)) refuse(LGBM_B200_INVALID_ARGUMENT, what, ": want a torch tensor");
-  return THPVariable_Unpack(o);
+  Tensor t = THPVariable_Unpack(o);
+  // nothing is recorded for autograd: a result would lose the gradient without a word
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    refuse(LGBM_B200_INVALID_ARGUMENT, what, ": an input requires a gradient, which autograd does "
+           "not get through here; call under torch.no_grad() and use the _backward functions");
+  return t;
 }
 
 // A [rows, width] matrix with a contiguous last axis.

@@ -17,7 +17,9 @@ current stream of that device and scratch comes from torch's allocator on that s
 tensor whose last axis is not contiguous is copied first; any row stride is read in place.
 The functions call the C ABI (lgbm_b200_experts_* in include/lgbm_b200.h) through the
 extension module built beside the library, and raise LightGBMError for arguments it refuses;
-there is no CPU path.
+there is no CPU path. Nothing is recorded for autograd: under gradient mode an input that requires
+a gradient is refused, so call under `torch.no_grad()` (or inside a `torch.autograd.Function`) and
+use the gradient beside each function.
 """
 
 from collections import namedtuple
@@ -91,6 +93,7 @@ def grouped_matmul_w4(x, q, scales, offsets, zeros=None, rows=None, group_size=1
     return _X.grouped_matmul_w4(x, q, scales, offsets, zeros, rows, group_size)
 
 
+@torch.no_grad()
 def quantize_w4(w, group_size=128, symmetric=False):
     """(q, scales, zeros) of weights [E, outer, inner] (bf16 or f16) for `grouped_matmul_w4`,
     once, when a trained layer is laid out for serving. Each group's range, stretched to hold

@@ -216,3 +216,38 @@ def test_check_errors_waits_for_side_streams(ops):
         done = side.record_event()
     ops.check_errors()
     assert done.query()
+
+
+# ----------------------------------------------------------------- the Python boundary
+
+
+def test_inputs_that_want_gradients_are_refused(ops):
+    """The functions record nothing for autograd: a result that does not require gradients though
+    its input does would lose them without a word."""
+    from lightgbm_rs_b200 import LightGBMError
+
+    c = lambda *s: torch.zeros(*s, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    want = lambda *s: c(*s).requires_grad_()  # noqa: E731
+    f32 = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+    off = torch.tensor([0, 2, 4], device="cuda", dtype=torch.int32)
+    pos = torch.arange(4, device="cuda", dtype=torch.int32).view(2, 2)
+    q = torch.zeros(2, 8, 16, device="cuda", dtype=torch.uint8)
+    r = ops.route(f32(4, 2), 1)
+    calls = [
+        lambda: ops.route(f32(4, 5).requires_grad_(), 2),
+        lambda: ops.route_backward(f32(4, 1).requires_grad_(), f32(4, 2), r),
+        lambda: ops.grouped_matmul(want(4, 8), c(2, 8, 8), off),
+        lambda: ops.grouped_matmul(c(4, 8), want(2, 8, 8), off),
+        lambda: ops.grouped_matmul_backward(c(4, 8), c(4, 8), want(2, 8, 8), off),
+        lambda: ops.grouped_matmul_w4(c(4, 8), q, want(2, 8, 1), off, group_size=32),
+        lambda: ops.combine(want(4, 8), pos),
+        lambda: ops.combine(c(4, 8), pos, f32(2, 2).requires_grad_()),
+        lambda: ops.combine_backward(want(2, 8), c(4, 8), pos),
+        lambda: ops.dropout(want(4, 8), 0.5, 1),
+        lambda: ops.dropout(c(4, 8), 0.5, 1, residual=want(4, 8)),
+    ]
+    for call in calls:
+        with pytest.raises(LightGBMError, match="no_grad"):
+            call()
+        with torch.no_grad():
+            call()
