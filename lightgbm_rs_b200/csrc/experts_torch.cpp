@@ -77,7 +77,8 @@ struct Matrix {
   const void* p() const { return t.data_ptr(); }
 };
 
-Matrix matrix(const char* what, Tensor t, bool halves) {
+// `reads`: its values are wanted, else only its shape.
+Matrix matrix(const char* what, Tensor t, bool halves, bool reads = true) {
   Matrix m;
   m.dtype = dtype_of(what, t, halves);
   if (t.dim() != 2 || !t.is_cuda())
@@ -86,7 +87,7 @@ Matrix matrix(const char* what, Tensor t, bool halves) {
   m.width = t.size(1);
   m.pitch = m.rows > 1 ? t.stride(0) : m.width;
   if ((m.width > 1 && t.stride(1) != 1) || m.pitch < m.width) {
-    t = t.contiguous();
+    if (reads) t = t.contiguous();
     m.pitch = m.width;
   }
   m.t = std::move(t);
@@ -246,15 +247,16 @@ void index_rows(const char* what, Product& p, PyObject* rows) {
   p.rows = t.size(0);
 }
 
-Product product(const char* what, PyObject* x, PyObject* w, PyObject* offsets, PyObject* rows) {
+Product product(const char* what, PyObject* x, PyObject* w, PyObject* offsets, PyObject* rows,
+                bool reads_x, bool reads_w) {
   Product p;
-  p.x = matrix(what, tensor(what, x), true);
+  p.x = matrix(what, tensor(what, x), true, reads_x);
   const auto dev = p.x.t.device();
   p.w = tensor(what, w);
   if (p.w.dim() != 3 || p.w.scalar_type() != p.x.t.scalar_type() || p.w.device() != dev)
     refuse(LGBM_B200_INVALID_ARGUMENT, what, ": want w [experts, outer, inner] like x, got ",
            describe(p.w), " with x ", describe(p.x.t));
-  if (!p.w.is_contiguous()) p.w = p.w.contiguous();
+  if (reads_w && !p.w.is_contiguous()) p.w = p.w.contiguous();
   p.experts = p.w.size(0);
   p.outer = p.w.size(1);
   p.inner = p.w.size(2);
@@ -270,7 +272,7 @@ Product product(const char* what, PyObject* x, PyObject* w, PyObject* offsets, P
 // grouped_matmul(x, w, offsets, rows) -> y
 PyObject* grouped_matmul(PyObject* const* a) {
   const char* what = "grouped_matmul";
-  const Product p = product(what, a[0], a[1], a[2], a[3]);
+  const Product p = product(what, a[0], a[1], a[2], a[3], true, true);
   const auto dev = p.x.t.device();
   On on(dev);
   Tensor y = make(dev, p.x.t.scalar_type(), {p.rows, p.outer});
@@ -287,7 +289,8 @@ PyObject* grouped_matmul(PyObject* const* a) {
 // grouped_matmul_backward(dy, x, w, offsets, rows, wide_dw, need_dx, need_dw) -> (dx, dw)
 PyObject* grouped_matmul_backward(PyObject* const* a) {
   const char* what = "grouped_matmul_backward";
-  const Product p = product(what, a[1], a[2], a[3], a[4]);
+  const bool need_dx = flag(a[6]), need_dw = flag(a[7]);
+  const Product p = product(what, a[1], a[2], a[3], a[4], need_dw, need_dx);
   const Matrix dy = matrix(what, tensor(what, a[0]), true);
   const auto dev = p.x.t.device();
   const auto type = p.x.t.scalar_type();
@@ -300,8 +303,8 @@ PyObject* grouped_matmul_backward(PyObject* const* a) {
   const int32_t experts = (int32_t)p.experts, inner = (int32_t)p.inner, outer = (int32_t)p.outer;
   On on(dev);
   Tensor dx, dw;
-  if (flag(a[6])) dx = make(dev, type, {p.rows, p.inner});
-  if (flag(a[7])) dw = make(dev, wide ? at::kFloat : type, {p.experts, p.outer, p.inner});
+  if (need_dx) dx = make(dev, type, {p.rows, p.inner});
+  if (need_dw) dw = make(dev, wide ? at::kFloat : type, {p.experts, p.outer, p.inner});
   if (dx.defined() || dw.defined()) {
     Scratch ws(dev, lgbm_b200_experts_matmul_backward_workspace(
                         dy.p(), dy.pitch, p.x.p(), p.x.pitch, p.ip(), p.w.data_ptr(), p.rows,

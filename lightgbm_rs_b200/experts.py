@@ -13,8 +13,12 @@ a token's k results; `dropout` regularises while training. Each has its gradient
     out = experts.combine(y, r.position, r.weights)             # [T, N]
 
 Inputs and results are torch tensors on one CUDA device; the work is enqueued on torch's
-current stream of that device and scratch comes from torch's allocator on that stream. A
-tensor whose last axis is not contiguous is copied first; any row stride is read in place.
+current stream of that device and scratch comes from torch's allocator on that stream.
+Matrices of rows (x, y, dy, dout, logits, dropout's 2-D inputs) may have any row stride; one
+whose last axis is not contiguous is copied first. Other tensors (w, q, scales, positions) are
+copied first when they are not contiguous as a whole: keep w as [E, outer, inner]. The products
+also copy, on the device, operands that the tensor cores' loads cannot walk: x read through
+`rows`, and x, dy or w whose rows do not start at multiples of 16 bytes.
 The functions call the C ABI (lgbm_b200_experts_* in include/lgbm_b200.h) through the
 extension module built beside the library, and raise LightGBMError for arguments it refuses;
 there is no CPU path. Nothing is recorded for autograd: under gradient mode an input that requires

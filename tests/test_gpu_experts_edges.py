@@ -251,3 +251,22 @@ def test_inputs_that_want_gradients_are_refused(ops):
             call()
         with torch.no_grad():
             call()
+
+
+def test_operands_that_are_not_read_are_not_copied(ops):
+    """Only dw is wanted, or only dx: w, or x, gives its shape, and its strides cost no memory."""
+    dy = torch.randn(4096, 512, device="cuda").to(torch.bfloat16)
+    x = torch.randn(512, 4096, device="cuda").to(torch.bfloat16).t()
+    w = torch.randn(8, 512, 512, device="cuda").to(torch.bfloat16).transpose(1, 2)
+    off = offsets_of([512] * 8)
+
+    def peak(x, w, **which):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        ops.grouped_matmul_backward(dy, x, w, off, **which)
+        return torch.cuda.max_memory_allocated() - before
+
+    straight_x, straight_w = x.contiguous(), w.contiguous()
+    assert peak(straight_x, w, need_dx=False) == peak(straight_x, straight_w, need_dx=False)
+    assert peak(x, straight_w, need_dw=False) == peak(straight_x, straight_w, need_dw=False)
