@@ -543,6 +543,7 @@ int lgbm_b200_predict(lgbm_b200_predictor* p, const double* rows, int64_t num_ro
  *    the _workspace function says, 16-byte aligned; it is free again once the stream has
  *    passed the call.
  *  - Pitches are in elements; the innermost axis is contiguous. Outputs are contiguous.
+ *    Arrays start at multiples of their elements' size.
  *  - offsets[E + 1], index, chosen and position are device data that the host does not
  *    check. Kernels clamp offsets to the rows given and skip indices outside them.
  *  - At most 512 experts, 16 chosen a token, 2^31 - 65537 rows, products 2^28 wide.

@@ -2,6 +2,7 @@
 // here allocates or throws, and nothing but lgbm_b200_experts_errors waits for the device.
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 
 #include "experts.cuh"
 
@@ -30,6 +31,24 @@ int launched(cudaError_t err, const char* what) {
 bool is_float(int32_t dtype) {
   return dtype == LGBM_B200_DTYPE_F32 || dtype == LGBM_B200_DTYPE_BF16 ||
          dtype == LGBM_B200_DTYPE_F16;
+}
+
+struct Array {
+  const void* p;
+  int size;  // bytes of an element
+};
+
+// An access off its element's size faults on the device. Null starts everywhere.
+int check_starts(const char* what, std::initializer_list<Array> arrays) {
+  int i = 0;
+  for (const Array& a : arrays) {
+    if (reinterpret_cast<uintptr_t>(a.p) % a.size != 0)
+      return refuse(LGBM_B200_INVALID_ARGUMENT,
+                    "%s: array %d at %p does not start at a multiple of its %d-byte elements", what,
+                    i, a.p, a.size);
+    ++i;
+  }
+  return LGBM_B200_OK;
 }
 
 // Grouped rows are counted in 32 bits, with room for a tile past the last one.
@@ -72,6 +91,15 @@ int check_product(const char* what, const MatmulCall& c) {
   if (!c.offsets || (c.rows > 0 && ((reads_x && !c.x) || (reads_dy && !c.dy))) ||
       (reads_w && !c.w))
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
+  if (int rc = check_starts(what, {{reads_x ? c.x : nullptr, 2},
+                                   {reads_dy ? c.dy : nullptr, 2},
+                                   {reads_w ? c.w : nullptr, 2},
+                                   {reads_x ? c.index : nullptr, 4},
+                                   {c.offsets, 4},
+                                   {c.y, 2},
+                                   {c.dx, 2},
+                                   {c.dw, c.dw ? elem_size(c.grad_dtype) : 1}}))
+    return rc;
   if (reads_x && (c.x_pitch < c.inner || c.x_rows < (c.rows > 0) ||
                   (!c.index && c.x_rows != c.rows)))
     return refuse(LGBM_B200_LENGTH_MISMATCH,
@@ -118,11 +146,18 @@ int lgbm_b200_experts_route(const void* logits, int32_t dtype, int64_t tokens, i
   if (int rc = check_gate(what, dtype, tokens, experts, pitch, k)) return rc;
   if (!offsets || (tokens > 0 && (!logits || !weights || !chosen || !position || !rows)))
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
+  if (int rc = check_starts(what, {{logits, elem_size(dtype)},
+                                   {weights, 4},
+                                   {chosen, 4},
+                                   {position, 4},
+                                   {rows, 4},
+                                   {offsets, 4}}))
+    return rc;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (tokens == 0)
     return launched(cudaMemsetAsync(offsets, 0, sizeof(int32_t) * (experts + 1), st), what);
   const int64_t need = route_workspace(tokens, experts, k);
-  if (workspace_bytes < need || (need > 0 && !workspace))
+  if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace))))
     return refuse(LGBM_B200_LENGTH_MISMATCH, "%s: workspace of %lld bytes, %lld are needed",
                   what, (long long)workspace_bytes, (long long)need);
   return launched(launch_route(logits, dtype, tokens, experts, pitch, k, normalize != 0, weights,
@@ -139,6 +174,12 @@ int lgbm_b200_experts_route_backward(const float* dweights, const float* weights
   if (tokens == 0) return LGBM_B200_OK;
   if (!dweights || !weights || !chosen || !logits || !dlogits)
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
+  if (int rc = check_starts(what, {{dweights, 4},
+                                   {weights, 4},
+                                   {chosen, 4},
+                                   {logits, elem_size(dtype)},
+                                   {dlogits, elem_size(dtype)}}))
+    return rc;
   return launched(launch_route_backward(dweights, weights, chosen, logits, dtype, tokens, experts,
                                         pitch, k, normalize != 0, dlogits,
                                         reinterpret_cast<cudaStream_t>(stream)),
@@ -159,6 +200,11 @@ int lgbm_b200_experts_combine(const void* y, int32_t dtype, int64_t rows, int32_
   if (tokens == 0) return LGBM_B200_OK;
   if (!position || !out || (rows > 0 && !y))
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
+  if (int rc = check_starts(what, {{y, elem_size(dtype)},
+                                   {position, 4},
+                                   {weights, 4},
+                                   {out, elem_size(dtype)}}))
+    return rc;
   return launched(launch_combine(y, dtype, rows, width, pitch, position, weights, tokens, k, out,
                                  reinterpret_cast<cudaStream_t>(stream)),
                   what);
@@ -184,6 +230,13 @@ int lgbm_b200_experts_combine_backward(const void* dout, const void* y, int32_t 
   if (tokens == 0) return LGBM_B200_OK;
   if (!dout || !position || !dy || (dweights && !y))
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
+  if (int rc = check_starts(what, {{dout, elem_size(dtype)},
+                                   {dweights ? y : nullptr, elem_size(dtype)},
+                                   {position, 4},
+                                   {weights, 4},
+                                   {dy, elem_size(dtype)},
+                                   {dweights, 4}}))
+    return rc;
   return launched(launch_combine_backward(dout, y, dtype, rows, width, dout_pitch, pitch,
                                           position, weights, tokens, k, dy, dweights,
                                           reinterpret_cast<cudaStream_t>(stream)),
@@ -204,6 +257,10 @@ int lgbm_b200_experts_dropout(const void* x, const void* residual, int32_t dtype
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: p %g is not in [0, 1]", what, p);
   if (rows == 0 || width == 0) return LGBM_B200_OK;
   if (!x || !out) return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
+  if (int rc = check_starts(what, {{x, elem_size(dtype)},
+                                   {residual, elem_size(dtype)},
+                                   {out, elem_size(dtype)}}))
+    return rc;
   const uint32_t drop = (uint32_t)(p * 65536.0 + 0.5);
   return launched(launch_dropout(x, residual, dtype, rows, width, pitch, residual_pitch, drop,
                                  seed, offset, out, reinterpret_cast<cudaStream_t>(stream)),
@@ -330,6 +387,7 @@ int lgbm_b200_experts_matmul_w4(const void* x, int64_t x_rows, int64_t x_pitch,
   if (!scales) return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
   if (!aligned16(q))
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: weights are not 16-byte aligned", what);
+  if (int rc = check_starts(what, {{scales, 2}})) return rc;
   if (rows == 0) return LGBM_B200_OK;
   FewCall f{dtype, x,      x_rows, x_pitch, index, q,     group_size, scales,
             zeros, offsets, rows,   experts, inner, outer, y};
