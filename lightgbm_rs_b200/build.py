@@ -1,5 +1,6 @@
 """Build the in-tree shared library lightgbm_rs_b200/liblgbm_b200.so for sm_100a, and the
-Python module lightgbm_rs_b200/_experts.so that hands torch tensors to it.
+Python module lightgbm_rs_b200/_experts.so that hands torch tensors to it (where torch is
+installed; the library does without).
 
 Incremental: objects under lightgbm_rs_b200/_build/ are rebuilt when a source or
 header is newer. Usage: python -m lightgbm_rs_b200.build [--force]
@@ -7,10 +8,12 @@ header is newer. Usage: python -m lightgbm_rs_b200.build [--force]
 
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -20,6 +23,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "liblgbm_b200.so")
 BINDING_SRC = os.path.join(CSRC, "experts_torch.cpp")
 BINDING = os.path.join(PKG, "_experts.so")
+BINDING_STAMP = os.path.join(BUILD, "experts_torch.stamp")
 NVCC = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
 HOST_CXX = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else (shutil.which("g++") or "g++")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -83,17 +87,38 @@ def build(force=False, verbose=False, ptxas_info=False):
     return LIB
 
 
-def build_binding(force=False):
-    """The torch binding, against the installed torch's headers; it finds the library beside
-    itself and torch's own libraries already loaded."""
-    build()
-    obj = os.path.join(BUILD, "experts_torch.cpp.o")
-    header = os.path.join(INCLUDE, "lgbm_b200.h")
-    if not force and not _stale(obj, BINDING_SRC, [header]) and os.path.exists(BINDING) and \
-            os.path.getmtime(BINDING) >= os.path.getmtime(obj):
-        return BINDING
-    import sysconfig
+def _torch_stamp():
+    """What the binding's object depends on besides its source: the torch installed (its version
+    file, read without importing it) and the Python ABI. None without torch."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    with open(os.path.join(os.path.dirname(spec.origin), "version.py")) as f:
+        return f"{sysconfig.get_config_var('SOABI')} {spec.origin}\n{f.read()}"
 
+
+def _binding_stale(obj):
+    if not os.path.exists(BINDING) or _stale(obj, BINDING_SRC, [
+            os.path.join(INCLUDE, "lgbm_b200.h")]) or \
+            os.path.getmtime(BINDING) < os.path.getmtime(obj):
+        return True
+    try:
+        with open(BINDING_STAMP) as f:
+            return f.read() != _torch_stamp()
+    except OSError:
+        return True
+
+
+def build_binding(force=False):
+    """The library, and the torch binding against the installed torch's headers: it finds the
+    library beside itself and torch's own libraries already loaded. Without torch there is
+    nothing to bind to: None, and the library alone."""
+    build()
+    if _torch_stamp() is None:
+        return None
+    obj = os.path.join(BUILD, "experts_torch.cpp.o")
+    if not force and not _binding_stale(obj):
+        return BINDING
     import torch
     from torch.utils import cpp_extension as ext
 
@@ -109,10 +134,12 @@ def build_binding(force=False):
     if r.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, BINDING)
+    with open(BINDING_STAMP, "w") as f:
+        f.write(_torch_stamp())
     return BINDING
 
 
 if __name__ == "__main__":
     lib = build(force="--force" in sys.argv, verbose=True, ptxas_info="--ptxas" in sys.argv)
     print(lib)
-    print(build_binding(force="--force" in sys.argv))
+    print(build_binding(force="--force" in sys.argv) or "no torch here: its binding _experts.so is not built")
