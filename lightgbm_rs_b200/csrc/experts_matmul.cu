@@ -63,6 +63,7 @@
 #include <cuda.h>  // types of the tensor map; the encoder is looked up at run time
 
 #include "experts.cuh"
+#include "experts_parts.h"
 
 namespace lgbm_b200 {
 namespace experts {
@@ -453,7 +454,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
       for (int i = lane; i <= g.experts; i += 32) {
         const int e = i / g.parts, part = i % g.parts;
         const int32_t n = e < experts ? off[e + 1] - off[e] : 0;
-        const int32_t each = (n / kTileK + g.parts) / g.parts * kTileK;
+        const int32_t each = part_rows(n, g.parts, kTileK);
         cum[i] = off[e] + (int32_t)min((int64_t)each * part, (int64_t)n);
       }
       __syncwarp();

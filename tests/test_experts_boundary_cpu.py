@@ -1,4 +1,8 @@
-"""CPU checks of the expert layers' boundary: what must not reach a device is refused before."""
+"""CPU checks of the expert layers: what must not reach a device is refused before, and the
+arithmetic that host and device share."""
+
+import ctypes
+import subprocess
 
 import pytest
 
@@ -44,3 +48,29 @@ def test_arrays_off_their_elements_are_refused(capi):
     args = list(calls["route"][0])
     args[12] += 4
     assert L.lgbm_b200_experts_route(*args) == capi.LENGTH_MISMATCH
+
+
+def compiled(tmp_path, body):
+    """C++ around the library's own headers, as a shared object."""
+    from lightgbm_rs_b200 import build
+
+    src, so = str(tmp_path / "shim.cpp"), str(tmp_path / "shim.so")
+    with open(src, "w") as f:
+        f.write(body)
+    subprocess.run([build.HOST_CXX, "-O1", "-std=c++17", "-shared", "-fPIC", f"-I{build.CSRC}",
+                    "-o", so, src], check=True)
+    return ctypes.CDLL(so)
+
+
+def test_parts_of_a_weight_gradient_are_even(tmp_path):
+    """Parts cover the rows in whole blocks of 64, and no smaller number of blocks would."""
+    lib = compiled(tmp_path, '#include "experts_parts.h"\n'
+                   'extern "C" int part_rows(int n, int parts, int block) {\n'
+                   '  return lgbm_b200::experts::part_rows(n, parts, block);\n}\n')
+    for parts in (1, 2, 3, 7, 24, 148):
+        for n in [0, 1, 63, 64, 65, 64 * parts, 64 * parts * 5, 64 * parts * 5 + 1, 2063,
+                  (1 << 31) - 65537]:
+            each = lib.part_rows(n, parts, 64)
+            assert each % 64 == 0 and each * parts >= n
+            assert n == 0 or (each // 64 - 1) * parts < -(-n // 64)
+    assert lib.part_rows(64 * 24 * 5, 24, 64) == 64 * 5  # not six blocks, four parts empty
