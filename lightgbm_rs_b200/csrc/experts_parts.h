@@ -3,11 +3,7 @@
 
 #include <cstdint>
 
-#ifdef __CUDACC__
-#define LGBM_HOST_DEVICE __host__ __device__ __forceinline__
-#else
-#define LGBM_HOST_DEVICE inline
-#endif
+#include "host_device.h"
 
 namespace lgbm_b200 {
 namespace experts {

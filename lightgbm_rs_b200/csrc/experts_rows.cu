@@ -1,6 +1,7 @@
 // Row operators of the expert layer: the weighted combination of each token's rows with its
 // gradient, and dropout from a counter-based generator.
 #include "experts.cuh"
+#include "philox.h"
 
 namespace lgbm_b200 {
 namespace experts {
@@ -121,27 +122,6 @@ __global__ void __launch_bounds__(kRowThreads)
   }
 }
 
-// Philox4x32-10 (J. Salmon, M. Moraes, R. Dror, D. Shaw, "Parallel random numbers: as easy
-// as 1, 2, 3", 2011): ten rounds of two 32 x 32 -> 64 bit products and xors on a counter of
-// 128 bits, keyed by 64 bits.
-__device__ __forceinline__ uint4 philox(uint64_t block, uint64_t offset, uint32_t k0,
-                                        uint32_t k1) {
-  uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32);
-  uint32_t c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t p = (uint64_t)0xD2511F53u * c0, q = (uint64_t)0xCD9E8D57u * c2;
-    const uint32_t n0 = (uint32_t)(q >> 32) ^ c1 ^ k0, n2 = (uint32_t)(p >> 32) ^ c3 ^ k1;
-    c1 = (uint32_t)q;
-    c3 = (uint32_t)p;
-    c0 = n0;
-    c2 = n2;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
-  }
-  return make_uint4(c0, c1, c2, c3);
-}
-
 // Blocks of eight elements a thread. Bound by memory: 32768 x 4096 bf16 take 87 us (537 MB at
 // 6.2 TB/s), with a residual 115 (805 MB at 7.0). The generator is about 60 of the 110
 // instructions of a block of eight; 32 bits an element instead of 16 would be two generators a
@@ -193,8 +173,8 @@ __device__ __forceinline__ void drop_block(const T* __restrict__ x, const T* __r
   for (int u = 0; u < kDropUnroll; ++u) {
     const int64_t b = b0 + u * kRowThreads;
     if (!FULL && b * 8 >= n) break;
-    const uint4 rnd = philox((uint64_t)b, offset, k0, k1);
-    const uint32_t words[4] = {rnd.x, rnd.y, rnd.z, rnd.w};
+    uint32_t words[4];
+    philox((uint64_t)b, offset, k0, k1, words);
 #pragma unroll
     for (int h = 0; h < kParts; ++h) {
       const int64_t at = b * 8 + h * V;

@@ -74,3 +74,40 @@ def test_parts_of_a_weight_gradient_are_even(tmp_path):
             assert each % 64 == 0 and each * parts >= n
             assert n == 0 or (each // 64 - 1) * parts < -(-n // 64)
     assert lib.part_rows(64 * 24 * 5, 24, 64) == 64 * 5  # not six blocks, four parts empty
+
+
+def test_philox_counter_words(tmp_path):
+    """The device's generator, compiled for the host, against the published known answers and
+    Python integers, with every word of the counter and the key in use: elements from 2^35 on have
+    block numbers past 32 bits, more than a test can hold in memory."""
+    lib = compiled(tmp_path, '#include "philox.h"\n'
+                   'extern "C" void philox(uint64_t block, uint64_t offset, uint64_t seed,\n'
+                   '                       uint32_t* out) {\n'
+                   '  uint32_t w[4];\n'
+                   '  lgbm_b200::experts::philox(block, offset, (uint32_t)seed,\n'
+                   '                             (uint32_t)(seed >> 32), w);\n'
+                   '  for (int i = 0; i < 4; ++i) out[i] = w[i];\n}\n')
+    u64 = ctypes.c_uint64
+
+    def words(block, offset, seed):
+        out = (ctypes.c_uint32 * 4)()
+        lib.philox(u64(block), u64(offset), u64(seed), out)
+        return list(out)
+
+    def integers(block, offset, seed):
+        low = 0xFFFFFFFF
+        c, k0, k1 = [block & low, block >> 32, offset & low, offset >> 32], seed & low, seed >> 32
+        for _ in range(10):
+            p, q = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+            c = [(q >> 32) ^ c[1] ^ k0, q & low, (p >> 32) ^ c[3] ^ k1, p & low]
+            k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+        return c
+
+    full = (1 << 64) - 1
+    assert words(0, 0, 0) == [0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8]
+    assert words(full, full, full) == [0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd]
+    for block in (5, 1 << 32, (1 << 32) + 5, 0xFEDCBA9876543210):
+        for offset in (0, 7, (3 << 32) + 1):
+            for seed in (1, 0x0123456789ABCDEF):
+                assert words(block, offset, seed) == integers(block, offset, seed)
+    assert words(5, 0, 1) != words((1 << 32) + 5, 0, 1)
