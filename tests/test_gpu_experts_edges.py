@@ -270,3 +270,91 @@ def test_operands_that_are_not_read_are_not_copied(ops):
     straight_x, straight_w = x.contiguous(), w.contiguous()
     assert peak(straight_x, w, need_dx=False) == peak(straight_x, straight_w, need_dx=False)
     assert peak(x, straight_w, need_dw=False) == peak(straight_x, straight_w, need_dw=False)
+
+
+@pytest.mark.parametrize("tokens,experts,k", [(3_000_017, 16, 2), (400_003, 255, 4)])
+def test_route_large_batches(ops, tokens, experts, k):
+    g = gen(experts)
+    x = torch.randn(tokens, experts, generator=g, device="cuda")
+    x.masked_fill_(torch.rand(tokens, experts, generator=g, device="cuda") > 0.9, -math.inf)
+    r = ops.route(x, k)
+    top, ids = x.sort(dim=1, descending=True, stable=True)
+    top, ids = top[:, :k], ids[:, :k].masked_fill(top[:, :k] == -math.inf, -1)
+    assert torch.equal(r.experts.long(), ids)
+    flat = torch.where(ids < 0, experts, ids).reshape(-1)
+    group, order = flat.sort(stable=True)
+    assert torch.equal(r.rows.long(), order // k)
+    assert torch.equal(r.position.reshape(-1).long()[order], torch.arange(tokens * k, device="cuda"))
+    assert torch.equal(r.offsets.long(),
+                       torch.searchsorted(group, torch.arange(experts + 1, device="cuda")))
+
+
+# ----------------------------------------------------------- infinities, odd addresses
+
+
+def same(got, want, slack):
+    """As close() of the main tests, with infinities of the same sign in the same places; `want`
+    in 64 bits, beyond the type's range where that is meant."""
+    w = want.to(got.dtype).double()
+    g = got.double()
+    assert torch.equal(torch.isnan(g), torch.isnan(w))
+    inf = torch.isinf(w)
+    assert torch.equal(g[inf], w[inf])
+    fin = torch.isfinite(w)
+    lim = slack + UNIT[got.dtype] * want.abs() + 2.0 ** -25
+    assert (((g - want).abs() <= lim) | ~fin).all()
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_overflow_and_infinities(ops, rows, dtype):
+    """Every second result row is far beyond f16's range, and one input is infinite. Whole
+    numbers below 2^24: the sums are exact."""
+    dt, g = DTYPES[dtype], gen(rows)
+    x = torch.randint(1, 3, (rows, 64), generator=g, device="cuda").to(dt)
+    x[::2] *= 64
+    w = torch.randint(1, 3, (2, 72, 64), generator=g, device="cuda").to(dt)
+    w[:, ::2] *= -64
+    x[0, 5] = math.inf
+    off = offsets_of([1, rows - 1])
+    _, y64, _ = product64(x, w, off, None)
+    y = ops.grouped_matmul(x, w, off)
+    same(y, y64, 0.0)
+    assert torch.isinf(y[0]).all() and (dtype == "bf16" or torch.isinf(y[2]).any())
+    dx, dw = ops.grouped_matmul_backward(y64.clamp(-64, 64).to(dt), x, w, off)
+    dy = y64.clamp(-64, 64).to(dt).double()
+    same(dx, product64(dy, w.transpose(1, 2), off, None)[1], 0.0)
+    for e, s in enumerate((slice(0, 1), slice(1, rows))):
+        same(dw[e], dy[s].T @ x[s].double(), 0.0)
+
+
+def test_rows_overflow(ops):
+    y = torch.full((4, 24), 60000.0, device="cuda", dtype=torch.float16)
+    y[2:] = -60000
+    pos = torch.tensor([[0, 1], [2, 3]], device="cuda", dtype=torch.int32)
+    out = ops.combine(y, pos)
+    assert (out[0] == math.inf).all() and (out[1] == -math.inf).all()
+    dy, dw = ops.combine_backward(out, y, pos, torch.full((2, 2), 0.5, device="cuda"))
+    assert (dy[:2] == math.inf).all() and (dy[2:] == -math.inf).all() and (dw == math.inf).all()
+    d = ops.dropout(y, 0.5, 3)
+    kept = d != 0
+    assert kept.any() and not kept.all()
+    assert torch.equal(d[kept], torch.where(y > 0, math.inf, -math.inf).half()[kept])
+
+
+@pytest.mark.parametrize("start", [1, 2, 3, 4])
+@pytest.mark.parametrize("rows", [3, 40, 300])
+@pytest.mark.parametrize("inner,outer", [(64, 72), (33, 130), (520, 24)])
+def test_weights_at_any_address(ops, inner, outer, rows, start):
+    """w starts 2 to 8 bytes past a multiple of 16, NaN around it; whole numbers, exact."""
+    g, E = gen(inner + start), 3
+    flat = torch.full((E * outer * inner + 16,), math.nan, device="cuda", dtype=torch.bfloat16)
+    w = flat[start:start + E * outer * inner].view(E, outer, inner)
+    w.copy_(torch.randint(-1, 2, (E, outer, inner), generator=g, device="cuda"))
+    x = torch.randint(-2, 3, (rows, inner), generator=g, device="cuda").to(torch.bfloat16)
+    dy = torch.randint(-1, 2, (rows, outer), generator=g, device="cuda").to(torch.bfloat16)
+    off = offsets_of([rows // 3, 0, rows - rows // 3])
+    want = product64(x, w, off, None)[1].to(torch.bfloat16)
+    assert torch.equal(ops.grouped_matmul(x, w, off), want)
+    want = product64(dy, w.transpose(1, 2), off, None)[1].to(torch.bfloat16)
+    assert torch.equal(ops.grouped_matmul_backward(dy, x, w, off, need_dw=False)[0], want)
