@@ -7,10 +7,12 @@ The layer trains with hand-written gradients and is then laid out in 4 bits to s
 rows:  python examples/leaf_experts.py
 """
 
+import copy
 import math
 import os
 import sys
 
+import numpy as np
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
@@ -21,13 +23,22 @@ from lightgbm_rs_b200 import experts, synthetic  # noqa: E402
 PER_LEAF, SHARED, HIDDEN, OUT, CHOSEN, DROP = 2, 4, 64, 8, 2, 0.1
 
 
+def leaf_numbers(model, tree, X):
+    """The leaf that tree number `tree` of the model sends each row to: the same tree with its
+    leaves' numbers as their values, predicted."""
+    t = dict(model.trees[tree])
+    t["leaf_value"] = np.arange(t["num_leaves"], dtype=np.float64)
+    numbered = copy.copy(model)
+    numbered.trees = [t]
+    return lgb.Predictor(numbered).predict(X, raw_score=True).astype(np.int64)
+
+
 def leaves_of(X, y, num_leaves=16):
     """One tree on the data: the rows' leaf numbers and raw scores."""
     params = {"objective": "binary", "num_leaves": num_leaves, "learning_rate": 1.0}
     booster = lgb.train(params, lgb.Dataset(X, y, params), num_boost_round=1)
-    score = torch.from_numpy(booster.predict(X, raw_score=True))
-    # one tree: a row's score is its leaf's value
-    return score.unique(return_inverse=True)[1].cuda(), score.float().cuda()
+    leaf = torch.from_numpy(leaf_numbers(booster.model(), 0, X))
+    return leaf.cuda(), torch.from_numpy(booster.predict(X, raw_score=True)).float().cuda()
 
 
 class LeafExperts:
