@@ -1130,16 +1130,30 @@ cudaError_t join_parts(const float* part, int parts, int64_t count, int experts,
 }  // namespace
 
 // Whether the forward product streams its weights (experts_few.cu) instead of multiplying
-// tiles. Measured, streamed against tiles, us: up to 2 rows an expert it saves the tiles'
-// longer start (8 experts of 4096 x 2048: 29.5, 35.0; at 4 rows 29.4, 28.8). Weights that TMA
-// cannot walk would be copied first (255 of 129 x 700: 16 rows 44.6, 49.0; 32 rows 50.8,
-// 52.7). Few tiles leave SMs idle, while streaming splits the inner axis (2 of 512 x 512:
-// 32 rows 8.5, 10.3); past 32 rows the weights are streamed again.
+// tiles. Measured, streamed / tiles in us, weights from memory, at rows an expert (all with rows):
+// - Weights that TMA walks: up to 2 rows it saves the tiles' longer start (8 experts of 4096 x
+//   2048: 2 rows 28.8 / 35.1, 4 28.9 / 28.9, 8 30.2 / 29.0). Few tiles leave SMs idle, while
+//   streaming splits the inner axis: up to 32 rows (2 of 512 x 512: 8.5 / 10.3).
+// - Others would be copied first, all experts' even where few have rows. Small weights: the
+//   copy's launch and latency cost more than streaming up to 32 rows (64 of 128 x 129: 10.5 /
+//   16.5; 64 of 256 x 257: 14.5 / 22.7).
+// - Rows at 4 bytes: to about 24 (32 of 4096 x 2002: 24 rows 253 / 269, 32 289 / 271), fewer where
+//   the last block of 128 outputs is mostly empty (255 of 129 x 700: 8 rows 41.4 / 42.3, 12 47.4
+//   / 44.1, 24 57.0 / 45.4).
+// - Rows at 2 bytes: they come by 2-byte loads, each waited for. Streaming pays while it leaves
+//   out half of the experts (32 of 4096 x 2001: rows of 16 experts 198 / 234, of 20 287 / 240, of
+//   32 383 / 295; 8 of 4096 x 4097: of 4 109 / 149, of 5 183 / 161).
+constexpr int64_t kSmallWeights = 12 << 20;
 static bool few_rows(const MatmulCall& c) {
   if (!c.y || c.rows > 32 * (int64_t)c.experts) return false;
-  if (c.rows <= 2 * (int64_t)c.experts) return true;
-  if (!(aligned16(c.w) && c.inner % 8 == 0)) return c.rows <= 24 * (int64_t)c.experts;
-  return (int64_t)c.experts * ((c.outer + 255) / 256) < 148 / 2;
+  const int64_t outputs = (int64_t)c.experts * c.outer;
+  if (aligned16(c.w) && c.inner % 8 == 0)
+    return c.rows <= 2 * (int64_t)c.experts ||
+           (int64_t)c.experts * ((c.outer + 255) / 256) < 148 / 2;
+  if (outputs * c.inner * 2 <= kSmallWeights) return true;
+  if (reinterpret_cast<uintptr_t>(c.w) % 4 == 0 && c.inner % 2 == 0)
+    return c.rows * ((c.outer + 127) / 128 * 128) <= 24 * outputs;
+  return 2 * c.rows <= c.experts;
 }
 static bool copies_x(const MatmulCall& c) {
   return ((c.y && !few_rows(c)) || c.dw) && (c.index || !walkable(c.x, c.x_pitch));

@@ -111,3 +111,19 @@ def test_philox_counter_words(tmp_path):
             for seed in (1, 0x0123456789ABCDEF):
                 assert words(block, offset, seed) == integers(block, offset, seed)
     assert words(5, 0, 1) != words((1 << 32) + 5, 0, 1)
+
+
+def test_streamed_or_copied_by_alignment(capi):
+    """Weights that the tiles' loads cannot walk are streamed while that is the shorter way:
+    workspace for their copy says which it is."""
+    ws, p = capi.lib().lgbm_b200_experts_matmul_workspace, 1 << 20
+    x = lambda inner: (p, (inner + 7) // 8 * 8, None)  # noqa: E731  aligned rows of x
+    assert ws(*x(2001), p, 16, 32, 2001, 4096) == 0        # rows at 2 bytes: half the experts
+    assert ws(*x(2001), p, 17, 32, 2001, 4096) > 0
+    assert ws(*x(2000), p + 2, 17, 32, 2000, 4096) > 0     # the base counts too
+    assert ws(*x(2002), p, 24 * 32, 32, 2002, 4096) == 0   # at 4 bytes: 24 an expert
+    assert ws(*x(2002), p, 24 * 32 + 1, 32, 2002, 4096) > 0
+    assert ws(*x(700), p, 12 * 255, 255, 700, 129) == 0    # half of the last block is empty
+    assert ws(*x(700), p, 13 * 255, 255, 700, 129) > 0
+    assert ws(*x(129), p, 32 * 64, 64, 129, 128) == 0      # small weights
+    assert ws(*x(129), p, 32 * 64 + 1, 64, 129, 128) > 0
