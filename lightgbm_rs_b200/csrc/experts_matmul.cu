@@ -64,6 +64,7 @@
 
 #include "experts.cuh"
 #include "experts_parts.h"
+#include "wait_budget.h"
 
 namespace lgbm_b200 {
 namespace experts {
@@ -73,7 +74,6 @@ constexpr int kTileM = 128;       // rows of D of a CTA
 constexpr int kTileK = 64;         // 128 bytes of a 16-bit type: one swizzle row
 constexpr int kStoreRow = 64;      // bytes of a row in a storing warp's staging block
 constexpr int kBandRows = 2048;    // rows of D of a band, see tile_of
-constexpr uint64_t kWaitNs = 2000000000;
 // Entries of the table of groups: the rows before the first expert's, the experts, the rows past
 // the last one's, the end.
 constexpr int kGroupSlots = kMaxExperts + 3;
@@ -139,15 +139,16 @@ __device__ __forceinline__ uint64_t now_ns() {
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-// A whole warp waits; bounded: false, in every lane, when two seconds were not enough for one.
+// A whole warp waits; bounded: false, in every lane, when two seconds on the device were not
+// enough for one.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
   bool done = bar_try(bar, parity);
   if (!done) {
-    const uint64_t start = now_ns();
+    WaitBudget budget(now_ns());
     do {
 #pragma unroll 1
       for (int i = 0; i < 32 && !done; ++i) done = bar_try(bar, parity);
-    } while (!done && now_ns() - start < kWaitNs);
+    } while (!done && budget.spend(now_ns()));
   }
   return __all_sync(0xFFFFFFFFu, done);
 }
@@ -1264,8 +1265,8 @@ cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st)
 
 // Moves the error bits to where no kernel sets any, in one step: a bit that another thread's
 // kernel sets meanwhile is in this answer or in the next.
-__device__ uint32_t g_taken_error;
-__global__ void k_take_errors() { g_taken_error = atomicExch(&g_matmul_error, 0u); }
+static __device__ uint32_t g_taken_error;
+static __global__ void k_take_errors() { g_taken_error = atomicExch(&g_matmul_error, 0u); }
 
 // Waits for the whole device: work on streams that do not order with the legacy default stream,
 // as those of torch's pool, would go unnoticed otherwise.

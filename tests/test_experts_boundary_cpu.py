@@ -127,3 +127,23 @@ def test_streamed_or_copied_by_alignment(capi):
     assert ws(*x(700), p, 13 * 255, 255, 700, 129) > 0
     assert ws(*x(129), p, 32 * 64, 64, 129, 128) == 0      # small weights
     assert ws(*x(129), p, 32 * 64 + 1, 64, 129, 128) > 0
+
+
+def test_waits_do_not_count_time_off_the_device(tmp_path):
+    """A wait that is polled ends after two seconds; one that was switched out for minutes has lost a
+    hundredth of its time; looks that are each late end it after a hundred of them."""
+    lib = compiled(tmp_path, '#include "wait_budget.h"\n'
+                   'using lgbm_b200::experts::WaitBudget;\n'
+                   'extern "C" long looks(unsigned long long every, unsigned long long gap, long at) {\n'
+                   '  unsigned long long now = 12345;\n'
+                   '  WaitBudget b(now);\n'
+                   '  for (long i = 1;; ++i) {\n'
+                   '    now += i == at ? gap : every;\n'
+                   '    if (!b.spend(now)) return i;\n'
+                   '  }\n}\n')
+    looks = lambda every, gap=0, at=-1: lib.looks(  # noqa: E731
+        ctypes.c_ulonglong(every), ctypes.c_ulonglong(gap), ctypes.c_long(at))
+    lib.looks.restype = ctypes.c_long
+    assert looks(10_000) == 200_000
+    assert looks(10_000, gap=300 * 10 ** 9, at=7) == 200_000 - 2000 + 1
+    assert looks(10 ** 9) == 100
