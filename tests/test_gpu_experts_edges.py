@@ -358,3 +358,27 @@ def test_weights_at_any_address(ops, inner, outer, rows, start):
     assert torch.equal(ops.grouped_matmul(x, w, off), want)
     want = product64(dy, w.transpose(1, 2), off, None)[1].to(torch.bfloat16)
     assert torch.equal(ops.grouped_matmul_backward(dy, x, w, off, need_dw=False)[0], want)
+
+
+def test_many_narrow_rows(ops):
+    """As a tree's rows are: 28 features, more than 2^31 elements, experts of one matrix a leaf.
+    Small whole numbers: every sum is exact."""
+    n, inner, outer, E = 80_000_003, 28, 8, 3
+    g = gen(71)
+    ints = lambda *s: torch.randint(-2, 3, s, generator=g, device="cuda", dtype=torch.int8)  # noqa
+    x, dy = ints(n, inner).to(torch.bfloat16), ints(n, outer).to(torch.bfloat16)
+    w = ints(E, outer, inner).to(torch.bfloat16)
+    off = torch.tensor([2, 30_000_001, 30_000_001, n - 5], device="cuda", dtype=torch.int32)
+    y = ops.grouped_matmul(x, w, off)
+    dx, dw = ops.grouped_matmul_backward(dy, x, w, off, grad_dtype=torch.float32)
+    o = off.tolist()
+    assert not y[:2].any() and not y[-5:].any() and not dx[:2].any() and not dx[-5:].any()
+    for e in range(E):
+        want = torch.zeros(outer, inner, device="cuda", dtype=torch.float64)
+        for a in range(o[e], o[e + 1], 1 << 23):
+            s = slice(a, min(a + (1 << 23), o[e + 1]))
+            assert torch.equal(y[s].float(), x[s].float() @ w[e].float().T)
+            assert torch.equal(dx[s].float(), dy[s].float() @ w[e].float())
+            want += dy[s].double().T @ x[s].double()
+        assert torch.equal(dw[e].double(), want)
+    assert not dw[1].any()
