@@ -611,7 +611,7 @@ int lgbm_b200_experts_matmul_backward(const void* dy, int64_t dy_pitch, const vo
  * q: the weight's 4 bits, packed like a 4-bit bin row: [experts][outer][stride] bytes, weight
  * 2i in the low half of byte i, stride = ceil(inner / 2) rounded up to 16, 16-byte aligned
  * base. scales: x's type, [experts][outer][ceil(inner / group_size)]. z: zeros[e][n][group]
- * (0..15), or 8 where zeros is NULL. Products of q - z are summed in f32 within a group,
+ * (0..15: its low 4 bits), or 8 where zeros is NULL. Products of q - z are summed in f32 within a group,
  * then scaled in f32: no weight is rounded to 16 bits. */
 int lgbm_b200_experts_matmul_w4(const void* x, int64_t x_rows, int64_t x_pitch,
                                 const int32_t* index, const uint8_t* q, const void* scales,

@@ -142,4 +142,5 @@ def build_binding(force=False):
 if __name__ == "__main__":
     lib = build(force="--force" in sys.argv, verbose=True, ptxas_info="--ptxas" in sys.argv)
     print(lib)
-    print(build_binding(force="--force" in sys.argv) or "no torch here: its binding _experts.so is not built")
+    print(build_binding(force="--force" in sys.argv) or
+          "no torch here: its binding _experts.so is not built")

@@ -19,9 +19,9 @@
 // The tokens are staged in that pair order, which a sum over k does not see. Products of
 // q - z are summed in f32 inside a scale group and the group's sum is multiplied by its
 // scale in f32: no weight is ever rounded.
-// Measured (8 rows or fewer an expert): 16 bits, 32 experts of 4096 x 2048, 537 MB: 90 us, 6.0
-// TB/s, memory; 8 experts, 31 us, 4.4 TB/s: 256 blocks are 1.7 an SM. 4 bits, 32 experts of 4096
-// x 2000: groups of 128 41 us (3.3 TB/s), of 32 50 us; bound by instructions, about 50 for the
+// Measured (2 rows an expert): 16 bits, 32 experts of 4096 x 2048, 537 MB: 90 to 92 us, 5.9 TB/s,
+// memory; 8 experts, 29 us, 4.6 TB/s: 256 blocks are 1.7 an SM. 4 bits, 32 experts of 4096 x
+// 2000: groups of 128 41 us (3.3 TB/s), of 64 45, of 32 51; bound by instructions, about 50 for the
 // 256 bytes that a warp unpacks and multiplies at a time, 14 of them shifts and masks on the
 // integer pipe. One row of 8 x 4096 x 4096, two experts: 10 us, of which launch, the joined
 // cluster and the chain offsets - index - tokens are most.

@@ -27,35 +27,36 @@
 //
 // Ragged ends. FORWARD / INPUT: a tile's rows past its group's end are computed from the next
 // group's rows and not stored (a row of A only reaches its own row of D). Rows past the last
-// group and rows before the first form two more groups without a reduction: zeros. WEIGHT: the reduction itself ends
-// inside a block. Steps of 16 past the end are left out, and in the last step the rows past
-// it are overwritten with zeros in shared memory, in both operands: an infinity or NaN of the
-// next group cannot make 0 * inf. In a pair each CTA's second warp does that to its own half
-// and the odd one tells the even one. (Gathering that block's rows one by one, with zeros
-// from TMA for those outside, took five times a block's time, once a tile.)
+// group and rows before the first form two more groups without a reduction: zeros. WEIGHT: the
+// reduction itself ends inside a block. Steps of 16 past the end are left out, and in the last
+// step the rows past it are overwritten with zeros in shared memory, in both operands: an
+// infinity or NaN of the next group cannot make 0 * inf. In a pair each CTA's second warp does
+// that to its own half and the odd one tells the even one. (Gathering that block's rows one by
+// one, with zeros from TMA for those outside, took five times a block's time, once a tile.)
 //
 // Precision. The tensor cores cut a sum off when they add to it: 16 terms at a time, at most
 // 2^-23 of the sum each time. With terms of one sign nearly all of that was measured at every
 // addition: 1.6e-3 of the result at 2^18 terms in one piece, three times f16's unit roundoff.
-// A reduction is therefore accumulated in runs, which the storing warps add up in f32
-// (a rounding of 2^-24 a run). Results of 16 bits: runs of 4096, which cut off at most 3.1e-5, a
+// A reduction is therefore accumulated in runs, which the storing warps add up in f32 (a
+// rounding of 2^-24 a run). Results of 16 bits: runs of 4096, which cut off at most 3.1e-5, a
 // sixteenth of f16's unit roundoff. The second run on goes to the other half of tensor memory
 // and is added to the first half there, while the tensor cores wait (16 groups of 4096 rows on
-// average, 4096 x 2048: 2 %). Holding the sums in registers instead cost the tiles of one run up
-// to 45 % (255 experts of 129 x 700: the code of their odd stores spilled). A weight
+// average, 4096 x 2048: 2 %). Holding the sums in registers instead cost the tiles of one run
+// up to 45 % (255 experts of 129 x 700: the code of their odd stores spilled). A weight
 // gradient kept in f32 would show runs of that length, so there they are of 768, alternate
-// between the halves without a wait, and the sums stay in the registers of twice as many storing
-// warps: 7e-7 of the result up to 2^16 rows of random sign (1.3e-6 of one sign), 1.0e-6 (1.4e-6)
-// at 2^20, against 1.7e-5 (1.2e-4) of f32 sums one by one.
+// between the halves without a wait, and the sums stay in the registers of twice as many
+// storing warps: 7e-7 of the result up to 2^16 rows of random sign (1.3e-6 of one sign),
+// 1.0e-6 (1.4e-6) at 2^20, against 1.7e-5 (1.2e-4) of f32 sums one by one.
 //
-// Measured, loops on a warm GPU: 65536 rows, 16 experts of 4096 x 2048: y 0.90, dx 0.90, dw
-// 0.90 (bf16) and 1.04 ms (f32), 1.2 PFLOP/s with the clock held near 1.3 GHz by the power
-// cap; cuBLAS's batched product of the same size 0.83, 0.80, 0.80. 8192 rows, 8 experts of
-// 4096 x 1024: 68, 68, 68 us against 66, 60, 65 (1.0 PFLOP/s); tensor pipe 60 % busy; the rest
-// is the last wave, tiles that groups of 1024 and a few rows leave partly empty, and loads at
-// the 64 bytes a cycle that an SM takes from L2. 40009 rows, 255 experts of 136 x 704: y 33,
-// dx 47, dw 47 and 59 us, 2 to 3 TB/s: two or three blocks of reduction a tile, bound by
-// writing tiles out. (Dealing dw's tiles out longest group first gained nothing.)
+// Measured, loops on a warm GPU, equal groups: 65536 rows, 16 experts of 4096 x 2048: y 0.76
+// to 0.91 ms as the power cap lets the clock (1.2 to 1.4 PFLOP/s), dx 0.86 to 0.91, dw 0.90 to
+// 0.92 (bf16) and 1.04 to 1.06 (f32); cuBLAS's batched product of the same size 0.81 to 0.85,
+// 0.81, 0.80 to 0.84. 8192 rows, 8 experts of 4096 x 1024: 58, 63 to 71, 67 us (f32 90)
+// against 57 to 67, 51 to 55, 60 to 70; tensor pipe 52 to 63 % busy; the rest is the last
+// wave, tiles that groups of 1024 and a few rows leave partly empty, and loads at the 64 bytes
+// a cycle that an SM takes from L2. 40009 rows, 255 experts of 136 x 704: y 32, dx 49, dw 48
+// and 59 us, 2 to 3 TB/s: two or three blocks of reduction a tile, bound by writing tiles out.
+// (Dealing dw's tiles out longest group first gained nothing.)
 #include <algorithm>
 #include <atomic>
 #include <mutex>

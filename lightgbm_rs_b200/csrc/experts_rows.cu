@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kRowThreads)
                                    k0, k1, offset, out);
 }
 
-// Threads that share a token's row: the smallest power of two that covers it, 32 to 256.
+// Threads that share a token's row: the smallest power of two that covers it, 1 to 256.
 int row_lanes(int64_t vectors) {
   int lanes = 1;
   while (lanes < kRowThreads && lanes < vectors) lanes *= 2;

@@ -5,7 +5,8 @@ for every token from a gate's logits (experts masked with -inf are never picked:
 all but those of the leaf a tree sends the token to) and groups the T * k slots by expert;
 `grouped_matmul` multiplies each expert's ragged range of rows by its matrix; `combine` joins
 a token's k results; `dropout` regularises while training. Each has its gradient beside it.
-`grouped_matmul_w4` serves a few rows from weights of 4 bits.
+`grouped_matmul_w4` serves a few rows from weights of 4 bits. The trees do not call these
+functions; examples/leaf_experts.py joins both.
 
     r = experts.route(logits, k)                                # [T, E]
     h = experts.grouped_matmul(x, w1, r.offsets, rows=r.rows)   # x [T, K], w1 [E, H, K]
@@ -24,6 +25,11 @@ extension module built beside the library, and raise LightGBMError for arguments
 there is no CPU path. Nothing is recorded for autograd: under gradient mode an input that requires
 a gradient is refused, so call under `torch.no_grad()` (or inside a `torch.autograd.Function`) and
 use the gradient beside each function.
+
+Calls return before their kernels have run. Waits inside the product kernels are bounded (two
+seconds on the device): one that runs out, which no correct run does, leaves an incomplete result
+and sets a bit. `check_errors` waits for the device and raises for it; call it wherever results are
+taken for good, as at the end of a step that is checked or saved.
 """
 
 from collections import namedtuple
@@ -93,7 +99,8 @@ def grouped_matmul_w4(x, q, scales, offsets, zeros=None, rows=None, group_size=1
     in groups of `group_size` (32, 64 or 128) along the inner axis. q [E, outer, stride]
     uint8 packed like a 4-bit bin row (weight 2i in the low half of byte i, stride
     ceil(inner / 2) rounded up to 16); scales [E, outer, groups] of x's type; zeros
-    [E, outer, groups] uint8 (None: 8). `quantize_w4` makes them."""
+    [E, outer, groups] uint8, 0 to 15: the low 4 bits are taken (None: 8).
+    `quantize_w4` makes them."""
     return _X.grouped_matmul_w4(x, q, scales, offsets, zeros, rows, group_size)
 
 
