@@ -533,8 +533,8 @@ int lgbm_b200_predict(lgbm_b200_predictor* p, const double* rows, int64_t num_ro
  *
  * The rows of a batch ("tokens") are routed to k of E experts each, the tokens * k slots
  * are grouped by expert, every expert multiplies its ragged range of rows, and a token's
- * k results are joined: what a leaf-wise model does with its leaves, with a learned matrix
- * in each. No counterpart in the reference.
+ * k results are joined: learned matrices in ragged ranges of rows, as the leaves of a
+ * leaf-wise model are. The calls above do not use them. No counterpart in the reference.
  *
  * Conventions of these entry points
  *  - All array pointers are DEVICE pointers on the current device. The work is enqueued on

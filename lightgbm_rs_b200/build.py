@@ -91,7 +91,7 @@ def _torch_stamp():
     """What the binding's object depends on besides its source: the torch installed (its version
     file, read without importing it) and the Python ABI. None without torch."""
     spec = importlib.util.find_spec("torch")
-    if spec is None:
+    if spec is None or spec.origin is None:
         return None
     with open(os.path.join(os.path.dirname(spec.origin), "version.py")) as f:
         return f"{sysconfig.get_config_var('SOABI')} {spec.origin}\n{f.read()}"
