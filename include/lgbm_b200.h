@@ -605,6 +605,63 @@ int lgbm_b200_experts_matmul_backward(const void* dy, int64_t dy_pitch, const vo
                                       int32_t grad_dtype, int64_t rows, int32_t experts,
                                       int32_t inner, int32_t outer, void* dx, void* dw,
                                       void* workspace, int64_t workspace_bytes, void* stream);
+/* Products with what follows them, in the same kernel. act is one of LGBM_B200_ACT_*: relu, silu
+ * v / (1 + e^-v), gelu v P(v) with P the distribution function of the normal law.
+ *   linear  y[r] = act(w[e] x[..] + bias[e]) + residual[r]     [rows][outer]
+ *   gated   h[r] = act(gate) * up                              [rows][hidden], where gate and up
+ *           are the first and the last `hidden` columns of w[e] x[..]; w [experts][2 hidden][inner]
+ * bias [experts][outer] and residual [rows][outer] (of any pitch) are of the inputs' type; either
+ * may be NULL. A row of no expert has y = residual (0 without one) and h = 0.
+ * pre (NULL: not wanted) keeps what the activation was given, rounded to the inputs' type, for
+ * the backward pass: [rows][ld], gated [rows][2][ld] (gate, then up), ld = the width rounded up
+ * to 8, 16-byte aligned; what lies between the width and ld is not defined. Everything before
+ * the results' one rounding is in f32.
+ * Workspace: lgbm_b200_experts_matmul_workspace with the same operands (gated: outer =
+ * 2 hidden). */
+#define LGBM_B200_ACT_NONE 0
+#define LGBM_B200_ACT_RELU 1
+#define LGBM_B200_ACT_SILU 2
+#define LGBM_B200_ACT_GELU 3
+int lgbm_b200_experts_linear(const void* x, int64_t x_rows, int64_t x_pitch,
+                             const int32_t* index, const void* w, const void* bias,
+                             const void* residual, int64_t residual_pitch, const int32_t* offsets,
+                             int32_t dtype, int32_t act, int64_t rows, int32_t experts,
+                             int32_t inner, int32_t outer, void* y, void* pre, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+int lgbm_b200_experts_gated(const void* x, int64_t x_rows, int64_t x_pitch, const int32_t* index,
+                            const void* w, const int32_t* offsets, int32_t dtype, int32_t act,
+                            int64_t rows, int32_t experts, int32_t inner, int32_t hidden, void* h,
+                            void* pre, void* workspace, int64_t workspace_bytes, void* stream);
+/* Their gradients from dy [rows][outer] or dh [rows][hidden] (any pitch) and `pre` as the
+ * forward call wrote it (linear without an activation: not read, may be NULL). dx, dw as
+ * lgbm_b200_experts_matmul_backward; dbias [experts][outer] of grad_dtype. NULL results are not
+ * wanted. The residual's gradient is dy. The gradient of what the activation was given goes to
+ * the workspace in the inputs' type, as the matrix products take it: the only rounding between
+ * pre and dx, dw, which they hold however wide they are stored. dbias is summed in f32 from its
+ * values before that rounding. */
+int64_t lgbm_b200_experts_linear_backward_workspace(
+    const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, const int32_t* index,
+    const void* w, int32_t act, int64_t rows, int32_t experts, int32_t inner, int32_t outer,
+    int32_t want_dx, int32_t want_dw, int32_t want_dbias);
+int lgbm_b200_experts_linear_backward(const void* dy, int64_t dy_pitch, const void* pre,
+                                      const void* x, int64_t x_rows, int64_t x_pitch,
+                                      const int32_t* index, const void* w, const int32_t* offsets,
+                                      int32_t dtype, int32_t grad_dtype, int32_t act, int64_t rows,
+                                      int32_t experts, int32_t inner, int32_t outer, void* dx,
+                                      void* dw, void* dbias, void* workspace,
+                                      int64_t workspace_bytes, void* stream);
+int64_t lgbm_b200_experts_gated_backward_workspace(const void* x, int64_t x_pitch,
+                                                   const int32_t* index, const void* w,
+                                                   int64_t rows, int32_t experts, int32_t inner,
+                                                   int32_t hidden, int32_t want_dx,
+                                                   int32_t want_dw);
+int lgbm_b200_experts_gated_backward(const void* dh, int64_t dh_pitch, const void* pre,
+                                     const void* x, int64_t x_rows, int64_t x_pitch,
+                                     const int32_t* index, const void* w, const int32_t* offsets,
+                                     int32_t dtype, int32_t grad_dtype, int32_t act, int64_t rows,
+                                     int32_t experts, int32_t inner, int32_t hidden, void* dx,
+                                     void* dw, void* workspace, int64_t workspace_bytes,
+                                     void* stream);
 /* y as lgbm_b200_experts_matmul, for a few rows an expert, with weights of 4 bits in groups
  * of group_size (32, 64 or 128) along the inner axis:
  *   w[e][n][k] = scales[e][n][k / group_size] * (q - z)

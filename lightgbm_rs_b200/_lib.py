@@ -168,6 +168,20 @@ _SIGS = {
                                                      _i32, _i32, _i32], _i64),
     "lgbm_b200_experts_matmul_backward": ([_P, _i64, _P, _i64, _i64, _P, _P, _P, _i32, _i32, _i64,
                                            _i32, _i32, _i32, _P, _P, _P, _i64, _P], ctypes.c_int),
+    "lgbm_b200_experts_linear": ([_P, _i64, _i64, _P, _P, _P, _P, _i64, _P, _i32, _i32, _i64, _i32,
+                                  _i32, _i32, _P, _P, _P, _i64, _P], ctypes.c_int),
+    "lgbm_b200_experts_gated": ([_P, _i64, _i64, _P, _P, _P, _i32, _i32, _i64, _i32, _i32, _i32,
+                                 _P, _P, _P, _i64, _P], ctypes.c_int),
+    "lgbm_b200_experts_linear_backward_workspace": ([_P, _i64, _P, _i64, _P, _P, _i32, _i64, _i32,
+                                                     _i32, _i32, _i32, _i32, _i32], _i64),
+    "lgbm_b200_experts_linear_backward": ([_P, _i64, _P, _P, _i64, _i64, _P, _P, _P, _i32, _i32,
+                                           _i32, _i64, _i32, _i32, _i32, _P, _P, _P, _P, _i64,
+                                           _P], ctypes.c_int),
+    "lgbm_b200_experts_gated_backward_workspace": ([_P, _i64, _P, _P, _i64, _i32, _i32, _i32, _i32,
+                                                    _i32], _i64),
+    "lgbm_b200_experts_gated_backward": ([_P, _i64, _P, _P, _i64, _i64, _P, _P, _P, _i32, _i32,
+                                          _i32, _i64, _i32, _i32, _i32, _P, _P, _P, _i64, _P],
+                                         ctypes.c_int),
     "lgbm_b200_experts_matmul_w4": ([_P, _i64, _i64, _P, _P, _P, _P, _i32, _P, _i32, _i64, _i32,
                                      _i32, _i32, _P, _P], ctypes.c_int),
     "lgbm_b200_experts_errors": ([_P], ctypes.c_int),

@@ -143,6 +143,20 @@ cudaError_t launch_dropout(const void* x, const void* residual, int32_t dtype, i
                            int64_t width, int64_t pitch, int64_t residual_pitch, uint32_t drop,
                            uint64_t seed, uint64_t offset, void* out, cudaStream_t st);
 
+// What follows a product on its way out: y = act(product + bias) + residual, or gated
+// (the product's first half of columns the gate, the other half up): y = act(gate) up.
+struct Epilogue {
+  bool on;                  // else the product alone
+  bool gated;
+  int32_t act;              // LGBM_B200_ACT_*
+  const void* bias;         // [experts][outer] or null
+  const void* residual;     // [rows][outer] or null
+  int64_t residual_pitch;
+  void* pre;                // what the activation was given, [rows][1 or 2][pre_pitch], or null
+};
+// Elements of a saved row: padded to 16 bytes, for loads and stores of 16 bytes at any width.
+inline int64_t pre_pitch(int64_t width) { return (width + 7) / 8 * 8; }
+
 // experts_matmul.cu
 struct MatmulCall {
   int32_t dtype, grad_dtype;
@@ -156,10 +170,34 @@ struct MatmulCall {
   int64_t rows;
   int32_t experts, inner, outer;
   void *y, *dx, *dw;        // results, null: not wanted
+  Epilogue epilogue;        // of y
 };
 int64_t matmul_workspace(const MatmulCall& c);
 cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st);
 cudaError_t take_matmul_errors(uint32_t* bits);
+
+// experts_act.cu
+// dpre of a gated layer, rows of `dpre_pitch`: gate's columns, then up's.
+cudaError_t launch_gated_grad(const void* dh, int64_t dh_pitch, const void* pre, int32_t dtype,
+                              int32_t act, int64_t rows, int32_t hidden, void* dpre,
+                              int64_t dpre_pitch, cudaStream_t st);
+// dpre = dy act'(pre) (null where act is NONE: dpre is dy) and the bias's gradient, dpre's sums
+// over each expert's rows (null: not wanted). `sums` is linear_grad_workspace bytes.
+struct LinearGrad {
+  const void* dy;
+  int64_t dy_pitch;
+  const void* pre;
+  int32_t dtype, grad_dtype, act;
+  const int32_t* offsets;
+  int64_t rows;
+  int32_t experts, outer;
+  void* dpre;
+  int64_t dpre_pitch;
+  void* dbias;
+  float* sums;
+};
+int64_t linear_grad_workspace(int64_t rows, int32_t experts, int32_t outer);
+cudaError_t launch_linear_grad(const LinearGrad& c, cudaStream_t st);
 
 // experts_few.cu
 struct FewCall {
@@ -175,6 +213,7 @@ struct FewCall {
   int64_t rows;
   int32_t experts, inner, outer;
   void* y;
+  Epilogue epilogue;       // weights of 16 bits only
 };
 cudaError_t launch_few(const FewCall& c, cudaStream_t st);
 

@@ -1,0 +1,110 @@
+// Activations of the expert layers in f32, and their derivatives.
+//
+// All three are exact to a few units of 2^-22 but gelu, which is good to 6e-6 of its value (a
+// ninetieth of f16's unit roundoff): results and saved values are rounded to 16 bits behind it.
+// act(0) is 0 for each.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "lgbm_b200.h"
+
+namespace lgbm_b200 {
+namespace experts {
+
+template <int ACT>
+struct Act;
+
+template <>
+struct Act<LGBM_B200_ACT_NONE> {
+  static __device__ __forceinline__ float value(float v) { return v; }
+  static __device__ __forceinline__ void both(float v, float& a, float& d) {
+    a = v;
+    d = 1.0f;
+  }
+};
+
+// NaN stays NaN; the slope at 0 is 0.
+template <>
+struct Act<LGBM_B200_ACT_RELU> {
+  static __device__ __forceinline__ float value(float v) { return v < 0.0f ? 0.0f : v; }
+  static __device__ __forceinline__ void both(float v, float& a, float& d) {
+    a = value(v);
+    d = v > 0.0f ? 1.0f : v <= 0.0f ? 0.0f : v;
+  }
+};
+
+// v s(v), s = 1 / (1 + e^-v). Where e^-v overflows (v < -88) the quotient is 0.
+template <>
+struct Act<LGBM_B200_ACT_SILU> {
+  static __device__ __forceinline__ float value(float v) {
+    return __fdividef(v, 1.0f + __expf(-v));
+  }
+  static __device__ __forceinline__ void both(float v, float& a, float& d) {
+    const float s = __fdividef(1.0f, 1.0f + __expf(-v));
+    a = v * s;
+    d = s * fmaf(v, 1.0f - s, 1.0f);
+  }
+};
+
+// v P(v), P the distribution function of the normal law. With t = 1 / (1 + q |v|) (Hastings'
+// form, 1955) the tail 1 - P(|v|) = e^(-v^2 / 2) (a1 t + .. + a6 t^6): coefficients fitted for the
+// smallest largest relative error on |v| <= 17, 5.1e-6. 1 + erf(v) would leave nothing of P at
+// v < -5, and erfcf takes twice the instructions.
+template <>
+struct Act<LGBM_B200_ACT_GELU> {
+  static __device__ __forceinline__ float tail(float v, float e) {
+    const float t = __fdividef(1.0f, fmaf(0.311f, fabsf(v), 1.0f));
+    float s = fmaf(-0.0731476133f, t, 0.175886592f);
+    s = fmaf(s, t, 0.0198684974f);
+    s = fmaf(s, t, 0.13196364f);
+    s = fmaf(s, t, 0.121193485f);
+    s = fmaf(s, t, 0.124232849f);
+    return s * t * e;
+  }
+  static __device__ __forceinline__ float value(float v) {
+    const float p = tail(v, __expf(-0.5f * v * v));
+    return v * (v < 0.0f ? p : 1.0f - p);
+  }
+  static __device__ __forceinline__ void both(float v, float& a, float& d) {
+    const float e = __expf(-0.5f * v * v), q = tail(v, e), p = v < 0.0f ? q : 1.0f - q;
+    a = v * p;
+    d = fmaf(v * 0.39894228f, e, p);  // 1 / sqrt(2 pi)
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void activate(int act, float (&v)[N]) {
+  if (act == LGBM_B200_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = Act<LGBM_B200_ACT_SILU>::value(v[i]);
+  } else if (act == LGBM_B200_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = Act<LGBM_B200_ACT_GELU>::value(v[i]);
+  } else if (act == LGBM_B200_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = Act<LGBM_B200_ACT_RELU>::value(v[i]);
+  }
+}
+
+// Values a and slopes d.
+template <int N>
+__device__ __forceinline__ void activate_both(int act, const float (&v)[N], float (&a)[N],
+                                              float (&d)[N]) {
+  if (act == LGBM_B200_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) Act<LGBM_B200_ACT_SILU>::both(v[i], a[i], d[i]);
+  } else if (act == LGBM_B200_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) Act<LGBM_B200_ACT_GELU>::both(v[i], a[i], d[i]);
+  } else if (act == LGBM_B200_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) Act<LGBM_B200_ACT_RELU>::both(v[i], a[i], d[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) Act<LGBM_B200_ACT_NONE>::both(v[i], a[i], d[i]);
+  }
+}
+
+}  // namespace experts
+}  // namespace lgbm_b200

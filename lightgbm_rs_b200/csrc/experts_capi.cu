@@ -111,9 +111,39 @@ int check_product(const char* what, const MatmulCall& c) {
   return LGBM_B200_OK;
 }
 
+bool is_act(int32_t act) {
+  return act == LGBM_B200_ACT_NONE || act == LGBM_B200_ACT_RELU || act == LGBM_B200_ACT_SILU ||
+         act == LGBM_B200_ACT_GELU;
+}
+
+// The weight rows of a gated layer, or -1 where its width is refused anyway.
+int32_t gated_outer(int32_t hidden) {
+  return hidden < 1 || hidden > kMaxWidth / 2 ? -1 : 2 * hidden;
+}
+int check_hidden(const char* what, int32_t hidden) {
+  if (hidden < 1) return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: hidden %d", what, hidden);
+  if (hidden > kMaxWidth / 2)
+    return refuse(LGBM_B200_CAPABILITY_UNAVAILABLE, "%s: hidden %d (at most %d)", what, hidden,
+                  kMaxWidth / 2);
+  return LGBM_B200_OK;
+}
+
+int check_epilogue(const char* what, const MatmulCall& c) {
+  const Epilogue& e = c.epilogue;
+  if (!is_act(e.act)) return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: activation %d", what, e.act);
+  if (e.residual && e.residual_pitch < c.outer)
+    return refuse(LGBM_B200_LENGTH_MISMATCH, "%s: residual pitch %lld < outer %d", what,
+                  (long long)e.residual_pitch, c.outer);
+  if (!aligned16(e.pre))
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: pre is not 16-byte aligned", what);
+  return check_starts(what, {{e.bias, 2}, {e.residual, 2}});
+}
+
 int run_product(const char* what, const MatmulCall& c, void* workspace, int64_t workspace_bytes,
                 void* stream) {
   if (int rc = check_product(what, c)) return rc;
+  if (c.epilogue.on)
+    if (int rc = check_epilogue(what, c)) return rc;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (c.rows == 0) {
     if (!c.dw) return LGBM_B200_OK;
@@ -127,6 +157,114 @@ int run_product(const char* what, const MatmulCall& c, void* workspace, int64_t 
     return refuse(LGBM_B200_LENGTH_MISMATCH, "%s: workspace of %lld bytes, %lld are needed",
                   what, (long long)workspace_bytes, (long long)need);
   return launched(launch_matmul(c, workspace, st), what);
+}
+
+// The gradient of what the activation was given, in the workspace ahead of what the products need.
+int64_t dpre_bytes(int64_t rows, int32_t outer) {
+  return (rows * pre_pitch(outer) * 2 + 255) / 256 * 256;
+}
+int64_t sums_bytes(int64_t rows, int32_t experts, int32_t outer) {
+  return (linear_grad_workspace(rows, experts, outer) + 255) / 256 * 256;
+}
+
+// Both gradients of a layer's products and what comes before them; c.dy, c.outer are the layer's.
+int run_layer_backward(const char* what, MatmulCall c, bool gated, int32_t act, const void* pre,
+                       void* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!is_act(act)) return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: activation %d", what, act);
+  if (!c.dx && !c.dw && !dbias && c.rows > 0)
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: no gradient is wanted", what);
+  if ((c.dw || dbias) && c.grad_dtype != c.dtype && c.grad_dtype != LGBM_B200_DTYPE_F32)
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: dtype %d of the weights' gradients", what,
+                  c.grad_dtype);
+  const int32_t width = gated ? c.outer / 2 : c.outer;  // of dy
+  const bool turns = gated || act != LGBM_B200_ACT_NONE;  // dpre is not dy itself
+  // what check_product sees of dy: a pitch that fits, where dpre takes its place
+  MatmulCall p = c;
+  if (turns) p.dy_pitch = pre_pitch(c.outer);
+  if (int rc = check_product(what, p)) return rc;
+  if (c.dy_pitch < width)
+    return refuse(LGBM_B200_LENGTH_MISMATCH, "%s: dy pitch %lld < %d", what,
+                  (long long)c.dy_pitch, width);
+  if (c.rows > 0 && (!c.dy || (turns && !pre)))
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
+  if (turns && !aligned16(pre))
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: pre is not 16-byte aligned", what);
+  if (int rc = check_starts(what, {{c.dy, 2}, {dbias, dbias ? elem_size(c.grad_dtype) : 1}}))
+    return rc;
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (c.rows == 0) {
+    cudaError_t err = cudaSuccess;
+    const int64_t size = elem_size(c.grad_dtype);
+    if (c.dw)
+      err = cudaMemsetAsync(c.dw, 0, (size_t)(size * c.experts * c.outer * c.inner), st);
+    if (err == cudaSuccess && dbias)
+      err = cudaMemsetAsync(dbias, 0, (size_t)(size * c.experts * c.outer), st);
+    return launched(err, what);
+  }
+  char* ws = static_cast<char*>(workspace);
+  int64_t need = 0;
+  if (turns) {
+    p.dy = ws;
+    need += dpre_bytes(c.rows, c.outer);
+  }
+  float* sums = reinterpret_cast<float*>(ws + need);
+  if (dbias) need += sums_bytes(c.rows, c.experts, c.outer);
+  const bool products = c.dx || c.dw;
+  const int64_t own = need;
+  if (turns) p.dy = reinterpret_cast<const void*>((uintptr_t)256);  // aligned, for the question
+  if (products) need += matmul_workspace(p);
+  if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace))))
+    return refuse(LGBM_B200_LENGTH_MISMATCH, "%s: workspace of %lld bytes, %lld are needed",
+                  what, (long long)workspace_bytes, (long long)need);
+  if (turns) p.dy = ws;
+  if (gated) {
+    if (int rc = launched(launch_gated_grad(c.dy, c.dy_pitch, pre, c.dtype, act, c.rows, width, ws,
+                                            p.dy_pitch, st),
+                          what))
+      return rc;
+  } else if (turns || dbias) {
+    LinearGrad l{};
+    l.dy = c.dy;
+    l.dy_pitch = c.dy_pitch;
+    l.pre = pre;
+    l.dtype = c.dtype;
+    l.grad_dtype = c.grad_dtype;
+    l.act = act;
+    l.offsets = c.offsets;
+    l.rows = c.rows;
+    l.experts = c.experts;
+    l.outer = c.outer;
+    l.dpre = turns ? ws : nullptr;
+    l.dpre_pitch = p.dy_pitch;
+    l.dbias = dbias;
+    l.sums = sums;
+    if (int rc = launched(launch_linear_grad(l, st), what)) return rc;
+  }
+  return products ? launched(launch_matmul(p, ws + own, st), what) : LGBM_B200_OK;
+}
+
+int64_t layer_backward_workspace(const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch,
+                                 const int32_t* index, const void* w, int32_t act, bool gated,
+                                 int64_t rows, int32_t experts, int32_t inner, int32_t outer,
+                                 int32_t want_dx, int32_t want_dw, int32_t want_dbias) {
+  if (rows < 1 || experts < 1 || inner < 1 || outer < 1) return 0;
+  const bool turns = gated || act != LGBM_B200_ACT_NONE;
+  int64_t need = (turns ? dpre_bytes(rows, outer) : 0) +
+                 (want_dbias ? sums_bytes(rows, experts, outer) : 0);
+  MatmulCall c{};
+  c.x = x;
+  c.x_pitch = x_pitch;
+  c.index = index;
+  c.dy = turns ? reinterpret_cast<const void*>((uintptr_t)256) : dy;
+  c.dy_pitch = turns ? pre_pitch(outer) : dy_pitch;
+  c.w = w;
+  c.rows = rows;
+  c.experts = experts;
+  c.inner = inner;
+  c.outer = outer;
+  c.dx = want_dx ? &c : nullptr;  // wanted; not written here
+  c.dw = want_dw ? &c : nullptr;
+  return c.dx || c.dw ? need + matmul_workspace(c) : need;
 }
 
 }  // namespace
@@ -357,6 +495,129 @@ int lgbm_b200_experts_matmul_backward(const void* dy, int64_t dy_pitch, const vo
   c.dx = dx;
   c.dw = dw;
   return run_product(what, c, workspace, workspace_bytes, stream);
+}
+
+int lgbm_b200_experts_linear(const void* x, int64_t x_rows, int64_t x_pitch,
+                             const int32_t* index, const void* w, const void* bias,
+                             const void* residual, int64_t residual_pitch, const int32_t* offsets,
+                             int32_t dtype, int32_t act, int64_t rows, int32_t experts,
+                             int32_t inner, int32_t outer, void* y, void* pre, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  const char* what = "experts_linear";
+  if (!y && rows > 0) return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
+  MatmulCall c{};
+  c.dtype = dtype;
+  c.x = x;
+  c.x_rows = x_rows;
+  c.x_pitch = x_pitch;
+  c.index = index;
+  c.w = w;
+  c.offsets = offsets;
+  c.rows = rows;
+  c.experts = experts;
+  c.inner = inner;
+  c.outer = outer;
+  c.y = y ? y : &c;  // no rows: nothing is written
+  c.epilogue = {true, false, act, bias, residual, residual_pitch, pre};
+  return run_product(what, c, workspace, workspace_bytes, stream);
+}
+
+int lgbm_b200_experts_gated(const void* x, int64_t x_rows, int64_t x_pitch, const int32_t* index,
+                            const void* w, const int32_t* offsets, int32_t dtype, int32_t act,
+                            int64_t rows, int32_t experts, int32_t inner, int32_t hidden, void* h,
+                            void* pre, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "experts_gated";
+  if (!h && rows > 0) return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
+  if (int rc = check_hidden(what, hidden)) return rc;
+  MatmulCall c{};
+  c.dtype = dtype;
+  c.x = x;
+  c.x_rows = x_rows;
+  c.x_pitch = x_pitch;
+  c.index = index;
+  c.w = w;
+  c.offsets = offsets;
+  c.rows = rows;
+  c.experts = experts;
+  c.inner = inner;
+  c.outer = gated_outer(hidden);
+  c.y = h ? h : &c;  // no rows: nothing is written
+  c.epilogue = {true, true, act, nullptr, nullptr, 0, pre};
+  return run_product(what, c, workspace, workspace_bytes, stream);
+}
+
+int64_t lgbm_b200_experts_linear_backward_workspace(
+    const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, const int32_t* index,
+    const void* w, int32_t act, int64_t rows, int32_t experts, int32_t inner, int32_t outer,
+    int32_t want_dx, int32_t want_dw, int32_t want_dbias) {
+  return layer_backward_workspace(dy, dy_pitch, x, x_pitch, index, w, act, false, rows, experts,
+                                  inner, outer, want_dx, want_dw, want_dbias);
+}
+
+int lgbm_b200_experts_linear_backward(const void* dy, int64_t dy_pitch, const void* pre,
+                                      const void* x, int64_t x_rows, int64_t x_pitch,
+                                      const int32_t* index, const void* w, const int32_t* offsets,
+                                      int32_t dtype, int32_t grad_dtype, int32_t act, int64_t rows,
+                                      int32_t experts, int32_t inner, int32_t outer, void* dx,
+                                      void* dw, void* dbias, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+  MatmulCall c{};
+  c.dtype = dtype;
+  c.grad_dtype = grad_dtype;
+  c.x = x;
+  c.x_rows = x_rows;
+  c.x_pitch = x_pitch;
+  c.index = index;
+  c.dy = dy;
+  c.dy_pitch = dy_pitch;
+  c.w = w;
+  c.offsets = offsets;
+  c.rows = rows;
+  c.experts = experts;
+  c.inner = inner;
+  c.outer = outer;
+  c.dx = dx;
+  c.dw = dw;
+  return run_layer_backward("experts_linear_backward", c, false, act, pre, dbias, workspace,
+                            workspace_bytes, stream);
+}
+
+int64_t lgbm_b200_experts_gated_backward_workspace(const void* x, int64_t x_pitch,
+                                                   const int32_t* index, const void* w,
+                                                   int64_t rows, int32_t experts, int32_t inner,
+                                                   int32_t hidden, int32_t want_dx,
+                                                   int32_t want_dw) {
+  return layer_backward_workspace(nullptr, 0, x, x_pitch, index, w, LGBM_B200_ACT_NONE, true, rows,
+                                  experts, inner, gated_outer(hidden), want_dx, want_dw, 0);
+}
+
+int lgbm_b200_experts_gated_backward(const void* dh, int64_t dh_pitch, const void* pre,
+                                     const void* x, int64_t x_rows, int64_t x_pitch,
+                                     const int32_t* index, const void* w, const int32_t* offsets,
+                                     int32_t dtype, int32_t grad_dtype, int32_t act, int64_t rows,
+                                     int32_t experts, int32_t inner, int32_t hidden, void* dx,
+                                     void* dw, void* workspace, int64_t workspace_bytes,
+                                     void* stream) {
+  const char* what = "experts_gated_backward";
+  if (int rc = check_hidden(what, hidden)) return rc;
+  MatmulCall c{};
+  c.dtype = dtype;
+  c.grad_dtype = grad_dtype;
+  c.x = x;
+  c.x_rows = x_rows;
+  c.x_pitch = x_pitch;
+  c.index = index;
+  c.dy = dh;
+  c.dy_pitch = dh_pitch;
+  c.w = w;
+  c.offsets = offsets;
+  c.rows = rows;
+  c.experts = experts;
+  c.inner = inner;
+  c.outer = gated_outer(hidden);
+  c.dx = dx;
+  c.dw = dw;
+  return run_layer_backward(what, c, true, act, pre, nullptr, workspace, workspace_bytes, stream);
 }
 
 int lgbm_b200_experts_matmul_w4(const void* x, int64_t x_rows, int64_t x_pitch,

@@ -31,6 +31,7 @@
 #include <cooperative_groups.h>
 
 #include "experts.cuh"
+#include "experts_act.cuh"
 
 namespace lgbm_b200 {
 namespace experts {
@@ -64,6 +65,9 @@ struct FewArgs {
   int32_t slice;           // inner length of each, a multiple of 256
   int32_t panel;           // inner length of x and scales staged at a time, same
   int32_t x_vec;           // x may be read 16 bytes at a time
+  Epilogue epilogue;       // PLAIN: not looked at
+  int32_t cols;            // columns of y: outer, or half of it when gated
+  int64_t pre_pitch;
 };
 
 __device__ __forceinline__ uint32_t shared_addr(const void* p) {
@@ -164,11 +168,17 @@ __device__ __forceinline__ uint32_t sub2<__nv_bfloat16>(uint32_t a, uint32_t b) 
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// What becomes of a product on its way out.
+enum Finish { PLAIN = 0, FINISH_LINEAR = 1, FINISH_GATED = 2 };
+
 // A kernel's variant: TILES column tiles of 8 rows make an item; SHIFT is log2 of the scale
 // group's size, 0 with weights of 16 bits, whose rows are aligned to ALIGN bytes.
-template <typename T_, int TILES_, int SHIFT_, bool ZEROS_, int ALIGN_>
+template <typename T_, int TILES_, int SHIFT_, bool ZEROS_, int ALIGN_, int FINISH_ = PLAIN>
 struct FewShape {
   using T = T_;
+  static constexpr int FINISH = FINISH_;
+  // columns of y of a block; gated, half of its warps take gate and half take up
+  static constexpr int kOut = FINISH == FINISH_GATED ? kOutBlock / 2 : kOutBlock;
   static constexpr int TILES = TILES_, SHIFT = SHIFT_, ALIGN = ALIGN_;
   static constexpr bool W4 = SHIFT > 0, ZEROS = ZEROS_;
   // Blocks that share an SM, and stages of a warp's ring: with 4 bits the arithmetic wants
@@ -252,9 +262,35 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   const int expert = item[0], begin = item[1], nrows = item[2];
   if (expert < 0) return;  // the whole cluster has the same item
   const int rank = blockIdx.x % g.split;
-  const int out0 = blockIdx.x / g.split % g.blocks * kOutBlock;
+  const int out0 = blockIdx.x / g.split % g.blocks * S::kOut;
   const int k_begin = rank * g.slice, k_end = min(g.inner, k_begin + g.slice);
   T* y = static_cast<T*>(g.y);
+  // Column n of row `row` of the result, from its product or the gate's and up's.
+  auto finish = [&](int64_t row, int n, float v, float up, bool live) {
+    const Epilogue& e = g.epilogue;
+    if (S::FINISH == FINISH_LINEAR && live && e.bias)
+      v += to_f32<T>(static_cast<const T*>(e.bias)[(int64_t)expert * g.cols + n]);
+    if (e.pre) {
+      constexpr int kHalves = S::FINISH == FINISH_GATED ? 2 : 1;
+      T* pre = static_cast<T*>(e.pre) + row * kHalves * g.pre_pitch + n;
+      *pre = from_f32<T>(v);
+      if (kHalves == 2) pre[g.pre_pitch] = from_f32<T>(up);
+    }
+    float a[1] = {v};
+    activate(e.act, a);
+    if (S::FINISH == FINISH_GATED) a[0] *= up;
+    if (S::FINISH == FINISH_LINEAR && e.residual)
+      a[0] += to_f32<T>(static_cast<const T*>(e.residual)[row * e.residual_pitch + n]);
+    y[row * g.cols + n] = from_f32<T>(a[0]);
+  };
+  if (S::FINISH != PLAIN && expert >= g.experts) {
+    if (rank == 0)
+      for (int i = threadIdx.x; i < nrows * S::kOut; i += kFewThreads) {
+        const int n = out0 + i % S::kOut;
+        if (n < g.cols) finish(begin + i / S::kOut, n, 0.0f, 0.0f, false);
+      }
+    return;
+  }
   if (expert >= g.experts) {
     if (rank == 0)
       for (int i = threadIdx.x; i < nrows * kOutBlock; i += kFewThreads) {
@@ -265,7 +301,10 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   }
 
   const int tiles = (nrows + 7) / 8;
-  const int my_row0 = out0 + warp * 16;
+  // This warp's first weight row, and the row that its outputs end at.
+  const bool upper = S::FINISH == FINISH_GATED && warp >= kFewWarps / 2;
+  const int my_row0 = (upper ? g.cols - S::kOut : 0) + out0 + warp * 16;
+  const int row_end = S::FINISH == FINISH_GATED && !upper ? g.cols : g.outer;
   const char* wbase = static_cast<const char*>(g.w) +
                       ((int64_t)expert * g.outer + my_row0) * g.w_pitch;
   const int row_bytes = W4 ? (int)g.w_pitch : g.inner * 2;
@@ -274,7 +313,7 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   // this lane's piece of rows lane / 8 + 4 j of a stage
   const char* src0 = wbase + (int64_t)(lane >> 3) * g.w_pitch + byte0 + (lane & 7) * 16;
   const uint32_t dst0 = shared_addr(ring) + (lane >> 3) * kRowPitch + (lane & 7) * 16;
-  const int rest0 = row_bytes - byte0 - (lane & 7) * 16, rows_in = g.outer - my_row0 - (lane >> 3);
+  const int rest0 = row_bytes - byte0 - (lane & 7) * 16, rows_in = row_end - my_row0 - (lane >> 3);
   const int64_t step4 = 4 * g.w_pitch;
   int load_slot = 0;
   auto load_stage = [&](int i) {
@@ -282,7 +321,7 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
       const char* src = src0 + i * kRowBytes;  // of the slice's stage i
       const uint32_t dst = dst0 + load_slot * kStageBytes;
       const int rest = rest0 - i * kRowBytes;
-      if (S::ALIGN == 16 && my_row0 + 16 <= g.outer &&
+      if (S::ALIGN == 16 && my_row0 + 16 <= row_end &&
           byte0 + (i + 1) * kRowBytes <= row_bytes) {  // all of it exists
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -565,6 +604,27 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
       at[8] = W4 ? acc[n][2] : total[n][2];
       at[kOutBlock + 8] = W4 ? acc[n][3] : total[n][3];
     }
+  if constexpr (S::FINISH != PLAIN) {
+    // the whole sum of element i of the blocks' partial sums, in the blocks' order
+    cg::cluster_group cluster = cg::this_cluster();
+    if (g.split == 1) __syncthreads();
+    else cluster.sync();
+    auto whole = [&](int i) {
+      if (g.split == 1) return sums[i];
+      float s = 0.0f;
+      for (int r = 0; r < g.split; ++r) s += cluster.map_shared_rank(sums, r)[i];
+      return s;
+    };
+    for (int i = rank * kFewThreads + threadIdx.x; i < nrows * S::kOut;
+         i += g.split * kFewThreads) {
+      const int r = i / S::kOut, n = i % S::kOut;
+      if (out0 + n < g.cols)
+        finish(begin + r, out0 + n, whole(r * kOutBlock + n),
+               S::FINISH == FINISH_GATED ? whole(r * kOutBlock + kOutBlock / 2 + n) : 0.0f, true);
+    }
+    if (g.split > 1) cluster.sync();
+    return;
+  }
   if (g.split == 1) {
     __syncthreads();
     for (int i = threadIdx.x; i < nrows * kOutBlock; i += kFewThreads) {
@@ -601,7 +661,7 @@ cudaError_t launch_few_shape(FewArgs g, cudaStream_t st) {
     if (err != cudaSuccess) return err;
     ready[dev].store(true, std::memory_order_release);
   }
-  const int64_t blocks = (g.outer + kOutBlock - 1) / kOutBlock;
+  const int64_t blocks = (g.cols + S::kOut - 1) / S::kOut;
   // every group of rows, the two without an expert among them, has one ragged item at most
   const int64_t items = std::min<int64_t>(g.experts + 2, g.rows) + g.rows / S::kRows;
   // Split the inner axis, in steps of at least 512, while the blocks would not fill the SMs.
@@ -629,17 +689,27 @@ cudaError_t launch_few_shape(FewArgs g, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, k_grouped_few<S>, g);
 }
 
-template <typename T, int SHIFT, bool ZEROS, int ALIGN>
+template <typename T, int SHIFT, bool ZEROS, int ALIGN, int FINISH = PLAIN>
 cudaError_t launch_few_rows(const FewArgs& g, cudaStream_t st) {
   // Items of 8 rows while few experts can have more: no test for absent column tiles in the
   // inner loop, and the tokens of twice the inner length in shared memory.
   return g.rows <= 4 * (int64_t)g.experts || g.rows <= 8
-             ? launch_few_shape<FewShape<T, 1, SHIFT, ZEROS, ALIGN>>(g, st)
-             : launch_few_shape<FewShape<T, 4, SHIFT, ZEROS, ALIGN>>(g, st);
+             ? launch_few_shape<FewShape<T, 1, SHIFT, ZEROS, ALIGN, FINISH>>(g, st)
+             : launch_few_shape<FewShape<T, 4, SHIFT, ZEROS, ALIGN, FINISH>>(g, st);
+}
+
+template <typename T, int FINISH>
+cudaError_t launch_few_finish(const FewArgs& g, int align, cudaStream_t st) {
+  if (align == 16) return launch_few_rows<T, 0, false, 16, FINISH>(g, st);
+  if (align == 4) return launch_few_rows<T, 0, false, 4, FINISH>(g, st);
+  return launch_few_rows<T, 0, false, 2, FINISH>(g, st);
 }
 
 template <typename T>
 cudaError_t launch_few_typed(const FewArgs& g, int group_size, int align, cudaStream_t st) {
+  if (g.epilogue.on)
+    return g.epilogue.gated ? launch_few_finish<T, FINISH_GATED>(g, align, st)
+                            : launch_few_finish<T, FINISH_LINEAR>(g, align, st);
   if (group_size == 0) {
     if (align == 16) return launch_few_rows<T, 0, false, 16>(g, st);
     if (align == 4) return launch_few_rows<T, 0, false, 4>(g, st);
@@ -671,6 +741,9 @@ cudaError_t launch_few(const FewCall& c, cudaStream_t st) {
   g.rows = c.rows;
   g.y = c.y;
   g.x_vec = aligned16(c.x) && c.x_pitch % 8 == 0;
+  g.epilogue = c.epilogue;
+  g.cols = c.epilogue.gated ? c.outer / 2 : c.outer;
+  g.pre_pitch = pre_pitch(g.cols);
   int align = 16;
   if (c.group_size == 0) {
     g.w_pitch = (int64_t)c.inner * 2;

@@ -64,6 +64,7 @@
 #include <cuda.h>  // types of the tensor map; the encoder is looked up at run time
 
 #include "experts.cuh"
+#include "experts_act.cuh"
 #include "experts_parts.h"
 #include "wait_budget.h"
 
@@ -79,7 +80,7 @@ constexpr int kBandRows = 2048;    // rows of D of a band, see tile_of
 // the last one's, the end.
 constexpr int kGroupSlots = kMaxExperts + 3;
 
-enum Mode { FORWARD = 0, INPUT = 1, WEIGHT = 2, WEIGHT_F32 = 3 };
+enum Mode { FORWARD = 0, INPUT = 1, WEIGHT = 2, WEIGHT_F32 = 3, LINEAR = 4, GATED = 5 };
 
 struct MatArgs {
   const int32_t* offsets;
@@ -95,6 +96,15 @@ struct MatArgs {
   int64_t out_pitch;
   void* out;
   uint32_t* error;
+  // LINEAR, GATED
+  int32_t act;
+  int32_t bias_vec;       // the bias may be read 16 bytes at a time
+  int32_t residual_unit;  // bytes of a load, as `unit`
+  const void* bias;
+  const void* residual;
+  int64_t residual_pitch;
+  void* pre;
+  int64_t pre_pitch;
 };
 
 // Set by a kernel whose bounded wait ran out; lgbm_b200_experts_errors reads and clears it.
@@ -306,11 +316,14 @@ __device__ __forceinline__ void tile_of(int t, int mt, int nt, int band, int& m,
 // multiplies, the others write results out.
 template <int KIND, int BN, int CTAS>
 struct Shape {
+  static constexpr bool kFused = KIND == LINEAR || KIND == GATED;
   static constexpr int kStoreWarps = KIND == WEIGHT_F32 ? 16 : 8;
   static constexpr int kRun = KIND == WEIGHT_F32 ? 768 : 4096;  // see "Precision" above
   static constexpr int kThreads = 64 + 32 * kStoreWarps;
-  static constexpr int kStoreBytes = kStoreWarps * 32 * kStoreRow;
+  static constexpr int kBlocks = kFused ? 2 : 1;  // staging blocks of a storing warp
+  static constexpr int kStoreBytes = kBlocks * kStoreWarps * 32 * kStoreRow;
   static constexpr int kRows = kTileM * CTAS;
+  static constexpr int kOutCols = KIND == GATED ? BN / 2 : BN;  // columns of the result
   static constexpr int kCols = BN / CTAS;  // columns of B that a CTA loads
   static constexpr int kStageBytes = (kTileM + kCols) * 128;
   static constexpr int kStages = (212992 - kStoreBytes) / kStageBytes;  // 3 to 8
@@ -368,16 +381,74 @@ __device__ __forceinline__ void store_rows(uint32_t stage, char* dst, int64_t pi
   }
 }
 
+// The way back: a 32-row block of `src` to a staging block, all loads first.
+template <int UNIT>
+__device__ __forceinline__ void load_rows(uint32_t stage, const char* src, int64_t pitch,
+                                          int nrows, int bytes, int lane) {
+  constexpr int kLanes = kStoreRow / UNIT;  // of a row
+  constexpr int kPerStep = 32 / kLanes;     // rows
+  constexpr int kSteps = 32 / kPerStep;
+  using T = std::conditional_t<
+      UNIT == 16, uint4,
+      std::conditional_t<UNIT == 8, uint2, std::conditional_t<UNIT == 4, uint32_t, uint16_t>>>;
+  const int at = lane % kLanes * UNIT;
+  if (at + UNIT > bytes) return;
+  const char* from = src + (lane / kLanes) * pitch + at;
+  T v[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i)
+    if (i * kPerStep + lane / kLanes < nrows)
+      v[i] = __ldg(reinterpret_cast<const T*>(from + i * kPerStep * pitch));
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int row = i * kPerStep + lane / kLanes;
+    const uint32_t to = stage + staged(row, at >> 4) + (at & 15);
+    if (row < nrows) {
+      if constexpr (UNIT == 16)
+        store_piece(to, v[i].x, v[i].y, v[i].z, v[i].w);
+      else if constexpr (UNIT == 8)
+        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(v[i].x), "r"(v[i].y)
+                     : "memory");
+      else if constexpr (UNIT == 4)
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(v[i]) : "memory");
+      else
+        asm volatile("st.shared.b16 [%0], %1;" ::"r"(to), "h"(v[i]) : "memory");
+    }
+  }
+}
+
+// Two 16-bit values of a word as f32, by the type of `kind`.
+__device__ __forceinline__ float2 unpack2(uint32_t w, bool bf16) {
+  if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ void pack32(const float (&f)[32], bool bf16, uint32_t (&w)[16]) {
+  if (bf16) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      w[i] = pack2<true>(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      w[i] = pack2<false>(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]));
+  }
+}
+
 struct Maps {
   CUtensorMap a, b;  // tiles of 64 columns
   CUtensorMap out;   // 32 rows of 64 bytes
 };
+struct FusedMaps : Maps {
+  CUtensorMap pre;   // 32 rows of 64 bytes of a half
+};
+template <int KIND>
+using MapsOf = std::conditional_t<KIND == LINEAR || KIND == GATED, FusedMaps, Maps>;
 
 template <int KIND, int BN, int CTAS>
 __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
-    k_grouped_matmul(const __grid_constant__ Maps maps, const MatArgs g) {
+    k_grouped_matmul(const __grid_constant__ MapsOf<KIND> maps, const MatArgs g) {
   using S = Shape<KIND, BN, CTAS>;
-  constexpr int MODE = KIND == WEIGHT_F32 ? (int)WEIGHT : KIND;
+  constexpr int MODE = KIND == WEIGHT_F32 ? (int)WEIGHT : S::kFused ? (int)FORWARD : KIND;
   constexpr int kLead = MODE == WEIGHT ? 0 : 1;  // groups before the first expert's
   constexpr bool kWide = KIND == WEIGHT_F32;  // results of 32 bits
   constexpr int kRun = S::kRun;
@@ -436,7 +507,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     // The groups' rows, clamped (off[i] to off[i + 1]; overlaps of offsets that decrease are
     // cut off), and the first tile of every group. The rows before the first offset are a group
     // of their own and so are those past the last; WEIGHT needs neither.
-    const int nt = (g.cols + BN - 1) / BN;
+    const int nt = (g.cols + S::kOutCols - 1) / S::kOutCols;
     int32_t carry = 0, reach = 0;
     const int experts = MODE == WEIGHT ? g.experts / g.parts : g.experts;
     for (int i0 = 0; i0 <= experts; i0 += 32) {
@@ -490,7 +561,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   const int tiles = cum[groups];
-  const int nt = (g.cols + BN - 1) / BN;
+  const int nt = (g.cols + S::kOutCols - 1) / S::kOutCols;
   const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   auto decode = [&](int t) {
@@ -505,7 +576,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     int m, n;
     const int drows = MODE == WEIGHT ? g.drows : e - b;
     tile_of(t - cum[lo], (drows + S::kRows - 1) / S::kRows, nt, S::kBand, m, n);
-    r.n0 = n * BN;
+    r.n0 = n * S::kOutCols;
     r.m0 = m * S::kRows + rank * kTileM;
     if (MODE == WEIGHT) {
       // Every group has the same tiles, the last row tile perhaps nearly empty: rotated by
@@ -541,7 +612,8 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     uint32_t it = 0, ends = 0;
     for (int t = first; ok && t < tiles; t += step) {
       const Tile r = decode(t);
-      const int nb = r.n0 + rank * S::kCols;  // first column of this CTA's share of B
+      // first column of this CTA's share of B; GATED: a pair's halves are gate and up
+      const int nb = r.n0 + rank * (KIND == GATED ? g.cols : S::kCols);
       for (int k0 = 0; k0 < r.red; k0 += kTileK, ++it) {
         const uint32_t s = it % kStages;
         if (it >= kStages && !(ok = bar_wait(empty + 8 * s, (it / kStages - 1) & 1))) break;
@@ -568,6 +640,8 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
             tma_load_2d<CTAS>(a, &maps.a, k0, r.m0, bar);
             if (MODE == FORWARD) {
               tma_load_3d<CTAS>(b, &maps.b, k0, nb, r.expert, bar);
+              if (KIND == GATED && CTAS == 1)  // one CTA loads both
+                tma_load_3d<CTAS>(b + BN / 2 * 128, &maps.b, k0, g.cols + nb, r.expert, bar);
             } else {
 #pragma unroll
               for (int j = 0; j < S::kCols / 64; ++j)
@@ -646,7 +720,8 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
   } else {
     const int quarter = warp & 3, part = (warp - 2) >> 2;  // of the lanes; of the chunks
     constexpr int kParts = S::kStoreWarps / 4;
-    const uint32_t stage = store_base + (warp - 2) * 32 * kStoreRow;
+    const uint32_t stage = store_base + (warp - 2) * S::kBlocks * 32 * kStoreRow;
+    uint32_t turn = 0;  // the staging block used last, where there are two
     constexpr int bytes = kWide ? 4 : 2;
     constexpr int per_chunk = kStoreRow / bytes;  // columns of a staging row
     const int64_t pitch = g.out_pitch * bytes;
@@ -663,9 +738,185 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
       const uint32_t bar = acc_empty + 8 * acc;
       if (lane == 0) bar_arrive_cluster(CTAS == 2 ? leader_addr(bar) : bar);
     };
+    // Each later run of a tile is added to the first one's half (at `from`), where the sum
+    // leaves from. A warp adds the columns that it stores.
+    auto add_runs = [&](const Tile& r, uint32_t from) {
+      for (int k0 = kRun; k0 < r.red; k0 += kRun) {
+        uint32_t other;
+        if (!accumulated(k0 / kRun, other)) return false;
+        constexpr int kHalves = BN / S::kOutCols;  // GATED: a column of gate and one of up
+#pragma unroll 1
+        for (int c0 = part * per_chunk; c0 < S::kOutCols; c0 += kParts * per_chunk)
+#pragma unroll 1
+          for (int i = 0; i < per_chunk * kHalves; i += 16) {
+            const int c = c0 + i + (i < per_chunk ? 0 : S::kOutCols - per_chunk);
+            uint32_t sum[16], v[16];
+            tmem_load16(from + c, sum);
+            tmem_load16(tmem + other * BN + lanes + c, v);
+            tmem_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              sum[j] = __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(v[j]));
+            tmem_store16(from + c, sum);
+          }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        release(other);
+      }
+      return true;
+    };
     for (int t = first; ok && t < tiles; t += step) {
       const Tile r = decode(t);
       const int row0 = r.m0 + quarter * 32;
+      if constexpr (S::kFused) {
+        const int ncols = min(S::kOutCols, g.cols - r.n0), nrows = min(32, r.m_end - row0);
+        const bool whole = nrows == 32, live = r.red > 0, bf16 = g.out_kind == LGBM_B200_DTYPE_BF16;
+        // the block that the store before the last one has read
+        auto block = [&] {
+          turn ^= 1;
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          __syncwarp();
+          return stage + turn * 32 * kStoreRow;
+        };
+        // this lane's row of 32 columns, through block `at`, to the result or the saved values
+        auto leave = [&](uint32_t at, const uint32_t (&w)[16], int c0, int saved) {
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+            store_piece(at + staged(lane, p), w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
+          if (whole && (saved >= 0 || g.unit == 16)) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              if (saved >= 0)
+                asm volatile(
+                    "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], "
+                    "[%4];" ::"l"(&maps.pre),
+                    "r"(r.n0 + c0), "r"(row0), "r"(saved), "r"(at)
+                    : "memory");
+              else
+                asm volatile(
+                    "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], "
+                    "[%3];" ::"l"(&maps.out),
+                    "r"(r.n0 + c0), "r"(row0), "r"(at)
+                    : "memory");
+            }
+          } else {
+            __syncwarp();
+            const int n = min(32, ncols - c0) * 2;
+            if (saved >= 0) {
+              constexpr int kHalves = KIND == GATED ? 2 : 1;
+              store_rows<16>(at,
+                             static_cast<char*>(g.pre) +
+                                 (((int64_t)row0 * kHalves + saved) * g.pre_pitch + r.n0 + c0) * 2,
+                             g.pre_pitch * kHalves * 2, nrows, (n + 15) / 16 * 16, lane);
+            } else {
+              char* dst = static_cast<char*>(g.out) + (int64_t)row0 * pitch + (int64_t)(r.n0 + c0) * 2;
+              if (g.unit == 16) store_rows<16>(at, dst, pitch, nrows, n, lane);
+              else if (g.unit == 8) store_rows<8>(at, dst, pitch, nrows, n, lane);
+              else if (g.unit == 4) store_rows<4>(at, dst, pitch, nrows, n, lane);
+              else store_rows<2>(at, dst, pitch, nrows, n, lane);
+            }
+          }
+          // a group for every block, empty without a bulk store: block() counts them
+          if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        };
+        uint32_t acc = 0;
+        if (live && !(ok = accumulated(0, acc))) break;
+        const uint32_t from = tmem + acc * BN + lanes;
+        if (!(ok = add_runs(r, from))) break;
+        for (int c0 = part * 32; c0 < ncols && nrows > 0; c0 += kParts * 32) {
+          uint32_t w[16];
+          float f[32], up[KIND == GATED ? 32 : 1];
+          if (live) {
+            uint32_t v[32];
+            tmem_load32(from + c0, v);
+            if constexpr (KIND == GATED) {
+              uint32_t u[32];
+              tmem_load32(from + S::kOutCols + c0, u);
+              tmem_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) up[i] = __uint_as_float(u[i]);
+            }
+            tmem_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+            if (KIND == LINEAR && g.bias) {
+              const uint16_t* bias = static_cast<const uint16_t*>(g.bias) +
+                                     (int64_t)r.expert * g.cols + r.n0 + c0;
+              const int n = ncols - c0;
+              if (g.bias_vec) {
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                  uint4 q = make_uint4(0, 0, 0, 0);
+                  if (8 * p < n) q = __ldg(reinterpret_cast<const uint4*>(bias) + p);
+                  w[4 * p] = q.x, w[4 * p + 1] = q.y, w[4 * p + 2] = q.z, w[4 * p + 3] = q.w;
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  w[i] = 2 * i < n ? __ldg(bias + 2 * i) : 0;
+                  if (2 * i + 1 < n) w[i] |= (uint32_t)__ldg(bias + 2 * i + 1) << 16;
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 b = unpack2(w[i], bf16);
+                f[2 * i] += b.x;
+                f[2 * i + 1] += b.y;
+              }
+            }
+          } else {  // rows of no expert
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+            if constexpr (KIND == GATED) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) up[i] = 0.0f;
+            }
+          }
+          if (g.pre) {
+            pack32(f, bf16, w);
+            leave(block(), w, c0, 0);
+            if constexpr (KIND == GATED) {
+              pack32(up, bf16, w);
+              leave(block(), w, c0, 1);
+            }
+          }
+          activate(g.act, f);
+          if constexpr (KIND == GATED) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] *= up[i];
+          }
+          const uint32_t at = block();
+          if (KIND == LINEAR && g.residual) {
+            const int n = min(32, ncols - c0) * 2;
+            const int64_t rp = g.residual_pitch * 2;
+            const char* src = static_cast<const char*>(g.residual) + (int64_t)row0 * rp +
+                              (int64_t)(r.n0 + c0) * 2;
+            if (g.residual_unit == 16) load_rows<16>(at, src, rp, nrows, n, lane);
+            else if (g.residual_unit == 8) load_rows<8>(at, src, rp, nrows, n, lane);
+            else if (g.residual_unit == 4) load_rows<4>(at, src, rp, nrows, n, lane);
+            else load_rows<2>(at, src, rp, nrows, n, lane);
+            __syncwarp();
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {  // this lane's own row, which leave() overwrites
+              uint32_t q[4];
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
+                           : "r"(at + staged(lane, p))
+                           : "memory");
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 b = unpack2(q[j], bf16);
+                f[8 * p + 2 * j] += b.x;
+                f[8 * p + 2 * j + 1] += b.y;
+              }
+            }
+          }
+          pack32(f, bf16, w);
+          leave(at, w, c0, -1);
+        }
+        if (live) release(acc);
+        continue;
+      }
       char* out = static_cast<char*>(g.out);
       int out_row = row0;  // of D as one matrix
       if (MODE == WEIGHT) {
@@ -737,27 +988,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
         if (r.red > 0 && !(ok = accumulated(0, acc))) break;
         const uint32_t from = tmem + acc * BN + lanes;
         if constexpr (!kWide) {
-          // each later run is added to the first one's half, where the sum leaves from
-          for (int k0 = kRun; k0 < r.red; k0 += kRun) {
-            uint32_t other;
-            if (!(ok = accumulated(k0 / kRun, other))) break;
-#pragma unroll 1
-            for (int c0 = part * per_chunk; c0 < BN; c0 += kParts * per_chunk)
-#pragma unroll 1
-              for (int c = c0; c < c0 + per_chunk; c += 16) {
-                uint32_t sum[16], v[16];
-                tmem_load16(from + c, sum);
-                tmem_load16(tmem + other * BN + lanes + c, v);
-                tmem_wait();
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  sum[j] = __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(v[j]));
-                tmem_store16(from + c, sum);
-              }
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            release(other);
-          }
-          if (!ok) break;
+          if (!(ok = add_runs(r, from))) break;
         }
         for (int c0 = part * per_chunk; c0 < ncols && nrows > 0; c0 += kParts * per_chunk) {
           uint32_t v[32], w[16];
@@ -947,7 +1178,7 @@ struct DeviceInfo {
 DeviceInfo g_devices[kMaxDevices];
 
 template <int KIND, int BN, int CTAS>
-cudaError_t launch_tiles(const Maps& maps, MatArgs g, int64_t most_tiles, cudaStream_t st) {
+cudaError_t launch_tiles(const MapsOf<KIND>& maps, MatArgs g, int64_t most_tiles, cudaStream_t st) {
   using S = Shape<KIND, BN, CTAS>;
   static std::atomic<int> most_ready[kMaxDevices];  // tiles at work at a time; 0: not set up
   int dev = 0;
@@ -1094,6 +1325,52 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
               : go(std::integral_constant<int, 256>(), One());
 }
 
+// The forward product with its epilogue; g.cols columns of the result.
+template <int KIND>
+cudaError_t run_fused(const Operand& x, const Operand& w, const MatmulCall& c, MatArgs g,
+                      cudaStream_t st) {
+  const Epilogue& e = c.epilogue;
+  constexpr int kHalves = KIND == GATED ? 2 : 1;
+  const auto unit = [&](const void* p, int64_t pitch) {
+    const uintptr_t bits =
+        reinterpret_cast<uintptr_t>(p) | (uintptr_t)(pitch * 2) | (uintptr_t)(g.cols * 2);
+    return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
+  };
+  g.unit = unit(g.out, g.out_pitch);
+  g.act = e.act;
+  g.bias = e.bias;
+  g.bias_vec = aligned16(e.bias) && g.cols % 8 == 0;
+  g.residual = e.residual;
+  g.residual_pitch = e.residual_pitch;
+  g.residual_unit = unit(e.residual, e.residual_pitch);
+  g.pre = e.pre;
+  g.pre_pitch = pre_pitch(g.cols);
+  auto go = [&](auto bn_c, auto ctas_c) -> cudaError_t {
+    constexpr int BN = decltype(bn_c)::value, CTAS = decltype(ctas_c)::value;
+    using S = Shape<KIND, BN, CTAS>;
+    FusedMaps maps;
+    const int64_t da[3] = {c.inner, g.rows, 1}, pa[2] = {x.pitch, 0};
+    const int64_t db[3] = {c.inner, c.outer, c.experts}, pb[2] = {w.pitch, w.pitch * c.outer};
+    bool fine = encode(&maps.a, c.dtype, x.p, 2, da, pa, kTileM) &&
+                encode(&maps.b, c.dtype, w.p, 3, db, pb, KIND == GATED ? BN / 2 : S::kCols);
+    maps.out = maps.pre = maps.a;  // not used unless set
+    const int64_t dd[3] = {g.cols, g.rows, kHalves}, pd[2] = {g.out_pitch, 0};
+    if (g.unit == 16) fine = fine && encode(&maps.out, c.dtype, g.out, 2, dd, pd, 32, kStoreRow);
+    const int64_t pp[2] = {g.pre_pitch * kHalves, g.pre_pitch};
+    if (g.pre) fine = fine && encode(&maps.pre, c.dtype, g.pre, 3, dd, pp, 32, kStoreRow);
+    if (!fine) return cudaErrorInvalidValue;
+    g.idesc = instruction(c.dtype, false, false, S::kRows, BN);
+    const int64_t nt = (g.cols + S::kOutCols - 1) / S::kOutCols;
+    return launch_tiles<KIND, BN, CTAS>(maps, g, (g.rows / S::kRows + g.experts + 2) * nt, st);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (g.cols * kHalves <= 64) return go(std::integral_constant<int, 64>(), One());
+  if (g.cols * kHalves <= 128) return go(std::integral_constant<int, 128>(), One());
+  return g.rows >= (int64_t)kTileM * g.experts ? go(std::integral_constant<int, 256>(), Two())
+                                               : go(std::integral_constant<int, 256>(), One());
+}
+
 // Sums of the parts of a weight gradient, always in the same order: part[e][p][n] to out[e][n],
 // n in [0, count). V elements a thread.
 template <typename T, int V>
@@ -1209,6 +1486,7 @@ cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st)
     f.inner = c.inner;
     f.outer = c.outer;
     f.y = c.y;
+    f.epilogue = c.epilogue;
     return launch_few(f, st);
   }
   char* ws = static_cast<char*>(workspace);
@@ -1228,10 +1506,11 @@ cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st)
   if (err == cudaSuccess && c.y) {
     g.out = c.y;
     g.out_kind = c.dtype;
-    g.cols = c.outer;
+    g.cols = g.out_pitch = c.epilogue.gated ? c.outer / 2 : c.outer;
     g.reduction = c.inner;
-    g.out_pitch = c.outer;
-    err = run_tiles<FORWARD>(x, c.inner, w, c.inner, c.dtype, g, st);
+    if (!c.epilogue.on) err = run_tiles<FORWARD>(x, c.inner, w, c.inner, c.dtype, g, st);
+    else if (c.epilogue.gated) err = run_fused<GATED>(x, w, c, g, st);
+    else err = run_fused<LINEAR>(x, w, c, g, st);
   }
   if (err == cudaSuccess && c.dx) {
     g.out = c.dx;

@@ -14,6 +14,7 @@
 
 #include <sstream>
 #include <string>
+#include <vector>
 
 #include "lgbm_b200.h"
 
@@ -318,6 +319,172 @@ PyObject* grouped_matmul_backward(PyObject* const* a) {
   return wrap_all(dx, dw);
 }
 
+// What a layer keeps for its gradient: [rows, width], gated [rows, 2, width], each row padded to
+// 16 bytes.
+int64_t saved_pitch(int64_t width) { return (width + 7) / 8 * 8; }
+
+Tensor make_saved(c10::Device dev, at::ScalarType type, int64_t rows, bool gated, int64_t width) {
+  const int64_t ld = saved_pitch(width);
+  Tensor t = gated ? make(dev, type, {rows, 2, ld}) : make(dev, type, {rows, ld});
+  return ld == width ? t : t.narrow(gated ? 2 : 1, 0, width);
+}
+
+// `o` as the kernels read it: as make_saved made it, or copied to that layout.
+Tensor saved(const char* what, PyObject* o, const Matrix& like, int64_t rows, bool gated,
+             int64_t width) {
+  Tensor t = tensor(what, o);
+  const std::vector<int64_t> shape =
+      gated ? std::vector<int64_t>{rows, 2, width} : std::vector<int64_t>{rows, width};
+  if (t.scalar_type() != like.t.scalar_type() || t.device() != like.t.device() ||
+      t.sizes() != at::IntArrayRef(shape))
+    refuse(LGBM_B200_INVALID_ARGUMENT, what, ": pre: want ", at::IntArrayRef(shape), " ",
+           like.t.scalar_type(), " on ", like.t.device(), ", got ", describe(t));
+  const int64_t ld = saved_pitch(width), halves = gated ? 2 : 1, last = t.dim() - 1;
+  const bool fits =
+      (width == 1 || t.stride(last) == 1) && (!gated || t.stride(1) == ld) &&
+      (rows < 2 || t.stride(0) == halves * ld) &&
+      (rows == 0 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) &&
+      // the padding of the last row is read too
+      (t.storage_offset() + rows * halves * ld) * 2 <= (int64_t)t.storage().nbytes();
+  if (fits) return t;
+  Tensor copy = make_saved(t.device(), t.scalar_type(), rows, gated, width);
+  copy.copy_(t);
+  return copy;
+}
+
+int activation(const char* what, PyObject* o) {
+  const int64_t v = whole(o);
+  if (v < 0 || v > INT32_MAX) refuse(LGBM_B200_INVALID_ARGUMENT, what, ": activation ", v);
+  return (int)v;
+}
+
+// grouped_linear(x, w, offsets, rows, bias, activation, residual, save) -> (y, pre)
+PyObject* grouped_linear(PyObject* const* a) {
+  const char* what = "grouped_linear";
+  const Product p = product(what, a[0], a[1], a[2], a[3], true, true);
+  const auto dev = p.x.t.device();
+  const auto type = p.x.t.scalar_type();
+  const int act = activation(what, a[5]);
+  Tensor bias;
+  if (a[4] != Py_None)
+    bias = same("grouped_linear: bias", tensor(what, a[4]), dev, type, {p.experts, p.outer});
+  Matrix residual;
+  if (a[6] != Py_None) {
+    residual = matrix(what, tensor(what, a[6]), true);
+    if (residual.dtype != p.x.dtype || residual.t.device() != dev)
+      refuse(LGBM_B200_INVALID_ARGUMENT, what, ": residual ", describe(residual.t), ", x ",
+             describe(p.x.t));
+    if (residual.rows != p.rows || residual.width != p.outer)
+      refuse(LGBM_B200_LENGTH_MISMATCH, what, ": residual ", describe(residual.t), ", want [",
+             p.rows, ", ", p.outer, "]");
+  }
+  On on(dev);
+  Tensor y = make(dev, type, {p.rows, p.outer}), pre;
+  if (flag(a[7]) && act != LGBM_B200_ACT_NONE)
+    pre = make_saved(dev, type, p.rows, false, p.outer);
+  Scratch ws(dev, lgbm_b200_experts_matmul_workspace(
+                      p.x.p(), p.x.pitch, p.ip(), p.w.data_ptr(), p.rows, (int32_t)p.experts,
+                      (int32_t)p.inner, (int32_t)p.outer));
+  check(lgbm_b200_experts_linear(
+      p.x.p(), p.x.rows, p.x.pitch, p.ip(), p.w.data_ptr(),
+      bias.defined() ? bias.data_ptr() : nullptr, residual.t.defined() ? residual.p() : nullptr,
+      residual.t.defined() ? residual.pitch : 0, p.offsets.data_ptr<int32_t>(), p.x.dtype, act,
+      p.rows, (int32_t)p.experts, (int32_t)p.inner, (int32_t)p.outer, y.data_ptr(),
+      pre.defined() ? pre.data_ptr() : nullptr, ws.p(), ws.bytes, on.stream));
+  return wrap_all(y, pre);
+}
+
+// The hidden width of a gated layer's w [experts, 2 hidden, inner].
+int64_t hidden_of(const char* what, const Product& p) {
+  if (p.outer % 2 != 0)
+    refuse(LGBM_B200_LENGTH_MISMATCH, what, ": w ", describe(p.w), ": want gate and up, 2 hidden");
+  return p.outer / 2;
+}
+
+// grouped_gated(x, w, offsets, rows, activation, save) -> (h, pre)
+PyObject* grouped_gated(PyObject* const* a) {
+  const char* what = "grouped_gated";
+  const Product p = product(what, a[0], a[1], a[2], a[3], true, true);
+  const int64_t hidden = hidden_of(what, p);
+  const auto dev = p.x.t.device();
+  const auto type = p.x.t.scalar_type();
+  const int act = activation(what, a[4]);
+  On on(dev);
+  Tensor h = make(dev, type, {p.rows, hidden}), pre;
+  if (flag(a[5])) pre = make_saved(dev, type, p.rows, true, hidden);
+  Scratch ws(dev, lgbm_b200_experts_matmul_workspace(
+                      p.x.p(), p.x.pitch, p.ip(), p.w.data_ptr(), p.rows, (int32_t)p.experts,
+                      (int32_t)p.inner, (int32_t)p.outer));
+  check(lgbm_b200_experts_gated(p.x.p(), p.x.rows, p.x.pitch, p.ip(), p.w.data_ptr(),
+                                p.offsets.data_ptr<int32_t>(), p.x.dtype, act, p.rows,
+                                (int32_t)p.experts, (int32_t)p.inner, (int32_t)hidden,
+                                h.data_ptr(), pre.defined() ? pre.data_ptr() : nullptr, ws.p(),
+                                ws.bytes, on.stream));
+  return wrap_all(h, pre);
+}
+
+// grouped_linear_backward(dy, pre, x, w, offsets, rows, activation, wide, need_dx, need_dw,
+//                         need_dbias) -> (dx, dw, dbias)
+// grouped_gated_backward(dh, pre, x, w, offsets, rows, activation, wide, need_dx, need_dw)
+//                        -> (dx, dw)
+PyObject* layer_backward(const char* what, PyObject* const* a, bool gated) {
+  const bool need_dx = flag(a[8]), need_dw = flag(a[9]), need_dbias = !gated && flag(a[10]);
+  const Product p = product(what, a[2], a[3], a[4], a[5], need_dw, need_dx);
+  const int64_t width = gated ? hidden_of(what, p) : p.outer;
+  const int act = activation(what, a[6]);
+  const Matrix dy = matrix(what, tensor(what, a[0]), true);
+  const auto dev = p.x.t.device();
+  const auto type = p.x.t.scalar_type();
+  if (dy.dtype != p.x.dtype || dy.t.device() != dev)
+    refuse(LGBM_B200_INVALID_ARGUMENT, what, ": gradient ", describe(dy.t), ", x ",
+           describe(p.x.t));
+  if (dy.rows != p.rows || dy.width != width)
+    refuse(LGBM_B200_LENGTH_MISMATCH, what, ": gradient ", describe(dy.t), ", want [", p.rows,
+           ", ", width, "]");
+  On on(dev);
+  Tensor pre;
+  if (gated || act != LGBM_B200_ACT_NONE)
+    pre = saved(what, a[1], p.x, p.rows, gated, width);
+  else if (a[1] != Py_None)
+    refuse(LGBM_B200_INVALID_ARGUMENT, what, ": pre without an activation");
+  const bool wide = flag(a[7]);
+  const int32_t experts = (int32_t)p.experts, inner = (int32_t)p.inner, outer = (int32_t)p.outer;
+  const auto grad = wide ? at::kFloat : type;
+  Tensor dx, dw, dbias;
+  if (need_dx) dx = make(dev, type, {p.rows, p.inner});
+  if (need_dw) dw = make(dev, grad, {p.experts, p.outer, p.inner});
+  if (need_dbias) dbias = make(dev, grad, {p.experts, p.outer});
+  if (dx.defined() || dw.defined() || dbias.defined()) {
+    auto out = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    const int dtype = p.x.dtype, grad_dtype = wide ? LGBM_B200_DTYPE_F32 : dtype;
+    const int32_t* offsets = p.offsets.data_ptr<int32_t>();
+    if (gated) {
+      Scratch ws(dev, lgbm_b200_experts_gated_backward_workspace(
+                          p.x.p(), p.x.pitch, p.ip(), p.w.data_ptr(), p.rows, experts, inner,
+                          (int32_t)width, need_dx, need_dw));
+      check(lgbm_b200_experts_gated_backward(
+          dy.p(), dy.pitch, out(pre), p.x.p(), p.x.rows, p.x.pitch, p.ip(), p.w.data_ptr(),
+          offsets, dtype, grad_dtype, act, p.rows, experts, inner, (int32_t)width, out(dx),
+          out(dw), ws.p(), ws.bytes, on.stream));
+    } else {
+      Scratch ws(dev, lgbm_b200_experts_linear_backward_workspace(
+                          dy.p(), dy.pitch, p.x.p(), p.x.pitch, p.ip(), p.w.data_ptr(), act,
+                          p.rows, experts, inner, outer, need_dx, need_dw, need_dbias));
+      check(lgbm_b200_experts_linear_backward(
+          dy.p(), dy.pitch, out(pre), p.x.p(), p.x.rows, p.x.pitch, p.ip(), p.w.data_ptr(),
+          offsets, dtype, grad_dtype, act, p.rows, experts, inner, outer, out(dx), out(dw),
+          out(dbias), ws.p(), ws.bytes, on.stream));
+    }
+  }
+  return gated ? wrap_all(dx, dw) : wrap_all(dx, dw, dbias);
+}
+PyObject* grouped_linear_backward(PyObject* const* a) {
+  return layer_backward("grouped_linear_backward", a, false);
+}
+PyObject* grouped_gated_backward(PyObject* const* a) {
+  return layer_backward("grouped_gated_backward", a, true);
+}
+
 // grouped_matmul_w4(x, q, scales, offsets, zeros, rows, group_size) -> y
 PyObject* grouped_matmul_w4(PyObject* const* a) {
   const char* what = "grouped_matmul_w4";
@@ -493,6 +660,12 @@ PyMethodDef g_methods[] = {
     {"route_backward", (PyCFunction)(void (*)())entry<route_backward, 5>, METH_FASTCALL, nullptr},
     {"grouped_matmul", (PyCFunction)(void (*)())entry<grouped_matmul, 4>, METH_FASTCALL, nullptr},
     {"grouped_matmul_backward", (PyCFunction)(void (*)())entry<grouped_matmul_backward, 8>,
+     METH_FASTCALL, nullptr},
+    {"grouped_linear", (PyCFunction)(void (*)())entry<grouped_linear, 8>, METH_FASTCALL, nullptr},
+    {"grouped_linear_backward", (PyCFunction)(void (*)())entry<grouped_linear_backward, 11>,
+     METH_FASTCALL, nullptr},
+    {"grouped_gated", (PyCFunction)(void (*)())entry<grouped_gated, 6>, METH_FASTCALL, nullptr},
+    {"grouped_gated_backward", (PyCFunction)(void (*)())entry<grouped_gated_backward, 10>,
      METH_FASTCALL, nullptr},
     {"grouped_matmul_w4", (PyCFunction)(void (*)())entry<grouped_matmul_w4, 7>, METH_FASTCALL,
      nullptr},

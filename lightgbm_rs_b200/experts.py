@@ -87,11 +87,68 @@ def grouped_matmul_backward(dy, x, w, offsets, rows=None, grad_dtype=None, need_
     grouped rows (with `rows`, `combine(dx, position)` sums it into the tokens); dw
     [E, outer, inner] has type `grad_dtype`: the weights' (default) or float32. One that is
     not needed is None."""
+    wide = _wide("grouped_matmul_backward", grad_dtype, w)
+    return _X.grouped_matmul_backward(dy, x, w, offsets, rows, wide, need_dx, need_dw)
+
+
+_ACTS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def _act(what, name):
+    if name not in _ACTS:
+        raise C.LightGBMError(C.INVALID_ARGUMENT, f"{what}: activation {name!r} is none of {_ACTS}")
+    return _ACTS[name]
+
+
+def _wide(what, grad_dtype, w):
     wide = grad_dtype is torch.float32
     if grad_dtype is not None and not wide and grad_dtype is not w.dtype:
-        raise C.LightGBMError(C.INVALID_ARGUMENT,
-                              f"grouped_matmul_backward: grad_dtype {grad_dtype}")
-    return _X.grouped_matmul_backward(dy, x, w, offsets, rows, wide, need_dx, need_dw)
+        raise C.LightGBMError(C.INVALID_ARGUMENT, f"{what}: grad_dtype {grad_dtype}")
+    return wide
+
+
+def grouped_linear(x, w, offsets, rows=None, bias=None, activation=None, residual=None,
+                   save=False):
+    """act(w[e] x[rows[r]] + bias[e]) + residual[r] for the grouped rows r of expert e, in one
+    pass: x, w, offsets and rows as for `grouped_matmul`, bias [E, outer], residual [M, outer] of
+    their type. activation: None, "relu", "silu" or "gelu" (by the normal distribution function).
+    Rows of no expert are the residual (0 without one). With save, (y, pre) for
+    `grouped_linear_backward`: pre [M, outer] is what the activation was given, rounded to x's
+    type, its rows padded to 16 bytes (None without an activation)."""
+    y, pre = _X.grouped_linear(x, w, offsets, rows, bias, _act("grouped_linear", activation),
+                               residual, save)
+    return (y, pre) if save else y
+
+
+def grouped_linear_backward(dy, pre, x, w, offsets, rows=None, activation=None, grad_dtype=None,
+                            need_dx=True, need_dw=True, need_dbias=True):
+    """Gradients of `grouped_linear`: (dx, dw, dbias) from dy [M, outer], with dx and dw as of
+    `grouped_matmul_backward` and dbias [E, outer] of type `grad_dtype`; pre is what the call with
+    save returned. The residual's gradient is dy. dx and dw are products of dy act'(pre) rounded
+    to 16 bits: dw in float32 holds the sum of those without another rounding. One that is not
+    needed is None."""
+    what = "grouped_linear_backward"
+    return _X.grouped_linear_backward(dy, pre, x, w, offsets, rows, _act(what, activation),
+                                      _wide(what, grad_dtype, w), need_dx, need_dw, need_dbias)
+
+
+def grouped_gated(x, w, offsets, rows=None, activation="silu", save=False):
+    """act(gate) * up for the grouped rows, [M, hidden], in one pass: gate and up are the first
+    and the last `hidden` columns of `grouped_matmul` with w [E, 2 * hidden, inner]; activation as
+    for `grouped_linear`. Rows of no expert are 0. With save, (h, pre) for
+    `grouped_gated_backward`: pre [M, 2, hidden] is gate and up rounded to x's type, its rows
+    padded to 16 bytes."""
+    h, pre = _X.grouped_gated(x, w, offsets, rows, _act("grouped_gated", activation), save)
+    return (h, pre) if save else h
+
+
+def grouped_gated_backward(dh, pre, x, w, offsets, rows=None, activation="silu", grad_dtype=None,
+                           need_dx=True, need_dw=True):
+    """Gradients of `grouped_gated`: (dx, dw) from dh [M, hidden] and what the call with save
+    returned, as of `grouped_linear_backward`; dw [E, 2 * hidden, inner]."""
+    what = "grouped_gated_backward"
+    return _X.grouped_gated_backward(dh, pre, x, w, offsets, rows, _act(what, activation),
+                                     _wide(what, grad_dtype, w), need_dx, need_dw)
 
 
 def grouped_matmul_w4(x, q, scales, offsets, zeros=None, rows=None, group_size=128):
