@@ -706,6 +706,28 @@ int lgbm_b200_experts_dropout(const void* x, const void* residual, int32_t dtype
                               int64_t width, int64_t pitch, int64_t residual_pitch, double p,
                               uint64_t seed, uint64_t offset, void* out, void* stream);
 
+/* A step's gradients: *norm (f32, on the device) = sqrt of the sum of the squares of all elements
+ * of all tensors, summed so that it is right wherever f32 can hold it. clip_grads also writes
+ * out = in * min(1, max_norm / norm), rounded once: in place where out == in (then left alone when
+ * the factor is 1), else to other memory that overlaps no tensor read or written. A norm of 0 has
+ * the factor 1. Where the norm is infinite the factor is 0, and where it is NaN all results are.
+ * `tensors` is an array of the HOST, read before the call returns; in and out are contiguous
+ * arrays on the current device. The order of the tensors is the order of the sum. */
+typedef struct lgbm_b200_experts_tensor {
+  const void* in;
+  void* out;       /* clip_grads only */
+  int64_t count;   /* elements, may be 0 */
+  int32_t dtype;   /* LGBM_B200_DTYPE_* */
+  int32_t reserved;
+} lgbm_b200_experts_tensor;
+int64_t lgbm_b200_experts_norm_workspace(int64_t tensors);
+int lgbm_b200_experts_grad_norm(const lgbm_b200_experts_tensor* tensors, int64_t count,
+                                float* norm, void* workspace, int64_t workspace_bytes,
+                                void* stream);
+int lgbm_b200_experts_clip_grads(const lgbm_b200_experts_tensor* tensors, int64_t count,
+                                 double max_norm, float* norm, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

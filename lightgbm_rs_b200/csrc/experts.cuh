@@ -199,6 +199,18 @@ struct LinearGrad {
 int64_t linear_grad_workspace(int64_t rows, int32_t experts, int32_t outer);
 cudaError_t launch_linear_grad(const LinearGrad& c, cudaStream_t st);
 
+// experts_norm.cu
+struct NormCall {
+  const lgbm_b200_experts_tensor* tensors;  // of the host
+  int64_t count;
+  bool scale;
+  double max_norm;
+  double* partial;
+  float* norm;
+};
+int64_t norm_workspace(int64_t tensors);
+cudaError_t launch_norm(const NormCall& c, cudaStream_t st);
+
 // experts_few.cu
 struct FewCall {
   int32_t dtype;

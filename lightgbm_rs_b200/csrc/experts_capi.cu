@@ -267,6 +267,44 @@ int64_t layer_backward_workspace(const void* dy, int64_t dy_pitch, const void* x
   return c.dx || c.dw ? need + matmul_workspace(c) : need;
 }
 
+constexpr int64_t kMaxNormBytes = 1ll << 44;  // of all tensors: their windows are counted in 32 bits
+
+int run_norm(const char* what, const lgbm_b200_experts_tensor* tensors, int64_t count, bool scale,
+             double max_norm, float* norm, void* workspace, int64_t workspace_bytes,
+             void* stream) {
+  if (count < 0 || (count > 0 && !tensors) || !norm)
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: %lld tensors, or a null argument", what,
+                  (long long)count);
+  if (count > (1 << 24))
+    return refuse(LGBM_B200_CAPABILITY_UNAVAILABLE, "%s: %lld tensors (at most %d)", what,
+                  (long long)count, 1 << 24);
+  if (scale && !(max_norm >= 0.0))
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: max_norm %g", what, max_norm);
+  if (int rc = check_starts(what, {{norm, 4}})) return rc;
+  int64_t left = kMaxNormBytes - count * 65536;  // a window of each may be nearly empty
+  for (int64_t i = 0; i < count; ++i) {
+    const lgbm_b200_experts_tensor& t = tensors[i];
+    if (!is_float(t.dtype) || t.count < 0 ||
+        (t.count > 0 && (!t.in || (scale && !t.out))))
+      return refuse(LGBM_B200_INVALID_ARGUMENT,
+                    "%s: tensor %lld: dtype %d, %lld elements, or a null argument", what,
+                    (long long)i, t.dtype, (long long)t.count);
+    const int size = elem_size(t.dtype);
+    if (t.count > left / size)
+      return refuse(LGBM_B200_CAPABILITY_UNAVAILABLE, "%s: more than %lld bytes", what,
+                    (long long)kMaxNormBytes);
+    left -= t.count * size;
+    if (t.count > 0)
+      if (int rc = check_starts(what, {{t.in, size}, {scale ? t.out : nullptr, size}})) return rc;
+  }
+  const int64_t need = norm_workspace(count);
+  if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace))))
+    return refuse(LGBM_B200_LENGTH_MISMATCH, "%s: workspace of %lld bytes, %lld are needed",
+                  what, (long long)workspace_bytes, (long long)need);
+  const NormCall c{tensors, count, scale, max_norm, static_cast<double*>(workspace), norm};
+  return launched(launch_norm(c, reinterpret_cast<cudaStream_t>(stream)), what);
+}
+
 }  // namespace
 
 extern "C" {
@@ -653,6 +691,24 @@ int lgbm_b200_experts_matmul_w4(const void* x, int64_t x_rows, int64_t x_pitch,
   FewCall f{dtype, x,      x_rows, x_pitch, index, q,     group_size, scales,
             zeros, offsets, rows,   experts, inner, outer, y};
   return launched(launch_few(f, reinterpret_cast<cudaStream_t>(stream)), what);
+}
+
+int64_t lgbm_b200_experts_norm_workspace(int64_t tensors) {
+  return tensors < 1 ? 0 : norm_workspace(tensors);
+}
+
+int lgbm_b200_experts_grad_norm(const lgbm_b200_experts_tensor* tensors, int64_t count,
+                                float* norm, void* workspace, int64_t workspace_bytes,
+                                void* stream) {
+  return run_norm("experts_grad_norm", tensors, count, false, 0.0, norm, workspace,
+                  workspace_bytes, stream);
+}
+
+int lgbm_b200_experts_clip_grads(const lgbm_b200_experts_tensor* tensors, int64_t count,
+                                 double max_norm, float* norm, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  return run_norm("experts_clip_grads", tensors, count, true, max_norm, norm, workspace,
+                  workspace_bytes, stream);
 }
 
 int lgbm_b200_experts_errors(uint32_t* bits_out) {

@@ -12,8 +12,11 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <optional>
 #include <sstream>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "lgbm_b200.h"
@@ -622,6 +625,157 @@ PyObject* dropout(PyObject* const* a) {
   return wrap(out);
 }
 
+// The tensors of a list as flat arrays. One whose memory has gaps is taken through a copy, which
+// goes back to its `target` afterwards.
+struct Flat {
+  std::vector<Tensor> kept;                        // what must live until the launch
+  std::vector<lgbm_b200_experts_tensor> items;
+  struct Back {
+    Tensor to, from;
+  };
+  std::vector<Back> back;
+};
+
+struct Range {
+  uintptr_t begin, end;
+  int64_t item;   // position in the list
+  bool written;
+};
+
+// Memory that is written overlaps nothing else but, at the same place, the tensor it is made from.
+void check_overlaps(const char* what, std::vector<Range>& r) {
+  const auto less = [](const Range& a, const Range& b) { return a.begin < b.begin; };
+  if (!std::is_sorted(r.begin(), r.end(), less)) std::sort(r.begin(), r.end(), less);
+  uintptr_t read_end = 0, write_end = 0;  // how far the ranges so far reach
+  for (const Range& v : r) {
+    if (v.begin < write_end || (v.written && v.begin < read_end))
+      refuse(LGBM_B200_INVALID_ARGUMENT, what, ": tensor ", v.item,
+             " overlaps another one's memory");
+    (v.written ? write_end : read_end) = std::max(v.written ? write_end : read_end, v.end);
+  }
+}
+
+// Whether every element has a place of its own: each axis steps over all that the axes of smaller
+// strides reach. (True for slices and permutations of such a tensor, not for expanded ones.)
+bool own_places(const Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> axes;  // stride, size
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1) axes.emplace_back(t.stride(d), t.size(d));
+  std::sort(axes.begin(), axes.end());
+  int64_t reach = 0;
+  for (const auto& [stride, size] : axes) {
+    if (stride <= reach) return false;
+    reach += (size - 1) * stride;
+  }
+  return true;
+}
+
+// clip_grads(grads, max_norm or None, out or None) -> norm
+PyObject* clip_grads(PyObject* const* a) {
+  const bool scale = a[1] != Py_None;
+  const char* what = scale ? "clip_grads" : "grad_norm";
+  double max_norm = 0.0;
+  if (scale) {
+    max_norm = PyFloat_AsDouble(a[1]);
+    if (max_norm == -1.0 && PyErr_Occurred()) throw python_error();
+  }
+  struct Held {
+    PyObject* list;
+    ~Held() { Py_XDECREF(list); }
+  };
+  const Held grads{PySequence_Fast(a[0], "a sequence of tensors is wanted")};
+  if (!grads.list) throw python_error();
+  const Held outs{a[2] == Py_None ? nullptr
+                                  : PySequence_Fast(a[2], "a sequence of tensors is wanted")};
+  if (a[2] != Py_None && !outs.list) throw python_error();
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(grads.list);
+  if (n == 0) refuse(LGBM_B200_INVALID_ARGUMENT, what, ": no tensors");
+  if (outs.list && PySequence_Fast_GET_SIZE(outs.list) != n)
+    refuse(LGBM_B200_LENGTH_MISMATCH, what, ": ", PySequence_Fast_GET_SIZE(outs.list),
+           " results for ", n, " tensors");
+  Flat f;
+  f.kept.reserve(n);
+  f.items.reserve(n);
+  std::vector<Range> ranges;
+  if (scale) ranges.reserve(outs.list ? 2 * n : n);
+  c10::Device dev(c10::kCUDA);
+  std::optional<On> on;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    Tensor g = tensor(what, PySequence_Fast_GET_ITEM(grads.list, i));
+    const int dtype = dtype_of(what, g, false);
+    if (!g.is_cuda()) refuse(LGBM_B200_INVALID_ARGUMENT, what, ": want CUDA tensors");
+    if (i == 0) {
+      dev = g.device();
+      on.emplace(dev);
+    } else if (g.device() != dev) {
+      refuse(LGBM_B200_INVALID_ARGUMENT, what, ": tensor ", i, " is on ", g.device(),
+             ", the first on ", dev);
+    }
+    Tensor o;
+    if (scale) {
+      o = outs.list ? tensor(what, PySequence_Fast_GET_ITEM(outs.list, i)) : g;
+      if (outs.list && (o.sizes() != g.sizes() || o.scalar_type() != g.scalar_type() ||
+                        o.device() != dev))
+        refuse(LGBM_B200_LENGTH_MISMATCH, what, ": result ", i, " ", describe(o), ", want ",
+               describe(g));
+    }
+    const int64_t count = g.numel();
+    if (count == 0) continue;
+    const auto reach = [](const Tensor& t) {  // bytes from the first element to behind the last
+      int64_t last = 0;
+      for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+      return (uintptr_t)(last + 1) * t.element_size();
+    };
+    const bool dense = g.is_non_overlapping_and_dense();
+    lgbm_b200_experts_tensor item{};
+    item.count = count;
+    item.dtype = dtype;
+    if (scale) {
+      const bool out_dense = o.is_non_overlapping_and_dense();
+      const uintptr_t gp = reinterpret_cast<uintptr_t>(g.data_ptr()),
+                      op = reinterpret_cast<uintptr_t>(o.data_ptr());
+      if (!out_dense && !own_places(o))
+        refuse(LGBM_B200_INVALID_ARGUMENT, what, ": result ", i,
+               " may hold several elements in one place");
+      const bool same_place = gp == op && g.strides() == o.strides();
+      ranges.push_back({op, op + reach(o), (int64_t)i, true});
+      if (!same_place) ranges.push_back({gp, gp + reach(g), (int64_t)i, false});
+      if (!(dense && out_dense && g.strides() == o.strides())) {
+        g = g.contiguous();
+        if (!o.is_contiguous()) {
+          Tensor t = make(dev, o.scalar_type(), o.sizes());
+          f.back.push_back({o, t});
+          o = t;
+        }
+      }
+      item.out = o.data_ptr();
+      f.kept.push_back(o);
+    } else if (!dense) {
+      g = g.contiguous();
+    }
+    item.in = g.data_ptr();
+    f.kept.push_back(std::move(g));
+    f.items.push_back(item);
+  }
+  check_overlaps(what, ranges);
+  Tensor norm = make(dev, at::kFloat, {});
+  const int64_t count = (int64_t)f.items.size();
+  Scratch ws(dev, lgbm_b200_experts_norm_workspace(count));
+  if (scale)
+    check(lgbm_b200_experts_clip_grads(f.items.data(), count, max_norm, norm.data_ptr<float>(),
+                                       ws.p(), ws.bytes, on->stream));
+  else
+    check(lgbm_b200_experts_grad_norm(f.items.data(), count, norm.data_ptr<float>(), ws.p(),
+                                      ws.bytes, on->stream));
+  for (const auto& b : f.back) b.to.copy_(b.from);
+  if (scale)  // autograd counts writes
+    for (Py_ssize_t i = 0; i < n; ++i)
+      THPVariable_Unpack(PySequence_Fast_GET_ITEM(outs.list ? outs.list : grads.list, i))
+          .unsafeGetTensorImpl()
+          ->bump_version();
+  return wrap(norm);
+}
+
 // errors() -> bits
 PyObject* errors(PyObject* const*) {
   uint32_t bits = 0;
@@ -673,6 +827,7 @@ PyMethodDef g_methods[] = {
     {"combine_backward", (PyCFunction)(void (*)())entry<combine_backward, 4>, METH_FASTCALL,
      nullptr},
     {"dropout", (PyCFunction)(void (*)())entry<dropout, 5>, METH_FASTCALL, nullptr},
+    {"clip_grads", (PyCFunction)(void (*)())entry<clip_grads, 3>, METH_FASTCALL, nullptr},
     {"errors", (PyCFunction)(void (*)())entry<errors, 0>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -46,8 +46,9 @@ except ImportError as e:
                       "it with `python -m lightgbm_rs_b200.build`") from e
 
 __all__ = ["Routing", "route", "route_backward", "grouped_matmul", "grouped_matmul_backward",
+           "grouped_linear", "grouped_linear_backward", "grouped_gated", "grouped_gated_backward",
            "grouped_matmul_w4", "quantize_w4", "combine", "combine_backward", "dropout",
-           "dropout_backward", "check_errors"]
+           "dropout_backward", "grad_norm", "clip_grads", "check_errors"]
 
 Routing = namedtuple("Routing", ["weights", "experts", "position", "rows", "offsets"])
 Routing.__doc__ = """What `route` returns, M = T * k slots:
@@ -215,6 +216,20 @@ def dropout_backward(dout, p, seed, offset=0):
     """Gradient of x from that of `dropout`'s result with the same p, seed and offset (the
     residual's gradient is dout itself)."""
     return _X.dropout(dout, p, seed, offset, None)
+
+
+def grad_norm(grads):
+    """sqrt of the sum of the squares of all elements of all tensors (f32, bf16 or f16, mixed, of
+    any shapes), as an f32 tensor without dimensions: right wherever f32 can hold it."""
+    return _X.clip_grads(grads, None, None)
+
+
+def clip_grads(grads, max_norm, out=None):
+    """Scales all tensors by min(1, max_norm / grad_norm(grads)) and returns the norm from before.
+    In place, or into the tensors of `out` (like grads in shapes and types). What is written must
+    not overlap what another tensor reads or writes. An infinite norm makes the factor 0, NaN
+    makes every result NaN: check the norm where gradients may not be finite."""
+    return _X.clip_grads(grads, float(max_norm), out)
 
 
 def check_errors():
