@@ -205,7 +205,7 @@ struct NormCall {
   int64_t count;
   bool scale;
   double max_norm;
-  double* partial;
+  void* workspace;
   float* norm;
 };
 int64_t norm_workspace(int64_t tensors);

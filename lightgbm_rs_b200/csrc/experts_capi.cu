@@ -301,7 +301,7 @@ int run_norm(const char* what, const lgbm_b200_experts_tensor* tensors, int64_t 
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace))))
     return refuse(LGBM_B200_LENGTH_MISMATCH, "%s: workspace of %lld bytes, %lld are needed",
                   what, (long long)workspace_bytes, (long long)need);
-  const NormCall c{tensors, count, scale, max_norm, static_cast<double*>(workspace), norm};
+  const NormCall c{tensors, count, scale, max_norm, workspace, norm};
   return launched(launch_norm(c, reinterpret_cast<cudaStream_t>(stream)), what);
 }
 
