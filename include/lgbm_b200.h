@@ -720,7 +720,7 @@ typedef struct lgbm_b200_experts_tensor {
   int32_t dtype;   /* LGBM_B200_DTYPE_* */
   int32_t reserved;
 } lgbm_b200_experts_tensor;
-int64_t lgbm_b200_experts_norm_workspace(int64_t tensors);
+int64_t lgbm_b200_experts_norm_workspace(const lgbm_b200_experts_tensor* tensors, int64_t count);
 int lgbm_b200_experts_grad_norm(const lgbm_b200_experts_tensor* tensors, int64_t count,
                                 float* norm, void* workspace, int64_t workspace_bytes,
                                 void* stream);

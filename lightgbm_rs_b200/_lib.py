@@ -185,7 +185,7 @@ _SIGS = {
     "lgbm_b200_experts_matmul_w4": ([_P, _i64, _i64, _P, _P, _P, _P, _i32, _P, _i32, _i64, _i32,
                                      _i32, _i32, _P, _P], ctypes.c_int),
     "lgbm_b200_experts_errors": ([_P], ctypes.c_int),
-    "lgbm_b200_experts_norm_workspace": ([_i64], _i64),
+    "lgbm_b200_experts_norm_workspace": ([_P, _i64], _i64),
     "lgbm_b200_experts_grad_norm": ([_P, _i64, _P, _P, _i64, _P], ctypes.c_int),
     "lgbm_b200_experts_clip_grads": ([_P, _i64, _f64, _P, _P, _i64, _P], ctypes.c_int),
     "lgbm_b200_experts_combine": ([_P, _i32, _i64, _i32, _i64, _P, _P, _i64, _i32, _P, _P],

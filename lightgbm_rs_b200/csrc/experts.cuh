@@ -208,7 +208,7 @@ struct NormCall {
   void* workspace;
   float* norm;
 };
-int64_t norm_workspace(int64_t tensors);
+int64_t norm_workspace(const lgbm_b200_experts_tensor* tensors, int64_t count);
 cudaError_t launch_norm(const NormCall& c, cudaStream_t st);
 
 // experts_few.cu

@@ -297,7 +297,7 @@ int run_norm(const char* what, const lgbm_b200_experts_tensor* tensors, int64_t 
     if (t.count > 0)
       if (int rc = check_starts(what, {{t.in, size}, {scale ? t.out : nullptr, size}})) return rc;
   }
-  const int64_t need = norm_workspace(count);
+  const int64_t need = norm_workspace(tensors, count);
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace))))
     return refuse(LGBM_B200_LENGTH_MISMATCH, "%s: workspace of %lld bytes, %lld are needed",
                   what, (long long)workspace_bytes, (long long)need);
@@ -693,8 +693,8 @@ int lgbm_b200_experts_matmul_w4(const void* x, int64_t x_rows, int64_t x_pitch,
   return launched(launch_few(f, reinterpret_cast<cudaStream_t>(stream)), what);
 }
 
-int64_t lgbm_b200_experts_norm_workspace(int64_t tensors) {
-  return tensors < 1 ? 0 : norm_workspace(tensors);
+int64_t lgbm_b200_experts_norm_workspace(const lgbm_b200_experts_tensor* tensors, int64_t count) {
+  return count < 1 || !tensors ? 0 : norm_workspace(tensors, count);
 }
 
 int lgbm_b200_experts_grad_norm(const lgbm_b200_experts_tensor* tensors, int64_t count,

@@ -777,7 +777,7 @@ PyObject* clip_grads(PyObject* const* a) {
     refuse(LGBM_B200_INVALID_ARGUMENT, what, ": a tensor that is written overlaps another one");
   Tensor norm = make(dev, at::kFloat, {});
   const int64_t count = (int64_t)items.size();
-  Scratch ws(dev, lgbm_b200_experts_norm_workspace(count));
+  Scratch ws(dev, lgbm_b200_experts_norm_workspace(items.data(), count));
   if (scale)
     check(lgbm_b200_experts_clip_grads(items.data(), count, max_norm, norm.data_ptr<float>(),
                                        ws.p(), ws.bytes, on->stream));
