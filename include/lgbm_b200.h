@@ -614,7 +614,7 @@ int lgbm_b200_experts_matmul_backward(const void* dy, int64_t dy_pitch, const vo
  * may be NULL. A row of no expert has y = residual (0 without one) and h = 0.
  * pre (NULL: not wanted) keeps what the activation was given, rounded to the inputs' type, for
  * the backward pass: [rows][ld], gated [rows][2][ld] (gate, then up), ld = the width rounded up
- * to 8, 16-byte aligned; what lies between the width and ld is not defined. Everything before
+ * to 16, 32-byte aligned; what lies between the width and ld is not defined. Everything before
  * the results' one rounding is in f32.
  * Workspace: lgbm_b200_experts_matmul_workspace with the same operands (gated: outer =
  * 2 hidden). */

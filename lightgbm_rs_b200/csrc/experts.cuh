@@ -116,6 +116,7 @@ struct Raw<T, 1> {
   }
 };
 
+inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 inline int elem_size(int32_t dtype) { return dtype == LGBM_B200_DTYPE_F32 ? 4 : 2; }
 
@@ -154,8 +155,8 @@ struct Epilogue {
   int64_t residual_pitch;
   void* pre;                // what the activation was given, [rows][1 or 2][pre_pitch], or null
 };
-// Elements of a saved row: padded to 16 bytes, for loads and stores of 16 bytes at any width.
-inline int64_t pre_pitch(int64_t width) { return (width + 7) / 8 * 8; }
+// Elements of a saved row: padded to 32 bytes, so that a lane writes whole sectors at any width.
+inline int64_t pre_pitch(int64_t width) { return (width + 15) / 16 * 16; }
 
 // experts_matmul.cu
 struct MatmulCall {

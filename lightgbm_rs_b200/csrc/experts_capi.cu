@@ -134,8 +134,8 @@ int check_epilogue(const char* what, const MatmulCall& c) {
   if (e.residual && e.residual_pitch < c.outer)
     return refuse(LGBM_B200_LENGTH_MISMATCH, "%s: residual pitch %lld < outer %d", what,
                   (long long)e.residual_pitch, c.outer);
-  if (!aligned16(e.pre))
-    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: pre is not 16-byte aligned", what);
+  if (!aligned32(e.pre))
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: pre is not 32-byte aligned", what);
   return check_starts(what, {{e.bias, 2}, {e.residual, 2}});
 }
 
@@ -160,8 +160,9 @@ int run_product(const char* what, const MatmulCall& c, void* workspace, int64_t 
 }
 
 // The gradient of what the activation was given, in the workspace ahead of what the products need.
+int64_t dpre_pitch(int32_t outer) { return ((int64_t)outer + 7) / 8 * 8; }
 int64_t dpre_bytes(int64_t rows, int32_t outer) {
-  return (rows * pre_pitch(outer) * 2 + 255) / 256 * 256;
+  return (rows * dpre_pitch(outer) * 2 + 255) / 256 * 256;
 }
 int64_t sums_bytes(int64_t rows, int32_t experts, int32_t outer) {
   return (linear_grad_workspace(rows, experts, outer) + 255) / 256 * 256;
@@ -180,15 +181,15 @@ int run_layer_backward(const char* what, MatmulCall c, bool gated, int32_t act, 
   const bool turns = gated || act != LGBM_B200_ACT_NONE;  // dpre is not dy itself
   // what check_product sees of dy: a pitch that fits, where dpre takes its place
   MatmulCall p = c;
-  if (turns) p.dy_pitch = pre_pitch(c.outer);
+  if (turns) p.dy_pitch = dpre_pitch(c.outer);
   if (int rc = check_product(what, p)) return rc;
   if (c.dy_pitch < width)
     return refuse(LGBM_B200_LENGTH_MISMATCH, "%s: dy pitch %lld < %d", what,
                   (long long)c.dy_pitch, width);
   if (c.rows > 0 && (!c.dy || (turns && !pre)))
     return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: null argument", what);
-  if (turns && !aligned16(pre))
-    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: pre is not 16-byte aligned", what);
+  if (turns && !aligned32(pre))
+    return refuse(LGBM_B200_INVALID_ARGUMENT, "%s: pre is not 32-byte aligned", what);
   if (int rc = check_starts(what, {{c.dy, 2}, {dbias, dbias ? elem_size(c.grad_dtype) : 1}}))
     return rc;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -256,7 +257,7 @@ int64_t layer_backward_workspace(const void* dy, int64_t dy_pitch, const void* x
   c.x_pitch = x_pitch;
   c.index = index;
   c.dy = turns ? reinterpret_cast<const void*>((uintptr_t)256) : dy;
-  c.dy_pitch = turns ? pre_pitch(outer) : dy_pitch;
+  c.dy_pitch = turns ? dpre_pitch(outer) : dy_pitch;
   c.w = w;
   c.rows = rows;
   c.experts = experts;

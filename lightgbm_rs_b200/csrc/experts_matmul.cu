@@ -98,7 +98,6 @@ struct MatArgs {
   uint32_t* error;
   // LINEAR, GATED
   int32_t act;
-  int32_t bias_vec;       // the bias may be read 16 bytes at a time
   int32_t residual_unit;  // bytes of a load, as `unit`
   const void* bias;
   const void* residual;
@@ -124,6 +123,12 @@ __device__ __forceinline__ uint32_t leader_addr(uint32_t addr) {
 }
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+// The same without making this thread's stores visible first, which waited a microsecond for
+// results on their way out: for one that says no more than that tensor memory has been read.
+__device__ __forceinline__ void bar_arrive_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
                : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
@@ -317,13 +322,14 @@ __device__ __forceinline__ void tile_of(int t, int mt, int nt, int band, int& m,
 template <int KIND, int BN, int CTAS>
 struct Shape {
   static constexpr bool kFused = KIND == LINEAR || KIND == GATED;
-  static constexpr int kStoreWarps = KIND == WEIGHT_F32 ? 16 : 8;
+  static constexpr int kStoreWarps = KIND == WEIGHT_F32 || kFused ? 16 : 8;
   static constexpr int kRun = KIND == WEIGHT_F32 ? 768 : 4096;  // see "Precision" above
   static constexpr int kThreads = 64 + 32 * kStoreWarps;
-  static constexpr int kBlocks = kFused ? 2 : 1;  // staging blocks of a storing warp
-  static constexpr int kStoreBytes = kBlocks * kStoreWarps * 32 * kStoreRow;
-  static constexpr int kRows = kTileM * CTAS;
   static constexpr int kOutCols = KIND == GATED ? BN / 2 : BN;  // columns of the result
+  // bytes of a row of a staging block; LINEAR, GATED: so that narrow tiles occupy all warps too
+  static constexpr int kRowBytes = kFused && kOutCols < 128 ? 32 : kStoreRow;
+  static constexpr int kStoreBytes = kStoreWarps * 32 * kRowBytes;
+  static constexpr int kRows = kTileM * CTAS;
   static constexpr int kCols = BN / CTAS;  // columns of B that a CTA loads
   static constexpr int kStageBytes = (kTileM + kCols) * 128;
   static constexpr int kStages = (212992 - kStoreBytes) / kStageBytes;  // 3 to 8
@@ -333,113 +339,163 @@ struct Shape {
       1024 + kStages * kStageBytes + kStoreBytes + 8 * kGroupSlots + 512;
 };
 
-// Where piece `p` (16 bytes) of row `row` lies in a staging block: the 64-byte swizzle of TMA.
+// Where piece `p` (16 bytes) of row `row` lies in a staging block of ROW-byte rows: TMA's swizzle
+// of rows of 64 bytes, and for the others the same idea: eight rows' piece p hit all banks.
+template <int ROW = kStoreRow>
 __device__ __forceinline__ uint32_t staged(int row, int p) {
-  return row * kStoreRow + ((p ^ ((row >> 1) & 3)) << 4);
+  constexpr int kShift = ROW == 128 ? 0 : ROW == 64 ? 1 : 2;
+  return row * ROW + ((p ^ ((row >> kShift) & (ROW / 16 - 1))) << 4);
 }
 
 // One 32-row block of a storing warp, from its staging block to `dst` (row pitch in bytes),
 // `bytes` of each row, UNIT bytes at a time.
-template <int UNIT>
+template <int UNIT, int ROW = kStoreRow>
 __device__ __forceinline__ void store_rows(uint32_t stage, char* dst, int64_t pitch, int nrows,
                                            int bytes, int lane) {
-  constexpr int kLanes = kStoreRow / UNIT;  // of a row
-  constexpr int kPerStep = 32 / kLanes;     // rows
-  const int at = lane % kLanes * UNIT;
-  if (at + UNIT > bytes) return;
-  char* to = dst + (lane / kLanes) * pitch + at;
+  constexpr int kLanes = ROW / UNIT < 32 ? ROW / UNIT : 32;  // of a row
+  constexpr int kPerStep = 32 / kLanes;                      // rows
+  auto lot = [&](int at) {  // the columns of one step
+    if (at + UNIT > bytes) return;
+    char* to = dst + (lane / kLanes) * pitch + at;
 #pragma unroll 8
-  for (int i0 = 0; i0 < 32; i0 += kPerStep) {
-    const int i = i0 + lane / kLanes;
-    if (i < nrows) {
-      const uint32_t from = stage + staged(i, at >> 4) + (at & 15);
-      if constexpr (UNIT == 16) {
-        uint32_t w[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                     : "r"(from)
-                     : "memory");
-        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-      } else if constexpr (UNIT == 8) {
-        uint32_t w[2];
-        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
-                     : "=r"(w[0]), "=r"(w[1])
-                     : "r"(from)
-                     : "memory");
-        *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-      } else if constexpr (UNIT == 4) {
-        uint32_t w;
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
-        *reinterpret_cast<uint32_t*>(to) = w;
-      } else {
-        uint16_t w;
-        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(from) : "memory");
-        *reinterpret_cast<uint16_t*>(to) = w;
+    for (int i0 = 0; i0 < 32; i0 += kPerStep) {
+      const int i = i0 + lane / kLanes;
+      if (i < nrows) {
+        const uint32_t from = stage + staged<ROW>(i, at >> 4) + (at & 15);
+        if constexpr (UNIT == 16) {
+          uint32_t w[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(from)
+                       : "memory");
+          *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else if constexpr (UNIT == 8) {
+          uint32_t w[2];
+          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                       : "=r"(w[0]), "=r"(w[1])
+                       : "r"(from)
+                       : "memory");
+          *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+        } else if constexpr (UNIT == 4) {
+          uint32_t w;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
+          *reinterpret_cast<uint32_t*>(to) = w;
+        } else {
+          uint16_t w;
+          asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(from) : "memory");
+          *reinterpret_cast<uint16_t*>(to) = w;
+        }
       }
+      to += kPerStep * pitch;
     }
-    to += kPerStep * pitch;
-  }
+  };
+  lot(lane % kLanes * UNIT);
+  if constexpr (ROW / UNIT > 32) lot((lane + 32) * UNIT);
 }
 
-// The way back: a 32-row block of `src` to a staging block, all loads first.
-template <int UNIT>
+// The way back, for rows that do not start at 16 bytes: a 32-row block of `src` to a staging block,
+// eight loads at a time.
+template <int UNIT, int ROW>
 __device__ __forceinline__ void load_rows(uint32_t stage, const char* src, int64_t pitch,
                                           int nrows, int bytes, int lane) {
-  constexpr int kLanes = kStoreRow / UNIT;  // of a row
-  constexpr int kPerStep = 32 / kLanes;     // rows
-  constexpr int kSteps = 32 / kPerStep;
-  using T = std::conditional_t<
-      UNIT == 16, uint4,
-      std::conditional_t<UNIT == 8, uint2, std::conditional_t<UNIT == 4, uint32_t, uint16_t>>>;
+  constexpr int kLanes = ROW / UNIT;     // of a row
+  constexpr int kPerStep = 32 / kLanes;  // rows
+  constexpr int kSteps = 8;              // at a time
+  using T =
+      std::conditional_t<UNIT == 8, uint2, std::conditional_t<UNIT == 4, uint32_t, uint16_t>>;
   const int at = lane % kLanes * UNIT;
   if (at + UNIT > bytes) return;
   const char* from = src + (lane / kLanes) * pitch + at;
-  T v[kSteps];
+#pragma unroll 1
+  for (int i0 = 0; i0 < 32; i0 += kSteps * kPerStep) {
+    T v[kSteps];
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i)
-    if (i * kPerStep + lane / kLanes < nrows)
-      v[i] = __ldg(reinterpret_cast<const T*>(from + i * kPerStep * pitch));
+    for (int i = 0; i < kSteps; ++i) {
+      const int row = i0 + i * kPerStep + lane / kLanes;
+      if (row < nrows)
+        v[i] = __ldg(reinterpret_cast<const T*>(from + (int64_t)(i0 + i * kPerStep) * pitch));
+    }
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int row = i * kPerStep + lane / kLanes;
-    const uint32_t to = stage + staged(row, at >> 4) + (at & 15);
-    if (row < nrows) {
-      if constexpr (UNIT == 16)
-        store_piece(to, v[i].x, v[i].y, v[i].z, v[i].w);
-      else if constexpr (UNIT == 8)
-        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(v[i].x), "r"(v[i].y)
-                     : "memory");
-      else if constexpr (UNIT == 4)
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(v[i]) : "memory");
-      else
-        asm volatile("st.shared.b16 [%0], %1;" ::"r"(to), "h"(v[i]) : "memory");
+    for (int i = 0; i < kSteps; ++i) {
+      const int row = i0 + i * kPerStep + lane / kLanes;
+      const uint32_t to = stage + staged<ROW>(row, at >> 4) + (at & 15);
+      if (row < nrows) {
+        if constexpr (UNIT == 8)
+          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(v[i].x), "r"(v[i].y)
+                       : "memory");
+        else if constexpr (UNIT == 4)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(v[i]) : "memory");
+        else
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(to), "h"(v[i]) : "memory");
+      }
     }
   }
 }
 
-// Two 16-bit values of a word as f32, by the type of `kind`.
+// Both out of line: inline their loops' addresses spilled.
+template <int ROW>
+__device__ __noinline__ void load_odd_rows(int unit, uint32_t stage, const char* src, int64_t pitch,
+                                           int nrows, int bytes, int lane) {
+  if (unit == 8) load_rows<8, ROW>(stage, src, pitch, nrows, bytes, lane);
+  else if (unit == 4) load_rows<4, ROW>(stage, src, pitch, nrows, bytes, lane);
+  else load_rows<2, ROW>(stage, src, pitch, nrows, bytes, lane);
+}
+template <int ROW>
+__device__ __noinline__ void store_odd_rows(int unit, uint32_t stage, char* dst, int64_t pitch,
+                                            int nrows, int bytes, int lane) {
+  if (unit == 8) store_rows<8, ROW>(stage, dst, pitch, nrows, bytes, lane);
+  else if (unit == 4) store_rows<4, ROW>(stage, dst, pitch, nrows, bytes, lane);
+  else store_rows<2, ROW>(stage, dst, pitch, nrows, bytes, lane);
+}
+
+// 32 bytes of a row that starts at `unit` (16 or 32) bytes; if there are fewer, `bytes` of them (a
+// multiple of 16).
+__device__ __forceinline__ void load32(uint32_t* w, const char* p, int unit, int bytes) {
+  if (unit == 32 && bytes >= 32) {
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
+                   "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+  } else {
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+    if (bytes >= 16) a = __ldg(reinterpret_cast<const uint4*>(p));
+    if (bytes >= 32) b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+    w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+  }
+}
+
+// Two 16-bit values of a word as f32.
 __device__ __forceinline__ float2 unpack2(uint32_t w, bool bf16) {
   if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
-__device__ __forceinline__ void pack32(const float (&f)[32], bool bf16, uint32_t (&w)[16]) {
+__device__ __forceinline__ void add16(float (&f)[16], const uint32_t* w, bool bf16) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 v = unpack2(w[i], bf16);
+    f[2 * i] += v.x;
+    f[2 * i + 1] += v.y;
+  }
+}
+__device__ __forceinline__ void pack16(const float (&f)[16], bool bf16, uint32_t (&w)[8]) {
   if (bf16) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 8; ++i)
       w[i] = pack2<true>(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]));
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 8; ++i)
       w[i] = pack2<false>(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]));
   }
 }
 
 struct Maps {
   CUtensorMap a, b;  // tiles of 64 columns
-  CUtensorMap out;   // 32 rows of 64 bytes
+  CUtensorMap out;   // 32 rows of kRowBytes
 };
 struct FusedMaps : Maps {
-  CUtensorMap pre;   // 32 rows of 64 bytes of a half
+  CUtensorMap pre;   // the same of a half
 };
 template <int KIND>
 using MapsOf = std::conditional_t<KIND == LINEAR || KIND == GATED, FusedMaps, Maps>;
@@ -720,8 +776,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
   } else {
     const int quarter = warp & 3, part = (warp - 2) >> 2;  // of the lanes; of the chunks
     constexpr int kParts = S::kStoreWarps / 4;
-    const uint32_t stage = store_base + (warp - 2) * S::kBlocks * 32 * kStoreRow;
-    uint32_t turn = 0;  // the staging block used last, where there are two
+    const uint32_t stage = store_base + (warp - 2) * 32 * S::kRowBytes;
     constexpr int bytes = kWide ? 4 : 2;
     constexpr int per_chunk = kStoreRow / bytes;  // columns of a staging row
     const int64_t pitch = g.out_pitch * bytes;
@@ -736,7 +791,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       const uint32_t bar = acc_empty + 8 * acc;
-      if (lane == 0) bar_arrive_cluster(CTAS == 2 ? leader_addr(bar) : bar);
+      if (lane == 0) bar_arrive_relaxed(CTAS == 2 ? leader_addr(bar) : bar);
     };
     // Each later run of a tile is added to the first one's half (at `from`), where the sum
     // leaves from. A warp adds the columns that it stores.
@@ -744,21 +799,30 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
       for (int k0 = kRun; k0 < r.red; k0 += kRun) {
         uint32_t other;
         if (!accumulated(k0 / kRun, other)) return false;
-        constexpr int kHalves = BN / S::kOutCols;  // GATED: a column of gate and one of up
-#pragma unroll 1
-        for (int c0 = part * per_chunk; c0 < S::kOutCols; c0 += kParts * per_chunk)
-#pragma unroll 1
-          for (int i = 0; i < per_chunk * kHalves; i += 16) {
-            const int c = c0 + i + (i < per_chunk ? 0 : S::kOutCols - per_chunk);
-            uint32_t sum[16], v[16];
-            tmem_load16(from + c, sum);
-            tmem_load16(tmem + other * BN + lanes + c, v);
-            tmem_wait();
+        auto add = [&](int c) {
+          uint32_t sum[16], v[16];
+          tmem_load16(from + c, sum);
+          tmem_load16(tmem + other * BN + lanes + c, v);
+          tmem_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              sum[j] = __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(v[j]));
-            tmem_store16(from + c, sum);
-          }
+          for (int j = 0; j < 16; ++j)
+            sum[j] = __float_as_uint(__uint_as_float(sum[j]) + __uint_as_float(v[j]));
+          tmem_store16(from + c, sum);
+        };
+        if constexpr (S::kFused) {
+          constexpr int kHalves = BN / S::kOutCols;  // GATED: gate and up
+          constexpr int kChunk = S::kRowBytes / 2;
+#pragma unroll 1
+          for (int c0 = part * kChunk; c0 < S::kOutCols; c0 += kParts * kChunk)
+#pragma unroll 1
+            for (int i = 0; i < kHalves * kChunk; i += 16)
+              add(i / kChunk * S::kOutCols + c0 + i % kChunk);
+        } else {
+#pragma unroll 1
+          for (int c0 = part * per_chunk; c0 < BN; c0 += kParts * per_chunk)
+#pragma unroll 1
+            for (int c = c0; c < c0 + per_chunk; c += 16) add(c);
+        }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         release(other);
       }
@@ -768,20 +832,20 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
       const Tile r = decode(t);
       const int row0 = r.m0 + quarter * 32;
       if constexpr (S::kFused) {
-        const int ncols = min(S::kOutCols, g.cols - r.n0), nrows = min(32, r.m_end - row0);
-        const bool whole = nrows == 32, live = r.red > 0, bf16 = g.out_kind == LGBM_B200_DTYPE_BF16;
-        // the block that the store before the last one has read
-        auto block = [&] {
-          turn ^= 1;
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        // A chunk of 16 or 32 columns at a time, each lane its row: read from tensor memory,
+        // finished in registers, and through the warp's staging block to the result.
+        constexpr int ROW = S::kRowBytes, kChunk = ROW / 2, kHalves = KIND == GATED ? 2 : 1;
+        const int nrows = min(32, r.m_end - row0);
+        const int ncols = nrows > 0 ? min(S::kOutCols, g.cols - r.n0) : 0;
+        const bool live = r.red > 0, bf16 = g.out_kind == LGBM_B200_DTYPE_BF16;
+        const bool whole = nrows == 32;
+        // the staging block, when the last store has read it
+        auto free_block = [&] {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
-          return stage + turn * 32 * kStoreRow;
         };
-        // this lane's row of 32 columns, through block `at`, to the result or the saved values
-        auto leave = [&](uint32_t at, const uint32_t (&w)[16], int c0, int saved) {
-#pragma unroll
-          for (int p = 0; p < 4; ++p)
-            store_piece(at + staged(lane, p), w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
+        // the block to columns c of the result (saved < 0) or of a half of the saved values
+        auto leave = [&](int c, int saved) {
           if (whole && (saved >= 0 || g.unit == 16)) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -790,228 +854,225 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
                 asm volatile(
                     "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], "
                     "[%4];" ::"l"(&maps.pre),
-                    "r"(r.n0 + c0), "r"(row0), "r"(saved), "r"(at)
+                    "r"(r.n0 + c), "r"(row0), "r"(saved), "r"(stage)
                     : "memory");
               else
                 asm volatile(
                     "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], "
                     "[%3];" ::"l"(&maps.out),
-                    "r"(r.n0 + c0), "r"(row0), "r"(at)
+                    "r"(r.n0 + c), "r"(row0), "r"(stage)
                     : "memory");
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
           } else {
             __syncwarp();
-            const int n = min(32, ncols - c0) * 2;
+            const int n = min(kChunk, ncols - c) * 2;
             if (saved >= 0) {
-              constexpr int kHalves = KIND == GATED ? 2 : 1;
-              store_rows<16>(at,
-                             static_cast<char*>(g.pre) +
-                                 (((int64_t)row0 * kHalves + saved) * g.pre_pitch + r.n0 + c0) * 2,
-                             g.pre_pitch * kHalves * 2, nrows, (n + 15) / 16 * 16, lane);
+              store_rows<16, ROW>(stage,
+                                  static_cast<char*>(g.pre) +
+                                      (((int64_t)row0 * kHalves + saved) * g.pre_pitch + r.n0 + c) *
+                                          2,
+                                  kHalves * g.pre_pitch * 2, nrows, (n + 15) / 16 * 16, lane);
             } else {
-              char* dst = static_cast<char*>(g.out) + (int64_t)row0 * pitch + (int64_t)(r.n0 + c0) * 2;
-              if (g.unit == 16) store_rows<16>(at, dst, pitch, nrows, n, lane);
-              else if (g.unit == 8) store_rows<8>(at, dst, pitch, nrows, n, lane);
-              else if (g.unit == 4) store_rows<4>(at, dst, pitch, nrows, n, lane);
-              else store_rows<2>(at, dst, pitch, nrows, n, lane);
+              char* dst = static_cast<char*>(g.out) + (int64_t)row0 * pitch + (r.n0 + c) * 2ll;
+              if (g.unit == 16) store_rows<16, ROW>(stage, dst, pitch, nrows, n, lane);
+              else store_odd_rows<ROW>(g.unit, stage, dst, pitch, nrows, n, lane);
             }
           }
-          // a group for every block, empty without a bulk store: block() counts them
-          if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         };
+        uint32_t bias = 0;           // of columns c + 2 lane and c + 2 lane + 1
+        uint32_t residual[kChunk / 2];
+        auto fetch = [&](int c) {  // what columns c add, ahead of use
+          if (KIND != LINEAR || c >= ncols) return;
+          if (live && g.bias && 2 * lane < kChunk) {
+            const uint16_t* p =
+                static_cast<const uint16_t*>(g.bias) + (int64_t)r.expert * g.cols + r.n0 + c;
+            bias = 2 * lane < ncols - c ? __ldg(p + 2 * lane) : 0;
+            if (2 * lane + 1 < ncols - c) bias |= (uint32_t)__ldg(p + 2 * lane + 1) << 16;
+          }
+          if (g.residual && g.residual_unit >= 16 && lane < nrows) {
+            const char* p = static_cast<const char*>(g.residual) +
+                            ((row0 + lane) * g.residual_pitch + r.n0 + c) * 2;
+#pragma unroll
+            for (int i = 0; i < kChunk / 16; ++i)
+              load32(residual + 8 * i, p + 32 * i, g.residual_unit, (ncols - c) * 2 - 32 * i);
+          }
+        };
+        fetch(part * kChunk);
         uint32_t acc = 0;
         if (live && !(ok = accumulated(0, acc))) break;
         const uint32_t from = tmem + acc * BN + lanes;
         if (!(ok = add_runs(r, from))) break;
-        for (int c0 = part * 32; c0 < ncols && nrows > 0; c0 += kParts * 32) {
-          uint32_t w[16];
-          float f[32], up[KIND == GATED ? 32 : 1];
+        // 16 columns of a half's products, with the bias
+        auto load = [&](int c0, int i, int half, float (&f)[16]) {
           if (live) {
-            uint32_t v[32];
-            tmem_load32(from + c0, v);
-            if constexpr (KIND == GATED) {
-              uint32_t u[32];
-              tmem_load32(from + S::kOutCols + c0, u);
-              tmem_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) up[i] = __uint_as_float(u[i]);
-            }
+            uint32_t v[16];
+            tmem_load16(from + half * S::kOutCols + c0 + 16 * i, v);
             tmem_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+            for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(v[j]);
             if (KIND == LINEAR && g.bias) {
-              const uint16_t* bias = static_cast<const uint16_t*>(g.bias) +
-                                     (int64_t)r.expert * g.cols + r.n0 + c0;
-              const int n = ncols - c0;
-              if (g.bias_vec) {
+              uint32_t b[8];
 #pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                  uint4 q = make_uint4(0, 0, 0, 0);
-                  if (8 * p < n) q = __ldg(reinterpret_cast<const uint4*>(bias) + p);
-                  w[4 * p] = q.x, w[4 * p + 1] = q.y, w[4 * p + 2] = q.z, w[4 * p + 3] = q.w;
-                }
-              } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  w[i] = 2 * i < n ? __ldg(bias + 2 * i) : 0;
-                  if (2 * i + 1 < n) w[i] |= (uint32_t)__ldg(bias + 2 * i + 1) << 16;
-                }
-              }
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 b = unpack2(w[i], bf16);
-                f[2 * i] += b.x;
-                f[2 * i + 1] += b.y;
-              }
+              for (int j = 0; j < 8; ++j) b[j] = __shfl_sync(0xFFFFFFFFu, bias, 8 * i + j);
+              add16(f, b, bf16);
             }
           } else {  // rows of no expert
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] = 0.0f;
-            if constexpr (KIND == GATED) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) up[i] = 0.0f;
-            }
+            for (int j = 0; j < 16; ++j) f[j] = 0.0f;
           }
+        };
+        auto put = [&](int i, const float (&f)[16]) {  // into this lane's row of the block
+          uint32_t w[8];
+          pack16(f, bf16, w);
+          store_piece(stage + staged<ROW>(lane, 2 * i), w[0], w[1], w[2], w[3]);
+          store_piece(stage + staged<ROW>(lane, 2 * i + 1), w[4], w[5], w[6], w[7]);
+        };
+#pragma unroll 1
+        for (int c = part * kChunk; c < ncols; c += kParts * kChunk) {
           if (g.pre) {
-            pack32(f, bf16, w);
-            leave(block(), w, c0, 0);
-            if constexpr (KIND == GATED) {
-              pack32(up, bf16, w);
-              leave(block(), w, c0, 1);
+#pragma unroll 1
+            for (int half = 0; half < kHalves; ++half) {
+              free_block();
+#pragma unroll
+              for (int i = 0; i < kChunk / 16; ++i) {
+                float f[16];
+                load(c, i, half, f);
+                put(i, f);
+              }
+              leave(c, half);
             }
           }
-          activate(g.act, f);
-          if constexpr (KIND == GATED) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] *= up[i];
-          }
-          const uint32_t at = block();
-          if (KIND == LINEAR && g.residual) {
-            const int n = min(32, ncols - c0) * 2;
-            const int64_t rp = g.residual_pitch * 2;
-            const char* src = static_cast<const char*>(g.residual) + (int64_t)row0 * rp +
-                              (int64_t)(r.n0 + c0) * 2;
-            if (g.residual_unit == 16) load_rows<16>(at, src, rp, nrows, n, lane);
-            else if (g.residual_unit == 8) load_rows<8>(at, src, rp, nrows, n, lane);
-            else if (g.residual_unit == 4) load_rows<4>(at, src, rp, nrows, n, lane);
-            else load_rows<2>(at, src, rp, nrows, n, lane);
+          free_block();
+          if (KIND == LINEAR && g.residual && g.residual_unit < 16) {
+            load_odd_rows<ROW>(g.residual_unit, stage,
+                               static_cast<const char*>(g.residual) +
+                                   ((int64_t)row0 * g.residual_pitch + r.n0 + c) * 2,
+                               g.residual_pitch * 2, nrows, min(kChunk, ncols - c) * 2, lane);
             __syncwarp();
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {  // this lane's own row, which leave() overwrites
-              uint32_t q[4];
+            for (int i = 0; i < kChunk / 8; ++i)
               asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
-                           : "r"(at + staged(lane, p))
+                           : "=r"(residual[4 * i]), "=r"(residual[4 * i + 1]),
+                             "=r"(residual[4 * i + 2]), "=r"(residual[4 * i + 3])
+                           : "r"(stage + staged<ROW>(lane, i))
                            : "memory");
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float2 b = unpack2(q[j], bf16);
-                f[8 * p + 2 * j] += b.x;
-                f[8 * p + 2 * j + 1] += b.y;
-              }
-            }
           }
-          pack32(f, bf16, w);
-          leave(at, w, c0, -1);
+#pragma unroll
+          for (int i = 0; i < kChunk / 16; ++i) {
+            float f[16];
+            load(c, i, 0, f);
+            activate(g.act, f);
+            if constexpr (KIND == GATED) {
+              float up[16];
+              load(c, i, 1, up);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) f[j] *= up[j];
+            }
+            if (KIND == LINEAR && g.residual) add16(f, residual + 8 * i, bf16);
+            put(i, f);
+          }
+          fetch(c + kParts * kChunk);
+          leave(c, -1);
         }
         if (live) release(acc);
-        continue;
-      }
-      char* out = static_cast<char*>(g.out);
-      int out_row = row0;  // of D as one matrix
-      if (MODE == WEIGHT) {
-        out += (int64_t)r.expert * g.drows * pitch;
-        out_row += r.expert * g.drows;
-      }
-      const int ncols = min(BN, g.cols - r.n0), nrows = min(32, r.m_end - row0);
-      // whole 32-row blocks leave by TMA, which also cuts off the last columns
-      const bool by_tma = g.unit == 16 && nrows == 32;
-      // this lane's row of a chunk, 64 bytes, through the staging block to D
-      auto put = [&](const uint32_t* w, int c0) {
-        // the staging block is free when the last store has read it
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        __syncwarp();
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-          store_piece(stage + staged(lane, p), w[4 * p], w[4 * p + 1], w[4 * p + 2],
-                      w[4 * p + 3]);
-        if (by_tma) {
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) {
-            asm volatile(
-                "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
-                    &maps.out),
-                "r"(r.n0 + c0), "r"(out_row), "r"(stage)
-                : "memory");
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          }
-        } else {
-          __syncwarp();
-          const int n = min(per_chunk, ncols - c0) * bytes;
-          char* dst = out + (int64_t)row0 * pitch + (int64_t)(r.n0 + c0) * bytes;
-          if (g.unit == 16) store_rows<16>(stage, dst, pitch, nrows, n, lane);
-          else if (g.unit == 8) store_rows<8>(stage, dst, pitch, nrows, n, lane);
-          else if (g.unit == 4) store_rows<4>(stage, dst, pitch, nrows, n, lane);
-          else store_rows<2>(stage, dst, pitch, nrows, n, lane);
-        }
-        __syncwarp();
-      };
-      uint32_t acc = 0;
-      if (kWide && r.red > kRun) {
-        constexpr int kMine = BN / per_chunk / kParts;  // chunks of this warp
-        uint32_t sum[kMine][16];
-#pragma unroll
-        for (int i = 0; i < kMine; ++i)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) sum[i][j] = 0;
-        for (int k0 = 0; k0 < r.red; k0 += kRun) {
-          if (!(ok = accumulated(k0 / kRun, acc))) break;
-          const uint32_t from = tmem + acc * BN + lanes + part * per_chunk;
-#pragma unroll
-          for (int i = 0; i < kMine; ++i) {
-            uint32_t v[16];
-            tmem_load16(from + i * kParts * per_chunk, v);
-            tmem_wait();
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              sum[i][j] = __float_as_uint(__uint_as_float(sum[i][j]) + __uint_as_float(v[j]));
-          }
-          release(acc);
-        }
-        if (!ok) break;
-#pragma unroll
-        for (int i = 0; i < kMine; ++i)
-          if ((i * kParts + part) * per_chunk < ncols && nrows > 0)
-            put(sum[i], (i * kParts + part) * per_chunk);
       } else {
-        if (r.red > 0 && !(ok = accumulated(0, acc))) break;
-        const uint32_t from = tmem + acc * BN + lanes;
-        if constexpr (!kWide) {
-          if (!(ok = add_runs(r, from))) break;
+        char* out = static_cast<char*>(g.out);
+        int out_row = row0;  // of D as one matrix
+        if (MODE == WEIGHT) {
+          out += (int64_t)r.expert * g.drows * pitch;
+          out_row += r.expert * g.drows;
         }
-        for (int c0 = part * per_chunk; c0 < ncols && nrows > 0; c0 += kParts * per_chunk) {
-          uint32_t v[32], w[16];
-          if (r.red == 0) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = 0;
-          } else if constexpr (kWide) {
-            tmem_load16(from + c0, w);
-            tmem_wait();
-          } else {
-            tmem_load32(from + c0, v);
-            tmem_wait();
-            if (g.out_kind == LGBM_B200_DTYPE_BF16) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = pack2<true>(v[2 * i], v[2 * i + 1]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = pack2<false>(v[2 * i], v[2 * i + 1]);
+        const int ncols = min(BN, g.cols - r.n0), nrows = min(32, r.m_end - row0);
+        // whole 32-row blocks leave by TMA, which also cuts off the last columns
+        const bool by_tma = g.unit == 16 && nrows == 32;
+        // this lane's row of a chunk, 64 bytes, through the staging block to D
+        auto put = [&](const uint32_t* w, int c0) {
+          // the staging block is free when the last store has read it
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+  #pragma unroll
+          for (int p = 0; p < 4; ++p)
+            store_piece(stage + staged(lane, p), w[4 * p], w[4 * p + 1], w[4 * p + 2],
+                        w[4 * p + 3]);
+          if (by_tma) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              asm volatile(
+                  "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], "
+                  "[%3];" ::"l"(&maps.out),
+                  "r"(r.n0 + c0), "r"(out_row), "r"(stage)
+                  : "memory");
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
+          } else {
+            __syncwarp();
+            const int n = min(per_chunk, ncols - c0) * bytes;
+            char* dst = out + (int64_t)row0 * pitch + (int64_t)(r.n0 + c0) * bytes;
+            if (g.unit == 16) store_rows<16>(stage, dst, pitch, nrows, n, lane);
+            else if (g.unit == 8) store_rows<8>(stage, dst, pitch, nrows, n, lane);
+            else if (g.unit == 4) store_rows<4>(stage, dst, pitch, nrows, n, lane);
+            else store_rows<2>(stage, dst, pitch, nrows, n, lane);
           }
-          put(w, c0);
+          __syncwarp();
+        };
+        uint32_t acc = 0;
+        if (kWide && r.red > kRun) {
+          constexpr int kMine = BN / per_chunk / kParts;  // chunks of this warp
+          uint32_t sum[kMine][16];
+  #pragma unroll
+          for (int i = 0; i < kMine; ++i)
+  #pragma unroll
+            for (int j = 0; j < 16; ++j) sum[i][j] = 0;
+          for (int k0 = 0; k0 < r.red; k0 += kRun) {
+            if (!(ok = accumulated(k0 / kRun, acc))) break;
+            const uint32_t from = tmem + acc * BN + lanes + part * per_chunk;
+  #pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+              uint32_t v[16];
+              tmem_load16(from + i * kParts * per_chunk, v);
+              tmem_wait();
+  #pragma unroll
+              for (int j = 0; j < 16; ++j)
+                sum[i][j] = __float_as_uint(__uint_as_float(sum[i][j]) + __uint_as_float(v[j]));
+            }
+            release(acc);
+          }
+          if (!ok) break;
+  #pragma unroll
+          for (int i = 0; i < kMine; ++i)
+            if ((i * kParts + part) * per_chunk < ncols && nrows > 0)
+              put(sum[i], (i * kParts + part) * per_chunk);
+        } else {
+          if (r.red > 0 && !(ok = accumulated(0, acc))) break;
+          const uint32_t from = tmem + acc * BN + lanes;
+          if constexpr (!kWide) {
+            if (!(ok = add_runs(r, from))) break;
+          }
+          for (int c0 = part * per_chunk; c0 < ncols && nrows > 0; c0 += kParts * per_chunk) {
+            uint32_t v[32], w[16];
+            if (r.red == 0) {
+  #pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = 0;
+            } else if constexpr (kWide) {
+              tmem_load16(from + c0, w);
+              tmem_wait();
+            } else {
+              tmem_load32(from + c0, v);
+              tmem_wait();
+              if (g.out_kind == LGBM_B200_DTYPE_BF16) {
+  #pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = pack2<true>(v[2 * i], v[2 * i + 1]);
+              } else {
+  #pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = pack2<false>(v[2 * i], v[2 * i + 1]);
+              }
+            }
+            put(w, c0);
+          }
+          if (r.red > 0) release(acc);
         }
-        if (r.red > 0) release(acc);
       }
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -1148,7 +1209,7 @@ EncodeTiled encoder() {
   return fn;
 }
 
-// A tensor, innermost axis first; boxes of `row` bytes (64 or 128, swizzled alike) x `box1`
+// A tensor, innermost axis first; boxes of `row` bytes (32, 64 or 128, swizzled alike) x `box1`
 // rows, zeros outside the tensor.
 bool encode(CUtensorMap* map, int32_t dtype, const void* base, int rank, const int64_t* dims,
             const int64_t* pitches, int box1, int row = 128) {
@@ -1164,7 +1225,9 @@ bool encode(CUtensorMap* map, int32_t dtype, const void* base, int rank, const i
                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                   (cuuint32_t)rank, const_cast<void*>(base), d, s, box, step,
                   CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  row == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                  : row == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                              : CU_TENSOR_MAP_SWIZZLE_32B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1339,10 +1402,12 @@ cudaError_t run_fused(const Operand& x, const Operand& w, const MatmulCall& c, M
   g.unit = unit(g.out, g.out_pitch);
   g.act = e.act;
   g.bias = e.bias;
-  g.bias_vec = aligned16(e.bias) && g.cols % 8 == 0;
   g.residual = e.residual;
   g.residual_pitch = e.residual_pitch;
   g.residual_unit = unit(e.residual, e.residual_pitch);
+  if (g.residual_unit == 16 &&
+      (reinterpret_cast<uintptr_t>(e.residual) | (uintptr_t)(e.residual_pitch * 2)) % 32 == 0)
+    g.residual_unit = 32;
   g.pre = e.pre;
   g.pre_pitch = pre_pitch(g.cols);
   auto go = [&](auto bn_c, auto ctas_c) -> cudaError_t {
@@ -1351,13 +1416,14 @@ cudaError_t run_fused(const Operand& x, const Operand& w, const MatmulCall& c, M
     FusedMaps maps;
     const int64_t da[3] = {c.inner, g.rows, 1}, pa[2] = {x.pitch, 0};
     const int64_t db[3] = {c.inner, c.outer, c.experts}, pb[2] = {w.pitch, w.pitch * c.outer};
-    bool fine = encode(&maps.a, c.dtype, x.p, 2, da, pa, kTileM) &&
-                encode(&maps.b, c.dtype, w.p, 3, db, pb, KIND == GATED ? BN / 2 : S::kCols);
+    bool fine =
+        encode(&maps.a, c.dtype, x.p, 2, da, pa, kTileM) &&
+        encode(&maps.b, c.dtype, w.p, 3, db, pb, KIND == GATED ? BN / 2 : S::kCols);
     maps.out = maps.pre = maps.a;  // not used unless set
     const int64_t dd[3] = {g.cols, g.rows, kHalves}, pd[2] = {g.out_pitch, 0};
-    if (g.unit == 16) fine = fine && encode(&maps.out, c.dtype, g.out, 2, dd, pd, 32, kStoreRow);
+    if (g.unit == 16) fine = fine && encode(&maps.out, c.dtype, g.out, 2, dd, pd, 32, S::kRowBytes);
     const int64_t pp[2] = {g.pre_pitch * kHalves, g.pre_pitch};
-    if (g.pre) fine = fine && encode(&maps.pre, c.dtype, g.pre, 3, dd, pp, 32, kStoreRow);
+    if (g.pre) fine = fine && encode(&maps.pre, c.dtype, g.pre, 3, dd, pp, 32, S::kRowBytes);
     if (!fine) return cudaErrorInvalidValue;
     g.idesc = instruction(c.dtype, false, false, S::kRows, BN);
     const int64_t nt = (g.cols + S::kOutCols - 1) / S::kOutCols;

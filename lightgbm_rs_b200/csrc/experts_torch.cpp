@@ -326,8 +326,8 @@ PyObject* grouped_matmul_backward(PyObject* const* a) {
 }
 
 // What a layer keeps for its gradient: [rows, width], gated [rows, 2, width], each row padded to
-// 16 bytes.
-int64_t saved_pitch(int64_t width) { return (width + 7) / 8 * 8; }
+// 32 bytes.
+int64_t saved_pitch(int64_t width) { return (width + 15) / 16 * 16; }
 
 Tensor make_saved(c10::Device dev, at::ScalarType type, int64_t rows, bool gated, int64_t width) {
   const int64_t ld = saved_pitch(width);
@@ -349,7 +349,7 @@ Tensor saved(const char* what, PyObject* o, const Matrix& like, int64_t rows, bo
   const bool fits =
       (width == 1 || t.stride(last) == 1) && (!gated || t.stride(1) == ld) &&
       (rows < 2 || t.stride(0) == halves * ld) &&
-      (rows == 0 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) &&
+      (rows == 0 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 32 == 0) &&
       // the padding of the last row is read too
       (t.storage_offset() + rows * halves * ld) * 2 <= (int64_t)t.storage().nbytes();
   if (fits) return t;

@@ -115,7 +115,7 @@ def grouped_linear(x, w, offsets, rows=None, bias=None, activation=None, residua
     their type. activation: None, "relu", "silu" or "gelu" (by the normal distribution function).
     Rows of no expert are the residual (0 without one). With save, (y, pre) for
     `grouped_linear_backward`: pre [M, outer] is what the activation was given, rounded to x's
-    type, its rows padded to 16 bytes (None without an activation)."""
+    type, its rows padded to 32 bytes (None without an activation)."""
     y, pre = _X.grouped_linear(x, w, offsets, rows, bias, _act("grouped_linear", activation),
                                residual, save)
     return (y, pre) if save else y
@@ -138,7 +138,7 @@ def grouped_gated(x, w, offsets, rows=None, activation="silu", save=False):
     and the last `hidden` columns of `grouped_matmul` with w [E, 2 * hidden, inner]; activation as
     for `grouped_linear`. Rows of no expert are 0. With save, (h, pre) for
     `grouped_gated_backward`: pre [M, 2, hidden] is gate and up rounded to x's type, its rows
-    padded to 16 bytes."""
+    padded to 32 bytes."""
     h, pre = _X.grouped_gated(x, w, offsets, rows, _act("grouped_gated", activation), save)
     return (h, pre) if save else h
 
