@@ -116,6 +116,30 @@ struct Raw<T, 1> {
   }
 };
 
+// 16 bytes from any even address: the one or two aligned pieces that hold it, loaded by
+// stage_load, shifted here. (Eight loads of 2 bytes a piece pass through L1 one by one.)
+struct StagePair { uint4 a, b; };
+__device__ __forceinline__ StagePair stage_load(const char* p, int left) {
+  const int s = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+  const uint4* q = reinterpret_cast<const uint4*>(p - s);
+  return {__ldg(q), __ldg(q + (s + min(left, 16) > 16))};
+}
+__device__ __forceinline__ uint4 stage_shift(const StagePair& v, int s, int left) {
+  uint32_t w[8] = {v.a.x, v.a.y, v.a.z, v.a.w, v.b.x, v.b.y, v.b.z, v.b.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = s & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = s & 4 ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = s & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+  if (left < 16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = left >= 4 * i + 4 ? w[i] : left > 4 * i ? w[i] & 0xFFFFu : 0;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 inline int elem_size(int32_t dtype) { return dtype == LGBM_B200_DTYPE_F32 ? 4 : 2; }
