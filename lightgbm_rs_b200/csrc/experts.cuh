@@ -25,6 +25,36 @@ namespace experts {
 constexpr int kMaxExperts = 512;
 constexpr int kMaxChosen = 16;
 
+// Launches of a layer follow one another within microseconds, and the next kernel may start while
+// the last one ends: it sets itself up, and waits in wait_for_stream() before it touches anything
+// that work before it in the stream reads or writes. Every thread of such a kernel calls it once;
+// let_next_start() says that no more blocks of this kernel are to come.
+__device__ __forceinline__ void wait_for_stream() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <typename... P, typename... A>
+cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st,
+                          const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  // by address: an argument of 30 KB is not copied on its way
+  auto go = [&](const P&... exact) {
+    void* a[] = {const_cast<void*>(static_cast<const void*>(&exact))...};
+    return cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kernel), a);
+  };
+  return go(args...);
+}
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
 template <>

@@ -84,6 +84,8 @@ __global__ void __launch_bounds__(kThreads)
                  int64_t pre_pitch, int act, int64_t rows, int hidden, T* __restrict__ dpre,
                  int64_t dpre_pitch) {
   constexpr int kLanes = 1 << LOG;
+  wait_for_stream();
+  let_next_start();
   const int lane = threadIdx.x % kLanes;
   const int64_t r0 = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
   const bool here = r0 < rows;
@@ -203,6 +205,8 @@ __global__ void __launch_bounds__(kThreads, 3)
                   int64_t rows, int64_t rows_a_block, int outer, int lanes, T* __restrict__ dpre,
                   int64_t dpre_pitch, float* __restrict__ sums) {
   __shared__ float part[kThreads / 32][32 * 8];
+  wait_for_stream();
+  let_next_start();
   const int lane = threadIdx.x % lanes, sub = threadIdx.x / lanes, subs = kThreads / lanes;
   const int64_t c = ((int64_t)blockIdx.x * lanes + lane) * 8;
   const int n = c < outer ? (int)min((int64_t)8, outer - c) : 0;
@@ -300,6 +304,8 @@ __global__ void __launch_bounds__(kThreads)
     k_join_bias(const float* __restrict__ sums, const int32_t* __restrict__ offsets, int64_t rows,
                 int64_t rows_a_block, int64_t blocks, int outer, T* __restrict__ dbias) {
   __shared__ float part[kThreads];
+  wait_for_stream();
+  let_next_start();
   const int e = blockIdx.y, j = threadIdx.x % 32, k = threadIdx.x / 32;
   const int64_t n = (int64_t)blockIdx.x * 32 + j;
   const int64_t lo = min(max((int64_t)offsets[e], (int64_t)0), rows),
@@ -326,11 +332,11 @@ cudaError_t gated_grad(const void* dh, int64_t dh_pitch, const void* pre, int32_
     constexpr int kRows = kThreads >> decltype(log)::value;
     const int64_t blocks = (rows + kRows - 1) / kRows;
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-    k_gated_grad<T, decltype(log)::value, decltype(vec)::value, decltype(odd)::value>
-        <<<(unsigned)blocks, kThreads, 0, st>>>(static_cast<const T*>(dh), dh_pitch,
-                                                static_cast<const T*>(pre), pre_pitch(hidden), act,
-                                                rows, hidden, static_cast<T*>(dpre), dpre_pitch);
-    return cudaGetLastError();
+    return launch_behind(
+        k_gated_grad<T, decltype(log)::value, decltype(vec)::value, decltype(odd)::value>,
+        dim3((unsigned)blocks), kThreads, st, static_cast<const T*>(dh), dh_pitch,
+        static_cast<const T*>(pre), pre_pitch(hidden), act, rows, hidden, static_cast<T*>(dpre),
+        dpre_pitch);
   };
   auto with_lanes = [&](auto vec, auto odd) {
     if (hidden <= 16) return go(std::integral_constant<int, 1>(), vec, odd);
@@ -351,25 +357,24 @@ cudaError_t linear_grad(const LinearGrad& c, cudaStream_t st) {
   const SumShape s = sum_shape(c.rows, c.outer);
   const dim3 grid((unsigned)s.slabs, (unsigned)s.blocks);
   auto go = [&](auto vec, auto through) {
-    k_linear_grad<T, decltype(vec)::value, decltype(through)::value><<<grid, kThreads, 0, st>>>(
+    return launch_behind(
+        k_linear_grad<T, decltype(vec)::value, decltype(through)::value>, grid, kThreads, st,
         static_cast<const T*>(c.dy), c.dy_pitch, static_cast<const T*>(c.pre), pre_pitch(c.outer),
         c.act, c.offsets, c.experts, c.rows, s.rows, c.outer, s.lanes, static_cast<T*>(c.dpre),
         c.dpre_pitch, c.dbias ? c.sums : nullptr);
   };
-  if (aligned16(c.dy) && c.dy_pitch % 8 == 0)
-    c.dpre ? go(std::true_type(), std::true_type()) : go(std::true_type(), std::false_type());
-  else
-    c.dpre ? go(std::false_type(), std::true_type()) : go(std::false_type(), std::false_type());
-  const cudaError_t err = cudaGetLastError();
+  const std::true_type yes;
+  const std::false_type no;
+  const cudaError_t err = aligned16(c.dy) && c.dy_pitch % 8 == 0
+                              ? (c.dpre ? go(yes, yes) : go(yes, no))
+                              : (c.dpre ? go(no, yes) : go(no, no));
   if (err != cudaSuccess || !c.dbias) return err;
   const dim3 joins((unsigned)((c.outer + 31) / 32), (unsigned)c.experts);
   if (c.grad_dtype == LGBM_B200_DTYPE_F32)
-    k_join_bias<float><<<joins, kThreads, 0, st>>>(c.sums, c.offsets, c.rows, s.rows, s.blocks,
-                                                   c.outer, static_cast<float*>(c.dbias));
-  else
-    k_join_bias<T><<<joins, kThreads, 0, st>>>(c.sums, c.offsets, c.rows, s.rows, s.blocks,
-                                               c.outer, static_cast<T*>(c.dbias));
-  return cudaGetLastError();
+    return launch_behind(k_join_bias<float>, joins, kThreads, st, c.sums, c.offsets, c.rows,
+                         s.rows, s.blocks, c.outer, static_cast<float*>(c.dbias));
+  return launch_behind(k_join_bias<T>, joins, kThreads, st, c.sums, c.offsets, c.rows, s.rows,
+                       s.blocks, c.outer, static_cast<T*>(c.dbias));
 }
 
 }  // namespace

@@ -223,6 +223,8 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   uint8_t* ring = smem + S::ring(g.panel) + warp * kRing * kStageBytes;
   const int gq = lane >> 2, tq = lane & 3;  // row and column quad of the matrix fragments
 
+  wait_for_stream();
+  let_next_start();
   // The item of this block: rows [begin, begin + n) of one expert. Items are numbered expert
   // by expert, then the rows past the last offset and those before the first (expert >= experts:
   // zeros).
@@ -680,12 +682,14 @@ cudaError_t launch_few_shape(FewArgs g, cudaStream_t st) {
   cfg.blockDim = dim3(kFewThreads, 1, 1);
   cfg.dynamicSmemBytes = (size_t)S::total(g.panel);
   cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)split;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = split > 1 ? 1 : 0;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see launch_behind
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, k_grouped_few<S>, g);
 }
 

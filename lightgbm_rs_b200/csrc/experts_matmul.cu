@@ -560,6 +560,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
   } else if (warp == 2) {
+    wait_for_stream();
     // The groups' rows, clamped (off[i] to off[i + 1]; overlaps of offsets that decrease are
     // cut off), and the first tile of every group. The rows before the first offset are a group
     // of their own and so are those past the last; WEIGHT needs neither.
@@ -611,6 +612,8 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
     }
     if (lane == 0) cum[groups] = carry;
   }
+  if (warp != 2) wait_for_stream();
+  let_next_start();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if constexpr (CTAS == 2) cluster_sync();  // the other CTA's barriers are set up too
@@ -1124,6 +1127,8 @@ __global__ void __launch_bounds__(256)
                  int64_t pitch, const int32_t* __restrict__ index, char* __restrict__ dst,
                  int dst_bytes) {
   constexpr int kLanes = 1 << LOG, kRunOf = LOG == 5 ? kStageRun : 2, kStep = 16 * kLanes;
+  wait_for_stream();
+  let_next_start();
   const int lane = threadIdx.x % kLanes;
   const int64_t r = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   if (r >= rows) return;
@@ -1240,12 +1245,14 @@ cudaError_t launch_tiles(const MapsOf<KIND>& maps, MatArgs g, int64_t most_tiles
   cfg.blockDim = dim3(S::kThreads, 1, 1);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = CTAS;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = CTAS == 2 ? 1 : 0;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see launch_behind
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CTAS;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CTAS == 2 ? 2 : 1;
   int most = most_ready[dev].load(std::memory_order_acquire);
   if (most == 0) {
     err = cudaFuncSetAttribute(k_grouped_matmul<KIND, BN, CTAS>,
@@ -1285,10 +1292,9 @@ cudaError_t stage(Operand& o, int64_t src_rows, int64_t rows, int width, const i
     constexpr int kRows = 256 >> decltype(log)::value;
     const int64_t blocks = (rows + kRows - 1) / kRows;
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-    k_stage_rows<decltype(unit)::value, decltype(log)::value><<<(unsigned)blocks, 256, 0, st>>>(
-        static_cast<const char*>(o.p), src_rows, rows, width * 2, o.pitch * 2, index, dst,
-        (int)(dst_pitch * 2));
-    return cudaGetLastError();
+    return launch_behind(k_stage_rows<decltype(unit)::value, decltype(log)::value>,
+                         dim3((unsigned)blocks), 256, st, static_cast<const char*>(o.p), src_rows,
+                         rows, width * 2, o.pitch * 2, index, dst, (int)(dst_pitch * 2));
   };
   auto with_lanes = [&](auto unit) {
     if (dst_pitch <= 32) return go(unit, std::integral_constant<int, 1>());
@@ -1418,6 +1424,8 @@ cudaError_t run_fused(const Operand& x, const Operand& w, const MatmulCall& c, M
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
     k_join_parts(const float* part, int parts, int64_t count, int64_t total, T* out) {
+  wait_for_stream();
+  let_next_start();
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
   if (i >= total) return;
   const int64_t e = i / count;
@@ -1442,10 +1450,10 @@ cudaError_t join_parts(const float* part, int parts, int64_t count, int experts,
   const int64_t total = count * experts;
   const auto blocks = [&](int v) { return (unsigned)((total / v + 255) / 256); };
   if (count % 4 == 0)
-    k_join_parts<T, 4><<<blocks(4), 256, 0, st>>>(part, parts, count, total, out);
-  else
-    k_join_parts<T, 1><<<blocks(1), 256, 0, st>>>(part, parts, count, total, out);
-  return cudaGetLastError();
+    return launch_behind(k_join_parts<T, 4>, dim3(blocks(4)), 256, st, part, parts, count, total,
+                         out);
+  return launch_behind(k_join_parts<T, 1>, dim3(blocks(1)), 256, st, part, parts, count, total,
+                       out);
 }
 
 }  // namespace

@@ -184,6 +184,8 @@ __global__ void __launch_bounds__(kThreads)
     k_sum_squares(const __grid_constant__ Table<ITEMS> t, double* __restrict__ partial,
                   Entry* __restrict__ entries, int32_t* __restrict__ last) {
   __shared__ double shared[kThreads / 32];
+  wait_for_stream();
+  let_next_start();
   for (int i = blockIdx.x * kThreads + threadIdx.x; i < t.items; i += gridDim.x * kThreads)
     entries[i] = {t.in[i], t.out[i], t.bytes[i], t.first[i], t.dtype[i]};
   const int windows = t.first[t.items];
@@ -228,6 +230,8 @@ __device__ __forceinline__ float norm_of(const double* partial, int count, doubl
 __global__ void __launch_bounds__(kThreads)
     k_norm(const double* __restrict__ partial, int count, float* __restrict__ norm) {
   __shared__ double shared[kThreads / 32];
+  wait_for_stream();
+  let_next_start();
   const float n = norm_of(partial, count, shared);
   if (threadIdx.x == 0) *norm = n;
 }
@@ -296,6 +300,8 @@ __global__ void __launch_bounds__(kThreads)
             float* __restrict__ norm) {
   __shared__ double shared[kThreads / 32];
   __shared__ float factor;
+  wait_for_stream();
+  let_next_start();
   int item = last[blockIdx.x];
   Entry t = entries[item];
   const float n = norm_of(partial, count, shared);
@@ -330,6 +336,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
   __shared__ double sum;
   __shared__ float factor;
   cg::cluster_group cluster = cg::this_cluster();
+  wait_for_stream();
+  let_next_start();
   const int windows = t.first[t.items];
   const int begin = share(windows, blockIdx.x, gridDim.x),
             count = share(windows, blockIdx.x + 1, gridDim.x) - begin;
@@ -393,19 +401,21 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
-void run_small(const Table<kFewItems>& t, const NormCall& c, cudaStream_t st) {
+cudaError_t run_small(const Table<kFewItems>& t, const NormCall& c, cudaStream_t st) {
   const int blocks = std::min(kSmallBlocks, t.first[t.items]);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)blocks, 1, 1);
   cfg.blockDim = dim3(kSmallThreads, 1, 1);
   cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)blocks;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, k_small, t, (int)c.scale, c.max_norm, c.norm);
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see launch_behind
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)blocks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, k_small, t, (int)c.scale, c.max_norm, c.norm);
 }
 
 int64_t launches_of(int64_t tensors) { return (tensors + kItems - 1) / kItems; }
@@ -456,32 +466,31 @@ cudaError_t run(const NormCall& c, cudaStream_t st) {
         t.items = items;
         t.first[items] = windows;
       }
-      go(windows);
-      const cudaError_t err = cudaGetLastError();
+      const cudaError_t err = go(windows);
       if (err != cudaSuccess) return err;
       ++launch;
     }
     return cudaSuccess;
   };
   if constexpr (ITEMS == kFewItems)
-    if (is_small(c.tensors, c.count)) return each([&](int) { run_small(t, c, st); }, true);
+    if (is_small(c.tensors, c.count)) return each([&](int) { return run_small(t, c, st); }, true);
   cudaError_t err = each(
       [&](int windows) {
-        k_sum_squares<ITEMS><<<shape(windows), kThreads, 0, st>>>(
-            t, partial + total, entries + launch * kItems, last + launch * kGrid);
+        const int at = total;
         total += shape(windows);
+        return launch_behind(k_sum_squares<ITEMS>, dim3((unsigned)shape(windows)), kThreads, st, t,
+                             partial + at, entries + launch * kItems, last + launch * kGrid);
       },
       true);
   if (err != cudaSuccess) return err;
   if (!c.scale || total == 0) {
-    k_norm<<<1, kThreads, 0, st>>>(partial, total, c.norm);
-    return cudaGetLastError();
+    return launch_behind(k_norm, dim3(1), kThreads, st, partial, total, c.norm);
   }
   return each(
       [&](int windows) {
-        k_scale<<<shape(windows), kThreads, 0, st>>>(entries + launch * kItems,
-                                                     last + launch * kGrid, windows, partial,
-                                                     total, c.max_norm, launch == 0 ? c.norm : nullptr);
+        return launch_behind(k_scale, dim3((unsigned)shape(windows)), kThreads, st,
+                             entries + launch * kItems, last + launch * kGrid, windows, partial,
+                             total, c.max_norm, launch == 0 ? c.norm : nullptr);
       },
       false);
 }
