@@ -322,130 +322,139 @@ __device__ __forceinline__ void tile_of(int t, int mt, int nt, int band, int& m,
 template <int KIND, int BN, int CTAS>
 struct Shape {
   static constexpr bool kFused = KIND == LINEAR || KIND == GATED;
-  static constexpr int kStoreWarps = KIND == WEIGHT_F32 || kFused ? 16 : 8;
+  // Narrow tiles are short of work for one CTA, whose stages of loading, multiplying and storing
+  // wait for one another: two share an SM.
+  static constexpr int kPerSm = BN == 64 ? 2 : 1;
+  static constexpr int kStoreWarps = BN > 64 && (KIND == WEIGHT_F32 || kFused) ? 16 : 8;
   static constexpr int kRun = KIND == WEIGHT_F32 ? 768 : 4096;  // see "Precision" above
   static constexpr int kThreads = 64 + 32 * kStoreWarps;
   static constexpr int kOutCols = KIND == GATED ? BN / 2 : BN;  // columns of the result
   // bytes of a row of a staging block; LINEAR, GATED: so that narrow tiles occupy all warps too
-  static constexpr int kRowBytes = kFused && kOutCols < 128 ? 32 : kStoreRow;
-  static constexpr int kStoreBytes = kStoreWarps * 32 * kRowBytes;
+  static constexpr int kRowBytes = kFused && kOutCols < 8 * kStoreWarps ? 32 : kStoreRow;
+  static constexpr int kBiasBytes = KIND == LINEAR ? kStoreWarps * 128 : 0;
+  static constexpr int kStoreBytes = kStoreWarps * 32 * kRowBytes + kBiasBytes;
   static constexpr int kRows = kTileM * CTAS;
   static constexpr int kCols = BN / CTAS;  // columns of B that a CTA loads
   static constexpr int kStageBytes = (kTileM + kCols) * 128;
-  static constexpr int kStages = (212992 - kStoreBytes) / kStageBytes;  // 3 to 8
+  // what tables, barriers and alignment leave of 227 KB: 3 to 8
+  static constexpr int kStages = (212992 / kPerSm - kStoreBytes) / kStageBytes;
   static constexpr int kTmemCols = 2 * BN;                              // two accumulators
   static constexpr int kBand = kBandRows / kRows;
   static constexpr int kSmem =
       1024 + kStages * kStageBytes + kStoreBytes + 8 * kGroupSlots + 512;
 };
 
-// Where piece `p` (16 bytes) of row `row` lies in a staging block of ROW-byte rows: TMA's swizzle
-// of rows of 64 bytes, and for the others the same idea: eight rows' piece p hit all banks.
-template <int ROW = kStoreRow>
+// Where piece `p` (16 bytes) of row `row` lies in a staging block of rows of 32 or 64 bytes: TMA's
+// swizzle of that width.
+template <int ROW>
 __device__ __forceinline__ uint32_t staged(int row, int p) {
-  constexpr int kShift = ROW == 128 ? 0 : ROW == 64 ? 1 : 2;
+  constexpr int kShift = ROW == 64 ? 1 : 2;
   return row * ROW + ((p ^ ((row >> kShift) & (ROW / 16 - 1))) << 4);
 }
 
 // One 32-row block of a storing warp, from its staging block to `dst` (row pitch in bytes),
 // `bytes` of each row, UNIT bytes at a time.
-template <int UNIT, int ROW = kStoreRow>
+template <int UNIT>
 __device__ __forceinline__ void store_rows(uint32_t stage, char* dst, int64_t pitch, int nrows,
                                            int bytes, int lane) {
-  constexpr int kLanes = ROW / UNIT < 32 ? ROW / UNIT : 32;  // of a row
-  constexpr int kPerStep = 32 / kLanes;                      // rows
-  auto lot = [&](int at) {  // the columns of one step
-    if (at + UNIT > bytes) return;
-    char* to = dst + (lane / kLanes) * pitch + at;
-#pragma unroll 8
-    for (int i0 = 0; i0 < 32; i0 += kPerStep) {
-      const int i = i0 + lane / kLanes;
-      if (i < nrows) {
-        const uint32_t from = stage + staged<ROW>(i, at >> 4) + (at & 15);
-        if constexpr (UNIT == 16) {
-          uint32_t w[4];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(from)
-                       : "memory");
-          *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else if constexpr (UNIT == 8) {
-          uint32_t w[2];
-          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
-                       : "=r"(w[0]), "=r"(w[1])
-                       : "r"(from)
-                       : "memory");
-          *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-        } else if constexpr (UNIT == 4) {
-          uint32_t w;
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
-          *reinterpret_cast<uint32_t*>(to) = w;
-        } else {
-          uint16_t w;
-          asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(from) : "memory");
-          *reinterpret_cast<uint16_t*>(to) = w;
-        }
-      }
-      to += kPerStep * pitch;
-    }
-  };
-  lot(lane % kLanes * UNIT);
-  if constexpr (ROW / UNIT > 32) lot((lane + 32) * UNIT);
-}
-
-// The way back, for rows that do not start at 16 bytes: a 32-row block of `src` to a staging block,
-// eight loads at a time.
-template <int UNIT, int ROW>
-__device__ __forceinline__ void load_rows(uint32_t stage, const char* src, int64_t pitch,
-                                          int nrows, int bytes, int lane) {
-  constexpr int kLanes = ROW / UNIT;     // of a row
-  constexpr int kPerStep = 32 / kLanes;  // rows
-  constexpr int kSteps = 8;              // at a time
-  using T =
-      std::conditional_t<UNIT == 8, uint2, std::conditional_t<UNIT == 4, uint32_t, uint16_t>>;
+  constexpr int kLanes = kStoreRow / UNIT;  // of a row
+  constexpr int kPerStep = 32 / kLanes;     // rows
   const int at = lane % kLanes * UNIT;
   if (at + UNIT > bytes) return;
-  const char* from = src + (lane / kLanes) * pitch + at;
-#pragma unroll 1
-  for (int i0 = 0; i0 < 32; i0 += kSteps * kPerStep) {
-    T v[kSteps];
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int row = i0 + i * kPerStep + lane / kLanes;
-      if (row < nrows)
-        v[i] = __ldg(reinterpret_cast<const T*>(from + (int64_t)(i0 + i * kPerStep) * pitch));
+  char* to = dst + (lane / kLanes) * pitch + at;
+#pragma unroll 8
+  for (int i0 = 0; i0 < 32; i0 += kPerStep) {
+    const int i = i0 + lane / kLanes;
+    if (i < nrows) {
+      const uint32_t from = stage + staged<kStoreRow>(i, at >> 4) + (at & 15);
+      if constexpr (UNIT == 16) {
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(from)
+                     : "memory");
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else if constexpr (UNIT == 8) {
+        uint32_t w[2];
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                     : "=r"(w[0]), "=r"(w[1])
+                     : "r"(from)
+                     : "memory");
+        *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+      } else if constexpr (UNIT == 4) {
+        uint32_t w;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
+        *reinterpret_cast<uint32_t*>(to) = w;
+      } else {
+        uint16_t w;
+        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(from) : "memory");
+        *reinterpret_cast<uint16_t*>(to) = w;
+      }
     }
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int row = i0 + i * kPerStep + lane / kLanes;
-      const uint32_t to = stage + staged<ROW>(row, at >> 4) + (at & 15);
-      if (row < nrows) {
-        if constexpr (UNIT == 8)
-          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(v[i].x), "r"(v[i].y)
-                       : "memory");
-        else if constexpr (UNIT == 4)
-          asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(v[i]) : "memory");
-        else
-          asm volatile("st.shared.b16 [%0], %1;" ::"r"(to), "h"(v[i]) : "memory");
+    to += kPerStep * pitch;
+  }
+}
+
+// Between a staging block and rows that are fewer than 32 or do not start at 16 bytes, a step of
+// UNIT bytes a lane at a time: few registers, which the storing warps of LINEAR are short of.
+template <int UNIT, int ROW, bool LOAD>
+__device__ __forceinline__ void move_rows(uint32_t stage, char* rows, int64_t pitch, int nrows,
+                                          int bytes, int lane) {
+  constexpr int kLanes = ROW / UNIT;     // of a row
+  constexpr int kPerStep = 32 / kLanes;  // rows
+  const int at = lane % kLanes * UNIT;
+  if (at + UNIT > bytes) return;
+  char* p = rows + (lane / kLanes) * pitch + at;
+#pragma unroll 2
+  for (int i = lane / kLanes; i < nrows; i += kPerStep, p += kPerStep * pitch) {
+    const uint32_t s = stage + staged<ROW>(i, at >> 4) + (at & 15);
+    if constexpr (UNIT == 16) {
+      static_assert(!LOAD, "rows at 16 bytes are read ahead");
+      uint32_t w[4];
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                   : "r"(s)
+                   : "memory");
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else if constexpr (UNIT == 8) {
+      uint2 w;
+      if constexpr (LOAD) {
+        w = __ldg(reinterpret_cast<const uint2*>(p));
+        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(s), "r"(w.x), "r"(w.y) : "memory");
+      } else {
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "r"(s) : "memory");
+        *reinterpret_cast<uint2*>(p) = w;
+      }
+    } else if constexpr (UNIT == 4) {
+      uint32_t w;
+      if constexpr (LOAD) {
+        w = __ldg(reinterpret_cast<const uint32_t*>(p));
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(s), "r"(w) : "memory");
+      } else {
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(s) : "memory");
+        *reinterpret_cast<uint32_t*>(p) = w;
+      }
+    } else {
+      uint16_t w;
+      if constexpr (LOAD) {
+        w = __ldg(reinterpret_cast<const uint16_t*>(p));
+        asm volatile("st.shared.b16 [%0], %1;" ::"r"(s), "h"(w) : "memory");
+      } else {
+        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(s) : "memory");
+        *reinterpret_cast<uint16_t*>(p) = w;
       }
     }
   }
 }
-
-// Both out of line: inline their loops' addresses spilled.
-template <int ROW>
-__device__ __noinline__ void load_odd_rows(int unit, uint32_t stage, const char* src, int64_t pitch,
-                                           int nrows, int bytes, int lane) {
-  if (unit == 8) load_rows<8, ROW>(stage, src, pitch, nrows, bytes, lane);
-  else if (unit == 4) load_rows<4, ROW>(stage, src, pitch, nrows, bytes, lane);
-  else load_rows<2, ROW>(stage, src, pitch, nrows, bytes, lane);
-}
-template <int ROW>
-__device__ __noinline__ void store_odd_rows(int unit, uint32_t stage, char* dst, int64_t pitch,
-                                            int nrows, int bytes, int lane) {
-  if (unit == 8) store_rows<8, ROW>(stage, dst, pitch, nrows, bytes, lane);
-  else if (unit == 4) store_rows<4, ROW>(stage, dst, pitch, nrows, bytes, lane);
-  else store_rows<2, ROW>(stage, dst, pitch, nrows, bytes, lane);
+template <int ROW, bool LOAD>
+__device__ __forceinline__ void move_rows(int unit, uint32_t stage, char* rows, int64_t pitch,
+                                          int nrows, int bytes, int lane) {
+  if constexpr (!LOAD) {
+    if (unit == 16) return move_rows<16, ROW, LOAD>(stage, rows, pitch, nrows, bytes, lane);
+  }
+  if (unit == 8) move_rows<8, ROW, LOAD>(stage, rows, pitch, nrows, bytes, lane);
+  else if (unit == 4) move_rows<4, ROW, LOAD>(stage, rows, pitch, nrows, bytes, lane);
+  else move_rows<2, ROW, LOAD>(stage, rows, pitch, nrows, bytes, lane);
 }
 
 // 32 bytes of a row that starts at `unit` (16 or 32) bytes; if there are fewer, `bytes` of them (a
@@ -466,28 +475,18 @@ __device__ __forceinline__ void load32(uint32_t* w, const char* p, int unit, int
 }
 
 // Two 16-bit values of a word as f32.
-__device__ __forceinline__ float2 unpack2(uint32_t w, bool bf16) {
-  if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (BF16)
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
-__device__ __forceinline__ void add16(float (&f)[16], const uint32_t* w, bool bf16) {
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&f)[16]) {
+  uint32_t v[16];
+  tmem_load16(addr, v);
+  tmem_wait();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 v = unpack2(w[i], bf16);
-    f[2 * i] += v.x;
-    f[2 * i + 1] += v.y;
-  }
-}
-__device__ __forceinline__ void pack16(const float (&f)[16], bool bf16, uint32_t (&w)[8]) {
-  if (bf16) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      w[i] = pack2<true>(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      w[i] = pack2<false>(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]));
-  }
+  for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
 }
 
 struct Maps {
@@ -501,7 +500,7 @@ template <int KIND>
 using MapsOf = std::conditional_t<KIND == LINEAR || KIND == GATED, FusedMaps, Maps>;
 
 template <int KIND, int BN, int CTAS>
-__global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
+__global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, BN, CTAS>::kPerSm)
     k_grouped_matmul(const __grid_constant__ MapsOf<KIND> maps, const MatArgs g) {
   using S = Shape<KIND, BN, CTAS>;
   constexpr int MODE = KIND == WEIGHT_F32 ? (int)WEIGHT : S::kFused ? (int)FORWARD : KIND;
@@ -831,155 +830,198 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
       }
       return true;
     };
-    for (int t = first; ok && t < tiles; t += step) {
-      const Tile r = decode(t);
-      const int row0 = r.m0 + quarter * 32;
-      if constexpr (S::kFused) {
-        // A chunk of 16 or 32 columns at a time, each lane its row: read from tensor memory,
-        // finished in registers, and through the warp's staging block to the result.
-        constexpr int ROW = S::kRowBytes, kChunk = ROW / 2, kHalves = KIND == GATED ? 2 : 1;
-        const int nrows = min(32, r.m_end - row0);
-        const int ncols = nrows > 0 ? min(S::kOutCols, g.cols - r.n0) : 0;
-        const bool live = r.red > 0, bf16 = g.out_kind == LGBM_B200_DTYPE_BF16;
-        const bool whole = nrows == 32;
-        // the staging block, when the last store has read it
-        auto free_block = [&] {
+    if constexpr (S::kFused) {
+      // A chunk of 16 or 32 columns at a time, each lane its row: read from tensor memory, finished
+      // in registers, and through the warp's staging block to the result. One body for every type
+      // and activation: with tests inside, a chunk took 400 instructions beside the activation's.
+      constexpr int ROW = S::kRowBytes, kChunk = ROW / 2;
+      constexpr uint32_t kSwizzle = ROW / 16 - 1;
+      const uint32_t own = stage + lane * ROW, swap = (lane >> (ROW == 64 ? 1 : 2)) & kSwizzle;
+      float* const bias_at = reinterpret_cast<float*>(
+          smem + kStages * S::kStageBytes + S::kStoreBytes - S::kBiasBytes + (warp - 2) * 128);
+      auto store_tiles = [&](auto bf16_c, auto act_c) {
+        constexpr bool BF16 = decltype(bf16_c)::value;
+        using A = Act<decltype(act_c)::value>;
+        // 16 columns' values into pieces 2 i and 2 i + 1 of this lane's row
+        auto put = [&](int i, const float* f) {
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            w[j] = pack2<BF16>(__float_as_uint(f[2 * j]), __float_as_uint(f[2 * j + 1]));
+          store_piece(own + (((2 * i) ^ swap) << 4), w[0], w[1], w[2], w[3]);
+          store_piece(own + (((2 * i + 1) ^ swap) << 4), w[4], w[5], w[6], w[7]);
+        };
+        auto free_block = [&] {  // the last bulk store has read it
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
         };
-        // the block to columns c of the result (saved < 0) or of a half of the saved values
-        auto leave = [&](int c, int saved) {
-          if (whole && (saved >= 0 || g.unit == 16)) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-              if (saved >= 0)
+        for (int t = first; t < tiles; t += step) {
+          const Tile r = decode(t);
+          const int row0 = r.m0 + quarter * 32, nrows = min(32, r.m_end - row0);
+          const int ncols = nrows > 0 ? min(S::kOutCols, g.cols - r.n0) : 0;
+          const bool live = r.red > 0;
+          const bool whole = nrows == 32;
+          // the block to columns c of half `half` of the saved values
+          auto save = [&](int c, int half) {
+            if (whole) {
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) {
                 asm volatile(
                     "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], "
                     "[%4];" ::"l"(&maps.pre),
-                    "r"(r.n0 + c), "r"(row0), "r"(saved), "r"(stage)
+                    "r"(r.n0 + c), "r"(row0), "r"(half), "r"(stage)
                     : "memory");
-              else
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+              }
+            } else {
+              constexpr int kHalves = KIND == GATED ? 2 : 1;
+              __syncwarp();
+              move_rows<16, ROW, false>(stage,
+                                  static_cast<char*>(g.pre) +
+                                      (((int64_t)row0 * kHalves + half) * g.pre_pitch + r.n0 + c) *
+                                          2,
+                                  kHalves * g.pre_pitch * 2, nrows,
+                                  (min(kChunk, ncols - c) * 2 + 15) / 16 * 16, lane);
+            }
+          };
+          float bias = 0.0f;  // of column c + lane
+          uint32_t residual[kChunk / 2];
+          auto fetch = [&](int c) {  // what columns c add, ahead of use
+            if (KIND != LINEAR || c >= ncols) return;
+            if (g.bias) {
+              uint32_t v = 0;
+              if (live && lane < min(kChunk, ncols - c))
+                v = __ldg(static_cast<const uint16_t*>(g.bias) + (int64_t)r.expert * g.cols + r.n0 +
+                          c + lane);
+              bias = unpack2<BF16>(v).x;
+            }
+            if (g.residual && g.residual_unit >= 16 && lane < nrows) {
+              const char* p = static_cast<const char*>(g.residual) +
+                              ((row0 + lane) * g.residual_pitch + r.n0 + c) * 2;
+#pragma unroll
+              for (int i = 0; i < kChunk / 16; ++i)
+                load32(residual + 8 * i, p + 32 * i, g.residual_unit, (ncols - c) * 2 - 32 * i);
+            }
+          };
+          fetch(part * kChunk);
+          uint32_t acc = 0;
+          if (live && !accumulated(0, acc)) return false;
+          const uint32_t from = tmem + acc * BN + lanes;
+          if (!add_runs(r, from)) return false;
+#pragma unroll 1
+          for (int c = part * kChunk; c < ncols; c += kParts * kChunk) {
+            if (KIND == LINEAR && g.bias) {
+              if (lane < kChunk) bias_at[lane] = bias;
+              __syncwarp();
+            }
+            // columns c + 16 i of a half's products, with the bias
+            auto load = [&](int half, int i, float (&f)[16]) {
+              if (live) {
+                tmem_load(from + half * S::kOutCols + c + 16 * i, f);
+              } else {  // rows of no expert
+#pragma unroll
+                for (int j = 0; j < 16; ++j) f[j] = 0.0f;
+              }
+              if (KIND == LINEAR && g.bias) {
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                  const float4 b = *reinterpret_cast<const float4*>(bias_at + 16 * i + j);
+                  f[j] += b.x;
+                  f[j + 1] += b.y;
+                  f[j + 2] += b.z;
+                  f[j + 3] += b.w;
+                }
+              }
+            };
+            if (g.pre) {
+#pragma unroll 1
+              for (int half = 0; half < (KIND == GATED ? 2 : 1); ++half) {
+                free_block();
+#pragma unroll
+                for (int i = 0; i < kChunk / 16; ++i) {
+                  float f[16];
+                  load(half, i, f);
+                  put(i, f);
+                }
+                save(c, half);
+              }
+            }
+            free_block();
+            if (KIND == LINEAR && g.residual && g.residual_unit < 16) {
+              move_rows<ROW, true>(g.residual_unit, stage,
+                                   const_cast<char*>(static_cast<const char*>(g.residual)) +
+                                       ((int64_t)row0 * g.residual_pitch + r.n0 + c) * 2,
+                                   g.residual_pitch * 2, nrows, min(kChunk, ncols - c) * 2, lane);
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < kChunk / 8; ++i)
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(residual[4 * i]), "=r"(residual[4 * i + 1]),
+                               "=r"(residual[4 * i + 2]), "=r"(residual[4 * i + 3])
+                             : "r"(own + ((i ^ swap) << 4))
+                             : "memory");
+            }
+#pragma unroll
+            for (int i = 0; i < kChunk / 16; ++i) {
+              float f[16];
+              load(0, i, f);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) f[j] = A::value(f[j]);
+              if constexpr (KIND == GATED) {
+                float up[16];
+                load(1, i, up);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) f[j] *= up[j];
+              } else if (g.residual) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const float2 v = unpack2<BF16>(residual[8 * i + j]);
+                  f[2 * j] += v.x;
+                  f[2 * j + 1] += v.y;
+                }
+              }
+              put(i, f);
+            }
+            fetch(c + kParts * kChunk);
+            if (whole && g.unit == 16) {
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) {
                 asm volatile(
                     "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], "
                     "[%3];" ::"l"(&maps.out),
                     "r"(r.n0 + c), "r"(row0), "r"(stage)
                     : "memory");
-              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            }
-          } else {
-            __syncwarp();
-            const int n = min(kChunk, ncols - c) * 2;
-            if (saved >= 0) {
-              store_rows<16, ROW>(stage,
-                                  static_cast<char*>(g.pre) +
-                                      (((int64_t)row0 * kHalves + saved) * g.pre_pitch + r.n0 + c) *
-                                          2,
-                                  kHalves * g.pre_pitch * 2, nrows, (n + 15) / 16 * 16, lane);
-            } else {
-              char* dst = static_cast<char*>(g.out) + (int64_t)row0 * pitch + (r.n0 + c) * 2ll;
-              if (g.unit == 16) store_rows<16, ROW>(stage, dst, pitch, nrows, n, lane);
-              else store_odd_rows<ROW>(g.unit, stage, dst, pitch, nrows, n, lane);
-            }
-          }
-        };
-        uint32_t bias = 0;           // of columns c + 2 lane and c + 2 lane + 1
-        uint32_t residual[kChunk / 2];
-        auto fetch = [&](int c) {  // what columns c add, ahead of use
-          if (KIND != LINEAR || c >= ncols) return;
-          if (live && g.bias && 2 * lane < kChunk) {
-            const uint16_t* p =
-                static_cast<const uint16_t*>(g.bias) + (int64_t)r.expert * g.cols + r.n0 + c;
-            bias = 2 * lane < ncols - c ? __ldg(p + 2 * lane) : 0;
-            if (2 * lane + 1 < ncols - c) bias |= (uint32_t)__ldg(p + 2 * lane + 1) << 16;
-          }
-          if (g.residual && g.residual_unit >= 16 && lane < nrows) {
-            const char* p = static_cast<const char*>(g.residual) +
-                            ((row0 + lane) * g.residual_pitch + r.n0 + c) * 2;
-#pragma unroll
-            for (int i = 0; i < kChunk / 16; ++i)
-              load32(residual + 8 * i, p + 32 * i, g.residual_unit, (ncols - c) * 2 - 32 * i);
-          }
-        };
-        fetch(part * kChunk);
-        uint32_t acc = 0;
-        if (live && !(ok = accumulated(0, acc))) break;
-        const uint32_t from = tmem + acc * BN + lanes;
-        if (!(ok = add_runs(r, from))) break;
-        // 16 columns of a half's products, with the bias
-        auto load = [&](int c0, int i, int half, float (&f)[16]) {
-          if (live) {
-            uint32_t v[16];
-            tmem_load16(from + half * S::kOutCols + c0 + 16 * i, v);
-            tmem_wait();
-#pragma unroll
-            for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(v[j]);
-            if (KIND == LINEAR && g.bias) {
-              uint32_t b[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) b[j] = __shfl_sync(0xFFFFFFFFu, bias, 8 * i + j);
-              add16(f, b, bf16);
-            }
-          } else {  // rows of no expert
-#pragma unroll
-            for (int j = 0; j < 16; ++j) f[j] = 0.0f;
-          }
-        };
-        auto put = [&](int i, const float (&f)[16]) {  // into this lane's row of the block
-          uint32_t w[8];
-          pack16(f, bf16, w);
-          store_piece(stage + staged<ROW>(lane, 2 * i), w[0], w[1], w[2], w[3]);
-          store_piece(stage + staged<ROW>(lane, 2 * i + 1), w[4], w[5], w[6], w[7]);
-        };
-#pragma unroll 1
-        for (int c = part * kChunk; c < ncols; c += kParts * kChunk) {
-          if (g.pre) {
-#pragma unroll 1
-            for (int half = 0; half < kHalves; ++half) {
-              free_block();
-#pragma unroll
-              for (int i = 0; i < kChunk / 16; ++i) {
-                float f[16];
-                load(c, i, half, f);
-                put(i, f);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
               }
-              leave(c, half);
+            } else {
+              __syncwarp();
+              move_rows<ROW, false>(g.unit, stage,
+                                  static_cast<char*>(g.out) + (int64_t)row0 * pitch +
+                                      (r.n0 + c) * 2ll,
+                                  pitch, nrows, min(kChunk, ncols - c) * 2, lane);
             }
           }
-          free_block();
-          if (KIND == LINEAR && g.residual && g.residual_unit < 16) {
-            load_odd_rows<ROW>(g.residual_unit, stage,
-                               static_cast<const char*>(g.residual) +
-                                   ((int64_t)row0 * g.residual_pitch + r.n0 + c) * 2,
-                               g.residual_pitch * 2, nrows, min(kChunk, ncols - c) * 2, lane);
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < kChunk / 8; ++i)
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(residual[4 * i]), "=r"(residual[4 * i + 1]),
-                             "=r"(residual[4 * i + 2]), "=r"(residual[4 * i + 3])
-                           : "r"(stage + staged<ROW>(lane, i))
-                           : "memory");
-          }
-#pragma unroll
-          for (int i = 0; i < kChunk / 16; ++i) {
-            float f[16];
-            load(c, i, 0, f);
-            activate(g.act, f);
-            if constexpr (KIND == GATED) {
-              float up[16];
-              load(c, i, 1, up);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) f[j] *= up[j];
-            }
-            if (KIND == LINEAR && g.residual) add16(f, residual + 8 * i, bf16);
-            put(i, f);
-          }
-          fetch(c + kParts * kChunk);
-          leave(c, -1);
+          if (live) release(acc);
         }
-        if (live) release(acc);
-      } else {
+        return true;
+      };
+      auto with_act = [&](auto bf16_c) {
+        if (g.act == LGBM_B200_ACT_SILU)
+          return store_tiles(bf16_c, std::integral_constant<int, LGBM_B200_ACT_SILU>());
+        if (g.act == LGBM_B200_ACT_GELU)
+          return store_tiles(bf16_c, std::integral_constant<int, LGBM_B200_ACT_GELU>());
+        if (g.act == LGBM_B200_ACT_RELU)
+          return store_tiles(bf16_c, std::integral_constant<int, LGBM_B200_ACT_RELU>());
+        return store_tiles(bf16_c, std::integral_constant<int, LGBM_B200_ACT_NONE>());
+      };
+      ok = g.out_kind == LGBM_B200_DTYPE_BF16 ? with_act(std::true_type())
+                                              : with_act(std::false_type());
+    } else {
+      for (int t = first; ok && t < tiles; t += step) {
+        const Tile r = decode(t);
+        const int row0 = r.m0 + quarter * 32;
         char* out = static_cast<char*>(g.out);
         int out_row = row0;  // of D as one matrix
         if (MODE == WEIGHT) {
@@ -996,7 +1038,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, 1)
           __syncwarp();
   #pragma unroll
           for (int p = 0; p < 4; ++p)
-            store_piece(stage + staged(lane, p), w[4 * p], w[4 * p + 1], w[4 * p + 2],
+            store_piece(stage + staged<kStoreRow>(lane, p), w[4 * p], w[4 * p + 1], w[4 * p + 2],
                         w[4 * p + 3]);
           if (by_tma) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1262,6 +1304,7 @@ cudaError_t launch_tiles(const MapsOf<KIND>& maps, MatArgs g, int64_t most_tiles
       err = cudaOccupancyMaxActiveClusters(&most, k_grouped_matmul<KIND, BN, CTAS>, &cfg);
     else if (err == cudaSuccess)
       err = cudaDeviceGetAttribute(&most, cudaDevAttrMultiProcessorCount, dev);
+    if (CTAS == 1) most *= S::kPerSm;
     if (err != cudaSuccess) return err;
     if (most < 1) return cudaErrorInvalidConfiguration;
     most_ready[dev].store(most, std::memory_order_release);
