@@ -313,8 +313,15 @@ __global__ void __launch_bounds__(kThreads)
   float s = 0.0f;
   if (n < outer && hi > lo) {
     const int64_t last = min((hi - 1) / rows_a_block, blocks - 1);
-    for (int64_t b = lo / rows_a_block + k; b <= last; b += kThreads / 32)
-      s += sums[(b + e) * outer + n];
+    constexpr int kStep = kThreads / 32, kLoads = 8;  // on their way at a time
+    for (int64_t b = lo / rows_a_block + k; b <= last; b += kStep * kLoads) {
+      float v[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        v[i] = b + i * kStep <= last ? sums[(b + i * kStep + e) * outer + n] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) s += v[i];
+    }
   }
   part[threadIdx.x] = s;
   __syncthreads();

@@ -317,6 +317,8 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   const uint32_t dst0 = shared_addr(ring) + (lane >> 3) * kRowPitch + (lane & 7) * 16;
   const int rest0 = row_bytes - byte0 - (lane & 7) * 16, rows_in = row_end - my_row0 - (lane >> 3);
   const int64_t step4 = 4 * g.w_pitch;
+  const char* const w_begin = static_cast<const char*>(g.w);
+  const char* const w_end = w_begin + (int64_t)g.experts * g.outer * g.w_pitch;
   int load_slot = 0;
   auto load_stage = [&](int i) {
     if (i < stages) {
@@ -330,6 +332,31 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 4 * j * kRowPitch),
                        "l"(src + j * step4)
                        : "memory");
+      } else if (S::ALIGN == 2) {
+        // rows at 2 bytes: the aligned pieces that hold these, all eight loads first; what is too
+        // near to an end of the weights for that, value by value
+        StagePair v[4];
+        auto valid = [&](int j) { return 4 * j < rows_in ? min(max(rest, 0), 16) : 0; };
+        auto inside = [&](int j) {
+          const char* p = src + j * step4;
+          return valid(j) > 0 && p - 15 >= w_begin && p + 32 <= w_end;
+        };
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (inside(j)) v[j] = stage_load(src + j * step4, valid(j));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (inside(j)) {
+            const int s = (int)(reinterpret_cast<uintptr_t>(src + j * step4) & 15);
+            const uint4 q = stage_shift(v[j], s, valid(j));
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 4 * j * kRowPitch),
+                         "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w)
+                         : "memory");
+          } else {
+            copy16<S::ALIGN>(dst + 4 * j * kRowPitch,
+                             valid(j) ? src + j * step4 : static_cast<const char*>(g.w), valid(j));
+          }
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {

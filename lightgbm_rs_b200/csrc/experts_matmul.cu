@@ -855,8 +855,32 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
         };
+        float bias = 0.0f;  // of column c + lane
+        uint32_t residual[kChunk / 2];
+        auto fetch = [&](const Tile& r, int c) {  // what columns c add, ahead of use
+          const int row = r.m0 + quarter * 32 + lane, n = min(S::kOutCols, g.cols - r.n0) - c;
+          if (KIND != LINEAR || n <= 0) return;
+          if (g.bias) {
+            uint32_t v = 0;
+            if (r.red > 0 && lane < min(kChunk, n))
+              v = __ldg(static_cast<const uint16_t*>(g.bias) + (int64_t)r.expert * g.cols + r.n0 +
+                        c + lane);
+            bias = unpack2<BF16>(v).x;
+          }
+          if (g.residual && g.residual_unit >= 16 && row < r.m_end) {
+            const char* p = static_cast<const char*>(g.residual) +
+                            (row * g.residual_pitch + r.n0 + c) * 2;
+#pragma unroll
+            for (int i = 0; i < kChunk / 16; ++i)
+              load32(residual + 8 * i, p + 32 * i, g.residual_unit, n * 2 - 32 * i);
+          }
+        };
+        Tile r;
+        if (first < tiles) {
+          r = decode(first);
+          fetch(r, part * kChunk);
+        }
         for (int t = first; t < tiles; t += step) {
-          const Tile r = decode(t);
           const int row0 = r.m0 + quarter * 32, nrows = min(32, r.m_end - row0);
           const int ncols = nrows > 0 ? min(S::kOutCols, g.cols - r.n0) : 0;
           const bool live = r.red > 0;
@@ -885,26 +909,6 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
                                   (min(kChunk, ncols - c) * 2 + 15) / 16 * 16, lane);
             }
           };
-          float bias = 0.0f;  // of column c + lane
-          uint32_t residual[kChunk / 2];
-          auto fetch = [&](int c) {  // what columns c add, ahead of use
-            if (KIND != LINEAR || c >= ncols) return;
-            if (g.bias) {
-              uint32_t v = 0;
-              if (live && lane < min(kChunk, ncols - c))
-                v = __ldg(static_cast<const uint16_t*>(g.bias) + (int64_t)r.expert * g.cols + r.n0 +
-                          c + lane);
-              bias = unpack2<BF16>(v).x;
-            }
-            if (g.residual && g.residual_unit >= 16 && lane < nrows) {
-              const char* p = static_cast<const char*>(g.residual) +
-                              ((row0 + lane) * g.residual_pitch + r.n0 + c) * 2;
-#pragma unroll
-              for (int i = 0; i < kChunk / 16; ++i)
-                load32(residual + 8 * i, p + 32 * i, g.residual_unit, (ncols - c) * 2 - 32 * i);
-            }
-          };
-          fetch(part * kChunk);
           uint32_t acc = 0;
           if (live && !accumulated(0, acc)) return false;
           const uint32_t from = tmem + acc * BN + lanes;
@@ -983,7 +987,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
               }
               put(i, f);
             }
-            fetch(c + kParts * kChunk);
+            if (c + kParts * kChunk < ncols) fetch(r, c + kParts * kChunk);
             if (whole && g.unit == 16) {
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
               __syncwarp();
@@ -1004,6 +1008,10 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
             }
           }
           if (live) release(acc);
+          if (t + step < tiles) {
+            r = decode(t + step);
+            fetch(r, part * kChunk);
+          }
         }
         return true;
       };
@@ -1474,14 +1482,27 @@ __global__ void __launch_bounds__(256)
   const int64_t e = i / count;
   const float* p = part + e * count * (parts - 1) + i;  // (e * parts) * count + i - e * count
   float sum[V] = {};
-#pragma unroll 4
-  for (int k = 0; k < parts; ++k, p += count) {
-    if constexpr (V == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(p);
-      sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
-    } else {
-      sum[0] += *p;
+  // sixteen on their way at a time: few outputs of many parts are a chain of latencies
+  constexpr int kAhead = 16;
+  for (int k0 = 0; k0 < parts; k0 += kAhead) {
+    float v[kAhead][V];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (k0 + k >= parts) break;
+      if constexpr (V == 4) {
+        const float4 q = *reinterpret_cast<const float4*>(p + k * count);
+        v[k][0] = q.x, v[k][1] = q.y, v[k][2] = q.z, v[k][3] = q.w;
+      } else {
+        v[k][0] = p[k * count];
+      }
     }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (k0 + k >= parts) break;
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += v[k][j];
+    }
+    p += kAhead * count;
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) out[i + j] = from_f32<T>(sum[j]);
