@@ -226,6 +226,7 @@ struct MatmulCall {
   int32_t experts, inner, outer;
   void *y, *dx, *dw;        // results, null: not wanted
   Epilogue epilogue;        // of y
+  bool layer;               // gradients of a gated or linear layer
 };
 int64_t matmul_workspace(const MatmulCall& c);
 cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st);

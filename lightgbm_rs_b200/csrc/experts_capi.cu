@@ -181,6 +181,7 @@ int run_layer_backward(const char* what, MatmulCall c, bool gated, int32_t act, 
   const bool turns = gated || act != LGBM_B200_ACT_NONE;  // dpre is not dy itself
   // what check_product sees of dy: a pitch that fits, where dpre takes its place
   MatmulCall p = c;
+  p.layer = true;
   if (turns) p.dy_pitch = dpre_pitch(c.outer);
   if (int rc = check_product(what, p)) return rc;
   if (c.dy_pitch < width)
@@ -265,6 +266,7 @@ int64_t layer_backward_workspace(const void* dy, int64_t dy_pitch, const void* x
   c.outer = outer;
   c.dx = want_dx ? &c : nullptr;  // wanted; not written here
   c.dw = want_dw ? &c : nullptr;
+  c.layer = true;
   return c.dx || c.dw ? need + matmul_workspace(c) : need;
 }
 

@@ -77,15 +77,20 @@ constexpr int kTileK = 64;         // 128 bytes of a 16-bit type: one swizzle ro
 constexpr int kStoreRow = 64;      // bytes of a row in a storing warp's staging block
 constexpr int kBandRows = 2048;    // rows of D of a band, see tile_of
 // Entries of the table of groups: the rows before the first expert's, the experts, the rows past
-// the last one's, the end.
-constexpr int kGroupSlots = kMaxExperts + 3;
+// the last one's, the end. Narrow tiles have room for parts of every expert.
+constexpr int kNarrowGroups = 1536;
+constexpr int group_slots(int bn) { return (bn == 64 ? kNarrowGroups : kMaxExperts) + 3; }
 
-enum Mode { FORWARD = 0, INPUT = 1, WEIGHT = 2, WEIGHT_F32 = 3, LINEAR = 4, GATED = 5 };
+enum Mode {
+  FORWARD = 0, INPUT = 1, WEIGHT = 2, WEIGHT_F32 = 3, LINEAR = 4, GATED = 5,
+  INPUT_F32 = 6  // parts of an input gradient's sums
+};
 
 struct MatArgs {
   const int32_t* offsets;
   int32_t experts;     // groups: WEIGHT has `parts` of each expert's
-  int32_t parts;
+  int32_t parts;       // of an expert's rows (WEIGHT), of the reduction (INPUT_F32)
+  int32_t part;        // INPUT_F32: length of a part of the reduction, whole blocks
   int32_t cols;        // columns of D in a group
   int32_t drows;       // WEIGHT: rows of D in a group
   int32_t reduction;   // FORWARD, INPUT: length of the reduction
@@ -304,8 +309,9 @@ struct Tile {
   int32_t m0;      // first row of D: of all rows (FORWARD, INPUT), of the group (WEIGHT)
   int32_t m_end;   // rows of D end here
   int32_t n0;
-  int32_t red0;    // WEIGHT: first row of the reduction
-  int32_t red;     // length of the reduction
+  int32_t red0;    // where the reduction begins
+  int32_t red;     // its length
+  int32_t part;    // INPUT_F32
 };
 
 // Tile `t` of a group of mt x nt tiles: bands of `band` row tiles, column by column inside a
@@ -322,11 +328,16 @@ __device__ __forceinline__ void tile_of(int t, int mt, int nt, int band, int& m,
 template <int KIND, int BN, int CTAS>
 struct Shape {
   static constexpr bool kFused = KIND == LINEAR || KIND == GATED;
+  static constexpr bool kWide = KIND == WEIGHT_F32 || KIND == INPUT_F32;  // results of 32 bits
+  static constexpr int kMode = KIND == WEIGHT_F32  ? (int)WEIGHT
+                               : KIND == INPUT_F32 ? (int)INPUT
+                               : kFused            ? (int)FORWARD
+                                                   : KIND;
   // Narrow tiles are short of work for one CTA, whose stages of loading, multiplying and storing
   // wait for one another: two share an SM.
   static constexpr int kPerSm = BN == 64 ? 2 : 1;
-  static constexpr int kStoreWarps = BN > 64 && (KIND == WEIGHT_F32 || kFused) ? 16 : 8;
-  static constexpr int kRun = KIND == WEIGHT_F32 ? 768 : 4096;  // see "Precision" above
+  static constexpr int kStoreWarps = BN > 64 && (kWide || kFused) ? 16 : 8;
+  static constexpr int kRun = kWide ? 768 : 4096;  // see "Precision" above
   static constexpr int kThreads = 64 + 32 * kStoreWarps;
   static constexpr int kOutCols = KIND == GATED ? BN / 2 : BN;  // columns of the result
   // bytes of a row of a staging block; LINEAR, GATED: so that narrow tiles occupy all warps too
@@ -337,9 +348,10 @@ struct Shape {
   static constexpr int kCols = BN / CTAS;  // columns of B that a CTA loads
   static constexpr int kStageBytes = (kTileM + kCols) * 128;
   // what tables, barriers and alignment leave of 227 KB: 3 to 8
-  static constexpr int kStages = (212992 / kPerSm - kStoreBytes) / kStageBytes;
+  static constexpr int kStages = ((kPerSm == 2 ? 97280 : 212992) - kStoreBytes) / kStageBytes;
   static constexpr int kTmemCols = 2 * BN;                              // two accumulators
   static constexpr int kBand = kBandRows / kRows;
+  static constexpr int kGroupSlots = group_slots(BN);
   static constexpr int kSmem =
       1024 + kStages * kStageBytes + kStoreBytes + 8 * kGroupSlots + 512;
 };
@@ -503,9 +515,9 @@ template <int KIND, int BN, int CTAS>
 __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, BN, CTAS>::kPerSm)
     k_grouped_matmul(const __grid_constant__ MapsOf<KIND> maps, const MatArgs g) {
   using S = Shape<KIND, BN, CTAS>;
-  constexpr int MODE = KIND == WEIGHT_F32 ? (int)WEIGHT : S::kFused ? (int)FORWARD : KIND;
+  constexpr int MODE = S::kMode;
   constexpr int kLead = MODE == WEIGHT ? 0 : 1;  // groups before the first expert's
-  constexpr bool kWide = KIND == WEIGHT_F32;  // results of 32 bits
+  constexpr bool kWide = S::kWide;
   constexpr int kRun = S::kRun;
   constexpr int kStages = S::kStages;
   constexpr uint32_t kABytes = kTileM * 128;
@@ -515,9 +527,9 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
   const uint32_t base = smem_addr(smem);
   const uint32_t store_base = base + kStages * S::kStageBytes;
   int32_t* cum = reinterpret_cast<int32_t*>(smem + kStages * S::kStageBytes + S::kStoreBytes);
-  int32_t* off = cum + kGroupSlots;  // the groups' first rows, then the end
+  int32_t* off = cum + S::kGroupSlots;  // the groups' first rows, then the end
   uint64_t* bars = reinterpret_cast<uint64_t*>(
-      (reinterpret_cast<uintptr_t>(off + kGroupSlots) + 15) & ~(uintptr_t)15);
+      (reinterpret_cast<uintptr_t>(off + S::kGroupSlots) + 15) & ~(uintptr_t)15);
   // end_full, end_peer (WEIGHT): a group's last block has landed in this CTA; the odd CTA has
   // zeroed its rows past the end. Used in turn, one a last block.
   const uint32_t full = smem_addr(bars), empty = full + 8 * kStages,
@@ -618,11 +630,17 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
   if constexpr (CTAS == 2) cluster_sync();  // the other CTA's barriers are set up too
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  const int tiles = cum[groups];
+  const int tiles = cum[groups] * (KIND == INPUT_F32 ? g.parts : 1);
   const int nt = (g.cols + S::kOutCols - 1) / S::kOutCols;
   const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   auto decode = [&](int t) {
+    int32_t red0 = 0, part = 0;
+    if (KIND == INPUT_F32) {  // a tile's parts are neighbours
+      part = t % g.parts;
+      t /= g.parts;
+      red0 = part * g.part;
+    }
     int lo = 0, hi = groups;  // the last group that starts at or before t
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -649,8 +667,10 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
     } else {
       r.m0 += b;
       r.m_end = e;
-      r.red0 = 0;
-      r.red = r.expert >= 0 && r.expert < g.experts ? g.reduction : 0;
+      r.red0 = red0;
+      r.red = r.expert >= 0 && r.expert < g.experts ? g.reduction - red0 : 0;
+      if (KIND == INPUT_F32) r.red = min(r.red, g.part);
+      r.part = part;
     }
     return r;
   };
@@ -695,7 +715,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
             for (int j = 0; j < S::kCols / 64; ++j)
               tma_load_2d<CTAS>(b + j * 8192, &maps.b, nb + 64 * j, r.red0 + k0, bar);
           } else {
-            tma_load_2d<CTAS>(a, &maps.a, k0, r.m0, bar);
+            tma_load_2d<CTAS>(a, &maps.a, r.red0 + k0, r.m0, bar);
             if (MODE == FORWARD) {
               tma_load_3d<CTAS>(b, &maps.b, k0, nb, r.expert, bar);
               if (KIND == GATED && CTAS == 1)  // one CTA loads both
@@ -703,7 +723,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
             } else {
 #pragma unroll
               for (int j = 0; j < S::kCols / 64; ++j)
-                tma_load_3d<CTAS>(b + j * 8192, &maps.b, nb + 64 * j, k0, r.expert, bar);
+                tma_load_3d<CTAS>(b + j * 8192, &maps.b, nb + 64 * j, r.red0 + k0, r.expert, bar);
             }
           }
         }
@@ -1035,6 +1055,9 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
         if (MODE == WEIGHT) {
           out += (int64_t)r.expert * g.drows * pitch;
           out_row += r.expert * g.drows;
+        } else if (KIND == INPUT_F32) {
+          out += r.part * g.rows * pitch;
+          out_row += (int)(r.part * g.rows);
         }
         const int ncols = min(BN, g.cols - r.n0), nrows = min(32, r.m_end - row0);
         // whole 32-row blocks leave by TMA, which also cuts off the last columns
@@ -1367,8 +1390,13 @@ uint32_t instruction(int32_t dtype, bool a_mn, bool b_mn, int m, int n) {
          ((uint32_t)b_mn << 16) | ((uint32_t)(n / 8) << 17) | ((uint32_t)(m / 16) << 24);
 }
 
-// Whether an expert's weight gradient of more than 128 columns is multiplied by pairs.
-bool weight_pairs(int64_t drows) { return drows >= kTileM * 3 / 2; }
+// Whether an expert's weight gradient of more than 128 columns is multiplied by pairs: where the
+// last pair's rows are not mostly empty (255 experts of 258 x 700, 157 rows each:
+// 87 us in pairs, 84 without).
+bool weight_pairs(int64_t drows) {
+  const int64_t singles = (drows + kTileM - 1) / kTileM, pairs = (singles + 1) / 2;
+  return drows >= kTileM * 3 / 2 && pairs * 2 * 4 <= singles * 5;
+}
 
 // a: x (FORWARD) or dy; b: w, or x (WEIGHT).
 template <int MODE>
@@ -1393,7 +1421,7 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
       fine = fine && encode(&maps.b, dtype, b.p, 3, db, pb, MODE == FORWARD ? S::kCols : 64);
     }
     maps.out = maps.a;  // not used unless set
-    const int64_t rows_d = MODE == WEIGHT ? (int64_t)g.experts * g.drows : g.rows;
+    const int64_t rows_d = MODE == WEIGHT ? (int64_t)g.experts * g.drows : g.rows * g.parts;
     if (g.unit == 16 && rows_d > INT32_MAX) g.unit = 8;  // no coordinate for its last rows
     if (g.unit == 16) {
       const int64_t dd[3] = {g.cols, rows_d, 1}, pd[2] = {g.out_pitch, 0};
@@ -1404,9 +1432,11 @@ cudaError_t run_tiles(const Operand& a, int64_t a_width, const Operand& b, int64
     const int64_t nt = (g.cols + BN - 1) / BN;
     const int64_t most = MODE == WEIGHT
                              ? (int64_t)g.experts * ((g.drows + S::kRows - 1) / S::kRows) * nt
-                             : (g.rows / S::kRows + g.experts + 2) * nt;
-    if (MODE == WEIGHT && g.out_kind == LGBM_B200_DTYPE_F32)
-      return launch_tiles<WEIGHT_F32, BN, CTAS>(maps, g, most, st);
+                             : (g.rows / S::kRows + g.experts + 2) * nt * g.parts;
+    constexpr int kWideKind = MODE == WEIGHT ? (int)WEIGHT_F32 : (int)INPUT_F32;
+    if constexpr (MODE != FORWARD)
+      if (g.out_kind == LGBM_B200_DTYPE_F32)
+        return launch_tiles<kWideKind, BN, CTAS>(maps, g, most, st);
     return launch_tiles<MODE, BN, CTAS>(maps, g, most, st);
   };
   using One = std::integral_constant<int, 1>;
@@ -1508,11 +1538,55 @@ __global__ void __launch_bounds__(256)
   for (int j = 0; j < V; ++j) out[i + j] = from_f32<T>(sum[j]);
 }
 
+// The same for few outputs of many parts: eight threads an output (or four neighbours), each the
+// parts k, k + 8, .., whose sums are added up in one order.
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+    k_join_few(const float* part, int parts, int64_t count, int64_t total, T* out) {
+  __shared__ float sums[8][32 * V];
+  wait_for_stream();
+  let_next_start();
+  const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+  const int64_t i = ((int64_t)blockIdx.x * 32 + lane) * V;
+  float sum[V] = {};
+  if (i < total) {
+    const int64_t e = i / count;
+    const float* p = part + e * count * (parts - 1) + i;
+#pragma unroll 8
+    for (int k = group; k < parts; k += 8) {
+      if constexpr (V == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p + k * count);
+        sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+      } else {
+        sum[0] += p[k * count];
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) sums[group][j * 32 + lane] = sum[j];
+  __syncthreads();
+  if (group == 0 && i < total) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += sums[k][j * 32 + lane];
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[i + j] = from_f32<T>(sum[j]);
+  }
+}
+
 template <typename T>
-cudaError_t join_parts(const float* part, int parts, int64_t count, int experts, T* out,
+cudaError_t join_parts(const float* part, int parts, int64_t count, int experts, bool layer, T* out,
                        cudaStream_t st) {
   const int64_t total = count * experts;
   const auto blocks = [&](int v) { return (unsigned)((total / v + 255) / 256); };
+  // One thread an output while that fills the SMs (148 parts of 56 x 168: 19 -> 7 us).
+  if (layer && parts >= 16 && total <= 4 * 256 * 148) {
+    const unsigned few = (unsigned)((total / (count % 4 == 0 ? 4 : 1) + 31) / 32);
+    if (count % 4 == 0)
+      return launch_behind(k_join_few<T, 4>, dim3(few), 256, st, part, parts, count, total, out);
+    return launch_behind(k_join_few<T, 1>, dim3(few), 256, st, part, parts, count, total, out);
+  }
   if (count % 4 == 0)
     return launch_behind(k_join_parts<T, 4>, dim3(blocks(4)), 256, st, part, parts, count, total,
                          out);
@@ -1570,13 +1644,34 @@ static int weight_parts(const MatmulCall& c) {
   const int64_t tile_rows = pairs ? 2 * kTileM : kTileM;
   const int64_t tiles =
       c.experts * ((c.outer + tile_rows - 1) / tile_rows) * ((c.inner + bn - 1) / bn);
-  const int64_t parts = std::min({(pairs ? 74 : 148) / tiles, c.rows / (256 * (int64_t)c.experts),
-                                  (int64_t)(kMaxExperts / c.experts)});
+  int64_t parts = std::min({(pairs ? 74 : 148) / tiles, c.rows / (256 * (int64_t)c.experts),
+                            (int64_t)(kMaxExperts / c.experts)});
+  // One narrow tile an expert: the time is the largest expert's rows, and parts of small outputs
+  // cost little. (200003 rows in 255 experts of 64 x 28, the largest of 4000: 71 ->
+  // 38 us with the joining.)
+  if (c.layer && c.inner <= 64 && c.outer <= tile_rows)
+    parts = std::max(parts, std::min(c.rows / (256 * (int64_t)c.experts),
+                                     (int64_t)(kNarrowGroups / c.experts)));
   return c.dw && parts > 1 ? (int)parts : 1;
 }
+// Parts that an input gradient's reduction is summed in: as few rows of a layer with a wide output
+// make few tiles of many blocks. (1840 rows, 20 experts of 6400 x 64: 44 -> 15
+// us with the joining.)
+static int32_t input_part(const MatmulCall& c) {
+  const int64_t bn = c.inner <= 64 ? 64 : c.inner <= 128 ? 128 : 256;
+  const int64_t tiles = (std::min<int64_t>(c.experts, c.rows) + c.rows / kTileM) *
+                        ((c.inner + bn - 1) / bn);
+  const int64_t parts =
+      std::min<int64_t>({(bn == 64 ? 296 : 148) / tiles, c.outer / 512, (int64_t)16});
+  if (!c.dx || !c.layer || parts < 2) return 0;
+  return (int32_t)((c.outer / parts + kTileK) / kTileK * kTileK);
+}
+// Partial sums of one gradient after the other.
 static int64_t parts_bytes(const MatmulCall& c) {
-  const int parts = weight_parts(c);
-  return parts > 1 ? sizeof(float) * parts * c.experts * (int64_t)c.outer * c.inner : 0;
+  const int64_t parts = weight_parts(c), part = input_part(c);
+  const int64_t weight = parts > 1 ? parts * c.experts * (int64_t)c.outer * c.inner : 0;
+  const int64_t input = part > 0 ? (c.outer + part - 1) / part * c.rows * c.inner : 0;
+  return (int64_t)sizeof(float) * std::max(weight, input);
 }
 
 int64_t matmul_workspace(const MatmulCall& c) {
@@ -1626,33 +1721,38 @@ cudaError_t launch_matmul(const MatmulCall& c, void* workspace, cudaStream_t st)
     else if (c.epilogue.gated) err = run_fused<GATED>(x, w, c, g, st);
     else err = run_fused<LINEAR>(x, w, c, g, st);
   }
+  // `ws`, the end of the copies, takes the partial sums
+  const float* const part = reinterpret_cast<const float*>(ws);
+  const auto join = [&](int parts, int64_t count, int experts, int32_t dtype, void* out) {
+    if (dtype == LGBM_B200_DTYPE_F32)
+      return join_parts(part, parts, count, experts, c.layer, static_cast<float*>(out), st);
+    if (dtype == LGBM_B200_DTYPE_BF16)
+      return join_parts(part, parts, count, experts, c.layer, static_cast<__nv_bfloat16*>(out), st);
+    return join_parts(part, parts, count, experts, c.layer, static_cast<__half*>(out), st);
+  };
   if (err == cudaSuccess && c.dx) {
-    g.out = c.dx;
-    g.out_kind = c.dtype;
+    g.part = input_part(c);
+    if (g.part > 0) g.parts = (c.outer + g.part - 1) / g.part;
+    g.out = g.parts > 1 ? ws : c.dx;
+    g.out_kind = g.parts > 1 ? (int32_t)LGBM_B200_DTYPE_F32 : c.dtype;
     g.cols = c.inner;
     g.reduction = c.outer;
     g.out_pitch = c.inner;
     err = run_tiles<INPUT>(dy, c.outer, w, c.inner, c.dtype, g, st);
+    if (err == cudaSuccess && g.parts > 1) err = join(g.parts, c.rows * c.inner, 1, c.dtype, c.dx);
+    g.parts = 1;
   }
   if (err == cudaSuccess && c.dw) {
     g.parts = weight_parts(c);
     g.experts *= g.parts;
-    g.out = g.parts > 1 ? ws : c.dw;  // ws: the end of the copies
+    g.out = g.parts > 1 ? ws : c.dw;
     g.out_kind = g.parts > 1 ? (int32_t)LGBM_B200_DTYPE_F32 : c.grad_dtype;
     g.cols = c.inner;
     g.drows = c.outer;
     g.out_pitch = c.inner;
     err = run_tiles<WEIGHT>(dy, c.outer, x, c.inner, c.dtype, g, st);
-    if (err == cudaSuccess && g.parts > 1) {
-      const int64_t count = (int64_t)c.outer * c.inner;
-      const float* part = reinterpret_cast<const float*>(ws);
-      if (c.grad_dtype == LGBM_B200_DTYPE_F32)
-        err = join_parts(part, g.parts, count, c.experts, static_cast<float*>(c.dw), st);
-      else if (c.grad_dtype == LGBM_B200_DTYPE_BF16)
-        err = join_parts(part, g.parts, count, c.experts, static_cast<__nv_bfloat16*>(c.dw), st);
-      else
-        err = join_parts(part, g.parts, count, c.experts, static_cast<__half*>(c.dw), st);
-    }
+    if (err == cudaSuccess && g.parts > 1)
+      err = join(g.parts, (int64_t)c.outer * c.inner, c.experts, c.grad_dtype, c.dw);
   }
   return err;
 }

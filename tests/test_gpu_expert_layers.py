@@ -103,6 +103,12 @@ LAYERS = [  # counts, tail rows, inner, outer
     ([130], 0, 4112, 24),              # two runs in tiles of 64 columns
     ([33] * 200, 9, 28, 64),           # many groups, little to multiply
     ([0, 0], 5, 48, 40),               # no expert has rows
+    ([3, 0, 40], 2, 40, 1100),         # input gradients summed in parts of the reduction
+    ([70, 9], 0, 130, 2050),
+    ([64], 1, 300, 1037),
+    ([4000, 1, 0, 900], 3, 56, 40),    # narrow weight gradients in parts of the rows
+    ([9000], 0, 30, 24),
+    ([5], 0, 24, 4099),                # few long rows, divided among blocks
 ]
 
 
