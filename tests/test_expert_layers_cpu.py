@@ -89,17 +89,17 @@ def test_workspace_of_the_backward_passes(capi):
     p, relu = 1 << 20, 1
     args = (p, 40, p, 64, None, p)
     # without an activation dy itself is multiplied: nothing to keep but an operand's copies
-    assert lin(*args, 0, 1000, 4, 64, 40, 1, 1, 0) == 0
-    assert lin(p, 33, p, 64, None, p, 0, 1000, 4, 64, 33, 1, 0, 0) >= 1000 * 40 * 2
-    assert lin(*args, relu, 1000, 4, 64, 40, 1, 1, 0) == 1000 * 40 * 2
-    assert lin(*args, relu, 1000, 4, 64, 33, 1, 0, 0) >= 1000 * 40 * 2
-    sums = lin(*args, 0, 1000, 4, 64, 40, 0, 0, 1)
+    assert lin(*args, 0, 1024, 4, 64, 40, 1, 1, 0) == 0
+    assert lin(p, 33, p, 64, None, p, 0, 1024, 4, 64, 33, 1, 0, 0) >= 1024 * 40 * 2
+    assert lin(*args, relu, 1024, 4, 64, 40, 1, 1, 0) == 1024 * 40 * 2
+    assert lin(*args, relu, 1024, 4, 64, 33, 1, 0, 0) >= 1024 * 40 * 2
+    sums = lin(*args, 0, 1024, 4, 64, 40, 0, 0, 1)
     assert 4 * 40 * 4 < sums < 1 << 20
-    assert lin(*args, relu, 1000, 4, 64, 40, 0, 0, 1) == 1000 * 40 * 2 + sums
+    assert lin(*args, relu, 1024, 4, 64, 40, 0, 0, 1) == 1024 * 40 * 2 + sums
     assert lin(*args, relu, 0, 4, 64, 40, 1, 1, 1) == 0
-    assert gat(p, 64, None, p, 1000, 4, 64, 20, 1, 1) == 1000 * 40 * 2
-    assert gat(p, 64, p, p, 1000, 4, 64, 20, 0, 1) >= 1000 * (40 + 64) * 2  # gathered x
-    assert gat(p, 64, None, p, 1000, 4, 64, 0, 1, 1) == 0
+    assert gat(p, 64, None, p, 1024, 4, 64, 20, 1, 1) == 1024 * 40 * 2
+    assert gat(p, 64, p, p, 1024, 4, 64, 20, 0, 1) >= 1024 * (40 + 64) * 2  # gathered x
+    assert gat(p, 64, None, p, 1024, 4, 64, 0, 1, 1) == 0
     # a long reduction of few tiles, in parts: 2 of 576 and 448 in f32
     assert gat(p, 64, None, p, 100, 60, 64, 512, 1, 0) == 100 * 1024 * 2 + 2 * 100 * 64 * 4
 
