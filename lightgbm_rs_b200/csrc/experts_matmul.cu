@@ -334,9 +334,11 @@ struct Shape {
                                : kFused            ? (int)FORWARD
                                                    : KIND;
   // Narrow tiles are short of work for one CTA, whose stages of loading, multiplying and storing
-  // wait for one another: two share an SM.
-  static constexpr int kPerSm = BN == 64 ? 2 : 1;
-  static constexpr int kStoreWarps = BN > 64 && (kWide || kFused) ? 16 : 8;
+  // wait for one another: two share an SM. (65536 rows, 16 experts of 128 x 128: y 14 -> 10 us. But
+  // not for weight gradients of 128 columns, whose long reductions want more stages than two: 8
+  // of 1024 x 128 42 us by one, 59 by two.)
+  static constexpr int kPerSm = BN == 64 || (BN == 128 && kMode != WEIGHT) ? 2 : 1;
+  static constexpr int kStoreWarps = kPerSm == 1 && (kWide || kFused) ? 16 : 8;
   static constexpr int kRun = kWide ? 768 : 4096;  // see "Precision" above
   static constexpr int kThreads = 64 + 32 * kStoreWarps;
   static constexpr int kOutCols = KIND == GATED ? BN / 2 : BN;  // columns of the result
