@@ -75,28 +75,10 @@ __device__ __forceinline__ uint32_t shared_addr(const void* p) {
 }
 
 // 16 bytes of global memory to shared, of which the first `valid` (0..16) are read and the
-// rest are zeros. ALIGN: of `src`, 16, 4 or 2 bytes.
-template <int ALIGN>
+// rest are zeros; `src` is 16-byte aligned.
 __device__ __forceinline__ void copy16(uint32_t dst, const char* src, int valid) {
-  if constexpr (ALIGN == 16) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-                 "r"(valid)
-                 : "memory");
-  } else if constexpr (ALIGN == 4) {
-#pragma unroll
-    for (int i = 0; i < 16; i += 4)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + i),
-                   "l"(valid > i ? src + i : src), "r"(min(max(valid - i, 0), 4))
-                   : "memory");
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      uint32_t v = 0;
-      if (valid > i) v = *reinterpret_cast<const uint16_t*>(src + i);
-      if (valid > i + 2) v |= (uint32_t)*reinterpret_cast<const uint16_t*>(src + i + 2) << 16;
-      asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + i), "r"(v) : "memory");
-    }
-  }
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid)
+               : "memory");
 }
 
 template <typename T>
@@ -172,14 +154,15 @@ __device__ __forceinline__ uint32_t sub2<__nv_bfloat16>(uint32_t a, uint32_t b) 
 enum Finish { PLAIN = 0, FINISH_LINEAR = 1, FINISH_GATED = 2 };
 
 // A kernel's variant: TILES column tiles of 8 rows make an item; SHIFT is log2 of the scale
-// group's size, 0 with weights of 16 bits, whose rows are aligned to ALIGN bytes.
-template <typename T_, int TILES_, int SHIFT_, bool ZEROS_, int ALIGN_, int FINISH_ = PLAIN>
+// group's size, 0 with weights of 16 bits, whose rows are ALIGNED to 16 bytes or not.
+template <typename T_, int TILES_, int SHIFT_, bool ZEROS_, bool ALIGNED_, int FINISH_ = PLAIN>
 struct FewShape {
   using T = T_;
   static constexpr int FINISH = FINISH_;
   // columns of y of a block; gated, half of its warps take gate and half take up
   static constexpr int kOut = FINISH == FINISH_GATED ? kOutBlock / 2 : kOutBlock;
-  static constexpr int TILES = TILES_, SHIFT = SHIFT_, ALIGN = ALIGN_;
+  static constexpr int TILES = TILES_, SHIFT = SHIFT_;
+  static constexpr bool ALIGNED = ALIGNED_;
   static constexpr bool W4 = SHIFT > 0, ZEROS = ZEROS_;
   // Blocks that share an SM, and stages of a warp's ring: with 4 bits the arithmetic wants
   // warps, with 16 bits the memory wants bytes in flight (4 x 16 KB a block).
@@ -319,50 +302,83 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   const int64_t step4 = 4 * g.w_pitch;
   const char* const w_begin = static_cast<const char*>(g.w);
   const char* const w_end = w_begin + (int64_t)g.experts * g.outer * g.w_pitch;
+  // Rows that do not start at 16 bytes: this lane's ninth piece, of row `lane`
+  const char* src9 = wbase + (int64_t)(lane & 15) * g.w_pitch + byte0 + kRowBytes;
+  const uint32_t dst9 = shared_addr(ring) + (lane & 15) * kRowPitch + kRowBytes;
+  const int rest9 = row_bytes - byte0 - kRowBytes;
+  // The aligned piece that `src` lies in; `rest` bytes of its row from src on. One that reaches out
+  // of the weights at either end value by value, one without any of the row not at all.
+  auto copy_aligned = [&](uint32_t dst, const char* src, int rest) {
+    const int s = (int)(reinterpret_cast<uintptr_t>(src) & 15);
+    const char* p = src - s;
+    if (rest + s <= 0) return;
+    if (p >= w_begin && p + 16 <= w_end) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(p) : "memory");
+    } else {
+#pragma unroll 1
+      for (int b = 0; b < 16; b += 2)
+        if (p + b >= w_begin && p + b < w_end)
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + b),
+                       "h"(*reinterpret_cast<const uint16_t*>(p + b))
+                       : "memory");
+    }
+  };
+  // Stage i in ring slot `at`: every row's bytes from the start of its first piece, zeros behind
+  // the row's end and for rows that do not exist.
+  auto realign = [&](int i, int at) {
+    const uint32_t row0 = dst0 + at * kStageBytes;
+    uint4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      StagePair q;
+      const uint32_t from = row0 + 4 * j * kRowPitch;
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(q.a.x), "=r"(q.a.y), "=r"(q.a.z), "=r"(q.a.w)
+                   : "r"(from)
+                   : "memory");
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(q.b.x), "=r"(q.b.y), "=r"(q.b.z), "=r"(q.b.w)
+                   : "r"(from + 16)
+                   : "memory");
+      const int left = 4 * j < rows_in ? min(max(rest0 - i * kRowBytes, 0), 16) : 0;
+      v[j] = stage_shift(q, (int)(reinterpret_cast<uintptr_t>(src0 + j * step4) & 15), left);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row0 + 4 * j * kRowPitch),
+                   "r"(v[j].x), "r"(v[j].y), "r"(v[j].z), "r"(v[j].w)
+                   : "memory");
+    __syncwarp();
+  };
   int load_slot = 0;
   auto load_stage = [&](int i) {
     if (i < stages) {
       const char* src = src0 + i * kRowBytes;  // of the slice's stage i
       const uint32_t dst = dst0 + load_slot * kStageBytes;
       const int rest = rest0 - i * kRowBytes;
-      if (S::ALIGN == 16 && my_row0 + 16 <= row_end &&
+      if (S::ALIGNED && my_row0 + 16 <= row_end &&
           byte0 + (i + 1) * kRowBytes <= row_bytes) {  // all of it exists
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 4 * j * kRowPitch),
                        "l"(src + j * step4)
                        : "memory");
-      } else if (S::ALIGN == 2) {
-        // rows at 2 bytes: the aligned pieces that hold these, all eight loads first; what is too
-        // near to an end of the weights for that, value by value
-        StagePair v[4];
-        auto valid = [&](int j) { return 4 * j < rows_in ? min(max(rest, 0), 16) : 0; };
-        auto inside = [&](int j) {
-          const char* p = src + j * step4;
-          return valid(j) > 0 && p - 15 >= w_begin && p + 32 <= w_end;
-        };
+      } else if (!S::ALIGNED) {
+        // rows at 2 or 4 bytes: the nine aligned pieces that hold the stage's 128, which realign() moves
+        // to their places once they are here
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (inside(j)) v[j] = stage_load(src + j * step4, valid(j));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (inside(j)) {
-            const int s = (int)(reinterpret_cast<uintptr_t>(src + j * step4) & 15);
-            const uint4 q = stage_shift(v[j], s, valid(j));
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 4 * j * kRowPitch),
-                         "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w)
-                         : "memory");
-          } else {
-            copy16<S::ALIGN>(dst + 4 * j * kRowPitch,
-                             valid(j) ? src + j * step4 : static_cast<const char*>(g.w), valid(j));
-          }
-        }
+          copy_aligned(dst + 4 * j * kRowPitch, src + j * step4, 4 * j < rows_in ? rest : -16);
+        if (lane < 16)
+          copy_aligned(dst9 + load_slot * kStageBytes, src9 + i * kRowBytes,
+                       lane < row_end - my_row0 ? rest9 - i * kRowBytes : -16);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int valid = 4 * j < rows_in ? min(max(rest, 0), 16) : 0;
-          copy16<S::ALIGN>(dst + 4 * j * kRowPitch,
-                           valid ? src + j * step4 : static_cast<const char*>(g.w), valid);
+          copy16(dst + 4 * j * kRowPitch,
+                 valid ? src + j * step4 : static_cast<const char*>(g.w), valid);
         }
       }
     }
@@ -461,11 +477,14 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
           if (g.x_vec && k + 8 <= k_end) {
             next_tokens[q][p] = __ldg(reinterpret_cast<const uint4*>(token_row[q] + k));
           } else {
-            uint32_t v[4] = {0, 0, 0, 0};
+            // (all loads without a test between them, which would wait for each)
+            uint32_t v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (k + j < k_end) v[j / 2] |= (uint32_t)token_row[q][k + j] << (16 * (j & 1));
-            next_tokens[q][p] = make_uint4(v[0], v[1], v[2], v[3]);
+            for (int j = 0; j < 8; ++j) v[j] = __ldg(token_row[q] + min(k + j, k_end - 1));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = k + j < k_end ? v[j] : 0;
+            next_tokens[q][p] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16,
+                                           v[4] | v[5] << 16, v[6] | v[7] << 16);
           }
         }
       }
@@ -530,6 +549,7 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
     if (i + 1 < stages) fetch_scales();
     asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
     __syncwarp();
+    if constexpr (!S::ALIGNED) realign(i, slot);
     const uint8_t* st = ring + slot * kStageBytes;
     slot = slot + 1 == kRing ? 0 : slot + 1;
     if constexpr (W4) {
@@ -724,40 +744,35 @@ cudaError_t launch_few_shape(FewArgs g, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, k_grouped_few<S>, g);
 }
 
-template <typename T, int SHIFT, bool ZEROS, int ALIGN, int FINISH = PLAIN>
+template <typename T, int SHIFT, bool ZEROS, bool ALIGNED, int FINISH = PLAIN>
 cudaError_t launch_few_rows(const FewArgs& g, cudaStream_t st) {
   // Items of 8 rows while few experts can have more: no test for absent column tiles in the
   // inner loop, and the tokens of twice the inner length in shared memory.
   return g.rows <= 4 * (int64_t)g.experts || g.rows <= 8
-             ? launch_few_shape<FewShape<T, 1, SHIFT, ZEROS, ALIGN, FINISH>>(g, st)
-             : launch_few_shape<FewShape<T, 4, SHIFT, ZEROS, ALIGN, FINISH>>(g, st);
+             ? launch_few_shape<FewShape<T, 1, SHIFT, ZEROS, ALIGNED, FINISH>>(g, st)
+             : launch_few_shape<FewShape<T, 4, SHIFT, ZEROS, ALIGNED, FINISH>>(g, st);
 }
 
 template <typename T, int FINISH>
-cudaError_t launch_few_finish(const FewArgs& g, int align, cudaStream_t st) {
-  if (align == 16) return launch_few_rows<T, 0, false, 16, FINISH>(g, st);
-  if (align == 4) return launch_few_rows<T, 0, false, 4, FINISH>(g, st);
-  return launch_few_rows<T, 0, false, 2, FINISH>(g, st);
+cudaError_t launch_few_finish(const FewArgs& g, bool aligned, cudaStream_t st) {
+  return aligned ? launch_few_rows<T, 0, false, true, FINISH>(g, st)
+                 : launch_few_rows<T, 0, false, false, FINISH>(g, st);
 }
 
 template <typename T>
-cudaError_t launch_few_typed(const FewArgs& g, int group_size, int align, cudaStream_t st) {
+cudaError_t launch_few_typed(const FewArgs& g, int group_size, bool aligned, cudaStream_t st) {
   if (g.epilogue.on)
-    return g.epilogue.gated ? launch_few_finish<T, FINISH_GATED>(g, align, st)
-                            : launch_few_finish<T, FINISH_LINEAR>(g, align, st);
-  if (group_size == 0) {
-    if (align == 16) return launch_few_rows<T, 0, false, 16>(g, st);
-    if (align == 4) return launch_few_rows<T, 0, false, 4>(g, st);
-    return launch_few_rows<T, 0, false, 2>(g, st);
-  }
+    return g.epilogue.gated ? launch_few_finish<T, FINISH_GATED>(g, aligned, st)
+                            : launch_few_finish<T, FINISH_LINEAR>(g, aligned, st);
+  if (group_size == 0) return launch_few_finish<T, PLAIN>(g, aligned, st);
   if (group_size == 32)
-    return g.zeros ? launch_few_rows<T, 5, true, 16>(g, st)
-                   : launch_few_rows<T, 5, false, 16>(g, st);
+    return g.zeros ? launch_few_rows<T, 5, true, true>(g, st)
+                   : launch_few_rows<T, 5, false, true>(g, st);
   if (group_size == 64)
-    return g.zeros ? launch_few_rows<T, 6, true, 16>(g, st)
-                   : launch_few_rows<T, 6, false, 16>(g, st);
-  return g.zeros ? launch_few_rows<T, 7, true, 16>(g, st)
-                 : launch_few_rows<T, 7, false, 16>(g, st);
+    return g.zeros ? launch_few_rows<T, 6, true, true>(g, st)
+                   : launch_few_rows<T, 6, false, true>(g, st);
+  return g.zeros ? launch_few_rows<T, 7, true, true>(g, st)
+                 : launch_few_rows<T, 7, false, true>(g, st);
 }
 
 }  // namespace
@@ -779,11 +794,10 @@ cudaError_t launch_few(const FewCall& c, cudaStream_t st) {
   g.epilogue = c.epilogue;
   g.cols = c.epilogue.gated ? c.outer / 2 : c.outer;
   g.pre_pitch = pre_pitch(g.cols);
-  int align = 16;
+  bool aligned = true;
   if (c.group_size == 0) {
     g.w_pitch = (int64_t)c.inner * 2;
-    const uintptr_t bits = reinterpret_cast<uintptr_t>(c.w) | (uintptr_t)g.w_pitch;
-    align = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
+    aligned = aligned16(c.w) && g.w_pitch % 16 == 0;
   } else {
     g.w_pitch = (c.inner + 31) / 32 * 16;
     g.scales = c.scales;
@@ -791,8 +805,8 @@ cudaError_t launch_few(const FewCall& c, cudaStream_t st) {
     g.groups = (c.inner + c.group_size - 1) / c.group_size;
   }
   return c.dtype == LGBM_B200_DTYPE_F16
-             ? launch_few_typed<__half>(g, c.group_size, align, st)
-             : launch_few_typed<__nv_bfloat16>(g, c.group_size, align, st);
+             ? launch_few_typed<__half>(g, c.group_size, aligned, st)
+             : launch_few_typed<__nv_bfloat16>(g, c.group_size, aligned, st);
 }
 
 }  // namespace experts
