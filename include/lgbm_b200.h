@@ -616,12 +616,15 @@ int lgbm_b200_experts_matmul_backward(const void* dy, int64_t dy_pitch, const vo
  * the backward pass: [rows][ld], gated [rows][2][ld] (gate, then up), ld = the width rounded up
  * to 16, 32-byte aligned; what lies between the width and ld is not defined. Everything before
  * the results' one rounding is in f32.
- * Workspace: lgbm_b200_experts_matmul_workspace with the same operands (gated: outer =
- * 2 hidden). */
+ * Workspace: lgbm_b200_experts_linear_workspace with the same operands (gated: outer =
+ * 2 hidden). Results overlap none of the inputs. */
 #define LGBM_B200_ACT_NONE 0
 #define LGBM_B200_ACT_RELU 1
 #define LGBM_B200_ACT_SILU 2
 #define LGBM_B200_ACT_GELU 3
+int64_t lgbm_b200_experts_linear_workspace(const void* x, int64_t x_pitch, const int32_t* index,
+                                           const void* w, int64_t rows, int32_t experts,
+                                           int32_t inner, int32_t outer);
 int lgbm_b200_experts_linear(const void* x, int64_t x_rows, int64_t x_pitch,
                              const int32_t* index, const void* w, const void* bias,
                              const void* residual, int64_t residual_pitch, const int32_t* offsets,

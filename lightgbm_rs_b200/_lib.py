@@ -168,6 +168,7 @@ _SIGS = {
                                                      _i32, _i32, _i32], _i64),
     "lgbm_b200_experts_matmul_backward": ([_P, _i64, _P, _i64, _i64, _P, _P, _P, _i32, _i32, _i64,
                                            _i32, _i32, _i32, _P, _P, _P, _i64, _P], ctypes.c_int),
+    "lgbm_b200_experts_linear_workspace": ([_P, _i64, _P, _P, _i64, _i32, _i32, _i32], _i64),
     "lgbm_b200_experts_linear": ([_P, _i64, _i64, _P, _P, _P, _P, _i64, _P, _i32, _i32, _i64, _i32,
                                   _i32, _i32, _P, _P, _P, _i64, _P], ctypes.c_int),
     "lgbm_b200_experts_gated": ([_P, _i64, _i64, _P, _P, _P, _i32, _i32, _i64, _i32, _i32, _i32,

@@ -538,6 +538,24 @@ int lgbm_b200_experts_matmul_backward(const void* dy, int64_t dy_pitch, const vo
   return run_product(what, c, workspace, workspace_bytes, stream);
 }
 
+int64_t lgbm_b200_experts_linear_workspace(const void* x, int64_t x_pitch, const int32_t* index,
+                                           const void* w, int64_t rows, int32_t experts,
+                                           int32_t inner, int32_t outer) {
+  if (rows < 1 || experts < 1 || inner < 1 || outer < 1) return 0;
+  MatmulCall c{};
+  c.x = x;
+  c.x_pitch = x_pitch;
+  c.index = index;
+  c.w = w;
+  c.rows = rows;
+  c.experts = experts;
+  c.inner = inner;
+  c.outer = outer;
+  c.y = &c;  // wanted; not written here
+  c.epilogue.on = true;
+  return matmul_workspace(c);
+}
+
 int lgbm_b200_experts_linear(const void* x, int64_t x_rows, int64_t x_pitch,
                              const int32_t* index, const void* w, const void* bias,
                              const void* residual, int64_t residual_pitch, const int32_t* offsets,

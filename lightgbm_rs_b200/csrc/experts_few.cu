@@ -75,10 +75,19 @@ __device__ __forceinline__ uint32_t shared_addr(const void* p) {
 }
 
 // 16 bytes of global memory to shared, of which the first `valid` (0..16) are read and the
-// rest are zeros; `src` is 16-byte aligned.
+// rest are zeros. ALIGN: of `src`, 16 or 4 bytes.
+template <int ALIGN>
 __device__ __forceinline__ void copy16(uint32_t dst, const char* src, int valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid)
-               : "memory");
+  if constexpr (ALIGN == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid)
+                 : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + i),
+                   "l"(valid > i ? src + i : src), "r"(min(max(valid - i, 0), 4))
+                   : "memory");
+  }
 }
 
 template <typename T>
@@ -154,15 +163,20 @@ __device__ __forceinline__ uint32_t sub2<__nv_bfloat16>(uint32_t a, uint32_t b) 
 enum Finish { PLAIN = 0, FINISH_LINEAR = 1, FINISH_GATED = 2 };
 
 // A kernel's variant: TILES column tiles of 8 rows make an item; SHIFT is log2 of the scale
-// group's size, 0 with weights of 16 bits, whose rows are ALIGNED to 16 bytes or not.
-template <typename T_, int TILES_, int SHIFT_, bool ZEROS_, bool ALIGNED_, int FINISH_ = PLAIN>
+// group's size, 0 with weights of 16 bits, whose rows are aligned to ALIGN bytes.
+template <typename T_, int TILES_, int SHIFT_, bool ZEROS_, int ALIGN_, int FINISH_ = PLAIN>
 struct FewShape {
   using T = T_;
   static constexpr int FINISH = FINISH_;
   // columns of y of a block; gated, half of its warps take gate and half take up
   static constexpr int kOut = FINISH == FINISH_GATED ? kOutBlock / 2 : kOutBlock;
-  static constexpr int TILES = TILES_, SHIFT = SHIFT_;
-  static constexpr bool ALIGNED = ALIGNED_;
+  static constexpr int TILES = TILES_, SHIFT = SHIFT_, ALIGN = ALIGN_;
+  // Rows that start at 2 bytes, and at 4 in items of 8 rows, come as the aligned pieces that hold
+  // them and are moved to their places when they are here; the others at 4 bytes in pieces of 4
+  // bytes, which leaves the items of 32 rows the time (32 experts of 4096 x 2002, 64 rows in all
+  // 156 us moved, 210 in pieces; 256 rows 203 and 189; at 2 bytes, 16 rows, 91 and, loaded by
+  // values, 198).
+  static constexpr bool kRealign = ALIGN == 2 || (ALIGN == 4 && TILES == 1);
   static constexpr bool W4 = SHIFT > 0, ZEROS = ZEROS_;
   // Blocks that share an SM, and stages of a warp's ring: with 4 bits the arithmetic wants
   // warps, with 16 bits the memory wants bytes in flight (4 x 16 KB a block).
@@ -250,30 +264,58 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   const int out0 = blockIdx.x / g.split % g.blocks * S::kOut;
   const int k_begin = rank * g.slice, k_end = min(g.inner, k_begin + g.slice);
   T* y = static_cast<T*>(g.y);
-  // Column n of row `row` of the result, from its product or the gate's and up's.
-  auto finish = [&](int64_t row, int n, float v, float up, bool live) {
+  // The rows of the result from their products, sum(row, column of the block): a thread has one
+  // column (gated, also the one of up) and every step-th row from the first one on, four at a time.
+  // `live`: an expert's rows.
+  auto finish = [&](int first, int step, bool live, auto&& sum) {
     const Epilogue& e = g.epilogue;
+    constexpr int kHalves = S::FINISH == FINISH_GATED ? 2 : 1;
+    const int n = threadIdx.x % S::kOut, col = out0 + n;
+    if (col >= g.cols) return;
+    float bias = 0.0f;
     if (S::FINISH == FINISH_LINEAR && live && e.bias)
-      v += to_f32<T>(static_cast<const T*>(e.bias)[(int64_t)expert * g.cols + n]);
-    if (e.pre) {
-      constexpr int kHalves = S::FINISH == FINISH_GATED ? 2 : 1;
-      T* pre = static_cast<T*>(e.pre) + row * kHalves * g.pre_pitch + n;
-      *pre = from_f32<T>(v);
-      if (kHalves == 2) pre[g.pre_pitch] = from_f32<T>(up);
+      bias = to_f32<T>(static_cast<const T*>(e.bias)[(int64_t)expert * g.cols + col]);
+    T* const out = y + (int64_t)begin * g.cols + col;
+    T* const pre = static_cast<T*>(e.pre) + (int64_t)begin * kHalves * g.pre_pitch + col;
+    const T* const residual =
+        static_cast<const T*>(e.residual) + (int64_t)begin * e.residual_pitch + col;
+    for (int r = first; r < nrows; r += 4 * step) {
+      float v[4], up[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[k] = 0.0f;
+        up[k] = 0.0f;
+        if (r + k * step < nrows) {
+          v[k] = sum(r + k * step, n);
+          if (kHalves == 2) up[k] = sum(r + k * step, n + S::kOut);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] += bias;
+      if (e.pre) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (r + k * step < nrows) {
+            T* p = pre + (int64_t)(r + k * step) * kHalves * g.pre_pitch;
+            *p = from_f32<T>(v[k]);
+            if (kHalves == 2) p[g.pre_pitch] = from_f32<T>(up[k]);
+          }
+      }
+      activate(e.act, v);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (r + k * step < nrows) {
+          if (kHalves == 2) v[k] *= up[k];
+          if (S::FINISH == FINISH_LINEAR && e.residual)
+            v[k] += to_f32<T>(residual[(int64_t)(r + k * step) * e.residual_pitch]);
+          out[(int64_t)(r + k * step) * g.cols] = from_f32<T>(v[k]);
+        }
     }
-    float a[1] = {v};
-    activate(e.act, a);
-    if (S::FINISH == FINISH_GATED) a[0] *= up;
-    if (S::FINISH == FINISH_LINEAR && e.residual)
-      a[0] += to_f32<T>(static_cast<const T*>(e.residual)[row * e.residual_pitch + n]);
-    y[row * g.cols + n] = from_f32<T>(a[0]);
   };
+  constexpr int kRowStep = kFewThreads / S::kOut;  // rows of one pass of the block's threads
   if (S::FINISH != PLAIN && expert >= g.experts) {
     if (rank == 0)
-      for (int i = threadIdx.x; i < nrows * S::kOut; i += kFewThreads) {
-        const int n = out0 + i % S::kOut;
-        if (n < g.cols) finish(begin + i / S::kOut, n, 0.0f, 0.0f, false);
-      }
+      finish(threadIdx.x / S::kOut, kRowStep, false, [](int, int) { return 0.0f; });
     return;
   }
   if (expert >= g.experts) {
@@ -357,14 +399,14 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
       const char* src = src0 + i * kRowBytes;  // of the slice's stage i
       const uint32_t dst = dst0 + load_slot * kStageBytes;
       const int rest = rest0 - i * kRowBytes;
-      if (S::ALIGNED && my_row0 + 16 <= row_end &&
+      if (S::ALIGN == 16 && my_row0 + 16 <= row_end &&
           byte0 + (i + 1) * kRowBytes <= row_bytes) {  // all of it exists
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 4 * j * kRowPitch),
                        "l"(src + j * step4)
                        : "memory");
-      } else if (!S::ALIGNED) {
+      } else if (S::kRealign) {
         // rows at 2 or 4 bytes: the nine aligned pieces that hold the stage's 128, which realign() moves
         // to their places once they are here
 #pragma unroll
@@ -377,8 +419,8 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int valid = 4 * j < rows_in ? min(max(rest, 0), 16) : 0;
-          copy16(dst + 4 * j * kRowPitch,
-                 valid ? src + j * step4 : static_cast<const char*>(g.w), valid);
+          copy16<S::ALIGN>(dst + 4 * j * kRowPitch,
+                           valid ? src + j * step4 : static_cast<const char*>(g.w), valid);
         }
       }
     }
@@ -549,7 +591,7 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
     if (i + 1 < stages) fetch_scales();
     asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
     __syncwarp();
-    if constexpr (!S::ALIGNED) realign(i, slot);
+    if constexpr (S::kRealign) realign(i, slot);
     const uint8_t* st = ring + slot * kStageBytes;
     slot = slot + 1 == kRing ? 0 : slot + 1;
     if constexpr (W4) {
@@ -654,24 +696,22 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
       at[kOutBlock + 8] = W4 ? acc[n][3] : total[n][3];
     }
   if constexpr (S::FINISH != PLAIN) {
-    // the whole sum of element i of the blocks' partial sums, in the blocks' order
     cg::cluster_group cluster = cg::this_cluster();
-    if (g.split == 1) __syncthreads();
-    else cluster.sync();
-    auto whole = [&](int i) {
-      if (g.split == 1) return sums[i];
-      float s = 0.0f;
-      for (int r = 0; r < g.split; ++r) s += cluster.map_shared_rank(sums, r)[i];
-      return s;
-    };
-    for (int i = rank * kFewThreads + threadIdx.x; i < nrows * S::kOut;
-         i += g.split * kFewThreads) {
-      const int r = i / S::kOut, n = i % S::kOut;
-      if (out0 + n < g.cols)
-        finish(begin + r, out0 + n, whole(r * kOutBlock + n),
-               S::FINISH == FINISH_GATED ? whole(r * kOutBlock + kOutBlock / 2 + n) : 0.0f, true);
+    if (g.split == 1) {
+      __syncthreads();
+      finish(threadIdx.x / S::kOut, kRowStep, true,
+             [&](int row, int n) { return sums[row * kOutBlock + n]; });
+      return;
     }
-    if (g.split > 1) cluster.sync();
+    cluster.sync();
+    // the blocks' partial sums in the blocks' order
+    finish(rank * kRowStep + threadIdx.x / S::kOut, g.split * kRowStep, true, [&](int row, int n) {
+      float s = 0.0f;
+      for (int r = 0; r < g.split; ++r)
+        s += cluster.map_shared_rank(sums, r)[row * kOutBlock + n];
+      return s;
+    });
+    cluster.sync();
     return;
   }
   if (g.split == 1) {
@@ -744,35 +784,36 @@ cudaError_t launch_few_shape(FewArgs g, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, k_grouped_few<S>, g);
 }
 
-template <typename T, int SHIFT, bool ZEROS, bool ALIGNED, int FINISH = PLAIN>
+template <typename T, int SHIFT, bool ZEROS, int ALIGN, int FINISH = PLAIN>
 cudaError_t launch_few_rows(const FewArgs& g, cudaStream_t st) {
   // Items of 8 rows while few experts can have more: no test for absent column tiles in the
   // inner loop, and the tokens of twice the inner length in shared memory.
   return g.rows <= 4 * (int64_t)g.experts || g.rows <= 8
-             ? launch_few_shape<FewShape<T, 1, SHIFT, ZEROS, ALIGNED, FINISH>>(g, st)
-             : launch_few_shape<FewShape<T, 4, SHIFT, ZEROS, ALIGNED, FINISH>>(g, st);
+             ? launch_few_shape<FewShape<T, 1, SHIFT, ZEROS, ALIGN, FINISH>>(g, st)
+             : launch_few_shape<FewShape<T, 4, SHIFT, ZEROS, ALIGN, FINISH>>(g, st);
 }
 
 template <typename T, int FINISH>
-cudaError_t launch_few_finish(const FewArgs& g, bool aligned, cudaStream_t st) {
-  return aligned ? launch_few_rows<T, 0, false, true, FINISH>(g, st)
-                 : launch_few_rows<T, 0, false, false, FINISH>(g, st);
+cudaError_t launch_few_finish(const FewArgs& g, int align, cudaStream_t st) {
+  if (align == 16) return launch_few_rows<T, 0, false, 16, FINISH>(g, st);
+  if (align == 4) return launch_few_rows<T, 0, false, 4, FINISH>(g, st);
+  return launch_few_rows<T, 0, false, 2, FINISH>(g, st);
 }
 
 template <typename T>
-cudaError_t launch_few_typed(const FewArgs& g, int group_size, bool aligned, cudaStream_t st) {
+cudaError_t launch_few_typed(const FewArgs& g, int group_size, int align, cudaStream_t st) {
   if (g.epilogue.on)
-    return g.epilogue.gated ? launch_few_finish<T, FINISH_GATED>(g, aligned, st)
-                            : launch_few_finish<T, FINISH_LINEAR>(g, aligned, st);
-  if (group_size == 0) return launch_few_finish<T, PLAIN>(g, aligned, st);
+    return g.epilogue.gated ? launch_few_finish<T, FINISH_GATED>(g, align, st)
+                            : launch_few_finish<T, FINISH_LINEAR>(g, align, st);
+  if (group_size == 0) return launch_few_finish<T, PLAIN>(g, align, st);
   if (group_size == 32)
-    return g.zeros ? launch_few_rows<T, 5, true, true>(g, st)
-                   : launch_few_rows<T, 5, false, true>(g, st);
+    return g.zeros ? launch_few_rows<T, 5, true, 16>(g, st)
+                   : launch_few_rows<T, 5, false, 16>(g, st);
   if (group_size == 64)
-    return g.zeros ? launch_few_rows<T, 6, true, true>(g, st)
-                   : launch_few_rows<T, 6, false, true>(g, st);
-  return g.zeros ? launch_few_rows<T, 7, true, true>(g, st)
-                 : launch_few_rows<T, 7, false, true>(g, st);
+    return g.zeros ? launch_few_rows<T, 6, true, 16>(g, st)
+                   : launch_few_rows<T, 6, false, 16>(g, st);
+  return g.zeros ? launch_few_rows<T, 7, true, 16>(g, st)
+                 : launch_few_rows<T, 7, false, 16>(g, st);
 }
 
 }  // namespace
@@ -794,10 +835,11 @@ cudaError_t launch_few(const FewCall& c, cudaStream_t st) {
   g.epilogue = c.epilogue;
   g.cols = c.epilogue.gated ? c.outer / 2 : c.outer;
   g.pre_pitch = pre_pitch(g.cols);
-  bool aligned = true;
+  int align = 16;
   if (c.group_size == 0) {
     g.w_pitch = (int64_t)c.inner * 2;
-    aligned = aligned16(c.w) && g.w_pitch % 16 == 0;
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(c.w) | (uintptr_t)g.w_pitch;
+    align = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
   } else {
     g.w_pitch = (c.inner + 31) / 32 * 16;
     g.scales = c.scales;
@@ -805,8 +847,8 @@ cudaError_t launch_few(const FewCall& c, cudaStream_t st) {
     g.groups = (c.inner + c.group_size - 1) / c.group_size;
   }
   return c.dtype == LGBM_B200_DTYPE_F16
-             ? launch_few_typed<__half>(g, c.group_size, aligned, st)
-             : launch_few_typed<__nv_bfloat16>(g, c.group_size, aligned, st);
+             ? launch_few_typed<__half>(g, c.group_size, align, st)
+             : launch_few_typed<__nv_bfloat16>(g, c.group_size, align, st);
 }
 
 }  // namespace experts

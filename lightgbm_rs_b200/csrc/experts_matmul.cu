@@ -1609,9 +1609,10 @@ cudaError_t join_parts(const float* part, int parts, int64_t count, int experts,
 // - Rows at 4 bytes: to about 24 (32 of 4096 x 2002: 24 rows 253 / 269, 32 289 / 271), fewer where
 //   the last block of 128 outputs is mostly empty (255 of 129 x 700: 8 rows 41.4 / 42.3, 12 47.4
 //   / 44.1, 24 57.0 / 45.4).
-// - Rows at 2 bytes: they come by 2-byte loads, each waited for. Streaming pays while it leaves
-//   out half of the experts (32 of 4096 x 2001: rows of 16 experts 198 / 234, of 20 287 / 240, of
-//   32 383 / 295; 8 of 4096 x 4097: of 4 109 / 149, of 5 183 / 161).
+// - Rows at 2 bytes: while streaming leaves out half of the experts (32 of 4096 x 2001: rows of 16
+//   experts 91 / 230; 8 of 4096 x 4097: of 4 53 / 148). It is the shorter way beyond that, and layers
+//   stream up to 8 rows an expert (32 of 4096 x 2001, all with rows: 1 row 164 / 265, 8 233 / 266,
+//   16 284 / 269), fewer where the last block of outputs is mostly empty.
 constexpr int64_t kSmallWeights = 12 << 20;
 static bool few_rows(const MatmulCall& c) {
   if (!c.y || c.rows > 32 * (int64_t)c.experts) return false;
@@ -1620,7 +1621,10 @@ static bool few_rows(const MatmulCall& c) {
     return c.rows <= 2 * (int64_t)c.experts ||
            (int64_t)c.experts * ((c.outer + 255) / 256) < 148 / 2;
   if (outputs <= kSmallWeights / 2 / c.inner) return true;
-  if (reinterpret_cast<uintptr_t>(c.w) % 4 == 0 && c.inner % 2 == 0)
+  const bool words = reinterpret_cast<uintptr_t>(c.w) % 4 == 0 && c.inner % 2 == 0;
+  if (c.epilogue.on && !words)
+    return c.rows * ((c.outer + 127) / 128 * 128) <= 8 * outputs;
+  if (words)
     return c.rows * ((c.outer + 127) / 128 * 128) <= 24 * outputs;
   return 2 * c.rows <= c.experts;
 }

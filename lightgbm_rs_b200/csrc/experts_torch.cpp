@@ -388,7 +388,7 @@ PyObject* grouped_linear(PyObject* const* a) {
   Tensor y = make(dev, type, {p.rows, p.outer}), pre;
   if (flag(a[7]) && act != LGBM_B200_ACT_NONE)
     pre = make_saved(dev, type, p.rows, false, p.outer);
-  Scratch ws(dev, lgbm_b200_experts_matmul_workspace(
+  Scratch ws(dev, lgbm_b200_experts_linear_workspace(
                       p.x.p(), p.x.pitch, p.ip(), p.w.data_ptr(), p.rows, (int32_t)p.experts,
                       (int32_t)p.inner, (int32_t)p.outer));
   check(lgbm_b200_experts_linear(
@@ -418,7 +418,7 @@ PyObject* grouped_gated(PyObject* const* a) {
   On on(dev);
   Tensor h = make(dev, type, {p.rows, hidden}), pre;
   if (flag(a[5])) pre = make_saved(dev, type, p.rows, true, hidden);
-  Scratch ws(dev, lgbm_b200_experts_matmul_workspace(
+  Scratch ws(dev, lgbm_b200_experts_linear_workspace(
                       p.x.p(), p.x.pitch, p.ip(), p.w.data_ptr(), p.rows, (int32_t)p.experts,
                       (int32_t)p.inner, (int32_t)p.outer));
   check(lgbm_b200_experts_gated(p.x.p(), p.x.rows, p.x.pitch, p.ip(), p.w.data_ptr(),
