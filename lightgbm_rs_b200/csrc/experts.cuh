@@ -1,5 +1,6 @@
 // Shared definitions of the expert-layer operators: routing rows to experts, products
-// grouped by expert, the combination of the experts' rows, dropout, 4-bit products.
+// grouped by expert with and without an epilogue, the combination of the experts' rows, dropout,
+// 4-bit products, the norm of gradients and their clipping.
 //
 // Group offsets, row indices and positions are device data that the host never sees. Every
 // kernel therefore clamps the offsets it reads to the rows it was given and skips an index
@@ -92,7 +93,8 @@ struct Raw {
     for (int i = 0; i < V; ++i)
       if (i < n) {
         if constexpr (sizeof(T) == 4) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
-        else w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p) + i) << (16 * (i & 1));
+        else
+          w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p) + i) << (16 * (i & 1));
       }
     bits = make_uint4(w[0], w[1], w[2], w[3]);
   }

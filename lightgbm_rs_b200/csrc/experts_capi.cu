@@ -270,7 +270,8 @@ int64_t layer_backward_workspace(const void* dy, int64_t dy_pitch, const void* x
   return c.dx || c.dw ? need + matmul_workspace(c) : need;
 }
 
-constexpr int64_t kMaxNormBytes = 1ll << 44;  // of all tensors: their windows are counted in 32 bits
+// Bytes of all tensors of a norm: their windows are counted in 32 bits.
+constexpr int64_t kMaxNormBytes = 1ll << 44;
 
 int run_norm(const char* what, const lgbm_b200_experts_tensor* tensors, int64_t count, bool scale,
              double max_norm, float* norm, void* workspace, int64_t workspace_bytes,

@@ -11,7 +11,9 @@
 // empty, and neither comes near its rate here: a warp multiplies 1 KB of weights in the time
 // in which an SM's share of the memory bandwidth delivers it several times over.) A long
 // inner axis is split over the blocks of a cluster when there are few outputs, and the
-// partial sums meet in distributed shared memory, added in the blocks' order.
+// partial sums meet in distributed shared memory, added in the blocks' order. The epilogue of a
+// linear or gated layer works on those sums; a gated block's warps take 64 rows of gate and 64 of
+// up.
 //
 // 4 bits: two weights a byte, the even one in the low half, so nibble i and i + 4 of a word
 // become a pair of 16-bit numbers with one mask and one subtraction: q | magic is exactly
@@ -407,8 +409,8 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
                        "l"(src + j * step4)
                        : "memory");
       } else if (S::kRealign) {
-        // rows at 2 or 4 bytes: the nine aligned pieces that hold the stage's 128, which realign() moves
-        // to their places once they are here
+        // the nine aligned pieces that hold the stage's 128 bytes, which realign() moves to their
+        // places once they are here
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           copy_aligned(dst + 4 * j * kRowPitch, src + j * step4, 4 * j < rows_in ? rest : -16);

@@ -4,14 +4,28 @@
 //   FORWARD   y[r, n]     = sum_k x[r, k] w[e(r), n, k]
 //   INPUT     dx[r, k]    = sum_n dy[r, n] w[e(r), n, k]
 //   WEIGHT    dw[e, n, k] = sum_{r in group e} dy[r, n] x[r, k]
+//   LINEAR    y = act(FORWARD + bias) + residual
+//   GATED     h = act(gate) up, gate and up the two halves of FORWARD's columns
 //
-// Rows are grouped: group e is rows offsets[e] .. offsets[e + 1]. All three are one kernel:
+// Rows are grouped: group e is rows offsets[e] .. offsets[e + 1]. All are one kernel:
 // D (f32 in tensor memory) += A B over blocks of 64 of the reduction; only the operands'
-// layouts differ. An operand whose reduction axis is contiguous in memory is staged K-major,
-// else MN-major (panels of 64 columns), both with 128-byte swizzle, so nothing is transposed
+// layouts and what becomes of D differ. An operand whose reduction axis is contiguous in memory is
+// staged K-major, else MN-major (panels of 64 columns), both with 128-byte swizzle, so nothing is transposed
 // on the way. A persistent grid walks the tiles of all groups; in every CTA one warp issues
-// TMA loads, one the matrix instructions, and eight write results out of one half of tensor
-// memory while the next tile accumulates in the other.
+// TMA loads, one the matrix instructions, and eight or sixteen write results out of one half of
+// tensor memory while the next tile accumulates in the other. That half is handed back by a
+// relaxed arrival: a release waited for the results on their way to memory (64 inner columns, a
+// tile of 256 x 256: 3.1 us, without that wait 2.2).
+//
+// Epilogues. A GATED tile is half gate and half up: in a pair each CTA loads one of them as its
+// half of B, so that a row of tensor memory holds both for the same outputs. 16 warps take 16 or
+// 32 columns at a time from tensor memory through registers and a staging block to a bulk store,
+// in one body of code for every type and activation; bias and residual are read a tile ahead. What
+// the backward pass needs leaves the same way before the activation. With 64 inner columns, where
+// nothing hides it, an epilogue's tile takes 2.4 us without an activation (the plain product's
+// 2.2), 5.0 with gelu (two special-function instructions and 16 others an output), 4.9 with a
+// residual, 5.7 with gelu and saved values; gated, 256 x 128, 2.3 and 3.1. From 1024 on most of it
+// is under the multiplication.
 //
 // Pairs. A 128 x 256 tile of one CTA takes in 48 KB for each 512 cycles of matrix work: the
 // SMs together ask more of L2 than it gives. Two CTAs of a cluster therefore share a
@@ -48,15 +62,15 @@
 // storing warps: 7e-7 of the result up to 2^16 rows of random sign (1.3e-6 of one sign),
 // 1.0e-6 (1.4e-6) at 2^20, against 1.7e-5 (1.2e-4) of cuBLAS's f32 product.
 //
-// Measured, loops on a warm GPU, equal groups: 65536 rows, 16 experts of 4096 x 2048: y 0.76
-// to 0.91 ms as the power cap lets the clock (1.2 to 1.4 PFLOP/s), dx 0.86 to 0.91, dw 0.90 to
-// 0.92 (bf16) and 1.04 to 1.06 (f32); cuBLAS's batched product of the same size 0.81 to 0.85,
-// 0.81, 0.80 to 0.84. 8192 rows, 8 experts of 4096 x 1024: 58, 63 to 71, 67 us (f32 90)
-// against 57 to 67, 51 to 55, 60 to 70; tensor pipe 52 to 63 % busy; the rest is the last
-// wave, tiles that groups of 1024 and a few rows leave partly empty, and loads at the 64 bytes
-// a cycle that an SM takes from L2. 40009 rows, 255 experts of 136 x 704: y 32, dx 49, dw 48
-// and 59 us, 2 to 3 TB/s: two or three blocks of reduction a tile, bound by writing tiles out.
-// (Dealing dw's tiles out longest group first gained nothing.)
+// Measured, loops, equal groups: 65536 rows, 16 experts of 4096 x 2048: y 0.76 to 0.88 ms as the
+// power cap lets the clock (1.2 to 1.4 PFLOP/s), dx 0.76 to 0.86, dw 0.78 to 0.90 (bf16) and 0.89
+// to 1.05 (f32); cuBLAS's batched product of the same size 0.81 to 0.85, 0.81, 0.80 to 0.84. 8192
+// rows, 8 experts of 4096 x 1024: 56, 56, 57 us (f32 74; under the cap 70, 63, 61) against 57 to
+// 67, 51 to 55, 60 to 70; tensor pipe 53 to 64 % busy; the rest is the last wave, tiles that groups
+// of 1024 and a few rows leave partly empty, and loads at the 64 bytes a cycle that an SM takes
+// from L2. 40009 rows, 255 experts of 136 x 704: y 30, dx 36, dw 37 and 45 us, 2 to 3 TB/s: two or
+// three blocks of reduction a tile, bound by writing tiles out. (Dealing dw's tiles out longest
+// group first gained nothing.)
 #include <algorithm>
 #include <atomic>
 #include <mutex>
@@ -1610,8 +1624,8 @@ cudaError_t join_parts(const float* part, int parts, int64_t count, int experts,
 //   the last block of 128 outputs is mostly empty (255 of 129 x 700: 8 rows 41.4 / 42.3, 12 47.4
 //   / 44.1, 24 57.0 / 45.4).
 // - Rows at 2 bytes: while streaming leaves out half of the experts (32 of 4096 x 2001: rows of 16
-//   experts 91 / 230; 8 of 4096 x 4097: of 4 53 / 148). It is the shorter way beyond that, and layers
-//   stream up to 8 rows an expert (32 of 4096 x 2001, all with rows: 1 row 164 / 265, 8 233 / 266,
+//   experts 91 / 230; 8 of 4096 x 4097: of 4 53 / 148). It is the shorter way beyond that, and
+//   layers stream up to 8 rows an expert (32 of 4096 x 2001, all with rows: 1 row 164 / 265, 8 233 / 266,
 //   16 284 / 269), fewer where the last block of outputs is mostly empty.
 constexpr int64_t kSmallWeights = 12 << 20;
 static bool few_rows(const MatmulCall& c) {

@@ -4,16 +4,22 @@
 //
 // Tensors of any number, size, type and alignment in one launch: a table of them is a kernel
 // argument (1024 a launch), which the first kernel leaves in memory for the second (30 KB of
-// arguments cost the host 7 us a launch). Each is cut into windows of 32 KB of memory that start at 16 bytes; a
-// block takes an equal share of all windows, one behind the other, so that one large tensor and a
-// thousand small ones are the same work. A thread has 8 loads of 16 bytes in flight. The scaling
-// kernel sums the blocks' partial sums itself (592 a launch of 1024 tensors) and walks each block's
-// windows from the last to the first: what the first pass read last is still in L2.
+// arguments cost the host 7 us a launch). Each is cut into windows of 32 KB of memory that start at
+// 16 bytes; a block takes an equal share of all windows, one behind the other, so that one large
+// tensor and a thousand small ones are the same work. A thread has 8 loads of 16 bytes in flight.
+// The scaling kernel sums the blocks' partial sums itself (592 a launch of 1024 tensors) and walks
+// each block's windows from the last to the first: what the first pass read last is still in L2.
 //
 // Sums. 32 or 64 squares of a thread in f32, then f64. A thread whose f32 sum left the range where
 // that is safe (squares overflow from 1.8e19 on, those below 1e-22 lose digits) takes its values
 // again in f64, so the norm is right wherever f32 can hold it. Blocks' sums are added in one
 // order: the same tensors give the same bits.
+//
+// Measured, clipped into other memory: 201 million f32 values in 12 tensors 392 us, of which the
+// sum is 119 (6.8 TB/s) and the scaling 267 (6.0); 60 million of three types in 1021 tensors 75,
+// 28 and 43 (a quarter of the windows are a tensor's ends); 150001 in 5 tensors 6.3, the launch and
+// three latencies. Tried without gain: a window ahead in registers (half the blocks an SM), 5 and
+// 6 blocks an SM, each window's pieces tested one by one.
 #include <algorithm>
 #include <cmath>
 
@@ -65,7 +71,8 @@ __device__ __noinline__ void edge_store(uint4 v, char* to, int from, int end) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 16; i += 2)
-    if (i >= from && i < end) *reinterpret_cast<uint16_t*>(to + i) = (uint16_t)(w[i / 4] >> (8 * (i & 2)));
+    if (i >= from && i < end)
+      *reinterpret_cast<uint16_t*>(to + i) = (uint16_t)(w[i / 4] >> (8 * (i & 2)));
 }
 
 template <typename T>

@@ -5,21 +5,31 @@ for every token from a gate's logits (experts masked with -inf are never picked:
 all but those of the leaf a tree sends the token to) and groups the T * k slots by expert;
 `grouped_matmul` multiplies each expert's ragged range of rows by its matrix; `combine` joins
 a token's k results; `dropout` regularises while training. Each has its gradient beside it.
-`grouped_matmul_w4` serves a few rows from weights of 4 bits. The trees do not call these
-functions; examples/leaf_experts.py joins both.
+`grouped_gated` and `grouped_linear` are products with what follows them in the same pass: the
+gated half of a feed-forward layer, or bias, activation and residual. `clip_grads` scales a step's
+gradients to a largest norm. `grouped_matmul_w4` serves a few rows from weights of 4 bits. The trees
+do not call these functions; examples/leaf_experts.py joins both.
 
     r = experts.route(logits, k)                                # [T, E]
     h = experts.grouped_matmul(x, w1, r.offsets, rows=r.rows)   # x [T, K], w1 [E, H, K]
     y = experts.grouped_matmul(h, w2, r.offsets)                # w2 [E, N, H]
     out = experts.combine(y, r.position, r.weights)             # [T, N]
 
+or, with a gated layer and its gradients,
+
+    h, pre = experts.grouped_gated(x, w1, r.offsets, rows=r.rows, save=True)  # w1 [E, 2 H, K]
+    y = experts.grouped_linear(h, w2, r.offsets, bias=b2)
+    dh, dw2, db2 = experts.grouped_linear_backward(dy, None, h, w2, r.offsets)
+    dx, dw1 = experts.grouped_gated_backward(dh, pre, x, w1, r.offsets, rows=r.rows)
+    norm = experts.clip_grads([dw1, dw2, db2], 1.0)
+
 Inputs and results are torch tensors on one CUDA device; the work is enqueued on torch's
 current stream of that device and scratch comes from torch's allocator on that stream.
-Matrices of rows (x, y, dy, dout, logits, dropout's 2-D inputs) may have any row stride; one
-whose last axis is not contiguous is copied first. Other tensors (w, q, scales, positions) are
-copied first when they are not contiguous as a whole: keep w as [E, outer, inner]. The products
-also copy, on the device, operands that the tensor cores' loads cannot walk: x read through
-`rows`, and x, dy or w whose rows do not start at multiples of 16 bytes.
+Matrices of rows (x, y, dy, dh, dout, residual, logits, dropout's 2-D inputs) may have any row
+stride; one whose last axis is not contiguous is copied first. Other tensors (w, bias, q, scales,
+positions) are copied first when they are not contiguous as a whole: keep w as [E, outer, inner].
+The products also copy, on the device, operands that the tensor cores' loads cannot walk: x read
+through `rows`, and x, dy or w whose rows do not start at multiples of 16 bytes.
 The functions call the C ABI (lgbm_b200_experts_* in include/lgbm_b200.h) through the
 extension module built beside the library, and raise LightGBMError for arguments it refuses;
 there is no CPU path. Nothing is recorded for autograd: under gradient mode an input that requires

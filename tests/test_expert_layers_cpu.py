@@ -1,5 +1,5 @@
-"""CPU checks of the gated and linear layers and of clipping: what must not reach a device is refused
-with a status and a message before anything touches one."""
+"""CPU checks of the gated and linear layers and of clipping: what must not reach a device is
+refused with a status and a message before anything touches one."""
 
 import ctypes
 
@@ -25,7 +25,8 @@ CALLS = {
     "gated": ([P, 4, 8, P, P, P, 1, 2, 4, 2, 8, 8, P, P, P, N, None],
               [(0, 1), (3, 2), (4, 1), (5, 2), (12, 1), (13, 16)]),
     "linear_backward": ([P, 8, P, P, 4, 8, P, P, P, 1, 0, 2, 4, 2, 8, 8, P, P, P, P, N, None],
-                        [(0, 1), (2, 16), (3, 1), (6, 2), (7, 1), (8, 2), (16, 1), (17, 2), (18, 2)]),
+                        [(0, 1), (2, 16), (3, 1), (6, 2), (7, 1), (8, 2), (16, 1), (17, 2),
+                         (18, 2)]),
     "gated_backward": ([P, 8, P, P, 4, 8, P, P, P, 1, 0, 2, 4, 2, 8, 8, P, P, P, N, None],
                        [(0, 1), (2, 16), (3, 1), (6, 2), (7, 1), (8, 2), (16, 1), (17, 2)]),
 }
@@ -115,8 +116,8 @@ def test_clipping_refuses(capi):
 
     def clip(items, most=1.0, norm=P, ws=P, size=N, n=None):
         a = (Item * max(1, len(items)))(*[Item(*i, 0) for i in items])
-        return L.lgbm_b200_experts_clip_grads(a, len(items) if n is None else n, most, norm, ws, size,
-                                              None)
+        return L.lgbm_b200_experts_clip_grads(a, len(items) if n is None else n, most, norm, ws,
+                                              size, None)
 
     assert clip([(P, P, 5, 3)]) == bad              # dtype
     assert clip([(P, P, -1, 0)]) == bad

@@ -147,7 +147,8 @@ def test_gated(ops, counts, tail, inner, outer, act, dtype):
     gate, up = pre[:, 0].double(), pre[:, 1].double()
     a, s = activation64(act, gate)
     dpre = torch.cat([d * up * s, d * a], 1)
-    err = torch.cat([(d * up).abs() * (SLOPE + 2.0 ** -22), (d * a).abs() * (VALUE + 2.0 ** -22)], 1)
+    err = torch.cat([(d * up).abs() * (SLOPE + 2.0 ** -22),
+                     (d * a).abs() * (VALUE + 2.0 ** -22)], 1)
     err += UNIT[dt] * (dpre.abs() + err) + (dpre != 0) * 2.0 ** -25
     dx64, xb, dw64, wb = gradients64(dpre, err, x, w, off)
     close(dx, dx64, xb)
@@ -252,8 +253,8 @@ def test_through_rows_is_the_gathered_call(ops, rows, inner, outer):
 @pytest.mark.parametrize("shift", [0, 1, 2, 4, 8])
 @pytest.mark.parametrize("rows,inner,outer", SIZES)
 def test_operands_at_any_address(ops, rows, inner, outer, shift):
-    """x, w, bias, residual, dy and pre somewhere inside larger memory, with row pitches of their own
-    and NaN around them: the same results as from memory of their own."""
+    """x, w, bias, residual, dy and pre somewhere inside larger memory, with row pitches of their
+    own and NaN around them: the same results as from memory of their own."""
     g, x, w, dy, off = small(8, rows, inner, outer)
     b = torch.randn(3, outer, generator=g, device="cuda").to(x.dtype)
     res = torch.randn(rows, outer, generator=g, device="cuda").to(x.dtype)
@@ -369,11 +370,13 @@ def test_activations_over_their_range(ops, act, dtype):
 
 def test_neighbours_do_not_leak(ops):
     """An expert's infinities and NaN, in rows, weights and bias, stay in its own results."""
-    for counts, inner, outer in (([37, 50, 41], 96, 72), ([200, 77, 300], 264, 272), ([3, 2, 4], 40, 24)):
+    for counts, inner, outer in (([37, 50, 41], 96, 72), ([200, 77, 300], 264, 272),
+                                 ([3, 2, 4], 40, 24)):
         g = gen(14)
         m = sum(counts)
         bf = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.bfloat16)  # noqa
-        x, w, w2, b, dy = bf(m, inner), bf(3, outer, inner), bf(3, 2 * outer, inner), bf(3, outer), bf(m, outer)
+        x, w, w2 = bf(m, inner), bf(3, outer, inner), bf(3, 2 * outer, inner)
+        b, dy = bf(3, outer), bf(m, outer)
         off = offsets_of(counts)
         s = slice(counts[0], counts[0] + counts[1])
 
@@ -396,7 +399,8 @@ def test_neighbours_do_not_leak(ops):
 def test_gradients_by_differences(ops, kind):
     """Directional differences of <dy, layer> in f64, whose error is h^2 / 6 of a third derivative
     (below 1e-4 of the slope at h = 1e-3), against the gradients; these hold at most three
-    roundings to 16 bits a factor (pre, dpre, the result): 3 * 2^-11 of the terms' 2-norms in f16."""
+    roundings to 16 bits a factor (pre, dpre, the result): 3 * 2^-11 of the terms' 2-norms in
+    f16."""
     halves = 2 if kind == "gated" else 1
     g, x, w, dy, off = small(15, 90, 40, 24, halves=halves, dt=torch.float16)
     b = torch.randn(3, 24, generator=g, device="cuda").to(torch.float16)
@@ -450,7 +454,8 @@ def block_inputs(seed, T=150, E=6, K=24, H=40, N=16):
             torch.randn(T, E, generator=g, device="cuda"), bf(T, N), bf(2 * T, N)]
 
 
-@pytest.mark.parametrize("sizes", [(150, 6, 24, 40, 16), (3000, 8, 72, 129, 40), (7, 9, 130, 33, 20)])
+@pytest.mark.parametrize("sizes", [(150, 6, 24, 40, 16), (3000, 8, 72, 129, 40),
+                                   (7, 9, 130, 33, 20)])
 def test_block_against_autograd(ops, sizes):
     """The operators together, tokens shared by two experts each, against torch's autograd in f64
     on the same bf16 weights. On the way to a gradient at most seven results are rounded to bf16
@@ -472,12 +477,14 @@ def test_block_against_autograd(ops, sizes):
         for k in range(E):
             at = (e[:, j] == k).nonzero()[:, 0]
             q = p[0][at] @ p[1][k].T
-            parts.append((at, (torch.nn.functional.silu(q[:, :H]) * q[:, H:]) @ p[2][k].T + p[3][k]))
+            h = torch.nn.functional.silu(q[:, :H]) * q[:, H:]
+            parts.append((at, h @ p[2][k].T + p[3][k]))
         order = torch.cat([a for a, _ in parts])
         y = y + torch.cat([v for _, v in parts])[order.argsort()]
         ref = ref + wt[:, j:j + 1] * y
     want = torch.autograd.grad(ref, p, dout.double())
     total = math.sqrt(sum(float(g.square().sum()) for g in want))
+    ref = ref.detach()
     assert float((out.double() - ref).norm() / ref.norm()) < 7 * 2.0 ** -8
     assert abs(float(norm) / total - 1) < 7 * 2.0 ** -8
     for a, b in zip(grads, want):

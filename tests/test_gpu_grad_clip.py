@@ -1,8 +1,8 @@
 """The norm of many gradients and their clipping, against 64 bits.
 
-A thread adds 32 (f32) or 64 squares in two chains of f32, so a square is rounded once and added up
-to 32 times: at most 34 * 2^-24 of the sum of squares, half of that of the norm; what follows is f64.
-The norm's one rounding adds 2^-24. A result is a value times a factor that holds the norm's
+A thread adds 32 (f32) or 64 squares in two chains of f32, so a square is rounded once and added
+up to 32 times: at most 34 * 2^-24 of the sum of squares, half of that of the norm; what follows
+is f64. The norm's one rounding adds 2^-24. A result is a value times a factor that holds the norm's
 error and a rounding, rounded twice (once to f32, once to its type).
 """
 
