@@ -573,6 +573,9 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
       asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.b) : "memory");
     }
   } else if (warp == 1) {
+    // Not while the kernel before runs: a block that holds columns and waits for a kernel one of
+    // whose blocks waits for columns would wait for good. (Behind the offsets' reads: no time.)
+    wait_for_stream();
     if constexpr (CTAS == 2) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                        smem_addr(tmem_slot)),
@@ -639,10 +642,10 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
     }
     if (lane == 0) cum[groups] = carry;
   }
-  if (warp != 2) wait_for_stream();
-  let_next_start();
+  if (warp != 1 && warp != 2) wait_for_stream();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  let_next_start();  // this block has its columns
   if constexpr (CTAS == 2) cluster_sync();  // the other CTA's barriers are set up too
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
