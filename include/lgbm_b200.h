@@ -713,7 +713,8 @@ int lgbm_b200_experts_dropout(const void* x, const void* residual, int32_t dtype
  * of all tensors, summed so that it is right wherever f32 can hold it. clip_grads also writes
  * out = in * min(1, max_norm / norm), rounded once: in place where out == in (then left alone when
  * the factor is 1), else to other memory that overlaps no tensor read or written. A norm of 0 has
- * the factor 1. Where the norm is infinite the factor is 0, and where it is NaN all results are.
+ * the factor 1, and so has any with an infinite max_norm. Where the norm is infinite and max_norm
+ * is not, the factor is 0; where the norm is NaN all results are.
  * `tensors` is an array of the HOST, read before the call returns; in and out are contiguous
  * arrays on the current device. The order of the tensors is the order of the sum. */
 typedef struct lgbm_b200_experts_tensor {

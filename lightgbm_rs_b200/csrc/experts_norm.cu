@@ -294,9 +294,10 @@ __device__ __forceinline__ void store_pieces(const uint4 (&v)[N], const char* at
     store_pieces<__half, N, THREADS>(v, at, begin, end, out, f);
 }
 
-// The factor that takes norm n to max_norm. A norm of 0 is not above any; NaN stays NaN.
+// The factor that takes norm n to max_norm. A norm of 0 is not above any; NaN stays NaN. A finite
+// max_norm beyond f32 is below an infinite norm only: 0, not the NaN of two infinities.
 __device__ __forceinline__ float factor_of(float n, double max_norm) {
-  return n <= max_norm ? 1.0f : __fdiv_rn((float)max_norm, n);
+  return n <= max_norm ? 1.0f : __fdiv_rn((float)fmin(max_norm, 3.4e38), n);
 }
 
 // Blocks and their windows as in the launch of k_sum_squares that left these entries; last[b] is

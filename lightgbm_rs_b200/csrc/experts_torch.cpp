@@ -66,6 +66,10 @@ int dtype_of(const char* what, const Tensor& t, bool halves) {
 const Tensor& listed(const char* what, PyObject* o) {
   if (!THPVariable_Check(o)) refuse(LGBM_B200_INVALID_ARGUMENT, what, ": want a torch tensor");
   const Tensor& t = THPVariable_Unpack(o);
+  // memory that is not the values: a lazy minus sign (`z.conj().imag`), sparse tensors
+  if (t.layout() != at::kStrided || t.is_neg())
+    refuse(LGBM_B200_INVALID_ARGUMENT, what, ": want tensors whose values are in memory as they "
+           "are, not sparse, not a view with a sign pending (resolve_neg)");
   // nothing is recorded for autograd: a result would lose the gradient without a word
   if (t.requires_grad() && at::GradMode::is_enabled())
     refuse(LGBM_B200_INVALID_ARGUMENT, what, ": an input requires a gradient, which autograd does "

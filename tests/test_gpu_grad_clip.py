@@ -150,6 +150,37 @@ def test_zeros_infinities_and_nan(ops):
     assert float(ops.clip_grads([e], 1.0)) == 0 and float(ops.grad_norm([e, e])) == 0
 
 
+@pytest.mark.parametrize("size", [5, 300_000])
+@pytest.mark.parametrize("max_norm", [1e39, 1.7e308])
+def test_a_largest_norm_beyond_f32(ops, size, max_norm):
+    """Finite, so above every norm of f32 but an infinite one, for which the factor is 0."""
+    a = torch.full((size,), 2.0, device="cuda")
+    ops.clip_grads([a], max_norm)
+    assert (a == 2).all()
+    a[1] = math.inf
+    assert float(ops.clip_grads([a], max_norm)) == math.inf
+    assert torch.isnan(a[1]) and a[0] == 0 and not a[2:].any()
+    a = torch.tensor([1.0, math.inf], device="cuda")
+    assert float(ops.clip_grads([a], math.inf)) == math.inf and a.tolist() == [1, math.inf]
+
+
+def lazy_values():
+    """Tensors whose memory does not hold their values as they are."""
+    z = torch.ones(4, dtype=torch.complex64, device="cuda")
+    return [z.conj().imag, z[:1].conj().imag, torch.ones(3, 3, device="cuda").to_sparse()]
+
+
+@pytest.mark.parametrize("i", range(3))
+def test_lazy_values_are_refused(ops, i):
+    from lightgbm_rs_b200 import LightGBMError
+
+    t = lazy_values()[i]
+    for call in (lambda: ops.grad_norm([t]), lambda: ops.clip_grads([t], 1.0),
+                 lambda: ops.dropout(t, 0.5, 1)):
+        with pytest.raises(LightGBMError, match="want tensors"):
+            call()
+
+
 def test_strides(ops):
     """Transposed tensors are taken as they lie; others go through a copy."""
     g = gen(9)
