@@ -337,6 +337,20 @@ __device__ __forceinline__ void tile_of(int t, int mt, int nt, int band, int& m,
   m = b * band + (r - n * h);
 }
 
+// The last of `groups` that starts at or before t, by a whole warp: two steps for up to 1024. (Every
+// warp asks once a tile, and with 2 or 3 blocks of reduction a tile the search by halves showed.)
+__device__ __forceinline__ int group_of(const int32_t* cum, int groups, int t, int lane) {
+  int lo = 0;
+  while (groups > 1) {
+    const int each = (groups + 31) / 32, i = lane * each;
+    const bool before = i < groups && cum[lo + i] <= t;
+    const int last = 31 - __clz(__ballot_sync(0xFFFFFFFFu, before || lane == 0));
+    lo += last * each;
+    groups = min(each, groups - last * each);
+  }
+  return lo;
+}
+
 // CTAS CTAs share a tile of 128 CTAS rows and BN columns of D. Warp 0 loads, warp 1
 // multiplies, the others write results out.
 template <int KIND, int BN, int CTAS>
@@ -593,7 +607,8 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
     wait_for_stream();
     // The groups' rows, clamped (off[i] to off[i + 1]; overlaps of offsets that decrease are
     // cut off), and the first tile of every group. The rows before the first offset are a group
-    // of their own and so are those past the last; WEIGHT needs neither.
+    // of their own and so are those past the last; WEIGHT needs neither, and its groups all have
+    // the same tiles.
     const int nt = (g.cols + S::kOutCols - 1) / S::kOutCols;
     int32_t carry = 0, reach = 0;
     const int experts = MODE == WEIGHT ? g.experts / g.parts : g.experts;
@@ -626,11 +641,10 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
       off[kLead + g.experts + 1] = (int32_t)g.rows;
     }
     __syncwarp();
-    for (int i0 = 0; i0 < groups; i0 += 32) {
+    for (int i0 = 0; MODE != WEIGHT && i0 < groups; i0 += 32) {
       const int i = i0 + lane;
       int32_t v = 0;
-      if (i < groups)
-        v = ((MODE == WEIGHT ? g.drows : off[i + 1] - off[i]) + S::kRows - 1) / S::kRows * nt;
+      if (i < groups) v = (off[i + 1] - off[i] + S::kRows - 1) / S::kRows * nt;
       int32_t s = v;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -649,8 +663,10 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
   if constexpr (CTAS == 2) cluster_sync();  // the other CTA's barriers are set up too
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  const int tiles = cum[groups] * (KIND == INPUT_F32 ? g.parts : 1);
   const int nt = (g.cols + S::kOutCols - 1) / S::kOutCols;
+  const int each = (g.drows + S::kRows - 1) / S::kRows * nt;  // WEIGHT: tiles of a group
+  const int tiles =
+      MODE == WEIGHT ? groups * each : cum[groups] * (KIND == INPUT_F32 ? g.parts : 1);
   const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   auto decode = [&](int t) {
@@ -660,17 +676,20 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
       t /= g.parts;
       red0 = part * g.part;
     }
-    int lo = 0, hi = groups;  // the last group that starts at or before t
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cum[mid] <= t) lo = mid; else hi = mid;
+    int lo;
+    if (MODE == WEIGHT) {
+      lo = t / each;
+      t -= lo * each;
+    } else {
+      lo = group_of(cum, groups, t, lane);
+      t -= cum[lo];
     }
     const int b = off[lo], e = off[lo + 1];
     Tile r;
     r.expert = lo - kLead;
     int m, n;
     const int drows = MODE == WEIGHT ? g.drows : e - b;
-    tile_of(t - cum[lo], (drows + S::kRows - 1) / S::kRows, nt, S::kBand, m, n);
+    tile_of(t, (drows + S::kRows - 1) / S::kRows, nt, S::kBand, m, n);
     r.n0 = n * S::kOutCols;
     r.m0 = m * S::kRows + rank * kTileM;
     if (MODE == WEIGHT) {
