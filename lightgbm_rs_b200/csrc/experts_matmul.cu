@@ -10,8 +10,8 @@
 // Rows are grouped: group e is rows offsets[e] .. offsets[e + 1]. All are one kernel:
 // D (f32 in tensor memory) += A B over blocks of 64 of the reduction; only the operands'
 // layouts and what becomes of D differ. An operand whose reduction axis is contiguous in memory is
-// staged K-major, else MN-major (panels of 64 columns), both with 128-byte swizzle, so nothing is transposed
-// on the way. A persistent grid walks the tiles of all groups; in every CTA one warp issues
+// staged K-major, else MN-major (panels of 64 columns), both with 128-byte swizzle, so nothing is
+// transposed on the way. A persistent grid walks the tiles of all groups; in every CTA one warp issues
 // TMA loads, one the matrix instructions, and eight or sixteen write results out of one half of
 // tensor memory while the next tile accumulates in the other. That half is handed back by a
 // relaxed arrival: a release waited for the results on their way to memory (64 inner columns, a
@@ -337,8 +337,8 @@ __device__ __forceinline__ void tile_of(int t, int mt, int nt, int band, int& m,
   m = b * band + (r - n * h);
 }
 
-// The last of `groups` that starts at or before t, by a whole warp: two steps for up to 1024. (Every
-// warp asks once a tile, and with 2 or 3 blocks of reduction a tile the search by halves showed.)
+// The last of `groups` that starts at or before t, by a whole warp: two steps for up to 1024.
+// (Every warp asks once a tile; with 2 or 3 blocks of reduction a tile a search by halves showed.)
 __device__ __forceinline__ int group_of(const int32_t* cum, int groups, int t, int lane) {
   int lo = 0;
   while (groups > 1) {
@@ -1647,8 +1647,8 @@ cudaError_t join_parts(const float* part, int parts, int64_t count, int experts,
 //   / 44.1, 24 57.0 / 45.4).
 // - Rows at 2 bytes: while streaming leaves out half of the experts (32 of 4096 x 2001: rows of 16
 //   experts 91 / 230; 8 of 4096 x 4097: of 4 53 / 148). It is the shorter way beyond that, and
-//   layers stream up to 8 rows an expert (32 of 4096 x 2001, all with rows: 1 row 164 / 265, 8 233 / 266,
-//   16 284 / 269), fewer where the last block of outputs is mostly empty.
+//   layers stream up to 8 rows an expert (32 of 4096 x 2001, all with rows: 1 row 164 / 265, 8
+//   233 / 266, 16 284 / 269), fewer where the last block of outputs is mostly empty.
 constexpr int64_t kSmallWeights = 12 << 20;
 static bool few_rows(const MatmulCall& c) {
   if (!c.y || c.rows > 32 * (int64_t)c.experts) return false;
