@@ -610,19 +610,31 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
     // of their own and so are those past the last; WEIGHT needs neither, and its groups all have
     // the same tiles.
     const int nt = (g.cols + S::kOutCols - 1) / S::kOutCols;
+    constexpr int kAtOnce = 8;
     int32_t carry = 0, reach = 0;
     const int experts = MODE == WEIGHT ? g.experts / g.parts : g.experts;
-    for (int i0 = 0; i0 <= experts; i0 += 32) {
-      const int i = i0 + lane;
-      int32_t b = i <= experts ? (int32_t)min(max((int64_t)g.offsets[i], (int64_t)0), g.rows) : 0;
-      b = max(b, reach);
+    for (int i0 = 0; i0 <= experts; i0 += 32 * kAtOnce) {
+      // one wait for memory, not one for every 32 experts (255 of them: 2 us)
+      int32_t raw[kAtOnce];
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int32_t o = __shfl_up_sync(0xFFFFFFFFu, b, d);
-        if (lane >= d) b = max(b, o);
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int i = i0 + 32 * j + lane;
+        raw[j] = i <= experts ? g.offsets[i] : 0;
       }
-      reach = __shfl_sync(0xFFFFFFFFu, b, 31);
-      if (i <= experts) off[kLead + i] = b;
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int i = i0 + 32 * j + lane;
+        if (i0 + 32 * j > experts) break;
+        int32_t b = (int32_t)min(max((int64_t)raw[j], (int64_t)0), g.rows);
+        b = max(b, reach);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int32_t o = __shfl_up_sync(0xFFFFFFFFu, b, d);
+          if (lane >= d) b = max(b, o);
+        }
+        reach = __shfl_sync(0xFFFFFFFFu, b, 31);
+        if (i <= experts) off[kLead + i] = b;
+      }
     }
     if (MODE == WEIGHT && g.parts > 1) {  // each expert's rows in equal parts of whole blocks
       __syncwarp();
