@@ -230,32 +230,45 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   if (warp == 0) {
     int want = blockIdx.x / (g.blocks * g.split);
     bool found = false;
-    for (int i0 = 0; i0 <= g.experts + 1 && !found; i0 += 32) {
-      const int e = i0 + lane;
-      int64_t b = 0, n = 0;
-      if (e <= g.experts + 1) {
-        b = min(max((int64_t)g.offsets[e <= g.experts ? e : 0], (int64_t)0), g.rows);
-        const int64_t end =
-            e < g.experts ? min(max((int64_t)g.offsets[e + 1], b), g.rows) : g.rows;
-        n = end - b;
-        if (e > g.experts) n = b, b = 0;
-      }
-      const int items = (int)((n + kFewRows - 1) / kFewRows);
-      int s = items;
+    // One wait for memory for 128 experts. (A row for the last expert of 255, 128 x 704: 7.9 -> 7.3
+    // us, of 500 9.7 -> 8.3; with 8 experts the longer code costs 0.1.)
+    constexpr int kAtOnce = 4;
+    for (int i0 = 0; i0 <= g.experts + 1 && !found; i0 += 32 * kAtOnce) {
+      int32_t from[kAtOnce], to[kAtOnce];
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xFFFFFFFFu, s, d);
-        if (lane >= d) s += o;
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int e = i0 + 32 * j + lane;
+        from[j] = e <= g.experts + 1 ? g.offsets[e <= g.experts ? e : 0] : 0;
+        to[j] = e < g.experts ? g.offsets[e + 1] : 0;
       }
-      const int first = s - items;
-      if (want >= first && want < s) {
-        item[0] = e;
-        item[1] = (int32_t)(b + (int64_t)(want - first) * kFewRows);
-        item[2] = (int32_t)min(n - (int64_t)(want - first) * kFewRows, (int64_t)kFewRows);
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int e = i0 + 32 * j + lane;
+        if (found || i0 + 32 * j > g.experts + 1) break;
+        int64_t b = 0, n = 0;
+        if (e <= g.experts + 1) {
+          b = min(max((int64_t)from[j], (int64_t)0), g.rows);
+          const int64_t end = e < g.experts ? min(max((int64_t)to[j], b), g.rows) : g.rows;
+          n = end - b;
+          if (e > g.experts) n = b, b = 0;
+        }
+        const int items = (int)((n + kFewRows - 1) / kFewRows);
+        int s = items;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int o = __shfl_up_sync(0xFFFFFFFFu, s, d);
+          if (lane >= d) s += o;
+        }
+        const int first = s - items;
+        if (want >= first && want < s) {
+          item[0] = e;
+          item[1] = (int32_t)(b + (int64_t)(want - first) * kFewRows);
+          item[2] = (int32_t)min(n - (int64_t)(want - first) * kFewRows, (int64_t)kFewRows);
+        }
+        const int total = __shfl_sync(0xFFFFFFFFu, s, 31);
+        found = want < total;
+        want -= total;
       }
-      const int total = __shfl_sync(0xFFFFFFFFu, s, 31);
-      found = want < total;
-      want -= total;
     }
     if (!found && lane == 0) item[0] = -1;
   }

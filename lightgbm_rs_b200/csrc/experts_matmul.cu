@@ -68,7 +68,7 @@
 // rows, 8 experts of 4096 x 1024: 56, 56, 57 us (f32 74; under the cap 70, 63, 61) against 57 to
 // 67, 51 to 55, 60 to 70; tensor pipe 53 to 64 % busy; the rest is the last wave, tiles that groups
 // of 1024 and a few rows leave partly empty, and loads at the 64 bytes a cycle that an SM takes
-// from L2. 40009 rows, 255 experts of 136 x 704: y 30, dx 36, dw 37 and 45 us, 2 to 3 TB/s: two or
+// from L2. 40009 rows, 255 experts of 136 x 704: y 28, dx 32, dw 31 and 42 us, 2 to 3 TB/s: two or
 // three blocks of reduction a tile, bound by writing tiles out. (Dealing dw's tiles out longest
 // group first gained nothing.)
 #include <algorithm>
