@@ -164,6 +164,25 @@ def test_a_largest_norm_beyond_f32(ops, size, max_norm):
     assert float(ops.clip_grads([a], math.inf)) == math.inf and a.tolist() == [1, math.inf]
 
 
+def test_in_inference_mode(ops):
+    with torch.inference_mode():
+        a = torch.full((4,), 3.0, device="cuda")
+        assert float(ops.clip_grads([a], 3.0)) == 6 and a.tolist() == [1.5] * 4
+    with pytest.raises(Exception, match="inference"):  # as for any write outside of that mode
+        ops.clip_grads([a], 1.0)
+    assert a.tolist() == [1.5] * 4 and float(ops.grad_norm([a])) == 3
+
+
+def test_counts_as_a_write_for_autograd(ops):
+    a = torch.full((4,), 3.0, device="cuda")
+    b = torch.zeros(4, device="cuda")
+    before = a._version, b._version
+    ops.clip_grads([a], 3.0, out=[b])
+    assert (a._version, b._version > before[1]) == (before[0], True)
+    ops.clip_grads([a], 3.0)
+    assert a._version > before[0]
+
+
 def lazy_values():
     """Tensors whose memory does not hold their values as they are."""
     z = torch.ones(4, dtype=torch.complex64, device="cuda")
