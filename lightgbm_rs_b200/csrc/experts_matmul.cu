@@ -814,10 +814,10 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
           if (!(ok = bar_wait(end_full + slot, parity))) break;
           const int rest = steps * 16 - valid;
           constexpr int kPanels = (kTileM + S::kCols) / 64;
-          for (int i = lane; i < rest * kPanels * 8; i += 32) {
-            const int panel = i / (rest * 8), row = i / 8 % rest;
-            store_piece(a + panel * 8192 + (valid + row) * 128 + (i & 7) * 16, 0, 0, 0, 0);
-          }
+          for (int row = valid + lane / 8; row < valid + rest; row += 4)
+#pragma unroll
+            for (int panel = 0; panel < kPanels; ++panel)
+              store_piece(a + panel * 8192 + row * 128 + lane % 8 * 16, 0, 0, 0, 0);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (rank == 1) {
