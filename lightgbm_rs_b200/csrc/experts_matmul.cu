@@ -330,9 +330,10 @@ struct Tile {
 
 // Tile `t` of a group of mt x nt tiles: bands of `band` row tiles, column by column inside a
 // band, so that the CTAs at work at one time share a few row tiles and a few column tiles.
-__device__ __forceinline__ void tile_of(int t, int mt, int nt, int band, int& m, int& n) {
-  const int b = t / (band * nt), r = t - b * band * nt;
-  const int h = min(band, mt - b * band);
+__device__ __forceinline__ void tile_of(unsigned t, int mt, int nt, int band, int& m, int& n) {
+  // (divisions are long chains ahead of every tile: of unsigned numbers, and none for one band)
+  const unsigned b = mt <= band ? 0 : t / (unsigned)(band * nt), r = t - b * band * nt;
+  const unsigned h = min(band, (int)(mt - b * band));
   n = r / h;
   m = b * band + (r - n * h);
 }
@@ -690,7 +691,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
     }
     int lo;
     if (MODE == WEIGHT) {
-      lo = t / each;
+      lo = (unsigned)t / (unsigned)each;
       t -= lo * each;
     } else {
       lo = group_of(cum, groups, t, lane);
@@ -709,7 +710,7 @@ __global__ void __launch_bounds__(Shape<KIND, BN, CTAS>::kThreads, Shape<KIND, B
       // group, so that a CTA does not meet the same one in each (their step through the tiles
       // is even).
       const int mt = (g.drows + S::kRows - 1) / S::kRows;
-      m = (m + lo) % mt;
+      m = (unsigned)(m + lo) % (unsigned)mt;
       r.m0 = m * S::kRows + rank * kTileM;
       r.m_end = g.drows;
       r.red0 = b;
