@@ -68,9 +68,10 @@
 // rows, 8 experts of 4096 x 1024: 56, 56, 57 us (f32 74; under the cap 70, 63, 61) against 57 to
 // 67, 51 to 55, 60 to 70; tensor pipe 53 to 64 % busy; the rest is the last wave, tiles that groups
 // of 1024 and a few rows leave partly empty, and loads at the 64 bytes a cycle that an SM takes
-// from L2. 40009 rows, 255 experts of 136 x 704: y 28, dx 32, dw 31 and 42 us, 2 to 3 TB/s: two or
-// three blocks of reduction a tile, bound by writing tiles out. (Dealing dw's tiles out longest
-// group first gained nothing.)
+// from L2. 40009 rows, 255 experts of 136 x 704: y 28, dx 32, dw 29 and 41 us, 2 to 3 TB/s: two or
+// three blocks of reduction a tile, whose chain of waits and decoding loads alone cannot fill.
+// (Dealing dw's tiles out longest group first gained nothing; in equal shares of neighbouring tiles
+// 258 x 700 took 61 for 58 us and 4096 x 2048 of 65536 rows 1369 for 766.)
 #include <algorithm>
 #include <atomic>
 #include <mutex>
