@@ -26,6 +26,22 @@ __device__ __forceinline__ float inverse_fast(float v) {
   return r;
 }
 
+// The larger and the smaller of two numbers; NaN stays NaN.
+__device__ __forceinline__ float not_below(float v, float least) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(least));
+  return r;
+}
+__device__ __forceinline__ float not_above(float v, float most) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
+  return r;
+}
+constexpr float kLargest = 3.402823466e38f;
+
+// value(v), and both: the value a and the slope d of what was saved. A product beyond f16's range
+// is saved as an infinity, so at infinities both() gives its limits: d 1 and a infinite above, d
+// and a 0 below.
 template <int ACT>
 struct Act;
 
@@ -55,9 +71,9 @@ struct Act<LGBM_B200_ACT_SILU> {
     return v * inverse_fast(1.0f + exp_fast(-v));
   }
   static __device__ __forceinline__ void both(float v, float& a, float& d) {
-    const float s = inverse_fast(1.0f + exp_fast(-v));
-    a = v * s;
-    d = s * fmaf(v, 1.0f - s, 1.0f);
+    const float s = inverse_fast(1.0f + exp_fast(-v)), lo = not_below(v, -kLargest);
+    a = lo * s;
+    d = s * fmaf(not_above(lo, kLargest), 1.0f - s, 1.0f);
   }
 };
 
@@ -82,8 +98,9 @@ struct Act<LGBM_B200_ACT_GELU> {
   }
   static __device__ __forceinline__ void both(float v, float& a, float& d) {
     const float e = exp_fast(-0.5f * v * v), q = tail(v, e), p = v < 0.0f ? q : 1.0f - q;
-    a = v * p;
-    d = fmaf(v * 0.39894228f, e, p);  // 1 / sqrt(2 pi)
+    const float lo = not_below(v, -kLargest);
+    a = lo * p;
+    d = fmaf(not_above(lo, kLargest) * 0.39894228f, e, p);  // 1 / sqrt(2 pi)
   }
 };
 

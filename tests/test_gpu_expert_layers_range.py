@@ -1,0 +1,106 @@
+"""Gated and linear expert layers where values leave f16's range or come near to nothing.
+
+Bounds as in test_gpu_expert_layers.py."""
+
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_experts import DTYPES, UNIT, close, gen, offsets_of  # noqa: E402
+from test_gpu_expert_layers import (SLOPE, VALUE, activation64, gradients64,  # noqa: E402
+                                    grouped64, ranges)
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from lightgbm_rs_b200 import experts
+
+    yield experts
+    experts.check_errors()
+
+
+COUNTS = [[2, 0, 3], [150, 90], [1000, 24]]  # streamed, tiles of 64 columns, of 128 and more
+
+
+def overflowing(counts, inner, outer, halves, signs, seed):
+    """f16 inputs whose products are +-84000 in every fourth column `signs` ({column: sign}), in
+    every third row, and ordinary elsewhere."""
+    g = gen(seed)
+    m, E = sum(counts), len(counts)
+    x = torch.randn(m, inner, generator=g, device="cuda")
+    w = torch.randn(E, halves * outer, inner, generator=g, device="cuda") * inner ** -0.5
+    x[:, 0] = 0
+    x[::3, 0] = 300
+    w[:, :, 0] = 0
+    for column, sign in signs.items():
+        w[:, column:outer:4, 0] = 280 * sign
+    dy = torch.randn(m, outer, generator=g, device="cuda")
+    big = torch.zeros(m, dtype=torch.bool, device="cuda")
+    big[::3] = True
+    return x.half(), w.half(), dy.half(), offsets_of(counts), big
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("outer", [24, 140])
+@pytest.mark.parametrize("counts", COUNTS)
+def test_linear_beyond_the_saved_type(ops, counts, outer, act):
+    """A product of +-84000 is saved as an infinity of f16: the activation's slope there is 1 or 0,
+    and all gradients are those of 64 bits."""
+    x, w, dy, off, big = overflowing(counts, 40, outer, 1, {0: 1, 1: -1}, 61)
+    p64, mag = grouped64(x, w, off)
+    y, pre = ops.grouped_linear(x, w, off, activation=act, save=True)
+    infinite = torch.isinf(pre)
+    assert torch.equal(infinite, p64.abs() > 65504) and infinite.any()
+    assert (pre[infinite].double().sign() == p64[infinite].sign()).all()
+    a, _ = activation64(act, p64)
+    close(y, a, 1.3 * 40 * 2.0 ** -23 * mag + (VALUE + 2.0 ** -22) * a.abs())
+    assert (y[infinite & (p64 > 0)] == math.inf).all() and not y[infinite & (p64 < 0)].any()
+    v = torch.where(infinite, p64, pre.double())
+    d = dy.double()
+    dpre = d * activation64(act, v)[1]
+    exact = d.abs() * (SLOPE + 2.0 ** -22)
+    err = exact + UNIT[x.dtype] * (dpre.abs() + exact) + (dpre != 0) * 2.0 ** -25
+    dx64, xb, dw64, wb = gradients64(dpre, err, x, w, off)
+    dx, dw, db = ops.grouped_linear_backward(dy, pre, x, w, off, activation=act)
+    close(dx, dx64, xb)
+    close(dw, dw64, wb)
+    for e, s in enumerate(ranges(off, len(counts))):
+        n = max(1, counts[e])
+        close(db[e], dpre[s].sum(0),
+              exact[s].sum(0) + n * 2.0 ** -23 * (dpre[s].abs() + exact[s]).sum(0))
+        # (close compares NaN's places; nothing here is infinite)
+        assert torch.isfinite(dx[s]).all() and torch.isfinite(dw[e]).all()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("outer", [24, 140])
+@pytest.mark.parametrize("counts", COUNTS)
+def test_gated_far_below_zero(ops, counts, outer, act):
+    """A gate of -84000 is saved as -infinity: h is 0 there, and nothing passes it backwards."""
+    x, w, dh, off, big = overflowing(counts, 40, outer, 2, {1: -1}, 62)
+    p64, mag = grouped64(x, w, off)
+    eps = 1.1 * 40 * 2.0 ** -23 * mag
+    h, pre = ops.grouped_gated(x, w, off, activation=act, save=True)
+    gate, up = p64[:, :outer], p64[:, outer:]
+    infinite = torch.isinf(pre[:, 0])
+    assert torch.equal(infinite, gate < -65504) and infinite.any()
+    a, _ = activation64(act, gate)
+    close(h, a * up, 1.2 * eps[:, :outer] * (up.abs() + eps[:, outer:]) * ~infinite +
+          a.abs() * eps[:, outer:] + (VALUE + 2.0 ** -22) * (a * up).abs())
+    assert not h[infinite].any()
+    gate, up = torch.where(infinite, gate, pre[:, 0].double()), pre[:, 1].double()
+    a, s = activation64(act, gate)
+    d = dh.double()
+    dpre = torch.cat([d * up * s, d * a], 1)
+    err = torch.cat([(d * up).abs() * (SLOPE + 2.0 ** -22), (d * a).abs() * (VALUE + 2.0 ** -22)],
+                    1)
+    err += UNIT[x.dtype] * (dpre.abs() + err) + (dpre != 0) * 2.0 ** -25
+    dx64, xb, dw64, wb = gradients64(dpre, err, x, w, off)
+    dx, dw = ops.grouped_gated_backward(dh, pre, x, w, off, activation=act)
+    close(dx, dx64, xb)
+    close(dw, dw64, wb)
+    assert torch.isfinite(dx).all() and torch.isfinite(dw).all()
