@@ -615,7 +615,7 @@ int lgbm_b200_experts_matmul_backward(const void* dy, int64_t dy_pitch, const vo
  * pre (NULL: not wanted) keeps what the activation was given, rounded to the inputs' type, for
  * the backward pass: [rows][ld], gated [rows][2][ld] (gate, then up), ld = the width rounded up
  * to 16, 32-byte aligned; what lies between the width and ld is not defined. Everything before
- * the results' one rounding is in f32.
+ * the results' one rounding is in f32. In f16 a value beyond 65504 is saved as an infinity.
  * Workspace: lgbm_b200_experts_linear_workspace with the same operands (gated: outer =
  * 2 hidden). Results overlap none of the inputs. */
 #define LGBM_B200_ACT_NONE 0
@@ -641,7 +641,12 @@ int lgbm_b200_experts_gated(const void* x, int64_t x_rows, int64_t x_pitch, cons
  * wanted. The residual's gradient is dy. The gradient of what the activation was given goes to
  * the workspace in the inputs' type, as the matrix products take it: the only rounding between
  * pre and dx, dw, which they hold however wide they are stored. dbias is summed in f32 from its
- * values before that rounding. */
+ * values before that rounding.
+ * The range of f16 holds for these steps too, in f32 dw as well: where |dy act'(pre)|, or
+ * |dh up act'(gate)| or |dh act(gate)|, passes 65504 the values are infinities, and the row of dx
+ * and the row of dw that they enter are not finite; below 2^-25 they are 0. Where pre was saved as
+ * an infinity the slopes are their limits, 1 or 0 (relu, silu, gelu), and act(gate) far below zero
+ * is 0; act(gate) far above and up are infinite factors. bf16 has f32's range. */
 int64_t lgbm_b200_experts_linear_backward_workspace(
     const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, const int32_t* index,
     const void* w, int32_t act, int64_t rows, int32_t experts, int32_t inner, int32_t outer,

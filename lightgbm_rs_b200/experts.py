@@ -125,7 +125,8 @@ def grouped_linear(x, w, offsets, rows=None, bias=None, activation=None, residua
     their type. activation: None, "relu", "silu" or "gelu" (by the normal distribution function).
     Rows of no expert are the residual (0 without one). With save, (y, pre) for
     `grouped_linear_backward`: pre [M, outer] is what the activation was given, rounded to x's
-    type, its rows padded to 32 bytes (None without an activation)."""
+    type (beyond f16's range an infinity), its rows padded to 32 bytes (None without an
+    activation)."""
     y, pre = _X.grouped_linear(x, w, offsets, rows, bias, _act("grouped_linear", activation),
                                residual, save)
     return (y, pre) if save else y
@@ -137,7 +138,8 @@ def grouped_linear_backward(dy, pre, x, w, offsets, rows=None, activation=None, 
     `grouped_matmul_backward` and dbias [E, outer] of type `grad_dtype`; pre is what the call with
     save returned. The residual's gradient is dy. dx and dw are products of dy act'(pre) rounded
     to 16 bits: dw in float32 holds the sum of those without another rounding. One that is not
-    needed is None."""
+    needed is None. In f16 that rounding has f16's range: beyond 65504 the rows of dx and dw that a
+    value enters are not finite, however dw is stored; scale the loss so that it stays below."""
     what = "grouped_linear_backward"
     return _X.grouped_linear_backward(dy, pre, x, w, offsets, rows, _act(what, activation),
                                       _wide(what, grad_dtype, w), need_dx, need_dw, need_dbias)
@@ -156,7 +158,9 @@ def grouped_gated(x, w, offsets, rows=None, activation="silu", save=False):
 def grouped_gated_backward(dh, pre, x, w, offsets, rows=None, activation="silu", grad_dtype=None,
                            need_dx=True, need_dw=True):
     """Gradients of `grouped_gated`: (dx, dw) from dh [M, hidden] and what the call with save
-    returned, as of `grouped_linear_backward`; dw [E, 2 * hidden, inner]."""
+    returned, as of `grouped_linear_backward`; dw [E, 2 * hidden, inner]. In f16 that holds where
+    dh up act'(gate) and dh act(gate) stay below 65504 and so did gate and up; a gate far below zero
+    passes nothing, saved as -infinity or not."""
     what = "grouped_gated_backward"
     return _X.grouped_gated_backward(dh, pre, x, w, offsets, rows, _act(what, activation),
                                      _wide(what, grad_dtype, w), need_dx, need_dw)

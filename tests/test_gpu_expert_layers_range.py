@@ -104,3 +104,61 @@ def test_gated_far_below_zero(ops, counts, outer, act):
     close(dx, dx64, xb)
     close(dw, dw64, wb)
     assert torch.isfinite(dx).all() and torch.isfinite(dw).all()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("counts", COUNTS)
+def test_gated_far_above_zero(ops, counts, act):
+    """A gate of 84000 is saved as infinity: its own gradient is that of 64 bits, and what act(gate)
+    is a factor of, up's, is infinite. Rows and weights that this does not enter keep theirs."""
+    outer = 24
+    x, w, dh, off, big = overflowing(counts, 40, outer, 2, {0: 1}, 63)
+    dh[dh == 0] = 1
+    p64, _ = grouped64(x, w, off)
+    _, pre = ops.grouped_gated(x, w, off, activation=act, save=True)
+    infinite = torch.isinf(pre[:, 0])
+    assert torch.equal(infinite, p64[:, :outer] > 65504) and infinite.any()
+    gate = torch.where(infinite, p64[:, :outer], pre[:, 0].double())
+    up = pre[:, 1].double()
+    a, s = activation64(act, gate)
+    d = dh.double()
+    dpre = torch.cat([d * up * s, torch.where(infinite, 0.0, d * a)], 1)
+    err = torch.cat([(d * up).abs() * (SLOPE + 2.0 ** -22),
+                     torch.where(infinite, 0.0, d * a).abs() * (VALUE + 2.0 ** -22)], 1)
+    err += UNIT[x.dtype] * (dpre.abs() + err) + (dpre != 0) * 2.0 ** -25
+    dx64, xb, dw64, wb = gradients64(dpre, err, x, w, off)
+    dx, dw = ops.grouped_gated_backward(dh, pre, x, w, off, activation=act)
+    assert not torch.isfinite(dx[big]).any()
+    close(dx[~big], dx64[~big], xb[~big])
+    for e, rows in enumerate(ranges(off, len(counts))):
+        enters = torch.zeros(2 * outer, dtype=torch.bool, device="cuda")
+        enters[outer:] = infinite[rows].any(0)
+        close(dw[e][~enters], dw64[e][~enters], wb[e][~enters])
+        assert not torch.isfinite(dw[e][enters][:, 0]).any()
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_gradients_at_the_range_of_f16(ops, wide):
+    """dh up act'(gate) of 60000 is exact, of 72000 an infinity, in f32 weight gradients too: in
+    its own row of dx and of dw and nowhere else."""
+    H, K = 8, 16
+    x = torch.eye(2, K, device="cuda").half()
+    w = torch.zeros(1, 2 * H, K, device="cuda").half()
+    w[0, :H, :2] = 2.0 ** -6                      # gate, slope 1
+    w[0, H:, 0], w[0, H:, 1] = 100.0, 120.0       # up
+    off = offsets_of([2])
+    _, pre = ops.grouped_gated(x, w, off, activation="relu", save=True)
+    dh = torch.zeros(2, H, device="cuda").half()
+    dh[0, 0], dh[1, 0], dh[1, 1] = 600.0, 600.0, 1.0
+    dx, dw = ops.grouped_gated_backward(dh, pre, x, w, off, activation="relu",
+                                        grad_dtype=torch.float32 if wide else None)
+    want = torch.tensor([60000.0 + 600.0 * 100.0, 60000.0 + 600.0 * 120.0], device="cuda") / 64
+    assert torch.equal(dx[0, :2], want.half()) and not dx[0, 2:].any()
+    assert not torch.isfinite(dx[1]).any()
+    assert not torch.isfinite(dw[0, 0]).any()
+    rest = dw[0, 1:].double()
+    exact = torch.zeros_like(rest)
+    exact[0, 1] = 120.0                           # dh up of the second hidden column
+    exact[H - 1, :2] = 600.0 * 2.0 ** -6          # dh act(gate)
+    exact[H, 1] = 2.0 ** -6
+    assert torch.equal(rest, exact)
