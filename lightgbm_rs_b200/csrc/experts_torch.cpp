@@ -747,7 +747,9 @@ PyObject* clip_grads(PyObject* const* a) {
         (o.sizes() != g.sizes() || o.scalar_type() != g.scalar_type() || o.device() != dev))
       refuse(LGBM_B200_LENGTH_MISMATCH, what, ": result ", i, " ", describe(o), ", want ",
              describe(g));
-    if (scale) o.unsafeGetTensorImpl()->bump_version();  // autograd counts writes
+    if (scale && o.is_inference() && !c10::InferenceMode::is_enabled())
+      refuse(LGBM_B200_INVALID_ARGUMENT, what, ": result ", i,
+             " is an inference tensor, which is written in inference mode only");
     if (item.count == 0) continue;
     const bool dense = g.is_non_overlapping_and_dense();
     item.in = g.data_ptr();
@@ -782,12 +784,21 @@ PyObject* clip_grads(PyObject* const* a) {
   Tensor norm = make(dev, at::kFloat, {});
   const int64_t count = (int64_t)items.size();
   Scratch ws(dev, lgbm_b200_experts_norm_workspace(items.data(), count));
-  if (scale)
-    check(lgbm_b200_experts_clip_grads(items.data(), count, max_norm, norm.data_ptr<float>(),
-                                       ws.p(), ws.bytes, on->stream));
-  else
+  if (scale) {
+    const int rc = lgbm_b200_experts_clip_grads(items.data(), count, max_norm,
+                                                norm.data_ptr<float>(), ws.p(), ws.bytes,
+                                                on->stream);
+    // autograd counts writes: a refused call made none, one that failed on the device may have
+    if (rc == LGBM_B200_OK || rc == LGBM_B200_RUNTIME)
+      for (Py_ssize_t i = 0; i < n; ++i)
+        listed(what, PySequence_Fast_GET_ITEM(outs.list ? outs.list : grads.list, i))
+            .unsafeGetTensorImpl()
+            ->bump_version();
+    check(rc);
+  } else {
     check(lgbm_b200_experts_grad_norm(items.data(), count, norm.data_ptr<float>(), ws.p(),
                                       ws.bytes, on->stream));
+  }
   for (const Back& b : back) b.to.copy_(b.from);
   return wrap(norm);
 }
