@@ -241,8 +241,9 @@ def grad_norm(grads):
 def clip_grads(grads, max_norm, out=None):
     """Scales all tensors by min(1, max_norm / grad_norm(grads)) and returns the norm from before.
     In place, or into the tensors of `out` (like grads in shapes and types). What is written must
-    not overlap what another tensor reads or writes. An infinite norm above max_norm makes the
-    factor 0, NaN makes every result NaN: check the norm where gradients may not be finite."""
+    not overlap what another tensor reads or writes; it may lie between its elements, as columns of
+    one matrix do. An infinite norm above max_norm makes the factor 0, NaN makes every result NaN:
+    check the norm where gradients may not be finite."""
     return _X.clip_grads(grads, float(max_norm), out)
 
 

@@ -88,3 +88,90 @@ def test_every_result_counts_as_written(ops):
     ops.grad_norm(grads + [base])
     assert [t._version for t in grads] + [base._version] == before
     assert all(t._version > 0 for t in out)
+
+
+def interleaved():
+    """Tensors that share memory's range and no element of it."""
+    n = lambda *s: torch.randn(*s, device="cuda")  # noqa: E731
+    a, b, c = n(40, 12), n(1001), n(6, 8, 10).bfloat16()
+    d, e = n(30, 2), torch.full((30, 4), 1.5, device="cuda").half()  # bits of f32 may be NaN in f16
+    return {
+        "columns": [a[:, :5], a[:, 5:]],
+        "columns and rows": [a[:20, :5], a[:20, 5:], a[20:]],
+        "every third": [b[::3], b[1::3], b[2::3]],
+        "blocks": [c[:, :4, :5], c[:, :4, 5:], c[:, 4:, ::2], c[:, 4:, 1::2]],
+        "transposed": [a.t()[:5], a.t()[5:7], a[:, 7:]],
+        "many columns": list(n(70, 300).unbind(1)),
+        "two types": [d.view(torch.float16)[:, 0], d.view(torch.float16)[:, 1], d[:, 1]],
+        "two types of numbers": [e[:, 0], e[:, 1], e.view(torch.float32)[:, 1]],
+    }
+
+
+@pytest.mark.parametrize("name", ["columns", "columns and rows", "every third", "blocks",
+                                  "transposed", "many columns", "two types",
+                                  "two types of numbers"])
+def test_tensors_between_one_another(ops, name):
+    """In place and as results: what tensors of their own give, and nothing else is written."""
+    torch.manual_seed(5)
+    same = lambda a, b: torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))  # noqa: E731
+    grads = interleaved()[name]
+    copies = [t.clone() for t in grads]
+    norm = ops.clip_grads(copies, 2.0)
+    held = [t.clone() for t in grads]
+    out = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in grads]
+    assert same(ops.clip_grads(grads, 2.0, out=out), norm)
+    assert all(same(a, b) for a, b in zip(grads, held))
+    assert all(same(a, b) for a, b in zip(out, copies))
+    results = interleaved()[name]
+    assert same(ops.clip_grads(grads, 2.0, out=results), norm)
+    assert all(same(a, b) for a, b in zip(results, copies))
+    assert same(ops.clip_grads(grads, 2.0), norm)
+    assert all(same(a, b) for a, b in zip(grads, copies))
+
+
+def test_strided_overlaps_are_found(ops):
+    """Random strided pieces of one buffer, of 2 and 4 bytes an element: refused when they share a
+    byte, and only then."""
+    import random
+
+    from lightgbm_rs_b200 import LightGBMError
+
+    rng = random.Random(6)
+    buffer = torch.ones(4096, device="cuda")
+    seen = {True: 0, False: 0}
+
+    def piece():
+        flat = buffer.view(torch.float16) if rng.random() < 0.4 else buffer
+        while True:
+            dims = rng.randint(1, 3)
+            size = [rng.randint(1, 7) for _ in range(dims)]
+            stride, reach = [], 0
+            for n in size:  # every element has a place of its own
+                stride.append(reach + rng.randint(1, 9))
+                reach += stride[-1] * (n - 1)
+            order = rng.sample(range(dims), dims)
+            start = rng.randint(0, 150)
+            if start + reach < flat.numel():
+                return flat.as_strided([size[i] for i in order], [stride[i] for i in order], start)
+
+    def places(t):
+        at = [t.storage_offset()]
+        for n, s in zip(t.shape, t.stride()):
+            at = [p + s * i for p in at for i in range(n)]
+        e = t.element_size()
+        return {p * e + k for p in at for k in range(e)}
+
+    for _ in range(400):
+        a, b = piece(), piece()
+        share = bool(places(a) & places(b))
+        buffer.fill_(1)
+        try:
+            ops.clip_grads([a, b], math.inf)
+            refused = False
+        except LightGBMError as e:
+            assert "overlaps" in str(e)
+            refused = True
+        assert refused == share, (a.shape, a.stride(), a.storage_offset(), a.dtype, b.shape,
+                                  b.stride(), b.storage_offset(), b.dtype)
+        seen[share] += 1
+    assert min(seen.values()) > 40
