@@ -243,21 +243,29 @@ __global__ void __launch_bounds__(kThreads)
   if (threadIdx.x == 0) *norm = n;
 }
 
+// What all values are multiplied by, one after the other: f, and 1 but for factors below f32's
+// normal numbers, where f is the power of two at or above the factor and `rest` keeps its digits. (A
+// product with f is then off by 2^-150 at most, and rest is at most 1.)
+struct Factor {
+  float f, rest;
+};
+
 template <typename T>
-__device__ __forceinline__ uint4 scaled(uint4 v, float f) {
+__device__ __forceinline__ uint4 scaled(uint4 v, Factor q) {
+  const auto times = [&](float x) { return x * q.f * q.rest; };
   uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (sizeof(T) == 4) {
-      w[i] = __float_as_uint(__uint_as_float(w[i]) * f);
+      w[i] = __float_as_uint(times(__uint_as_float(w[i])));
     } else {
       const float2 x = values<T>(w[i]);
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        const __nv_bfloat162 q = __floats2bfloat162_rn(x.x * f, x.y * f);
-        w[i] = *reinterpret_cast<const uint32_t*>(&q);
+        const __nv_bfloat162 q2 = __floats2bfloat162_rn(times(x.x), times(x.y));
+        w[i] = *reinterpret_cast<const uint32_t*>(&q2);
       } else {
-        const __half2 q = __floats2half2_rn(x.x * f, x.y * f);
-        w[i] = *reinterpret_cast<const uint32_t*>(&q);
+        const __half2 q2 = __floats2half2_rn(times(x.x), times(x.y));
+        w[i] = *reinterpret_cast<const uint32_t*>(&q2);
       }
     }
   }
@@ -267,7 +275,7 @@ __device__ __forceinline__ uint4 scaled(uint4 v, float f) {
 // Pieces scaled, to the same places from `out` on (where the tensor's first element goes).
 template <typename T, int N, int THREADS>
 __device__ __forceinline__ void store_pieces(const uint4 (&v)[N], const char* at, const char* begin,
-                                             const char* end, char* out, float f) {
+                                             const char* end, char* out, Factor f) {
   // the two start alike: 16 bytes of one are 16 bytes of the other
   const bool alike =
       ((reinterpret_cast<uintptr_t>(begin) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
@@ -285,7 +293,8 @@ __device__ __forceinline__ void store_pieces(const uint4 (&v)[N], const char* at
 }
 template <int N, int THREADS>
 __device__ __forceinline__ void store_pieces(const uint4 (&v)[N], const char* at, const char* begin,
-                                             const char* end, char* out, float f, int dtype) {
+                                             const char* end, char* out, Factor f,
+                                             int dtype) {
   if (dtype == LGBM_B200_DTYPE_F32)
     store_pieces<float, N, THREADS>(v, at, begin, end, out, f);
   else if (dtype == LGBM_B200_DTYPE_BF16)
@@ -296,8 +305,17 @@ __device__ __forceinline__ void store_pieces(const uint4 (&v)[N], const char* at
 
 // The factor that takes norm n to max_norm. A norm of 0 is not above any; NaN stays NaN. A finite
 // max_norm beyond f32 is below an infinite norm only: 0, not the NaN of two infinities.
-__device__ __forceinline__ float factor_of(float n, double max_norm) {
-  return n <= max_norm ? 1.0f : __fdiv_rn((float)fmin(max_norm, 3.4e38), n);
+constexpr float kLargest = 3.402823466e38f, kLeastNormal = 1.175494351e-38f;
+__device__ __noinline__ Factor small_factor(float n, double max_norm) {
+  const double q = max_norm / n;
+  if (!(q > 0.0)) return {0.0f, 1.0f};
+  const int e = max(ilogb(q) + 1, -149);
+  return {ldexpf(1.0f, e), (float)ldexp(q, -e)};
+}
+__device__ __forceinline__ Factor factor_of(float n, double max_norm) {
+  if (n <= max_norm) return {1.0f, 1.0f};
+  const float f = __fdiv_rn((float)fmin(max_norm, (double)kLargest), n);
+  return f < kLeastNormal && n <= kLargest ? small_factor(n, max_norm) : Factor{f, 1.0f};
 }
 
 // Blocks and their windows as in the launch of k_sum_squares that left these entries; last[b] is
@@ -307,7 +325,7 @@ __global__ void __launch_bounds__(kThreads)
             const double* __restrict__ partial, int count, double max_norm,
             float* __restrict__ norm) {
   __shared__ double shared[kThreads / 32];
-  __shared__ float factor;
+  __shared__ Factor factor;
   wait_for_stream();
   let_next_start();
   int item = last[blockIdx.x];
@@ -318,12 +336,12 @@ __global__ void __launch_bounds__(kThreads)
     factor = factor_of(n, max_norm);
   }
   __syncthreads();
-  const float f = factor;
+  const Factor f = factor;
   const int begin = share(windows, blockIdx.x, gridDim.x),
             end = share(windows, blockIdx.x + 1, gridDim.x);
   for (int w = end - 1; w >= begin; --w) {
     while (w < t.first) t = entries[--item];
-    if (f == 1.0f && t.out == t.in) continue;
+    if (f.f == 1.0f && t.out == t.in) continue;
     const char* at = t.in - (reinterpret_cast<uintptr_t>(t.in) & 15) +
                      (int64_t)(w - t.first) * kWindow;
     uint4 v[kPieces];
@@ -342,7 +360,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
             float* __restrict__ norm) {
   __shared__ double warps[kSmallThreads / 32];
   __shared__ double sum;
-  __shared__ float factor;
+  __shared__ Factor factor;
   cg::cluster_group cluster = cg::this_cluster();
   wait_for_stream();
   let_next_start();
@@ -395,7 +413,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
   __syncthreads();
   // this block has read the others' sums; none leaves before all have
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  const float f = factor;
+  const Factor f = factor;
 #pragma unroll
   for (int k = 0; k < kSmallEach; ++k) {
     if (!scale || k >= count) continue;
@@ -403,7 +421,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
     const char *at, *from, *to;
     place(begin + k, i, at, from, to);
     char* out = t.out[i];
-    if (f == 1.0f && out == from) continue;
+    if (f.f == 1.0f && out == from) continue;
     store_pieces<kSmallPieces, kSmallThreads>(v[k], at, from, to, out, f, t.dtype[i]);
   }
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");

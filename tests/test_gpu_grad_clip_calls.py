@@ -11,6 +11,9 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
+from test_gpu_experts import DTYPES, UNIT, gen  # noqa: E402
+from test_gpu_grad_clip import NORM, check_scaled, norm64  # noqa: E402
+
 
 @pytest.fixture(scope="module")
 def ops():
@@ -175,3 +178,33 @@ def test_strided_overlaps_are_found(ops):
                                   b.stride(), b.storage_offset(), b.dtype)
         seen[share] += 1
     assert min(seen.values()) > 40
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [50, 700_000])
+@pytest.mark.parametrize("scale,most", [(1e38, 1e-3), (1e36, 1e-5), (1e30, 1e-20), (1e34, 1e-30),
+                                        (3e37, 2e-7), (1e20, 1e-18), (1.0, 1e-39)])
+def test_factors_below_f32(ops, scale, most, size, dtype):
+    """max_norm / norm from 1e-38 down to 1e-65: the results have the wanted norm where the type
+    holds them, and their digits."""
+    dt = DTYPES[dtype]
+    g = (torch.rand(size, generator=gen(8), device="cuda") * scale / size ** 0.5).to(dt)
+    small = g.clone()
+    small[::2] *= 1e-3
+    grads = [g, small[1:]]  # one that starts off 16 bytes
+    n = norm64(grads)
+    out = [torch.empty_like(t) for t in grads]
+    assert abs(float(ops.clip_grads(grads, most, out=out)) - n) <= NORM * n
+    check_scaled(out, grads, most / n)
+    ops.clip_grads(grads, most)
+    assert all(torch.equal(a, b) for a, b in zip(grads, out))
+    assert abs(norm64(out) / most - 1) < UNIT[dt] + 2.0 ** -16 or most < 1e-35
+
+
+def test_a_norm_at_the_end_of_f32(ops):
+    """Norm and max_norm above 3.4e38, both finite."""
+    top = torch.finfo(torch.float32).max
+    a = torch.full((4,), top / 2, device="cuda")
+    most = top * (1 - 2.0 ** -12)
+    assert float(ops.clip_grads([a], most)) == top
+    assert (a.double() / (top / 2) - (1 - 2.0 ** -12)).abs().max() <= 2.0 ** -22
