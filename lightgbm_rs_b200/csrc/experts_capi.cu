@@ -294,12 +294,15 @@ int run_norm(const char* what, const lgbm_b200_experts_tensor* tensors, int64_t 
                     "%s: tensor %lld: dtype %d, %lld elements, or a null argument", what,
                     (long long)i, t.dtype, (long long)t.count);
     const int size = elem_size(t.dtype);
-    if (t.count > left / size)
+    // (no division a tensor: those of 1021 took the host 5 us)
+    if (t.count > left >> (size == 4 ? 2 : 1))
       return refuse(LGBM_B200_CAPABILITY_UNAVAILABLE, "%s: more than %lld bytes", what,
                     (long long)kMaxNormBytes);
     left -= t.count * size;
-    if (t.count > 0)
-      if (int rc = check_starts(what, {{t.in, size}, {scale ? t.out : nullptr, size}})) return rc;
+    const void* const out = scale ? t.out : nullptr;
+    if (t.count > 0 &&
+        ((reinterpret_cast<uintptr_t>(t.in) | reinterpret_cast<uintptr_t>(out)) & (size - 1)))
+      if (int rc = check_starts(what, {{t.in, size}, {out, size}})) return rc;
   }
   const int64_t need = norm_workspace(tensors, count);
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace))))

@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <memory>
 #include <optional>
 #include <sstream>
 #include <string>
@@ -636,7 +637,7 @@ PyObject* dropout(PyObject* const* a) {
 struct Range {
   uintptr_t begin, end;
   bool written;
-  const Tensor* gaps;  // null: all of it
+  int32_t gaps;  // the tensor's number, -1: all of it
 };
 
 // Whether two ranges that overlap have a byte in common. A byte's place is a sum of strides times
@@ -664,8 +665,8 @@ bool meets(const std::vector<Axis>& axes, size_t left, int64_t by, int64_t reach
     if (meets(axes, left - 1, by - t * x.stride, reach_a, reach_b, trials)) return true;
   return false;
 }
-bool common(const Range& a, const Range& b) {
-  if (!a.gaps && !b.gaps) return true;
+bool common(const Range& a, const Range& b, const std::vector<const Tensor*>& tensors) {
+  if (a.gaps < 0 && b.gaps < 0) return true;
   std::vector<Axis> axes;
   int64_t reach_a = 0, reach_b = 0;
   auto add = [&](const Range& r, int64_t Axis::*more, int64_t& reach) {
@@ -677,11 +678,11 @@ bool common(const Range& a, const Range& b) {
       (*at).*more += size - 1;
       reach += stride * (size - 1);
     };
-    if (!r.gaps) return axis(1, (int64_t)(r.end - r.begin));
-    const int64_t bytes = (int64_t)r.gaps->element_size();
+    if (r.gaps < 0) return axis(1, (int64_t)(r.end - r.begin));
+    const Tensor& t = *tensors[r.gaps];
+    const int64_t bytes = (int64_t)t.element_size();
     axis(1, bytes);
-    for (int64_t d = 0; d < r.gaps->dim(); ++d)
-      axis(r.gaps->stride(d) * bytes, r.gaps->size(d));
+    for (int64_t d = 0; d < t.dim(); ++d) axis(t.stride(d) * bytes, t.size(d));
   };
   add(a, &Axis::more_a, reach_a);
   add(b, &Axis::more_b, reach_b);
@@ -692,36 +693,40 @@ bool common(const Range& a, const Range& b) {
 
 // Memory that is written overlaps nothing else. Sorting the ranges of 1021 tensors in three
 // buffers took 60 us, as long as their kernels; laid one behind the other they are a few hulls.
-bool disjoint(std::vector<Range>& r) {
+[[gnu::noinline]] bool disjoint_sorted(Range* r, size_t n,
+                                       const std::vector<const Tensor*>& tensors) {
+  std::sort(r, r + n, [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  uintptr_t read_end = 0, write_end = 0;  // how far the ranges so far reach
+  for (const Range* v = r; v < r + n; ++v) {
+    if (v->begin < write_end || (v->written && v->begin < read_end))
+      for (const Range* o = r; o < v; ++o)  // tensors may lie in each other's gaps
+        if (o->end > v->begin && (v->written || o->written) && common(*o, *v, tensors))
+          return false;
+    uintptr_t& end = v->written ? write_end : read_end;
+    end = std::max(end, v->end);
+  }
+  return true;
+}
+bool disjoint(Range* r, size_t n, const std::vector<const Tensor*>& tensors) {
   constexpr size_t kMost = 16;
   constexpr uintptr_t kGap = 512;
   Range hull[kMost];
   size_t hulls = 0;
   bool few = true;
-  for (const Range& v : r) {
+  for (const Range* v = r; v < r + n; ++v) {
     size_t i = 0;
-    while (i < hulls && !(v.begin >= hull[i].end && v.begin - hull[i].end <= kGap)) ++i;
+    while (i < hulls && !(v->begin >= hull[i].end && v->begin - hull[i].end <= kGap)) ++i;
     if (i == hulls) {
       if (!(few = hulls < kMost)) break;
-      hull[hulls++] = v;
+      hull[hulls++] = *v;
     } else {
-      hull[i].end = v.end;
+      hull[i].end = v->end;
     }
   }
   for (size_t i = 0; few && i < hulls; ++i)
     for (size_t j = 0; few && j < i; ++j)
       few = hull[i].end <= hull[j].begin || hull[j].end <= hull[i].begin;
-  if (few) return true;
-  std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
-  uintptr_t read_end = 0, write_end = 0;  // how far the ranges so far reach
-  for (const Range& v : r) {
-    if (v.begin < write_end || (v.written && v.begin < read_end))
-      for (const Range* o = r.data(); o < &v; ++o)  // tensors may lie in each other's gaps
-        if (o->end > v.begin && (v.written || o->written) && common(*o, v)) return false;
-    uintptr_t& end = v.written ? write_end : read_end;
-    end = std::max(end, v.end);
-  }
-  return true;
+  return few || disjoint_sorted(r, n, tensors);
 }
 
 // Bytes from a tensor's first element to behind its last.
@@ -775,10 +780,17 @@ PyObject* clip_grads(PyObject* const* a) {
     Tensor to, from;
   };
   std::vector<Back> back;
-  std::vector<lgbm_b200_experts_tensor> items;
-  std::vector<Range> ranges;
-  items.reserve(n);
-  if (scale) ranges.reserve(outs.list ? 2 * n : n);
+  std::vector<const Tensor*> gaps;  // tensors with such, by number
+  const auto with_gaps = [&gaps](uintptr_t p, const Tensor& t, bool writes) {
+    gaps.push_back(&t);
+    return Range{p, p + reach(t), writes, (int32_t)gaps.size() - 1};
+  };
+  // (plain arrays: pushing into vectors took a tenth of a call with 1021 tensors)
+  const std::unique_ptr<lgbm_b200_experts_tensor[]> items(new lgbm_b200_experts_tensor[n]);
+  const std::unique_ptr<Range[]> ranges(new Range[scale ? 2 * n : 0]);
+  lgbm_b200_experts_tensor* items_end = items.get();
+  Range* ranges_end = ranges.get();
+  const bool inference = c10::InferenceMode::is_enabled();
   c10::Device dev(c10::kCUDA);
   std::optional<On> on;
   // (the lists hold their tensors, and nothing here gives up the GIL)
@@ -801,7 +813,7 @@ PyObject* clip_grads(PyObject* const* a) {
         (o.sizes() != g.sizes() || o.scalar_type() != g.scalar_type() || o.device() != dev))
       refuse(LGBM_B200_LENGTH_MISMATCH, what, ": result ", i, " ", describe(o), ", want ",
              describe(g));
-    if (scale && o.is_inference() && !c10::InferenceMode::is_enabled())
+    if (scale && !inference && !o.unsafeGetTensorImpl()->version_counter().enabled())
       refuse(LGBM_B200_INVALID_ARGUMENT, what, ": result ", i,
              " is an inference tensor, which is written in inference mode only");
     if (item.count == 0) continue;
@@ -817,9 +829,9 @@ PyObject* clip_grads(PyObject* const* a) {
                       op = reinterpret_cast<uintptr_t>(item.out);
       const bool alike = !outs.list || g.strides() == o.strides();
       const uintptr_t size = (uintptr_t)item.count * elem_bytes(item.dtype);
-      ranges.push_back({op, op + (out_dense ? size : reach(o)), true, out_dense ? nullptr : &o});
+      *ranges_end++ = out_dense ? Range{op, op + size, true, -1} : with_gaps(op, o, true);
       if (gp != op || !alike)
-        ranges.push_back({gp, gp + (dense ? size : reach(g)), false, dense ? nullptr : &g});
+        *ranges_end++ = dense ? Range{gp, gp + size, false, -1} : with_gaps(gp, g, false);
       if (!(dense && out_dense && alike)) {
         kept.push_back(g.contiguous());
         item.in = kept.back().data_ptr();
@@ -832,26 +844,25 @@ PyObject* clip_grads(PyObject* const* a) {
       kept.push_back(g.contiguous());
       item.in = kept.back().data_ptr();
     }
-    items.push_back(item);
+    *items_end++ = item;
   }
-  if (!disjoint(ranges))
+  if (!disjoint(ranges.get(), ranges_end - ranges.get(), gaps))
     refuse(LGBM_B200_INVALID_ARGUMENT, what, ": a tensor that is written overlaps another one");
   Tensor norm = make(dev, at::kFloat, {});
-  const int64_t count = (int64_t)items.size();
-  Scratch ws(dev, lgbm_b200_experts_norm_workspace(items.data(), count));
+  const int64_t count = items_end - items.get();
+  Scratch ws(dev, lgbm_b200_experts_norm_workspace(items.get(), count));
   if (scale) {
-    const int rc = lgbm_b200_experts_clip_grads(items.data(), count, max_norm,
+    const int rc = lgbm_b200_experts_clip_grads(items.get(), count, max_norm,
                                                 norm.data_ptr<float>(), ws.p(), ws.bytes,
                                                 on->stream);
+    PyObject* const written = outs.list ? outs.list : grads.list;
     // autograd counts writes: a refused call made none, one that failed on the device may have
     if (rc == LGBM_B200_OK || rc == LGBM_B200_RUNTIME)
-      for (Py_ssize_t i = 0; i < n; ++i)
-        listed(what, PySequence_Fast_GET_ITEM(outs.list ? outs.list : grads.list, i))
-            .unsafeGetTensorImpl()
-            ->bump_version();
+      for (PyObject *const *p = PySequence_Fast_ITEMS(written), *const *end = p + n; p < end; ++p)
+        THPVariable_Unpack(*p).unsafeGetTensorImpl()->bump_version();
     check(rc);
   } else {
-    check(lgbm_b200_experts_grad_norm(items.data(), count, norm.data_ptr<float>(), ws.p(),
+    check(lgbm_b200_experts_grad_norm(items.get(), count, norm.data_ptr<float>(), ws.p(),
                                       ws.bytes, on->stream));
   }
   for (const Back& b : back) b.to.copy_(b.from);
