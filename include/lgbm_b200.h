@@ -716,11 +716,11 @@ int lgbm_b200_experts_dropout(const void* x, const void* residual, int32_t dtype
 
 /* A step's gradients: *norm (f32, on the device) = sqrt of the sum of the squares of all elements
  * of all tensors, summed so that it is right wherever f32 can hold it. clip_grads also writes
- * out = in * min(1, max_norm / norm), the factor from the norm's f32 value and itself rounded to
- * f32's 24 bits (with f64's range), the product to f32 and then to out's type: in place where out == in (then left alone when
- * the factor is 1), else to other memory that overlaps no tensor read or written. A norm of 0 has
- * the factor 1, and so has any with an infinite max_norm. Where the norm is infinite and max_norm
- * is not, the factor is 0; where the norm is NaN all results are.
+ * out = in * min(1, max_norm / norm): the factor, from the norm as it is returned, is rounded to 24
+ * bits (in a wider range than f32's), a product to f32 and then to out's type. In place where out
+ * == in (then left alone when the factor is 1), else to other memory that overlaps no tensor read
+ * or written. A norm of 0 has the factor 1, and so has any with an infinite max_norm. Where the
+ * norm is infinite and max_norm is not, the factor is 0; where the norm is NaN all results are.
  * `tensors` is an array of the HOST, read before the call returns; in and out are contiguous
  * arrays on the current device. The order of the tensors is the order of the sum. */
 typedef struct lgbm_b200_experts_tensor {

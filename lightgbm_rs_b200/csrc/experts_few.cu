@@ -222,8 +222,11 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
   uint8_t* ring = smem + S::ring(g.panel) + warp * kRing * kStageBytes;
   const int gq = lane >> 2, tq = lane & 3;  // row and column quad of the matrix fragments
 
+  // (No let_next_start: a kernel's next one may start anyhow when its last block ends. Started
+  // earlier, its blocks take the places of the first to end, two or three to an SM, and the others
+  // stay empty: 8 rows of 8 experts of 4096 x 2048 22.6 us, so 19.4, and 21.5 without any overlap; 4
+  // bits, a row of 8192 x 8192 28.4, 21.6 and 24.5.)
   wait_for_stream();
-  let_next_start();
   // The item of this block: rows [begin, begin + n) of one expert. Items are numbered expert
   // by expert, then the rows past the last offset and those before the first (expert >= experts:
   // zeros).
@@ -533,6 +536,14 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
         if (k < k_end && (lane + 32 * p) * 8 < g.panel) {
           if (g.x_vec && k + 8 <= k_end) {
             next_tokens[q][p] = __ldg(reinterpret_cast<const uint4*>(token_row[q] + k));
+          } else if constexpr (W4) {
+            // (in the registers that the loads below would hold: 64 rows of 8 x 4096 x 4096 51.6
+            // us with those, 47.4 with these, for x at 16 bytes too)
+            uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (k + j < k_end) v[j / 2] |= (uint32_t)token_row[q][k + j] << (16 * (j & 1));
+            next_tokens[q][p] = make_uint4(v[0], v[1], v[2], v[3]);
           } else {
             // (all loads without a test between them, which would wait for each)
             uint32_t v[8];
