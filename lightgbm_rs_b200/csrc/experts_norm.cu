@@ -250,21 +250,36 @@ struct Factor {
   float f, rest;
 };
 
+// Two products in one instruction, so that the second factor costs none. (32 tensors of 27458 f16
+// values in one cluster: 9.25 us as with one factor, by single products 9.48.)
+__device__ __forceinline__ float2 times2(float2 x, float f) {
+  uint64_t a, b, r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(x.x), "f"(x.y));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(b) : "f"(f));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x.x), "=f"(x.y) : "l"(r));
+  return x;
+}
 template <typename T>
 __device__ __forceinline__ uint4 scaled(uint4 v, Factor q) {
-  const auto times = [&](float x) { return x * q.f * q.rest; };
+  const auto times = [&](float2 x) { return times2(times2(x, q.f), q.rest); };
   uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 4) {
-      w[i] = __float_as_uint(times(__uint_as_float(w[i])));
-    } else {
-      const float2 x = values<T>(w[i]);
+    for (int i = 0; i < 4; i += 2) {
+      const float2 x = times(make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1])));
+      w[i] = __float_as_uint(x.x);
+      w[i + 1] = __float_as_uint(x.y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = times(values<T>(w[i]));
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        const __nv_bfloat162 q2 = __floats2bfloat162_rn(times(x.x), times(x.y));
+        const __nv_bfloat162 q2 = __floats2bfloat162_rn(x.x, x.y);
         w[i] = *reinterpret_cast<const uint32_t*>(&q2);
       } else {
-        const __half2 q2 = __floats2half2_rn(times(x.x), times(x.y));
+        const __half2 q2 = __floats2half2_rn(x.x, x.y);
         w[i] = *reinterpret_cast<const uint32_t*>(&q2);
       }
     }
@@ -305,17 +320,16 @@ __device__ __forceinline__ void store_pieces(const uint4 (&v)[N], const char* at
 
 // The factor that takes norm n to max_norm. A norm of 0 is not above any; NaN stays NaN. A finite
 // max_norm beyond f32 is below an infinite norm only: 0, not the NaN of two infinities.
-constexpr float kLargest = 3.402823466e38f, kLeastNormal = 1.175494351e-38f;
-__device__ __noinline__ Factor small_factor(float n, double max_norm) {
-  const double q = max_norm / n;
-  if (!(q > 0.0)) return {0.0f, 1.0f};
-  const int e = max(ilogb(q) + 1, -149);
-  return {ldexpf(1.0f, e), (float)ldexp(q, -e)};
-}
 __device__ __forceinline__ Factor factor_of(float n, double max_norm) {
+  constexpr float kLargest = 3.402823466e38f;
   if (n <= max_norm) return {1.0f, 1.0f};
-  const float f = __fdiv_rn((float)fmin(max_norm, (double)kLargest), n);
-  return f < kLeastNormal && n <= kLargest ? small_factor(n, max_norm) : Factor{f, 1.0f};
+  if (n > kLargest || !(max_norm < n * 0x1p-126))
+    return {__fdiv_rn((float)fmin(max_norm, (double)kLargest), n), 1.0f};
+  if (max_norm < 0x1p-150) return {0.0f, 1.0f};  // no result is larger
+  // The factor is in [2^-278, 2^-126), max_norm < 4 and n > 2^-24; q, 2^160 times it, is normal.
+  const float q = __fdiv_rn((float)(max_norm * 0x1p100), n * 0x1p-60f);
+  const int e = max((__float_as_int(q) >> 23) - 127 - 159, -149);
+  return {__int_as_float(1 << (e + 149)), q * __int_as_float((-160 - e + 127) << 23)};
 }
 
 // Blocks and their windows as in the launch of k_sum_squares that left these entries; last[b] is
