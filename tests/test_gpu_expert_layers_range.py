@@ -162,3 +162,51 @@ def test_gradients_at_the_range_of_f16(ops, wide):
     exact[H - 1, :2] = 600.0 * 2.0 ** -6          # dh act(gate)
     exact[H, 1] = 2.0 ** -6
     assert torch.equal(rest, exact)
+
+
+U = 2.0 ** -23
+
+
+def relative(act, v):
+    """How far values and slopes (below -2) may be off, relative to themselves, before they are
+    rounded to 16 bits. e^v by one instruction (2 units of U) on an argument rounded twice (0.62 |v|).
+    silu: a sum (0.5), a reciprocal (1) and a product (0.5) follow; above 0 the exp's part of 1 + e^-v
+    falls faster than its error grows. gelu: a tail fitted to 5.4e-6, e^(-v^2 / 2) with two more
+    roundings of its argument (0.5 v^2 / 2), and seven operations of the polynomial.
+    Slopes: s (1 + v (1 - s)) adds at most 4.5 units below -2; v phi(v) + P(v) is, there, a
+    difference of terms whose sum is 1.53 times as large."""
+    if act == "silu":
+        a = torch.where(v < 0, 4 + 0.62 * v.abs(), 5.0) * U
+        return a, a + 4.5 * U
+    a = torch.where(v < 0, 5.4e-6 + (9 + 0.56 * v * v) * U, 1.2e-5)
+    return a, 1.53 * (5.4e-6 + (10 + 0.56 * v * v) * U)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("streamed", [False, True])
+def test_small_values_keep_their_digits(ops, act, dtype, streamed):
+    """The activation itself (one input column, weights of 1), relative to its own size down to
+    where e^v leaves f32's normal numbers: silu to -87, gelu to -13; below that nearly nothing."""
+    dt = DTYPES[dtype]
+    end = -87.0 if act == "silu" else -13.1
+    x = torch.cat([torch.linspace(end, 0, 6001), torch.linspace(0, 12, 500),
+                   -torch.logspace(-6, 2, 1600)]).to("cuda").to(dt)[:, None].contiguous()
+    m, E = x.shape[0], 512 if streamed else 1
+    off = offsets_of([m // E + (e < m % E) for e in range(E)])
+    w = torch.ones(E, 1, 1, device="cuda", dtype=dt)
+    y, pre = ops.grouped_linear(x, w, off, activation=act, save=True)
+    v = x.double()
+    a, s = activation64(act, v)
+    rel, slope = relative(act, v)
+    least = 2.0 ** -25 if dt is torch.float16 else 2.0 ** -134
+    usual = v >= end
+    lim = a.abs() * (UNIT[dt] + 1.01 * rel) + least
+    assert ((y.double() - a).abs() <= lim)[usual].all()
+    assert (y.double().abs() <= 1.1e-36 + least)[~usual].all() and (~usual).any()
+    d = ops.grouped_linear_backward(torch.ones_like(x), pre, x, w, off, activation=act,
+                                    need_dw=False, need_dbias=False)[0]
+    lim = s.abs() * (UNIT[dt] + 1.01 * slope) + least
+    assert ((d.double() - s).abs() <= lim)[usual & (v < -2)].all()
+    assert (d.double().abs() <= 1.1e-36 + least)[~usual].all()
+    assert bool(y[(v > -5) & (v < -4.9)].any()) and bool(d[(v > -5) & (v < -4.9)].any())
