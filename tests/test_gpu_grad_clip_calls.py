@@ -208,3 +208,14 @@ def test_a_norm_at_the_end_of_f32(ops):
     most = top * (1 - 2.0 ** -12)
     assert float(ops.clip_grads([a], most)) == top
     assert (a.double() / (top / 2) - (1 - 2.0 ** -12)).abs().max() <= 2.0 ** -22
+
+
+@pytest.mark.parametrize("value,most,want", [
+    (1.0, 2.0 ** -151, 0.0), (2.0 ** -149, 2.0 ** -150, 0.0), (2.0 ** -148, 2.0 ** -148, 2.0 ** -149),
+    (1.0, 2.0 ** -149, 0.0), (1.0, 2.0 ** -140, 2.0 ** -141), (2.0 ** 126, 2.0 ** -148, 2.0 ** -149),
+    (1.0, 1e-300, 0.0)])
+def test_a_largest_norm_at_the_least_of_f32(ops, value, most, want):
+    """Four equal values, so a norm of twice the value; 2^-150 rounds to the even 0."""
+    a = torch.full((4,), value, device="cuda")
+    assert float(ops.clip_grads([a], most)) == 2 * value
+    assert a.tolist() == [want] * 4
