@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kFewThreads, S::kBlocks) k_grouped_few(const F
     int want = blockIdx.x / (g.blocks * g.split);
     bool found = false;
     // One wait for memory for 128 experts. (A row for the last expert of 255, 128 x 704: 7.9 -> 7.3
-    // us, of 500 9.7 -> 8.3; with 8 experts the longer code costs 0.1.)
+    // us, of 500 9.7 -> 8.3; with 8 experts no difference.)
     constexpr int kAtOnce = 4;
     for (int i0 = 0; i0 <= g.experts + 1 && !found; i0 += 32 * kAtOnce) {
       int32_t from[kAtOnce], to[kAtOnce];

@@ -97,7 +97,10 @@ def grouped_matmul_backward(dy, x, w, offsets, rows=None, grad_dtype=None, need_
     """Gradients of `grouped_matmul`: (dx, dw) from dy [M, outer]. dx [M, inner] is of the
     grouped rows (with `rows`, `combine(dx, position)` sums it into the tokens); dw
     [E, outer, inner] has type `grad_dtype`: the weights' (default) or float32. One that is
-    not needed is None."""
+    not needed is None. `grouped_linear_backward` with pre None gives the same products, sums those
+    of few tiles in parts (1840 rows, 20 experts of 6400 x 64, dx: 15 us instead of 44) and so
+    adds in another order; here the order stays as it was. dw in float32 takes 1.2 to 1.5 times as
+    long as in 16 bits."""
     wide = _wide("grouped_matmul_backward", grad_dtype, w)
     return _X.grouped_matmul_backward(dy, x, w, offsets, rows, wide, need_dx, need_dw)
 
