@@ -644,11 +644,13 @@ struct Range {
 // positions, so a common one solves `by` = sum over the strides of stride * difference of positions
 // (the bytes of an element count as an axis of stride 1). The largest stride's difference is tried
 // first, as far as the smaller ones can make up for the rest: one or two values where every axis
-// steps over those of smaller strides. Ranges that take more than kMost trials count as common.
+// steps over those of smaller strides. Ranges that take more trials, or have more axes than are
+// kept, count as common.
+constexpr int kMostTrials = 1000;
 struct Axis {
   int64_t stride, more_a, more_b;  // positions past the first of each tensor
 };
-bool meets(const std::vector<Axis>& axes, size_t left, int64_t by, int64_t reach_a, int64_t reach_b,
+bool meets(const Axis* axes, int left, int64_t by, int64_t reach_a, int64_t reach_b,
            int& trials) {
   if (--trials < 0) return true;
   if (by < -reach_b || by > reach_a) return false;
@@ -667,15 +669,24 @@ bool meets(const std::vector<Axis>& axes, size_t left, int64_t by, int64_t reach
 }
 bool common(const Range& a, const Range& b, const std::vector<const Tensor*>& tensors) {
   if (a.gaps < 0 && b.gaps < 0) return true;
-  std::vector<Axis> axes;
+  // by rising strides; on the stack, since a thousand columns of a matrix are half a million pairs
+  constexpr int kMostAxes = 16;
+  Axis axes[kMostAxes];
+  int count = 0;
   int64_t reach_a = 0, reach_b = 0;
+  bool fits = true;
   auto add = [&](const Range& r, int64_t Axis::*more, int64_t& reach) {
     auto axis = [&](int64_t stride, int64_t size) {
       if (size < 2 || stride == 0) return;
-      auto at = std::find_if(axes.begin(), axes.end(),
-                             [&](const Axis& x) { return x.stride >= stride; });
-      if (at == axes.end() || at->stride != stride) at = axes.insert(at, Axis{stride, 0, 0});
-      (*at).*more += size - 1;
+      int at = 0;
+      while (at < count && axes[at].stride < stride) ++at;
+      if (at == count || axes[at].stride != stride) {
+        if (!(fits = fits && count < kMostAxes)) return;
+        std::copy_backward(axes + at, axes + count, axes + count + 1);
+        axes[at] = Axis{stride, 0, 0};
+        ++count;
+      }
+      axes[at].*more += size - 1;
       reach += stride * (size - 1);
     };
     if (r.gaps < 0) return axis(1, (int64_t)(r.end - r.begin));
@@ -686,9 +697,8 @@ bool common(const Range& a, const Range& b, const std::vector<const Tensor*>& te
   };
   add(a, &Axis::more_a, reach_a);
   add(b, &Axis::more_b, reach_b);
-  constexpr int kMost = 1000;
-  int trials = kMost;
-  return meets(axes, axes.size(), (int64_t)(b.begin - a.begin), reach_a, reach_b, trials);
+  int trials = kMostTrials;
+  return !fits || meets(axes, count, (int64_t)(b.begin - a.begin), reach_a, reach_b, trials);
 }
 
 // Memory that is written overlaps nothing else. Sorting the ranges of 1021 tensors in three
